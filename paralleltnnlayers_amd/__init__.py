@@ -1,5 +1,6 @@
 """MI355X-native fused CP4-decomposed Conv2d (forward, backward-data,
-backward-filter) behind a C ABI.
+backward-filter) behind a C ABI; dense projections with low-rank adapters (``adapter_forward``,
+``torch_ops.adapter_linear``) and an AdamW step over many tensors (``optim``) beside it.
 
 This Python package is only the loader/binding of ``csrc/libcp4conv.so`` used
 by the tests and the bench; the product is the shared library and the C++ host
@@ -20,6 +21,6 @@ from .capi import (Shape, Geometry, geometry, conv2d_forward_ex, conv2d_backward
                    forward_variants, default_variant, recompose, count_exceeding,
                    random_uniform, time_copy, cp3_shape_for, cp3_expand_factors,
                    cp3_fold_gradients, cp3_conv2d_forward, cp3_conv2d_backward_data,
-                   cp3_conv2d_backward_filter)
+                   cp3_conv2d_backward_filter, adapter_forward, adapter_backward)
 
 __all__ = [n for n in dir() if not n.startswith("_")]

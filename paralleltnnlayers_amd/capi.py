@@ -46,6 +46,26 @@ class RcpDims(ctypes.Structure):
     _fields_ = [(k, ctypes.c_uint) for k in ("S0", "S1", "T0", "T1")]
 
 
+class AdapterShape(ctypes.Structure):
+    """cp4_adapter_shape: tokens, inputs, outputs, rank, adapters, row strides."""
+    _fields_ = ([("T", ctypes.c_size_t)] + [(k, ctypes.c_uint) for k in ("K", "N", "R", "G")] +
+                [(k, ctypes.c_size_t) for k in ("ldx", "ldw", "lddy")])
+
+
+class AdamwTensor(ctypes.Structure):
+    """cp4_adamw_tensor."""
+    _fields_ = ([(k, ctypes.c_void_p) for k in ("param", "grad", "exp_avg", "exp_avg_sq", "scale", "scale_sq",
+                                                "copy")] + [("n", ctypes.c_size_t)] +
+                [(k, ctypes.c_int) for k in ("param_dtype", "grad_dtype", "copy_dtype", "bits")] +
+                [("group", ctypes.c_uint)])
+
+
+class AdamwGroup(ctypes.Structure):
+    """cp4_adamw_group."""
+    _fields_ = ([(k, ctypes.c_double) for k in ("lr", "beta1", "beta2", "eps", "weight_decay")] +
+                [("counter", ctypes.c_void_p)])
+
+
 class _Missing:
     """Stands for the binding until it is built: every call of it says so."""
 
@@ -199,6 +219,23 @@ def lib():
     L.cp4_random_uniform.argtypes = [_F, ctypes.c_size_t, ctypes.c_ulonglong, ctypes.c_void_p]
     L.cp4_copy_f32.argtypes = [_F, _F, ctypes.c_size_t, ctypes.c_void_p]
     L.cp4_time_copy_f32.argtypes = [_F, _F, ctypes.c_size_t] + timing
+    L.cp4_adapter_kept_bytes.restype = ctypes.c_size_t
+    L.cp4_adapter_kept_bytes.argtypes = [ctypes.POINTER(AdapterShape)]
+    for name in ("forward", "backward"):
+        need = getattr(L, f"cp4_adapter_{name}_workspace_bytes")
+        need.restype = ctypes.c_size_t
+        need.argtypes = [ctypes.POINTER(AdapterShape), ctypes.c_int]
+    L.cp4_adapter_forward.argtypes = ([ctypes.POINTER(AdapterShape), ctypes.c_int] + [ctypes.c_void_p] * 10 +
+                                      [ctypes.c_size_t, ctypes.c_void_p])
+    L.cp4_adapter_backward.argtypes = ([ctypes.POINTER(AdapterShape), ctypes.c_int] + [ctypes.c_void_p] * 12 +
+                                       [ctypes.c_size_t, ctypes.c_void_p])
+    L.cp4_adamw_workspace_bytes.restype = ctypes.c_size_t
+    _T = ctypes.POINTER(AdamwTensor)
+    L.cp4_adamw_step.argtypes = [_T, ctypes.c_size_t, ctypes.POINTER(AdamwGroup), ctypes.c_size_t, ctypes.c_float,
+                                 ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t,
+                                 ctypes.c_void_p]
+    for name in ("cp4_adamw_moments", "cp4_adamw_set_moments"):
+        getattr(L, name).argtypes = [_T, ctypes.c_size_t] + [ctypes.POINTER(ctypes.c_void_p)] * 2 + [ctypes.c_void_p]
     L.cp4_device_malloc.argtypes = [ctypes.POINTER(ctypes.c_void_p), ctypes.c_size_t]
     L.cp4_device_free.argtypes = [ctypes.c_void_p]
     L.cp4_host_malloc.argtypes = [ctypes.POINTER(ctypes.c_void_p), ctypes.c_size_t]
@@ -284,6 +321,30 @@ def conv2d_forward(x, FK, FC, FH, FW, pad=1, out=None, variant=-1, stream=None):
     if stream is None or out is not None:              # (allocates y only)
         return _native.forward(x, FK, FC, FH, FW, pad, out, variant, stream)
     return _ordered(stream, _native.forward, x, FK, FC, FH, FW, pad, out, variant, stream)
+
+
+def adapter_forward(x, W, A, B, ids, scale=None, bias=None, out=None, keep=False, stream=None):
+    """y = x W^T + bias with the low-rank adapter of each token beside it.
+
+    ``y[t] = W x[t] + bias + scale[a] B[a] (A[a] x[t])`` with ``a = ids[t]``; an id outside
+    0 .. adapters - 1 (say -1) is a token without one.  x [..., K], W [N, K], A [adapters, R, K]
+    and B [adapters, N, R] of one type (float32, bfloat16, float16); scale [adapters] and bias
+    [N] float32; ids one int32 or int64 a token, in any order.  ``keep``: also returns what
+    ``adapter_backward`` needs of this pass.
+    """
+    if stream is None:
+        return _native.adapter_forward(x, W, A, B, ids, scale, bias, out, keep, stream)
+    return _ordered(stream, _native.adapter_forward, x, W, A, B, ids, scale, bias, out, keep, stream)
+
+
+def adapter_backward(dy, x, W, A, B, ids, scale=None, kept=None, want_dx=True, want_factors=True,
+                     stream=None):
+    """(dx, dA, dB) of ``adapter_forward`` for dy [..., N]; ``kept``: what that call left.
+    What is not wanted is None (x and kept may be None without the adapters' gradients)."""
+    args = (dy, x, W, A, B, ids, scale, kept, want_dx, want_factors, stream)
+    if stream is None:
+        return _native.adapter_backward(*args)
+    return _ordered(stream, _native.adapter_backward, *args)
 
 
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1}

@@ -1,0 +1,199 @@
+// Interface between the adapters' C ABI (adapter_capi.hip) and their kernels.
+#ifndef CP4_ADAPTER_INTERNAL_H
+#define CP4_ADAPTER_INTERNAL_H
+
+#include <hip/hip_runtime.h>
+
+#include "cp4/adapter.h"
+#include "cp4_internal.h"
+#include "value_types.h"
+
+namespace cp4 {
+namespace adapter {
+
+// h[t][r] = scale_a sum_k z[t][k] F_a(r, k), F_a(r, k) at f + a * R * K + r * fr + k * fk.
+// h has rows of Rp values (R rounded up to 16s): zero beyond R and for tokens without an adapter.
+struct ShrinkArgs {
+  const void* z;          // [T][K], rows ldz apart
+  const void* f;
+  const int* ids;
+  const float* scale;     // [G] or null
+  float* h;               // [T][Rp]
+  size_t T, ldz;
+  int K, R, Rp, G;
+  int fr, fk;
+};
+
+// y[t][n] = sum_k z[t][k] w(n, k) + bias[n] + sum_r h[t][r] F_a(n, r), F_a(n, r) at
+// f + a * R * N + n * fn + r * fr; w(n, k) at w + n * ldw + k, or (nn) at w + k * ldw + n.
+struct ProjectArgs {
+  const void *z, *w, *f;
+  const float *h, *bias;
+  const int* ids;
+  void* y;                // [T][N]
+  size_t T, ldz, ldw;
+  int K, N, R, Rp, G;
+  int fn, fr;
+};
+
+// out[a][r][c] = sum over tokens with ids[t] = a of p[t][r] z[t][c], at out + a * R * C + r * outr +
+// c * outc; with splits > 1 the sums of each range of tokens go to part [splits][G][R][C]
+// (in out's order) and are added up by a second launch.
+struct GradArgs {
+  const float* p;         // [T][Rp]
+  const void* z;          // [T][C], rows ldz apart
+  const int* ids;
+  void* out;
+  float* part;
+  size_t T, ldz;
+  int C, R, Rp, G;
+  int outr, outc;
+  int splits;
+};
+
+hipError_t shrink_launch(const ShrinkArgs&, int dtype, hipStream_t);
+hipError_t project_launch(const ProjectArgs&, int dtype, bool nn, hipStream_t);
+int grad_splits(size_t T, int C, int R, int G);
+hipError_t grad_launch(const GradArgs&, int dtype, hipStream_t);
+
+// ---- device side ------------------------------------------------------------------------
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// 16 x 16 blocks of products, 32 deep: of a lane's eight values, row (or column) lane & 15 and depth
+// 8 * (lane >> 4) + j; the result's column is lane & 15, its row 4 * (lane >> 4) + v.
+__device__ __forceinline__ f32x4 mfma_bf16(u16x8 a, u16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <class T>
+__device__ __forceinline__ f32x4 mfma_16(u16x8 a, u16x8 b, f32x4 c) {
+  if constexpr (__is_same(T, BF16)) return mfma_bf16(a, b, c);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+// The same 4 deep in fp32: one value a lane, depth lane >> 4.
+__device__ __forceinline__ f32x4 mfma_f32(float a, float b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+
+// A value as two bfloat16 parts: to nearest, and what that leaves.
+__device__ __forceinline__ void two_parts(float x, unsigned short& hi, unsigned short& lo) {
+  hi = BF16::narrow(x);
+  lo = BF16::narrow(x - BF16::widen(hi));
+}
+__device__ __forceinline__ void two_parts(const float (&x)[8], u16x8& hi, u16x8& lo) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    unsigned short h, l;
+    two_parts(x[j], h, l);
+    hi[j] = h;
+    lo[j] = l;
+  }
+}
+
+// The different adapters of up to 64 tokens, one lane an id (-1: none): take() gives the next
+// one and the lanes whose it is.
+struct Adapters {
+  unsigned long long left;
+  int id;
+  __device__ __forceinline__ Adapters(int id_) : left(__ballot(id_ >= 0)), id(id_) {}
+  __device__ __forceinline__ bool take(int& a, unsigned long long& whose) {
+    if (!left) return false;
+    a = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
+    whose = __ballot(id == a);
+    left &= ~whose;
+    return true;
+  }
+};
+
+// Adds h F_a^T to the 16 x 16 blocks of MB blocks of rows and NB of columns, for the rows whose bit of
+// `whose` is set (block i's: 16 i ..).  h: this lane's row (lane & 15) of block 0, rows 16 * Rp
+// floats further in the next; n0: column of block 0's lane 0.  16-bit types: depth 0 .. 15 are the first
+// parts of h, 16 .. 31 what they leave, against F_a twice (f16: F_a in two parts as well, in two products).
+// Rows that are not the adapter's are left as they are, not added zeros: an infinity or a NaN in one
+// adapter is no other token's.
+template <class T, int MB, int NB>
+__device__ __forceinline__ void expand(const float* h, int Rp, unsigned long long whose, const typename T::raw* f,
+                                       int fn, int fr, int n0, int N, int R, f32x4 (&acc)[MB][NB]) {
+  const int lane = threadIdx.x & 63, l = lane & 15, g = lane >> 4;
+  for (int r0 = 0; r0 < R; r0 += 16) {
+    float hf[MB][4];
+    u16x8 ha[MB];
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+      const bool mine = whose >> (16 * i + l) & 1;
+      const float* const row = h + (size_t)16 * i * Rp + r0;
+      if constexpr (__is_same(T, F32)) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) hf[i][q] = mine ? row[4 * q + g] : 0.0f;
+      } else {
+        float x[8] = {};
+        if (mine) {
+          const f32x4* p = reinterpret_cast<const f32x4*>(row + 8 * (g & 1));
+          const f32x4 u = p[0], v = p[1];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[j] = u[j], x[4 + j] = v[j];
+        }
+        u16x8 hi, lo;
+        two_parts(x, hi, lo);
+        ha[i] = g < 2 ? hi : lo;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const int n = n0 + 16 * j + l;
+      float ff[4];
+      u16x8 fv = {}, fl = {};
+      if constexpr (__is_same(T, F32)) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int r = r0 + 4 * q + g;
+          ff[q] = n < N && r < R ? f[(size_t)n * fn + (size_t)r * fr] : 0.0f;
+        }
+      } else {
+        if (n < N) {
+          const typename T::raw* const p = f + (size_t)n * fn;
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const int r = r0 + 8 * (g & 1) + q;
+            if (r < R) fv[q] = p[(size_t)r * fr];
+          }
+        }
+        if constexpr (__is_same(T, F16)) {
+          float x[8];
+#pragma unroll
+          for (int q = 0; q < 8; ++q) x[q] = F16::widen(fv[q]);
+          two_parts(x, fv, fl);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < MB; ++i) {
+        const unsigned rows = (unsigned)(whose >> (16 * i)) & 0xffffu;
+        if (!rows) continue;
+        f32x4 d = acc[i][j];
+        if constexpr (__is_same(T, F32)) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) d = mfma_f32(hf[i][q], ff[q], d);
+        } else {
+          if constexpr (__is_same(T, F16)) d = mfma_bf16(ha[i], fl, d);
+          d = mfma_bf16(ha[i], fv, d);
+        }
+        if (rows == 0xffffu) {
+          acc[i][j] = d;
+        } else {
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            if (rows >> (4 * g + v) & 1) acc[i][j][v] = d[v];
+        }
+      }
+    }
+  }
+}
+
+}  // namespace adapter
+}  // namespace cp4
+#endif

@@ -1,0 +1,147 @@
+// C ABI of the adapters beside a shared projection (include/cp4/adapter.h): checks, workspace, launches.
+#include <algorithm>
+
+#include "adapter.h"
+
+namespace {
+
+using cp4::fail_hip;
+using cp4::fail_with;
+using namespace cp4::adapter;
+
+size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
+int padded(const cp4_adapter_shape& s) { return (int)((s.R + 15) / 16 * 16); }
+size_t value_bytes(int dtype) { return dtype == CP4_DTYPE_F32 ? 4 : 2; }
+
+cp4_status check_shape(const cp4_adapter_shape* s, int dtype) {
+  if (!s) return fail_with(CP4_ERR_NULL_POINTER, "shape is NULL");
+  if (dtype != CP4_DTYPE_F32 && dtype != CP4_DTYPE_BF16 && dtype != CP4_DTYPE_F16)
+    return fail_with(CP4_ERR_SHAPE, "unknown dtype");
+  if (!s->K || !s->N || !s->R || !s->G) return fail_with(CP4_ERR_SHAPE, "K, N, R and G must be 1 or more");
+  if (s->R > 256) return fail_with(CP4_ERR_SHAPE, "adapters of a rank above 256");
+  if (s->G > 65535) return fail_with(CP4_ERR_SHAPE, "more than 65535 adapters");
+  if (s->K > 1u << 22 || s->N > 1u << 22) return fail_with(CP4_ERR_SHAPE, "K or N above 2^22");
+  if (s->T > (size_t)1 << 31) return fail_with(CP4_ERR_SHAPE, "more than 2^31 tokens");
+  if ((s->ldx && s->ldx < s->K) || (s->ldw && s->ldw < s->K) || (s->lddy && s->lddy < s->N))
+    return fail_with(CP4_ERR_SHAPE, "a row stride is smaller than the row");
+  if (std::max({s->ldx, s->ldw, s->lddy}) > (size_t)1 << 30)
+    return fail_with(CP4_ERR_SHAPE, "a row stride above 2^30");
+  return CP4_OK;
+}
+cp4_status check_pointers(size_t bytes, std::initializer_list<const void*> values,
+                          std::initializer_list<const void*> floats) {
+  for (const void* p : values)
+    if ((size_t)p % bytes) return fail_with(CP4_ERR_SHAPE, "a pointer is not aligned to its element type");
+  for (const void* p : floats)
+    if ((size_t)p & 3) return fail_with(CP4_ERR_SHAPE, "a pointer is not aligned to its element type");
+  return CP4_OK;
+}
+
+struct BackwardPlan {
+  int splits_a, splits_b;
+  size_t dh_at, part_at, total;
+};
+BackwardPlan backward_plan(const cp4_adapter_shape& s) {
+  BackwardPlan p{};
+  p.splits_a = grad_splits(s.T, (int)s.K, (int)s.R, (int)s.G);
+  p.splits_b = grad_splits(s.T, (int)s.N, (int)s.R, (int)s.G);
+  p.part_at = align256(s.T * padded(s) * 4);
+  const size_t each = (size_t)s.G * s.R * 4;
+  const size_t pa = p.splits_a > 1 ? p.splits_a * each * s.K : 0, pb = p.splits_b > 1 ? p.splits_b * each * s.N : 0;
+  p.total = p.part_at + align256(std::max(pa, pb));    // (one after the other)
+  return p;
+}
+
+}  // namespace
+
+extern "C" size_t cp4_adapter_kept_bytes(const cp4_adapter_shape* s) {
+  return s ? s->T * padded(*s) * 4 : 0;
+}
+
+extern "C" size_t cp4_adapter_forward_workspace_bytes(const cp4_adapter_shape* s, int dtype) {
+  if (check_shape(s, dtype) != CP4_OK) return 0;
+  return align256(cp4_adapter_kept_bytes(s));
+}
+
+extern "C" cp4_status cp4_adapter_forward(const cp4_adapter_shape* s, int dtype, const void* x, const void* W,
+                                          const void* A, const void* B, const int* ids, const float* scale,
+                                          const float* bias, void* y, float* kept, void* workspace,
+                                          size_t workspace_bytes, cp4_stream stream) {
+  if (const cp4_status rc = check_shape(s, dtype)) return rc;
+  if (!s->T) return CP4_OK;
+  if (!x || !W || !A || !B || !ids || !y) return fail_with(CP4_ERR_NULL_POINTER, "an operand is NULL");
+  if (const cp4_status rc = check_pointers(value_bytes(dtype), {x, W, A, B, y}, {ids, scale, bias})) return rc;
+  const size_t need = cp4_adapter_forward_workspace_bytes(s, dtype);
+  if (!workspace || workspace_bytes < need || ((size_t)workspace & 255))
+    return fail_with(CP4_ERR_WORKSPACE, "workspace missing, too small or not aligned to 256 bytes");
+  if ((size_t)kept & 15) return fail_with(CP4_ERR_WORKSPACE, "kept is not aligned to 16 bytes");
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  float* const h = kept ? kept : static_cast<float*>(workspace);
+  ShrinkArgs sh{};
+  sh.z = x; sh.f = A; sh.ids = ids; sh.scale = scale; sh.h = h;
+  sh.T = s->T; sh.ldz = s->ldx ? s->ldx : s->K;
+  sh.K = (int)s->K; sh.R = (int)s->R; sh.Rp = padded(*s); sh.G = (int)s->G;
+  sh.fr = (int)s->K; sh.fk = 1;
+  if (const hipError_t e = shrink_launch(sh, dtype, st)) return fail_hip(e, "cp4_adapter_forward");
+  ProjectArgs p{};
+  p.z = x; p.w = W; p.f = B; p.h = h; p.bias = bias; p.ids = ids; p.y = y;
+  p.T = s->T; p.ldz = sh.ldz; p.ldw = s->ldw ? s->ldw : s->K;
+  p.K = (int)s->K; p.N = (int)s->N; p.R = (int)s->R; p.Rp = sh.Rp; p.G = (int)s->G;
+  p.fn = (int)s->R; p.fr = 1;
+  if (const hipError_t e = project_launch(p, dtype, false, st)) return fail_hip(e, "cp4_adapter_forward");
+  return CP4_OK;
+}
+
+extern "C" size_t cp4_adapter_backward_workspace_bytes(const cp4_adapter_shape* s, int dtype) {
+  if (check_shape(s, dtype) != CP4_OK) return 0;
+  return backward_plan(*s).total;
+}
+
+extern "C" cp4_status cp4_adapter_backward(const cp4_adapter_shape* s, int dtype, const void* dy, const void* x,
+                                           const void* W, const void* A, const void* B, const int* ids,
+                                           const float* scale, const float* kept, void* dx, void* dA, void* dB,
+                                           void* workspace, size_t workspace_bytes, cp4_stream stream) {
+  if (const cp4_status rc = check_shape(s, dtype)) return rc;
+  if (!dA != !dB) return fail_with(CP4_ERR_NULL_POINTER, "dA without dB");
+  if (s->T) {
+    if (!dy || !W || !A || !B || !ids || (dA && (!x || !kept)))
+      return fail_with(CP4_ERR_NULL_POINTER, "an operand is NULL");
+    if (const cp4_status rc = check_pointers(value_bytes(dtype), {dy, x, W, A, B, dx, dA, dB}, {ids, scale})) return rc;
+    if ((size_t)kept & 15) return fail_with(CP4_ERR_WORKSPACE, "kept is not aligned to 16 bytes");
+  }
+  const BackwardPlan plan = backward_plan(*s);
+  if (plan.total && (!workspace || workspace_bytes < plan.total || ((size_t)workspace & 255)))
+    return fail_with(CP4_ERR_WORKSPACE, "workspace missing, too small or not aligned to 256 bytes");
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  float* const dh = static_cast<float*>(workspace);
+  float* const part = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.part_at);
+  const int Rp = padded(*s);
+  const size_t lddy = s->lddy ? s->lddy : s->N, ldx = s->ldx ? s->ldx : s->K;
+  if (s->T && (dx || dA)) {
+    ShrinkArgs sh{};
+    sh.z = dy; sh.f = B; sh.ids = ids; sh.scale = scale; sh.h = dh;
+    sh.T = s->T; sh.ldz = lddy;
+    sh.K = (int)s->N; sh.R = (int)s->R; sh.Rp = Rp; sh.G = (int)s->G;
+    sh.fr = 1; sh.fk = (int)s->R;
+    if (const hipError_t e = shrink_launch(sh, dtype, st)) return fail_hip(e, "cp4_adapter_backward");
+  }
+  if (s->T && dx) {
+    ProjectArgs p{};
+    p.z = dy; p.w = W; p.f = A; p.h = dh; p.ids = ids; p.y = dx;
+    p.T = s->T; p.ldz = lddy; p.ldw = s->ldw ? s->ldw : s->K;
+    p.K = (int)s->N; p.N = (int)s->K; p.R = (int)s->R; p.Rp = Rp; p.G = (int)s->G;
+    p.fn = 1; p.fr = (int)s->K;
+    if (const hipError_t e = project_launch(p, dtype, true, st)) return fail_hip(e, "cp4_adapter_backward");
+  }
+  if (dA) {
+    GradArgs g{};
+    g.ids = ids; g.part = part; g.T = s->T; g.R = (int)s->R; g.Rp = Rp; g.G = (int)s->G;
+    g.p = dh; g.z = x; g.out = dA; g.ldz = ldx; g.C = (int)s->K; g.outr = (int)s->K; g.outc = 1;
+    g.splits = plan.splits_a;
+    if (const hipError_t e = grad_launch(g, dtype, st)) return fail_hip(e, "cp4_adapter_backward");
+    g.p = kept; g.z = dy; g.out = dB; g.ldz = lddy; g.C = (int)s->N; g.outr = 1; g.outc = (int)s->R;
+    g.splits = plan.splits_b;
+    if (const hipError_t e = grad_launch(g, dtype, st)) return fail_hip(e, "cp4_adapter_backward");
+  }
+  return CP4_OK;
+}

@@ -1,0 +1,123 @@
+// The shared projection with the adapters' second product beside it (include/cp4/adapter.h): a GEMM
+// whose accumulators also take h B_a^T, for the adapters that the tile's rows have, before they are
+// rounded and stored.
+#include <algorithm>
+
+#include "adapter.h"
+
+namespace cp4 {
+namespace adapter {
+namespace {
+
+// ---- any strides and alignment ------------------------------------------------------------
+
+constexpr int kTile = 64, kDepth = 32;
+
+// A tile of 64 x 64 outputs, 32 deep through the LDS, element by element; four waves of 32 x 32.
+template <class T, bool NN>
+__global__ __launch_bounds__(256) void general_kernel(const ProjectArgs a) {
+  typedef typename T::raw Raw;
+  constexpr int kRow = kDepth + 16 / sizeof(Raw);                    // (rows start on other banks)
+  __shared__ Raw lz[kTile][kRow], lw[kTile][kRow];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
+  const size_t t0 = (size_t)blockIdx.y * kTile;
+  const int n0 = blockIdx.x * kTile, wm = 32 * (wave >> 1), wn = 32 * (wave & 1);
+  const Raw* const z = static_cast<const Raw*>(a.z);
+  const Raw* const w = static_cast<const Raw*>(a.w);
+  f32x4 acc[2][2] = {};
+  for (int k0 = 0; k0 < a.K; k0 += kDepth) {
+    Raw zr[8], wr[8];
+    const int kc = threadIdx.x & 31, row0 = threadIdx.x >> 5;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = row0 + 8 * i, k = k0 + kc;
+      zr[i] = t0 + row < a.T && k < a.K ? z[(t0 + row) * a.ldz + k] : Raw(0);
+      if constexpr (NN) {
+        const int kr = k0 + (threadIdx.x >> 6) + 4 * i, n = n0 + (threadIdx.x & 63);
+        wr[i] = kr < a.K && n < a.N ? w[(size_t)kr * a.ldw + n] : Raw(0);
+      } else {
+        wr[i] = n0 + row < a.N && k < a.K ? w[(size_t)(n0 + row) * a.ldw + k] : Raw(0);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      lz[row0 + 8 * i][kc] = zr[i];
+      if constexpr (NN) lw[threadIdx.x & 63][(threadIdx.x >> 6) + 4 * i] = wr[i];
+      else lw[row0 + 8 * i][kc] = wr[i];
+    }
+    __syncthreads();
+    if constexpr (__is_same(T, F32)) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            acc[i][j] = mfma_f32(lz[wm + 16 * i + l][4 * q + g], lw[wn + 16 * j + l][4 * q + g], acc[i][j]);
+    } else {
+      u16x8 za[2], wb[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        za[i] = *reinterpret_cast<const u16x8*>(&lz[wm + 16 * i + l][8 * g]);
+        wb[i] = *reinterpret_cast<const u16x8*>(&lw[wn + 16 * i + l][8 * g]);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = mfma_16<T>(za[i], wb[j], acc[i][j]);
+    }
+  }
+  // the adapters of this wave's 32 rows
+  int id = lane < 32 && t0 + wm + lane < a.T ? a.ids[t0 + wm + lane] : -1;
+  if (id < 0 || id >= a.G) id = -1;
+  Adapters todo(id);
+  int ad;
+  unsigned long long whose;
+  while (todo.take(ad, whose)) {
+    const Raw* const f = static_cast<const Raw*>(a.f) + (size_t)ad * a.R * a.N;
+    expand<T>(a.h + (t0 + wm + l) * a.Rp, a.Rp, whose, f, a.fn, a.fr, n0 + wn, a.N, a.R, acc);
+  }
+  Raw* const y = static_cast<Raw*>(a.y);
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int n = n0 + wn + 16 * j + l;
+    if (n >= a.N) continue;
+    const float b = a.bias ? a.bias[n] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const size_t t = t0 + wm + 16 * i + 4 * g + v;
+        if (t < a.T) y[t * a.N + n] = T::narrow(acc[i][j][v] + b);
+      }
+  }
+}
+
+template <class T>
+void general(const ProjectArgs& a, bool nn, hipStream_t st) {
+  ProjectArgs p = a;
+  const size_t most = (size_t)65535 * kTile;                         // (rows of one launch's grid)
+  for (size_t t = 0; t < a.T; t += most) {
+    p.T = std::min(most, a.T - t);
+    p.z = static_cast<const typename T::raw*>(a.z) + t * a.ldz;
+    p.h = a.h + t * a.Rp;
+    p.ids = a.ids + t;
+    p.y = static_cast<typename T::raw*>(a.y) + t * a.N;
+    const dim3 grid((a.N + kTile - 1) / kTile, (unsigned)((p.T + kTile - 1) / kTile));
+    if (nn) general_kernel<T, true><<<grid, 256, 0, st>>>(p);
+    else general_kernel<T, false><<<grid, 256, 0, st>>>(p);
+  }
+}
+
+}  // namespace
+
+hipError_t project_launch(const ProjectArgs& a, int dtype, bool nn, hipStream_t st) {
+  if (dtype == CP4_DTYPE_F32) general<F32>(a, nn, st);
+  else if (dtype == CP4_DTYPE_BF16) general<BF16>(a, nn, st);
+  else general<F16>(a, nn, st);
+  return hipGetLastError();
+}
+
+}  // namespace adapter
+}  // namespace cp4

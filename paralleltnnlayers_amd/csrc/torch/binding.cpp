@@ -24,7 +24,10 @@
 #include <atomic>
 #include <optional>
 #include <string>
+#include <vector>
 
+#include "cp4/adamw.h"
+#include "cp4/adapter.h"
 #include "cp4/capi.h"
 
 namespace {
@@ -445,6 +448,408 @@ PyObject* layer(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- adapters beside a shared projection (capi.adapter_*, torch_ops.adapter_linear) ---------
+
+int dtype_of(const Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return CP4_DTYPE_F32;
+    case at::kBFloat16: return CP4_DTYPE_BF16;
+    case at::kHalf: return CP4_DTYPE_F16;
+    default: fail(PyExc_AssertionError, "expected float32, bfloat16 or float16");
+  }
+}
+std::optional<Tensor> optional_tensor(PyObject* o) {
+  if (o == Py_None) return std::nullopt;
+  return tensor(o);
+}
+// [..., cols] as rows that lie `stride` apart; copied where its last dimensions do not allow that.
+Tensor rows_of(const Tensor& t, size_t* stride) {
+  const int64_t cols = t.size(-1);
+  if (t.dim() == 2 && (cols == 1 || t.stride(1) == 1) && t.stride(0) >= cols) {
+    *stride = (size_t)t.stride(0);
+    return t;
+  }
+  *stride = (size_t)cols;
+  return t.contiguous();
+}
+
+struct Adapters {
+  cp4_adapter_shape shape{};
+  int dtype = 0;
+  Tensor x, W, A, B, ids, scale, bias;             // as the C ABI takes them
+};
+// Checks the operands of an adapter call; x: [..., K] (dy of a backward call: [..., N]).
+Adapters adapters(const Tensor& x, const Tensor& W, const Tensor& A, const Tensor& B, const Tensor& ids,
+                  const std::optional<Tensor>& scale, const std::optional<Tensor>& bias, bool is_dy = false) {
+  Adapters p;
+  require(x.dim() >= 1 && W.dim() == 2 && A.dim() == 3 && B.dim() == 3,
+          "expected x [..., K], W [N, K], A [adapters, R, K] and B [adapters, N, R]");
+  const int64_t N = W.size(0), K = W.size(1), G = A.size(0), R = A.size(1);
+  require(x.size(-1) == (is_dy ? N : K) && A.size(2) == K && B.size(0) == G && B.size(1) == N && B.size(2) == R,
+          "x, W, A and B do not match");
+  for (const Tensor* t : {&x, &W, &A, &B})
+    require(t->is_cuda() && t->device() == x.device() && t->scalar_type() == x.scalar_type(),
+            "x, W, A and B must be of one type on one device");
+  p.dtype = dtype_of(x);
+  for (const auto& t : {scale, bias})
+    require(!t || (t->is_cuda() && t->device() == x.device() && t->scalar_type() == at::kFloat && t->dim() == 1),
+            "scale and bias must be float32 vectors on x's device");
+  require(!scale || scale->size(0) == G, "scale holds one value an adapter");
+  require(!bias || bias->size(0) == N, "bias does not match W");
+  const int64_t rows = x.numel() / std::max<int64_t>(1, x.size(-1));
+  require(ids.is_cuda() && ids.device() == x.device() && ids.numel() == (x.size(-1) ? rows : ids.numel()) &&
+              (ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong),
+          "ids must be one int32 or int64 a token, on x's device");
+  require(N <= 1 << 22 && K <= 1 << 22 && G <= 65535 && R <= 256, "adapters: K, N <= 2^22, R <= 256, G <= 65535");
+  p.shape.T = (size_t)ids.numel();
+  p.shape.K = (unsigned)K; p.shape.N = (unsigned)N; p.shape.R = (unsigned)R; p.shape.G = (unsigned)G;
+  p.x = rows_of(x, is_dy ? &p.shape.lddy : &p.shape.ldx);
+  p.W = rows_of(W, &p.shape.ldw);
+  p.A = A.contiguous();
+  p.B = B.contiguous();
+  p.ids = ids.contiguous();
+  if (ids.scalar_type() == at::kLong)                // (an id beyond 32 bits is no adapter's)
+    p.ids = at::where((p.ids >= 0).logical_and(p.ids < G), p.ids, at::full({}, -1, p.ids.options())).to(at::kInt);
+  if (scale) p.scale = scale->contiguous();
+  if (bias) p.bias = bias->contiguous();
+  return p;
+}
+const float* floats(const Tensor& t) { return t.defined() ? static_cast<const float*>(t.data_ptr()) : nullptr; }
+const int* ints(const Tensor& t) { return static_cast<const int*>(t.data_ptr()); }
+std::vector<int64_t> with_last(at::IntArrayRef sizes, int64_t last) {
+  std::vector<int64_t> s = sizes.vec();
+  s.back() = last;
+  return s;
+}
+
+// y, and where `kept` is given what the backward call needs.
+Tensor adapter_run(const Adapters& p, at::IntArrayRef sizes, Tensor y, Tensor* kept, void* st) {
+  if (!y.defined()) y = empty(with_last(sizes, p.shape.N), p.x.scalar_type(), p.x);
+  if (kept) *kept = empty({(int64_t)(cp4_adapter_kept_bytes(&p.shape) / 4)}, at::kFloat, p.x);
+  const size_t need = cp4_adapter_forward_workspace_bytes(&p.shape, p.dtype);
+  const Tensor ws = scratch(need, p.x);
+  check(cp4_adapter_forward(&p.shape, p.dtype, ptr(p.x), ptr(p.W), ptr(p.A), ptr(p.B), ints(p.ids), floats(p.scale),
+                            floats(p.bias), ptr(y), kept ? static_cast<float*>(ptr(*kept)) : nullptr, ptr(ws), need, st));
+  return y;
+}
+// dx, dA, dB as far as they are wanted; p.x is dy.
+void adapter_run_backward(const Adapters& p, const Tensor& x_in, const Tensor& kept, at::IntArrayRef sizes, Tensor* dx,
+                          Tensor* dA, Tensor* dB, void* st) {
+  cp4_adapter_shape s = p.shape;
+  Tensor x;
+  if (dA) {
+    require(x_in.is_cuda() && x_in.device() == p.x.device() && x_in.scalar_type() == p.x.scalar_type() &&
+                x_in.dim() >= 1 && x_in.size(-1) == (int64_t)s.K && x_in.numel() == (int64_t)(s.T * s.K),
+            "x does not match dy");
+    x = rows_of(x_in, &s.ldx);
+    require(kept.defined() && kept.is_cuda() && kept.scalar_type() == at::kFloat && kept.is_contiguous() &&
+                (size_t)kept.numel() * 4 == cp4_adapter_kept_bytes(&s),
+            "kept is not what the forward call left");
+    *dA = empty({(int64_t)s.G, (int64_t)s.R, (int64_t)s.K}, p.x.scalar_type(), p.x);
+    *dB = empty({(int64_t)s.G, (int64_t)s.N, (int64_t)s.R}, p.x.scalar_type(), p.x);
+  }
+  if (dx) *dx = empty(with_last(sizes, s.K), p.x.scalar_type(), p.x);
+  const size_t need = cp4_adapter_backward_workspace_bytes(&s, p.dtype);
+  const Tensor ws = scratch(need, p.x);
+  check(cp4_adapter_backward(&s, p.dtype, ptr(p.x), ptr(x), ptr(p.W), ptr(p.A), ptr(p.B), ints(p.ids), floats(p.scale),
+                             static_cast<const float*>(ptr(kept)), dx ? ptr(*dx) : nullptr, dA ? ptr(*dA) : nullptr,
+                             dB ? ptr(*dB) : nullptr, ptr(ws), need, st));
+}
+
+// (x, W, A, B, ids, scale, bias, out, keep, stream) -> y, or (y, kept)
+PyObject* adapter_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  require(n == 10);
+  const Tensor &x = tensor(a[0]), &W = tensor(a[1]), &A = tensor(a[2]), &B = tensor(a[3]), &ids = tensor(a[4]);
+  const auto scale = optional_tensor(a[5]), bias = optional_tensor(a[6]);
+  require(x.is_cuda(), "expected device tensors");
+  const c10::DeviceGuard guard(x.device());
+  Tensor y = a[7] != Py_None ? tensor(a[7]) : Tensor(), kept;
+  const bool keep = PyObject_IsTrue(a[8]) == 1;
+  void* st = stream_of(a[9]);
+  {
+    NoGil unlocked;
+    const at::NoGradGuard no_grad;
+    const Adapters p = adapters(x, W, A, B, ids, scale, bias);
+    require(!y.defined() || (y.is_cuda() && y.device() == x.device() && y.scalar_type() == x.scalar_type() &&
+                             y.is_contiguous() && y.numel() == (int64_t)(p.shape.T * p.shape.N)),
+            "out does not match the result");
+    y = adapter_run(p, x.sizes(), y, keep ? &kept : nullptr, st);
+  }
+  PyObject* py = THPVariable_Wrap(std::move(y));
+  return keep ? Py_BuildValue("(NN)", py, THPVariable_Wrap(std::move(kept))) : py;
+  END_HANDLE_TH_ERRORS
+}
+
+// (dy, x, W, A, B, ids, scale, kept, want_dx, want_factors, stream) -> (dx, dA, dB)
+PyObject* adapter_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  require(n == 11);
+  const Tensor &dy = tensor(a[0]), &W = tensor(a[2]), &A = tensor(a[3]), &B = tensor(a[4]), &ids = tensor(a[5]);
+  const auto x = optional_tensor(a[1]), scale = optional_tensor(a[6]), kept = optional_tensor(a[7]);
+  const bool want_dx = PyObject_IsTrue(a[8]) == 1, want = PyObject_IsTrue(a[9]) == 1;
+  require(!want || (x && kept), "the adapters' gradients need x and what the forward call kept");
+  require(dy.is_cuda(), "expected device tensors");
+  const c10::DeviceGuard guard(dy.device());
+  void* st = stream_of(a[10]);
+  Tensor g[3];
+  {
+    NoGil unlocked;
+    const at::NoGradGuard no_grad;
+    const Adapters p = adapters(dy, W, A, B, ids, scale, std::nullopt, true);
+    adapter_run_backward(p, want ? *x : Tensor(), want ? *kept : Tensor(), dy.sizes(), want_dx ? &g[0] : nullptr,
+                         want ? &g[1] : nullptr, want ? &g[2] : nullptr, st);
+  }
+  PyObject* out = PyTuple_New(3);
+  if (!out) throw python_error();
+  for (int i = 0; i < 3; ++i) {
+    PyObject* o = Py_None;
+    if (g[i].defined()) o = THPVariable_Wrap(std::move(g[i]));
+    else Py_INCREF(o);
+    PyTuple_SET_ITEM(out, i, o);
+  }
+  return out;
+  END_HANDLE_TH_ERRORS
+}
+
+struct AdapterFunction : torch::autograd::Function<AdapterFunction> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& W, const Tensor& A,
+                        const Tensor& B, const Tensor& ids, const std::optional<Tensor>& scale,
+                        const std::optional<Tensor>& bias) {
+    const Adapters p = adapters(x, W, A, B, ids, scale, bias);
+    const bool factors = A.requires_grad() || B.requires_grad();
+    Tensor kept;
+    Tensor y = adapter_run(p, x.sizes(), Tensor(), factors ? &kept : nullptr,
+                           c10::hip::getCurrentHIPStream(x.device().index()).stream());
+    ctx->save_for_backward({factors ? x : Tensor(), W, A, B, ids, scale ? *scale : Tensor(), kept});
+    return y;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grad) {
+    const auto s = ctx->get_saved_variables();
+    torch::autograd::variable_list out(7);
+    if (!grad[0].defined()) return out;
+    Tensor dy = grad[0];
+    if (dy.scalar_type() != s[1].scalar_type()) dy = dy.to(s[1].scalar_type());
+    const bool want_dx = ctx->needs_input_grad(0), want = ctx->needs_input_grad(2) || ctx->needs_input_grad(3);
+    const std::optional<Tensor> scale = s[5].defined() ? std::optional<Tensor>(s[5]) : std::nullopt;
+    const Adapters p = adapters(dy, s[1], s[2], s[3], s[4], scale, std::nullopt, true);
+    Tensor dx, dA, dB;
+    void* st = c10::hip::getCurrentHIPStream(dy.device().index()).stream();
+    adapter_run_backward(p, s[0], s[6], dy.sizes(), want_dx ? &dx : nullptr, want ? &dA : nullptr,
+                         want ? &dB : nullptr, st);
+    out[0] = dx;
+    if (ctx->needs_input_grad(2)) out[2] = dA;
+    if (ctx->needs_input_grad(3)) out[3] = dB;
+    return out;
+  }
+};
+
+// (x, W, A, B, ids, scale, bias) -> y; see torch_ops.adapter_linear
+PyObject* adapter_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  require(n == 7);
+  const Tensor &x = tensor(a[0]), &W = tensor(a[1]), &A = tensor(a[2]), &B = tensor(a[3]), &ids = tensor(a[4]);
+  const auto scale = optional_tensor(a[5]), bias = optional_tensor(a[6]);
+  auto tracked = [](const Tensor& t) {
+    return (at::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined();
+  };
+  if (tracked(W) || (bias && tracked(*bias)) || (scale && tracked(*scale)))
+    fail(PyExc_ValueError, "the projection, its bias and the scales are not trained: detach them");
+  require(x.is_cuda(), "expected device tensors");
+  const c10::DeviceGuard guard(x.device());
+  Tensor y;
+  {
+    NoGil unlocked;
+    if (tracked(x) || tracked(A) || tracked(B)) {
+      y = AdapterFunction::apply(x, W, A, B, ids, scale, bias);
+    } else {
+      const Adapters p = adapters(x, W, A, B, ids, scale, bias);
+      y = adapter_run(p, x.sizes(), Tensor(), nullptr, c10::hip::getCurrentHIPStream(x.device().index()).stream());
+    }
+  }
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// ---- AdamW over many tensors (optim.py) --------------------------------------------------------
+
+// The tensors of a list or tuple; None stays undefined (where `holes`).
+std::vector<Tensor> tensors(PyObject* o, size_t count, const char* what, bool holes = false) {
+  std::vector<Tensor> out(count);
+  if (o == Py_None && holes) return out;
+  PyObject* seq = PySequence_Fast(o, "expected a list of tensors");
+  if (!seq) throw python_error();
+  const bool fits = (size_t)PySequence_Fast_GET_SIZE(seq) == count;
+  bool good = fits;
+  for (size_t i = 0; good && i < count; ++i) {
+    PyObject* v = PySequence_Fast_GET_ITEM(seq, i);
+    if (THPVariable_Check(v)) out[i] = THPVariable_Unpack(v);
+    else good = holes && v == Py_None;
+  }
+  Py_DECREF(seq);
+  require(good, what);
+  return out;
+}
+size_t length(PyObject* o) {
+  const Py_ssize_t n = PySequence_Size(o);
+  if (n < 0) throw python_error();
+  return (size_t)n;
+}
+void* dense(const Tensor& t, int64_t n, const Tensor& like, const char* what) {
+  require(t.is_cuda() && t.device() == like.device() && t.numel() == n && t.is_contiguous(), what);
+  return t.data_ptr();
+}
+constexpr int64_t kMomentBlock = 256;
+// The moments of tensor i: 32 bits, or 8 with their scales [2, blocks].
+void moments_of(cp4_adamw_tensor& t, const Tensor& m, const Tensor& v, const Tensor& scales, const Tensor& like) {
+  const int64_t n = (int64_t)t.n;
+  t.exp_avg = dense(m, n, like, "a moment does not match its tensor");
+  t.exp_avg_sq = dense(v, n, like, "a moment does not match its tensor");
+  if (m.scalar_type() == at::kFloat) {
+    require(v.scalar_type() == at::kFloat, "moments are float32 both, or int8 and uint8");
+    t.bits = 32;
+    return;
+  }
+  require(m.scalar_type() == at::kChar && v.scalar_type() == at::kByte, "moments are float32 both, or int8 and uint8");
+  const int64_t blocks = (n + kMomentBlock - 1) / kMomentBlock;
+  require(scales.defined() && scales.is_cuda() && scales.device() == like.device() &&
+              scales.scalar_type() == at::kFloat && scales.dim() == 2 && scales.size(0) == 2 &&
+              scales.size(1) == blocks && (blocks <= 1 || scales.stride(1) == 1),
+          "8-bit moments have float32 scales [2, ceil(n / 256)]");
+  t.bits = 8;
+  t.scale = static_cast<float*>(scales.data_ptr());
+  t.scale_sq = t.scale + scales.stride(0);
+}
+// What autograd has saved of a tensor that is written here is out of date.
+void written(const std::vector<Tensor>& list) {
+  for (const Tensor& t : list)
+    if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+// (params, grads, exp_avgs, exp_avg_sqs, scales, copies, group of each or None,
+//  [(lr, beta1, beta2, eps, weight_decay, counter)], max_norm, grad_scale, stream) -> norm or None
+PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  require(n_args == 11);
+  const size_t n = length(a[0]), n_groups = length(a[7]);
+  const auto params = tensors(a[0], n, "expected a list of tensors");
+  const auto grads = tensors(a[1], n, "one gradient a parameter", true);
+  const auto ms = tensors(a[2], n, "one first moment a parameter"), vs = tensors(a[3], n, "one second moment a parameter");
+  const auto scales = tensors(a[4], n, "one pair of scales (or None) a parameter", true);
+  const auto copies = tensors(a[5], n, "one copy (or None) a parameter", true);
+  std::vector<cp4_adamw_group> groups(n_groups);
+  std::vector<Tensor> counters(n_groups);
+  PyObject* seq = PySequence_Fast(a[7], "expected a list of groups");
+  if (!seq) throw python_error();
+  for (size_t k = 0; k < n_groups; ++k) {
+    cp4_adamw_group& g = groups[k];
+    PyObject* counter;
+    if (!PyArg_ParseTuple(PySequence_Fast_GET_ITEM(seq, k), "dddddO", &g.lr, &g.beta1, &g.beta2, &g.eps,
+                          &g.weight_decay, &counter)) {
+      Py_DECREF(seq);
+      throw python_error();
+    }
+    if (THPVariable_Check(counter)) counters[k] = THPVariable_Unpack(counter);
+  }
+  Py_DECREF(seq);
+  require(n_groups > 0, "at least one group");
+  const Tensor& like = counters[0];
+  for (size_t k = 0; k < n_groups; ++k) {
+    const Tensor& c = counters[k];
+    require(c.defined() && c.is_cuda() && c.device() == like.device() && c.scalar_type() == at::kDouble &&
+                c.numel() == 4 && c.is_contiguous(),
+            "a counter is four contiguous float64 on the tensors' device");
+    groups[k].counter = static_cast<double*>(c.data_ptr());
+  }
+  std::vector<cp4_adamw_tensor> list;
+  list.reserve(n);
+  for (size_t i = 0; i < n; ++i) {
+    if (!grads[i].defined()) continue;
+    cp4_adamw_tensor t{};
+    t.n = (size_t)params[i].numel();
+    t.param = dense(params[i], (int64_t)t.n, like, "a parameter is not a contiguous tensor on the counter's device");
+    t.param_dtype = dtype_of(params[i]);
+    t.grad = dense(grads[i], (int64_t)t.n, like, "a gradient does not match its parameter");
+    t.grad_dtype = dtype_of(grads[i]);
+    if (copies[i].defined()) {
+      t.copy = dense(copies[i], (int64_t)t.n, like, "a copy does not match its parameter");
+      t.copy_dtype = dtype_of(copies[i]);
+    }
+    moments_of(t, ms[i], vs[i], scales[i], like);
+    if (a[6] != Py_None) {
+      PyObject* g = PySequence_GetItem(a[6], (Py_ssize_t)i);
+      if (!g) throw python_error();
+      const long k = PyLong_AsLong(g);
+      Py_DECREF(g);
+      if (PyErr_Occurred()) throw python_error();
+      require(k >= 0 && (size_t)k < n_groups, "a parameter of a group that is not there");
+      t.group = (unsigned)k;
+    }
+    list.push_back(t);
+  }
+  const double max_norm = a[8] == Py_None ? 0.0 : PyFloat_AsDouble(a[8]);
+  const double grad_scale = PyFloat_AsDouble(a[9]);
+  if (PyErr_Occurred()) throw python_error();
+  require(a[8] == Py_None || max_norm > 0, "max_norm must be above 0");
+  const c10::DeviceGuard guard(like.device());
+  void* st = stream_of(a[10]);
+  Tensor norm;
+  {
+    NoGil unlocked;
+    size_t need = 0;
+    Tensor ws;
+    if (max_norm > 0) {
+      need = cp4_adamw_workspace_bytes();
+      ws = scratch(need, like);
+      norm = empty({}, at::kFloat, like);
+    }
+    check(cp4_adamw_step(list.data(), list.size(), groups.data(), n_groups, (float)grad_scale, (float)max_norm,
+                         static_cast<float*>(ptr(norm)), ptr(ws), need, st));
+    for (const auto* l : {&params, &ms, &vs, &scales, &copies}) written(*l);
+    written(counters);
+  }
+  if (!norm.defined()) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(norm));
+  END_HANDLE_TH_ERRORS
+}
+
+// (exp_avgs, exp_avg_sqs, scales, values, values_sq, encode, stream): codes to values, or back
+PyObject* adamw_moments(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  require(n_args == 7);
+  const size_t n = length(a[0]);
+  const auto ms = tensors(a[0], n, "expected a list of tensors"), vs = tensors(a[1], n, "one second moment a first");
+  const auto scales = tensors(a[2], n, "one pair of scales a moment");
+  const auto to_m = tensors(a[3], n, "one tensor of values a moment"), to_v = tensors(a[4], n, "one tensor of values a moment");
+  const bool encode = PyObject_IsTrue(a[5]) == 1;
+  if (!n) Py_RETURN_NONE;
+  std::vector<cp4_adamw_tensor> list(n);
+  std::vector<float*> pm(n), pv(n);
+  for (size_t i = 0; i < n; ++i) {
+    list[i].n = (size_t)ms[i].numel();
+    moments_of(list[i], ms[i], vs[i], scales[i], ms[0]);
+    require(list[i].bits == 8, "expected 8-bit moments");
+    require(to_m[i].scalar_type() == at::kFloat && to_v[i].scalar_type() == at::kFloat, "values are float32");
+    pm[i] = static_cast<float*>(dense(to_m[i], (int64_t)list[i].n, ms[0], "values do not match their moment"));
+    pv[i] = static_cast<float*>(dense(to_v[i], (int64_t)list[i].n, ms[0], "values do not match their moment"));
+  }
+  const c10::DeviceGuard guard(ms[0].device());
+  void* st = stream_of(a[6]);
+  {
+    NoGil unlocked;
+    if (encode) {
+      check(cp4_adamw_set_moments(list.data(), n, pm.data(), pv.data(), st));
+      for (const auto* l : {&ms, &vs, &scales}) written(*l);
+    } else {
+      check(cp4_adamw_moments(list.data(), n, pm.data(), pv.data(), st));
+      for (const auto* l : {&to_m, &to_v}) written(*l);
+    }
+  }
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 PyObject* set_error(PyObject*, PyObject* type) {
   Py_XINCREF(type);
   Py_XSETREF(g_error, type);
@@ -461,6 +866,11 @@ PyMethodDef kMethods[] = {
     {"backward_data", FAST(backward_data), nullptr},
     {"backward_filter", FAST(backward_filter), nullptr},
     {"layer", FAST(layer), nullptr},
+    {"adapter_forward", FAST(adapter_forward), nullptr},
+    {"adapter_backward", FAST(adapter_backward), nullptr},
+    {"adapter_linear", FAST(adapter_linear), nullptr},
+    {"adamw_step", FAST(adamw_step), nullptr},
+    {"adamw_moments", FAST(adamw_moments), nullptr},
     {"set_error", set_error, METH_O, nullptr},
     {"set_check_backward", set_check_backward, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};

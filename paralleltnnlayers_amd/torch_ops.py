@@ -289,3 +289,38 @@ class RCPConv2dFunction(torch.autograd.Function):
 def rcp_conv2d(x, K0, K1, KC, pad):
     """Functional form of the differentiable reshaped-CP convolution (NCHW)."""
     return RCPConv2dFunction.apply(x, K0, K1, KC, pad)
+
+
+def adapter_linear(x, W, A, B, ids, scale=None, bias=None):
+    """Functional form of a dense projection with the low-rank adapters of many requests
+    beside it (``capi.adapter_forward``), differentiable in x, A and B.
+
+    W and bias are frozen: a call that asks for their gradient raises ``ValueError``."""
+    return capi._native.adapter_linear(x, W, A, B, ids, scale, bias)
+
+
+class AdapterLinear(torch.nn.Module):
+    """A frozen dense projection [out_features, in_features] with ``adapters`` low-rank
+    adapters of rank ``rank`` that are trained, each token through the one that ``ids`` names.
+
+    A starts as normal(0, 1 / sqrt(in_features)), B as zero, so that an adapter starts as
+    nothing; ``alpha / rank`` scales all of them.  ``weight`` and ``bias``: the projection's, as of
+    a trained layer (kept as buffers); without them it starts as a Kaiming-normal one."""
+
+    def __init__(self, in_features, out_features, rank, adapters=1, alpha=None, weight=None, bias=None,
+                 dtype=torch.float32, device="cuda"):
+        super().__init__()
+        if weight is None:
+            weight = torch.randn(out_features, in_features, device=device) * (2.0 / in_features) ** 0.5
+        if tuple(weight.shape) != (out_features, in_features):
+            raise ValueError("weight must be [out_features, in_features]")
+        self.register_buffer("weight", weight.detach().to(device, dtype))
+        self.register_buffer("bias", None if bias is None else bias.detach().to(device, torch.float32))
+        self.register_buffer("scale", torch.full((adapters,), (rank if alpha is None else alpha) / rank,
+                                                 device=device))
+        self.A = torch.nn.Parameter((torch.randn(adapters, rank, in_features, device=device) *
+                                     in_features ** -0.5).to(dtype))
+        self.B = torch.nn.Parameter(torch.zeros(adapters, out_features, rank, device=device, dtype=dtype))
+
+    def forward(self, x, ids):
+        return adapter_linear(x, self.weight, self.A, self.B, ids, self.scale, self.bias)
