@@ -34,6 +34,7 @@ struct ProjectArgs {
   size_t T, ldz, ldw;
   int K, N, R, Rp, G;
   int fn, fr;
+  int planes;             // h is the sum of so many planes [T][Rp]
 };
 
 // out[a][r][c] = sum over tokens with ids[t] = a of p[t][r] z[t][c], at out + a * R * C + r * outr +
@@ -52,7 +53,18 @@ struct GradArgs {
 };
 
 hipError_t shrink_launch(const ShrinkArgs&, int dtype, hipStream_t);
-hipError_t project_launch(const ProjectArgs&, int dtype, bool nn, hipStream_t);
+// part: project_part_bytes of scratch memory.
+size_t project_part_bytes(size_t T, int K, int N, int dtype);
+hipError_t project_launch(const ProjectArgs&, float* part, int dtype, bool nn, hipStream_t);
+// The tiles of a projection on the matrix cores, its depth in `splits` parts of `each` steps, whose partial
+// sums take tile_part_bytes.
+struct TilePlan {
+  int which, splits, each;
+};
+TilePlan tile_plan(size_t T, int K, int N, int dtype);
+size_t tile_part_bytes(const TilePlan&, size_t T, int N);
+bool tile_supported(const ProjectArgs&, int dtype, bool nn);
+hipError_t tile_launch(const ProjectArgs&, const TilePlan&, float* part, int dtype, bool nn, hipStream_t);
 int grad_splits(size_t T, int C, int R, int G);
 hipError_t grad_launch(const GradArgs&, int dtype, hipStream_t);
 

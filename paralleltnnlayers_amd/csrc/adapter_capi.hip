@@ -41,14 +41,14 @@ struct BackwardPlan {
   int splits_a, splits_b;
   size_t dh_at, part_at, total;
 };
-BackwardPlan backward_plan(const cp4_adapter_shape& s) {
+BackwardPlan backward_plan(const cp4_adapter_shape& s, int dtype) {
   BackwardPlan p{};
   p.splits_a = grad_splits(s.T, (int)s.K, (int)s.R, (int)s.G);
   p.splits_b = grad_splits(s.T, (int)s.N, (int)s.R, (int)s.G);
   p.part_at = align256(s.T * padded(s) * 4);
   const size_t each = (size_t)s.G * s.R * 4;
   const size_t pa = p.splits_a > 1 ? p.splits_a * each * s.K : 0, pb = p.splits_b > 1 ? p.splits_b * each * s.N : 0;
-  p.total = p.part_at + align256(std::max(pa, pb));    // (one after the other)
+  p.total = p.part_at + align256(std::max({pa, pb, project_part_bytes(s.T, (int)s.N, (int)s.K, dtype)}));   // (one after the other)
   return p;
 }
 
@@ -60,7 +60,7 @@ extern "C" size_t cp4_adapter_kept_bytes(const cp4_adapter_shape* s) {
 
 extern "C" size_t cp4_adapter_forward_workspace_bytes(const cp4_adapter_shape* s, int dtype) {
   if (check_shape(s, dtype) != CP4_OK) return 0;
-  return align256(cp4_adapter_kept_bytes(s));
+  return align256(cp4_adapter_kept_bytes(s)) + align256(project_part_bytes(s->T, (int)s->K, (int)s->N, dtype));
 }
 
 extern "C" cp4_status cp4_adapter_forward(const cp4_adapter_shape* s, int dtype, const void* x, const void* W,
@@ -87,14 +87,15 @@ extern "C" cp4_status cp4_adapter_forward(const cp4_adapter_shape* s, int dtype,
   p.z = x; p.w = W; p.f = B; p.h = h; p.bias = bias; p.ids = ids; p.y = y;
   p.T = s->T; p.ldz = sh.ldz; p.ldw = s->ldw ? s->ldw : s->K;
   p.K = (int)s->K; p.N = (int)s->N; p.R = (int)s->R; p.Rp = sh.Rp; p.G = (int)s->G;
-  p.fn = (int)s->R; p.fr = 1;
-  if (const hipError_t e = project_launch(p, dtype, false, st)) return fail_hip(e, "cp4_adapter_forward");
+  p.fn = (int)s->R; p.fr = 1; p.planes = 1;
+  float* const part = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(cp4_adapter_kept_bytes(s)));
+  if (const hipError_t e = project_launch(p, part, dtype, false, st)) return fail_hip(e, "cp4_adapter_forward");
   return CP4_OK;
 }
 
 extern "C" size_t cp4_adapter_backward_workspace_bytes(const cp4_adapter_shape* s, int dtype) {
   if (check_shape(s, dtype) != CP4_OK) return 0;
-  return backward_plan(*s).total;
+  return backward_plan(*s, dtype).total;
 }
 
 extern "C" cp4_status cp4_adapter_backward(const cp4_adapter_shape* s, int dtype, const void* dy, const void* x,
@@ -109,7 +110,7 @@ extern "C" cp4_status cp4_adapter_backward(const cp4_adapter_shape* s, int dtype
     if (const cp4_status rc = check_pointers(value_bytes(dtype), {dy, x, W, A, B, dx, dA, dB}, {ids, scale})) return rc;
     if ((size_t)kept & 15) return fail_with(CP4_ERR_WORKSPACE, "kept is not aligned to 16 bytes");
   }
-  const BackwardPlan plan = backward_plan(*s);
+  const BackwardPlan plan = backward_plan(*s, dtype);
   if (plan.total && (!workspace || workspace_bytes < plan.total || ((size_t)workspace & 255)))
     return fail_with(CP4_ERR_WORKSPACE, "workspace missing, too small or not aligned to 256 bytes");
   const hipStream_t st = static_cast<hipStream_t>(stream);
@@ -130,8 +131,8 @@ extern "C" cp4_status cp4_adapter_backward(const cp4_adapter_shape* s, int dtype
     p.z = dy; p.w = W; p.f = A; p.h = dh; p.ids = ids; p.y = dx;
     p.T = s->T; p.ldz = lddy; p.ldw = s->ldw ? s->ldw : s->K;
     p.K = (int)s->N; p.N = (int)s->K; p.R = (int)s->R; p.Rp = Rp; p.G = (int)s->G;
-    p.fn = 1; p.fr = (int)s->K;
-    if (const hipError_t e = project_launch(p, dtype, true, st)) return fail_hip(e, "cp4_adapter_backward");
+    p.fn = 1; p.fr = (int)s->K; p.planes = 1;
+    if (const hipError_t e = project_launch(p, part, dtype, true, st)) return fail_hip(e, "cp4_adapter_backward");
   }
   if (dA) {
     GradArgs g{};

@@ -112,7 +112,12 @@ void general(const ProjectArgs& a, bool nn, hipStream_t st) {
 
 }  // namespace
 
-hipError_t project_launch(const ProjectArgs& a, int dtype, bool nn, hipStream_t st) {
+size_t project_part_bytes(size_t T, int K, int N, int dtype) {
+  return tile_part_bytes(tile_plan(T, K, N, dtype), T, N);
+}
+
+hipError_t project_launch(const ProjectArgs& a, float* part, int dtype, bool nn, hipStream_t st) {
+  if (tile_supported(a, dtype, nn)) return tile_launch(a, tile_plan(a.T, a.K, a.N, dtype), part, dtype, nn, st);
   if (dtype == CP4_DTYPE_F32) general<F32>(a, nn, st);
   else if (dtype == CP4_DTYPE_BF16) general<BF16>(a, nn, st);
   else general<F16>(a, nn, st);

@@ -1,0 +1,524 @@
+// The shared projection on the matrix cores (include/cp4/adapter.h), for rows that start on 16-byte
+// boundaries: tiles of 64 or 128 rows x 128 or 256 columns, fed through the LDS by loads that never
+// pass a register.
+//
+// A step is 64 bytes of depth (32 values of 16 bits, 16 of fp32) of all the tile's rows and columns.
+// Three steps' room in the LDS: while one is multiplied the next two are on their way, and
+// one barrier a step says both that the next one has arrived and that the last one's room is free.
+// A wave has 64 rows and 64 or 128 columns in registers; two workgroups on a compute unit keep its
+// matrix cores busy over each other's barriers.
+//
+// A wave's column block j holds the columns n0 + NB * l + j (l: lane & 15), not 16 j + l: a lane then
+// has NB consecutive values of every output row (one or two 16-byte stores), and where w is [K][N] (nn)
+// the same order lets one load bring NB blocks' values, which are turned in registers (one byte permute
+// for two values).
+//
+// The adapters: when a tile's sum is done, h F_a^T is added for each adapter that the wave's rows have (a
+// 16-deep product a rank block against a sum over thousands of inputs), so y is written once.
+//
+// Little work for the chip is split over the depth: the partial tiles go to the workspace in
+// fp32 (the first one with the adapters' part) and a second launch adds them up in their order.
+#include <algorithm>
+
+#include "adapter.h"
+#include "die_order.h"
+
+namespace cp4 {
+namespace adapter {
+namespace {
+
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
+
+template <class T>
+constexpr int kStep = 64 / sizeof(typename T::raw);                  // depth of a step
+template <class T>
+constexpr int kVec = 16 / sizeof(typename T::raw);                   // values of a 16-byte load
+
+// s_waitcnt's operand: all but `loads` memory loads done, and all of the LDS's.
+constexpr int wait_for(int loads) { return (loads & 15) | (loads >> 4) << 14 | 7 << 4; }
+
+// 8 rows (depths) of NB columns in 16 bits -> NB columns of 8 depths.
+template <int NB>
+__device__ __forceinline__ void turn(const unsigned (&in)[8][NB / 2], u16x8 (&out)[NB]) {
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    u32x4 d;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      d[q] = __builtin_amdgcn_perm(in[2 * q + 1][j / 2], in[2 * q][j / 2], j & 1 ? 0x07060302u : 0x05040100u);
+    out[j] = __builtin_bit_cast(u16x8, d);
+  }
+}
+
+// `count` (may be <= 0 or beyond n) values of p, zero behind; vec: p is on a 16-byte boundary.
+template <int n, class Raw>
+__device__ __forceinline__ void load_some(const Raw* p, int count, bool vec, Raw (&v)[n]) {
+  if (vec && count >= n) {
+    constexpr int each = 16 / sizeof(Raw);
+    if constexpr (n >= each) {
+#pragma unroll
+      for (int i = 0; i < n / each; ++i) {
+        const u32x4 d = reinterpret_cast<const u32x4*>(p)[i];
+        __builtin_memcpy(&v[i * each], &d, 16);
+      }
+      return;
+    } else if constexpr (n * sizeof(Raw) == 8) {
+      const u32x2 d = *reinterpret_cast<const u32x2*>(p);
+      __builtin_memcpy(&v[0], &d, 8);
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < n; ++i) v[i] = i < count ? p[i] : Raw(0);
+}
+
+// Adds h F_a^T to a wave's MB x NB blocks (columns as above) for the rows whose bit is set; see expand()
+// in adapter.h.  planes: h is the sum of so many planes of T * Rp values.
+template <class T, bool NN, int MB, int NB>
+__device__ __forceinline__ void expand_wave(const ProjectArgs& a, const float* h, unsigned long long whose,
+                                            const typename T::raw* f, bool vec, int n0, f32x4 (&acc)[MB][NB]) {
+  typedef typename T::raw Raw;
+  const int lane = threadIdx.x & 63, l = lane & 15, g = lane >> 4, n = n0 + NB * l;
+  constexpr bool kF32 = __is_same(T, F32);
+  for (int r0 = 0; r0 < a.R; r0 += 16) {
+    // fp32: depth 4 g + q in product q; 16 bits: ranks 8 (g & 1) + q, first parts for g < 2
+    const int rl = kF32 ? 4 * g : 8 * (g & 1);
+    constexpr int kOwn = kF32 ? 4 : 8;
+    float hv[MB][kOwn];
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+#pragma unroll
+      for (int q = 0; q < kOwn; ++q) hv[i][q] = 0.0f;
+      if (whose >> (16 * i + l) & 1) {
+        const float* p = h + (size_t)16 * i * a.Rp + r0 + rl;
+        for (int s = 0; s < a.planes; ++s, p += a.T * (size_t)a.Rp)
+#pragma unroll
+          for (int q = 0; q < kOwn; q += 4) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(p + q);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) hv[i][q + e] += x[e];
+          }
+      }
+    }
+    Raw fv[NB][kOwn];                                                // [column][rank]
+    if constexpr (NN) {
+      Raw fr[kOwn][NB];
+#pragma unroll
+      for (int q = 0; q < kOwn; ++q)
+        load_some<NB>(f + (size_t)(r0 + rl + q) * a.fr + n, r0 + rl + q < a.R ? a.N - n : 0, vec, fr[q]);
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int q = 0; q < kOwn; ++q) fv[j][q] = fr[q][j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+        load_some<kOwn>(f + (size_t)(n + j) * a.fn + r0 + rl, n + j < a.N ? a.R - r0 - rl : 0, vec, fv[j]);
+    }
+    u16x8 ha[MB];
+    if constexpr (!kF32) {
+#pragma unroll
+      for (int i = 0; i < MB; ++i) {
+        u16x8 hi, lo;
+        two_parts(hv[i], hi, lo);
+        ha[i] = g < 2 ? hi : lo;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      u16x8 fh = {}, fl = {};
+      if constexpr (__is_same(T, F16)) {
+        float x[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) x[q] = F16::widen(fv[j][q]);
+        two_parts(x, fh, fl);
+      } else if constexpr (!kF32) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) fh[q] = fv[j][q];
+      }
+#pragma unroll
+      for (int i = 0; i < MB; ++i) {
+        const unsigned rows = (unsigned)(whose >> (16 * i)) & 0xffffu;
+        if (!rows) continue;
+        f32x4 d = acc[i][j];
+        if constexpr (kF32) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) d = mfma_f32(hv[i][q], fv[j][q], d);
+        } else {
+          if constexpr (__is_same(T, F16)) d = mfma_bf16(ha[i], fl, d);
+          d = mfma_bf16(ha[i], fh, d);
+        }
+        if (rows == 0xffffu) {
+          acc[i][j] = d;
+        } else {
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            if (rows >> (4 * g + v) & 1) acc[i][j][v] = d[v];
+        }
+      }
+    }
+  }
+}
+
+struct TileArgs {
+  ProjectArgs p;
+  float* part;            // [splits][T][N], or null: y
+  int mt, nt, splits;     // tiles, and parts of the depth
+  int steps;              // of a part (the last one may have fewer)
+};
+
+// One wave of a tile: MB x NB blocks of 16 x 16.
+template <class T, bool NN, int MB, int NB, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta) {
+  typedef typename T::raw Raw;
+  constexpr int kThreads = 64 * WM * WN, BM = 16 * MB * WM, BN = 16 * NB * WN, KS = kStep<T>;
+  constexpr int kZ = BM * 4 / kThreads, kW = BN * 4 / kThreads;      // 16-byte loads of a thread and step
+  static_assert(BM * 4 % kThreads == 0 && BN * 4 % kThreads == 0, "whole loads");
+  // (three variables, so that the compiler knows a load into one from a read of another)
+  __shared__ __attribute__((aligned(1024))) char lds0[(BM + BN) * 64], lds1[(BM + BN) * 64], lds2[(BM + BN) * 64];
+  const ProjectArgs& a = ta.p;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 15, g = lane >> 4;
+  // the place of this workgroup: each die a contiguous run of tiles, up to eight columns of tiles wide
+  const int place = die_place(blockIdx.x, ta.mt * ta.nt * ta.splits);
+  if (place < 0) return;
+  const int split = place % ta.splits, tile = place / ta.splits;
+  const int band = tile / (8 * ta.mt), in_band = tile % (8 * ta.mt), wide = min(8, ta.nt - 8 * band);
+  const int tm = in_band / wide, tn = 8 * band + in_band % wide;
+  const size_t t0 = (size_t)tm * BM;
+  const int n0 = tn * BN, wm = 16 * MB * (wave / WN), wn = 16 * NB * (wave % WN);
+  const int rows = (int)min((size_t)BM, a.T - t0), cols = min(BN, a.N - n0);
+  const int k_first = split * ta.steps * KS, k_last = min(a.K, k_first + ta.steps * KS);
+  const int steps = (k_last - k_first) / KS;
+
+  const char* zb = reinterpret_cast<const char*>(static_cast<const Raw*>(a.z) + t0 * a.ldz + k_first);
+  const char* wb = reinterpret_cast<const char*>(static_cast<const Raw*>(a.w) +
+                                                 (NN ? (size_t)k_first * a.ldw + n0 : (size_t)n0 * a.ldw + k_first));
+  const size_t w_next = NN ? (size_t)KS * a.ldw * sizeof(Raw) : 64;
+  // What each thread brings: the LDS is filled in the threads' order; which 16 bytes come there is theirs to choose.
+  // Rows beyond the operand's are read again from its last one: what they give is not stored.
+  unsigned zo[kZ], wo[kW];
+#pragma unroll
+  for (int i = 0; i < kZ; ++i) {
+    const int at = i * kThreads + threadIdx.x, row = at >> 2, chunk = (at & 3) ^ (row >> 1 & 3);
+    zo[i] = (unsigned)(min(row, rows - 1) * a.ldz * sizeof(Raw)) + chunk * 16;
+  }
+#pragma unroll
+  for (int i = 0; i < kW; ++i) {
+    const int at = i * kThreads + threadIdx.x;
+    if constexpr (NN) {
+      constexpr int kRow = BN / kVec<T>;                             // 16-byte pieces of a row
+      wo[i] = (unsigned)(at / kRow * a.ldw * sizeof(Raw)) + min(at % kRow, (cols - 1) / kVec<T>) * 16;
+    } else {
+      const int slot = at >> 2, chunk = (at & 3) ^ (slot >> 1 & 3), in = slot % (16 * NB);
+      const int col = slot - in + NB * (in & 15) + in / 16;
+      wo[i] = (unsigned)(min(col, cols - 1) * a.ldw * sizeof(Raw)) + chunk * 16;
+    }
+  }
+  int brought = 0;
+  auto bring = [&](char* lds) {
+#pragma unroll
+    for (int i = 0; i < kZ; ++i)
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(zb + zo[i]),
+                                       (__attribute__((address_space(3))) void*)(lds + (i * kThreads + wave * 64) * 16), 16, 0, 0);
+#pragma unroll
+    for (int i = 0; i < kW; ++i)
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(wb + wo[i]),
+                                       (__attribute__((address_space(3))) void*)(lds + BM * 64 + (i * kThreads + wave * 64) * 16), 16, 0, 0);
+    const bool more = ++brought < steps;                             // (beyond the last step that one again)
+    zb += more ? 64 : 0;
+    wb += more ? w_next : 0;
+  };
+
+  f32x4 acc[MB][NB] = {};
+  const int z_at = (wm + l) * 64 + ((g ^ (l >> 1 & 3)) * 16), w_at = BM * 64 + (NN ? 0 : (wn + l) * 64 + ((g ^ (l >> 1 & 3)) * 16));
+  auto multiply = [&](const char* lds) {
+    if constexpr (__is_same(T, F32)) {
+      f32x4 zf[MB];
+#pragma unroll
+      for (int i = 0; i < MB; ++i) zf[i] = *reinterpret_cast<const f32x4*>(lds + z_at + i * 1024);
+      float wf[4][NB];
+      if constexpr (NN) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int j = 0; j < NB; j += 4) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(lds + w_at + ((4 * g + q) * BN + wn + NB * l + j) * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) wf[q][j + e] = x[e];
+          }
+      } else {
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          const f32x4 x = *reinterpret_cast<const f32x4*>(lds + w_at + j * 1024);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) wf[q][j] = x[q];
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+          for (int i = 0; i < MB; ++i) acc[i][j] = mfma_f32(zf[i][q], wf[q][j], acc[i][j]);
+    } else {
+      u16x8 zf[MB], wf[NB];
+#pragma unroll
+      for (int i = 0; i < MB; ++i) zf[i] = *reinterpret_cast<const u16x8*>(lds + z_at + i * 1024);
+      if constexpr (NN) {
+        unsigned in[8][NB / 2];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const char* const p = lds + w_at + ((8 * g + q) * BN + wn + NB * l) * 2;
+          if constexpr (NB == 8) {
+            const u32x4 x = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) in[q][e] = x[e];
+          } else {
+            const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+            in[q][0] = x[0];
+            in[q][1] = x[1];
+          }
+        }
+        turn<NB>(in, wf);
+      } else {
+#pragma unroll
+        for (int j = 0; j < NB; ++j) wf[j] = *reinterpret_cast<const u16x8*>(lds + w_at + j * 1024);
+      }
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int i = 0; i < MB; ++i) acc[i][j] = mfma_16<T>(zf[i], wf[j], acc[i][j]);
+    }
+  };
+  // A step: its own loads have arrived (those of the next one may still be on their way), and nobody reads the
+  // last one's room any more.  Every step brings one, so that no branch keeps the compiler from
+  // counting the loads under way.
+  auto step = [&](const char* lds, char* into) {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(wait_for(kZ + kW));
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    bring(into);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(lds);
+  };
+  if (steps > 0) {
+    bring(lds0);
+    asm volatile("" ::: "memory");                                   // (their order is what the waits count on)
+    __builtin_amdgcn_sched_barrier(0);
+    bring(lds1);
+    int left = steps;                                                // (no way out in the middle: the same reason)
+    for (; left >= 3; left -= 3) {
+      step(lds0, lds2);
+      step(lds1, lds0);
+      step(lds2, lds1);
+    }
+    if (left > 0) step(lds0, lds2);
+    if (left > 1) step(lds1, lds0);
+    __builtin_amdgcn_s_waitcnt(wait_for(0));                         // (the loads beyond the last step)
+  }
+  if (k_first + steps * KS < k_last) {
+    // The depth's rest, through registers, zero behind it.
+    const int left = k_last - k_first - steps * KS;
+    zb = reinterpret_cast<const char*>(static_cast<const Raw*>(a.z) + t0 * a.ldz + k_last - left);
+    wb = reinterpret_cast<const char*>(static_cast<const Raw*>(a.w) + (NN ? (size_t)(k_last - left) * a.ldw + n0
+                                                                          : (size_t)n0 * a.ldw + k_last - left));
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kZ; ++i) {
+      const int at = i * kThreads + threadIdx.x, chunk = (at & 3) ^ (at >> 3 & 3);
+      u32x4 x = {};
+      if (chunk * kVec<T> < left) {
+        if constexpr (NN) {                                          // (z's row may end inside the 16 bytes)
+          Raw v[kVec<T>];
+          load_some<kVec<T>>(reinterpret_cast<const Raw*>(zb + zo[i]), left - chunk * kVec<T>, true, v);
+          __builtin_memcpy(&x, v, 16);
+        } else {
+          x = *reinterpret_cast<const u32x4*>(zb + zo[i]);
+        }
+      }
+      *reinterpret_cast<u32x4*>(lds0 + at * 16) = x;
+    }
+#pragma unroll
+    for (int i = 0; i < kW; ++i) {
+      const int at = i * kThreads + threadIdx.x;
+      const int depth = NN ? at / (BN / kVec<T>) : ((at & 3) ^ (at >> 3 & 3)) * kVec<T>;
+      u32x4 x = {};
+      if (depth < left) x = *reinterpret_cast<const u32x4*>(wb + wo[i]);
+      *reinterpret_cast<u32x4*>(lds0 + BM * 64 + at * 16) = x;
+    }
+    __syncthreads();
+    multiply(lds0);
+  }
+
+  const bool even_f = ((size_t)a.f & 15) == 0 && (NN ? a.N : a.R) % kVec<T> == 0;
+  if (split == 0) {
+    const size_t row = t0 + wm + lane;
+    int id = lane < 16 * MB && row < a.T ? a.ids[row] : -1;
+    if (id >= a.G) id = -1;
+    Adapters todo(id);
+    int ad;
+    unsigned long long whose;
+    while (todo.take(ad, whose))
+      expand_wave<T, NN, MB, NB>(a, a.h + (t0 + wm + l) * a.Rp, whose, static_cast<const Raw*>(a.f) + (size_t)ad * a.R * a.N,
+                                 even_f, n0 + wn, acc);
+  }
+  const int n = n0 + wn + NB * l;
+  if (n >= a.N) return;
+  if (ta.part) {
+    float* const y = ta.part + ((size_t)split * a.T + t0 + wm) * a.N + n;
+    const bool whole = n + NB <= a.N && a.N % 4 == 0;
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const int row = 16 * i + 4 * g + v;
+        if (t0 + wm + row >= a.T) continue;
+        float* const p = y + (size_t)row * a.N;
+        if (whole) {
+#pragma unroll
+          for (int j = 0; j < NB; j += 4)
+            *reinterpret_cast<f32x4*>(p + j) = f32x4{acc[i][j][v], acc[i][j + 1][v], acc[i][j + 2][v], acc[i][j + 3][v]};
+        } else {
+#pragma unroll
+          for (int j = 0; j < NB; ++j)
+            if (n + j < a.N) p[j] = acc[i][j][v];
+        }
+      }
+    return;
+  }
+  float bias[NB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) bias[j] = a.bias && n + j < a.N ? a.bias[n + j] : 0.0f;
+  Raw* const y = static_cast<Raw*>(a.y) + (t0 + wm) * a.N + n;
+  const bool whole = n + NB <= a.N && a.N * sizeof(Raw) % (NB == 4 && sizeof(Raw) == 2 ? 8 : 16) == 0 && ((size_t)a.y & 15) == 0;
+#pragma unroll
+  for (int i = 0; i < MB; ++i)
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const int row = 16 * i + 4 * g + v;
+      if (t0 + wm + row >= a.T) continue;
+      Raw* const p = y + (size_t)row * a.N;
+      Raw o[NB];
+#pragma unroll
+      for (int j = 0; j < NB; ++j) o[j] = T::narrow(acc[i][j][v] + bias[j]);
+      if (whole) {
+        if constexpr (sizeof(o) == 8) {
+          u32x2 d;
+          __builtin_memcpy(&d, o, 8);
+          *reinterpret_cast<u32x2*>(p) = d;
+        } else {
+#pragma unroll
+          for (int j = 0; j < NB; j += kVec<T>) {
+            u32x4 d;
+            __builtin_memcpy(&d, o + j, 16);
+            *reinterpret_cast<u32x4*>(p + j) = d;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+          if (n + j < a.N) p[j] = o[j];
+      }
+    }
+}
+
+// The depth's parts, in their order, and the bias.
+template <class T>
+__global__ __launch_bounds__(256) void join_kernel(const float* part, const float* bias, void* y, size_t n, int N, int splits) {
+  const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  typename T::raw* const o = static_cast<typename T::raw*>(y) + i;
+  if (n % 4 == 0 && N % 4 == 0) {
+    f32x4 x = *reinterpret_cast<const f32x4*>(part + i);
+    for (int s = 1; s < splits; ++s) x += *reinterpret_cast<const f32x4*>(part + s * n + i);
+    if (bias) {
+      const int c = (int)(i % N);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] += bias[c + j];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = T::narrow(x[j]);
+    return;
+  }
+  for (int j = 0; j < 4 && i + j < n; ++j) {
+    float x = part[i + j];
+    for (int s = 1; s < splits; ++s) x += part[s * n + i + j];
+    if (bias) x += bias[(i + j) % N];
+    o[j] = T::narrow(x);
+  }
+}
+
+template <class T, bool NN, int MB, int NB, int WM, int WN>
+void launch(TileArgs t, hipStream_t st) {
+  tile_kernel<T, NN, MB, NB, WM, WN><<<die_grid((long)t.mt * t.nt * t.splits), 64 * WM * WN, 0, st>>>(t);
+  if (t.splits > 1) {
+    const size_t n = t.p.T * (size_t)t.p.N;
+    join_kernel<T><<<(unsigned)((n + 1023) / 1024), 256, 0, st>>>(t.part, t.p.bias, t.p.y, n, t.p.N, t.splits);
+  }
+}
+template <class T, bool NN>
+void launch_shape(const TileArgs& t, int which, hipStream_t st) {
+  if (which == 0) launch<T, NN, 4, 8, 2, 2>(t, st);
+  else if (which == 1) launch<T, NN, 4, 4, 2, 2>(t, st);
+  else launch<T, NN, 4, 4, 1, 4>(t, st);
+}
+
+constexpr int kRows[3] = {128, 128, 64}, kCols[3] = {256, 128, 256};
+
+}  // namespace
+
+TilePlan tile_plan(size_t T, int K, int N, int dtype) {
+  const int KS = dtype == CP4_DTYPE_F32 ? 16 : 32;
+  const long slots = 2L * num_compute_units();
+  const int steps = (K + KS - 1) / KS;
+  TilePlan best{};
+  double least = 0;
+  for (int w = 0; w < 3; ++w) {
+    const long tiles = (long)((T + kRows[w] - 1) / kRows[w]) * ((N + kCols[w] - 1) / kCols[w]);
+    for (int s = 1; s <= 64 && s <= std::max(1, steps / 4); s *= 2) {
+      const int each = (steps + s - 1) / s;
+      const long wgs = tiles * ((steps + each - 1) / each);
+      // steps of a round of workgroups, by what a step takes of the matrix cores, and the parts' way to memory and back
+      const double rate = w == 0 ? 1.0 : w == 1 ? 0.65 : 0.65;
+      const double per = (double)kRows[w] * kCols[w] / rate * each + 256.0 * 128 * 12;
+      double cost = per * ((wgs + slots - 1) / slots);
+      if (s > 1) cost += 256.0 * 128 * 40 + (double)T * N * (s + 1) * 4.0 * 0.11;
+      if (!best.splits || cost < least) {
+        least = cost;
+        best.which = w;
+        best.each = each;
+        best.splits = (steps + each - 1) / each;
+      }
+    }
+  }
+  return best;
+}
+size_t tile_part_bytes(const TilePlan& p, size_t T, int N) { return p.splits > 1 ? (size_t)p.splits * T * N * 4 : 0; }
+
+bool tile_supported(const ProjectArgs& a, int dtype, bool nn) {
+  const size_t e = dtype == CP4_DTYPE_F32 ? 4 : 2, vec = 16 / e;
+  if (((size_t)a.z & 15) || ((size_t)a.w & 15) || a.ldz % vec || a.ldw % vec) return false;
+  if (nn ? a.N % vec : a.K % vec) return false;
+  // (a thread's places in a tile are 32-bit byte offsets)
+  return a.ldz * e * 128 < (size_t)1 << 31 && a.ldw * e * 256 < (size_t)1 << 31 && a.T < ((size_t)1 << 31) - 256;
+}
+
+hipError_t tile_launch(const ProjectArgs& a, const TilePlan& plan, float* part, int dtype, bool nn, hipStream_t st) {
+  TileArgs t{};
+  t.p = a;
+  t.part = plan.splits > 1 ? part : nullptr;
+  t.mt = (int)((a.T + kRows[plan.which] - 1) / kRows[plan.which]);
+  t.nt = (a.N + kCols[plan.which] - 1) / kCols[plan.which];
+  t.splits = plan.splits;
+  t.steps = plan.each;
+  if (dtype == CP4_DTYPE_F32) nn ? launch_shape<F32, true>(t, plan.which, st) : launch_shape<F32, false>(t, plan.which, st);
+  else if (dtype == CP4_DTYPE_BF16) nn ? launch_shape<BF16, true>(t, plan.which, st) : launch_shape<BF16, false>(t, plan.which, st);
+  else nn ? launch_shape<F16, true>(t, plan.which, st) : launch_shape<F16, false>(t, plan.which, st);
+  return hipGetLastError();
+}
+
+}  // namespace adapter
+}  // namespace cp4
