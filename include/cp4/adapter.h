@@ -39,7 +39,7 @@ typedef struct cp4_adapter_shape {
 } cp4_adapter_shape;
 
 /* What a forward call leaves for the backward call: h, cp4_adapter_kept_bytes() of device memory. */
-size_t cp4_adapter_kept_bytes(const cp4_adapter_shape* shape);
+size_t cp4_adapter_kept_bytes(const cp4_adapter_shape* shape, int dtype);
 
 /* `kept` may be NULL (inference).  scale NULL: all 1; bias may be NULL.  workspace: device memory of
  * cp4_adapter_forward_workspace_bytes(), 256-byte aligned, its contents scratch. */

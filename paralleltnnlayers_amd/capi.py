@@ -220,7 +220,7 @@ def lib():
     L.cp4_copy_f32.argtypes = [_F, _F, ctypes.c_size_t, ctypes.c_void_p]
     L.cp4_time_copy_f32.argtypes = [_F, _F, ctypes.c_size_t] + timing
     L.cp4_adapter_kept_bytes.restype = ctypes.c_size_t
-    L.cp4_adapter_kept_bytes.argtypes = [ctypes.POINTER(AdapterShape)]
+    L.cp4_adapter_kept_bytes.argtypes = [ctypes.POINTER(AdapterShape), ctypes.c_int]
     for name in ("forward", "backward"):
         need = getattr(L, f"cp4_adapter_{name}_workspace_bytes")
         need.restype = ctypes.c_size_t

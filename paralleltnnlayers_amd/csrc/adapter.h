@@ -12,16 +12,18 @@ namespace cp4 {
 namespace adapter {
 
 // h[t][r] = scale_a sum_k z[t][k] F_a(r, k), F_a(r, k) at f + a * R * K + r * fr + k * fk.
-// h has rows of Rp values (R rounded up to 16s): zero beyond R and for tokens without an adapter.
+// h has rows of Rp values (R rounded up to 16s), zero beyond R; those of tokens without an adapter are not
+// written.  It is the sum of `planes` planes [T][Rp], one for each part of the inputs.
 struct ShrinkArgs {
   const void* z;          // [T][K], rows ldz apart
   const void* f;
   const int* ids;
   const float* scale;     // [G] or null
-  float* h;               // [T][Rp]
+  float* h;               // [planes][T][Rp]
   size_t T, ldz;
   int K, R, Rp, G;
-  int fr, fk;
+  int fr, fk;             // K and 1, or 1 and R
+  int planes;
 };
 
 // y[t][n] = sum_k z[t][k] w(n, k) + bias[n] + sum_r h[t][r] F_a(n, r), F_a(n, r) at
@@ -34,7 +36,8 @@ struct ProjectArgs {
   size_t T, ldz, ldw;
   int K, N, R, Rp, G;
   int fn, fr;
-  int planes;             // h is the sum of so many planes [T][Rp]
+  int planes;             // h is the sum of so many planes ...
+  size_t plane;           // ... so many values apart
 };
 
 // out[a][r][c] = sum over tokens with ids[t] = a of p[t][r] z[t][c], at out + a * R * C + r * outr +
@@ -50,8 +53,11 @@ struct GradArgs {
   int C, R, Rp, G;
   int outr, outc;
   int splits;
+  int planes;             // p is the sum of so many planes [T][Rp]
 };
 
+constexpr size_t kShrinkWide = 4096;     // tokens from which a workgroup takes 32 of them
+int shrink_planes(size_t T, int K, int dtype);
 hipError_t shrink_launch(const ShrinkArgs&, int dtype, hipStream_t);
 // part: project_part_bytes of scratch memory.
 size_t project_part_bytes(size_t T, int K, int N, int dtype);
@@ -129,8 +135,9 @@ struct Adapters {
 // Rows that are not the adapter's are left as they are, not added zeros: an infinity or a NaN in one
 // adapter is no other token's.
 template <class T, int MB, int NB>
-__device__ __forceinline__ void expand(const float* h, int Rp, unsigned long long whose, const typename T::raw* f,
-                                       int fn, int fr, int n0, int N, int R, f32x4 (&acc)[MB][NB]) {
+__device__ __forceinline__ void expand(const float* h, int Rp, int planes, size_t plane, unsigned long long whose,
+                                       const typename T::raw* f, int fn, int fr, int n0, int N, int R,
+                                       f32x4 (&acc)[MB][NB]) {
   const int lane = threadIdx.x & 63, l = lane & 15, g = lane >> 4;
   for (int r0 = 0; r0 < R; r0 += 16) {
     float hf[MB][4];
@@ -141,15 +148,20 @@ __device__ __forceinline__ void expand(const float* h, int Rp, unsigned long lon
       const float* const row = h + (size_t)16 * i * Rp + r0;
       if constexpr (__is_same(T, F32)) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) hf[i][q] = mine ? row[4 * q + g] : 0.0f;
+        for (int q = 0; q < 4; ++q) {
+          hf[i][q] = 0.0f;
+          if (mine)
+            for (int s = 0; s < planes; ++s) hf[i][q] += row[s * plane + 4 * q + g];
+        }
       } else {
         float x[8] = {};
-        if (mine) {
-          const f32x4* p = reinterpret_cast<const f32x4*>(row + 8 * (g & 1));
-          const f32x4 u = p[0], v = p[1];
+        if (mine)
+          for (int s = 0; s < planes; ++s) {
+            const f32x4* p = reinterpret_cast<const f32x4*>(row + s * plane + 8 * (g & 1));
+            const f32x4 u = p[0], v = p[1];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) x[j] = u[j], x[4 + j] = v[j];
-        }
+            for (int j = 0; j < 4; ++j) x[j] += u[j], x[4 + j] += v[j];
+          }
         u16x8 hi, lo;
         two_parts(x, hi, lo);
         ha[i] = g < 2 ? hi : lo;

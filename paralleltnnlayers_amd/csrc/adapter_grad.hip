@@ -24,6 +24,11 @@ __global__ __launch_bounds__(256) void general_kernel(const GradArgs a) {
   const size_t per = (a.T + a.splits - 1) / a.splits;
   const size_t first = min(a.T, split * per), last = min(a.T, first + per);
   const Raw* const z = static_cast<const Raw*>(a.z);
+  auto row_of = [&](size_t t, int r) {
+    float x = 0.0f;
+    for (int s = 0; s < a.planes; ++s) x += a.p[(s * a.T + t) * a.Rp + r];
+    return x;
+  };
   f32x4 acc[4] = {};
   for (size_t w0 = first; w0 < last; w0 += kList) {
     const int here = (int)min((size_t)kList, last - w0);
@@ -53,7 +58,7 @@ __global__ __launch_bounds__(256) void general_kernel(const GradArgs a) {
           const float zv = t >= 0 && c < a.C ? z[(w0 + t) * a.ldz + c] : 0.0f;
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (i < ranks) acc[i] = mfma_f32(t >= 0 ? a.p[(w0 + t) * a.Rp + r0 + 16 * i + l] : 0.0f, zv, acc[i]);
+            if (i < ranks) acc[i] = mfma_f32(t >= 0 ? row_of(w0 + t, r0 + 16 * i + l) : 0.0f, zv, acc[i]);
         }
       } else {
         u16x8 zv = {};
@@ -75,7 +80,7 @@ __global__ __launch_bounds__(256) void general_kernel(const GradArgs a) {
           if (i < ranks) {
             float x[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = t[j] >= 0 ? a.p[(w0 + t[j]) * a.Rp + r0 + 16 * i + l] : 0.0f;
+            for (int j = 0; j < 8; ++j) x[j] = t[j] >= 0 ? row_of(w0 + t[j], r0 + 16 * i + l) : 0.0f;
             u16x8 ph, pl;
             two_parts(x, ph, pl);
             if constexpr (__is_same(T, F16)) acc[i] = mfma_bf16(ph, zl, acc[i]);

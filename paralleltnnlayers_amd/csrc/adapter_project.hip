@@ -76,7 +76,7 @@ __global__ __launch_bounds__(256) void general_kernel(const ProjectArgs a) {
   unsigned long long whose;
   while (todo.take(ad, whose)) {
     const Raw* const f = static_cast<const Raw*>(a.f) + (size_t)ad * a.R * a.N;
-    expand<T>(a.h + (t0 + wm + l) * a.Rp, a.Rp, whose, f, a.fn, a.fr, n0 + wn, a.N, a.R, acc);
+    expand<T>(a.h + (t0 + wm + l) * a.Rp, a.Rp, a.planes, a.plane, whose, f, a.fn, a.fr, n0 + wn, a.N, a.R, acc);
   }
   Raw* const y = static_cast<Raw*>(a.y);
 #pragma unroll

@@ -1,5 +1,15 @@
 // h = scale A_a x, token by token (include/cp4/adapter.h): a product with as few columns as the adapters
 // have ranks, bound by reading x and the adapters in use once.
+//
+// A workgroup takes 16 or 32 tokens and one part of the inputs, straight from memory to the matrix cores:
+// nothing is read twice within it, so the LDS would only be a detour.  Its eight waves share the adapters that
+// these tokens have - one of a prompt, sixteen of single tokens - and, where there are fewer, the
+// inputs.  All rows are multiplied with each adapter and the rows that are not its own keep what they had; the
+// waves' sums meet in the LDS once, at the end.  With few tokens the inputs are split over workgroups as
+// well: each part leaves a plane of h of its own, and who reads h adds them up.
+//
+// A lane's ranks are RB * (lane & 15) + j, not 16 j + (lane & 15), so that factors that lie rank by rank
+// (B, in the backward pass) come with loads of RB values.
 #include <algorithm>
 
 #include "adapter.h"
@@ -8,77 +18,199 @@ namespace cp4 {
 namespace adapter {
 namespace {
 
-constexpr int kWaves = 4;
-
-// Any strides and alignment: a workgroup takes 16 tokens; its waves share the inputs in steps of 32 and
-// go through the adapters that these tokens have, all sixteen rows against each, so that a batch in which
-// every token has its own reads each adapter once and one in which all have the same does a single
-// product.
+constexpr int kWaves = 8;
 template <class T>
-__global__ __launch_bounds__(64 * kWaves) void general_kernel(const ShrinkArgs a) {
+constexpr int kUnit = 128 / sizeof(typename T::raw);                 // inputs of a loop's turn: a cache line a row
+
+// One operand's row of a turn: 8 (fp32: 4) values from each half of 32 bytes; zero from `left` on.
+template <class T, bool Vec>
+__device__ __forceinline__ void load_row(const typename T::raw* p, int left, bool full, u32x4 (&v)[2]) {
   typedef typename T::raw Raw;
-  __shared__ float sum[kWaves][16][17];
-  __shared__ int own[16];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
-  const size_t t0 = (size_t)blockIdx.x * 16;
-  const int rows = (int)min((size_t)16, a.T - t0);
+  constexpr int n = 16 / sizeof(Raw);
+  if constexpr (Vec) {
+    if (full) {
+      v[0] = reinterpret_cast<const u32x4*>(p)[0];
+      v[1] = reinterpret_cast<const u32x4*>(p)[1];
+      return;
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    Raw x[n];
+#pragma unroll
+    for (int q = 0; q < n; ++q) x[q] = n * h + q < left ? p[n * h + q] : Raw(0);
+    __builtin_memcpy(&v[h], x, 16);
+  }
+}
+
+// Vec: rows of z (and of f where it lies input by input, !TR) start on 16-byte boundaries.
+template <class T, bool TR, bool Vec, int MB, int RB>
+__global__ __launch_bounds__(64 * kWaves) void shrink_kernel(const ShrinkArgs a) {
+  typedef typename T::raw Raw;
+  constexpr int n = 16 / sizeof(Raw), U = kUnit<T>, kRows = 16 * MB;
+  __shared__ float sum[kWaves][16][16 * RB + 4];
+  __shared__ int own[kRows];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 15, g = lane >> 4;
+  const size_t t0 = (size_t)blockIdx.x * kRows;
+  const int rows = (int)min((size_t)kRows, a.T - t0);
   int id = lane < rows ? a.ids[t0 + lane] : -1;
   if (id < 0 || id >= a.G) id = -1;
-  const Raw* const z = static_cast<const Raw*>(a.z) + (t0 + min(l, rows - 1)) * a.ldz;
-  if (threadIdx.x < 16) own[lane] = id;
-  __syncthreads();
-  for (int i = threadIdx.x; i < rows * a.Rp; i += 64 * kWaves)       // tokens without an adapter
-    if (own[i / a.Rp] < 0) a.h[t0 * a.Rp + i] = 0.0f;
-  Adapters todo(id);
-  int ad;
-  unsigned long long whose;
-  while (todo.take(ad, whose)) {
-    const Raw* const f = static_cast<const Raw*>(a.f) + (size_t)ad * a.R * a.K;
-    const float s = a.scale ? a.scale[ad] : 1.0f;
-    for (int r0 = 0; r0 < a.Rp; r0 += 16) {
-      const int r = r0 + l;
-      const Raw* const fr = f + (size_t)min(r, a.R - 1) * a.fr;
-      f32x4 acc = {};
-      for (int k0 = 32 * wave; k0 < a.K; k0 += 32 * kWaves) {
-        if constexpr (__is_same(T, F32)) {
+  if (threadIdx.x < kRows) own[lane] = id;
+  int different = 0;
+  {
+    Adapters each(id);
+    int ad;
+    unsigned long long whose;
+    while (different < kWaves && each.take(ad, whose)) ++different;
+  }
+  if (!different) return;
+  // ways: how many waves go through the adapters in turn; the others share the inputs
+  const int ways = different >= 8 ? 8 : different >= 4 ? 4 : different >= 2 ? 2 : 1;
+  const int mine = wave & (ways - 1), slice = wave / ways, slices = kWaves / ways;
+  const int units = (a.K + U - 1) / U, per = (units + a.planes - 1) / a.planes;
+  const int u0 = min(units, (int)blockIdx.y * per), u1 = min(units, u0 + per);
+  const int each = (u1 - u0 + slices - 1) / slices;
+  const int first = min(u1, u0 + slice * each), last = min(u1, first + each);
+  const int whole = min(last, a.K / U);                              // (from there on a turn has fewer inputs)
+
+  const bool even = a.R % RB == 0 && ((size_t)a.f & (RB * sizeof(Raw) - 1)) == 0;
+  const Raw* z[MB];
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const int k = k0 + 4 * q + g;
-            const float zv = k < a.K ? z[k] : 0.0f;
-            const float fv = k < a.K && r < a.R ? fr[(size_t)k * a.fk] : 0.0f;
-            acc = mfma_f32(zv, fv, acc);
+  for (int i = 0; i < MB; ++i) z[i] = static_cast<const Raw*>(a.z) + (t0 + min(16 * i + l, rows - 1)) * a.ldz + 2 * n * g;
+
+  for (int r0 = 0; r0 < a.Rp; r0 += 16 * RB) {
+    f32x4 acc[MB][RB] = {};
+    Adapters todo(id);
+    int ad, turn = 0;
+    unsigned long long whose;
+    while (todo.take(ad, whose)) {
+      if ((turn++ & (ways - 1)) != mine) continue;
+      const Raw* const f = static_cast<const Raw*>(a.f) + (size_t)ad * a.R * a.K;
+      f32x4 d[MB][RB] = {};
+      auto multiply = [&](int u, bool full) {
+        const int k = u * U + 2 * n * g, left = full ? 2 * n : a.K - k;
+        u32x4 zv[MB][2], fv[RB][2];
+#pragma unroll
+        for (int i = 0; i < MB; ++i) load_row<T, Vec>(z[i] + (size_t)u * U, left, full, zv[i]);
+        if constexpr (!TR) {
+#pragma unroll
+          for (int j = 0; j < RB; ++j) {
+            const int r = r0 + RB * l + j;
+            load_row<T, Vec>(f + (size_t)min(r, a.R - 1) * a.K + k, left, full, fv[j]);
+            if (r >= a.R) fv[j][0] = fv[j][1] = u32x4{};
           }
         } else {
-          u16x8 zv = {}, fv = {};
+          const int r = r0 + RB * l;
+          Raw x[2 * n][RB];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int k = k0 + 8 * g + j;
-            if (k < a.K) zv[j] = z[k];
-            if (k < a.K && r < a.R) fv[j] = fr[(size_t)k * a.fk];
+          for (int q = 0; q < 2 * n; ++q) {
+            const Raw* const p = f + (size_t)(k + q) * a.R + r;
+            if (RB > 1 && even) {                                    // (whole lanes of ranks)
+              if (r < a.R && q < left) __builtin_memcpy(x[q], __builtin_assume_aligned(p, RB * sizeof(Raw)), RB * sizeof(Raw));
+              else
+#pragma unroll
+                for (int j = 0; j < RB; ++j) x[q][j] = Raw(0);
+            } else {
+#pragma unroll
+              for (int j = 0; j < RB; ++j) x[q][j] = r + j < a.R && q < left ? p[j] : Raw(0);
+            }
           }
-          acc = mfma_16<T>(zv, fv, acc);
+#pragma unroll
+          for (int j = 0; j < RB; ++j) {
+            Raw y[2][n];
+#pragma unroll
+            for (int q = 0; q < 2 * n; ++q) y[q / n][q % n] = x[q][j];
+            __builtin_memcpy(&fv[j][0], y[0], 16);
+            __builtin_memcpy(&fv[j][1], y[1], 16);
+          }
         }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < RB; ++j)
+#pragma unroll
+            for (int i = 0; i < MB; ++i) {
+              if constexpr (__is_same(T, F32)) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                  d[i][j] = mfma_f32(__uint_as_float(zv[i][h][q]), __uint_as_float(fv[j][h][q]), d[i][j]);
+              } else {
+                d[i][j] = mfma_16<T>(__builtin_bit_cast(u16x8, zv[i][h]), __builtin_bit_cast(u16x8, fv[j][h]), d[i][j]);
+              }
+            }
+      };
+      int u = first;
+      for (; u + 4 <= whole; u += 4) {                               // (the loads of four turns before their products)
+        multiply(u, true);
+        multiply(u + 1, true);
+        multiply(u + 2, true);
+        multiply(u + 3, true);
       }
+      for (; u < whole; ++u) multiply(u, true);
+      for (; u < last; ++u) multiply(u, false);
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int j = 0; j < RB; ++j)
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            if (whose >> (16 * i + 4 * g + v) & 1) acc[i][j][v] = d[i][j][v];
+    }
+    for (int i = 0; i < MB; ++i) {
       __syncthreads();
 #pragma unroll
-      for (int v = 0; v < 4; ++v) sum[wave][4 * g + v][l] = acc[v];
-      __syncthreads();
-      const int row = threadIdx.x >> 4, col = threadIdx.x & 15;      // (256 threads: one sum each)
-      float x = 0.0f;
+      for (int j = 0; j < RB; ++j)
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) x += sum[w][row][col];
-      if (whose >> row & 1) a.h[(t0 + row) * a.Rp + r0 + col] = r0 + col < a.R ? x * s : 0.0f;
+        for (int v = 0; v < 4; ++v) sum[wave][4 * g + v][RB * l + j] = acc[i][j][v];
+      __syncthreads();
+      for (int at = threadIdx.x; at < 256 * RB; at += 64 * kWaves) {
+        const int row = at / (16 * RB), r = at % (16 * RB), ad_of = own[16 * i + row];
+        if (ad_of < 0 || r0 + r >= a.Rp) continue;
+        float x = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) x += sum[w][row][r];
+        a.h[((size_t)blockIdx.y * a.T + t0 + 16 * i + row) * a.Rp + r0 + r] = a.scale ? x * a.scale[ad_of] : x;
+      }
     }
   }
 }
 
+template <class T, bool TR, bool Vec, int MB>
+void launch_ranks(const ShrinkArgs& a, hipStream_t st) {
+  const dim3 grid((unsigned)((a.T + 16 * MB - 1) / (16 * MB)), a.planes);
+  if (a.Rp <= 16) shrink_kernel<T, TR, Vec, MB, 1><<<grid, 64 * kWaves, 0, st>>>(a);
+  else if (a.Rp <= 32) shrink_kernel<T, TR, Vec, MB, 2><<<grid, 64 * kWaves, 0, st>>>(a);
+  else shrink_kernel<T, TR, Vec, MB, 4><<<grid, 64 * kWaves, 0, st>>>(a);
+}
+template <class T, bool TR, bool Vec>
+void launch_rows(const ShrinkArgs& a, hipStream_t st) {
+  if (a.T >= kShrinkWide) launch_ranks<T, TR, Vec, 2>(a, st);
+  else launch_ranks<T, TR, Vec, 1>(a, st);
+}
+template <class T>
+void launch(const ShrinkArgs& a, hipStream_t st) {
+  constexpr size_t n = 16 / sizeof(typename T::raw);
+  const bool tr = a.fk != 1 || a.K == 1;
+  bool vec = ((size_t)a.z & 15) == 0 && a.ldz % n == 0;
+  if (!tr) vec = vec && ((size_t)a.f & 15) == 0 && a.K % n == 0;
+  if (tr) vec ? launch_rows<T, true, true>(a, st) : launch_rows<T, true, false>(a, st);
+  else vec ? launch_rows<T, false, true>(a, st) : launch_rows<T, false, false>(a, st);
+}
+
 }  // namespace
 
+// Parts of the inputs: enough workgroups for the chip, none with less than a turn for each wave.
+int shrink_planes(size_t T, int K, int dtype) {
+  const int unit = dtype == CP4_DTYPE_F32 ? kUnit<F32> : kUnit<BF16>;
+  const size_t wide = T >= kShrinkWide ? 32 : 16, tiles = std::max<size_t>(1, (T + wide - 1) / wide);
+  const size_t most = std::max(1, (K + unit - 1) / unit / 4);
+  return (int)std::max<size_t>(1, std::min({(size_t)num_compute_units() / tiles, most, (size_t)16}));
+}
+
 hipError_t shrink_launch(const ShrinkArgs& a, int dtype, hipStream_t st) {
-  const unsigned grid = (unsigned)((a.T + 15) / 16);
-  if (dtype == CP4_DTYPE_F32) general_kernel<F32><<<grid, 64 * kWaves, 0, st>>>(a);
-  else if (dtype == CP4_DTYPE_BF16) general_kernel<BF16><<<grid, 64 * kWaves, 0, st>>>(a);
-  else general_kernel<F16><<<grid, 64 * kWaves, 0, st>>>(a);
+  if (dtype == CP4_DTYPE_F32) launch<F32>(a, st);
+  else if (dtype == CP4_DTYPE_BF16) launch<BF16>(a, st);
+  else launch<F16>(a, st);
   return hipGetLastError();
 }
 

@@ -74,7 +74,7 @@ __device__ __forceinline__ void load_some(const Raw* p, int count, bool vec, Raw
 }
 
 // Adds h F_a^T to a wave's MB x NB blocks (columns as above) for the rows whose bit is set; see expand()
-// in adapter.h.  planes: h is the sum of so many planes of T * Rp values.
+// in adapter.h.  h is the sum of a.planes planes.
 template <class T, bool NN, int MB, int NB>
 __device__ __forceinline__ void expand_wave(const ProjectArgs& a, const float* h, unsigned long long whose,
                                             const typename T::raw* f, bool vec, int n0, f32x4 (&acc)[MB][NB]) {
@@ -92,7 +92,7 @@ __device__ __forceinline__ void expand_wave(const ProjectArgs& a, const float* h
       for (int q = 0; q < kOwn; ++q) hv[i][q] = 0.0f;
       if (whose >> (16 * i + l) & 1) {
         const float* p = h + (size_t)16 * i * a.Rp + r0 + rl;
-        for (int s = 0; s < a.planes; ++s, p += a.T * (size_t)a.Rp)
+        for (int s = 0; s < a.planes; ++s, p += a.plane)
 #pragma unroll
           for (int q = 0; q < kOwn; q += 4) {
             const f32x4 x = *reinterpret_cast<const f32x4*>(p + q);

@@ -525,7 +525,7 @@ std::vector<int64_t> with_last(at::IntArrayRef sizes, int64_t last) {
 // y, and where `kept` is given what the backward call needs.
 Tensor adapter_run(const Adapters& p, at::IntArrayRef sizes, Tensor y, Tensor* kept, void* st) {
   if (!y.defined()) y = empty(with_last(sizes, p.shape.N), p.x.scalar_type(), p.x);
-  if (kept) *kept = empty({(int64_t)(cp4_adapter_kept_bytes(&p.shape) / 4)}, at::kFloat, p.x);
+  if (kept) *kept = empty({(int64_t)(cp4_adapter_kept_bytes(&p.shape, p.dtype) / 4)}, at::kFloat, p.x);
   const size_t need = cp4_adapter_forward_workspace_bytes(&p.shape, p.dtype);
   const Tensor ws = scratch(need, p.x);
   check(cp4_adapter_forward(&p.shape, p.dtype, ptr(p.x), ptr(p.W), ptr(p.A), ptr(p.B), ints(p.ids), floats(p.scale),
@@ -543,7 +543,7 @@ void adapter_run_backward(const Adapters& p, const Tensor& x_in, const Tensor& k
             "x does not match dy");
     x = rows_of(x_in, &s.ldx);
     require(kept.defined() && kept.is_cuda() && kept.scalar_type() == at::kFloat && kept.is_contiguous() &&
-                (size_t)kept.numel() * 4 == cp4_adapter_kept_bytes(&s),
+                (size_t)kept.numel() * 4 == cp4_adapter_kept_bytes(&s, p.dtype),
             "kept is not what the forward call left");
     *dA = empty({(int64_t)s.G, (int64_t)s.R, (int64_t)s.K}, p.x.scalar_type(), p.x);
     *dB = empty({(int64_t)s.G, (int64_t)s.N, (int64_t)s.R}, p.x.scalar_type(), p.x);

@@ -31,7 +31,7 @@ def test_adapter_shapes_are_refused(capi):
     L = capi.lib()
     good = dict(T=4, K=32, N=24, R=4, G=2, ldx=0, ldw=0, lddy=0)
     assert L.cp4_adapter_forward_workspace_bytes(ctypes.byref(capi.AdapterShape(**good)), 0) == 4 * 16 * 4
-    assert L.cp4_adapter_kept_bytes(ctypes.byref(capi.AdapterShape(**good))) == 4 * 16 * 4
+    assert L.cp4_adapter_kept_bytes(ctypes.byref(capi.AdapterShape(**good)), 0) == 4 * 16 * 4
     bad = [dict(K=0), dict(N=0), dict(R=0), dict(G=0), dict(R=257), dict(G=65536), dict(K=(1 << 22) + 1),
            dict(N=(1 << 22) + 1), dict(T=(1 << 31) + 1), dict(ldx=31), dict(ldw=31), dict(lddy=23), dict(ldx=(1 << 30) + 1)]
     fwd = lambda s, dtype=0, p=[ONE] * 8: L.cp4_adapter_forward(s, dtype, *p, None, ONE, 1 << 30, None)
