@@ -71,6 +71,15 @@ TilePlan tile_plan(size_t T, int K, int N, int dtype);
 size_t tile_part_bytes(const TilePlan&, size_t T, int N);
 bool tile_supported(const ProjectArgs&, int dtype, bool nn);
 hipError_t tile_launch(const ProjectArgs&, const TilePlan&, float* part, int dtype, bool nn, hipStream_t);
+// y = the sum of [splits][T][N] partial sums, and the bias (may be null).
+hipError_t parts_join(const float* part, const float* bias, void* y, size_t T, int N, int splits, int dtype, hipStream_t);
+// Up to 64 tokens (w [N][K], rows on 16-byte boundaries): nb blocks of 16 columns a workgroup; nb 0: not for this
+// kernel.
+struct RowsPlan {
+  int nb, splits;
+};
+RowsPlan rows_plan(size_t T, int K, int N, int dtype);
+hipError_t rows_launch(const ProjectArgs&, const RowsPlan&, float* part, int dtype, hipStream_t);
 int grad_splits(size_t T, int C, int R, int G);
 hipError_t grad_launch(const GradArgs&, int dtype, hipStream_t);
 
@@ -127,96 +136,6 @@ struct Adapters {
     return true;
   }
 };
-
-// Adds h F_a^T to the 16 x 16 blocks of MB blocks of rows and NB of columns, for the rows whose bit of
-// `whose` is set (block i's: 16 i ..).  h: this lane's row (lane & 15) of block 0, rows 16 * Rp
-// floats further in the next; n0: column of block 0's lane 0.  16-bit types: depth 0 .. 15 are the first
-// parts of h, 16 .. 31 what they leave, against F_a twice (f16: F_a in two parts as well, in two products).
-// Rows that are not the adapter's are left as they are, not added zeros: an infinity or a NaN in one
-// adapter is no other token's.
-template <class T, int MB, int NB>
-__device__ __forceinline__ void expand(const float* h, int Rp, int planes, size_t plane, unsigned long long whose,
-                                       const typename T::raw* f, int fn, int fr, int n0, int N, int R,
-                                       f32x4 (&acc)[MB][NB]) {
-  const int lane = threadIdx.x & 63, l = lane & 15, g = lane >> 4;
-  for (int r0 = 0; r0 < R; r0 += 16) {
-    float hf[MB][4];
-    u16x8 ha[MB];
-#pragma unroll
-    for (int i = 0; i < MB; ++i) {
-      const bool mine = whose >> (16 * i + l) & 1;
-      const float* const row = h + (size_t)16 * i * Rp + r0;
-      if constexpr (__is_same(T, F32)) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          hf[i][q] = 0.0f;
-          if (mine)
-            for (int s = 0; s < planes; ++s) hf[i][q] += row[s * plane + 4 * q + g];
-        }
-      } else {
-        float x[8] = {};
-        if (mine)
-          for (int s = 0; s < planes; ++s) {
-            const f32x4* p = reinterpret_cast<const f32x4*>(row + s * plane + 8 * (g & 1));
-            const f32x4 u = p[0], v = p[1];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] += u[j], x[4 + j] += v[j];
-          }
-        u16x8 hi, lo;
-        two_parts(x, hi, lo);
-        ha[i] = g < 2 ? hi : lo;
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < NB; ++j) {
-      const int n = n0 + 16 * j + l;
-      float ff[4];
-      u16x8 fv = {}, fl = {};
-      if constexpr (__is_same(T, F32)) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int r = r0 + 4 * q + g;
-          ff[q] = n < N && r < R ? f[(size_t)n * fn + (size_t)r * fr] : 0.0f;
-        }
-      } else {
-        if (n < N) {
-          const typename T::raw* const p = f + (size_t)n * fn;
-#pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const int r = r0 + 8 * (g & 1) + q;
-            if (r < R) fv[q] = p[(size_t)r * fr];
-          }
-        }
-        if constexpr (__is_same(T, F16)) {
-          float x[8];
-#pragma unroll
-          for (int q = 0; q < 8; ++q) x[q] = F16::widen(fv[q]);
-          two_parts(x, fv, fl);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < MB; ++i) {
-        const unsigned rows = (unsigned)(whose >> (16 * i)) & 0xffffu;
-        if (!rows) continue;
-        f32x4 d = acc[i][j];
-        if constexpr (__is_same(T, F32)) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) d = mfma_f32(hf[i][q], ff[q], d);
-        } else {
-          if constexpr (__is_same(T, F16)) d = mfma_bf16(ha[i], fl, d);
-          d = mfma_bf16(ha[i], fv, d);
-        }
-        if (rows == 0xffffu) {
-          acc[i][j] = d;
-        } else {
-#pragma unroll
-          for (int v = 0; v < 4; ++v)
-            if (rows >> (4 * g + v) & 1) acc[i][j][v] = d[v];
-        }
-      }
-    }
-  }
-}
 
 }  // namespace adapter
 }  // namespace cp4

@@ -1,108 +1,152 @@
 // The adapters' gradients (include/cp4/adapter.h): for each adapter a sum over its tokens of the outer products
-// of an fp32 row of h or dh and a row of dy or x.
+// of an fp32 row of h or dh and a row of dy or x: a product as deep as the adapter has tokens and as high as
+// it has ranks, bound by reading x and dy once.
+//
+// A workgroup takes 128 columns of one adapter.  It picks the adapter's tokens out of 8192 ids at a time
+// into a list in the LDS (in order, so that sums do not change from call to call); its eight waves share the list,
+// 32 tokens (fp32: 16) a turn, straight from memory: a lane reads eight consecutive columns of each
+// of its tokens' rows and turns them in registers into eight column blocks' operands.  The waves' sums
+// meet in the LDS at the end.  Rows of h enter as two bfloat16 parts, and so do half-precision rows of dy and x
+// (exactly).  Few workgroups (few adapters, short rows): the tokens are split over workgroups too, and a
+// second launch adds the parts up in their order.
 #include <algorithm>
 
 #include "adapter.h"
+#include "adapter_load.h"
 
 namespace cp4 {
 namespace adapter {
 namespace {
 
-constexpr int kCols = 64, kList = 2048;
+constexpr int kCols = 128, kWindow = 8192, kWaves = 8, kPad = 4;
 
-// A workgroup sums 64 columns of one adapter over one range of tokens, 64 ranks at a time: it picks the
-// adapter's tokens out of the range, in order, into a list in the LDS and goes through that 32 at a time;
-// each wave has 16 columns.  Tokens of other adapters cost a look at their id.
-template <class T>
-__global__ __launch_bounds__(256) void general_kernel(const GradArgs a) {
+template <class T, bool Vec, int RB>
+__global__ __launch_bounds__(64 * kWaves, 2) void grad_kernel(const GradArgs a) {
   typedef typename T::raw Raw;
-  __shared__ int list[kList + 32];
-  __shared__ int counts[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
-  const int ad = blockIdx.y % a.G, split = blockIdx.y / a.G, r0 = blockIdx.z * 64;
-  const int c = blockIdx.x * kCols + 16 * wave + l, ranks = min(64, a.Rp - r0) / 16;
+  constexpr bool kF32 = __is_same(T, F32);
+  constexpr int kTurn = kF32 ? 16 : 32, kOwn = kTurn / 4;            // tokens of a turn, and of a lane
+  __shared__ __attribute__((aligned(16))) union {
+    unsigned short list[kWindow + 64];
+    float sum[kWaves][16][kCols + kPad];
+  } lds;
+  __shared__ int counts[kWaves];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 15, g = lane >> 4;
+  const int ad = blockIdx.y % a.G, split = blockIdx.y / a.G, r0 = blockIdx.z * 16 * RB;
+  const int c0 = blockIdx.x * kCols, c = c0 + 8 * l;
   const size_t per = (a.T + a.splits - 1) / a.splits;
   const size_t first = min(a.T, split * per), last = min(a.T, first + per);
-  const Raw* const z = static_cast<const Raw*>(a.z);
-  auto row_of = [&](size_t t, int r) {
-    float x = 0.0f;
-    for (int s = 0; s < a.planes; ++s) x += a.p[(s * a.T + t) * a.Rp + r];
-    return x;
-  };
-  f32x4 acc[4] = {};
-  for (size_t w0 = first; w0 < last; w0 += kList) {
-    const int here = (int)min((size_t)kList, last - w0);
-    int n = 0;
-    __syncthreads();                                                 // (the list is read no more)
-    for (int i0 = 0; i0 < here; i0 += 256) {
-      const int i = i0 + (int)threadIdx.x;
-      const bool mine = i < here && a.ids[w0 + i] == ad;
-      const unsigned long long m = __ballot(mine);
-      if (lane == 0) counts[wave] = __popcll(m);
-      __syncthreads();
-      int at = n;
-      for (int w = 0; w < 4; ++w) {
-        if (w < wave) at += counts[w];
-        n += counts[w];
-      }
-      if (mine) list[at + __popcll(m & ((1ull << lane) - 1))] = i;
-      __syncthreads();
+  const Raw* const z = static_cast<const Raw*>(a.z) + min(c, a.C - 1);
+  const int cols = a.C - c;
+  const size_t plane = a.T * a.Rp;
+  f32x4 acc[RB][8] = {};
+  for (size_t w0 = first; w0 < last; w0 += kWindow) {
+    // the list: each wave looks through its eighth of the window
+    const int here = (int)min((size_t)kWindow, last - w0), share = (here + 8 * 64 - 1) / (8 * 64);   // (64s of a wave)
+    unsigned long long mine[kWindow / 512];
+    int n_wave = 0;
+#pragma unroll
+    for (int i = 0; i < kWindow / 512; ++i) {
+      const int at = (wave * share + i) * 64 + lane;
+      mine[i] = __ballot(i < share && at < here && a.ids[w0 + at] == ad);
+      n_wave += __popcll(mine[i]);
     }
-    if (threadIdx.x < 32) list[n + threadIdx.x] = -1;
+    __syncthreads();                                                 // (nobody reads the last list)
+    if (lane == 0) counts[wave] = n_wave;
     __syncthreads();
-    for (int b = 0; b < n; b += 32) {
-      if constexpr (__is_same(T, F32)) {
+    int at = 0, n = 0;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const int t = list[b + 4 * q + g];
-          const float zv = t >= 0 && c < a.C ? z[(w0 + t) * a.ldz + c] : 0.0f;
+    for (int w = 0; w < kWaves; ++w) {
+      if (w < wave) at += counts[w];
+      n += counts[w];
+    }
+    if (!n) continue;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (i < ranks) acc[i] = mfma_f32(t >= 0 ? row_of(w0 + t, r0 + 16 * i + l) : 0.0f, zv, acc[i]);
-        }
+    for (int i = 0; i < kWindow / 512; ++i) {
+      if (mine[i] >> lane & 1)
+        lds.list[at + __popcll(mine[i] & ((1ull << lane) - 1))] = (unsigned short)((wave * share + i) * 64 + lane);
+      at += __popcll(mine[i]);
+    }
+    __syncthreads();
+    // (a turn's missing tokens are its last one again, times zero)
+    const int turns = (n + kTurn - 1) / kTurn, each = (turns + kWaves - 1) / kWaves;
+    const int end = min(turns, (wave + 1) * each);
+    for (int b = wave * each; b < end; ++b) {
+      int t[kOwn];
+      float p[RB][kOwn];
+      Raw x[kOwn][8];
+#pragma unroll
+      for (int q = 0; q < kOwn; ++q) {
+        const int i = b * kTurn + kOwn * g + q;
+        t[q] = lds.list[min(i, n - 1)];
+        load_some<8>(z + (w0 + t[q]) * a.ldz, cols, Vec, x[q]);
+      }
+#pragma unroll
+      for (int q = 0; q < kOwn; ++q) {
+        const bool there = b * kTurn + kOwn * g + q < n;
+        const float* const row = a.p + (w0 + t[q]) * a.Rp + r0 + l;
+#pragma unroll
+        for (int i = 0; i < RB; ++i) p[i][q] = there && r0 + 16 * i < a.Rp ? row[16 * i] : 0.0f;
+        for (int s = 1; s < a.planes; ++s)
+#pragma unroll
+          for (int i = 0; i < RB; ++i) p[i][q] += there && r0 + 16 * i < a.Rp ? row[s * plane + 16 * i] : 0.0f;
+      }
+      if constexpr (kF32) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int i = 0; i < RB; ++i) acc[i][j] = mfma_f32(p[i][q], x[q][j], acc[i][j]);
       } else {
-        u16x8 zv = {};
-        int t[8];
+        unsigned in[8][4];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) __builtin_memcpy(in[q], x[q], 16);
+        u16x8 zv[8], ph[RB], pl[RB];
+        turn<8>(in, zv);
+#pragma unroll
+        for (int i = 0; i < RB; ++i) two_parts(p[i], ph[i], pl[i]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          t[j] = list[b + 8 * g + j];
-          if (t[j] >= 0 && c < a.C) zv[j] = z[(w0 + t[j]) * a.ldz + c];
-        }
-        u16x8 zh = zv, zl = {};
-        if constexpr (__is_same(T, F16)) {
-          float x[8];
+          u16x8 zh = zv[j], zl = {};
+          if constexpr (__is_same(T, F16)) {
+            float f[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = F16::widen(zv[j]);
-          two_parts(x, zh, zl);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (i < ranks) {
-            float x[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = t[j] >= 0 ? row_of(w0 + t[j], r0 + 16 * i + l) : 0.0f;
-            u16x8 ph, pl;
-            two_parts(x, ph, pl);
-            if constexpr (__is_same(T, F16)) acc[i] = mfma_bf16(ph, zl, acc[i]);
-            acc[i] = mfma_bf16(pl, zh, acc[i]);
-            acc[i] = mfma_bf16(ph, zh, acc[i]);
+            for (int q = 0; q < 8; ++q) f[q] = F16::widen(zv[j][q]);
+            two_parts(f, zh, zl);
           }
+#pragma unroll
+          for (int i = 0; i < RB; ++i) {
+            if constexpr (__is_same(T, F16)) acc[i][j] = mfma_bf16(ph[i], zl, acc[i][j]);
+            acc[i][j] = mfma_bf16(pl[i], zh, acc[i][j]);
+            acc[i][j] = mfma_bf16(ph[i], zh, acc[i][j]);
+          }
+        }
       }
     }
   }
-  if (c >= a.C) return;
   const size_t size = (size_t)a.R * a.C;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (i < ranks)
+  for (int i = 0; i < RB; ++i) {
+    if (r0 + 16 * i >= a.R) break;
+    __syncthreads();
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const int r = r0 + 16 * i + 4 * g + v;
-        if (r >= a.R) continue;
-        const size_t at = (size_t)ad * size + (size_t)r * a.outr + (size_t)c * a.outc;
-        if (a.splits > 1) a.part[(size_t)split * a.G * size + at] = acc[i][v];
-        else static_cast<Raw*>(a.out)[at] = T::narrow(acc[i][v]);
-      }
+    for (int v = 0; v < 4; ++v)
+#pragma unroll
+      for (int j = 0; j < 8; j += 4)
+        *reinterpret_cast<f32x4*>(&lds.sum[wave][4 * g + v][8 * l + j]) =
+            f32x4{acc[i][j][v], acc[i][j + 1][v], acc[i][j + 2][v], acc[i][j + 3][v]};
+    __syncthreads();
+    for (int o = threadIdx.x; o < 16 * kCols; o += 64 * kWaves) {    // (in the output's order)
+      const int r = a.outc == 1 ? o / kCols : o % 16, col = a.outc == 1 ? o % kCols : o / 16;
+      if (r0 + 16 * i + r >= a.R || c0 + col >= a.C) continue;
+      float x = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) x += lds.sum[w][r][col];
+      const size_t at = (size_t)ad * size + (size_t)(r0 + 16 * i + r) * a.outr + (size_t)(c0 + col) * a.outc;
+      if (a.splits > 1) a.part[(size_t)split * a.G * size + at] = x;
+      else static_cast<Raw*>(a.out)[at] = T::narrow(x);
+    }
+  }
 }
 
 // The ranges' sums, in their order.
@@ -115,22 +159,31 @@ __global__ __launch_bounds__(256) void join_kernel(const float* part, void* out,
   static_cast<typename T::raw*>(out)[i] = T::narrow(x);
 }
 
-template <class T>
+template <class T, bool Vec>
 void launch(const GradArgs& a, hipStream_t st) {
-  const dim3 grid((a.C + kCols - 1) / kCols, a.G * a.splits, (a.Rp + 63) / 64);
-  general_kernel<T><<<grid, 256, 0, st>>>(a);
+  const int rb = a.Rp <= 16 ? 1 : a.Rp <= 32 ? 2 : 4;
+  const dim3 grid((a.C + kCols - 1) / kCols, a.G * a.splits, (a.Rp + 16 * rb - 1) / (16 * rb));
+  if (rb == 1) grad_kernel<T, Vec, 1><<<grid, 64 * kWaves, 0, st>>>(a);
+  else if (rb == 2) grad_kernel<T, Vec, 2><<<grid, 64 * kWaves, 0, st>>>(a);
+  else grad_kernel<T, Vec, 4><<<grid, 64 * kWaves, 0, st>>>(a);
   if (a.splits > 1) {
     const size_t n = (size_t)a.G * a.R * a.C;
     join_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(a.part, a.out, n, a.splits);
   }
 }
+template <class T>
+void launch(const GradArgs& a, hipStream_t st) {
+  constexpr size_t n = 16 / sizeof(typename T::raw);
+  const bool vec = ((size_t)a.z & 15) == 0 && a.ldz % n == 0;
+  vec ? launch<T, true>(a, st) : launch<T, false>(a, st);
+}
 
 }  // namespace
 
-// Ranges of tokens: enough workgroups for every compute unit to have a few, none of fewer than 256 tokens.
+// Ranges of tokens: two workgroups for each compute unit, none with fewer than 256 tokens.
 int grad_splits(size_t T, int C, int R, int G) {
   const size_t wgs = (size_t)((C + kCols - 1) / kCols) * G * ((R + 63) / 64);
-  const size_t want = (4 * (size_t)num_compute_units() + wgs - 1) / wgs;
+  const size_t want = (2 * (size_t)num_compute_units() + wgs - 1) / wgs;
   const size_t most = std::min<size_t>((T + 255) / 256, 65535 / G);
   return (int)std::max<size_t>(1, std::min(want, most));
 }

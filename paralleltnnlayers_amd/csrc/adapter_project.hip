@@ -4,6 +4,7 @@
 #include <algorithm>
 
 #include "adapter.h"
+#include "adapter_load.h"
 
 namespace cp4 {
 namespace adapter {
@@ -54,13 +55,13 @@ __global__ __launch_bounds__(256) void general_kernel(const ProjectArgs a) {
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int j = 0; j < 2; ++j)
-            acc[i][j] = mfma_f32(lz[wm + 16 * i + l][4 * q + g], lw[wn + 16 * j + l][4 * q + g], acc[i][j]);
+            acc[i][j] = mfma_f32(lz[wm + 16 * i + l][4 * q + g], lw[wn + 2 * l + j][4 * q + g], acc[i][j]);
     } else {
       u16x8 za[2], wb[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         za[i] = *reinterpret_cast<const u16x8*>(&lz[wm + 16 * i + l][8 * g]);
-        wb[i] = *reinterpret_cast<const u16x8*>(&lw[wn + 16 * i + l][8 * g]);
+        wb[i] = *reinterpret_cast<const u16x8*>(&lw[wn + 2 * l + i][8 * g]);
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -71,17 +72,12 @@ __global__ __launch_bounds__(256) void general_kernel(const ProjectArgs a) {
   // the adapters of this wave's 32 rows
   int id = lane < 32 && t0 + wm + lane < a.T ? a.ids[t0 + wm + lane] : -1;
   if (id < 0 || id >= a.G) id = -1;
-  Adapters todo(id);
-  int ad;
-  unsigned long long whose;
-  while (todo.take(ad, whose)) {
-    const Raw* const f = static_cast<const Raw*>(a.f) + (size_t)ad * a.R * a.N;
-    expand<T>(a.h + (t0 + wm + l) * a.Rp, a.Rp, a.planes, a.plane, whose, f, a.fn, a.fr, n0 + wn, a.N, a.R, acc);
-  }
+  expand_wave<T, NN, 2, 2>(a, id, [&](int i, int r, auto& x) { sum_planes(a, t0 + wm + 16 * i + l, r, x); }, false,
+                           n0 + wn, 1, 0, acc);
   Raw* const y = static_cast<Raw*>(a.y);
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    const int n = n0 + wn + 16 * j + l;
+    const int n = n0 + wn + 2 * l + j;
     if (n >= a.N) continue;
     const float b = a.bias ? a.bias[n] : 0.0f;
 #pragma unroll
@@ -113,11 +109,17 @@ void general(const ProjectArgs& a, bool nn, hipStream_t st) {
 }  // namespace
 
 size_t project_part_bytes(size_t T, int K, int N, int dtype) {
-  return tile_part_bytes(tile_plan(T, K, N, dtype), T, N);
+  const RowsPlan rows = rows_plan(T, K, N, dtype);
+  return std::max(tile_part_bytes(tile_plan(T, K, N, dtype), T, N),
+                  rows.splits > 1 ? (size_t)rows.splits * T * N * 4 : 0);
 }
 
 hipError_t project_launch(const ProjectArgs& a, float* part, int dtype, bool nn, hipStream_t st) {
-  if (tile_supported(a, dtype, nn)) return tile_launch(a, tile_plan(a.T, a.K, a.N, dtype), part, dtype, nn, st);
+  if (tile_supported(a, dtype, nn)) {
+    const RowsPlan rows = nn ? RowsPlan{} : rows_plan(a.T, a.K, a.N, dtype);
+    if (rows.nb) return rows_launch(a, rows, part, dtype, st);
+    return tile_launch(a, tile_plan(a.T, a.K, a.N, dtype), part, dtype, nn, st);
+  }
   if (dtype == CP4_DTYPE_F32) general<F32>(a, nn, st);
   else if (dtype == CP4_DTYPE_BF16) general<BF16>(a, nn, st);
   else general<F16>(a, nn, st);

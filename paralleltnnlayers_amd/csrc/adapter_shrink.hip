@@ -87,9 +87,8 @@ __global__ __launch_bounds__(64 * kWaves) void shrink_kernel(const ShrinkArgs a)
       if ((turn++ & (ways - 1)) != mine) continue;
       const Raw* const f = static_cast<const Raw*>(a.f) + (size_t)ad * a.R * a.K;
       f32x4 d[MB][RB] = {};
-      auto multiply = [&](int u, bool full) {
+      auto load = [&](int u, bool full, u32x4 (&zv)[MB][2], u32x4 (&fv)[RB][2]) {
         const int k = u * U + 2 * n * g, left = full ? 2 * n : a.K - k;
-        u32x4 zv[MB][2], fv[RB][2];
 #pragma unroll
         for (int i = 0; i < MB; ++i) load_row<T, Vec>(z[i] + (size_t)u * U, left, full, zv[i]);
         if constexpr (!TR) {
@@ -124,6 +123,8 @@ __global__ __launch_bounds__(64 * kWaves) void shrink_kernel(const ShrinkArgs a)
             __builtin_memcpy(&fv[j][1], y[1], 16);
           }
         }
+      };
+      auto multiply = [&](const u32x4 (&zv)[MB][2], const u32x4 (&fv)[RB][2]) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -139,15 +140,21 @@ __global__ __launch_bounds__(64 * kWaves) void shrink_kernel(const ShrinkArgs a)
               }
             }
       };
+      constexpr int kAhead = MB + RB <= 3 ? 4 : 2;                   // turns whose loads come before their products
       int u = first;
-      for (; u + 4 <= whole; u += 4) {                               // (the loads of four turns before their products)
-        multiply(u, true);
-        multiply(u + 1, true);
-        multiply(u + 2, true);
-        multiply(u + 3, true);
+      for (; u + kAhead <= whole; u += kAhead) {
+        u32x4 zv[kAhead][MB][2], fv[kAhead][RB][2];
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e) load(u + e, true, zv[e], fv[e]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e) multiply(zv[e], fv[e]);
       }
-      for (; u < whole; ++u) multiply(u, true);
-      for (; u < last; ++u) multiply(u, false);
+      for (; u < last; ++u) {
+        u32x4 zv[MB][2], fv[RB][2];
+        load(u, u < whole, zv, fv);
+        multiply(zv, fv);
+      }
 #pragma unroll
       for (int i = 0; i < MB; ++i)
 #pragma unroll

@@ -21,14 +21,12 @@
 #include <algorithm>
 
 #include "adapter.h"
+#include "adapter_load.h"
 #include "die_order.h"
 
 namespace cp4 {
 namespace adapter {
 namespace {
-
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
 
 template <class T>
 constexpr int kStep = 64 / sizeof(typename T::raw);                  // depth of a step
@@ -37,129 +35,6 @@ constexpr int kVec = 16 / sizeof(typename T::raw);                   // values o
 
 // s_waitcnt's operand: all but `loads` memory loads done, and all of the LDS's.
 constexpr int wait_for(int loads) { return (loads & 15) | (loads >> 4) << 14 | 7 << 4; }
-
-// 8 rows (depths) of NB columns in 16 bits -> NB columns of 8 depths.
-template <int NB>
-__device__ __forceinline__ void turn(const unsigned (&in)[8][NB / 2], u16x8 (&out)[NB]) {
-#pragma unroll
-  for (int j = 0; j < NB; ++j) {
-    u32x4 d;
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      d[q] = __builtin_amdgcn_perm(in[2 * q + 1][j / 2], in[2 * q][j / 2], j & 1 ? 0x07060302u : 0x05040100u);
-    out[j] = __builtin_bit_cast(u16x8, d);
-  }
-}
-
-// `count` (may be <= 0 or beyond n) values of p, zero behind; vec: p is on a 16-byte boundary.
-template <int n, class Raw>
-__device__ __forceinline__ void load_some(const Raw* p, int count, bool vec, Raw (&v)[n]) {
-  if (vec && count >= n) {
-    constexpr int each = 16 / sizeof(Raw);
-    if constexpr (n >= each) {
-#pragma unroll
-      for (int i = 0; i < n / each; ++i) {
-        const u32x4 d = reinterpret_cast<const u32x4*>(p)[i];
-        __builtin_memcpy(&v[i * each], &d, 16);
-      }
-      return;
-    } else if constexpr (n * sizeof(Raw) == 8) {
-      const u32x2 d = *reinterpret_cast<const u32x2*>(p);
-      __builtin_memcpy(&v[0], &d, 8);
-      return;
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < n; ++i) v[i] = i < count ? p[i] : Raw(0);
-}
-
-// Adds h F_a^T to a wave's MB x NB blocks (columns as above) for the rows whose bit is set; see expand()
-// in adapter.h.  h is the sum of a.planes planes.
-template <class T, bool NN, int MB, int NB>
-__device__ __forceinline__ void expand_wave(const ProjectArgs& a, const float* h, unsigned long long whose,
-                                            const typename T::raw* f, bool vec, int n0, f32x4 (&acc)[MB][NB]) {
-  typedef typename T::raw Raw;
-  const int lane = threadIdx.x & 63, l = lane & 15, g = lane >> 4, n = n0 + NB * l;
-  constexpr bool kF32 = __is_same(T, F32);
-  for (int r0 = 0; r0 < a.R; r0 += 16) {
-    // fp32: depth 4 g + q in product q; 16 bits: ranks 8 (g & 1) + q, first parts for g < 2
-    const int rl = kF32 ? 4 * g : 8 * (g & 1);
-    constexpr int kOwn = kF32 ? 4 : 8;
-    float hv[MB][kOwn];
-#pragma unroll
-    for (int i = 0; i < MB; ++i) {
-#pragma unroll
-      for (int q = 0; q < kOwn; ++q) hv[i][q] = 0.0f;
-      if (whose >> (16 * i + l) & 1) {
-        const float* p = h + (size_t)16 * i * a.Rp + r0 + rl;
-        for (int s = 0; s < a.planes; ++s, p += a.plane)
-#pragma unroll
-          for (int q = 0; q < kOwn; q += 4) {
-            const f32x4 x = *reinterpret_cast<const f32x4*>(p + q);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) hv[i][q + e] += x[e];
-          }
-      }
-    }
-    Raw fv[NB][kOwn];                                                // [column][rank]
-    if constexpr (NN) {
-      Raw fr[kOwn][NB];
-#pragma unroll
-      for (int q = 0; q < kOwn; ++q)
-        load_some<NB>(f + (size_t)(r0 + rl + q) * a.fr + n, r0 + rl + q < a.R ? a.N - n : 0, vec, fr[q]);
-#pragma unroll
-      for (int j = 0; j < NB; ++j)
-#pragma unroll
-        for (int q = 0; q < kOwn; ++q) fv[j][q] = fr[q][j];
-    } else {
-#pragma unroll
-      for (int j = 0; j < NB; ++j)
-        load_some<kOwn>(f + (size_t)(n + j) * a.fn + r0 + rl, n + j < a.N ? a.R - r0 - rl : 0, vec, fv[j]);
-    }
-    u16x8 ha[MB];
-    if constexpr (!kF32) {
-#pragma unroll
-      for (int i = 0; i < MB; ++i) {
-        u16x8 hi, lo;
-        two_parts(hv[i], hi, lo);
-        ha[i] = g < 2 ? hi : lo;
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < NB; ++j) {
-      u16x8 fh = {}, fl = {};
-      if constexpr (__is_same(T, F16)) {
-        float x[8];
-#pragma unroll
-        for (int q = 0; q < 8; ++q) x[q] = F16::widen(fv[j][q]);
-        two_parts(x, fh, fl);
-      } else if constexpr (!kF32) {
-#pragma unroll
-        for (int q = 0; q < 8; ++q) fh[q] = fv[j][q];
-      }
-#pragma unroll
-      for (int i = 0; i < MB; ++i) {
-        const unsigned rows = (unsigned)(whose >> (16 * i)) & 0xffffu;
-        if (!rows) continue;
-        f32x4 d = acc[i][j];
-        if constexpr (kF32) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) d = mfma_f32(hv[i][q], fv[j][q], d);
-        } else {
-          if constexpr (__is_same(T, F16)) d = mfma_bf16(ha[i], fl, d);
-          d = mfma_bf16(ha[i], fh, d);
-        }
-        if (rows == 0xffffu) {
-          acc[i][j] = d;
-        } else {
-#pragma unroll
-          for (int v = 0; v < 4; ++v)
-            if (rows >> (4 * g + v) & 1) acc[i][j][v] = d[v];
-        }
-      }
-    }
-  }
-}
 
 struct TileArgs {
   ProjectArgs p;
@@ -358,12 +233,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
     const size_t row = t0 + wm + lane;
     int id = lane < 16 * MB && row < a.T ? a.ids[row] : -1;
     if (id >= a.G) id = -1;
-    Adapters todo(id);
-    int ad;
-    unsigned long long whose;
-    while (todo.take(ad, whose))
-      expand_wave<T, NN, MB, NB>(a, a.h + (t0 + wm + l) * a.Rp, whose, static_cast<const Raw*>(a.f) + (size_t)ad * a.R * a.N,
-                                 even_f, n0 + wn, acc);
+    expand_wave<T, NN, MB, NB>(a, id, [&](int i, int r, auto& x) { sum_planes(a, t0 + wm + 16 * i + l, r, x); }, even_f,
+                               n0 + wn, 1, 0, acc);
   }
   const int n = n0 + wn + NB * l;
   if (n >= a.N) return;
@@ -454,10 +325,6 @@ __global__ __launch_bounds__(256) void join_kernel(const float* part, const floa
 template <class T, bool NN, int MB, int NB, int WM, int WN>
 void launch(TileArgs t, hipStream_t st) {
   tile_kernel<T, NN, MB, NB, WM, WN><<<die_grid((long)t.mt * t.nt * t.splits), 64 * WM * WN, 0, st>>>(t);
-  if (t.splits > 1) {
-    const size_t n = t.p.T * (size_t)t.p.N;
-    join_kernel<T><<<(unsigned)((n + 1023) / 1024), 256, 0, st>>>(t.part, t.p.bias, t.p.y, n, t.p.N, t.splits);
-  }
 }
 template <class T, bool NN>
 void launch_shape(const TileArgs& t, int which, hipStream_t st) {
@@ -472,7 +339,7 @@ constexpr int kRows[3] = {128, 128, 64}, kCols[3] = {256, 128, 256};
 
 TilePlan tile_plan(size_t T, int K, int N, int dtype) {
   const int KS = dtype == CP4_DTYPE_F32 ? 16 : 32;
-  const long slots = 2L * num_compute_units();
+  const long units = num_compute_units();
   const int steps = (K + KS - 1) / KS;
   TilePlan best{};
   double least = 0;
@@ -481,11 +348,12 @@ TilePlan tile_plan(size_t T, int K, int N, int dtype) {
     for (int s = 1; s <= 64 && s <= std::max(1, steps / 4); s *= 2) {
       const int each = (steps + s - 1) / s;
       const long wgs = tiles * ((steps + each - 1) / each);
-      // steps of a round of workgroups, by what a step takes of the matrix cores, and the parts' way to memory and back
-      const double rate = w == 0 ? 1.0 : w == 1 ? 0.65 : 0.65;
-      const double per = (double)kRows[w] * kCols[w] / rate * each + 256.0 * 128 * 12;
-      double cost = per * ((wgs + slots - 1) / slots);
-      if (s > 1) cost += 256.0 * 128 * 40 + (double)T * N * (s + 1) * 4.0 * 0.11;
+      // microseconds: a compute unit's tiles one after the other at its share of the matrix cores' rate (a
+      // workgroup alone reaches less of it), their starts and ends, the parts' way to memory and back
+      const double flops = 2.0 * kRows[w] * kCols[w] * KS * each, rate = (dtype == CP4_DTYPE_F32 ? 0.5e6 : w == 0 ? 5.0e6 : 3.6e6);
+      const long most = (wgs + units - 1) / units;
+      double cost = most * flops / (most == 1 ? 0.7 * rate : rate) + 2.0 + most;
+      if (s > 1) cost += 4.0 + (double)T * N * (s + 0.5) * 4.0 / 2.0e6;
       if (!best.splits || cost < least) {
         least = cost;
         best.which = w;
@@ -506,6 +374,15 @@ bool tile_supported(const ProjectArgs& a, int dtype, bool nn) {
   return a.ldz * e * 128 < (size_t)1 << 31 && a.ldw * e * 256 < (size_t)1 << 31 && a.T < ((size_t)1 << 31) - 256;
 }
 
+hipError_t parts_join(const float* part, const float* bias, void* y, size_t T, int N, int splits, int dtype, hipStream_t st) {
+  const size_t n = T * (size_t)N;
+  const unsigned grid = (unsigned)((n + 1023) / 1024);
+  if (dtype == CP4_DTYPE_F32) join_kernel<F32><<<grid, 256, 0, st>>>(part, bias, y, n, N, splits);
+  else if (dtype == CP4_DTYPE_BF16) join_kernel<BF16><<<grid, 256, 0, st>>>(part, bias, y, n, N, splits);
+  else join_kernel<F16><<<grid, 256, 0, st>>>(part, bias, y, n, N, splits);
+  return hipGetLastError();
+}
+
 hipError_t tile_launch(const ProjectArgs& a, const TilePlan& plan, float* part, int dtype, bool nn, hipStream_t st) {
   TileArgs t{};
   t.p = a;
@@ -517,7 +394,8 @@ hipError_t tile_launch(const ProjectArgs& a, const TilePlan& plan, float* part, 
   if (dtype == CP4_DTYPE_F32) nn ? launch_shape<F32, true>(t, plan.which, st) : launch_shape<F32, false>(t, plan.which, st);
   else if (dtype == CP4_DTYPE_BF16) nn ? launch_shape<BF16, true>(t, plan.which, st) : launch_shape<BF16, false>(t, plan.which, st);
   else nn ? launch_shape<F16, true>(t, plan.which, st) : launch_shape<F16, false>(t, plan.which, st);
-  return hipGetLastError();
+  if (const hipError_t e = hipGetLastError()) return e;
+  return plan.splits > 1 ? parts_join(part, a.bias, a.y, a.T, a.N, plan.splits, dtype, st) : hipSuccess;
 }
 
 }  // namespace adapter
