@@ -73,10 +73,9 @@ bool tile_supported(const ProjectArgs&, int dtype, bool nn);
 hipError_t tile_launch(const ProjectArgs&, const TilePlan&, float* part, int dtype, bool nn, hipStream_t);
 // y = the sum of [splits][T][N] partial sums, and the bias (may be null).
 hipError_t parts_join(const float* part, const float* bias, void* y, size_t T, int N, int splits, int dtype, hipStream_t);
-// Up to 64 tokens (w [N][K], rows on 16-byte boundaries): nb blocks of 16 columns a workgroup; nb 0: not for this
-// kernel.
+// Up to 64 tokens in 16 bits, 32 in fp32 (w [N][K], rows on 16-byte boundaries).  splits 0: not for this kernel.
 struct RowsPlan {
-  int nb, splits;
+  int splits;
 };
 RowsPlan rows_plan(size_t T, int K, int N, int dtype);
 hipError_t rows_launch(const ProjectArgs&, const RowsPlan&, float* part, int dtype, hipStream_t);

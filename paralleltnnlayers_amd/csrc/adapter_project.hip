@@ -117,7 +117,7 @@ size_t project_part_bytes(size_t T, int K, int N, int dtype) {
 hipError_t project_launch(const ProjectArgs& a, float* part, int dtype, bool nn, hipStream_t st) {
   if (tile_supported(a, dtype, nn)) {
     const RowsPlan rows = nn ? RowsPlan{} : rows_plan(a.T, a.K, a.N, dtype);
-    if (rows.nb) return rows_launch(a, rows, part, dtype, st);
+    if (rows.splits) return rows_launch(a, rows, part, dtype, st);
     return tile_launch(a, tile_plan(a.T, a.K, a.N, dtype), part, dtype, nn, st);
   }
   if (dtype == CP4_DTYPE_F32) general<F32>(a, nn, st);

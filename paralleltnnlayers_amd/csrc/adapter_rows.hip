@@ -1,13 +1,11 @@
 // The shared projection of up to 64 tokens (include/cp4/adapter.h): bound by reading W once, so nothing
 // stands between memory and the matrix cores.
 //
-// A workgroup takes 16 or 64 columns (rows of W) of all tokens; its eight waves share the inputs, a cache
+// A workgroup takes 16 columns (rows of W) of all tokens; its eight waves share the inputs, a cache
 // line of every row a turn and four turns' loads ahead of their products, which keeps 64 KB of W under way
-// on every compute unit.  x comes from the L2 again for every workgroup: with few tokens that is less than
-// W itself, with many a workgroup takes more columns and the inputs are split over workgroups instead.  The
-// adapters' parts are shared out over the waves; all sums meet in the LDS.
+// on every compute unit.  x comes from the L2 again for every workgroup.  Where there are few columns the inputs
+// are split over workgroups too.  The adapters' parts are shared out over the waves; all sums meet in the LDS.
 #include <algorithm>
-#include <cstdlib>
 
 #include "adapter.h"
 #include "adapter_load.h"
@@ -24,10 +22,10 @@ struct RowsArgs {
   int splits;
 };
 
-template <class T, int MB, int NB>
+template <class T, int MB>
 __global__ __launch_bounds__(64 * kWaves, 2) void rows_kernel(const RowsArgs ra) {
   typedef typename T::raw Raw;
-  constexpr int n = 16 / sizeof(Raw), U = 128 / sizeof(Raw), kRow = 16 * NB + 4, kAhead = MB + NB <= 5 ? 4 : 2;
+  constexpr int n = 16 / sizeof(Raw), U = 128 / sizeof(Raw), NB = 1, kRow = 16 * NB + 4, kAhead = 4;
   constexpr int kSum = kWaves * 16 * MB * kRow, kH = 16 * MB * 256;
   __shared__ __attribute__((aligned(16))) float lds[kSum > kH ? kSum : kH];
   float* const hl = lds;                                             // [T][Rp], and then ...
@@ -136,35 +134,29 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows_kernel(const RowsArgs ra)
   }
 }
 
-template <class T, int MB, int NB>
+template <class T, int MB>
 void launch(const RowsArgs& r, hipStream_t st) {
-  rows_kernel<T, MB, NB><<<dim3((r.p.N + 16 * NB - 1) / (16 * NB), r.splits), 64 * kWaves, 0, st>>>(r);
-}
-template <class T, int NB>
-void launch_rows(const RowsArgs& r, hipStream_t st) {
-  const int mb = (int)(r.p.T + 15) / 16;
-  if (mb == 1) launch<T, 1, NB>(r, st);
-  else if (mb == 2) launch<T, 2, NB>(r, st);
-  else if (mb == 3) launch<T, 3, NB>(r, st);
-  else launch<T, 4, NB>(r, st);
+  rows_kernel<T, MB><<<dim3((r.p.N + 15) / 16, r.splits), 64 * kWaves, 0, st>>>(r);
 }
 template <class T>
-void launch_cols(const RowsArgs& r, int nb, hipStream_t st) {
-  if (nb == 1) launch_rows<T, 1>(r, st);
-  else launch_rows<T, 4>(r, st);
+void launch_rows(const RowsArgs& r, hipStream_t st) {
+  const int mb = (int)(r.p.T + 15) / 16;
+  if (mb == 1) launch<T, 1>(r, st);
+  else if (mb == 2) launch<T, 2>(r, st);
+  if constexpr (sizeof(typename T::raw) == 2) {
+    if (mb == 3) launch<T, 3>(r, st);
+    else if (mb == 4) launch<T, 4>(r, st);
+  }
 }
 
 }  // namespace
 
 RowsPlan rows_plan(size_t T, int K, int N, int dtype) {
   RowsPlan p{};
-  if (T > 64) return p;
-  const int mb = (int)(T + 15) / 16, units = (K * (dtype == CP4_DTYPE_F32 ? 4 : 2) + 127) / 128;
-  static const char* e = getenv("NB");
-  p.nb = e ? atoi(e) : mb <= 2 ? 1 : dtype == CP4_DTYPE_F32 ? 4 : 1;
-  const int tiles = (N + 16 * p.nb - 1) / (16 * p.nb);
+  if (T > (dtype == CP4_DTYPE_F32 ? 32 : 64)) return p;
+  const int units = (K * (dtype == CP4_DTYPE_F32 ? 4 : 2) + 127) / 128, tiles = (N + 15) / 16;
   p.splits = std::max(1, std::min(num_compute_units() / tiles, units / (2 * kWaves)));
-  if (p.nb == 1 && p.splits < 4) p.splits = 1;
+  if (p.splits < 4) p.splits = 1;
   return p;
 }
 
@@ -173,9 +165,9 @@ hipError_t rows_launch(const ProjectArgs& a, const RowsPlan& plan, float* part, 
   r.p = a;
   r.part = plan.splits > 1 ? part : nullptr;
   r.splits = plan.splits;
-  if (dtype == CP4_DTYPE_F32) launch_cols<F32>(r, plan.nb, st);
-  else if (dtype == CP4_DTYPE_BF16) launch_cols<BF16>(r, plan.nb, st);
-  else launch_cols<F16>(r, plan.nb, st);
+  if (dtype == CP4_DTYPE_F32) launch_rows<F32>(r, st);
+  else if (dtype == CP4_DTYPE_BF16) launch_rows<BF16>(r, st);
+  else launch_rows<F16>(r, st);
   if (const hipError_t e = hipGetLastError()) return e;
   return plan.splits > 1 ? parts_join(part, a.bias, a.y, a.T, a.N, plan.splits, dtype, st) : hipSuccess;
 }

@@ -36,6 +36,124 @@ constexpr int kVec = 16 / sizeof(typename T::raw);                   // values o
 // s_waitcnt's operand: all but `loads` memory loads done, and all of the LDS's.
 constexpr int wait_for(int loads) { return (loads & 15) | (loads >> 4) << 14 | 7 << 4; }
 
+// Adds h F_a^T to a tile, one adapter of its rows after the other: the adapter's 16 ranks of all columns come
+// into the LDS, whatever their strides and alignment, and each wave multiplies them with its own rows.
+//
+// 16-bit types: depth 0 .. 15 of a product are the first parts of h, 16 .. 31 what they leave, against F_a twice
+// (f16: F_a in two parts as well, in two products).  Ranks beyond R are zero in h and read F_a's last one
+// again; columns beyond N read its last ones and are not stored.  A product is added only to the rows that are the
+// adapter's: an infinity or a NaN in one adapter is no other token's.
+template <class T, bool NN, int MB, int NB, int WM, int WN>
+__device__ __forceinline__ void expand_tile(const ProjectArgs& a, size_t t0, int n0, char* lds, f32x4 (&acc)[MB][NB]) {
+  typedef typename T::raw Raw;
+  constexpr bool kF32 = __is_same(T, F32);
+  constexpr int kThreads = 64 * WM * WN, BN = 16 * NB * WN, kUnits = 2 * BN / kThreads;   // 8 ranks of a column each
+  static_assert(MB == 4 && WM <= 2 && 2 * BN % kThreads == 0, "a wave's rows are a ballot");
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 15, g = lane >> 4;
+  const int wm = wave / WN, wn = 16 * NB * (wave % WN);
+  int id[WM];
+  unsigned long long have[WM], any = 0;
+#pragma unroll
+  for (int w = 0; w < WM; ++w) {
+    const size_t row = t0 + 64 * w + lane;
+    id[w] = row < a.T ? a.ids[row] : -1;
+    if (id[w] < 0 || id[w] >= a.G) id[w] = -1;
+    any |= have[w] = __ballot(id[w] >= 0);
+  }
+  if (!any) return;
+  const bool vec = !NN && ((size_t)a.f & 15) == 0 && a.R % 8 == 0;
+  const float* const h = a.h + (t0 + 64 * wm + l) * a.Rp;
+  for (int r0 = 0; r0 < a.R; r0 += 16) {
+    f32x4 hv[MB];                                                    // fp32: ranks 4 g ..
+    u16x8 ha[MB];                                                    // 16 bits: ranks 8 (g & 1) .., first parts for g < 2
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+      float x[8] = {};
+      if (have[WM == 2 ? wm : 0] >> (16 * i + l) & 1) {
+        const float* p = h + (size_t)16 * i * a.Rp + r0 + (kF32 ? 4 * g : 8 * (g & 1));
+        for (int s = 0; s < a.planes; ++s, p += a.plane)
+#pragma unroll
+          for (int q = 0; q < (kF32 ? 4 : 8); ++q) x[q] += p[q];
+      }
+      hv[i] = f32x4{x[0], x[1], x[2], x[3]};
+      u16x8 hi, lo;
+      two_parts(x, hi, lo);
+      ha[i] = g < 2 ? hi : lo;
+    }
+    unsigned long long left[WM];
+#pragma unroll
+    for (int w = 0; w < WM; ++w) left[w] = have[w];
+    for (;;) {
+      int ad = -1;
+#pragma unroll
+      for (int w = 0; w < WM; ++w)
+        if (ad < 0 && left[w]) ad = __builtin_amdgcn_readlane(id[w], __builtin_ctzll(left[w]));
+      if (ad < 0) break;
+      unsigned long long mine = 0;
+#pragma unroll
+      for (int w = 0; w < WM; ++w) {
+        const unsigned long long whose = __ballot(id[w] == ad);
+        left[w] &= ~whose;
+        if (w == wm) mine = whose;
+      }
+      const Raw* const f = static_cast<const Raw*>(a.f) + (size_t)ad * a.R * a.N;
+      __syncthreads();                                               // (nobody reads what was there)
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        const int at = u * kThreads + threadIdx.x, col = at % BN, half = at / BN, r = r0 + 8 * half;
+        const Raw* const p = f + (size_t)min(n0 + col, a.N - 1) * a.fn;
+        Raw x[8];
+        if (vec) {
+          const u32x4* const q = reinterpret_cast<const u32x4*>(p + min(r, a.R - 8));
+          __builtin_memcpy(x, q, 16);
+          if constexpr (kF32) __builtin_memcpy(x + 4, q + 1, 16);
+        } else {
+#pragma unroll
+          for (int q = 0; q < 8; ++q) x[q] = p[(size_t)min(r + q, a.R - 1) * a.fr];
+        }
+        const int in = col % (16 * NB), slot = col - in + 16 * (in % NB) + in / NB;      // block j's columns side by side
+        if constexpr (kF32) {
+          __builtin_memcpy(__builtin_assume_aligned(lds + slot * 64 + half * 32, 16), x, 32);
+        } else if constexpr (__is_same(T, F16)) {
+          float y[8];
+#pragma unroll
+          for (int q = 0; q < 8; ++q) y[q] = F16::widen(x[q]);
+          u16x8 hi, lo;
+          two_parts(y, hi, lo);
+          *reinterpret_cast<u16x8*>(lds + slot * 64 + half * 16) = hi;
+          *reinterpret_cast<u16x8*>(lds + slot * 64 + 32 + half * 16) = lo;
+        } else {
+          __builtin_memcpy(__builtin_assume_aligned(lds + slot * 32 + half * 16, 16), x, 16);
+        }
+      }
+      __syncthreads();
+      if (!mine) continue;
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        const char* const at = lds + (wn + 16 * j + l) * (__is_same(T, BF16) ? 32 : 64);
+        f32x4 fv = {};
+        u16x8 fh = {}, fl = {};
+        if constexpr (kF32) fv = *reinterpret_cast<const f32x4*>(at + g * 16);
+        else fh = *reinterpret_cast<const u16x8*>(at + (g & 1) * 16);
+        if constexpr (__is_same(T, F16)) fl = *reinterpret_cast<const u16x8*>(at + 32 + (g & 1) * 16);
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+          f32x4 d = {};
+          if constexpr (kF32) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) d = mfma_f32(hv[i][q], fv[q], d);
+          } else {
+            if constexpr (__is_same(T, F16)) d = mfma_bf16(ha[i], fl, d);
+            d = mfma_bf16(ha[i], fh, d);
+          }
+#pragma unroll
+          for (int v = 0; v < 4; ++v) acc[i][j][v] += mine >> (16 * i + 4 * g + v) & 1 ? d[v] : 0.0f;
+        }
+      }
+    }
+  }
+}
+
 struct TileArgs {
   ProjectArgs p;
   float* part;            // [splits][T][N], or null: y
@@ -228,14 +346,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
     multiply(lds0);
   }
 
-  const bool even_f = ((size_t)a.f & 15) == 0 && (NN ? a.N : a.R) % kVec<T> == 0;
-  if (split == 0) {
-    const size_t row = t0 + wm + lane;
-    int id = lane < 16 * MB && row < a.T ? a.ids[row] : -1;
-    if (id >= a.G) id = -1;
-    expand_wave<T, NN, MB, NB>(a, id, [&](int i, int r, auto& x) { sum_planes(a, t0 + wm + 16 * i + l, r, x); }, even_f,
-                               n0 + wn, 1, 0, acc);
-  }
+  if (split == 0) expand_tile<T, NN, MB, NB, WM, WN>(a, t0, n0, lds0, acc);
   const int n = n0 + wn + NB * l;
   if (n >= a.N) return;
   if (ta.part) {
