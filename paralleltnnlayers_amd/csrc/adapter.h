@@ -37,7 +37,7 @@ struct ProjectArgs {
   int K, N, R, Rp, G;
   int fn, fr;
   int planes;             // h is the sum of so many planes ...
-  size_t plane;           // ... so many values apart
+  size_t plane;           // ... so many values apart (more than one: only where project_sums_planes)
 };
 
 // out[a][r][c] = sum over tokens with ids[t] = a of p[t][r] z[t][c], at out + a * R * C + r * outr +
@@ -53,12 +53,15 @@ struct GradArgs {
   int C, R, Rp, G;
   int outr, outc;
   int splits;
-  int planes;             // p is the sum of so many planes [T][Rp]
 };
 
 constexpr size_t kShrinkWide = 4096;     // tokens from which a workgroup takes 32 of them
 int shrink_planes(size_t T, int K, int dtype);
 hipError_t shrink_launch(const ShrinkArgs&, int dtype, hipStream_t);
+// h [n] = the sum of `planes` planes of n values (n: a multiple of 4), the first of which may be h.
+hipError_t planes_join(float* h, const float* from, size_t n, int planes, hipStream_t);
+// Whether the projection that these operands get adds up the planes of h itself.
+bool project_sums_planes(const ProjectArgs&, int dtype, bool nn);
 // part: project_part_bytes of scratch memory.
 size_t project_part_bytes(size_t T, int K, int N, int dtype);
 hipError_t project_launch(const ProjectArgs&, float* part, int dtype, bool nn, hipStream_t);
@@ -66,6 +69,7 @@ hipError_t project_launch(const ProjectArgs&, float* part, int dtype, bool nn, h
 // sums take tile_part_bytes.
 struct TilePlan {
   int which, splits, each;
+  double cost;            // microseconds, about
 };
 TilePlan tile_plan(size_t T, int K, int N, int dtype);
 size_t tile_part_bytes(const TilePlan&, size_t T, int N);

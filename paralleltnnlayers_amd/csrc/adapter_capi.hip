@@ -37,9 +37,7 @@ cp4_status check_pointers(size_t bytes, std::initializer_list<const void*> value
   return CP4_OK;
 }
 
-size_t kept_bytes(const cp4_adapter_shape& s, int dtype) {
-  return (size_t)shrink_planes(s.T, (int)s.K, dtype) * s.T * padded(s) * 4;
-}
+size_t h_bytes(const cp4_adapter_shape& s) { return s.T * padded(s) * 4; }
 
 struct BackwardPlan {
   int splits_a, splits_b, dh_planes;
@@ -50,7 +48,7 @@ BackwardPlan backward_plan(const cp4_adapter_shape& s, int dtype) {
   p.splits_a = grad_splits(s.T, (int)s.K, (int)s.R, (int)s.G);
   p.splits_b = grad_splits(s.T, (int)s.N, (int)s.R, (int)s.G);
   p.dh_planes = shrink_planes(s.T, (int)s.N, dtype);
-  p.part_at = align256((size_t)p.dh_planes * s.T * padded(s) * 4);
+  p.part_at = align256(p.dh_planes * h_bytes(s));
   const size_t each = (size_t)s.G * s.R * 4;
   const size_t pa = p.splits_a > 1 ? p.splits_a * each * s.K : 0, pb = p.splits_b > 1 ? p.splits_b * each * s.N : 0;
   p.total = p.part_at + align256(std::max({pa, pb, project_part_bytes(s.T, (int)s.N, (int)s.K, dtype)}));   // (one after the other)
@@ -60,12 +58,12 @@ BackwardPlan backward_plan(const cp4_adapter_shape& s, int dtype) {
 }  // namespace
 
 extern "C" size_t cp4_adapter_kept_bytes(const cp4_adapter_shape* s, int dtype) {
-  return check_shape(s, dtype) == CP4_OK ? kept_bytes(*s, dtype) : 0;
+  return check_shape(s, dtype) == CP4_OK ? h_bytes(*s) : 0;
 }
 
 extern "C" size_t cp4_adapter_forward_workspace_bytes(const cp4_adapter_shape* s, int dtype) {
   if (check_shape(s, dtype) != CP4_OK) return 0;
-  return align256(kept_bytes(*s, dtype)) + align256(project_part_bytes(s->T, (int)s->K, (int)s->N, dtype));
+  return align256(shrink_planes(s->T, (int)s->K, dtype) * h_bytes(*s)) + align256(project_part_bytes(s->T, (int)s->K, (int)s->N, dtype));
 }
 
 extern "C" cp4_status cp4_adapter_forward(const cp4_adapter_shape* s, int dtype, const void* x, const void* W,
@@ -81,19 +79,26 @@ extern "C" cp4_status cp4_adapter_forward(const cp4_adapter_shape* s, int dtype,
     return fail_with(CP4_ERR_WORKSPACE, "workspace missing, too small or not aligned to 256 bytes");
   if ((size_t)kept & 15) return fail_with(CP4_ERR_WORKSPACE, "kept is not aligned to 16 bytes");
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  float* const h = kept ? kept : static_cast<float*>(workspace);
+  float* const planes = static_cast<float*>(workspace);
   ShrinkArgs sh{};
-  sh.z = x; sh.f = A; sh.ids = ids; sh.scale = scale; sh.h = h;
+  sh.z = x; sh.f = A; sh.ids = ids; sh.scale = scale;
   sh.T = s->T; sh.ldz = s->ldx ? s->ldx : s->K;
   sh.K = (int)s->K; sh.R = (int)s->R; sh.Rp = padded(*s); sh.G = (int)s->G;
   sh.fr = (int)s->K; sh.fk = 1; sh.planes = shrink_planes(s->T, (int)s->K, dtype);
+  sh.h = sh.planes == 1 && kept ? kept : planes;
   if (const hipError_t e = shrink_launch(sh, dtype, st)) return fail_hip(e, "cp4_adapter_forward");
   ProjectArgs p{};
-  p.z = x; p.w = W; p.f = B; p.h = h; p.bias = bias; p.ids = ids; p.y = y;
+  p.z = x; p.w = W; p.f = B; p.h = sh.h; p.bias = bias; p.ids = ids; p.y = y;
   p.T = s->T; p.ldz = sh.ldz; p.ldw = s->ldw ? s->ldw : s->K;
   p.K = (int)s->K; p.N = (int)s->N; p.R = (int)s->R; p.Rp = sh.Rp; p.G = (int)s->G;
   p.fn = (int)s->R; p.fr = 1; p.planes = sh.planes; p.plane = p.T * p.Rp;
-  float* const part = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(kept_bytes(*s, dtype)));
+  if (p.planes > 1 && (kept || !project_sums_planes(p, dtype, false))) {
+    float* const h = kept ? kept : planes;
+    if (const hipError_t e = planes_join(h, planes, p.plane, p.planes, st)) return fail_hip(e, "cp4_adapter_forward");
+    p.h = h;
+    p.planes = 1;
+  }
+  float* const part = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(sh.planes * h_bytes(*s)));
   if (const hipError_t e = project_launch(p, part, dtype, false, st)) return fail_hip(e, "cp4_adapter_forward");
   return CP4_OK;
 }
@@ -130,23 +135,25 @@ extern "C" cp4_status cp4_adapter_backward(const cp4_adapter_shape* s, int dtype
     sh.K = (int)s->N; sh.R = (int)s->R; sh.Rp = Rp; sh.G = (int)s->G;
     sh.fr = 1; sh.fk = (int)s->R; sh.planes = plan.dh_planes;
     if (const hipError_t e = shrink_launch(sh, dtype, st)) return fail_hip(e, "cp4_adapter_backward");
+    if (sh.planes > 1)
+      if (const hipError_t e = planes_join(dh, dh, s->T * Rp, sh.planes, st)) return fail_hip(e, "cp4_adapter_backward");
   }
   if (s->T && dx) {
     ProjectArgs p{};
     p.z = dy; p.w = W; p.f = A; p.h = dh; p.ids = ids; p.y = dx;
     p.T = s->T; p.ldz = lddy; p.ldw = s->ldw ? s->ldw : s->K;
     p.K = (int)s->N; p.N = (int)s->K; p.R = (int)s->R; p.Rp = Rp; p.G = (int)s->G;
-    p.fn = 1; p.fr = (int)s->K; p.planes = plan.dh_planes; p.plane = p.T * p.Rp;
+    p.fn = 1; p.fr = (int)s->K; p.planes = 1;
     if (const hipError_t e = project_launch(p, part, dtype, true, st)) return fail_hip(e, "cp4_adapter_backward");
   }
   if (dA) {
     GradArgs g{};
     g.ids = ids; g.part = part; g.T = s->T; g.R = (int)s->R; g.Rp = Rp; g.G = (int)s->G;
     g.p = dh; g.z = x; g.out = dA; g.ldz = ldx; g.C = (int)s->K; g.outr = (int)s->K; g.outc = 1;
-    g.splits = plan.splits_a; g.planes = plan.dh_planes;
+    g.splits = plan.splits_a;
     if (const hipError_t e = grad_launch(g, dtype, st)) return fail_hip(e, "cp4_adapter_backward");
     g.p = kept; g.z = dy; g.out = dB; g.ldz = lddy; g.C = (int)s->N; g.outr = 1; g.outc = (int)s->R;
-    g.splits = plan.splits_b; g.planes = shrink_planes(s->T, (int)s->K, dtype);
+    g.splits = plan.splits_b;
     if (const hipError_t e = grad_launch(g, dtype, st)) return fail_hip(e, "cp4_adapter_backward");
   }
   return CP4_OK;

@@ -37,7 +37,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void grad_kernel(const GradArgs a) 
   const size_t first = min(a.T, split * per), last = min(a.T, first + per);
   const Raw* const z = static_cast<const Raw*>(a.z) + min(c, a.C - 1);
   const int cols = a.C - c;
-  const size_t plane = a.T * a.Rp;
   f32x4 acc[RB][8] = {};
   for (size_t w0 = first; w0 < last; w0 += kWindow) {
     // the list: each wave looks through its eighth of the window
@@ -86,9 +85,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void grad_kernel(const GradArgs a) 
         const float* const row = a.p + (w0 + t[q]) * a.Rp + r0 + l;
 #pragma unroll
         for (int i = 0; i < RB; ++i) p[i][q] = there && r0 + 16 * i < a.Rp ? row[16 * i] : 0.0f;
-        for (int s = 1; s < a.planes; ++s)
-#pragma unroll
-          for (int i = 0; i < RB; ++i) p[i][q] += there && r0 + 16 * i < a.Rp ? row[s * plane + 16 * i] : 0.0f;
       }
       if constexpr (kF32) {
 #pragma unroll

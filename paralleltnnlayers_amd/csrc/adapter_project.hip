@@ -108,16 +108,64 @@ void general(const ProjectArgs& a, bool nn, hipStream_t st) {
 
 }  // namespace
 
-size_t project_part_bytes(size_t T, int K, int N, int dtype) {
+// A tile's worth of rows that the last round of tiles would be for can be cheaper on its own.
+static size_t main_rows(size_t T, int K, int N, int dtype, bool nn) {
+  const TilePlan all = tile_plan(T, K, N, dtype);
+  size_t best = T;
+  double least = all.cost;
+  for (size_t tile : {256, 128}) {
+    const size_t rest = T % tile;
+    if (!rest || T <= 2 * tile) continue;
+    // (the rest's own launches: some microseconds, and W once more)
+    const bool rows = !nn && rows_plan(rest, K, N, dtype).splits;
+    const double w = (double)K * N * (dtype == CP4_DTYPE_F32 ? 4 : 2) / 3.0e6;
+    const double cost = tile_plan(T - rest, K, N, dtype).cost + 4.0 + (rows ? 6.0 + w : std::max(w, tile_plan(rest, K, N, dtype).cost));
+    if (cost < least) {
+      least = cost;
+      best = T - rest;
+    }
+  }
+  return best;
+}
+
+static size_t plan_bytes(size_t T, int K, int N, int dtype) {
   const RowsPlan rows = rows_plan(T, K, N, dtype);
   return std::max(tile_part_bytes(tile_plan(T, K, N, dtype), T, N),
                   rows.splits > 1 ? (size_t)rows.splits * T * N * 4 : 0);
+}
+
+size_t project_part_bytes(size_t T, int K, int N, int dtype) {
+  size_t most = plan_bytes(T, K, N, dtype);
+  for (bool nn : {false, true}) {
+    const size_t main = main_rows(T, K, N, dtype, nn);
+    if (main < T) most = std::max({most, plan_bytes(main, K, N, dtype), plan_bytes(T - main, K, N, dtype)});
+  }
+  return most;
+}
+
+bool project_sums_planes(const ProjectArgs& a, int dtype, bool nn) {
+  return !nn && tile_supported(a, dtype, nn) && rows_plan(a.T, a.K, a.N, dtype).splits;
 }
 
 hipError_t project_launch(const ProjectArgs& a, float* part, int dtype, bool nn, hipStream_t st) {
   if (tile_supported(a, dtype, nn)) {
     const RowsPlan rows = nn ? RowsPlan{} : rows_plan(a.T, a.K, a.N, dtype);
     if (rows.splits) return rows_launch(a, rows, part, dtype, st);
+    const size_t main = main_rows(a.T, a.K, a.N, dtype, nn);
+    if (main < a.T) {
+      const size_t e = dtype == CP4_DTYPE_F32 ? 4 : 2;
+      ProjectArgs p = a, q = a;
+      p.T = main;
+      q.T = a.T - main;
+      q.z = static_cast<const char*>(a.z) + main * a.ldz * e;
+      q.h = a.h + main * a.Rp;
+      q.ids = a.ids + main;
+      q.y = static_cast<char*>(a.y) + main * a.N * e;
+      if (const hipError_t err = tile_launch(p, tile_plan(p.T, p.K, p.N, dtype), part, dtype, nn, st)) return err;
+      const RowsPlan few = nn ? RowsPlan{} : rows_plan(q.T, q.K, q.N, dtype);
+      if (few.splits) return rows_launch(q, few, part, dtype, st);
+      return tile_launch(q, tile_plan(q.T, q.K, q.N, dtype), part, dtype, nn, st);
+    }
     return tile_launch(a, tile_plan(a.T, a.K, a.N, dtype), part, dtype, nn, st);
   }
   if (dtype == CP4_DTYPE_F32) general<F32>(a, nn, st);

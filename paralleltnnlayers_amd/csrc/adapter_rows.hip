@@ -44,15 +44,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows_kernel(const RowsArgs ra)
     }
   const Raw *z[MB], *w[NB];
 #pragma unroll
-  for (int i = 0; i < MB; ++i) z[i] = static_cast<const Raw*>(a.z) + min(16 * i + l, rows - 1) * a.ldz + 2 * n * g;
+  for (int i = 0; i < MB; ++i) z[i] = static_cast<const Raw*>(a.z) + min(16 * i + l, rows - 1) * a.ldz + n * g;
 #pragma unroll
-  for (int j = 0; j < NB; ++j) w[j] = static_cast<const Raw*>(a.w) + min(n0 + NB * l + j, a.N - 1) * a.ldw + 2 * n * g;
+  for (int j = 0; j < NB; ++j) w[j] = static_cast<const Raw*>(a.w) + min(n0 + NB * l + j, a.N - 1) * a.ldw + n * g;
   const int units = (a.K + U - 1) / U, shares = kWaves * ra.splits, share = split * kWaves + wave;
   const int first = (int)((long)units * share / shares), last = (int)((long)units * (share + 1) / shares);
   const int whole = min(last, a.K / U);
 
   f32x4 acc[MB][NB] = {};
-  auto multiply = [&](const u32x4 (&zv)[MB][2], const u32x4 (&wv)[NB][2]) {
+  auto multiply = [&](const u32x4 (&zv)[MB][2], const u32x4 (&wv)[NB][2]) __attribute__((always_inline)) {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -68,7 +68,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows_kernel(const RowsArgs ra)
           }
         }
   };
-  auto ahead = [&](int u, auto count) {
+  auto ahead = [&](int u, auto count) __attribute__((always_inline)) {
     constexpr int c = decltype(count)::value;
     u32x4 zv[c][MB][2], wv[c][NB][2];
 #pragma unroll
@@ -76,11 +76,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows_kernel(const RowsArgs ra)
 #pragma unroll
       for (int j = 0; j < NB; ++j)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) wv[e][j][h] = reinterpret_cast<const u32x4*>(w[j] + (size_t)(u + e) * U)[h];
+        for (int h = 0; h < 2; ++h) wv[e][j][h] = reinterpret_cast<const u32x4*>(w[j] + (size_t)(u + e) * U)[4 * h];
 #pragma unroll
       for (int i = 0; i < MB; ++i)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) zv[e][i][h] = reinterpret_cast<const u32x4*>(z[i] + (size_t)(u + e) * U)[h];
+        for (int h = 0; h < 2; ++h) zv[e][i][h] = reinterpret_cast<const u32x4*>(z[i] + (size_t)(u + e) * U)[4 * h];
     }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -93,11 +93,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows_kernel(const RowsArgs ra)
     u32x4 zv[MB][2], wv[NB][2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const bool there = u * U + 2 * n * g + n * h < a.K;
+      const bool there = u * U + n * (4 * h + g) < a.K;
 #pragma unroll
-      for (int i = 0; i < MB; ++i) zv[i][h] = there ? reinterpret_cast<const u32x4*>(z[i] + (size_t)u * U)[h] : u32x4{};
+      for (int i = 0; i < MB; ++i) zv[i][h] = there ? reinterpret_cast<const u32x4*>(z[i] + (size_t)u * U)[4 * h] : u32x4{};
 #pragma unroll
-      for (int j = 0; j < NB; ++j) wv[j][h] = there ? reinterpret_cast<const u32x4*>(w[j] + (size_t)u * U)[h] : u32x4{};
+      for (int j = 0; j < NB; ++j) wv[j][h] = there ? reinterpret_cast<const u32x4*>(w[j] + (size_t)u * U)[4 * h] : u32x4{};
     }
     multiply(zv, wv);
   }

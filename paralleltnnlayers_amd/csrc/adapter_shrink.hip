@@ -6,7 +6,8 @@
 // these tokens have - one of a prompt, sixteen of single tokens - and, where there are fewer, the
 // inputs.  All rows are multiplied with each adapter and the rows that are not its own keep what they had; the
 // waves' sums meet in the LDS once, at the end.  With few tokens the inputs are split over workgroups as
-// well: each part leaves a plane of h of its own, and who reads h adds them up.
+// well: each part leaves a plane of h of its own, which the projection of few tokens adds up as it reads them and a
+// small launch does before any other.
 //
 // A lane's ranks are RB * (lane & 15) + j, not 16 j + (lane & 15), so that factors that lie rank by rank
 // (B, in the backward pass) come with loads of RB values.
@@ -22,7 +23,7 @@ constexpr int kWaves = 8;
 template <class T>
 constexpr int kUnit = 128 / sizeof(typename T::raw);                 // inputs of a loop's turn: a cache line a row
 
-// One operand's row of a turn: 8 (fp32: 4) values from each half of 32 bytes; zero from `left` on.
+// One operand's row of a turn: 16 bytes of each half (64 bytes on); zero from `left` on.
 template <class T, bool Vec>
 __device__ __forceinline__ void load_row(const typename T::raw* p, int left, bool full, u32x4 (&v)[2]) {
   typedef typename T::raw Raw;
@@ -30,7 +31,7 @@ __device__ __forceinline__ void load_row(const typename T::raw* p, int left, boo
   if constexpr (Vec) {
     if (full) {
       v[0] = reinterpret_cast<const u32x4*>(p)[0];
-      v[1] = reinterpret_cast<const u32x4*>(p)[1];
+      v[1] = reinterpret_cast<const u32x4*>(p)[4];
       return;
     }
   }
@@ -38,7 +39,7 @@ __device__ __forceinline__ void load_row(const typename T::raw* p, int left, boo
   for (int h = 0; h < 2; ++h) {
     Raw x[n];
 #pragma unroll
-    for (int q = 0; q < n; ++q) x[q] = n * h + q < left ? p[n * h + q] : Raw(0);
+    for (int q = 0; q < n; ++q) x[q] = full || 4 * n * h + q < left ? p[4 * n * h + q] : Raw(0);
     __builtin_memcpy(&v[h], x, 16);
   }
 }
@@ -76,7 +77,7 @@ __global__ __launch_bounds__(64 * kWaves) void shrink_kernel(const ShrinkArgs a)
   const bool even = a.R % RB == 0 && ((size_t)a.f & (RB * sizeof(Raw) - 1)) == 0;
   const Raw* z[MB];
 #pragma unroll
-  for (int i = 0; i < MB; ++i) z[i] = static_cast<const Raw*>(a.z) + (t0 + min(16 * i + l, rows - 1)) * a.ldz + 2 * n * g;
+  for (int i = 0; i < MB; ++i) z[i] = static_cast<const Raw*>(a.z) + (t0 + min(16 * i + l, rows - 1)) * a.ldz + n * g;
 
   for (int r0 = 0; r0 < a.Rp; r0 += 16 * RB) {
     f32x4 acc[MB][RB] = {};
@@ -87,8 +88,8 @@ __global__ __launch_bounds__(64 * kWaves) void shrink_kernel(const ShrinkArgs a)
       if ((turn++ & (ways - 1)) != mine) continue;
       const Raw* const f = static_cast<const Raw*>(a.f) + (size_t)ad * a.R * a.K;
       f32x4 d[MB][RB] = {};
-      auto load = [&](int u, bool full, u32x4 (&zv)[MB][2], u32x4 (&fv)[RB][2]) {
-        const int k = u * U + 2 * n * g, left = full ? 2 * n : a.K - k;
+      auto load = [&](int u, bool full, u32x4 (&zv)[MB][2], u32x4 (&fv)[RB][2]) __attribute__((always_inline)) {
+        const int k = u * U + n * g, left = full ? U : a.K - k;
 #pragma unroll
         for (int i = 0; i < MB; ++i) load_row<T, Vec>(z[i] + (size_t)u * U, left, full, zv[i]);
         if constexpr (!TR) {
@@ -103,15 +104,16 @@ __global__ __launch_bounds__(64 * kWaves) void shrink_kernel(const ShrinkArgs a)
           Raw x[2 * n][RB];
 #pragma unroll
           for (int q = 0; q < 2 * n; ++q) {
-            const Raw* const p = f + (size_t)(k + q) * a.R + r;
+            const int kq = q < n ? q : q + 3 * n;                     // (the second half lies 4 n inputs on)
+            const Raw* const p = f + (size_t)(k + kq) * a.R + r;
             if (RB > 1 && even) {                                    // (whole lanes of ranks)
-              if (r < a.R && q < left) __builtin_memcpy(x[q], __builtin_assume_aligned(p, RB * sizeof(Raw)), RB * sizeof(Raw));
+              if (r < a.R && kq < left) __builtin_memcpy(x[q], __builtin_assume_aligned(p, RB * sizeof(Raw)), RB * sizeof(Raw));
               else
 #pragma unroll
                 for (int j = 0; j < RB; ++j) x[q][j] = Raw(0);
             } else {
 #pragma unroll
-              for (int j = 0; j < RB; ++j) x[q][j] = r + j < a.R && q < left ? p[j] : Raw(0);
+              for (int j = 0; j < RB; ++j) x[q][j] = r + j < a.R && kq < left ? p[j] : Raw(0);
             }
           }
 #pragma unroll
@@ -124,7 +126,7 @@ __global__ __launch_bounds__(64 * kWaves) void shrink_kernel(const ShrinkArgs a)
           }
         }
       };
-      auto multiply = [&](const u32x4 (&zv)[MB][2], const u32x4 (&fv)[RB][2]) {
+      auto multiply = [&](const u32x4 (&zv)[MB][2], const u32x4 (&fv)[RB][2]) __attribute__((always_inline)) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -204,14 +206,27 @@ void launch(const ShrinkArgs& a, hipStream_t st) {
   else vec ? launch_rows<T, false, true>(a, st) : launch_rows<T, false, false>(a, st);
 }
 
+__global__ __launch_bounds__(256) void planes_kernel(float* h, const float* from, size_t n, int planes) {
+  const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  f32x4 x = *reinterpret_cast<const f32x4*>(from + i);
+  for (int s = 1; s < planes; ++s) x += *reinterpret_cast<const f32x4*>(from + s * n + i);
+  *reinterpret_cast<f32x4*>(h + i) = x;
+}
+
 }  // namespace
 
-// Parts of the inputs: enough workgroups for the chip, none with less than a turn for each wave.
+hipError_t planes_join(float* h, const float* from, size_t n, int planes, hipStream_t st) {
+  planes_kernel<<<(unsigned)((n + 1023) / 1024), 256, 0, st>>>(h, from, n, planes);
+  return hipGetLastError();
+}
+
+// Parts of the inputs: two workgroups for each compute unit, four turns or more a part.
 int shrink_planes(size_t T, int K, int dtype) {
   const int unit = dtype == CP4_DTYPE_F32 ? kUnit<F32> : kUnit<BF16>;
   const size_t wide = T >= kShrinkWide ? 32 : 16, tiles = std::max<size_t>(1, (T + wide - 1) / wide);
   const size_t most = std::max(1, (K + unit - 1) / unit / 4);
-  return (int)std::max<size_t>(1, std::min({(size_t)num_compute_units() / tiles, most, (size_t)16}));
+  return (int)std::max<size_t>(1, std::min({(2 * (size_t)num_compute_units() + tiles - 1) / tiles, most, (size_t)64}));
 }
 
 hipError_t shrink_launch(const ShrinkArgs& a, int dtype, hipStream_t st) {

@@ -19,67 +19,92 @@
 // Little work for the chip is split over the depth: the partial tiles go to the workspace in
 // fp32 (the first one with the adapters' part) and a second launch adds them up in their order.
 #include <algorithm>
+#include <cstdlib>
 
 #include "adapter.h"
 #include "adapter_load.h"
 #include "die_order.h"
+#include "split_bf16.h"
 
 namespace cp4 {
 namespace adapter {
 namespace {
 
 template <class T>
-constexpr int kStep = 64 / sizeof(typename T::raw);                  // depth of a step
-template <class T>
 constexpr int kVec = 16 / sizeof(typename T::raw);                   // values of a 16-byte load
 
 // s_waitcnt's operand: all but `loads` memory loads done, and all of the LDS's.
 constexpr int wait_for(int loads) { return (loads & 15) | (loads >> 4) << 14 | 7 << 4; }
 
-// Adds h F_a^T to a tile, one adapter of its rows after the other: the adapter's 16 ranks of all columns come
-// into the LDS, whatever their strides and alignment, and each wave multiplies them with its own rows.
+// n consecutive values in pieces of up to 16 bytes (whole: they are there and p is aligned to a piece), or the
+// first `count` of them one by one.
+template <int n, class Raw>
+__device__ __forceinline__ void store_some(Raw* p, const Raw (&o)[n], int count, bool whole) {
+  constexpr int kPiece = n * sizeof(Raw) < 16 ? n : 16 / sizeof(Raw);
+  if (whole) {
+#pragma unroll
+    for (int j = 0; j < n; j += kPiece)
+      __builtin_memcpy(__builtin_assume_aligned(p + j, kPiece * sizeof(Raw)), o + j, kPiece * sizeof(Raw));
+  } else {
+#pragma unroll
+    for (int j = 0; j < n; ++j)
+      if (j < count) p[j] = o[j];
+  }
+}
+
+__device__ __forceinline__ f32x4 mfma_parts(u32x4 a, u32x4 b, f32x4 c) {
+  return mfma_bf16(__builtin_bit_cast(u16x8, a), __builtin_bit_cast(u16x8, b), c);
+}
+
+// Adds h F_a^T to a tile, one adapter of its rows after the other: the adapter's ranks, 16 or 32 at a time, of
+// all columns come into the LDS, whatever their strides and alignment, and each wave multiplies them with its own rows.
 //
 // 16-bit types: depth 0 .. 15 of a product are the first parts of h, 16 .. 31 what they leave, against F_a twice
 // (f16: F_a in two parts as well, in two products).  Ranks beyond R are zero in h and read F_a's last one
 // again; columns beyond N read its last ones and are not stored.  A product is added only to the rows that are the
 // adapter's: an infinity or a NaN in one adapter is no other token's.
 template <class T, bool NN, int MB, int NB, int WM, int WN>
-__device__ __forceinline__ void expand_tile(const ProjectArgs& a, size_t t0, int n0, char* lds, f32x4 (&acc)[MB][NB]) {
+__device__ __forceinline__ void expand_tile(const ProjectArgs& a, size_t t0, int n0, char* lds0, char* lds1,
+                                            f32x4 (&acc)[MB][NB]) {
   typedef typename T::raw Raw;
   constexpr bool kF32 = __is_same(T, F32);
-  constexpr int kThreads = 64 * WM * WN, BN = 16 * NB * WN, kUnits = 2 * BN / kThreads;   // 8 ranks of a column each
-  static_assert(MB == 4 && WM <= 2 && 2 * BN % kThreads == 0, "a wave's rows are a ballot");
+  constexpr int kThreads = 64 * WM * WN, BN = 16 * NB * WN, kUnits = (2 * BN + kThreads - 1) / kThreads;   // 8 ranks of a column each
+  static_assert(MB == 4, "a wave's rows are a ballot");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 15, g = lane >> 4;
   const int wm = wave / WN, wn = 16 * NB * (wave % WN);
   int id[WM];
-  unsigned long long have[WM], any = 0;
+  unsigned long long have[WM], any = 0, have_mine = 0;
 #pragma unroll
   for (int w = 0; w < WM; ++w) {
     const size_t row = t0 + 64 * w + lane;
     id[w] = row < a.T ? a.ids[row] : -1;
     if (id[w] < 0 || id[w] >= a.G) id[w] = -1;
     any |= have[w] = __ballot(id[w] >= 0);
+    if (w == wm) have_mine = have[w];
   }
   if (!any) return;
   const bool vec = !NN && ((size_t)a.f & 15) == 0 && a.R % 8 == 0;
   const float* const h = a.h + (t0 + 64 * wm + l) * a.Rp;
-  for (int r0 = 0; r0 < a.R; r0 += 16) {
-    f32x4 hv[MB];                                                    // fp32: ranks 4 g ..
-    u16x8 ha[MB];                                                    // 16 bits: ranks 8 (g & 1) .., first parts for g < 2
+  constexpr int kB = NB == 2 ? 2 : 1;                                // blocks of ranks a wait for memory, as registers allow
+  for (int r0 = 0; r0 < a.R; r0 += 16 * kB) {
+    const int blocks = min(kB, (a.R - r0 + 15) / 16);
+    f32x4 hv[kB][MB];                                                 // fp32: ranks 4 g ..
+    u16x8 ha[kB][MB];                                                 // 16 bits: ranks 8 (g & 1) .., first parts for g < 2
 #pragma unroll
-    for (int i = 0; i < MB; ++i) {
-      float x[8] = {};
-      if (have[WM == 2 ? wm : 0] >> (16 * i + l) & 1) {
-        const float* p = h + (size_t)16 * i * a.Rp + r0 + (kF32 ? 4 * g : 8 * (g & 1));
-        for (int s = 0; s < a.planes; ++s, p += a.plane)
+    for (int b = 0; b < kB; ++b)
 #pragma unroll
-          for (int q = 0; q < (kF32 ? 4 : 8); ++q) x[q] += p[q];
+      for (int i = 0; i < MB; ++i) {
+        float x[8] = {};
+        if (b < blocks && have_mine >> (16 * i + l) & 1) {
+          const float* p = h + (size_t)16 * i * a.Rp + r0 + 16 * b + (kF32 ? 4 * g : 8 * (g & 1));
+          __builtin_memcpy(x, __builtin_assume_aligned(p, 16), 16);
+          if constexpr (!kF32) __builtin_memcpy(x + 4, __builtin_assume_aligned(p + 4, 16), 16);
+        }
+        hv[b][i] = f32x4{x[0], x[1], x[2], x[3]};
+        u16x8 hi, lo;
+        two_parts(x, hi, lo);
+        ha[b][i] = g < 2 ? hi : lo;
       }
-      hv[i] = f32x4{x[0], x[1], x[2], x[3]};
-      u16x8 hi, lo;
-      two_parts(x, hi, lo);
-      ha[i] = g < 2 ? hi : lo;
-    }
     unsigned long long left[WM];
 #pragma unroll
     for (int w = 0; w < WM; ++w) left[w] = have[w];
@@ -97,57 +122,74 @@ __device__ __forceinline__ void expand_tile(const ProjectArgs& a, size_t t0, int
         if (w == wm) mine = whose;
       }
       const Raw* const f = static_cast<const Raw*>(a.f) + (size_t)ad * a.R * a.N;
+      Raw x[kB][kUnits][8];
+#pragma unroll
+      for (int b = 0; b < kB; ++b)
+        if (b < blocks)
+#pragma unroll
+          for (int u = 0; u < kUnits; ++u) {
+            const int at = u * kThreads + threadIdx.x, r = r0 + 16 * b + at / BN * 8;
+            if (at >= 2 * BN) continue;
+            const Raw* const p = f + (size_t)min(n0 + at % BN, a.N - 1) * a.fn;
+            if (vec) {
+              const u32x4* const q = reinterpret_cast<const u32x4*>(p + min(r, a.R - 8));
+              __builtin_memcpy(x[b][u], q, 16);
+              if constexpr (kF32) __builtin_memcpy(x[b][u] + 4, q + 1, 16);
+            } else {
+#pragma unroll
+              for (int q = 0; q < 8; ++q) x[b][u][q] = p[(size_t)min(r + q, a.R - 1) * a.fr];
+            }
+          }
       __syncthreads();                                               // (nobody reads what was there)
 #pragma unroll
-      for (int u = 0; u < kUnits; ++u) {
-        const int at = u * kThreads + threadIdx.x, col = at % BN, half = at / BN, r = r0 + 8 * half;
-        const Raw* const p = f + (size_t)min(n0 + col, a.N - 1) * a.fn;
-        Raw x[8];
-        if (vec) {
-          const u32x4* const q = reinterpret_cast<const u32x4*>(p + min(r, a.R - 8));
-          __builtin_memcpy(x, q, 16);
-          if constexpr (kF32) __builtin_memcpy(x + 4, q + 1, 16);
-        } else {
+      for (int b = 0; b < kB; ++b)
+        if (b < blocks)
 #pragma unroll
-          for (int q = 0; q < 8; ++q) x[q] = p[(size_t)min(r + q, a.R - 1) * a.fr];
-        }
-        const int in = col % (16 * NB), slot = col - in + 16 * (in % NB) + in / NB;      // block j's columns side by side
-        if constexpr (kF32) {
-          __builtin_memcpy(__builtin_assume_aligned(lds + slot * 64 + half * 32, 16), x, 32);
-        } else if constexpr (__is_same(T, F16)) {
-          float y[8];
+          for (int u = 0; u < kUnits; ++u) {
+            const int at = u * kThreads + threadIdx.x, col = at % BN, half = at / BN;
+            if (at >= 2 * BN) continue;
+            const int in = col % (16 * NB), slot = col - in + 16 * (in % NB) + in / NB;    // block j's columns side by side
+            char* const to = b ? lds1 : lds0;
+            if constexpr (kF32) {
+              __builtin_memcpy(__builtin_assume_aligned(to + slot * 64 + half * 32, 16), x[b][u], 32);
+            } else if constexpr (__is_same(T, F16)) {
+              float y[8];
 #pragma unroll
-          for (int q = 0; q < 8; ++q) y[q] = F16::widen(x[q]);
-          u16x8 hi, lo;
-          two_parts(y, hi, lo);
-          *reinterpret_cast<u16x8*>(lds + slot * 64 + half * 16) = hi;
-          *reinterpret_cast<u16x8*>(lds + slot * 64 + 32 + half * 16) = lo;
-        } else {
-          __builtin_memcpy(__builtin_assume_aligned(lds + slot * 32 + half * 16, 16), x, 16);
-        }
-      }
+              for (int q = 0; q < 8; ++q) y[q] = F16::widen(x[b][u][q]);
+              u16x8 hi, lo;
+              two_parts(y, hi, lo);
+              *reinterpret_cast<u16x8*>(to + slot * 64 + half * 16) = hi;
+              *reinterpret_cast<u16x8*>(to + slot * 64 + 32 + half * 16) = lo;
+            } else {
+              __builtin_memcpy(__builtin_assume_aligned(to + slot * 32 + half * 16, 16), x[b][u], 16);
+            }
+          }
       __syncthreads();
       if (!mine) continue;
 #pragma unroll
-      for (int j = 0; j < NB; ++j) {
-        const char* const at = lds + (wn + 16 * j + l) * (__is_same(T, BF16) ? 32 : 64);
-        f32x4 fv = {};
-        u16x8 fh = {}, fl = {};
-        if constexpr (kF32) fv = *reinterpret_cast<const f32x4*>(at + g * 16);
-        else fh = *reinterpret_cast<const u16x8*>(at + (g & 1) * 16);
-        if constexpr (__is_same(T, F16)) fl = *reinterpret_cast<const u16x8*>(at + 32 + (g & 1) * 16);
+      for (int b = 0; b < kB; ++b) {
+        if (b >= blocks) continue;
 #pragma unroll
-        for (int i = 0; i < MB; ++i) {
-          f32x4 d = {};
-          if constexpr (kF32) {
+        for (int j = 0; j < NB; ++j) {
+          const char* const at = (b ? lds1 : lds0) + (wn + 16 * j + l) * (__is_same(T, BF16) ? 32 : 64);
+          f32x4 fv = {};
+          u16x8 fh = {}, fl = {};
+          if constexpr (kF32) fv = *reinterpret_cast<const f32x4*>(at + g * 16);
+          else fh = *reinterpret_cast<const u16x8*>(at + (g & 1) * 16);
+          if constexpr (__is_same(T, F16)) fl = *reinterpret_cast<const u16x8*>(at + 32 + (g & 1) * 16);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) d = mfma_f32(hv[i][q], fv[q], d);
-          } else {
-            if constexpr (__is_same(T, F16)) d = mfma_bf16(ha[i], fl, d);
-            d = mfma_bf16(ha[i], fh, d);
+          for (int i = 0; i < MB; ++i) {
+            f32x4 d = {};
+            if constexpr (kF32) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) d = mfma_f32(hv[b][i][q], fv[q], d);
+            } else {
+              if constexpr (__is_same(T, F16)) d = mfma_bf16(ha[b][i], fl, d);
+              d = mfma_bf16(ha[b][i], fh, d);
+            }
+#pragma unroll
+            for (int v = 0; v < 4; ++v) acc[i][j][v] += mine >> (16 * i + 4 * g + v) & 1 ? d[v] : 0.0f;
           }
-#pragma unroll
-          for (int v = 0; v < 4; ++v) acc[i][j][v] += mine >> (16 * i + 4 * g + v) & 1 ? d[v] : 0.0f;
         }
       }
     }
@@ -162,14 +204,15 @@ struct TileArgs {
 };
 
 // One wave of a tile: MB x NB blocks of 16 x 16.
-template <class T, bool NN, int MB, int NB, int WM, int WN>
+template <class T, bool NN, int MB, int NB, int WM, int WN, int RB>
 __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta) {
   typedef typename T::raw Raw;
-  constexpr int kThreads = 64 * WM * WN, BM = 16 * MB * WM, BN = 16 * NB * WN, KS = kStep<T>;
-  constexpr int kZ = BM * 4 / kThreads, kW = BN * 4 / kThreads;      // 16-byte loads of a thread and step
-  static_assert(BM * 4 % kThreads == 0 && BN * 4 % kThreads == 0, "whole loads");
+  constexpr int kThreads = 64 * WM * WN, BM = 16 * MB * WM, BN = 16 * NB * WN, KS = RB / (int)sizeof(Raw);
+  constexpr int RC = RB / 16, kRooms = RB == 128 ? 2 : 3;            // a row's bytes of a step: 16-byte pieces
+  constexpr int kZ = BM * RC / kThreads, kW = BN * RC / kThreads;    // 16-byte loads of a thread and step
+  static_assert(BM * RC % kThreads == 0 && BN * RC % kThreads == 0, "whole loads");
   // (three variables, so that the compiler knows a load into one from a read of another)
-  __shared__ __attribute__((aligned(1024))) char lds0[(BM + BN) * 64], lds1[(BM + BN) * 64], lds2[(BM + BN) * 64];
+  __shared__ __attribute__((aligned(1024))) char lds0[(BM + BN) * RB], lds1[(BM + BN) * RB], lds2[kRooms == 3 ? (BM + BN) * RB : 16];
   const ProjectArgs& a = ta.p;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 15, g = lane >> 4;
   // the place of this workgroup: each die a contiguous run of tiles, up to eight columns of tiles wide
@@ -187,13 +230,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
   const char* zb = reinterpret_cast<const char*>(static_cast<const Raw*>(a.z) + t0 * a.ldz + k_first);
   const char* wb = reinterpret_cast<const char*>(static_cast<const Raw*>(a.w) +
                                                  (NN ? (size_t)k_first * a.ldw + n0 : (size_t)n0 * a.ldw + k_first));
-  const size_t w_next = NN ? (size_t)KS * a.ldw * sizeof(Raw) : 64;
+  const size_t w_next = NN ? (size_t)KS * a.ldw * sizeof(Raw) : RB;
+  // (a row's pieces in another order in each row, so that a column of them lies in all banks)
+  auto piece = [](int slot, int row) __attribute__((always_inline)) { return RC == 4 ? slot ^ (row >> 1 & 3) : slot ^ (row & 7); };
   // What each thread brings: the LDS is filled in the threads' order; which 16 bytes come there is theirs to choose.
   // Rows beyond the operand's are read again from its last one: what they give is not stored.
   unsigned zo[kZ], wo[kW];
 #pragma unroll
   for (int i = 0; i < kZ; ++i) {
-    const int at = i * kThreads + threadIdx.x, row = at >> 2, chunk = (at & 3) ^ (row >> 1 & 3);
+    const int at = i * kThreads + threadIdx.x, row = at / RC, chunk = piece(at % RC, row);
     zo[i] = (unsigned)(min(row, rows - 1) * a.ldz * sizeof(Raw)) + chunk * 16;
   }
 #pragma unroll
@@ -203,13 +248,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
       constexpr int kRow = BN / kVec<T>;                             // 16-byte pieces of a row
       wo[i] = (unsigned)(at / kRow * a.ldw * sizeof(Raw)) + min(at % kRow, (cols - 1) / kVec<T>) * 16;
     } else {
-      const int slot = at >> 2, chunk = (at & 3) ^ (slot >> 1 & 3), in = slot % (16 * NB);
+      const int slot = at / RC, chunk = piece(at % RC, slot), in = slot % (16 * NB);
       const int col = slot - in + NB * (in & 15) + in / 16;
       wo[i] = (unsigned)(min(col, cols - 1) * a.ldw * sizeof(Raw)) + chunk * 16;
     }
   }
   int brought = 0;
-  auto bring = [&](char* lds) {
+  auto bring = [&](char* lds) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < kZ; ++i)
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(zb + zo[i]),
@@ -217,79 +262,97 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
 #pragma unroll
     for (int i = 0; i < kW; ++i)
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(wb + wo[i]),
-                                       (__attribute__((address_space(3))) void*)(lds + BM * 64 + (i * kThreads + wave * 64) * 16), 16, 0, 0);
+                                       (__attribute__((address_space(3))) void*)(lds + BM * RB + (i * kThreads + wave * 64) * 16), 16, 0, 0);
     const bool more = ++brought < steps;                             // (beyond the last step that one again)
-    zb += more ? 64 : 0;
+    zb += more ? RB : 0;
     wb += more ? w_next : 0;
   };
 
   f32x4 acc[MB][NB] = {};
-  const int z_at = (wm + l) * 64 + ((g ^ (l >> 1 & 3)) * 16), w_at = BM * 64 + (NN ? 0 : (wn + l) * 64 + ((g ^ (l >> 1 & 3)) * 16));
-  auto multiply = [&](const char* lds) {
+  // (16-bit: piece g of a row; fp32: pieces 2 g and 2 g + 1)
+  const int z_at = (wm + l) * RB, w_at = BM * RB + (NN ? 0 : (wn + l) * RB);
+  auto multiply = [&](const char* lds) __attribute__((always_inline)) {
     if constexpr (__is_same(T, F32)) {
-      f32x4 zf[MB];
+      // fp32 values as three bfloat16 parts, a product as the six largest partial products
+      const int p0 = piece(2 * g, l) * 16, p1 = piece(2 * g + 1, l) * 16;
+      u32x4 zh[MB], zm[MB], zl[MB];
 #pragma unroll
-      for (int i = 0; i < MB; ++i) zf[i] = *reinterpret_cast<const f32x4*>(lds + z_at + i * 1024);
-      float wf[4][NB];
+      for (int i = 0; i < MB; ++i) {
+        float x[8];
+        __builtin_memcpy(x, __builtin_assume_aligned(lds + z_at + i * 16 * RB + p0, 16), 16);
+        __builtin_memcpy(x + 4, __builtin_assume_aligned(lds + z_at + i * 16 * RB + p1, 16), 16);
+        split::split8(x, zh[i], zm[i], zl[i]);
+      }
+      typedef float Row __attribute__((ext_vector_type(NB)));
+      Row in[8];
       if constexpr (NN) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-          for (int j = 0; j < NB; j += 4) {
-            const f32x4 x = *reinterpret_cast<const f32x4*>(lds + w_at + ((4 * g + q) * BN + wn + NB * l + j) * 4);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) wf[q][j + e] = x[e];
-          }
-      } else {
-#pragma unroll
-        for (int j = 0; j < NB; ++j) {
-          const f32x4 x = *reinterpret_cast<const f32x4*>(lds + w_at + j * 1024);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) wf[q][j] = x[q];
-        }
+        for (int q = 0; q < 8; ++q) in[q] = *reinterpret_cast<const Row*>(lds + w_at + ((8 * g + q) * BN + wn + NB * l) * 4);
       }
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
+      for (int j = 0; j < NB; ++j) {
+        float x[8];
+        if constexpr (NN) {
+#pragma unroll
+          for (int q = 0; q < 8; ++q) x[q] = in[q][j];
+        } else {
+          __builtin_memcpy(x, __builtin_assume_aligned(lds + w_at + j * 16 * RB + p0, 16), 16);
+          __builtin_memcpy(x + 4, __builtin_assume_aligned(lds + w_at + j * 16 * RB + p1, 16), 16);
+        }
+        u32x4 wh, wmid, wl;
+        split::split8(x, wh, wmid, wl);
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+          acc[i][j] = mfma_parts(zl[i], wh, acc[i][j]);
+          acc[i][j] = mfma_parts(zm[i], wmid, acc[i][j]);
+          acc[i][j] = mfma_parts(zh[i], wl, acc[i][j]);
+          acc[i][j] = mfma_parts(zm[i], wh, acc[i][j]);
+          acc[i][j] = mfma_parts(zh[i], wmid, acc[i][j]);
+          acc[i][j] = mfma_parts(zh[i], wh, acc[i][j]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int kk = 0; kk < RB / 64; ++kk) {
+        const int at = piece(4 * kk + g, l) * 16;
+        u16x8 zf[MB], wf[NB];
+#pragma unroll
+        for (int i = 0; i < MB; ++i) zf[i] = *reinterpret_cast<const u16x8*>(lds + z_at + at + i * 16 * RB);
+        if constexpr (NN) {
+          unsigned in[8][NB / 2];
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const char* const p = lds + w_at + ((32 * kk + 8 * g + q) * BN + wn + NB * l) * 2;
+            if constexpr (NB == 2) {
+              in[q][0] = *reinterpret_cast<const unsigned*>(p);
+            } else if constexpr (NB == 8) {
+              const u32x4 x = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) in[q][e] = x[e];
+            } else {
+              const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+              in[q][0] = x[0];
+              in[q][1] = x[1];
+            }
+          }
+          turn<NB>(in, wf);
+        } else {
+#pragma unroll
+          for (int j = 0; j < NB; ++j) wf[j] = *reinterpret_cast<const u16x8*>(lds + w_at + at + j * 16 * RB);
+        }
 #pragma unroll
         for (int j = 0; j < NB; ++j)
 #pragma unroll
-          for (int i = 0; i < MB; ++i) acc[i][j] = mfma_f32(zf[i][q], wf[q][j], acc[i][j]);
-    } else {
-      u16x8 zf[MB], wf[NB];
-#pragma unroll
-      for (int i = 0; i < MB; ++i) zf[i] = *reinterpret_cast<const u16x8*>(lds + z_at + i * 1024);
-      if constexpr (NN) {
-        unsigned in[8][NB / 2];
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const char* const p = lds + w_at + ((8 * g + q) * BN + wn + NB * l) * 2;
-          if constexpr (NB == 8) {
-            const u32x4 x = *reinterpret_cast<const u32x4*>(p);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) in[q][e] = x[e];
-          } else {
-            const u32x2 x = *reinterpret_cast<const u32x2*>(p);
-            in[q][0] = x[0];
-            in[q][1] = x[1];
-          }
-        }
-        turn<NB>(in, wf);
-      } else {
-#pragma unroll
-        for (int j = 0; j < NB; ++j) wf[j] = *reinterpret_cast<const u16x8*>(lds + w_at + j * 1024);
+          for (int i = 0; i < MB; ++i) acc[i][j] = mfma_16<T>(zf[i], wf[j], acc[i][j]);
       }
-#pragma unroll
-      for (int j = 0; j < NB; ++j)
-#pragma unroll
-        for (int i = 0; i < MB; ++i) acc[i][j] = mfma_16<T>(zf[i], wf[j], acc[i][j]);
     }
   };
-  // A step: its own loads have arrived (those of the next one may still be on their way), and nobody reads the
-  // last one's room any more.  Every step brings one, so that no branch keeps the compiler from
-  // counting the loads under way.
-  auto step = [&](const char* lds, char* into) {
+  // A step: its own loads have arrived (with three rooms those of the next one may still be on their way), and
+  // nobody reads the last one's room any more.  Every step brings one, so that no branch keeps the compiler
+  // from counting the loads under way.
+  auto step = [&](const char* lds, char* into) __attribute__((always_inline)) {
     asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(wait_for(kZ + kW));
+    __builtin_amdgcn_s_waitcnt(wait_for(kRooms == 3 ? kZ + kW : 0));
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
@@ -299,17 +362,25 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
   };
   if (steps > 0) {
     bring(lds0);
-    asm volatile("" ::: "memory");                                   // (their order is what the waits count on)
-    __builtin_amdgcn_sched_barrier(0);
-    bring(lds1);
     int left = steps;                                                // (no way out in the middle: the same reason)
-    for (; left >= 3; left -= 3) {
-      step(lds0, lds2);
-      step(lds1, lds0);
-      step(lds2, lds1);
+    if constexpr (kRooms == 3) {
+      asm volatile("" ::: "memory");                                 // (their order is what the waits count on)
+      __builtin_amdgcn_sched_barrier(0);
+      bring(lds1);
+      for (; left >= 3; left -= 3) {
+        step(lds0, lds2);
+        step(lds1, lds0);
+        step(lds2, lds1);
+      }
+      if (left > 0) step(lds0, lds2);
+      if (left > 1) step(lds1, lds0);
+    } else {
+      for (; left >= 2; left -= 2) {
+        step(lds0, lds1);
+        step(lds1, lds0);
+      }
+      if (left > 0) step(lds0, lds1);
     }
-    if (left > 0) step(lds0, lds2);
-    if (left > 1) step(lds1, lds0);
     __builtin_amdgcn_s_waitcnt(wait_for(0));                         // (the loads beyond the last step)
   }
   if (k_first + steps * KS < k_last) {
@@ -321,7 +392,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kZ; ++i) {
-      const int at = i * kThreads + threadIdx.x, chunk = (at & 3) ^ (at >> 3 & 3);
+      const int at = i * kThreads + threadIdx.x, chunk = piece(at % RC, at / RC);
       u32x4 x = {};
       if (chunk * kVec<T> < left) {
         if constexpr (NN) {                                          // (z's row may end inside the 16 bytes)
@@ -337,21 +408,21 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
 #pragma unroll
     for (int i = 0; i < kW; ++i) {
       const int at = i * kThreads + threadIdx.x;
-      const int depth = NN ? at / (BN / kVec<T>) : ((at & 3) ^ (at >> 3 & 3)) * kVec<T>;
+      const int depth = NN ? at / (BN / kVec<T>) : piece(at % RC, at / RC) * kVec<T>;
       u32x4 x = {};
       if (depth < left) x = *reinterpret_cast<const u32x4*>(wb + wo[i]);
-      *reinterpret_cast<u32x4*>(lds0 + BM * 64 + at * 16) = x;
+      *reinterpret_cast<u32x4*>(lds0 + BM * RB + at * 16) = x;
     }
     __syncthreads();
     multiply(lds0);
   }
 
-  if (split == 0) expand_tile<T, NN, MB, NB, WM, WN>(a, t0, n0, lds0, acc);
+  if (split == 0) expand_tile<T, NN, MB, NB, WM, WN>(a, t0, n0, lds0, lds1, acc);
   const int n = n0 + wn + NB * l;
   if (n >= a.N) return;
   if (ta.part) {
     float* const y = ta.part + ((size_t)split * a.T + t0 + wm) * a.N + n;
-    const bool whole = n + NB <= a.N && a.N % 4 == 0;
+    const bool whole = n + NB <= a.N && a.N % (NB < 4 ? NB : 4) == 0;
 #pragma unroll
     for (int i = 0; i < MB; ++i)
 #pragma unroll
@@ -359,15 +430,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
         const int row = 16 * i + 4 * g + v;
         if (t0 + wm + row >= a.T) continue;
         float* const p = y + (size_t)row * a.N;
-        if (whole) {
+        float o[NB];
 #pragma unroll
-          for (int j = 0; j < NB; j += 4)
-            *reinterpret_cast<f32x4*>(p + j) = f32x4{acc[i][j][v], acc[i][j + 1][v], acc[i][j + 2][v], acc[i][j + 3][v]};
-        } else {
-#pragma unroll
-          for (int j = 0; j < NB; ++j)
-            if (n + j < a.N) p[j] = acc[i][j][v];
-        }
+        for (int j = 0; j < NB; ++j) o[j] = acc[i][j][v];
+        store_some(p, o, a.N - n, whole);
       }
     return;
   }
@@ -375,35 +441,18 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
 #pragma unroll
   for (int j = 0; j < NB; ++j) bias[j] = a.bias && n + j < a.N ? a.bias[n + j] : 0.0f;
   Raw* const y = static_cast<Raw*>(a.y) + (t0 + wm) * a.N + n;
-  const bool whole = n + NB <= a.N && a.N * sizeof(Raw) % (NB == 4 && sizeof(Raw) == 2 ? 8 : 16) == 0 && ((size_t)a.y & 15) == 0;
+  constexpr size_t kPiece = NB * sizeof(Raw) < 16 ? NB * sizeof(Raw) : 16;
+  const bool whole = n + NB <= a.N && a.N * sizeof(Raw) % kPiece == 0 && ((size_t)a.y & 15) == 0;
 #pragma unroll
   for (int i = 0; i < MB; ++i)
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
       const int row = 16 * i + 4 * g + v;
       if (t0 + wm + row >= a.T) continue;
-      Raw* const p = y + (size_t)row * a.N;
       Raw o[NB];
 #pragma unroll
       for (int j = 0; j < NB; ++j) o[j] = T::narrow(acc[i][j][v] + bias[j]);
-      if (whole) {
-        if constexpr (sizeof(o) == 8) {
-          u32x2 d;
-          __builtin_memcpy(&d, o, 8);
-          *reinterpret_cast<u32x2*>(p) = d;
-        } else {
-#pragma unroll
-          for (int j = 0; j < NB; j += kVec<T>) {
-            u32x4 d;
-            __builtin_memcpy(&d, o + j, 16);
-            *reinterpret_cast<u32x4*>(p + j) = d;
-          }
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < NB; ++j)
-          if (n + j < a.N) p[j] = o[j];
-      }
+      store_some(y + (size_t)row * a.N, o, a.N - n, whole);
     }
 }
 
@@ -433,42 +482,52 @@ __global__ __launch_bounds__(256) void join_kernel(const float* part, const floa
   }
 }
 
-template <class T, bool NN, int MB, int NB, int WM, int WN>
-void launch(TileArgs t, hipStream_t st) {
-  tile_kernel<T, NN, MB, NB, WM, WN><<<die_grid((long)t.mt * t.nt * t.splits), 64 * WM * WN, 0, st>>>(t);
+template <class T, bool NN, int MB, int NB, int WM, int WN, int RB>
+void launch(const TileArgs& t, hipStream_t st) {
+  tile_kernel<T, NN, MB, NB, WM, WN, RB><<<die_grid((long)t.mt * t.nt * t.splits), 64 * WM * WN, 0, st>>>(t);
 }
+// (fp32: its parts take the registers of 128 columns a wave)
 template <class T, bool NN>
 void launch_shape(const TileArgs& t, int which, hipStream_t st) {
-  if (which == 0) launch<T, NN, 4, 8, 2, 2>(t, st);
-  else if (which == 1) launch<T, NN, 4, 4, 2, 2>(t, st);
-  else launch<T, NN, 4, 4, 1, 4>(t, st);
+  if constexpr (__is_same(T, F32)) {
+    if (which == 1) launch<T, NN, 4, 2, 2, 4, 128>(t, st);
+    else launch<T, NN, 4, 4, 1, 4, 128>(t, st);
+  } else {
+    if (which == 0) launch<T, NN, 4, 8, 2, 2, 64>(t, st);
+    else if (which == 1) launch<T, NN, 4, 2, 2, 4, 64>(t, st);
+    else if (which == 2) launch<T, NN, 4, 4, 1, 4, 64>(t, st);
+    else launch<T, NN, 4, 8, 4, 2, 128>(t, st);
+  }
 }
 
-constexpr int kRows[3] = {128, 128, 64}, kCols[3] = {256, 128, 256};
+constexpr int kShapes = 4, kRows[kShapes] = {128, 128, 64, 256}, kCols[kShapes] = {256, 128, 256, 256};
 
 }  // namespace
 
 TilePlan tile_plan(size_t T, int K, int N, int dtype) {
-  const int KS = dtype == CP4_DTYPE_F32 ? 16 : 32;
   const long units = num_compute_units();
-  const int steps = (K + KS - 1) / KS;
+  const bool f32 = dtype == CP4_DTYPE_F32;
   TilePlan best{};
   double least = 0;
-  for (int w = 0; w < 3; ++w) {
+  static const char* force = getenv("WHICH");
+  for (int w = f32 ? 1 : 0; w < (f32 ? 3 : kShapes); ++w) {
+    if (force && w != atoi(force)) continue;
+    const int KS = w == 3 ? 64 : 32, steps = (K + KS - 1) / KS;
     const long tiles = (long)((T + kRows[w] - 1) / kRows[w]) * ((N + kCols[w] - 1) / kCols[w]);
     for (int s = 1; s <= 64 && s <= std::max(1, steps / 4); s *= 2) {
       const int each = (steps + s - 1) / s;
       const long wgs = tiles * ((steps + each - 1) / each);
       // microseconds: a compute unit's tiles one after the other at its share of the matrix cores' rate (a
       // workgroup alone reaches less of it), their starts and ends, the parts' way to memory and back
-      const double flops = 2.0 * kRows[w] * kCols[w] * KS * each, rate = (dtype == CP4_DTYPE_F32 ? 0.5e6 : w == 0 ? 5.0e6 : 3.6e6);
+      const double flops = 2.0 * kRows[w] * kCols[w] * KS * each, rate = f32 ? 1.2e6 : w == 0 ? 4.6e6 : w == 3 ? 5.5e6 : 3.6e6;
       const long most = (wgs + units - 1) / units;
-      double cost = most * flops / (most == 1 ? 0.7 * rate : rate) + 2.0 + most;
+      double cost = most * flops / (most == 1 && w != 3 ? 0.7 * rate : rate) + 2.0 + most;
       if (s > 1) cost += 4.0 + (double)T * N * (s + 0.5) * 4.0 / 2.0e6;
       if (!best.splits || cost < least) {
         least = cost;
         best.which = w;
         best.each = each;
+        best.cost = cost;
         best.splits = (steps + each - 1) / each;
       }
     }
