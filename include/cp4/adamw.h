@@ -56,7 +56,7 @@ typedef struct cp4_adamw_group {
  * grad_scale: what all gradients are multiplied by (1: as they are).  With max_norm > 0 the norm of
  * all gradients of the call is written to *norm (device memory; may be NULL), and a step whose norm
  * is infinite or NaN changes nothing, the counters included.  Asynchronous on `stream`: one launch
- * for up to 48 tensors of the same group and types; with max_norm, one more before them for up to 192
+ * for up to 75 (8-bit moments: 57) tensors of the same group and types; with max_norm, one more before them for up to 192
  * of the same gradient type.  `workspace`: cp4_adamw_workspace_bytes() of device memory, 16-byte
  * aligned; with max_norm == 0 it may be NULL.  Tensors must not overlap one another. */
 size_t cp4_adamw_workspace_bytes(void);

@@ -10,6 +10,7 @@
 // the kernel's arguments: no copy to the device that a captured graph would have to repeat.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 #include <vector>
 
 #include "cp4/adamw.h"
@@ -28,33 +29,37 @@ using cp4::F32;
 constexpr int kBlock = 256;                        // values that share a scale
 constexpr int kUnroll = 4;                         // blocks that a wave loads at once
 constexpr size_t kChunk = kBlock * kUnroll;        // values of a wave's turn
-constexpr int kTensors = 48;                       // of a launch: kernel arguments below 4 KB
-constexpr int kNormTensors = 192;
+constexpr int kTensors32 = 75, kTensors8 = 57;     // of a launch: kernel arguments below 4 KB
+constexpr int kNormTensors = 192, kMomentTensors = 57;
 constexpr unsigned kWaves = 4;                     // of a workgroup
 constexpr unsigned kMostParts = 16384;             // partial sums of the norm
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
-struct Item {
+struct Item32 {
   void* p;
   const void* g;
-  void *m, *v;
-  float *s, *s2;
-  void* copy;
+  void *m, *v, *copy;
   size_t n;
 };
+struct Item8 : Item32 {
+  float *s, *s2;
+};
+template <bool Eight>
 struct StepArgs {
+  typedef std::conditional_t<Eight, Item8, Item32> Item;
+  static constexpr int kTensors = Eight ? kTensors8 : kTensors32;
   Item item[kTensors];
   unsigned first[kTensors];                        // each tensor's first chunk
-  unsigned chunks, blocks;                         // blocks: of all the step's launches
+  unsigned chunks, blocks;                         // blocks: of all the group's launches
   int count, copy_dtype;
   double* counter;
   const float* coefficient;                        // {factor of the gradients, 1: go on}; null: `scale`
   double lr, beta1, beta2;
   float b1, c1, b2, c2, decay, eps, scale;
 };
-static_assert(sizeof(StepArgs) <= 4096, "kernel arguments");
+static_assert(sizeof(StepArgs<false>) <= 4096 && sizeof(StepArgs<true>) <= 4096, "kernel arguments");
 struct NormArgs {
   const void* g[kNormTensors];
   unsigned first[kNormTensors];
@@ -103,11 +108,20 @@ __device__ __forceinline__ bool aligned_four(const Raw* p) {
 
 // ---- 8-bit moments ------------------------------------------------------------------------
 
-// The largest of the wave's values; as bits, so that infinities and NaN come out on top.
+// The largest of the wave's values; as bits, so that infinities and NaN come out on top.  (Shifts within rows of 16
+// lanes and from row to row; lanes that nothing is shifted into take 0.)
+template <int kControl, int kRows>
+__device__ __forceinline__ unsigned max_from(unsigned x) {
+  return max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, kControl, kRows, 0xf, false));
+}
 __device__ __forceinline__ unsigned wave_max(unsigned x) {
-#pragma unroll
-  for (int s = 32; s; s >>= 1) x = max(x, (unsigned)__shfl_xor((int)x, s));
-  return x;
+  x = max_from<0x111, 0xf>(x);
+  x = max_from<0x112, 0xf>(x);
+  x = max_from<0x114, 0xf>(x);
+  x = max_from<0x118, 0xf>(x);
+  x = max_from<0x142, 0xa>(x);
+  x = max_from<0x143, 0xc>(x);
+  return (unsigned)__builtin_amdgcn_readlane((int)x, 63);
 }
 constexpr float kUnitM = (float)(1.0 / (127.0 * 127.0));
 constexpr float kUnitV = (float)(1.0 / (255.0 * 255.0 * 255.0 * 255.0));
@@ -127,16 +141,12 @@ __device__ __forceinline__ float scale_of(unsigned top, float* over) {
   *over = 1.0f / __uint_as_float(top);
   return __uint_as_float(top);
 }
-__device__ __forceinline__ signed char code_m(float m, float over) {
-  const int q = (int)rintf(sqrtf(fabsf(m) * over) * 127.0f);
-  return (signed char)(m < 0.0f ? -q : q);
-}
-__device__ __forceinline__ unsigned char code_v(float v, float over) {
-  const int q = (int)rintf(sqrtf(sqrtf(v * over)) * 255.0f);
-  return (unsigned char)(q < 1 && v > 0.0f && over > 0.0f ? 1 : q);
-}
+__device__ __forceinline__ int signed_code(int q, float m) { return m < 0.0f ? -q : q; }
 
-// Codes and scales of one block of 256 values: four a lane, those beyond the tensor zero.
+// Codes and scales of one block of 256 values: four a lane, those beyond the tensor zero.  A code is defined by
+// correctly rounded roots; the hardware's, a unit in the last place off, give the same one but near the middle of
+// two codes, where the few blocks that have such a value take the long way (12 instructions a root
+// less for the others: 134 M values 720 us with the long way alone).
 __device__ __forceinline__ void encode_block(const float (&m)[4], const float (&v)[4], Four<signed char>& qm,
                                              Four<unsigned char>& qv, float& sm, float& sv) {
   unsigned tm = 0, tv = 0;
@@ -148,11 +158,27 @@ __device__ __forceinline__ void encode_block(const float (&m)[4], const float (&
   float om, ov;
   sm = scale_of(wave_max(tm), &om);
   sv = scale_of(wave_max(tv), &ov);
+  bool near = false;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    qm.v[j] = code_m(m[j], om);
-    qv.v[j] = code_v(v[j], ov);
+    // off by some 2 units in the last place of 127, by 3 of 255
+    const float a = __builtin_amdgcn_sqrtf(fabsf(m[j]) * om) * 127.0f;
+    const float b = __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(v[j] * ov)) * 255.0f;
+    const float ra = rintf(a), rb = rintf(b);
+    near = near || !(fabsf(a - ra) < 0.5f - 6e-5f) || !(fabsf(b - rb) < 0.5f - 2e-4f);
+    qm.v[j] = (signed char)signed_code((int)ra, m[j]);
+    qv.v[j] = (unsigned char)(int)rb;
   }
+  if (__builtin_expect(__any(near), 0)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      qm.v[j] = (signed char)signed_code((int)rintf(sqrtf(fabsf(m[j]) * om) * 127.0f), m[j]);
+      qv.v[j] = (unsigned char)(int)rintf(sqrtf(sqrtf(v[j] * ov)) * 255.0f);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (qv.v[j] == 0 && v[j] > 0.0f && ov > 0.0f) qv.v[j] = 1;
 }
 
 // ---- which tensor ---------------------------------------------------------------------------
@@ -172,7 +198,7 @@ __device__ __forceinline__ int tensor_of(const Args& a, unsigned chunk) {
 // ---- the step ---------------------------------------------------------------------------------
 
 template <class P, class G, bool Eight>
-__global__ __launch_bounds__(64 * kWaves, 4) void step_kernel(const StepArgs a) {
+__global__ __launch_bounds__(64 * kWaves, 4) void step_kernel(const StepArgs<Eight> a) {
   typedef typename P::raw RawP;
   typedef typename G::raw RawG;
   const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -185,7 +211,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void step_kernel(const StepArgs a) 
     const float rate = (float)(a.lr / (1.0 - power1)), root = (float)(1.0 / sqrt(1.0 - power2));
     for (unsigned c = blockIdx.x * kWaves + wave; c < a.chunks; c += gridDim.x * kWaves) {
       const int t = tensor_of(a, c);
-      const Item& it = a.item[t];
+      const auto& it = a.item[t];
       const size_t n = it.n, at0 = (size_t)(c - a.first[t]) * kChunk;
       RawP* const p = static_cast<RawP*>(it.p);
       const RawG* const g = static_cast<const RawG*>(it.g);
@@ -337,15 +363,16 @@ __global__ __launch_bounds__(64 * kWaves, 4) void norm_kernel(const NormArgs a) 
   }
   sum = block_sum(sum, lds);
   if (threadIdx.x == 0) {
-    a.partial[a.part + blockIdx.x] = sum;
-    __threadfence();
+    // (what the workgroups hand over goes past their dies' caches: no write-back of everything else there)
+    __hip_atomic_store(a.partial + a.part + blockIdx.x, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+    __builtin_amdgcn_s_waitcnt(0);                                   // (it has arrived)
     unsigned* const ticket = reinterpret_cast<unsigned*>(a.counter + 3) + 1;
-    last = atomicAdd(ticket, 1u) + 1 == a.blocks;
+    last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == a.blocks;
     if (last) *ticket = 0;
   }
   __syncthreads();
   if (!last) return;
-  __threadfence();
   sum = 0.0;
   for (unsigned i = threadIdx.x; i < a.parts; i += 64 * kWaves)
     sum += __hip_atomic_load(a.partial + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -368,8 +395,8 @@ struct MomentItem {
   size_t n;
 };
 struct MomentArgs {
-  MomentItem item[kTensors];
-  unsigned first[kTensors];
+  MomentItem item[kMomentTensors];
+  unsigned first[kMomentTensors];
   unsigned chunks;
   int count;
 };
@@ -385,34 +412,45 @@ __global__ __launch_bounds__(64 * kWaves, 4) void moments_kernel(const MomentArg
     const bool even = (((size_t)it.m | (size_t)it.v) & 3) == 0 && (((size_t)it.to_m | (size_t)it.to_v) & 15) == 0;
     signed char* const m8 = static_cast<signed char*>(it.m);
     unsigned char* const v8 = static_cast<unsigned char*>(it.v);
+    Four<signed char> qm[kUnroll];
+    Four<unsigned char> qv[kUnroll];
+    Four<float> fm[kUnroll], fv[kUnroll];
+    float um[kUnroll], uv[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const size_t at = at0 + u * kBlock + lane * 4, b = at0 / kBlock + u;
       const bool whole = even && at + 4 <= n, there = at0 + u * kBlock < n;
-      Four<signed char> qm;
-      Four<unsigned char> qv;
       if constexpr (Encode) {
-        const Four<float> fm = load_four(it.to_m, at, n, whole), fv = load_four(it.to_v, at, n, whole);
+        fm[u] = load_four(it.to_m, at, n, whole);
+        fv[u] = load_four(it.to_v, at, n, whole);
+      } else {
+        qm[u] = load_four(m8, at, n, whole);
+        qv[u] = load_four(v8, at, n, whole);
+        um[u] = there ? it.s[b] * kUnitM : 0.0f;
+        uv[u] = there ? it.s2[b] * kUnitV : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const size_t at = at0 + u * kBlock + lane * 4, b = at0 / kBlock + u;
+      const bool whole = even && at + 4 <= n;
+      if constexpr (Encode) {
         float tm, tv;
-        encode_block(fm.v, fv.v, qm, qv, tm, tv);
-        store_four(m8, at, n, whole, qm);
-        store_four(v8, at, n, whole, qv);
-        if (lane == 0 && there) {
+        encode_block(fm[u].v, fv[u].v, qm[u], qv[u], tm, tv);
+        store_four(m8, at, n, whole, qm[u]);
+        store_four(v8, at, n, whole, qv[u]);
+        if (lane == 0 && at0 + u * kBlock < n) {
           it.s[b] = tm;
           it.s2[b] = tv;
         }
       } else {
-        qm = load_four(m8, at, n, whole);
-        qv = load_four(v8, at, n, whole);
-        const float um = there ? it.s[b] * kUnitM : 0.0f, uv = there ? it.s2[b] * kUnitV : 0.0f;
-        Four<float> fm, fv;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          fm.v[j] = decode_m(qm.v[j], um);
-          fv.v[j] = decode_v(qv.v[j], uv);
+          fm[u].v[j] = decode_m(qm[u].v[j], um[u]);
+          fv[u].v[j] = decode_v(qv[u].v[j], uv[u]);
         }
-        store_four(it.to_m, at, n, whole, fm);
-        store_four(it.to_v, at, n, whole, fv);
+        store_four(it.to_m, at, n, whole, fm[u]);
+        store_four(it.to_v, at, n, whole, fv[u]);
       }
     }
   }
@@ -429,21 +467,17 @@ unsigned grid_for(size_t chunks, unsigned most) {
 size_t chunks_of(size_t n) { return (n + kChunk - 1) / kChunk; }
 bool dtype_ok(int d) { return d == CP4_DTYPE_F32 || d == CP4_DTYPE_BF16 || d == CP4_DTYPE_F16; }
 
-template <class P, class G>
-void launch_bits(const StepArgs& a, unsigned grid, bool eight, hipStream_t st) {
-  if (eight) step_kernel<P, G, true><<<grid, 64 * kWaves, 0, st>>>(a);
-  else step_kernel<P, G, false><<<grid, 64 * kWaves, 0, st>>>(a);
+template <class P, bool Eight>
+void launch_grad(const StepArgs<Eight>& a, unsigned grid, int g, hipStream_t st) {
+  if (g == CP4_DTYPE_F32) step_kernel<P, F32, Eight><<<grid, 64 * kWaves, 0, st>>>(a);
+  else if (g == CP4_DTYPE_BF16) step_kernel<P, BF16, Eight><<<grid, 64 * kWaves, 0, st>>>(a);
+  else step_kernel<P, F16, Eight><<<grid, 64 * kWaves, 0, st>>>(a);
 }
-template <class P>
-void launch_grad(const StepArgs& a, unsigned grid, int g, bool eight, hipStream_t st) {
-  if (g == CP4_DTYPE_F32) launch_bits<P, F32>(a, grid, eight, st);
-  else if (g == CP4_DTYPE_BF16) launch_bits<P, BF16>(a, grid, eight, st);
-  else launch_bits<P, F16>(a, grid, eight, st);
-}
-void launch_step(const StepArgs& a, unsigned grid, int p, int g, bool eight, hipStream_t st) {
-  if (p == CP4_DTYPE_F32) launch_grad<F32>(a, grid, g, eight, st);
-  else if (p == CP4_DTYPE_BF16) launch_grad<BF16>(a, grid, g, eight, st);
-  else launch_grad<F16>(a, grid, g, eight, st);
+template <bool Eight>
+void launch_step(const StepArgs<Eight>& a, unsigned grid, int p, int g, hipStream_t st) {
+  if (p == CP4_DTYPE_F32) launch_grad<F32>(a, grid, g, st);
+  else if (p == CP4_DTYPE_BF16) launch_grad<BF16>(a, grid, g, st);
+  else launch_grad<F16>(a, grid, g, st);
 }
 
 // Tensors of a list that one launch takes: the same kernel, at most `most` of them with values, fewer
@@ -453,16 +487,16 @@ struct Launch {
   size_t chunks = 0;
   unsigned group = 0;
 };
-template <class Same>
-std::vector<Launch> launches_of(const cp4_adamw_tensor* t, size_t count, size_t most, Same same) {
+template <class Most, class Same>
+std::vector<Launch> launches_of(const cp4_adamw_tensor* t, size_t count, Most most, Same same) {
   std::vector<Launch> out;
   size_t open = 0;                                 // (those before it are full)
   for (size_t i = 0; i < count; ++i) {
     if (!t[i].n) continue;
     const size_t c = chunks_of(t[i].n);
-    while (open < out.size() && out[open].tensors.size() == most) ++open;
+    while (open < out.size() && out[open].tensors.size() == most(t[out[open].tensors[0]])) ++open;
     size_t k = open;
-    while (k < out.size() && !(same(t[out[k].tensors[0]], t[i]) && out[k].tensors.size() < most &&
+    while (k < out.size() && !(same(t[out[k].tensors[0]], t[i]) && out[k].tensors.size() < most(t[i]) &&
                                out[k].chunks + c < (1u << 31)))
       ++k;
     if (k == out.size()) out.emplace_back();
@@ -470,6 +504,42 @@ std::vector<Launch> launches_of(const cp4_adamw_tensor* t, size_t count, size_t 
     out[k].chunks += c;
   }
   return out;
+}
+
+template <bool Eight>
+hipError_t step_launch(const cp4_adamw_tensor* t, const Launch& run, const cp4_adamw_group& o, unsigned blocks,
+                       unsigned most, const float* coefficient, float grad_scale, hipStream_t st) {
+  StepArgs<Eight> a{};
+  size_t chunks = 0;
+  for (size_t i : run.tensors) {
+    a.first[a.count] = (unsigned)chunks;
+    auto& item = a.item[a.count++];
+    static_cast<Item32&>(item) = Item32{t[i].param, t[i].grad, t[i].exp_avg, t[i].exp_avg_sq, t[i].copy, t[i].n};
+    if constexpr (Eight) {
+      item.s = t[i].scale;
+      item.s2 = t[i].scale_sq;
+    }
+    chunks += chunks_of(t[i].n);
+  }
+  const cp4_adamw_tensor none{};
+  const cp4_adamw_tensor& x = run.tensors.empty() ? none : t[run.tensors[0]];
+  a.copy_dtype = x.copy_dtype;
+  a.chunks = (unsigned)chunks;
+  a.blocks = blocks;
+  a.counter = o.counter;
+  a.coefficient = coefficient;
+  a.lr = o.lr;
+  a.beta1 = o.beta1;
+  a.beta2 = o.beta2;
+  a.b1 = (float)o.beta1;
+  a.c1 = (float)(1.0 - o.beta1);
+  a.b2 = (float)o.beta2;
+  a.c2 = (float)(1.0 - o.beta2);
+  a.decay = (float)(1.0 - o.lr * o.weight_decay);
+  a.eps = (float)o.eps;
+  a.scale = grad_scale;
+  launch_step<Eight>(a, grid_for(chunks, most), x.param_dtype, x.grad_dtype, st);
+  return hipGetLastError();
 }
 
 cp4_status check_tensors(const cp4_adamw_tensor* t, size_t count, bool step) {
@@ -497,7 +567,8 @@ cp4_status moments(const cp4_adamw_tensor* t, size_t count, float* const* vm, fl
   for (size_t i = 0; i < count; ++i)
     if (t[i].n && (!vm[i] || !vv[i])) return fail_with(CP4_ERR_NULL_POINTER, "a tensor's values are NULL");
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  for (const Launch& run : launches_of(t, count, kTensors, [](auto&, auto&) { return true; })) {
+  for (const Launch& run : launches_of(t, count, [](auto&) { return (size_t)kMomentTensors; },
+                                       [](auto&, auto&) { return true; })) {
     MomentArgs a{};
     size_t chunks = 0;
     for (size_t i : run.tensors) {
@@ -544,7 +615,8 @@ extern "C" cp4_status cp4_adamw_step(const cp4_adamw_tensor* t, size_t count, co
     if (!workspace || workspace_bytes < cp4_adamw_workspace_bytes() || ((size_t)workspace & 15))
       return fail_with(CP4_ERR_WORKSPACE, "max_norm needs cp4_adamw_workspace_bytes() of workspace, aligned to 16");
     coefficient = static_cast<float*>(workspace);
-    auto runs = launches_of(t, count, kNormTensors, [](auto& x, auto& y) { return x.grad_dtype == y.grad_dtype; });
+    auto runs = launches_of(t, count, [](auto&) { return (size_t)kNormTensors; },
+                            [](auto& x, auto& y) { return x.grad_dtype == y.grad_dtype; });
     if (runs.empty()) runs.emplace_back();
     if (runs.size() > kMostParts) return fail_with(CP4_ERR_SHAPE, "too many tensors");
     const unsigned each = std::max(1u, std::min<unsigned>(most, kMostParts / (unsigned)runs.size()));
@@ -578,7 +650,7 @@ extern "C" cp4_status cp4_adamw_step(const cp4_adamw_tensor* t, size_t count, co
       if (const hipError_t e = hipGetLastError()) return fail_hip(e, "cp4_adamw_step");
     }
   }
-  auto runs = launches_of(t, count, kTensors, [](auto& x, auto& y) {
+  auto runs = launches_of(t, count, [](auto& x) { return (size_t)(x.bits == 8 ? kTensors8 : kTensors32); }, [](auto& x, auto& y) {
     return x.group == y.group && x.param_dtype == y.param_dtype && x.grad_dtype == y.grad_dtype &&
            x.bits == y.bits && (x.copy ? x.copy_dtype : -1) == (y.copy ? y.copy_dtype : -1);
   });
@@ -591,34 +663,10 @@ extern "C" cp4_status cp4_adamw_step(const cp4_adamw_tensor* t, size_t count, co
     runs.back().group = (unsigned)k;
   }
   for (const Launch& run : runs) {
-    const cp4_adamw_group& o = group[run.group];
-    StepArgs a{};
-    size_t chunks = 0;
-    for (size_t i : run.tensors) {
-      a.first[a.count] = (unsigned)chunks;
-      a.item[a.count++] = Item{t[i].param, t[i].grad, t[i].exp_avg, t[i].exp_avg_sq, t[i].scale, t[i].scale_sq,
-                               t[i].copy, t[i].n};
-      chunks += chunks_of(t[i].n);
-    }
-    const cp4_adamw_tensor none{};
-    const cp4_adamw_tensor& x = run.tensors.empty() ? none : t[run.tensors[0]];
-    a.copy_dtype = x.copy_dtype;
-    a.chunks = (unsigned)chunks;
-    a.blocks = blocks[run.group];
-    a.counter = o.counter;
-    a.coefficient = coefficient;
-    a.lr = o.lr;
-    a.beta1 = o.beta1;
-    a.beta2 = o.beta2;
-    a.b1 = (float)o.beta1;
-    a.c1 = (float)(1.0 - o.beta1);
-    a.b2 = (float)o.beta2;
-    a.c2 = (float)(1.0 - o.beta2);
-    a.decay = (float)(1.0 - o.lr * o.weight_decay);
-    a.eps = (float)o.eps;
-    a.scale = grad_scale;
-    launch_step(a, grid_for(chunks, most), x.param_dtype, x.grad_dtype, x.bits == 8, st);
-    if (const hipError_t e = hipGetLastError()) return fail_hip(e, "cp4_adamw_step");
+    const bool eight = !run.tensors.empty() && t[run.tensors[0]].bits == 8;
+    const hipError_t e = eight ? step_launch<true>(t, run, group[run.group], blocks[run.group], most, coefficient, grad_scale, st)
+                               : step_launch<false>(t, run, group[run.group], blocks[run.group], most, coefficient, grad_scale, st);
+    if (e) return fail_hip(e, "cp4_adamw_step");
   }
   return CP4_OK;
 } catch (const std::exception& e) {

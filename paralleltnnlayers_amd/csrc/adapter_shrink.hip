@@ -206,18 +206,26 @@ void launch(const ShrinkArgs& a, hipStream_t st) {
   else vec ? launch_rows<T, false, true>(a, st) : launch_rows<T, false, false>(a, st);
 }
 
-__global__ __launch_bounds__(256) void planes_kernel(float* h, const float* from, size_t n, int planes) {
-  const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
+__global__ __launch_bounds__(64) void planes_kernel(float* h, const float* from, size_t n, int planes) {
+  const size_t i = ((size_t)blockIdx.x * 64 + threadIdx.x) * 4;
   if (i >= n) return;
-  f32x4 x = *reinterpret_cast<const f32x4*>(from + i);
-  for (int s = 1; s < planes; ++s) x += *reinterpret_cast<const f32x4*>(from + s * n + i);
+  f32x4 x = {};
+  int s = 0;
+  for (; s + 8 <= planes; s += 8) {
+    f32x4 y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = *reinterpret_cast<const f32x4*>(from + (s + e) * n + i);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x += y[e];
+  }
+  for (; s < planes; ++s) x += *reinterpret_cast<const f32x4*>(from + s * n + i);
   *reinterpret_cast<f32x4*>(h + i) = x;
 }
 
 }  // namespace
 
 hipError_t planes_join(float* h, const float* from, size_t n, int planes, hipStream_t st) {
-  planes_kernel<<<(unsigned)((n + 1023) / 1024), 256, 0, st>>>(h, from, n, planes);
+  planes_kernel<<<(unsigned)((n + 255) / 256), 64, 0, st>>>(h, from, n, planes);
   return hipGetLastError();
 }
 
