@@ -71,13 +71,14 @@ struct TilePlan {
   int which, splits, each;
   double cost;            // microseconds, about
 };
-TilePlan tile_plan(size_t T, int K, int N, int dtype);
+TilePlan tile_plan(size_t T, int K, int N, int dtype, bool direct);
 size_t tile_part_bytes(const TilePlan&, size_t T, int N);
-bool tile_supported(const ProjectArgs&, int dtype, bool nn);
+// Whether these operands go from memory to the LDS without passing a register.
+bool tile_direct(const ProjectArgs&, int dtype, bool nn);
 hipError_t tile_launch(const ProjectArgs&, const TilePlan&, float* part, int dtype, bool nn, hipStream_t);
 // y = the sum of [splits][T][N] partial sums, and the bias (may be null).
 hipError_t parts_join(const float* part, const float* bias, void* y, size_t T, int N, int splits, int dtype, hipStream_t);
-// Up to 64 tokens in 16 bits, 32 in fp32 (w [N][K], rows on 16-byte boundaries).  splits 0: not for this kernel.
+// Up to 64 tokens in 16 bits, 32 in fp32 (w [N][K]).  splits 0: not for this kernel.
 struct RowsPlan {
   int splits;
 };

@@ -20,7 +20,7 @@ namespace {
 
 constexpr int kCols = 128, kWindow = 8192, kWaves = 8, kPad = 4;
 
-template <class T, bool Vec, int RB>
+template <class T, int RB>
 __global__ __launch_bounds__(64 * kWaves, 2) void grad_kernel(const GradArgs a) {
   typedef typename T::raw Raw;
   constexpr bool kF32 = __is_same(T, F32);
@@ -69,6 +69,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void grad_kernel(const GradArgs a) 
     // (a turn's missing tokens are its last one again, times zero)
     const int turns = (n + kTurn - 1) / kTurn, each = (turns + kWaves - 1) / kWaves;
     const int end = min(turns, (wave + 1) * each);
+    const bool whole = c0 + kCols <= a.C;
     for (int b = wave * each; b < end; ++b) {
       int t[kOwn];
       float p[RB][kOwn];
@@ -77,7 +78,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void grad_kernel(const GradArgs a) 
       for (int q = 0; q < kOwn; ++q) {
         const int i = b * kTurn + kOwn * g + q;
         t[q] = lds.list[min(i, n - 1)];
-        load_some<8>(z + (w0 + t[q]) * a.ldz, cols, Vec, x[q]);
+      }
+      if (whole) {
+#pragma unroll
+        for (int q = 0; q < kOwn; ++q) __builtin_memcpy(x[q], z + (w0 + t[q]) * a.ldz, sizeof(x[q]));
+      } else {
+#pragma unroll
+        for (int q = 0; q < kOwn; ++q) load_some(z + (w0 + t[q]) * a.ldz, cols, x[q]);
       }
 #pragma unroll
       for (int q = 0; q < kOwn; ++q) {
@@ -155,23 +162,17 @@ __global__ __launch_bounds__(256) void join_kernel(const float* part, void* out,
   static_cast<typename T::raw*>(out)[i] = T::narrow(x);
 }
 
-template <class T, bool Vec>
+template <class T>
 void launch(const GradArgs& a, hipStream_t st) {
   const int rb = a.Rp <= 16 ? 1 : a.Rp <= 32 ? 2 : 4;
   const dim3 grid((a.C + kCols - 1) / kCols, a.G * a.splits, (a.Rp + 16 * rb - 1) / (16 * rb));
-  if (rb == 1) grad_kernel<T, Vec, 1><<<grid, 64 * kWaves, 0, st>>>(a);
-  else if (rb == 2) grad_kernel<T, Vec, 2><<<grid, 64 * kWaves, 0, st>>>(a);
-  else grad_kernel<T, Vec, 4><<<grid, 64 * kWaves, 0, st>>>(a);
+  if (rb == 1) grad_kernel<T, 1><<<grid, 64 * kWaves, 0, st>>>(a);
+  else if (rb == 2) grad_kernel<T, 2><<<grid, 64 * kWaves, 0, st>>>(a);
+  else grad_kernel<T, 4><<<grid, 64 * kWaves, 0, st>>>(a);
   if (a.splits > 1) {
     const size_t n = (size_t)a.G * a.R * a.C;
     join_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(a.part, a.out, n, a.splits);
   }
-}
-template <class T>
-void launch(const GradArgs& a, hipStream_t st) {
-  constexpr size_t n = 16 / sizeof(typename T::raw);
-  const bool vec = ((size_t)a.z & 15) == 0 && a.ldz % n == 0;
-  vec ? launch<T, true>(a, st) : launch<T, false>(a, st);
 }
 
 }  // namespace

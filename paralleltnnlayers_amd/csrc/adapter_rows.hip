@@ -22,108 +22,185 @@ struct RowsArgs {
   int splits;
 };
 
+// Four of the adapters of a wave's turn at a time, so that their loads wait together.
+constexpr int kTogether = 4;
+
+// Adds h B_a^T for every kWaves-th of the rows' adapters, from the wave's own on (16 columns; depths as in
+// adapter_tiles.hip).  hl: h [T][Rp] in the LDS.
+template <class T, int MB>
+__device__ __forceinline__ void expand_rows(const ProjectArgs& a, int id, const float* hl, int n0, int wave, f32x4 (&acc)[MB]) {
+  typedef typename T::raw Raw;
+  constexpr bool kF32 = __is_same(T, F32);
+  constexpr int kOwn = kF32 ? 4 : 8;
+  const int lane = threadIdx.x & 63, l = lane & 15, g = lane >> 4;
+  const unsigned long long have = __ballot(id >= 0);
+  for (int r0 = 0; r0 < a.R; r0 += 16) {
+    const int rl = r0 + (kF32 ? 4 * g : 8 * (g & 1));
+    float hv[MB][kOwn];
+    u16x8 ha[MB];
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+#pragma unroll
+      for (int q = 0; q < kOwn; ++q) hv[i][q] = 0.0f;
+      if (have >> (16 * i + l) & 1) __builtin_memcpy(hv[i], __builtin_assume_aligned(hl + (16 * i + l) * a.Rp + rl, 16), sizeof(hv[i]));
+      if constexpr (!kF32) {
+        u16x8 hi, lo;
+        two_parts(hv[i], hi, lo);
+        ha[i] = g < 2 ? hi : lo;
+      }
+    }
+    Adapters todo(id);
+    int turn_of = 0;
+    for (;;) {
+      unsigned long long whose[kTogether];
+      Raw f[kTogether][kOwn];
+      bool any = false;
+#pragma unroll
+      for (int e = 0; e < kTogether; ++e) {
+        whose[e] = 0;
+        int ad = 0;
+        unsigned long long w;
+        while (!whose[e] && todo.take(ad, w))
+          if (turn_of++ % kWaves == wave) whose[e] = w;
+        if (!whose[e]) continue;
+        any = true;
+        const Raw* const p = static_cast<const Raw*>(a.f) + ((size_t)ad * a.N + min(n0 + l, a.N - 1)) * a.R;
+        load_some(p + min(rl, a.R - 1), a.R - rl, f[e]);             // (beyond R: zero, and h is as well)
+      }
+      if (!any) break;
+#pragma unroll
+      for (int e = 0; e < kTogether; ++e) {
+        if (!whose[e]) continue;
+        u16x8 fh = {}, fl = {};
+        if constexpr (__is_same(T, F16)) {
+          float x[8];
+#pragma unroll
+          for (int q = 0; q < 8; ++q) x[q] = F16::widen(f[e][q]);
+          two_parts(x, fh, fl);
+        } else if constexpr (!kF32) {
+          fh = __builtin_bit_cast(u16x8, f[e]);
+        }
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+          f32x4 d = {};
+          if constexpr (kF32) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) d = mfma_f32(hv[i][q], f[e][q], d);
+          } else {
+            if constexpr (__is_same(T, F16)) d = mfma_bf16(ha[i], fl, d);
+            d = mfma_bf16(ha[i], fh, d);
+          }
+#pragma unroll
+          for (int v = 0; v < 4; ++v) acc[i][v] += whose[e] >> (16 * i + 4 * g + v) & 1 ? d[v] : 0.0f;
+        }
+      }
+    }
+  }
+}
+
 template <class T, int MB>
 __global__ __launch_bounds__(64 * kWaves, 2) void rows_kernel(const RowsArgs ra) {
   typedef typename T::raw Raw;
-  constexpr int n = 16 / sizeof(Raw), U = 128 / sizeof(Raw), NB = 1, kRow = 16 * NB + 4, kAhead = 4;
+  constexpr int n = 16 / sizeof(Raw), U = 128 / sizeof(Raw), kRow = 20, kAhead = 4;
   constexpr int kSum = kWaves * 16 * MB * kRow, kH = 16 * MB * 256;
   __shared__ __attribute__((aligned(16))) float lds[kSum > kH ? kSum : kH];
   float* const hl = lds;                                             // [T][Rp], and then ...
   float* const sum = lds;                                            // ... [kWaves][16 MB][kRow]
   const ProjectArgs& a = ra.p;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 15, g = lane >> 4;
-  const int rows = (int)a.T, n0 = blockIdx.x * 16 * NB, split = blockIdx.y;
+  const int rows = (int)a.T, n0 = blockIdx.x * 16, split = blockIdx.y;
   int id = lane < rows ? a.ids[lane] : -1;
-  if (id >= a.G) id = -1;
+  if (id < 0 || id >= a.G) id = -1;
   const bool adapters = split == 0 && __ballot(id >= 0);
-  if (adapters)
-    for (int i = threadIdx.x * 4; i < rows * a.Rp; i += 64 * kWaves * 4) {
-      float x[4] = {};
-      sum_planes(a, 0, i, x);
-      *reinterpret_cast<f32x4*>(hl + i) = f32x4{x[0], x[1], x[2], x[3]};
-    }
-  const Raw *z[MB], *w[NB];
+  const Raw *z[MB], *const w = static_cast<const Raw*>(a.w) + min(n0 + l, a.N - 1) * a.ldw + n * g;
 #pragma unroll
   for (int i = 0; i < MB; ++i) z[i] = static_cast<const Raw*>(a.z) + min(16 * i + l, rows - 1) * a.ldz + n * g;
-#pragma unroll
-  for (int j = 0; j < NB; ++j) w[j] = static_cast<const Raw*>(a.w) + min(n0 + NB * l + j, a.N - 1) * a.ldw + n * g;
   const int units = (a.K + U - 1) / U, shares = kWaves * ra.splits, share = split * kWaves + wave;
   const int first = (int)((long)units * share / shares), last = (int)((long)units * (share + 1) / shares);
   const int whole = min(last, a.K / U);
 
-  f32x4 acc[MB][NB] = {};
-  auto multiply = [&](const u32x4 (&zv)[MB][2], const u32x4 (&wv)[NB][2]) __attribute__((always_inline)) {
+  f32x4 acc[MB] = {};
+  u32x4 zv[kAhead][MB][2], wv[kAhead][2];
+  auto load = [&](int u, int e) __attribute__((always_inline)) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) wv[e][h] = load_16(w + (size_t)u * U + 4 * n * h);
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) zv[e][i][h] = load_16(z[i] + (size_t)u * U + 4 * n * h);
+  };
+  auto multiply = [&](int e) __attribute__((always_inline)) {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int j = 0; j < NB; ++j)
+      for (int i = 0; i < MB; ++i) {
+        if constexpr (__is_same(T, F32)) {
 #pragma unroll
-        for (int i = 0; i < MB; ++i) {
-          if constexpr (__is_same(T, F32)) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              acc[i][j] = mfma_f32(__uint_as_float(zv[i][h][q]), __uint_as_float(wv[j][h][q]), acc[i][j]);
-          } else {
-            acc[i][j] = mfma_16<T>(__builtin_bit_cast(u16x8, zv[i][h]), __builtin_bit_cast(u16x8, wv[j][h]), acc[i][j]);
-          }
+          for (int q = 0; q < 4; ++q)
+            acc[i] = mfma_f32(__uint_as_float(zv[e][i][h][q]), __uint_as_float(wv[e][h][q]), acc[i]);
+        } else {
+          acc[i] = mfma_16<T>(__builtin_bit_cast(u16x8, zv[e][i][h]), __builtin_bit_cast(u16x8, wv[e][h]), acc[i]);
         }
+      }
   };
-  auto ahead = [&](int u, auto count) __attribute__((always_inline)) {
-    constexpr int c = decltype(count)::value;
-    u32x4 zv[c][MB][2], wv[c][NB][2];
+  // The first turns' loads, h's planes while they are on their way, and then the other turns.
+  int u = first;
+  const bool head = u + kAhead <= whole;
+  if (head) {
 #pragma unroll
-    for (int e = 0; e < c; ++e) {
+    for (int e = 0; e < kAhead; ++e) load(u + e, e);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  if (adapters)
+    for (int i = threadIdx.x * 4; i < rows * a.Rp; i += 64 * kWaves * 4) {
+      f32x4 x = {};
+      int s = 0;
+      for (; s + 8 <= a.planes; s += 8) {
+        f32x4 y[8];
 #pragma unroll
-      for (int j = 0; j < NB; ++j)
+        for (int e = 0; e < 8; ++e) y[e] = *reinterpret_cast<const f32x4*>(a.h + (s + e) * a.plane + i);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) wv[e][j][h] = reinterpret_cast<const u32x4*>(w[j] + (size_t)(u + e) * U)[4 * h];
-#pragma unroll
-      for (int i = 0; i < MB; ++i)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) zv[e][i][h] = reinterpret_cast<const u32x4*>(z[i] + (size_t)(u + e) * U)[4 * h];
+        for (int e = 0; e < 8; ++e) x += y[e];
+      }
+      for (; s < a.planes; ++s) x += *reinterpret_cast<const f32x4*>(a.h + s * a.plane + i);
+      *reinterpret_cast<f32x4*>(hl + i) = x;
     }
+  if (head) {
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) multiply(e);
+    u += kAhead;
+  }
+  for (; u + kAhead <= whole; u += kAhead) {
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) load(u + e, e);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int e = 0; e < c; ++e) multiply(zv[e], wv[e]);
-  };
-  int u = first;
-  for (; u + kAhead <= whole; u += kAhead) ahead(u, std::integral_constant<int, kAhead>());
-  for (; u < whole; ++u) ahead(u, std::integral_constant<int, 1>());
+    for (int e = 0; e < kAhead; ++e) multiply(e);
+  }
+  for (; u < whole; ++u) {
+    load(u, 0);
+    multiply(0);
+  }
   if (u < last) {                                                    // (the inputs' rest)
-    u32x4 zv[MB][2], wv[NB][2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const bool there = u * U + n * (4 * h + g) < a.K;
+      const int left = a.K - u * U - n * g - 4 * n * h;
+      wv[0][h] = load_16(w + (size_t)u * U + 4 * n * h, left);
 #pragma unroll
-      for (int i = 0; i < MB; ++i) zv[i][h] = there ? reinterpret_cast<const u32x4*>(z[i] + (size_t)u * U)[4 * h] : u32x4{};
-#pragma unroll
-      for (int j = 0; j < NB; ++j) wv[j][h] = there ? reinterpret_cast<const u32x4*>(w[j] + (size_t)u * U)[4 * h] : u32x4{};
+      for (int i = 0; i < MB; ++i) zv[0][i][h] = load_16(z[i] + (size_t)u * U + 4 * n * h, left);
     }
-    multiply(zv, wv);
+    multiply(0);
   }
   __syncthreads();
-  if (adapters)
-    expand_wave<T, false, MB, NB>(
-        a, id,
-        [&](int i, int r, auto& x) {
-#pragma unroll
-          for (int q = 0; q < (int)(sizeof(x) / 4); q += 4) {
-            const f32x4 v = *reinterpret_cast<const f32x4*>(hl + (16 * i + l) * a.Rp + r + q);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[q + e] = v[e];
-          }
-        },
-        ((size_t)a.f & 15) == 0 && a.R % n == 0, n0, kWaves, wave, acc);
+  if (adapters) expand_rows<T, MB>(a, id, hl, n0, wave, acc);
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < MB; ++i)
 #pragma unroll
-    for (int v = 0; v < 4; ++v)
-#pragma unroll
-      for (int j = 0; j < NB; ++j) sum[(wave * 16 * MB + 16 * i + 4 * g + v) * kRow + NB * l + j] = acc[i][j][v];
+    for (int v = 0; v < 4; ++v) sum[(wave * 16 * MB + 16 * i + 4 * g + v) * kRow + l] = acc[i][v];
   __syncthreads();
-  for (int o = threadIdx.x; o < rows * 16 * NB; o += 64 * kWaves) {
-    const int row = o / (16 * NB), col = o % (16 * NB);
+  for (int o = threadIdx.x; o < rows * 16; o += 64 * kWaves) {
+    const int row = o / 16, col = o % 16;
     if (n0 + col >= a.N) continue;
     float x = 0.0f;
 #pragma unroll

@@ -14,6 +14,7 @@
 #include <algorithm>
 
 #include "adapter.h"
+#include "adapter_load.h"
 
 namespace cp4 {
 namespace adapter {
@@ -24,28 +25,19 @@ template <class T>
 constexpr int kUnit = 128 / sizeof(typename T::raw);                 // inputs of a loop's turn: a cache line a row
 
 // One operand's row of a turn: 16 bytes of each half (64 bytes on); zero from `left` on.
-template <class T, bool Vec>
-__device__ __forceinline__ void load_row(const typename T::raw* p, int left, bool full, u32x4 (&v)[2]) {
-  typedef typename T::raw Raw;
+template <class Raw>
+__device__ __forceinline__ void load_row(const Raw* p, int left, bool full, u32x4 (&v)[2]) {
   constexpr int n = 16 / sizeof(Raw);
-  if constexpr (Vec) {
-    if (full) {
-      v[0] = reinterpret_cast<const u32x4*>(p)[0];
-      v[1] = reinterpret_cast<const u32x4*>(p)[4];
-      return;
-    }
-  }
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    Raw x[n];
-#pragma unroll
-    for (int q = 0; q < n; ++q) x[q] = full || 4 * n * h + q < left ? p[4 * n * h + q] : Raw(0);
-    __builtin_memcpy(&v[h], x, 16);
+  if (full) {
+    v[0] = load_16(p);
+    v[1] = load_16(p + 4 * n);
+  } else {
+    v[0] = load_16(p, left);
+    v[1] = load_16(p + 4 * n, left - 4 * n);
   }
 }
 
-// Vec: rows of z (and of f where it lies input by input, !TR) start on 16-byte boundaries.
-template <class T, bool TR, bool Vec, int MB, int RB>
+template <class T, bool TR, int MB, int RB>
 __global__ __launch_bounds__(64 * kWaves) void shrink_kernel(const ShrinkArgs a) {
   typedef typename T::raw Raw;
   constexpr int n = 16 / sizeof(Raw), U = kUnit<T>, kRows = 16 * MB;
@@ -74,7 +66,6 @@ __global__ __launch_bounds__(64 * kWaves) void shrink_kernel(const ShrinkArgs a)
   const int first = min(u1, u0 + slice * each), last = min(u1, first + each);
   const int whole = min(last, a.K / U);                              // (from there on a turn has fewer inputs)
 
-  const bool even = a.R % RB == 0 && ((size_t)a.f & (RB * sizeof(Raw) - 1)) == 0;
   const Raw* z[MB];
 #pragma unroll
   for (int i = 0; i < MB; ++i) z[i] = static_cast<const Raw*>(a.z) + (t0 + min(16 * i + l, rows - 1)) * a.ldz + n * g;
@@ -91,12 +82,12 @@ __global__ __launch_bounds__(64 * kWaves) void shrink_kernel(const ShrinkArgs a)
       auto load = [&](int u, bool full, u32x4 (&zv)[MB][2], u32x4 (&fv)[RB][2]) __attribute__((always_inline)) {
         const int k = u * U + n * g, left = full ? U : a.K - k;
 #pragma unroll
-        for (int i = 0; i < MB; ++i) load_row<T, Vec>(z[i] + (size_t)u * U, left, full, zv[i]);
+        for (int i = 0; i < MB; ++i) load_row(z[i] + (size_t)u * U, left, full, zv[i]);
         if constexpr (!TR) {
 #pragma unroll
           for (int j = 0; j < RB; ++j) {
             const int r = r0 + RB * l + j;
-            load_row<T, Vec>(f + (size_t)min(r, a.R - 1) * a.K + k, left, full, fv[j]);
+            load_row(f + (size_t)min(r, a.R - 1) * a.K + k, left, full, fv[j]);
             if (r >= a.R) fv[j][0] = fv[j][1] = u32x4{};
           }
         } else {
@@ -106,15 +97,7 @@ __global__ __launch_bounds__(64 * kWaves) void shrink_kernel(const ShrinkArgs a)
           for (int q = 0; q < 2 * n; ++q) {
             const int kq = q < n ? q : q + 3 * n;                     // (the second half lies 4 n inputs on)
             const Raw* const p = f + (size_t)(k + kq) * a.R + r;
-            if (RB > 1 && even) {                                    // (whole lanes of ranks)
-              if (r < a.R && kq < left) __builtin_memcpy(x[q], __builtin_assume_aligned(p, RB * sizeof(Raw)), RB * sizeof(Raw));
-              else
-#pragma unroll
-                for (int j = 0; j < RB; ++j) x[q][j] = Raw(0);
-            } else {
-#pragma unroll
-              for (int j = 0; j < RB; ++j) x[q][j] = r + j < a.R && kq < left ? p[j] : Raw(0);
-            }
+            load_some(p, kq < left ? a.R - r : 0, x[q]);
           }
 #pragma unroll
           for (int j = 0; j < RB; ++j) {
@@ -184,26 +167,18 @@ __global__ __launch_bounds__(64 * kWaves) void shrink_kernel(const ShrinkArgs a)
   }
 }
 
-template <class T, bool TR, bool Vec, int MB>
+template <class T, bool TR, int MB>
 void launch_ranks(const ShrinkArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)((a.T + 16 * MB - 1) / (16 * MB)), a.planes);
-  if (a.Rp <= 16) shrink_kernel<T, TR, Vec, MB, 1><<<grid, 64 * kWaves, 0, st>>>(a);
-  else if (a.Rp <= 32) shrink_kernel<T, TR, Vec, MB, 2><<<grid, 64 * kWaves, 0, st>>>(a);
-  else shrink_kernel<T, TR, Vec, MB, 4><<<grid, 64 * kWaves, 0, st>>>(a);
-}
-template <class T, bool TR, bool Vec>
-void launch_rows(const ShrinkArgs& a, hipStream_t st) {
-  if (a.T >= kShrinkWide) launch_ranks<T, TR, Vec, 2>(a, st);
-  else launch_ranks<T, TR, Vec, 1>(a, st);
+  if (a.Rp <= 16) shrink_kernel<T, TR, MB, 1><<<grid, 64 * kWaves, 0, st>>>(a);
+  else if (a.Rp <= 32) shrink_kernel<T, TR, MB, 2><<<grid, 64 * kWaves, 0, st>>>(a);
+  else shrink_kernel<T, TR, MB, 4><<<grid, 64 * kWaves, 0, st>>>(a);
 }
 template <class T>
 void launch(const ShrinkArgs& a, hipStream_t st) {
-  constexpr size_t n = 16 / sizeof(typename T::raw);
-  const bool tr = a.fk != 1 || a.K == 1;
-  bool vec = ((size_t)a.z & 15) == 0 && a.ldz % n == 0;
-  if (!tr) vec = vec && ((size_t)a.f & 15) == 0 && a.K % n == 0;
-  if (tr) vec ? launch_rows<T, true, true>(a, st) : launch_rows<T, true, false>(a, st);
-  else vec ? launch_rows<T, false, true>(a, st) : launch_rows<T, false, false>(a, st);
+  const bool wide = a.T >= kShrinkWide;
+  if (a.fk != 1) wide ? launch_ranks<T, true, 2>(a, st) : launch_ranks<T, true, 1>(a, st);
+  else wide ? launch_ranks<T, false, 2>(a, st) : launch_ranks<T, false, 1>(a, st);
 }
 
 __global__ __launch_bounds__(64) void planes_kernel(float* h, const float* from, size_t n, int planes) {

@@ -1,6 +1,5 @@
-// The shared projection on the matrix cores (include/cp4/adapter.h), for rows that start on 16-byte
-// boundaries: tiles of 64 or 128 rows x 128 or 256 columns, fed through the LDS by loads that never
-// pass a register.
+// The shared projection on the matrix cores (include/cp4/adapter.h): tiles of 64 to 256 rows x 128 or 256
+// columns, fed through the LDS, by loads that never pass a register where rows start on 16-byte boundaries.
 //
 // A step is 64 bytes of depth (32 values of 16 bits, 16 of fp32) of all the tile's rows and columns.
 // Three steps' room in the LDS: while one is multiplied the next two are on their way, and
@@ -19,7 +18,7 @@
 // Little work for the chip is split over the depth: the partial tiles go to the workspace in
 // fp32 (the first one with the adapters' part) and a second launch adds them up in their order.
 #include <algorithm>
-#include <cstdlib>
+#include <type_traits>
 
 #include "adapter.h"
 #include "adapter_load.h"
@@ -36,15 +35,11 @@ constexpr int kVec = 16 / sizeof(typename T::raw);                   // values o
 // s_waitcnt's operand: all but `loads` memory loads done, and all of the LDS's.
 constexpr int wait_for(int loads) { return (loads & 15) | (loads >> 4) << 14 | 7 << 4; }
 
-// n consecutive values in pieces of up to 16 bytes (whole: they are there and p is aligned to a piece), or the
-// first `count` of them one by one.
+// The first `count` of n consecutive values, whatever p's alignment.
 template <int n, class Raw>
-__device__ __forceinline__ void store_some(Raw* p, const Raw (&o)[n], int count, bool whole) {
-  constexpr int kPiece = n * sizeof(Raw) < 16 ? n : 16 / sizeof(Raw);
-  if (whole) {
-#pragma unroll
-    for (int j = 0; j < n; j += kPiece)
-      __builtin_memcpy(__builtin_assume_aligned(p + j, kPiece * sizeof(Raw)), o + j, kPiece * sizeof(Raw));
+__device__ __forceinline__ void store_some(Raw* p, const Raw (&o)[n], int count) {
+  if (count >= n) {
+    __builtin_memcpy(p, o, n * sizeof(Raw));
   } else {
 #pragma unroll
     for (int j = 0; j < n; ++j)
@@ -64,7 +59,7 @@ __device__ __forceinline__ f32x4 mfma_parts(u32x4 a, u32x4 b, f32x4 c) {
 // again; columns beyond N read its last ones and are not stored.  A product is added only to the rows that are the
 // adapter's: an infinity or a NaN in one adapter is no other token's.
 template <class T, bool NN, int MB, int NB, int WM, int WN>
-__device__ __forceinline__ void expand_tile(const ProjectArgs& a, size_t t0, int n0, char* lds0, char* lds1,
+__device__ __forceinline__ void expand_tile(const ProjectArgs& a, size_t t0, int n0, char* lds0,
                                             f32x4 (&acc)[MB][NB]) {
   typedef typename T::raw Raw;
   constexpr bool kF32 = __is_same(T, F32);
@@ -83,9 +78,9 @@ __device__ __forceinline__ void expand_tile(const ProjectArgs& a, size_t t0, int
     if (w == wm) have_mine = have[w];
   }
   if (!any) return;
-  const bool vec = !NN && ((size_t)a.f & 15) == 0 && a.R % 8 == 0;
   const float* const h = a.h + (t0 + 64 * wm + l) * a.Rp;
   constexpr int kB = NB == 2 ? 2 : 1;                                // blocks of ranks a wait for memory, as registers allow
+  constexpr int kBlock = BN * (__is_same(T, BF16) ? 32 : 64);        // bytes of one in the LDS
   for (int r0 = 0; r0 < a.R; r0 += 16 * kB) {
     const int blocks = min(kB, (a.R - r0 + 15) / 16);
     f32x4 hv[kB][MB];                                                 // fp32: ranks 4 g ..
@@ -108,13 +103,15 @@ __device__ __forceinline__ void expand_tile(const ProjectArgs& a, size_t t0, int
     unsigned long long left[WM];
 #pragma unroll
     for (int w = 0; w < WM; ++w) left[w] = have[w];
-    for (;;) {
+    // The next adapter (-1: none), which of this wave's rows are its own, and its ranks on their way.
+    unsigned long long mine = 0;
+    Raw x[kB][kUnits][8];
+    auto next = [&]() __attribute__((always_inline)) {
       int ad = -1;
 #pragma unroll
       for (int w = 0; w < WM; ++w)
         if (ad < 0 && left[w]) ad = __builtin_amdgcn_readlane(id[w], __builtin_ctzll(left[w]));
-      if (ad < 0) break;
-      unsigned long long mine = 0;
+      if (ad < 0) return false;
 #pragma unroll
       for (int w = 0; w < WM; ++w) {
         const unsigned long long whose = __ballot(id[w] == ad);
@@ -122,7 +119,6 @@ __device__ __forceinline__ void expand_tile(const ProjectArgs& a, size_t t0, int
         if (w == wm) mine = whose;
       }
       const Raw* const f = static_cast<const Raw*>(a.f) + (size_t)ad * a.R * a.N;
-      Raw x[kB][kUnits][8];
 #pragma unroll
       for (int b = 0; b < kB; ++b)
         if (b < blocks)
@@ -131,15 +127,18 @@ __device__ __forceinline__ void expand_tile(const ProjectArgs& a, size_t t0, int
             const int at = u * kThreads + threadIdx.x, r = r0 + 16 * b + at / BN * 8;
             if (at >= 2 * BN) continue;
             const Raw* const p = f + (size_t)min(n0 + at % BN, a.N - 1) * a.fn;
-            if (vec) {
-              const u32x4* const q = reinterpret_cast<const u32x4*>(p + min(r, a.R - 8));
-              __builtin_memcpy(x[b][u], q, 16);
-              if constexpr (kF32) __builtin_memcpy(x[b][u] + 4, q + 1, 16);
+            if (!NN && r + 8 <= a.R) {
+              __builtin_memcpy(x[b][u], p + r, sizeof(x[b][u]));
             } else {
 #pragma unroll
               for (int q = 0; q < 8; ++q) x[b][u][q] = p[(size_t)min(r + q, a.R - 1) * a.fr];
             }
           }
+      return true;
+    };
+    bool more = next();
+    while (more) {
+      const unsigned long long rows = mine;
       __syncthreads();                                               // (nobody reads what was there)
 #pragma unroll
       for (int b = 0; b < kB; ++b)
@@ -149,7 +148,7 @@ __device__ __forceinline__ void expand_tile(const ProjectArgs& a, size_t t0, int
             const int at = u * kThreads + threadIdx.x, col = at % BN, half = at / BN;
             if (at >= 2 * BN) continue;
             const int in = col % (16 * NB), slot = col - in + 16 * (in % NB) + in / NB;    // block j's columns side by side
-            char* const to = b ? lds1 : lds0;
+            char* const to = lds0 + b * kBlock;
             if constexpr (kF32) {
               __builtin_memcpy(__builtin_assume_aligned(to + slot * 64 + half * 32, 16), x[b][u], 32);
             } else if constexpr (__is_same(T, F16)) {
@@ -164,31 +163,33 @@ __device__ __forceinline__ void expand_tile(const ProjectArgs& a, size_t t0, int
               __builtin_memcpy(__builtin_assume_aligned(to + slot * 32 + half * 16, 16), x[b][u], 16);
             }
           }
+      more = next();
       __syncthreads();
-      if (!mine) continue;
 #pragma unroll
-      for (int b = 0; b < kB; ++b) {
-        if (b >= blocks) continue;
+      for (int i = 0; i < MB; ++i) {
+        if (!(rows >> (16 * i) & 0xffff)) continue;
+        // (a product's bits where the row is the adapter's, none elsewhere)
+        const unsigned bits = (unsigned)(rows >> (16 * i)) >> (4 * g);
+        unsigned keep[4];
 #pragma unroll
-        for (int j = 0; j < NB; ++j) {
-          const char* const at = (b ? lds1 : lds0) + (wn + 16 * j + l) * (__is_same(T, BF16) ? 32 : 64);
-          f32x4 fv = {};
-          u16x8 fh = {}, fl = {};
-          if constexpr (kF32) fv = *reinterpret_cast<const f32x4*>(at + g * 16);
-          else fh = *reinterpret_cast<const u16x8*>(at + (g & 1) * 16);
-          if constexpr (__is_same(T, F16)) fl = *reinterpret_cast<const u16x8*>(at + 32 + (g & 1) * 16);
+        for (int v = 0; v < 4; ++v) keep[v] = (unsigned)__builtin_amdgcn_sbfe((int)bits, v, 1);
 #pragma unroll
-          for (int i = 0; i < MB; ++i) {
-            f32x4 d = {};
+        for (int b = 0; b < kB; ++b) {
+          if (b >= blocks) continue;
+#pragma unroll
+          for (int j = 0; j < NB; ++j) {
+            const char* const at = lds0 + b * kBlock + (wn + 16 * j + l) * (__is_same(T, BF16) ? 32 : 64);
+            f32x4 e = {};
             if constexpr (kF32) {
+              const f32x4 fv = *reinterpret_cast<const f32x4*>(at + g * 16);
 #pragma unroll
-              for (int q = 0; q < 4; ++q) d = mfma_f32(hv[b][i][q], fv[q], d);
+              for (int q = 0; q < 4; ++q) e = mfma_f32(hv[b][i][q], fv[q], e);
             } else {
-              if constexpr (__is_same(T, F16)) d = mfma_bf16(ha[b][i], fl, d);
-              d = mfma_bf16(ha[b][i], fh, d);
+              if constexpr (__is_same(T, F16)) e = mfma_bf16(ha[b][i], *reinterpret_cast<const u16x8*>(at + 32 + (g & 1) * 16), e);
+              e = mfma_bf16(ha[b][i], *reinterpret_cast<const u16x8*>(at + (g & 1) * 16), e);
             }
 #pragma unroll
-            for (int v = 0; v < 4; ++v) acc[i][j][v] += mine >> (16 * i + 4 * g + v) & 1 ? d[v] : 0.0f;
+            for (int v = 0; v < 4; ++v) acc[i][j][v] += __uint_as_float(__float_as_uint(e[v]) & keep[v]);
           }
         }
       }
@@ -204,7 +205,7 @@ struct TileArgs {
 };
 
 // One wave of a tile: MB x NB blocks of 16 x 16.
-template <class T, bool NN, int MB, int NB, int WM, int WN, int RB>
+template <class T, bool NN, bool Direct, int MB, int NB, int WM, int WN, int RB>
 __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta) {
   typedef typename T::raw Raw;
   constexpr int kThreads = 64 * WM * WN, BM = 16 * MB * WM, BN = 16 * NB * WN, KS = RB / (int)sizeof(Raw);
@@ -235,37 +236,63 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
   auto piece = [](int slot, int row) __attribute__((always_inline)) { return RC == 4 ? slot ^ (row >> 1 & 3) : slot ^ (row & 7); };
   // What each thread brings: the LDS is filled in the threads' order; which 16 bytes come there is theirs to choose.
   // Rows beyond the operand's are read again from its last one: what they give is not stored.
-  unsigned zo[kZ], wo[kW];
+  typedef std::conditional_t<Direct, unsigned, size_t> Offset;       // (bytes)
+  Offset zo[kZ], wo[kW];
+  int w_count[kW];                                                   // values there of a piece of w's row (nn)
 #pragma unroll
   for (int i = 0; i < kZ; ++i) {
     const int at = i * kThreads + threadIdx.x, row = at / RC, chunk = piece(at % RC, row);
-    zo[i] = (unsigned)(min(row, rows - 1) * a.ldz * sizeof(Raw)) + chunk * 16;
+    zo[i] = (Offset)(min(row, rows - 1) * a.ldz * sizeof(Raw)) + chunk * 16;
   }
 #pragma unroll
   for (int i = 0; i < kW; ++i) {
     const int at = i * kThreads + threadIdx.x;
     if constexpr (NN) {
       constexpr int kRow = BN / kVec<T>;                             // 16-byte pieces of a row
-      wo[i] = (unsigned)(at / kRow * a.ldw * sizeof(Raw)) + min(at % kRow, (cols - 1) / kVec<T>) * 16;
+      const int last = min(at % kRow, (cols - 1) / kVec<T>);
+      wo[i] = (Offset)(at / kRow * a.ldw * sizeof(Raw)) + last * 16;
+      w_count[i] = cols - last * kVec<T>;
     } else {
       const int slot = at / RC, chunk = piece(at % RC, slot), in = slot % (16 * NB);
       const int col = slot - in + NB * (in & 15) + in / 16;
-      wo[i] = (unsigned)(min(col, cols - 1) * a.ldw * sizeof(Raw)) + chunk * 16;
+      wo[i] = (Offset)(min(col, cols - 1) * a.ldw * sizeof(Raw)) + chunk * 16;
+      w_count[i] = kVec<T>;
     }
   }
   int brought = 0;
-  auto bring = [&](char* lds) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < kZ; ++i)
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(zb + zo[i]),
-                                       (__attribute__((address_space(3))) void*)(lds + (i * kThreads + wave * 64) * 16), 16, 0, 0);
-#pragma unroll
-    for (int i = 0; i < kW; ++i)
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(wb + wo[i]),
-                                       (__attribute__((address_space(3))) void*)(lds + BM * RB + (i * kThreads + wave * 64) * 16), 16, 0, 0);
+  auto advance = [&]() __attribute__((always_inline)) {
     const bool more = ++brought < steps;                             // (beyond the last step that one again)
     zb += more ? RB : 0;
     wb += more ? w_next : 0;
+  };
+  // Operands on 16-byte boundaries go from memory to the LDS by themselves; others through registers, which put()
+  // writes when the step that hid their way is multiplied.
+  u32x4 zr[Direct ? 1 : kZ], wr[Direct ? 1 : kW];
+  auto bring = [&](char* lds) __attribute__((always_inline)) {
+    if constexpr (Direct) {
+#pragma unroll
+      for (int i = 0; i < kZ; ++i)
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(zb + zo[i]),
+                                         (__attribute__((address_space(3))) void*)(lds + (i * kThreads + wave * 64) * 16), 16, 0, 0);
+#pragma unroll
+      for (int i = 0; i < kW; ++i)
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(wb + wo[i]),
+                                         (__attribute__((address_space(3))) void*)(lds + BM * RB + (i * kThreads + wave * 64) * 16), 16, 0, 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kZ; ++i) zr[i] = load_16(reinterpret_cast<const Raw*>(zb + zo[i]));
+#pragma unroll
+      for (int i = 0; i < kW; ++i) wr[i] = load_16(reinterpret_cast<const Raw*>(wb + wo[i]), NN ? w_count[i] : kVec<T>);
+    }
+    advance();
+  };
+  auto put = [&](char* lds) __attribute__((always_inline)) {
+    if constexpr (!Direct) {
+#pragma unroll
+      for (int i = 0; i < kZ; ++i) *reinterpret_cast<u32x4*>(lds + (i * kThreads + threadIdx.x) * 16) = zr[i];
+#pragma unroll
+      for (int i = 0; i < kW; ++i) *reinterpret_cast<u32x4*>(lds + BM * RB + (i * kThreads + threadIdx.x) * 16) = wr[i];
+    }
   };
 
   f32x4 acc[MB][NB] = {};
@@ -352,21 +379,25 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
   // from counting the loads under way.
   auto step = [&](const char* lds, char* into) __attribute__((always_inline)) {
     asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(wait_for(kRooms == 3 ? kZ + kW : 0));
+    if constexpr (Direct) __builtin_amdgcn_s_waitcnt(wait_for(kRooms == 3 ? kZ + kW : 0));
+    else __builtin_amdgcn_s_waitcnt(wait_for(63));                   // (the LDS alone)
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
     bring(into);
     __builtin_amdgcn_sched_barrier(0);
     multiply(lds);
+    put(into);
   };
   if (steps > 0) {
     bring(lds0);
+    put(lds0);
     int left = steps;                                                // (no way out in the middle: the same reason)
     if constexpr (kRooms == 3) {
       asm volatile("" ::: "memory");                                 // (their order is what the waits count on)
       __builtin_amdgcn_sched_barrier(0);
       bring(lds1);
+      put(lds1);
       for (; left >= 3; left -= 3) {
         step(lds0, lds2);
         step(lds1, lds0);
@@ -392,17 +423,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kZ; ++i) {
-      const int at = i * kThreads + threadIdx.x, chunk = piece(at % RC, at / RC);
+      const int at = i * kThreads + threadIdx.x, depth = piece(at % RC, at / RC) * kVec<T>;
       u32x4 x = {};
-      if (chunk * kVec<T> < left) {
-        if constexpr (NN) {                                          // (z's row may end inside the 16 bytes)
-          Raw v[kVec<T>];
-          load_some<kVec<T>>(reinterpret_cast<const Raw*>(zb + zo[i]), left - chunk * kVec<T>, true, v);
-          __builtin_memcpy(&x, v, 16);
-        } else {
-          x = *reinterpret_cast<const u32x4*>(zb + zo[i]);
-        }
-      }
+      if (depth < left) x = load_16(reinterpret_cast<const Raw*>(zb + zo[i]), left - depth);
       *reinterpret_cast<u32x4*>(lds0 + at * 16) = x;
     }
 #pragma unroll
@@ -410,19 +433,18 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
       const int at = i * kThreads + threadIdx.x;
       const int depth = NN ? at / (BN / kVec<T>) : piece(at % RC, at / RC) * kVec<T>;
       u32x4 x = {};
-      if (depth < left) x = *reinterpret_cast<const u32x4*>(wb + wo[i]);
+      if (depth < left) x = load_16(reinterpret_cast<const Raw*>(wb + wo[i]), NN ? w_count[i] : left - depth);
       *reinterpret_cast<u32x4*>(lds0 + BM * RB + at * 16) = x;
     }
     __syncthreads();
     multiply(lds0);
   }
 
-  if (split == 0) expand_tile<T, NN, MB, NB, WM, WN>(a, t0, n0, lds0, lds1, acc);
+  if (split == 0) expand_tile<T, NN, MB, NB, WM, WN>(a, t0, n0, lds0, acc);
   const int n = n0 + wn + NB * l;
   if (n >= a.N) return;
   if (ta.part) {
     float* const y = ta.part + ((size_t)split * a.T + t0 + wm) * a.N + n;
-    const bool whole = n + NB <= a.N && a.N % (NB < 4 ? NB : 4) == 0;
 #pragma unroll
     for (int i = 0; i < MB; ++i)
 #pragma unroll
@@ -433,7 +455,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
         float o[NB];
 #pragma unroll
         for (int j = 0; j < NB; ++j) o[j] = acc[i][j][v];
-        store_some(p, o, a.N - n, whole);
+        store_some(p, o, a.N - n);
       }
     return;
   }
@@ -441,8 +463,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
 #pragma unroll
   for (int j = 0; j < NB; ++j) bias[j] = a.bias && n + j < a.N ? a.bias[n + j] : 0.0f;
   Raw* const y = static_cast<Raw*>(a.y) + (t0 + wm) * a.N + n;
-  constexpr size_t kPiece = NB * sizeof(Raw) < 16 ? NB * sizeof(Raw) : 16;
-  const bool whole = n + NB <= a.N && a.N * sizeof(Raw) % kPiece == 0 && ((size_t)a.y & 15) == 0;
 #pragma unroll
   for (int i = 0; i < MB; ++i)
 #pragma unroll
@@ -452,7 +472,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
       Raw o[NB];
 #pragma unroll
       for (int j = 0; j < NB; ++j) o[j] = T::narrow(acc[i][j][v] + bias[j]);
-      store_some(y + (size_t)row * a.N, o, a.N - n, whole);
+      store_some(y + (size_t)row * a.N, o, a.N - n);
     }
 }
 
@@ -463,8 +483,16 @@ __global__ __launch_bounds__(256) void join_kernel(const float* part, const floa
   if (i >= n) return;
   typename T::raw* const o = static_cast<typename T::raw*>(y) + i;
   if (n % 4 == 0 && N % 4 == 0) {
-    f32x4 x = *reinterpret_cast<const f32x4*>(part + i);
-    for (int s = 1; s < splits; ++s) x += *reinterpret_cast<const f32x4*>(part + s * n + i);
+    f32x4 x = {};
+    int s = 0;
+    for (; s + 8 <= splits; s += 8) {
+      f32x4 y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = *reinterpret_cast<const f32x4*>(part + (s + e) * n + i);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x += y[e];
+    }
+    for (; s < splits; ++s) x += *reinterpret_cast<const f32x4*>(part + s * n + i);
     if (bias) {
       const int c = (int)(i % N);
 #pragma unroll
@@ -482,36 +510,38 @@ __global__ __launch_bounds__(256) void join_kernel(const float* part, const floa
   }
 }
 
-template <class T, bool NN, int MB, int NB, int WM, int WN, int RB>
+template <class T, bool NN, bool Direct, int MB, int NB, int WM, int WN, int RB>
 void launch(const TileArgs& t, hipStream_t st) {
-  tile_kernel<T, NN, MB, NB, WM, WN, RB><<<die_grid((long)t.mt * t.nt * t.splits), 64 * WM * WN, 0, st>>>(t);
+  tile_kernel<T, NN, Direct, MB, NB, WM, WN, RB><<<die_grid((long)t.mt * t.nt * t.splits), 64 * WM * WN, 0, st>>>(t);
 }
-// (fp32: its parts take the registers of 128 columns a wave)
-template <class T, bool NN>
+// (fp32: its parts take the registers of 128 columns a wave; through registers: the two smaller shapes)
+template <class T, bool NN, bool Direct>
 void launch_shape(const TileArgs& t, int which, hipStream_t st) {
-  if constexpr (__is_same(T, F32)) {
-    if (which == 1) launch<T, NN, 4, 2, 2, 4, 128>(t, st);
-    else launch<T, NN, 4, 4, 1, 4, 128>(t, st);
-  } else {
-    if (which == 0) launch<T, NN, 4, 8, 2, 2, 64>(t, st);
-    else if (which == 1) launch<T, NN, 4, 2, 2, 4, 64>(t, st);
-    else if (which == 2) launch<T, NN, 4, 4, 1, 4, 64>(t, st);
-    else launch<T, NN, 4, 8, 4, 2, 128>(t, st);
+  constexpr int RB = __is_same(T, F32) ? 128 : 64;
+  if constexpr (Direct && !__is_same(T, F32)) {
+    if (which == 0) return launch<T, NN, true, 4, 8, 2, 2, 64>(t, st);
+    if (which == 3) return launch<T, NN, true, 4, 8, 4, 2, 128>(t, st);
   }
+  if (which == 1) launch<T, NN, Direct, 4, 2, 2, 4, RB>(t, st);
+  else launch<T, NN, Direct, 4, 4, 1, 4, RB>(t, st);
+}
+template <class T>
+void launch_type(const TileArgs& t, int which, bool nn, bool direct, hipStream_t st) {
+  if (direct) nn ? launch_shape<T, true, true>(t, which, st) : launch_shape<T, false, true>(t, which, st);
+  else nn ? launch_shape<T, true, false>(t, which, st) : launch_shape<T, false, false>(t, which, st);
 }
 
 constexpr int kShapes = 4, kRows[kShapes] = {128, 128, 64, 256}, kCols[kShapes] = {256, 128, 256, 256};
 
 }  // namespace
 
-TilePlan tile_plan(size_t T, int K, int N, int dtype) {
+TilePlan tile_plan(size_t T, int K, int N, int dtype, bool aligned) {
   const long units = num_compute_units();
   const bool f32 = dtype == CP4_DTYPE_F32;
   TilePlan best{};
   double least = 0;
-  static const char* force = getenv("WHICH");
-  for (int w = f32 ? 1 : 0; w < (f32 ? 3 : kShapes); ++w) {
-    if (force && w != atoi(force)) continue;
+  const bool some = f32 || !aligned;
+  for (int w = some ? 1 : 0; w < (some ? 3 : kShapes); ++w) {
     const int KS = w == 3 ? 64 : 32, steps = (K + KS - 1) / KS;
     const long tiles = (long)((T + kRows[w] - 1) / kRows[w]) * ((N + kCols[w] - 1) / kCols[w]);
     for (int s = 1; s <= 64 && s <= std::max(1, steps / 4); s *= 2) {
@@ -536,12 +566,11 @@ TilePlan tile_plan(size_t T, int K, int N, int dtype) {
 }
 size_t tile_part_bytes(const TilePlan& p, size_t T, int N) { return p.splits > 1 ? (size_t)p.splits * T * N * 4 : 0; }
 
-bool tile_supported(const ProjectArgs& a, int dtype, bool nn) {
+// Whether the LDS can be filled directly: 16-byte boundaries, and a thread's places in a tile as 32-bit byte offsets.
+bool tile_direct(const ProjectArgs& a, int dtype, bool nn) {
   const size_t e = dtype == CP4_DTYPE_F32 ? 4 : 2, vec = 16 / e;
-  if (((size_t)a.z & 15) || ((size_t)a.w & 15) || a.ldz % vec || a.ldw % vec) return false;
-  if (nn ? a.N % vec : a.K % vec) return false;
-  // (a thread's places in a tile are 32-bit byte offsets)
-  return a.ldz * e * 128 < (size_t)1 << 31 && a.ldw * e * 256 < (size_t)1 << 31 && a.T < ((size_t)1 << 31) - 256;
+  if (((size_t)a.z & 15) || ((size_t)a.w & 15) || a.ldz % vec || a.ldw % vec || (nn ? a.N : a.K) % vec) return false;
+  return a.ldz * e * 256 < (size_t)1 << 31 && a.ldw * e * 256 < (size_t)1 << 31;
 }
 
 hipError_t parts_join(const float* part, const float* bias, void* y, size_t T, int N, int splits, int dtype, hipStream_t st) {
@@ -561,9 +590,10 @@ hipError_t tile_launch(const ProjectArgs& a, const TilePlan& plan, float* part, 
   t.nt = (a.N + kCols[plan.which] - 1) / kCols[plan.which];
   t.splits = plan.splits;
   t.steps = plan.each;
-  if (dtype == CP4_DTYPE_F32) nn ? launch_shape<F32, true>(t, plan.which, st) : launch_shape<F32, false>(t, plan.which, st);
-  else if (dtype == CP4_DTYPE_BF16) nn ? launch_shape<BF16, true>(t, plan.which, st) : launch_shape<BF16, false>(t, plan.which, st);
-  else nn ? launch_shape<F16, true>(t, plan.which, st) : launch_shape<F16, false>(t, plan.which, st);
+  const bool d = tile_direct(a, dtype, nn);
+  if (dtype == CP4_DTYPE_F32) launch_type<F32>(t, plan.which, nn, d, st);
+  else if (dtype == CP4_DTYPE_BF16) launch_type<BF16>(t, plan.which, nn, d, st);
+  else launch_type<F16>(t, plan.which, nn, d, st);
   if (const hipError_t e = hipGetLastError()) return e;
   return plan.splits > 1 ? parts_join(part, a.bias, a.y, a.T, a.N, plan.splits, dtype, st) : hipSuccess;
 }
