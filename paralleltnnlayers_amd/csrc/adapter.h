@@ -55,7 +55,6 @@ struct GradArgs {
   int splits;
 };
 
-constexpr size_t kShrinkWide = 4096;     // tokens from which a workgroup takes 32 of them
 int shrink_planes(size_t T, int K, int dtype);
 hipError_t shrink_launch(const ShrinkArgs&, int dtype, hipStream_t);
 // h [n] = the sum of `planes` planes of n values (n: a multiple of 4), the first of which may be h.

@@ -1,7 +1,7 @@
 // h = scale A_a x, token by token (include/cp4/adapter.h): a product with as few columns as the adapters
 // have ranks, bound by reading x and the adapters in use once.
 //
-// A workgroup takes 16 or 32 tokens and one part of the inputs, straight from memory to the matrix cores:
+// A workgroup takes 16 tokens and one part of the inputs, straight from memory to the matrix cores:
 // nothing is read twice within it, so the LDS would only be a detour.  Its eight waves share the adapters that
 // these tokens have - one of a prompt, sixteen of single tokens - and, where there are fewer, the
 // inputs.  All rows are multiplied with each adapter and the rows that are not its own keep what they had; the
@@ -37,10 +37,10 @@ __device__ __forceinline__ void load_row(const Raw* p, int left, bool full, u32x
   }
 }
 
-template <class T, bool TR, int MB, int RB>
+template <class T, bool TR, int RB>
 __global__ __launch_bounds__(64 * kWaves) void shrink_kernel(const ShrinkArgs a) {
   typedef typename T::raw Raw;
-  constexpr int n = 16 / sizeof(Raw), U = kUnit<T>, kRows = 16 * MB;
+  constexpr int n = 16 / sizeof(Raw), U = kUnit<T>, MB = 1, kRows = 16 * MB;
   __shared__ float sum[kWaves][16][16 * RB + 4];
   __shared__ int own[kRows];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 15, g = lane >> 4;
@@ -125,7 +125,7 @@ __global__ __launch_bounds__(64 * kWaves) void shrink_kernel(const ShrinkArgs a)
               }
             }
       };
-      constexpr int kAhead = MB + RB <= 3 ? 4 : 2;                   // turns whose loads come before their products
+      constexpr int kAhead = RB <= 2 ? 4 : 2;                   // turns whose loads come before their products
       int u = first;
       for (; u + kAhead <= whole; u += kAhead) {
         u32x4 zv[kAhead][MB][2], fv[kAhead][RB][2];
@@ -167,18 +167,16 @@ __global__ __launch_bounds__(64 * kWaves) void shrink_kernel(const ShrinkArgs a)
   }
 }
 
-template <class T, bool TR, int MB>
+template <class T, bool TR>
 void launch_ranks(const ShrinkArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)((a.T + 16 * MB - 1) / (16 * MB)), a.planes);
-  if (a.Rp <= 16) shrink_kernel<T, TR, MB, 1><<<grid, 64 * kWaves, 0, st>>>(a);
-  else if (a.Rp <= 32) shrink_kernel<T, TR, MB, 2><<<grid, 64 * kWaves, 0, st>>>(a);
-  else shrink_kernel<T, TR, MB, 4><<<grid, 64 * kWaves, 0, st>>>(a);
+  const dim3 grid((unsigned)((a.T + 15) / 16), a.planes);
+  if (a.Rp <= 16) shrink_kernel<T, TR, 1><<<grid, 64 * kWaves, 0, st>>>(a);
+  else if (a.Rp <= 32) shrink_kernel<T, TR, 2><<<grid, 64 * kWaves, 0, st>>>(a);
+  else shrink_kernel<T, TR, 4><<<grid, 64 * kWaves, 0, st>>>(a);
 }
 template <class T>
 void launch(const ShrinkArgs& a, hipStream_t st) {
-  const bool wide = a.T >= kShrinkWide;
-  if (a.fk != 1) wide ? launch_ranks<T, true, 2>(a, st) : launch_ranks<T, true, 1>(a, st);
-  else wide ? launch_ranks<T, false, 2>(a, st) : launch_ranks<T, false, 1>(a, st);
+  a.fk != 1 ? launch_ranks<T, true>(a, st) : launch_ranks<T, false>(a, st);
 }
 
 __global__ __launch_bounds__(64) void planes_kernel(float* h, const float* from, size_t n, int planes) {
@@ -204,12 +202,12 @@ hipError_t planes_join(float* h, const float* from, size_t n, int planes, hipStr
   return hipGetLastError();
 }
 
-// Parts of the inputs: two workgroups for each compute unit, four turns or more a part.
+// Parts of the inputs: a workgroup for each compute unit, four turns or more a part.
 int shrink_planes(size_t T, int K, int dtype) {
   const int unit = dtype == CP4_DTYPE_F32 ? kUnit<F32> : kUnit<BF16>;
-  const size_t wide = T >= kShrinkWide ? 32 : 16, tiles = std::max<size_t>(1, (T + wide - 1) / wide);
+  const size_t tiles = std::max<size_t>(1, (T + 15) / 16);
   const size_t most = std::max(1, (K + unit - 1) / unit / 4);
-  return (int)std::max<size_t>(1, std::min({(2 * (size_t)num_compute_units() + tiles - 1) / tiles, most, (size_t)64}));
+  return (int)std::max<size_t>(1, std::min({((size_t)num_compute_units() + tiles - 1) / tiles, most, (size_t)64}));
 }
 
 hipError_t shrink_launch(const ShrinkArgs& a, int dtype, hipStream_t st) {

@@ -298,6 +298,40 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
   f32x4 acc[MB][NB] = {};
   // (16-bit: piece g of a row; fp32: pieces 2 g and 2 g + 1)
   const int z_at = (wm + l) * RB, w_at = BM * RB + (NN ? 0 : (wn + l) * RB);
+  // (16 bits) the operands of 32 of a step's depths, and their products
+  auto read = [&](const char* lds, int kk, u16x8 (&zf)[MB], u16x8 (&wf)[NB]) __attribute__((always_inline)) {
+    const int at = piece(4 * kk + g, l) * 16;
+#pragma unroll
+    for (int i = 0; i < MB; ++i) zf[i] = *reinterpret_cast<const u16x8*>(lds + z_at + at + i * 16 * RB);
+    if constexpr (NN) {
+      unsigned in[8][NB / 2];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const char* const p = lds + w_at + ((32 * kk + 8 * g + q) * BN + wn + NB * l) * 2;
+        if constexpr (NB == 2) {
+          in[q][0] = *reinterpret_cast<const unsigned*>(p);
+        } else if constexpr (NB == 8) {
+          const u32x4 x = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) in[q][e] = x[e];
+        } else {
+          const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+          in[q][0] = x[0];
+          in[q][1] = x[1];
+        }
+      }
+      turn<NB>(in, wf);
+    } else {
+#pragma unroll
+      for (int j = 0; j < NB; ++j) wf[j] = *reinterpret_cast<const u16x8*>(lds + w_at + at + j * 16 * RB);
+    }
+  };
+  auto products = [&](const u16x8 (&zf)[MB], const u16x8 (&wf)[NB]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int i = 0; i < MB; ++i) acc[i][j] = mfma_16<T>(zf[i], wf[j], acc[i][j]);
+  };
   auto multiply = [&](const char* lds) __attribute__((always_inline)) {
     if constexpr (__is_same(T, F32)) {
       // fp32 values as three bfloat16 parts, a product as the six largest partial products
@@ -341,36 +375,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
     } else {
 #pragma unroll
       for (int kk = 0; kk < RB / 64; ++kk) {
-        const int at = piece(4 * kk + g, l) * 16;
         u16x8 zf[MB], wf[NB];
-#pragma unroll
-        for (int i = 0; i < MB; ++i) zf[i] = *reinterpret_cast<const u16x8*>(lds + z_at + at + i * 16 * RB);
-        if constexpr (NN) {
-          unsigned in[8][NB / 2];
-#pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const char* const p = lds + w_at + ((32 * kk + 8 * g + q) * BN + wn + NB * l) * 2;
-            if constexpr (NB == 2) {
-              in[q][0] = *reinterpret_cast<const unsigned*>(p);
-            } else if constexpr (NB == 8) {
-              const u32x4 x = *reinterpret_cast<const u32x4*>(p);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) in[q][e] = x[e];
-            } else {
-              const u32x2 x = *reinterpret_cast<const u32x2*>(p);
-              in[q][0] = x[0];
-              in[q][1] = x[1];
-            }
-          }
-          turn<NB>(in, wf);
-        } else {
-#pragma unroll
-          for (int j = 0; j < NB; ++j) wf[j] = *reinterpret_cast<const u16x8*>(lds + w_at + at + j * 16 * RB);
-        }
-#pragma unroll
-        for (int j = 0; j < NB; ++j)
-#pragma unroll
-          for (int i = 0; i < MB; ++i) acc[i][j] = mfma_16<T>(zf[i], wf[j], acc[i][j]);
+        read(lds, kk, zf, wf);
+        products(zf, wf);
       }
     }
   };
@@ -389,7 +396,54 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
     multiply(lds);
     put(into);
   };
-  if (steps > 0) {
+  if constexpr (Direct && !NN && RB == 128 && !__is_same(T, F32)) {
+    // The large tile: a half step's operands are read while the other half's are multiplied, so that the LDS and the
+    // matrix cores work at the same time.  In the middle of a step its room is free - all have read the second
+    // half - and the next one's has arrived.  (8192x4096x4096 bf16: 216 us, 243 one after the other.  With w [K][N] the
+    // turned operands do not fit beside: 255 us with what spills, 243.)
+    u16x8 za[MB], wa[NB], zc[MB], wc[NB];
+    auto turns = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < MB + NB; ++e) {                            // (a read, two products)
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+      }
+    };
+    auto both = [&](char* lds, const char* then) __attribute__((always_inline)) {
+      read(lds, 1, zc, wc);
+      products(za, wa);
+      turns();
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_waitcnt(wait_for(0));
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      bring(lds);
+      __builtin_amdgcn_sched_barrier(0);
+      read(then, 0, za, wa);
+      products(zc, wc);
+      turns();
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    if (steps > 0) {
+      bring(lds0);
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      bring(lds1);
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_waitcnt(wait_for(kZ + kW));
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      read(lds0, 0, za, wa);
+      int left = steps;
+      for (; left >= 2; left -= 2) {
+        both(lds0, lds1);
+        both(lds1, lds0);
+      }
+      if (left > 0) both(lds0, lds1);
+      __builtin_amdgcn_s_waitcnt(wait_for(0));                       // (the loads beyond the last step)
+    }
+  } else if (steps > 0) {
     bring(lds0);
     put(lds0);
     int left = steps;                                                // (no way out in the middle: the same reason)

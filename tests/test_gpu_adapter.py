@@ -360,3 +360,16 @@ def test_refusals(cp4):
         p = {**d, **frozen}
         with pytest.raises(ValueError, match="not trained"):
             torch_ops.adapter_linear(p["x"], p["W"], p["A"], p["B"], p["ids"], p["scale"], p["bias"])
+
+
+def test_example_trains_and_serves(cp4):
+    """The example: a CP convolution and adapters trained by the library's AdamW, then served together."""
+    import importlib.util
+    import os
+    at = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "adapters.py")
+    spec = importlib.util.spec_from_file_location("adapters_example", at)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    before, after, agree = module.run(users=4, steps=10, images=64)
+    assert after < before
+    assert agree == 1.0
