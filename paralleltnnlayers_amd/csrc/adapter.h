@@ -83,8 +83,9 @@ struct RowsPlan {
 };
 RowsPlan rows_plan(size_t T, int K, int N, int dtype);
 hipError_t rows_launch(const ProjectArgs&, const RowsPlan&, float* part, int dtype, hipStream_t);
-int grad_splits(size_t T, int C, int R, int G);
-hipError_t grad_launch(const GradArgs&, int dtype, hipStream_t);
+// Two sums over the same tokens and adapters, their R, G and splits the same.
+int grad_splits(size_t T, int C0, int C1, int R, int G);
+hipError_t grad_launch(const GradArgs&, const GradArgs&, int dtype, hipStream_t);
 
 // ---- device side ------------------------------------------------------------------------
 

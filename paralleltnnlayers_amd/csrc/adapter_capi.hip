@@ -40,18 +40,17 @@ cp4_status check_pointers(size_t bytes, std::initializer_list<const void*> value
 size_t h_bytes(const cp4_adapter_shape& s) { return s.T * padded(s) * 4; }
 
 struct BackwardPlan {
-  int splits_a, splits_b, dh_planes;
-  size_t part_at, total;                               // (dh comes first)
+  int splits, dh_planes;
+  size_t part_at, part_b, total;                       // (dh comes first; B's partial sums: floats behind A's)
 };
 BackwardPlan backward_plan(const cp4_adapter_shape& s, int dtype) {
   BackwardPlan p{};
-  p.splits_a = grad_splits(s.T, (int)s.K, (int)s.R, (int)s.G);
-  p.splits_b = grad_splits(s.T, (int)s.N, (int)s.R, (int)s.G);
+  p.splits = grad_splits(s.T, (int)s.K, (int)s.N, (int)s.R, (int)s.G);
   p.dh_planes = shrink_planes(s.T, (int)s.N, dtype);
   p.part_at = align256(p.dh_planes * h_bytes(s));
-  const size_t each = (size_t)s.G * s.R * 4;
-  const size_t pa = p.splits_a > 1 ? p.splits_a * each * s.K : 0, pb = p.splits_b > 1 ? p.splits_b * each * s.N : 0;
-  p.total = p.part_at + align256(std::max({pa, pb, project_part_bytes(s.T, (int)s.N, (int)s.K, dtype)}));   // (one after the other)
+  p.part_b = p.splits > 1 ? (size_t)p.splits * s.G * s.R * s.K : 0;
+  const size_t parts = p.splits > 1 ? (p.part_b + (size_t)p.splits * s.G * s.R * s.N) * 4 : 0;
+  p.total = p.part_at + align256(std::max(parts, project_part_bytes(s.T, (int)s.N, (int)s.K, dtype)));  // (one after the other)
   return p;
 }
 
@@ -147,14 +146,12 @@ extern "C" cp4_status cp4_adapter_backward(const cp4_adapter_shape* s, int dtype
     if (const hipError_t e = project_launch(p, part, dtype, true, st)) return fail_hip(e, "cp4_adapter_backward");
   }
   if (dA) {
-    GradArgs g{};
-    g.ids = ids; g.part = part; g.T = s->T; g.R = (int)s->R; g.Rp = Rp; g.G = (int)s->G;
-    g.p = dh; g.z = x; g.out = dA; g.ldz = ldx; g.C = (int)s->K; g.outr = (int)s->K; g.outc = 1;
-    g.splits = plan.splits_a;
-    if (const hipError_t e = grad_launch(g, dtype, st)) return fail_hip(e, "cp4_adapter_backward");
-    g.p = kept; g.z = dy; g.out = dB; g.ldz = lddy; g.C = (int)s->N; g.outr = 1; g.outc = (int)s->R;
-    g.splits = plan.splits_b;
-    if (const hipError_t e = grad_launch(g, dtype, st)) return fail_hip(e, "cp4_adapter_backward");
+    GradArgs ga{};
+    ga.ids = ids; ga.T = s->T; ga.R = (int)s->R; ga.Rp = Rp; ga.G = (int)s->G; ga.splits = plan.splits;
+    GradArgs gb = ga;
+    ga.p = dh; ga.z = x; ga.out = dA; ga.part = part; ga.ldz = ldx; ga.C = (int)s->K; ga.outr = (int)s->K; ga.outc = 1;
+    gb.p = kept; gb.z = dy; gb.out = dB; gb.part = part + plan.part_b; gb.ldz = lddy; gb.C = (int)s->N; gb.outr = 1; gb.outc = (int)s->R;
+    if (const hipError_t e = grad_launch(ga, gb, dtype, st)) return fail_hip(e, "cp4_adapter_backward");
   }
   return CP4_OK;
 }

@@ -2,7 +2,7 @@
 // of an fp32 row of h or dh and a row of dy or x: a product as deep as the adapter has tokens and as high as
 // it has ranks, bound by reading x and dy once.
 //
-// A workgroup takes 128 columns of one adapter.  It picks the adapter's tokens out of 8192 ids at a time
+// Both gradients of a call are one launch.  A workgroup takes 128 columns of one adapter.  It picks the adapter's tokens out of 8192 ids at a time
 // into a list in the LDS (in order, so that sums do not change from call to call); its eight waves share the list,
 // 32 tokens (fp32: 16) a turn, straight from memory: a lane reads eight consecutive columns of each
 // of its tokens' rows and turns them in registers into eight column blocks' operands.  The waves' sums
@@ -18,10 +18,17 @@ namespace cp4 {
 namespace adapter {
 namespace {
 
+// Both gradients of a call.
+struct GradPair {
+  GradArgs g[2];
+  int tiles;              // workgroups along the first one's columns
+};
+
 constexpr int kCols = 128, kWindow = 8192, kWaves = 8, kPad = 4;
 
 template <class T, int RB>
-__global__ __launch_bounds__(64 * kWaves, 2) void grad_kernel(const GradArgs a) {
+__global__ __launch_bounds__(64 * kWaves, 2) void grad_kernel(const GradPair pair) {
+  const GradArgs& a = pair.g[(int)blockIdx.x >= pair.tiles];
   typedef typename T::raw Raw;
   constexpr bool kF32 = __is_same(T, F32);
   constexpr int kTurn = kF32 ? 16 : 32, kOwn = kTurn / 4;            // tokens of a turn, and of a lane
@@ -32,7 +39,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void grad_kernel(const GradArgs a) 
   __shared__ int counts[kWaves];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 15, g = lane >> 4;
   const int ad = blockIdx.y % a.G, split = blockIdx.y / a.G, r0 = blockIdx.z * 16 * RB;
-  const int c0 = blockIdx.x * kCols, c = c0 + 8 * l;
+  const int c0 = (blockIdx.x - ((int)blockIdx.x >= pair.tiles ? pair.tiles : 0)) * kCols, c = c0 + 8 * l;
   const size_t per = (a.T + a.splits - 1) / a.splits;
   const size_t first = min(a.T, split * per), last = min(a.T, first + per);
   const Raw* const z = static_cast<const Raw*>(a.z) + min(c, a.C - 1);
@@ -154,41 +161,47 @@ __global__ __launch_bounds__(64 * kWaves, 2) void grad_kernel(const GradArgs a) 
 
 // The ranges' sums, in their order.
 template <class T>
-__global__ __launch_bounds__(256) void join_kernel(const float* part, void* out, size_t n, int splits) {
-  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+__global__ __launch_bounds__(256) void join_kernel(const GradPair pair, size_t n0, size_t n1) {
+  size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+  const bool second = i >= n0;
+  if (second) i -= n0;
+  const size_t n = second ? n1 : n0;
   if (i >= n) return;
+  const float* const part = second ? pair.g[1].part : pair.g[0].part;
   float x = part[i];
-  for (int s = 1; s < splits; ++s) x += part[(size_t)s * n + i];
-  static_cast<typename T::raw*>(out)[i] = T::narrow(x);
+  for (int s = 1; s < pair.g[0].splits; ++s) x += part[(size_t)s * n + i];
+  static_cast<typename T::raw*>(second ? pair.g[1].out : pair.g[0].out)[i] = T::narrow(x);
 }
 
 template <class T>
-void launch(const GradArgs& a, hipStream_t st) {
+void launch(const GradPair& p, hipStream_t st) {
+  const GradArgs &a = p.g[0], &b = p.g[1];
   const int rb = a.Rp <= 16 ? 1 : a.Rp <= 32 ? 2 : 4;
-  const dim3 grid((a.C + kCols - 1) / kCols, a.G * a.splits, (a.Rp + 16 * rb - 1) / (16 * rb));
-  if (rb == 1) grad_kernel<T, 1><<<grid, 64 * kWaves, 0, st>>>(a);
-  else if (rb == 2) grad_kernel<T, 2><<<grid, 64 * kWaves, 0, st>>>(a);
-  else grad_kernel<T, 4><<<grid, 64 * kWaves, 0, st>>>(a);
+  const dim3 grid(p.tiles + (b.C + kCols - 1) / kCols, a.G * a.splits, (a.Rp + 16 * rb - 1) / (16 * rb));
+  if (rb == 1) grad_kernel<T, 1><<<grid, 64 * kWaves, 0, st>>>(p);
+  else if (rb == 2) grad_kernel<T, 2><<<grid, 64 * kWaves, 0, st>>>(p);
+  else grad_kernel<T, 4><<<grid, 64 * kWaves, 0, st>>>(p);
   if (a.splits > 1) {
-    const size_t n = (size_t)a.G * a.R * a.C;
-    join_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(a.part, a.out, n, a.splits);
+    const size_t each = (size_t)a.G * a.R, n = each * (a.C + b.C);
+    join_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(p, each * a.C, each * b.C);
   }
 }
 
 }  // namespace
 
 // Ranges of tokens: two workgroups for each compute unit, none with fewer than 256 tokens.
-int grad_splits(size_t T, int C, int R, int G) {
-  const size_t wgs = (size_t)((C + kCols - 1) / kCols) * G * ((R + 63) / 64);
+int grad_splits(size_t T, int C0, int C1, int R, int G) {
+  const size_t wgs = (size_t)((C0 + kCols - 1) / kCols + (C1 + kCols - 1) / kCols) * G * ((R + 63) / 64);
   const size_t want = (2 * (size_t)num_compute_units() + wgs - 1) / wgs;
   const size_t most = std::min<size_t>((T + 255) / 256, 65535 / G);
   return (int)std::max<size_t>(1, std::min(want, most));
 }
 
-hipError_t grad_launch(const GradArgs& a, int dtype, hipStream_t st) {
-  if (dtype == CP4_DTYPE_F32) launch<F32>(a, st);
-  else if (dtype == CP4_DTYPE_BF16) launch<BF16>(a, st);
-  else launch<F16>(a, st);
+hipError_t grad_launch(const GradArgs& a, const GradArgs& b, int dtype, hipStream_t st) {
+  const GradPair p{{a, b}, (a.C + kCols - 1) / kCols};
+  if (dtype == CP4_DTYPE_F32) launch<F32>(p, st);
+  else if (dtype == CP4_DTYPE_BF16) launch<BF16>(p, st);
+  else launch<F16>(p, st);
   return hipGetLastError();
 }
 

@@ -396,7 +396,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
     multiply(lds);
     put(into);
   };
-  if constexpr (Direct && !NN && RB == 128 && !__is_same(T, F32)) {
+  if constexpr (Direct && !NN && NB == 8 && RB == 128) {
     // The large tile: a half step's operands are read while the other half's are multiplied, so that the LDS and the
     // matrix cores work at the same time.  In the middle of a step its room is free - all have read the second
     // half - and the next one's has arrived.  (8192x4096x4096 bf16: 216 us, 243 one after the other.  With w [K][N] the
@@ -571,13 +571,12 @@ void launch(const TileArgs& t, hipStream_t st) {
 // (fp32: its parts take the registers of 128 columns a wave; through registers: the two smaller shapes)
 template <class T, bool NN, bool Direct>
 void launch_shape(const TileArgs& t, int which, hipStream_t st) {
-  constexpr int RB = __is_same(T, F32) ? 128 : 64;
   if constexpr (Direct && !__is_same(T, F32)) {
     if (which == 0) return launch<T, NN, true, 4, 8, 2, 2, 64>(t, st);
     if (which == 3) return launch<T, NN, true, 4, 8, 4, 2, 128>(t, st);
   }
-  if (which == 1) launch<T, NN, Direct, 4, 2, 2, 4, RB>(t, st);
-  else launch<T, NN, Direct, 4, 4, 1, 4, RB>(t, st);
+  if (which == 1) launch<T, NN, Direct, 4, 2, 2, 4, 128>(t, st);
+  else launch<T, NN, Direct, 4, 4, 1, 4, 128>(t, st);
 }
 template <class T>
 void launch_type(const TileArgs& t, int which, bool nn, bool direct, hipStream_t st) {
@@ -596,7 +595,7 @@ TilePlan tile_plan(size_t T, int K, int N, int dtype, bool aligned) {
   double least = 0;
   const bool some = f32 || !aligned;
   for (int w = some ? 1 : 0; w < (some ? 3 : kShapes); ++w) {
-    const int KS = w == 3 ? 64 : 32, steps = (K + KS - 1) / KS;
+    const int KS = f32 || w == 0 ? 32 : 64, steps = (K + KS - 1) / KS;
     const long tiles = (long)((T + kRows[w] - 1) / kRows[w]) * ((N + kCols[w] - 1) / kCols[w]);
     for (int s = 1; s <= 64 && s <= std::max(1, steps / 4); s *= 2) {
       const int each = (steps + s - 1) / s;
