@@ -2,8 +2,8 @@
 // columns, fed through the LDS, by loads that never pass a register where rows start on 16-byte boundaries.
 //
 // A step is 64 bytes of depth (32 values of 16 bits, 16 of fp32) of all the tile's rows and columns.
-// Three steps' room in the LDS: while one is multiplied the next two are on their way, and
-// one barrier a step says both that the next one has arrived and that the last one's room is free.
+// The LDS has room for two to four steps: while one is multiplied the next ones are on their way, and one barrier a
+// step says both that the next one has arrived and that the last one's room is free.
 // A wave has 64 rows and 64 or 128 columns in registers; two workgroups on a compute unit keep its
 // matrix cores busy over each other's barriers.
 //
@@ -205,15 +205,16 @@ struct TileArgs {
 };
 
 // One wave of a tile: MB x NB blocks of 16 x 16.
-template <class T, bool NN, bool Direct, int MB, int NB, int WM, int WN, int RB>
+template <class T, bool NN, bool Direct, int MB, int NB, int WM, int WN, int RB, int Rooms>
 __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta) {
   typedef typename T::raw Raw;
   constexpr int kThreads = 64 * WM * WN, BM = 16 * MB * WM, BN = 16 * NB * WN, KS = RB / (int)sizeof(Raw);
-  constexpr int RC = RB / 16, kRooms = RB == 128 ? 2 : 3;            // a row's bytes of a step: 16-byte pieces
+  constexpr int RC = RB / 16;                                        // a row's bytes of a step: 16-byte pieces
   constexpr int kZ = BM * RC / kThreads, kW = BN * RC / kThreads;    // 16-byte loads of a thread and step
   static_assert(BM * RC % kThreads == 0 && BN * RC % kThreads == 0, "whole loads");
-  // (three variables, so that the compiler knows a load into one from a read of another)
-  __shared__ __attribute__((aligned(1024))) char lds0[(BM + BN) * RB], lds1[(BM + BN) * RB], lds2[kRooms == 3 ? (BM + BN) * RB : 16];
+  // (variables of their own, so that the compiler knows a load into one from a read of another)
+  constexpr int kRoom = (BM + BN) * RB;
+  __shared__ __attribute__((aligned(1024))) char lds0[kRoom], lds1[kRoom], lds2[Rooms > 2 ? kRoom : 16], lds3[Rooms > 3 ? kRoom : 16];
   const ProjectArgs& a = ta.p;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 15, g = lane >> 4;
   // the place of this workgroup: each die a contiguous run of tiles, up to eight columns of tiles wide
@@ -381,12 +382,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
       }
     }
   };
-  // A step: its own loads have arrived (with three rooms those of the next one may still be on their way), and
-  // nobody reads the last one's room any more.  Every step brings one, so that no branch keeps the compiler
-  // from counting the loads under way.
+  // A step: its own loads have arrived (with more than two rooms those of the next ones may still be on their way),
+  // and nobody reads the last one's room any more.  Every step brings one, so that no branch keeps the
+  // compiler from counting the loads under way.
   auto step = [&](const char* lds, char* into) __attribute__((always_inline)) {
     asm volatile("" ::: "memory");
-    if constexpr (Direct) __builtin_amdgcn_s_waitcnt(wait_for(kRooms == 3 ? kZ + kW : 0));
+    if constexpr (Direct) __builtin_amdgcn_s_waitcnt(wait_for((Rooms - 2) * (kZ + kW)));
     else __builtin_amdgcn_s_waitcnt(wait_for(63));                   // (the LDS alone)
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -397,11 +398,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
     put(into);
   };
   if constexpr (Direct && !NN && NB == 8 && RB == 128) {
-    // The large tile: a half step's operands are read while the other half's are multiplied, so that the LDS and the
-    // matrix cores work at the same time.  In the middle of a step its room is free - all have read the second
-    // half - and the next one's has arrived.  (8192x4096x4096 bf16: 216 us, 243 one after the other.  With w [K][N] the
-    // turned operands do not fit beside: 255 us with what spills, 243.)
+    // A half step's operands are read while the other half's are multiplied, so that the LDS and the matrix cores
+    // work at the same time.  In the middle of a step its room is free - all have read the second half - and
+    // the next one's has arrived.  (8192x4096x4096 bf16: 216 us, 243 one after the other.  With w [K][N] the turned
+    // operands of 128 columns do not fit beside: 255 us with what spills, 243.)
     u16x8 za[MB], wa[NB], zc[MB], wc[NB];
+    static_assert(Rooms == 2, "the loop below");
     auto turns = [&]() __attribute__((always_inline)) {
 #pragma unroll
       for (int e = 0; e < MB + NB; ++e) {                            // (a read, two products)
@@ -427,7 +429,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
     };
     if (steps > 0) {
       bring(lds0);
-      asm volatile("" ::: "memory");
+      asm volatile("" ::: "memory");                                 // (their order is what the wait counts on)
       __builtin_amdgcn_sched_barrier(0);
       bring(lds1);
       asm volatile("" ::: "memory");
@@ -444,28 +446,36 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
       __builtin_amdgcn_s_waitcnt(wait_for(0));                       // (the loads beyond the last step)
     }
   } else if (steps > 0) {
-    bring(lds0);
-    put(lds0);
-    int left = steps;                                                // (no way out in the middle: the same reason)
-    if constexpr (kRooms == 3) {
+    auto ahead = [&](char* lds) __attribute__((always_inline)) {
+      bring(lds);
+      put(lds);
       asm volatile("" ::: "memory");                                 // (their order is what the waits count on)
       __builtin_amdgcn_sched_barrier(0);
-      bring(lds1);
-      put(lds1);
-      for (; left >= 3; left -= 3) {
+    };
+    ahead(lds0);
+    if constexpr (Rooms > 2) ahead(lds1);
+    if constexpr (Rooms > 3) ahead(lds2);
+    int left = steps;                                                // (no way out in the middle: the same reason)
+    for (; left >= Rooms; left -= Rooms) {
+      if constexpr (Rooms == 2) {
+        step(lds0, lds1);
+        step(lds1, lds0);
+      } else if constexpr (Rooms == 3) {
         step(lds0, lds2);
         step(lds1, lds0);
         step(lds2, lds1);
-      }
-      if (left > 0) step(lds0, lds2);
-      if (left > 1) step(lds1, lds0);
-    } else {
-      for (; left >= 2; left -= 2) {
-        step(lds0, lds1);
+      } else {
+        step(lds0, lds3);
         step(lds1, lds0);
+        step(lds2, lds1);
+        step(lds3, lds2);
       }
-      if (left > 0) step(lds0, lds1);
     }
+    if (left > 0) step(lds0, Rooms == 2 ? lds1 : Rooms == 3 ? lds2 : lds3);
+    if constexpr (Rooms > 2)
+      if (left > 1) step(lds1, lds0);
+    if constexpr (Rooms > 3)
+      if (left > 2) step(lds2, lds1);
     __builtin_amdgcn_s_waitcnt(wait_for(0));                         // (the loads beyond the last step)
   }
   if (k_first + steps * KS < k_last) {
@@ -564,19 +574,19 @@ __global__ __launch_bounds__(256) void join_kernel(const float* part, const floa
   }
 }
 
-template <class T, bool NN, bool Direct, int MB, int NB, int WM, int WN, int RB>
+template <class T, bool NN, bool Direct, int MB, int NB, int WM, int WN, int RB, int Rooms>
 void launch(const TileArgs& t, hipStream_t st) {
-  tile_kernel<T, NN, Direct, MB, NB, WM, WN, RB><<<die_grid((long)t.mt * t.nt * t.splits), 64 * WM * WN, 0, st>>>(t);
+  tile_kernel<T, NN, Direct, MB, NB, WM, WN, RB, Rooms><<<die_grid((long)t.mt * t.nt * t.splits), 64 * WM * WN, 0, st>>>(t);
 }
 // (fp32: its parts take the registers of 128 columns a wave; through registers: the two smaller shapes)
 template <class T, bool NN, bool Direct>
 void launch_shape(const TileArgs& t, int which, hipStream_t st) {
   if constexpr (Direct && !__is_same(T, F32)) {
-    if (which == 0) return launch<T, NN, true, 4, 8, 2, 2, 64>(t, st);
-    if (which == 3) return launch<T, NN, true, 4, 8, 4, 2, 128>(t, st);
+    if (which == 0) return launch<T, NN, true, 4, 8, 2, 2, 64, 3>(t, st);
+    if (which == 3) return launch<T, NN, true, 4, 8, 4, 2, 128, 2>(t, st);
   }
-  if (which == 1) launch<T, NN, Direct, 4, 2, 2, 4, 128>(t, st);
-  else launch<T, NN, Direct, 4, 4, 1, 4, 128>(t, st);
+  if (which == 1) return launch<T, NN, Direct, 4, 2, 2, 4, 128, Direct ? 4 : 2>(t, st);
+  launch<T, NN, Direct, 4, 4, 1, 4, 128, 2>(t, st);
 }
 template <class T>
 void launch_type(const TileArgs& t, int which, bool nn, bool direct, hipStream_t st) {

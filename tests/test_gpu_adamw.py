@@ -446,3 +446,22 @@ def test_refusals(optim):
         optim.AdamW([torch.nn.Parameter(p)], betas=(0.9, 1.0))
     with pytest.raises(ValueError):
         optim.AdamW([torch.nn.Parameter(p)], max_norm=0)
+
+
+def test_more_than_2_to_the_32_values(optim):
+    """The last values of a tensor beyond 32-bit offsets step like those of a small one."""
+    n, tail = (1 << 32) + 1027, 2048 + 3          # (the tail starts with a block of the scales: n - tail is a multiple of 256)
+    assert (n - tail) % 256 == 0
+    gen = torch.Generator().manual_seed(13)
+    p, g = torch.randn(tail, generator=gen), gradients(gen, tail).bfloat16()
+    P = torch.zeros(n, device="cuda")
+    G = torch.zeros(n, device="cuda", dtype=torch.bfloat16)
+    P[n - tail:], G[n - tail:] = p.cuda(), g.cuda()
+    m, v, s = optim.empty_moments(P, 8)
+    optim.adamw_step([P], [G], [m], [v], optim.counter(), scales=[s], **HYPER)
+    want = numpy_step(p.numpy(), g.float().numpy(), np.zeros(tail, F), np.zeros(tail, F), 1, **HYPER)
+    q = codes(*want[1:])
+    assert np.array_equal(P[n - tail:].cpu().numpy(), want[0])
+    assert np.array_equal(m[n - tail:].cpu().numpy(), q[0]) and np.array_equal(v[n - tail:].cpu().numpy(), q[1])
+    assert np.array_equal(s[:, -q[2].shape[1]:].cpu().numpy(), q[2])
+    assert not P[:4096].any() and not m[(1 << 32) - 5000:(1 << 32) - 3000].any()

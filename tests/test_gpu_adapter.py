@@ -373,3 +373,59 @@ def test_example_trains_and_serves(cp4):
     before, after, agree = module.run(users=4, steps=10, images=64)
     assert after < before
     assert agree == 1.0
+
+
+@pytest.mark.parametrize("T, ld", [(5, 1 << 29), (40, 1 << 27), (300, 1 << 24)])
+def test_rows_beyond_32_bit_offsets(cp4, T, ld):
+    """Rows so far apart that the last ones lie beyond 2^32 bytes."""
+    K, N, R, G = 264, 200, 8, 3
+    d = make("bf16", T, K, N, R, G, "mixed", seed=23)
+    want = formula(d, "bf16")
+    g = {k: v.cuda() for k, v in d.items()}
+    room = torch.empty((T - 1) * ld + 512, dtype=torch.bfloat16, device="cuda")
+    assert room.numel() * 2 > 1 << 32
+    x = room.as_strided((T, K), (ld, 1))
+    x.copy_(g["x"])
+    y, kept = cp4.adapter_forward(x, g["W"], g["A"], g["B"], g["ids"], g["scale"], g["bias"], keep=True)
+    check(y, want["y"], "y")
+    dy = room.as_strided((T, N), (ld, 1), 272)
+    if 272 + N > 512:
+        dy = room.as_strided((T, N), (ld, 1))
+        x = g["x"]
+    dy.copy_(g["dy"])
+    for k, v in zip(("dx", "dA", "dB"), cp4.adapter_backward(dy, x, g["W"], g["A"], g["B"], g["ids"], g["scale"], kept)):
+        check(v, want[k], k)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("size", [(2077, 512, 1024, 32, 5), (700, 2048, 264, 16, 4), (1500, 192, 2112, 24, 3),
+                                  (4200, 130, 257, 9, 6)], ids=lambda s: "x".join(map(str, s)))
+def test_every_shape_of_tile(cp4, dtype, size):
+    """Batches beyond one tile, with rows left over."""
+    T, K, N, R, G = size
+    d = make(dtype, T, K, N, R, G, "runs", seed=29)
+    want = formula(d, dtype)
+    g = {k: v.cuda() for k, v in d.items()}
+    y, kept = cp4.adapter_forward(g["x"], g["W"], g["A"], g["B"], g["ids"], g["scale"], g["bias"], keep=True)
+    check(y, want["y"], "y")
+    for k, v in zip(("dx", "dA", "dB"), cp4.adapter_backward(g["dy"], g["x"], g["W"], g["A"], g["B"], g["ids"], g["scale"], kept)):
+        check(v, want[k], k)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_large_tiles(cp4, dtype):
+    """The 256 x 256 tiles of both directions, on sampled rows and columns."""
+    T, K, N, R, G = 4096 + 40, 2048 + 72, 4096, 16, 8
+    gen = torch.Generator(device="cuda").manual_seed(31)
+    n = lambda *s, std=1.0: (torch.randn(*s, device="cuda", generator=gen) * std).to(DTYPES[dtype])
+    x, W, A, B, dy = n(T, K), n(N, K, std=K ** -0.5), n(G, R, K, std=K ** -0.5), n(G, N, R, std=R ** -0.5), n(T, N)
+    ids = ids_of("runs", T, G, torch.Generator().manual_seed(32))
+    scale = torch.full((G,), 0.5, device="cuda")
+    y, kept = cp4.adapter_forward(x, W, A, B, ids.cuda(), scale, keep=True)
+    dx = cp4.adapter_backward(dy, None, W, A, B, ids.cuda(), scale, want_factors=False)[0]
+    rows = torch.cat([torch.arange(0, T, 97), torch.arange(T - 45, T)])
+    d = dict(x=x.cpu()[rows], W=W.cpu(), A=A.cpu(), B=B.cpu(), dy=dy.cpu()[rows], ids=ids[rows], scale=scale.cpu(),
+             bias=torch.zeros(N))
+    want = formula(d, dtype, bias=False)
+    check(y.cpu()[rows], want["y"], "y")
+    check(dx.cpu()[rows], want["dx"], "dx")
