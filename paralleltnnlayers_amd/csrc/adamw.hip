@@ -3,8 +3,10 @@
 //
 // A value costs its memory traffic alone: 4 + 4 bytes of parameter, 2 or 4 of gradient, 16 of fp32
 // moments or 4.06 of 8-bit ones, read and written once.  So the pass is bound by HBM, and everything is
-// made to keep many wide loads in flight: a wave takes 1024 consecutive values of a tensor as four
-// blocks of 256 (one 16-byte load a lane and array), all of their loads before any arithmetic.  A block
+// made to keep many wide loads in flight (134 M values with 8-bit moments 403 us, 4.7 TB/s; 50 M with fp32 moments and
+// bfloat16 copies 246 us, 5.1 TB/s; a large copy reaches 5.1): a wave takes 1024 consecutive values of a tensor as four
+// blocks of 256 (one 16-byte load a lane and array), all of their loads before any arithmetic (with a branch around each
+// load for a tensor's end 612 us instead of 403).  A block
 // of 256 values is one wave's register, so its largest magnitude is a reduction inside the wave
 // and a moment is never written before it is rounded for good.  The tensors of a launch are a table in
 // the kernel's arguments: no copy to the device that a captured graph would have to repeat.
@@ -32,10 +34,8 @@ constexpr size_t kChunk = kBlock * kUnroll;        // values of a wave's turn
 constexpr int kTensors32 = 75, kTensors8 = 57;     // of a launch: kernel arguments below 4 KB
 constexpr int kNormTensors = 192, kMomentTensors = 57;
 constexpr unsigned kWaves = 4;                     // of a workgroup
+constexpr unsigned kNormWaves = 16;                // of the norm's: fewer that hand in a partial sum
 constexpr unsigned kMostParts = 16384;             // partial sums of the norm
-
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 struct Item32 {
   void* p;
@@ -72,16 +72,15 @@ struct NormArgs {
 };
 static_assert(sizeof(NormArgs) <= 4096, "kernel arguments");
 
-// Four consecutive values of an array, as they lie in memory.
+// Four consecutive values of an array, as they lie in memory: one load or store at any alignment.  All: they are
+// there (a wave's whole turn is; the branch is then the wave's, and nothing lies between its loads).
 template <class Raw>
 struct Four { Raw v[4]; };
-template <class Raw>
-__device__ __forceinline__ Four<Raw> load_four(const Raw* p, size_t at, size_t n, bool whole) {
+template <bool All, class Raw>
+__device__ __forceinline__ Four<Raw> load_four(const Raw* p, size_t at, size_t n) {
   Four<Raw> r{};
-  if (whole) {
-    if constexpr (sizeof(Raw) == 4) r = __builtin_bit_cast(Four<Raw>, *reinterpret_cast<const f32x4*>(p + at));
-    else if constexpr (sizeof(Raw) == 2) r = __builtin_bit_cast(Four<Raw>, *reinterpret_cast<const u32x2*>(p + at));
-    else r = __builtin_bit_cast(Four<Raw>, *reinterpret_cast<const unsigned*>(p + at));
+  if (All || at + 4 <= n) {
+    __builtin_memcpy(r.v, p + at, sizeof(r.v));
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -89,21 +88,15 @@ __device__ __forceinline__ Four<Raw> load_four(const Raw* p, size_t at, size_t n
   }
   return r;
 }
-template <class Raw>
-__device__ __forceinline__ void store_four(Raw* p, size_t at, size_t n, bool whole, const Four<Raw>& r) {
-  if (whole) {
-    if constexpr (sizeof(Raw) == 4) *reinterpret_cast<f32x4*>(p + at) = __builtin_bit_cast(f32x4, r);
-    else if constexpr (sizeof(Raw) == 2) *reinterpret_cast<u32x2*>(p + at) = __builtin_bit_cast(u32x2, r);
-    else *reinterpret_cast<unsigned*>(p + at) = __builtin_bit_cast(unsigned, r);
+template <bool All, class Raw>
+__device__ __forceinline__ void store_four(Raw* p, size_t at, size_t n, const Four<Raw>& r) {
+  if (All || at + 4 <= n) {
+    __builtin_memcpy(p + at, r.v, sizeof(r.v));
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (at + j < n) p[at + j] = r.v[j];
   }
-}
-template <class Raw>
-__device__ __forceinline__ bool aligned_four(const Raw* p) {
-  return ((size_t)p & (4 * sizeof(Raw) - 1)) == 0;
 }
 
 // ---- 8-bit moments ------------------------------------------------------------------------
@@ -145,8 +138,8 @@ __device__ __forceinline__ int signed_code(int q, float m) { return m < 0.0f ? -
 
 // Codes and scales of one block of 256 values: four a lane, those beyond the tensor zero.  A code is defined by
 // correctly rounded roots; the hardware's, a unit in the last place off, give the same one but near the middle of
-// two codes, where the few blocks that have such a value take the long way (12 instructions a root
-// less for the others: 134 M values 720 us with the long way alone).
+// two codes, where the few blocks that have such a value take the long way (134 M values 720 us with
+// the long way alone, 622 so).
 __device__ __forceinline__ void encode_block(const float (&m)[4], const float (&v)[4], Four<signed char>& qm,
                                              Four<unsigned char>& qv, float& sm, float& sv) {
   unsigned tm = 0, tv = 0;
@@ -215,95 +208,93 @@ __global__ __launch_bounds__(64 * kWaves, 4) void step_kernel(const StepArgs<Eig
       const size_t n = it.n, at0 = (size_t)(c - a.first[t]) * kChunk;
       RawP* const p = static_cast<RawP*>(it.p);
       const RawG* const g = static_cast<const RawG*>(it.g);
-      bool even = aligned_four(p) && aligned_four(g);
-      if constexpr (Eight) even = even && (((size_t)it.m | (size_t)it.v) & 3) == 0;
-      else even = even && (((size_t)it.m | (size_t)it.v) & 15) == 0;
-      if (it.copy) even = even && ((size_t)it.copy & (a.copy_dtype == CP4_DTYPE_F32 ? 15 : 7)) == 0;
-
-      Four<RawP> rp[kUnroll];
-      Four<RawG> rg[kUnroll];
-      Four<float> m32[kUnroll], v32[kUnroll];
-      Four<signed char> m8[kUnroll];
-      Four<unsigned char> v8[kUnroll];
-      float sm[kUnroll], sv[kUnroll];
+      auto turn = [&](auto all) __attribute__((always_inline)) {
+        constexpr bool kAll = decltype(all)::value;
+        Four<RawP> rp[kUnroll];
+        Four<RawG> rg[kUnroll];
+        Four<float> m32[kUnroll], v32[kUnroll];
+        Four<signed char> m8[kUnroll];
+        Four<unsigned char> v8[kUnroll];
+        float sm[kUnroll], sv[kUnroll];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const size_t at = at0 + u * kBlock + lane * 4;
-        const bool whole = even && at + 4 <= n;
-        rp[u] = load_four(p, at, n, whole);
-        rg[u] = load_four(g, at, n, whole);
-        if constexpr (Eight) {
-          m8[u] = load_four(static_cast<signed char*>(it.m), at, n, whole);
-          v8[u] = load_four(static_cast<unsigned char*>(it.v), at, n, whole);
-          const size_t b = (at0 + u * kBlock) / kBlock;
-          const bool there = at0 + u * kBlock < n;
-          sm[u] = there ? it.s[b] : 0.0f;
-          sv[u] = there ? it.s2[b] : 0.0f;
-        } else {
-          m32[u] = load_four(static_cast<float*>(it.m), at, n, whole);
-          v32[u] = load_four(static_cast<float*>(it.v), at, n, whole);
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const size_t at = at0 + u * kBlock + lane * 4;
-        const bool whole = even && at + 4 <= n;
-        float m[4], v[4];
-        Four<RawP> np;
-        Four<float> wide;
-        const float um = Eight ? sm[u] * kUnitM : 0.0f, uv = Eight ? sv[u] * kUnitV : 0.0f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int u = 0; u < kUnroll; ++u) {
+          const size_t at = at0 + u * kBlock + lane * 4;
+          rp[u] = load_four<kAll>(p, at, n);
+          rg[u] = load_four<kAll>(g, at, n);
           if constexpr (Eight) {
-            m[j] = decode_m(m8[u].v[j], um);
-            v[j] = decode_v(v8[u].v[j], uv);
+            m8[u] = load_four<kAll>(static_cast<signed char*>(it.m), at, n);
+            v8[u] = load_four<kAll>(static_cast<unsigned char*>(it.v), at, n);
+            const size_t b = (at0 + u * kBlock) / kBlock;
+            const bool there = kAll || at0 + u * kBlock < n;
+            sm[u] = there ? it.s[b] : 0.0f;
+            sv[u] = there ? it.s2[b] : 0.0f;
           } else {
-            m[j] = m32[u].v[j];
-            v[j] = v32[u].v[j];
+            m32[u] = load_four<kAll>(static_cast<float*>(it.m), at, n);
+            v32[u] = load_four<kAll>(static_cast<float*>(it.v), at, n);
           }
-          const float x = G::widen(rg[u].v[j]) * factor;
-          m[j] = m[j] * a.b1 + x * a.c1;
-          v[j] = v[j] * a.b2 + (x * x) * a.c2;
-          const float to = m[j] / (sqrtf(v[j]) * root + a.eps);
-          wide.v[j] = P::widen(rp[u].v[j]) * a.decay - to * rate;
-          np.v[j] = P::narrow(wide.v[j]);
         }
-        store_four(p, at, n, whole, np);
-        if (it.copy) {
-          if (a.copy_dtype == CP4_DTYPE_F32) {
-            store_four(static_cast<float*>(it.copy), at, n, whole, wide);
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+          const size_t at = at0 + u * kBlock + lane * 4;
+          float m[4], v[4];
+          Four<RawP> np;
+          Four<float> wide;
+          const float um = Eight ? sm[u] * kUnitM : 0.0f, uv = Eight ? sv[u] * kUnitV : 0.0f;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if constexpr (Eight) {
+              m[j] = decode_m(m8[u].v[j], um);
+              v[j] = decode_v(v8[u].v[j], uv);
+            } else {
+              m[j] = m32[u].v[j];
+              v[j] = v32[u].v[j];
+            }
+            const float x = G::widen(rg[u].v[j]) * factor;
+            m[j] = m[j] * a.b1 + x * a.c1;
+            v[j] = v[j] * a.b2 + (x * x) * a.c2;
+            const float to = m[j] / (sqrtf(v[j]) * root + a.eps);
+            wide.v[j] = P::widen(rp[u].v[j]) * a.decay - to * rate;
+            np.v[j] = P::narrow(wide.v[j]);
+          }
+          store_four<kAll>(p, at, n, np);
+          if (it.copy) {
+            if (a.copy_dtype == CP4_DTYPE_F32) {
+              store_four<kAll>(static_cast<float*>(it.copy), at, n, wide);
+            } else {
+              Four<unsigned short> h;
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                h.v[j] = a.copy_dtype == CP4_DTYPE_BF16 ? BF16::narrow(wide.v[j]) : F16::narrow(wide.v[j]);
+              store_four<kAll>(static_cast<unsigned short*>(it.copy), at, n, h);
+            }
+          }
+          if constexpr (Eight) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)              // (what lies beyond a NaN scale's block is not there)
+              if (!kAll && at + j >= n) m[j] = v[j] = 0.0f;
+            Four<signed char> qm;
+            Four<unsigned char> qv;
+            float tm, tv;
+            encode_block(m, v, qm, qv, tm, tv);
+            store_four<kAll>(static_cast<signed char*>(it.m), at, n, qm);
+            store_four<kAll>(static_cast<unsigned char*>(it.v), at, n, qv);
+            if (lane == 0 && (kAll || at0 + u * kBlock < n)) {
+              it.s[(at0 + u * kBlock) / kBlock] = tm;
+              it.s2[(at0 + u * kBlock) / kBlock] = tv;
+            }
           } else {
-            Four<unsigned short> h;
+            Four<float> o;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              h.v[j] = a.copy_dtype == CP4_DTYPE_BF16 ? BF16::narrow(wide.v[j]) : F16::narrow(wide.v[j]);
-            store_four(static_cast<unsigned short*>(it.copy), at, n, whole, h);
+            for (int j = 0; j < 4; ++j) o.v[j] = m[j];
+            store_four<kAll>(static_cast<float*>(it.m), at, n, o);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o.v[j] = v[j];
+            store_four<kAll>(static_cast<float*>(it.v), at, n, o);
           }
         }
-        if constexpr (Eight) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)              // (what lies beyond a NaN scale's block is not there)
-            if (at + j >= n) m[j] = v[j] = 0.0f;
-          Four<signed char> qm;
-          Four<unsigned char> qv;
-          float tm, tv;
-          encode_block(m, v, qm, qv, tm, tv);
-          store_four(static_cast<signed char*>(it.m), at, n, whole, qm);
-          store_four(static_cast<unsigned char*>(it.v), at, n, whole, qv);
-          if (lane == 0 && at0 + u * kBlock < n) {
-            it.s[(at0 + u * kBlock) / kBlock] = tm;
-            it.s2[(at0 + u * kBlock) / kBlock] = tv;
-          }
-        } else {
-          Four<float> o;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) o.v[j] = m[j];
-          store_four(static_cast<float*>(it.m), at, n, whole, o);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) o.v[j] = v[j];
-          store_four(static_cast<float*>(it.v), at, n, whole, o);
-        }
-      }
+      };
+      if (at0 + kChunk <= n) turn(std::true_type());
+      else turn(std::false_type());
     }
   }
   __syncthreads();
@@ -328,38 +319,49 @@ __device__ __forceinline__ double block_sum(double x, double* lds) {
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
   __syncthreads();
   double sum = 0.0;
-  for (unsigned w = 0; w < kWaves; ++w) sum += lds[w];
+  for (unsigned w = 0; w < kNormWaves; ++w) sum += lds[w];
   return sum;
 }
 
 // The squares' sum in 64 bits: a partial sum a workgroup, added up in their order by the workgroup that
 // is done last, so that the norm does not depend on which that is.
 template <class G>
-__global__ __launch_bounds__(64 * kWaves, 4) void norm_kernel(const NormArgs a) {
+__global__ __launch_bounds__(64 * kNormWaves, 8) void norm_kernel(const NormArgs a) {
   typedef typename G::raw Raw;
-  __shared__ double lds[kWaves];
+  __shared__ double lds[kNormWaves];
   __shared__ bool last;
   const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   double sum = 0.0;
-  for (unsigned c = blockIdx.x * kWaves + wave; c < a.chunks; c += gridDim.x * kWaves) {
+  auto fetch = [&](unsigned c, Four<Raw> (&r)[kUnroll]) __attribute__((always_inline)) {
     const int t = tensor_of(a, c);
     const unsigned end = t + 1 < a.count ? a.first[t + 1] : a.chunks;
     const size_t n = (size_t)(end - 1 - a.first[t]) * kChunk + a.left[t], at0 = (size_t)(c - a.first[t]) * kChunk;
     const Raw* const g = static_cast<const Raw*>(a.g[t]);
-    const bool even = aligned_four(g);
-    Four<Raw> r[kUnroll];
+    const bool all = at0 + kChunk <= n;
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const size_t at = at0 + u * kBlock + lane * 4;
-      r[u] = load_four(g, at, n, even && at + 4 <= n);
+      r[u] = all ? load_four<true>(g, at, n) : load_four<false>(g, at, n);
     }
+  };
+  // (a turn's loads are on their way while the last one's are summed)
+  const unsigned stride = gridDim.x * kNormWaves;
+  unsigned c = blockIdx.x * kNormWaves + wave;
+  Four<Raw> r[kUnroll];
+  if (c < a.chunks) fetch(c, r);
+  while (c < a.chunks) {
+    Four<Raw> next[kUnroll] = {};
+    c += stride;
+    if (c < a.chunks) fetch(c, next);
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
+    for (int u = 0; u < kUnroll; ++u) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const double x = (double)G::widen(r[u].v[j]);
         sum += x * x;
       }
+      r[u] = next[u];
+    }
   }
   sum = block_sum(sum, lds);
   if (threadIdx.x == 0) {
@@ -374,7 +376,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void norm_kernel(const NormArgs a) 
   __syncthreads();
   if (!last) return;
   sum = 0.0;
-  for (unsigned i = threadIdx.x; i < a.parts; i += 64 * kWaves)
+  for (unsigned i = threadIdx.x; i < a.parts; i += 64 * kNormWaves)
     sum += __hip_atomic_load(a.partial + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
   sum = block_sum(sum, lds);
@@ -409,50 +411,53 @@ __global__ __launch_bounds__(64 * kWaves, 4) void moments_kernel(const MomentArg
     const int t = tensor_of(a, c);
     const MomentItem& it = a.item[t];
     const size_t n = it.n, at0 = (size_t)(c - a.first[t]) * kChunk;
-    const bool even = (((size_t)it.m | (size_t)it.v) & 3) == 0 && (((size_t)it.to_m | (size_t)it.to_v) & 15) == 0;
     signed char* const m8 = static_cast<signed char*>(it.m);
     unsigned char* const v8 = static_cast<unsigned char*>(it.v);
-    Four<signed char> qm[kUnroll];
-    Four<unsigned char> qv[kUnroll];
-    Four<float> fm[kUnroll], fv[kUnroll];
-    float um[kUnroll], uv[kUnroll];
+    auto turn = [&](auto all) __attribute__((always_inline)) {
+      constexpr bool kAll = decltype(all)::value;
+      Four<signed char> qm[kUnroll];
+      Four<unsigned char> qv[kUnroll];
+      Four<float> fm[kUnroll], fv[kUnroll];
+      float um[kUnroll], uv[kUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const size_t at = at0 + u * kBlock + lane * 4, b = at0 / kBlock + u;
-      const bool whole = even && at + 4 <= n, there = at0 + u * kBlock < n;
-      if constexpr (Encode) {
-        fm[u] = load_four(it.to_m, at, n, whole);
-        fv[u] = load_four(it.to_v, at, n, whole);
-      } else {
-        qm[u] = load_four(m8, at, n, whole);
-        qv[u] = load_four(v8, at, n, whole);
-        um[u] = there ? it.s[b] * kUnitM : 0.0f;
-        uv[u] = there ? it.s2[b] * kUnitV : 0.0f;
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const size_t at = at0 + u * kBlock + lane * 4, b = at0 / kBlock + u;
-      const bool whole = even && at + 4 <= n;
-      if constexpr (Encode) {
-        float tm, tv;
-        encode_block(fm[u].v, fv[u].v, qm[u], qv[u], tm, tv);
-        store_four(m8, at, n, whole, qm[u]);
-        store_four(v8, at, n, whole, qv[u]);
-        if (lane == 0 && at0 + u * kBlock < n) {
-          it.s[b] = tm;
-          it.s2[b] = tv;
+      for (int u = 0; u < kUnroll; ++u) {
+        const size_t at = at0 + u * kBlock + lane * 4, b = at0 / kBlock + u;
+        const bool there = kAll || at0 + u * kBlock < n;
+        if constexpr (Encode) {
+          fm[u] = load_four<kAll>(it.to_m, at, n);
+          fv[u] = load_four<kAll>(it.to_v, at, n);
+        } else {
+          qm[u] = load_four<kAll>(m8, at, n);
+          qv[u] = load_four<kAll>(v8, at, n);
+          um[u] = there ? it.s[b] * kUnitM : 0.0f;
+          uv[u] = there ? it.s2[b] * kUnitV : 0.0f;
         }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          fm[u].v[j] = decode_m(qm[u].v[j], um[u]);
-          fv[u].v[j] = decode_v(qv[u].v[j], uv[u]);
-        }
-        store_four(it.to_m, at, n, whole, fm[u]);
-        store_four(it.to_v, at, n, whole, fv[u]);
       }
-    }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const size_t at = at0 + u * kBlock + lane * 4, b = at0 / kBlock + u;
+        if constexpr (Encode) {
+          float tm, tv;
+          encode_block(fm[u].v, fv[u].v, qm[u], qv[u], tm, tv);
+          store_four<kAll>(m8, at, n, qm[u]);
+          store_four<kAll>(v8, at, n, qv[u]);
+          if (lane == 0 && (kAll || at0 + u * kBlock < n)) {
+            it.s[b] = tm;
+            it.s2[b] = tv;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            fm[u].v[j] = decode_m(qm[u].v[j], um[u]);
+            fv[u].v[j] = decode_v(qv[u].v[j], uv[u]);
+          }
+          store_four<kAll>(it.to_m, at, n, fm[u]);
+          store_four<kAll>(it.to_v, at, n, fv[u]);
+        }
+      }
+    };
+    if (at0 + kChunk <= n) turn(std::true_type());
+    else turn(std::false_type());
   }
 }
 
@@ -461,8 +466,8 @@ __global__ __launch_bounds__(64 * kWaves, 4) void moments_kernel(const MomentArg
 using cp4::fail_hip;
 using cp4::fail_with;
 
-unsigned grid_for(size_t chunks, unsigned most) {
-  return (unsigned)std::max<size_t>(1, std::min<size_t>((chunks + kWaves - 1) / kWaves, most));
+unsigned grid_for(size_t chunks, unsigned most, unsigned waves = kWaves) {
+  return (unsigned)std::max<size_t>(1, std::min<size_t>((chunks + waves - 1) / waves, most));
 }
 size_t chunks_of(size_t n) { return (n + kChunk - 1) / kChunk; }
 bool dtype_ok(int d) { return d == CP4_DTYPE_F32 || d == CP4_DTYPE_BF16 || d == CP4_DTYPE_F16; }
@@ -619,9 +624,9 @@ extern "C" cp4_status cp4_adamw_step(const cp4_adamw_tensor* t, size_t count, co
                             [](auto& x, auto& y) { return x.grad_dtype == y.grad_dtype; });
     if (runs.empty()) runs.emplace_back();
     if (runs.size() > kMostParts) return fail_with(CP4_ERR_SHAPE, "too many tensors");
-    const unsigned each = std::max(1u, std::min<unsigned>(most, kMostParts / (unsigned)runs.size()));
+    const unsigned each = std::max(1u, std::min<unsigned>(2 * cp4::num_compute_units(), kMostParts / (unsigned)runs.size()));
     unsigned parts = 0;
-    for (const Launch& run : runs) parts += grid_for(run.chunks, each);
+    for (const Launch& run : runs) parts += grid_for(run.chunks, each, kNormWaves);
     unsigned part = 0;
     for (const Launch& run : runs) {
       NormArgs a{};
@@ -641,12 +646,12 @@ extern "C" cp4_status cp4_adamw_step(const cp4_adamw_tensor* t, size_t count, co
       a.norm = norm;
       a.scale = grad_scale;
       a.max_norm = max_norm;
-      const unsigned grid = grid_for(chunks, each);
+      const unsigned grid = grid_for(chunks, each, kNormWaves);
       part += grid;
       const int g = run.tensors.empty() ? CP4_DTYPE_F32 : t[run.tensors[0]].grad_dtype;
-      if (g == CP4_DTYPE_F32) norm_kernel<F32><<<grid, 64 * kWaves, 0, st>>>(a);
-      else if (g == CP4_DTYPE_BF16) norm_kernel<BF16><<<grid, 64 * kWaves, 0, st>>>(a);
-      else norm_kernel<F16><<<grid, 64 * kWaves, 0, st>>>(a);
+      if (g == CP4_DTYPE_F32) norm_kernel<F32><<<grid, 64 * kNormWaves, 0, st>>>(a);
+      else if (g == CP4_DTYPE_BF16) norm_kernel<BF16><<<grid, 64 * kNormWaves, 0, st>>>(a);
+      else norm_kernel<F16><<<grid, 64 * kNormWaves, 0, st>>>(a);
       if (const hipError_t e = hipGetLastError()) return fail_hip(e, "cp4_adamw_step");
     }
   }
