@@ -674,23 +674,36 @@ PyObject* adapter_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 // ---- AdamW over many tensors (optim.py) --------------------------------------------------------
 
-// The tensors of a list or tuple; None stays undefined (where `holes`).
-std::vector<Tensor> tensors(PyObject* o, size_t count, const char* what, bool holes = false) {
-  std::vector<Tensor> out(count);
-  if (o == Py_None && holes) return out;
-  PyObject* seq = PySequence_Fast(o, "expected a list of tensors");
-  if (!seq) throw python_error();
-  const bool fits = (size_t)PySequence_Fast_GET_SIZE(seq) == count;
-  bool good = fits;
-  for (size_t i = 0; good && i < count; ++i) {
-    PyObject* v = PySequence_Fast_GET_ITEM(seq, i);
-    if (THPVariable_Check(v)) out[i] = THPVariable_Unpack(v);
-    else good = holes && v == Py_None;
+// The tensors of a list or tuple, held by a tuple of their own (a Tensor's count of owners is an atomic: 65
+// parameters with their gradients and moments cost 6 us of those); where there may be holes, None is none.
+class TensorList {
+ public:
+  TensorList(PyObject* o, size_t count, const char* what, bool holes = false) : count_(count) {
+    if (o == Py_None && holes) return;
+    items_ = PySequence_Tuple(o);
+    if (!items_) throw python_error();
+    bool good = (size_t)PyTuple_GET_SIZE(items_) == count;
+    for (size_t i = 0; good && i < count; ++i) {
+      PyObject* v = PyTuple_GET_ITEM(items_, i);
+      good = THPVariable_Check(v) || (holes && v == Py_None);
+    }
+    if (!good) {
+      Py_CLEAR(items_);
+      fail(PyExc_AssertionError, what);
+    }
   }
-  Py_DECREF(seq);
-  require(good, what);
-  return out;
-}
+  ~TensorList() { Py_XDECREF(items_); }              // (with the interpreter lock)
+  TensorList(const TensorList&) = delete;
+  TensorList& operator=(const TensorList&) = delete;
+  bool has(size_t i) const { return items_ && PyTuple_GET_ITEM(items_, i) != Py_None; }
+  const Tensor& operator[](size_t i) const { return has(i) ? THPVariable_Unpack(PyTuple_GET_ITEM(items_, i)) : none_; }
+  size_t size() const { return count_; }
+
+ private:
+  PyObject* items_ = nullptr;
+  size_t count_;
+  Tensor none_;
+};
 size_t length(PyObject* o) {
   const Py_ssize_t n = PySequence_Size(o);
   if (n < 0) throw python_error();
@@ -722,9 +735,9 @@ void moments_of(cp4_adamw_tensor& t, const Tensor& m, const Tensor& v, const Ten
   t.scale_sq = t.scale + scales.stride(0);
 }
 // What autograd has saved of a tensor that is written here is out of date.
-void written(const std::vector<Tensor>& list) {
-  for (const Tensor& t : list)
-    if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+void written(const TensorList& list) {
+  for (size_t i = 0; i < list.size(); ++i)
+    if (list.has(i) && !list[i].is_inference()) list[i].unsafeGetTensorImpl()->bump_version();
 }
 
 // (params, grads, exp_avgs, exp_avg_sqs, scales, copies, group of each or None,
@@ -733,11 +746,10 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
   require(n_args == 11);
   const size_t n = length(a[0]), n_groups = length(a[7]);
-  const auto params = tensors(a[0], n, "expected a list of tensors");
-  const auto grads = tensors(a[1], n, "one gradient a parameter", true);
-  const auto ms = tensors(a[2], n, "one first moment a parameter"), vs = tensors(a[3], n, "one second moment a parameter");
-  const auto scales = tensors(a[4], n, "one pair of scales (or None) a parameter", true);
-  const auto copies = tensors(a[5], n, "one copy (or None) a parameter", true);
+  const TensorList params(a[0], n, "expected a list of tensors"), grads(a[1], n, "one gradient a parameter", true);
+  const TensorList ms(a[2], n, "one first moment a parameter"), vs(a[3], n, "one second moment a parameter");
+  const TensorList scales(a[4], n, "one pair of scales (or None) a parameter", true);
+  const TensorList copies(a[5], n, "one copy (or None) a parameter", true);
   std::vector<cp4_adamw_group> groups(n_groups);
   std::vector<Tensor> counters(n_groups);
   PyObject* seq = PySequence_Fast(a[7], "expected a list of groups");
@@ -765,14 +777,14 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   std::vector<cp4_adamw_tensor> list;
   list.reserve(n);
   for (size_t i = 0; i < n; ++i) {
-    if (!grads[i].defined()) continue;
+    if (!grads.has(i)) continue;
     cp4_adamw_tensor t{};
     t.n = (size_t)params[i].numel();
     t.param = dense(params[i], (int64_t)t.n, like, "a parameter is not a contiguous tensor on the counter's device");
     t.param_dtype = dtype_of(params[i]);
     t.grad = dense(grads[i], (int64_t)t.n, like, "a gradient does not match its parameter");
     t.grad_dtype = dtype_of(grads[i]);
-    if (copies[i].defined()) {
+    if (copies.has(i)) {
       t.copy = dense(copies[i], (int64_t)t.n, like, "a copy does not match its parameter");
       t.copy_dtype = dtype_of(copies[i]);
     }
@@ -806,9 +818,10 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     }
     check(cp4_adamw_step(list.data(), list.size(), groups.data(), n_groups, (float)grad_scale, (float)max_norm,
                          static_cast<float*>(ptr(norm)), ptr(ws), need, st));
-    for (const auto* l : {&params, &ms, &vs, &scales, &copies}) written(*l);
-    written(counters);
   }
+  for (const auto* l : {&params, &ms, &vs, &scales, &copies}) written(*l);
+  for (const Tensor& c : counters)
+    if (!c.is_inference()) c.unsafeGetTensorImpl()->bump_version();
   if (!norm.defined()) Py_RETURN_NONE;
   return THPVariable_Wrap(std::move(norm));
   END_HANDLE_TH_ERRORS
@@ -819,9 +832,9 @@ PyObject* adamw_moments(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
   require(n_args == 7);
   const size_t n = length(a[0]);
-  const auto ms = tensors(a[0], n, "expected a list of tensors"), vs = tensors(a[1], n, "one second moment a first");
-  const auto scales = tensors(a[2], n, "one pair of scales a moment");
-  const auto to_m = tensors(a[3], n, "one tensor of values a moment"), to_v = tensors(a[4], n, "one tensor of values a moment");
+  const TensorList ms(a[0], n, "expected a list of tensors"), vs(a[1], n, "one second moment a first");
+  const TensorList scales(a[2], n, "one pair of scales a moment");
+  const TensorList to_m(a[3], n, "one tensor of values a moment"), to_v(a[4], n, "one tensor of values a moment");
   const bool encode = PyObject_IsTrue(a[5]) == 1;
   if (!n) Py_RETURN_NONE;
   std::vector<cp4_adamw_tensor> list(n);
@@ -838,14 +851,13 @@ PyObject* adamw_moments(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   void* st = stream_of(a[6]);
   {
     NoGil unlocked;
-    if (encode) {
-      check(cp4_adamw_set_moments(list.data(), n, pm.data(), pv.data(), st));
-      for (const auto* l : {&ms, &vs, &scales}) written(*l);
-    } else {
-      check(cp4_adamw_moments(list.data(), n, pm.data(), pv.data(), st));
-      for (const auto* l : {&to_m, &to_v}) written(*l);
-    }
+    check(encode ? cp4_adamw_set_moments(list.data(), n, pm.data(), pv.data(), st)
+                 : cp4_adamw_moments(list.data(), n, pm.data(), pv.data(), st));
   }
+  if (encode)
+    for (const auto* l : {&ms, &vs, &scales}) written(*l);
+  else
+    for (const auto* l : {&to_m, &to_v}) written(*l);
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
