@@ -38,6 +38,7 @@ struct ProjectArgs {
   int fn, fr;
   int planes;             // h is the sum of so many planes ...
   size_t plane;           // ... so many values apart (more than one: only where project_sums_planes)
+  float* keep;            // with planes > 1: where their sum goes as well, or null
 };
 
 // out[a][r][c] = sum over tokens with ids[t] = a of p[t][r] z[t][c], at out + a * R * C + r * outr +
@@ -62,7 +63,7 @@ hipError_t planes_join(float* h, const float* from, size_t n, int planes, hipStr
 // Whether the projection that these operands get adds up the planes of h itself.
 bool project_sums_planes(const ProjectArgs&, int dtype, bool nn);
 // part: project_part_bytes of scratch memory.
-size_t project_part_bytes(size_t T, int K, int N, int dtype);
+size_t project_part_bytes(size_t T, int K, int N, int G, int dtype, bool nn);
 hipError_t project_launch(const ProjectArgs&, float* part, int dtype, bool nn, hipStream_t);
 // The tiles of a projection on the matrix cores, its depth in `splits` parts of `each` steps, whose partial
 // sums take tile_part_bytes.
@@ -70,7 +71,7 @@ struct TilePlan {
   int which, splits, each;
   double cost;            // microseconds, about
 };
-TilePlan tile_plan(size_t T, int K, int N, int dtype, bool direct);
+TilePlan tile_plan(size_t T, int K, int N, int dtype, bool nn, bool direct);
 size_t tile_part_bytes(const TilePlan&, size_t T, int N);
 // Whether these operands go from memory to the LDS without passing a register.
 bool tile_direct(const ProjectArgs&, int dtype, bool nn);
@@ -80,6 +81,7 @@ hipError_t parts_join(const float* part, const float* bias, void* y, size_t T, i
 // Up to 64 tokens in 16 bits, 32 in fp32 (w [N][K]).  splits 0: not for this kernel.
 struct RowsPlan {
   int splits;
+  double cost, adapter;   // microseconds, about, and for each adapter
 };
 RowsPlan rows_plan(size_t T, int K, int N, int dtype);
 hipError_t rows_launch(const ProjectArgs&, const RowsPlan&, float* part, int dtype, hipStream_t);

@@ -21,7 +21,7 @@ cp4_status check_shape(const cp4_adapter_shape* s, int dtype) {
   if (s->R > 256) return fail_with(CP4_ERR_SHAPE, "adapters of a rank above 256");
   if (s->G > 65535) return fail_with(CP4_ERR_SHAPE, "more than 65535 adapters");
   if (s->K > 1u << 22 || s->N > 1u << 22) return fail_with(CP4_ERR_SHAPE, "K or N above 2^22");
-  if (s->T > (size_t)1 << 31) return fail_with(CP4_ERR_SHAPE, "more than 2^31 tokens");
+  if (s->T > (size_t)1 << 26) return fail_with(CP4_ERR_SHAPE, "more than 2^26 tokens");
   if ((s->ldx && s->ldx < s->K) || (s->ldw && s->ldw < s->K) || (s->lddy && s->lddy < s->N))
     return fail_with(CP4_ERR_SHAPE, "a row stride is smaller than the row");
   if (std::max({s->ldx, s->ldw, s->lddy}) > (size_t)1 << 30)
@@ -50,7 +50,7 @@ BackwardPlan backward_plan(const cp4_adapter_shape& s, int dtype) {
   p.part_at = align256(p.dh_planes * h_bytes(s));
   p.part_b = p.splits > 1 ? (size_t)p.splits * s.G * s.R * s.K : 0;
   const size_t parts = p.splits > 1 ? (p.part_b + (size_t)p.splits * s.G * s.R * s.N) * 4 : 0;
-  p.total = p.part_at + align256(std::max(parts, project_part_bytes(s.T, (int)s.N, (int)s.K, dtype)));  // (one after the other)
+  p.total = p.part_at + align256(std::max(parts, project_part_bytes(s.T, (int)s.N, (int)s.K, (int)s.G, dtype, true)));  // (one after the other)
   return p;
 }
 
@@ -62,7 +62,7 @@ extern "C" size_t cp4_adapter_kept_bytes(const cp4_adapter_shape* s, int dtype) 
 
 extern "C" size_t cp4_adapter_forward_workspace_bytes(const cp4_adapter_shape* s, int dtype) {
   if (check_shape(s, dtype) != CP4_OK) return 0;
-  return align256(shrink_planes(s->T, (int)s->K, dtype) * h_bytes(*s)) + align256(project_part_bytes(s->T, (int)s->K, (int)s->N, dtype));
+  return align256(shrink_planes(s->T, (int)s->K, dtype) * h_bytes(*s)) + align256(project_part_bytes(s->T, (int)s->K, (int)s->N, (int)s->G, dtype, false));
 }
 
 extern "C" cp4_status cp4_adapter_forward(const cp4_adapter_shape* s, int dtype, const void* x, const void* W,
@@ -91,7 +91,9 @@ extern "C" cp4_status cp4_adapter_forward(const cp4_adapter_shape* s, int dtype,
   p.T = s->T; p.ldz = sh.ldz; p.ldw = s->ldw ? s->ldw : s->K;
   p.K = (int)s->K; p.N = (int)s->N; p.R = (int)s->R; p.Rp = sh.Rp; p.G = (int)s->G;
   p.fn = (int)s->R; p.fr = 1; p.planes = sh.planes; p.plane = p.T * p.Rp;
-  if (p.planes > 1 && (kept || !project_sums_planes(p, dtype, false))) {
+  if (p.planes > 1 && project_sums_planes(p, dtype, false)) {
+    p.keep = kept;
+  } else if (p.planes > 1) {
     float* const h = kept ? kept : planes;
     if (const hipError_t e = planes_join(h, planes, p.plane, p.planes, st)) return fail_hip(e, "cp4_adapter_forward");
     p.h = h;

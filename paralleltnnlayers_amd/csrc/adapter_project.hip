@@ -7,20 +7,30 @@ namespace cp4 {
 namespace adapter {
 namespace {
 
+// The rows kernel or tiles, for tokens that both take.  A tile takes its adapters a few at a time, some 0.6 us each
+// (fp32: 1.2), the rows kernel's waves share them; how many different ones there are only the device knows: at most G.
+// (bf16, 4096 x 4096, rank 16, rows kernel and tiles: 20 tokens of 2 adapters 17 us and 21, of 20 adapters 26 and 40; 64 tokens of
+// 2 adapters 26 and 22, of 64 adapters 42 and 55; 4096 x 14336, 20 tokens of 2 adapters 50 and 33.)
+bool by_rows(size_t T, int K, int N, int G, int dtype, bool nn, bool direct) {
+  const RowsPlan rows = nn ? RowsPlan{} : rows_plan(T, K, N, dtype);
+  if (!rows.splits || T <= 16) return rows.splits;                   // (up to 16 tokens: within 8 % of the tiles at worst)
+  const double adapters = (double)std::min<size_t>(T, G);
+  return rows.cost + rows.adapter * adapters <=
+         tile_plan(T, K, N, dtype, nn, direct).cost + (dtype == CP4_DTYPE_F32 ? 1.2 : 0.6) * adapters;
+}
+
 // Rows of the tiles' launch; the rest, less than a tile's, is cheaper on its own where it would take a round of
 // tiles of its own.
-size_t main_rows(size_t T, int K, int N, int dtype, bool nn, bool direct) {
-  const TilePlan all = tile_plan(T, K, N, dtype, direct);
+size_t main_rows(size_t T, int K, int N, int G, int dtype, bool nn, bool direct) {
+  if (T <= 256) return T;
   size_t best = T;
-  double least = all.cost;
+  double least = tile_plan(T, K, N, dtype, nn, direct).cost;
   for (size_t tile : {256, 128}) {
     const size_t rest = T % tile;
     if (!rest || T <= 2 * tile) continue;
-    // (the rest's own launches: some microseconds, and W once more)
-    const bool rows = !nn && rows_plan(rest, K, N, dtype).splits;
-    const double w = (double)K * N * (dtype == CP4_DTYPE_F32 ? 4 : 2) / 3.0e6;
-    const double cost = tile_plan(T - rest, K, N, dtype, direct).cost + 4.0 +
-                        (rows ? 6.0 + w : std::max(w, tile_plan(rest, K, N, dtype, direct).cost));
+    const double other = by_rows(rest, K, N, G, dtype, nn, direct) ? rows_plan(rest, K, N, dtype).cost
+                                                                   : tile_plan(rest, K, N, dtype, nn, direct).cost;
+    const double cost = tile_plan(T - rest, K, N, dtype, nn, direct).cost + other + 6.0;    // (a launch and its start)
     if (cost < least) {
       least = cost;
       best = T - rest;
@@ -29,40 +39,39 @@ size_t main_rows(size_t T, int K, int N, int dtype, bool nn, bool direct) {
   return best;
 }
 
-size_t plan_bytes(size_t T, int K, int N, int dtype, bool direct) {
-  const RowsPlan rows = rows_plan(T, K, N, dtype);
-  return std::max(tile_part_bytes(tile_plan(T, K, N, dtype, direct), T, N),
-                  rows.splits > 1 ? (size_t)rows.splits * T * N * 4 : 0);
-}
-
 hipError_t launch(const ProjectArgs& a, float* part, int dtype, bool nn, bool direct, hipStream_t st) {
-  const RowsPlan rows = nn ? RowsPlan{} : rows_plan(a.T, a.K, a.N, dtype);
-  if (rows.splits) return rows_launch(a, rows, part, dtype, st);
-  return tile_launch(a, tile_plan(a.T, a.K, a.N, dtype, direct), part, dtype, nn, st);
+  if (by_rows(a.T, a.K, a.N, a.G, dtype, nn, direct)) return rows_launch(a, rows_plan(a.T, a.K, a.N, dtype), part, dtype, st);
+  return tile_launch(a, tile_plan(a.T, a.K, a.N, dtype, nn, direct), part, dtype, nn, st);
 }
 
 }  // namespace
 
-size_t project_part_bytes(size_t T, int K, int N, int dtype) {
+// Enough for each choice that the operands' alignment makes.
+size_t project_part_bytes(size_t T, int K, int N, int G, int dtype, bool nn) {
   size_t most = 0;
+  const auto part = [&](size_t rows, bool direct) {
+    const RowsPlan few = rows_plan(rows, K, N, dtype);
+    if (by_rows(rows, K, N, G, dtype, nn, direct)) most = std::max(most, few.splits > 1 ? few.splits * rows * N * 4 : 0);
+    else most = std::max(most, tile_part_bytes(tile_plan(rows, K, N, dtype, nn, direct), rows, N));
+  };
   for (bool direct : {false, true}) {
-    most = std::max(most, plan_bytes(T, K, N, dtype, direct));
-    for (bool nn : {false, true}) {
-      const size_t main = main_rows(T, K, N, dtype, nn, direct);
-      if (main < T)
-        most = std::max({most, plan_bytes(main, K, N, dtype, direct), plan_bytes(T - main, K, N, dtype, direct)});
-    }
+    if (direct && dtype == CP4_DTYPE_F32) break;                     // (the same plans)
+    const size_t main = main_rows(T, K, N, G, dtype, nn, direct);
+    part(T, direct);
+    if (main == T) continue;
+    part(main, direct);
+    part(T - main, direct);
   }
   return most;
 }
 
 bool project_sums_planes(const ProjectArgs& a, int dtype, bool nn) {
-  return !nn && rows_plan(a.T, a.K, a.N, dtype).splits;
+  return by_rows(a.T, a.K, a.N, a.G, dtype, nn, tile_direct(a, dtype, nn));
 }
 
 hipError_t project_launch(const ProjectArgs& a, float* part, int dtype, bool nn, hipStream_t st) {
   const bool direct = tile_direct(a, dtype, nn);
-  const size_t main = project_sums_planes(a, dtype, nn) ? a.T : main_rows(a.T, a.K, a.N, dtype, nn, direct);
+  const size_t main = main_rows(a.T, a.K, a.N, a.G, dtype, nn, direct);
   if (main == a.T) return launch(a, part, dtype, nn, direct, st);
   const size_t e = dtype == CP4_DTYPE_F32 ? 4 : 2;
   ProjectArgs first = a, rest = a;

@@ -40,15 +40,19 @@ __device__ __forceinline__ void load_row(const Raw* p, int left, bool full, u32x
 template <class T, bool TR, int RB>
 __global__ __launch_bounds__(64 * kWaves) void shrink_kernel(const ShrinkArgs a) {
   typedef typename T::raw Raw;
-  constexpr int n = 16 / sizeof(Raw), U = kUnit<T>, MB = 1, kRows = 16 * MB;
+  constexpr int n = 16 / sizeof(Raw), U = kUnit<T>, kRows = 16;
   __shared__ float sum[kWaves][16][16 * RB + 4];
   __shared__ int own[kRows];
+  __shared__ float factor[kRows];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 15, g = lane >> 4;
   const size_t t0 = (size_t)blockIdx.x * kRows;
   const int rows = (int)min((size_t)kRows, a.T - t0);
   int id = lane < rows ? a.ids[t0 + lane] : -1;
   if (id < 0 || id >= a.G) id = -1;
-  if (threadIdx.x < kRows) own[lane] = id;
+  if (threadIdx.x < kRows) {
+    own[lane] = id;
+    factor[lane] = a.scale && id >= 0 ? a.scale[id] : 1.0f;
+  }
   int different = 0;
   {
     Adapters each(id);
@@ -66,23 +70,20 @@ __global__ __launch_bounds__(64 * kWaves) void shrink_kernel(const ShrinkArgs a)
   const int first = min(u1, u0 + slice * each), last = min(u1, first + each);
   const int whole = min(last, a.K / U);                              // (from there on a turn has fewer inputs)
 
-  const Raw* z[MB];
-#pragma unroll
-  for (int i = 0; i < MB; ++i) z[i] = static_cast<const Raw*>(a.z) + (t0 + min(16 * i + l, rows - 1)) * a.ldz + n * g;
+  const Raw* const z = static_cast<const Raw*>(a.z) + (t0 + min(l, rows - 1)) * a.ldz + n * g;
 
   for (int r0 = 0; r0 < a.Rp; r0 += 16 * RB) {
-    f32x4 acc[MB][RB] = {};
+    f32x4 acc[RB] = {};
     Adapters todo(id);
     int ad, turn = 0;
     unsigned long long whose;
     while (todo.take(ad, whose)) {
       if ((turn++ & (ways - 1)) != mine) continue;
       const Raw* const f = static_cast<const Raw*>(a.f) + (size_t)ad * a.R * a.K;
-      f32x4 d[MB][RB] = {};
-      auto load = [&](int u, bool full, u32x4 (&zv)[MB][2], u32x4 (&fv)[RB][2]) __attribute__((always_inline)) {
+      f32x4 d[RB] = {};
+      auto load = [&](int u, bool full, u32x4 (&zv)[2], u32x4 (&fv)[RB][2]) __attribute__((always_inline)) {
         const int k = u * U + n * g, left = full ? U : a.K - k;
-#pragma unroll
-        for (int i = 0; i < MB; ++i) load_row(z[i] + (size_t)u * U, left, full, zv[i]);
+        load_row(z + (size_t)u * U, left, full, zv);
         if constexpr (!TR) {
 #pragma unroll
           for (int j = 0; j < RB; ++j) {
@@ -109,26 +110,23 @@ __global__ __launch_bounds__(64 * kWaves) void shrink_kernel(const ShrinkArgs a)
           }
         }
       };
-      auto multiply = [&](const u32x4 (&zv)[MB][2], const u32x4 (&fv)[RB][2]) __attribute__((always_inline)) {
+      auto multiply = [&](const u32x4 (&zv)[2], const u32x4 (&fv)[RB][2]) __attribute__((always_inline)) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int j = 0; j < RB; ++j)
+          for (int j = 0; j < RB; ++j) {
+            if constexpr (__is_same(T, F32)) {
 #pragma unroll
-            for (int i = 0; i < MB; ++i) {
-              if constexpr (__is_same(T, F32)) {
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                  d[i][j] = mfma_f32(__uint_as_float(zv[i][h][q]), __uint_as_float(fv[j][h][q]), d[i][j]);
-              } else {
-                d[i][j] = mfma_16<T>(__builtin_bit_cast(u16x8, zv[i][h]), __builtin_bit_cast(u16x8, fv[j][h]), d[i][j]);
-              }
+              for (int q = 0; q < 4; ++q) d[j] = mfma_f32(__uint_as_float(zv[h][q]), __uint_as_float(fv[j][h][q]), d[j]);
+            } else {
+              d[j] = mfma_16<T>(__builtin_bit_cast(u16x8, zv[h]), __builtin_bit_cast(u16x8, fv[j][h]), d[j]);
             }
+          }
       };
       constexpr int kAhead = RB <= 2 ? 4 : 2;                   // turns whose loads come before their products
       int u = first;
       for (; u + kAhead <= whole; u += kAhead) {
-        u32x4 zv[kAhead][MB][2], fv[kAhead][RB][2];
+        u32x4 zv[kAhead][2], fv[kAhead][RB][2];
 #pragma unroll
         for (int e = 0; e < kAhead; ++e) load(u + e, true, zv[e], fv[e]);
         __builtin_amdgcn_sched_barrier(0);
@@ -136,33 +134,29 @@ __global__ __launch_bounds__(64 * kWaves) void shrink_kernel(const ShrinkArgs a)
         for (int e = 0; e < kAhead; ++e) multiply(zv[e], fv[e]);
       }
       for (; u < last; ++u) {
-        u32x4 zv[MB][2], fv[RB][2];
+        u32x4 zv[2], fv[RB][2];
         load(u, u < whole, zv, fv);
         multiply(zv, fv);
       }
 #pragma unroll
-      for (int i = 0; i < MB; ++i)
-#pragma unroll
-        for (int j = 0; j < RB; ++j)
-#pragma unroll
-          for (int v = 0; v < 4; ++v)
-            if (whose >> (16 * i + 4 * g + v) & 1) acc[i][j][v] = d[i][j][v];
-    }
-    for (int i = 0; i < MB; ++i) {
-      __syncthreads();
-#pragma unroll
       for (int j = 0; j < RB; ++j)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) sum[wave][4 * g + v][RB * l + j] = acc[i][j][v];
-      __syncthreads();
-      for (int at = threadIdx.x; at < 256 * RB; at += 64 * kWaves) {
-        const int row = at / (16 * RB), r = at % (16 * RB), ad_of = own[16 * i + row];
-        if (ad_of < 0 || r0 + r >= a.Rp) continue;
-        float x = 0.0f;
+        for (int v = 0; v < 4; ++v)
+          if (whose >> (4 * g + v) & 1) acc[j][v] = d[j][v];
+    }
+    __syncthreads();
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) x += sum[w][row][r];
-        a.h[((size_t)blockIdx.y * a.T + t0 + 16 * i + row) * a.Rp + r0 + r] = a.scale ? x * a.scale[ad_of] : x;
-      }
+    for (int j = 0; j < RB; ++j)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) sum[wave][4 * g + v][RB * l + j] = acc[j][v];
+    __syncthreads();
+    for (int at = threadIdx.x; at < 256 * RB; at += 64 * kWaves) {
+      const int row = at / (16 * RB), r = at % (16 * RB);
+      if (own[row] < 0 || r0 + r >= a.Rp) continue;
+      float x = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) x += sum[w][row][r];
+      a.h[((size_t)blockIdx.y * a.T + t0 + row) * a.Rp + r0 + r] = x * factor[row];
     }
   }
 }

@@ -58,7 +58,7 @@ __device__ __forceinline__ f32x4 mfma_parts(u32x4 a, u32x4 b, f32x4 c) {
 // (f16: F_a in two parts as well, in two products).  Ranks beyond R are zero in h and read F_a's last one
 // again; columns beyond N read its last ones and are not stored.  A product is added only to the rows that are the
 // adapter's: an infinity or a NaN in one adapter is no other token's.
-template <class T, bool NN, int MB, int NB, int WM, int WN>
+template <class T, bool NN, int MB, int NB, int WM, int WN, int RB>
 __device__ __forceinline__ void expand_tile(const ProjectArgs& a, size_t t0, int n0, char* lds0,
                                             f32x4 (&acc)[MB][NB]) {
   typedef typename T::raw Raw;
@@ -81,6 +81,7 @@ __device__ __forceinline__ void expand_tile(const ProjectArgs& a, size_t t0, int
   const float* const h = a.h + (t0 + 64 * wm + l) * a.Rp;
   constexpr int kB = NB == 2 ? 2 : 1;                                // blocks of ranks a wait for memory, as registers allow
   constexpr int kBlock = BN * (__is_same(T, BF16) ? 32 : 64);        // bytes of one in the LDS
+  constexpr int kFit = (16 * MB * WM + BN) * RB / (kB * kBlock), kE = WM == 4 ? 2 : kFit < 4 ? kFit : 4;   // adapters a wait
   for (int r0 = 0; r0 < a.R; r0 += 16 * kB) {
     const int blocks = min(kB, (a.R - r0 + 15) / 16);
     f32x4 hv[kB][MB];                                                 // fp32: ranks 4 g ..
@@ -103,93 +104,107 @@ __device__ __forceinline__ void expand_tile(const ProjectArgs& a, size_t t0, int
     unsigned long long left[WM];
 #pragma unroll
     for (int w = 0; w < WM; ++w) left[w] = have[w];
-    // The next adapter (-1: none), which of this wave's rows are its own, and its ranks on their way.
-    unsigned long long mine = 0;
-    Raw x[kB][kUnits][8];
+    // The next adapters, which of this wave's rows are each one's own, and their ranks on their way.
+    unsigned long long mine[kE];
+    Raw x[kE][kB][kUnits][8];
     auto next = [&]() __attribute__((always_inline)) {
-      int ad = -1;
+      int count = 0;
 #pragma unroll
-      for (int w = 0; w < WM; ++w)
-        if (ad < 0 && left[w]) ad = __builtin_amdgcn_readlane(id[w], __builtin_ctzll(left[w]));
-      if (ad < 0) return false;
+      for (int e = 0; e < kE; ++e) {
+        int ad = -1;
 #pragma unroll
-      for (int w = 0; w < WM; ++w) {
-        const unsigned long long whose = __ballot(id[w] == ad);
-        left[w] &= ~whose;
-        if (w == wm) mine = whose;
-      }
-      const Raw* const f = static_cast<const Raw*>(a.f) + (size_t)ad * a.R * a.N;
+        for (int w = 0; w < WM; ++w)
+          if (ad < 0 && left[w]) ad = __builtin_amdgcn_readlane(id[w], __builtin_ctzll(left[w]));
+        mine[e] = 0;
+        if (ad < 0) continue;
+        ++count;
 #pragma unroll
-      for (int b = 0; b < kB; ++b)
-        if (b < blocks)
+        for (int w = 0; w < WM; ++w) {
+          const unsigned long long whose = __ballot(id[w] == ad);
+          left[w] &= ~whose;
+          if (w == wm) mine[e] = whose;
+        }
+        const Raw* const f = static_cast<const Raw*>(a.f) + (size_t)ad * a.R * a.N;
 #pragma unroll
-          for (int u = 0; u < kUnits; ++u) {
-            const int at = u * kThreads + threadIdx.x, r = r0 + 16 * b + at / BN * 8;
-            if (at >= 2 * BN) continue;
-            const Raw* const p = f + (size_t)min(n0 + at % BN, a.N - 1) * a.fn;
-            if (!NN && r + 8 <= a.R) {
-              __builtin_memcpy(x[b][u], p + r, sizeof(x[b][u]));
-            } else {
+        for (int b = 0; b < kB; ++b)
+          if (b < blocks)
 #pragma unroll
-              for (int q = 0; q < 8; ++q) x[b][u][q] = p[(size_t)min(r + q, a.R - 1) * a.fr];
+            for (int u = 0; u < kUnits; ++u) {
+              const int at = u * kThreads + threadIdx.x, r = r0 + 16 * b + at / BN * 8;
+              if (at >= 2 * BN) continue;
+              const Raw* const p = f + (size_t)min(n0 + at % BN, a.N - 1) * a.fn;
+              if (!NN && r + 8 <= a.R) {
+                __builtin_memcpy(x[e][b][u], p + r, sizeof(x[e][b][u]));
+              } else {
+#pragma unroll
+                for (int q = 0; q < 8; ++q) x[e][b][u][q] = p[(size_t)min(r + q, a.R - 1) * a.fr];
+              }
             }
-          }
-      return true;
+      }
+      return count;
     };
-    bool more = next();
-    while (more) {
-      const unsigned long long rows = mine;
+    int count = next();
+    while (count) {
+      unsigned long long rows[kE];
+#pragma unroll
+      for (int e = 0; e < kE; ++e) rows[e] = mine[e];
       __syncthreads();                                               // (nobody reads what was there)
 #pragma unroll
-      for (int b = 0; b < kB; ++b)
-        if (b < blocks)
+      for (int e = 0; e < kE; ++e)
 #pragma unroll
-          for (int u = 0; u < kUnits; ++u) {
-            const int at = u * kThreads + threadIdx.x, col = at % BN, half = at / BN;
-            if (at >= 2 * BN) continue;
-            const int in = col % (16 * NB), slot = col - in + 16 * (in % NB) + in / NB;    // block j's columns side by side
-            char* const to = lds0 + b * kBlock;
-            if constexpr (kF32) {
-              __builtin_memcpy(__builtin_assume_aligned(to + slot * 64 + half * 32, 16), x[b][u], 32);
-            } else if constexpr (__is_same(T, F16)) {
-              float y[8];
+        for (int b = 0; b < kB; ++b)
+          if (e < count && b < blocks)
 #pragma unroll
-              for (int q = 0; q < 8; ++q) y[q] = F16::widen(x[b][u][q]);
-              u16x8 hi, lo;
-              two_parts(y, hi, lo);
-              *reinterpret_cast<u16x8*>(to + slot * 64 + half * 16) = hi;
-              *reinterpret_cast<u16x8*>(to + slot * 64 + 32 + half * 16) = lo;
-            } else {
-              __builtin_memcpy(__builtin_assume_aligned(to + slot * 32 + half * 16, 16), x[b][u], 16);
+            for (int u = 0; u < kUnits; ++u) {
+              const int at = u * kThreads + threadIdx.x, col = at % BN, half = at / BN;
+              if (at >= 2 * BN) continue;
+              const int in = col % (16 * NB), slot = col - in + 16 * (in % NB) + in / NB;    // block j's columns side by side
+              char* const to = lds0 + (e * kB + b) * kBlock;
+              if constexpr (kF32) {
+                __builtin_memcpy(__builtin_assume_aligned(to + slot * 64 + half * 32, 16), x[e][b][u], 32);
+              } else if constexpr (__is_same(T, F16)) {
+                float y[8];
+#pragma unroll
+                for (int q = 0; q < 8; ++q) y[q] = F16::widen(x[e][b][u][q]);
+                u16x8 hi, lo;
+                two_parts(y, hi, lo);
+                *reinterpret_cast<u16x8*>(to + slot * 64 + half * 16) = hi;
+                *reinterpret_cast<u16x8*>(to + slot * 64 + 32 + half * 16) = lo;
+              } else {
+                __builtin_memcpy(__builtin_assume_aligned(to + slot * 32 + half * 16, 16), x[e][b][u], 16);
+              }
             }
-          }
-      more = next();
+      count = next();
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < MB; ++i) {
-        if (!(rows >> (16 * i) & 0xffff)) continue;
-        // (a product's bits where the row is the adapter's, none elsewhere)
-        const unsigned bits = (unsigned)(rows >> (16 * i)) >> (4 * g);
-        unsigned keep[4];
+      for (int e = 0; e < kE; ++e) {
+        if (!rows[e]) continue;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) keep[v] = (unsigned)__builtin_amdgcn_sbfe((int)bits, v, 1);
+        for (int i = 0; i < MB; ++i) {
+          if (!(rows[e] >> (16 * i) & 0xffff)) continue;
+          // (a product's bits where the row is the adapter's, none elsewhere)
+          const unsigned bits = (unsigned)(rows[e] >> (16 * i)) >> (4 * g);
+          unsigned keep[4];
 #pragma unroll
-        for (int b = 0; b < kB; ++b) {
-          if (b >= blocks) continue;
+          for (int v = 0; v < 4; ++v) keep[v] = (unsigned)__builtin_amdgcn_sbfe((int)bits, v, 1);
 #pragma unroll
-          for (int j = 0; j < NB; ++j) {
-            const char* const at = lds0 + b * kBlock + (wn + 16 * j + l) * (__is_same(T, BF16) ? 32 : 64);
-            f32x4 e = {};
-            if constexpr (kF32) {
-              const f32x4 fv = *reinterpret_cast<const f32x4*>(at + g * 16);
+          for (int b = 0; b < kB; ++b) {
+            if (b >= blocks) continue;
 #pragma unroll
-              for (int q = 0; q < 4; ++q) e = mfma_f32(hv[b][i][q], fv[q], e);
-            } else {
-              if constexpr (__is_same(T, F16)) e = mfma_bf16(ha[b][i], *reinterpret_cast<const u16x8*>(at + 32 + (g & 1) * 16), e);
-              e = mfma_bf16(ha[b][i], *reinterpret_cast<const u16x8*>(at + (g & 1) * 16), e);
+            for (int j = 0; j < NB; ++j) {
+              const char* const at = lds0 + (e * kB + b) * kBlock + (wn + 16 * j + l) * (__is_same(T, BF16) ? 32 : 64);
+              f32x4 d = {};
+              if constexpr (kF32) {
+                const f32x4 fv = *reinterpret_cast<const f32x4*>(at + g * 16);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) d = mfma_f32(hv[b][i][q], fv[q], d);
+              } else {
+                if constexpr (__is_same(T, F16)) d = mfma_bf16(ha[b][i], *reinterpret_cast<const u16x8*>(at + 32 + (g & 1) * 16), d);
+                d = mfma_bf16(ha[b][i], *reinterpret_cast<const u16x8*>(at + (g & 1) * 16), d);
+              }
+#pragma unroll
+              for (int v = 0; v < 4; ++v) acc[i][j][v] += __uint_as_float(__float_as_uint(d[v]) & keep[v]);
             }
-#pragma unroll
-            for (int v = 0; v < 4; ++v) acc[i][j][v] += __uint_as_float(__float_as_uint(e[v]) & keep[v]);
           }
         }
       }
@@ -504,7 +519,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
     multiply(lds0);
   }
 
-  if (split == 0) expand_tile<T, NN, MB, NB, WM, WN>(a, t0, n0, lds0, acc);
+  if (split == 0) expand_tile<T, NN, MB, NB, WM, WN, RB>(a, t0, n0, lds0, acc);
   const int n = n0 + wn + NB * l;
   if (n >= a.N) return;
   if (ta.part) {
@@ -598,31 +613,32 @@ constexpr int kShapes = 4, kRows[kShapes] = {128, 128, 64, 256}, kCols[kShapes] 
 
 }  // namespace
 
-TilePlan tile_plan(size_t T, int K, int N, int dtype, bool aligned) {
+// Which shape of tile, and in how many parts its depth: the least time by a model of what was measured at depth 4096
+// (microseconds; 16-bit types, fp32 in brackets): one tile on a compute unit, and two of them, whose waits
+// overlap where the LDS has room for both.
+//   128 x 256: 74, 132 (nn 71, 97)            128 x 128: 37, 75 (nn 43, 84)      [192, 390]
+//   64 x 256: 51, 69 (nn 56, 68) [218, 340; nn 213, 293]      256 x 256: 97, 194, with up to 5 of 8 units busy 80 (nn 97)
+// The parts of a split depth cost their way to memory and back at 2.5 TB/s and a launch of 5 us.  The model's choice was
+// within 10 % of the best of all shapes and splits at 40 sizes of 64 .. 8192 tokens (largest miss 15 %), where the
+// shapes differ by up to 3 times: 100 tokens 25 us (128 x 128 in four parts) against 82 (256 x 256), 8192
+// tokens 222 us (256 x 256) against 331 (128 x 128).
+TilePlan tile_plan(size_t T, int K, int N, int dtype, bool nn, bool aligned) {
+  static constexpr float k16[2][kShapes][2] = {{{74, 132}, {37, 75}, {51, 69}, {97, 194}}, {{71, 97}, {43, 84}, {56, 68}, {97, 194}}};
+  static constexpr float k32[2][kShapes][2] = {{{}, {192, 390}, {218, 340}, {}}, {{}, {190, 376}, {213, 293}, {}}};
   const long units = num_compute_units();
-  const bool f32 = dtype == CP4_DTYPE_F32;
+  const bool f32 = dtype == CP4_DTYPE_F32, some = f32 || !aligned;
   TilePlan best{};
-  double least = 0;
-  const bool some = f32 || !aligned;
   for (int w = some ? 1 : 0; w < (some ? 3 : kShapes); ++w) {
     const int KS = f32 || w == 0 ? 32 : 64, steps = (K + KS - 1) / KS;
     const long tiles = (long)((T + kRows[w] - 1) / kRows[w]) * ((N + kCols[w] - 1) / kCols[w]);
-    for (int s = 1; s <= 64 && s <= std::max(1, steps / 4); s *= 2) {
-      const int each = (steps + s - 1) / s;
-      const long wgs = tiles * ((steps + each - 1) / each);
-      // microseconds: a compute unit's tiles one after the other at its share of the matrix cores' rate (a
-      // workgroup alone reaches less of it), their starts and ends, the parts' way to memory and back
-      const double flops = 2.0 * kRows[w] * kCols[w] * KS * each, rate = f32 ? 1.2e6 : w == 0 ? 4.6e6 : w == 3 ? 5.5e6 : 3.6e6;
-      const long most = (wgs + units - 1) / units;
-      double cost = most * flops / (most == 1 && w != 3 ? 0.7 * rate : rate) + 2.0 + most;
-      if (s > 1) cost += 4.0 + (double)T * N * (s + 0.5) * 4.0 / 2.0e6;
-      if (!best.splits || cost < least) {
-        least = cost;
-        best.which = w;
-        best.each = each;
-        best.cost = cost;
-        best.splits = (steps + each - 1) / each;
-      }
+    const float* const us = f32 ? k32[nn][w] : k16[nn][w];
+    for (int s = 1; s <= 64 && s <= std::max(1, steps / 4) && (s == 1 || tiles * s <= 4 * units); s *= 2) {
+      const int each = (steps + s - 1) / s, parts = (steps + each - 1) / each;
+      const long wgs = tiles * parts, most = (wgs + units - 1) / units;
+      const double deep = KS * each / 4096.0;
+      double cost = 3.0 + deep * (most / 2 * us[1] + most % 2 * (w == 3 && !nn && wgs <= units * 5 / 8 ? 80.0 : us[0]));
+      if (s > 1) cost += 5.0 + (double)T * N * (parts + 0.5) * 4.0 / 2.5e6;
+      if (!best.splits || cost < best.cost) best = {w, parts, each, cost};
     }
   }
   return best;
