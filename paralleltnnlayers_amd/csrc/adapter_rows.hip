@@ -3,8 +3,13 @@
 //
 // A workgroup takes 16 columns (rows of W) of all tokens; its eight waves share the inputs, a cache
 // line of every row a turn and four turns' loads ahead of their products, which keeps 64 KB of W under way
-// on every compute unit.  x comes from the L2 again for every workgroup.  Where there are few columns the inputs
-// are split over workgroups too.  The adapters' parts are shared out over the waves; all sums meet in the LDS.
+// on every compute unit (eight turns ahead: 45 us instead of 43 on the fp32 case below).  x comes from the L2 again for
+// every workgroup, which is what bounds it beyond 16 tokens.  Where there are few columns the inputs
+// are split over workgroups too.  The adapters' parts are shared out over the waves, h's planes are added up while the first
+// turns' loads are on their way, and all sums meet in the LDS.
+//
+// Measured: 16 tokens fp32, 9216 -> 4096: 43 us, 3.5 TB/s; 48 tokens of 40 adapters bf16, 4096 x 4096: 22 us (9 us without
+// adapters and with 16 tokens); one token, 1024 x 1024: 6 us.
 #include <algorithm>
 
 #include "adapter.h"

@@ -1,22 +1,31 @@
 // The shared projection on the matrix cores (include/cp4/adapter.h): tiles of 64 to 256 rows x 128 or 256
 // columns, fed through the LDS, by loads that never pass a register where rows start on 16-byte boundaries.
 //
-// A step is 64 bytes of depth (32 values of 16 bits, 16 of fp32) of all the tile's rows and columns.
-// The LDS has room for two to four steps: while one is multiplied the next ones are on their way, and one barrier a
-// step says both that the next one has arrived and that the last one's room is free.
-// A wave has 64 rows and 64 or 128 columns in registers; two workgroups on a compute unit keep its
-// matrix cores busy over each other's barriers.
+// A step is RB bytes of depth (64 or 128: 32 or 64 values of 16 bits, half of that in fp32) of all the tile's rows and
+// columns.  The LDS has room for two to four steps: while one is multiplied the next ones are on their way, and one
+// barrier a step says both that the next one has arrived and that the last one's room is free.  A wave has 64 rows and
+// 32 to 128 columns in registers.  Two workgroups of the 64-row and the 128 x 256 tile share a compute unit and keep its
+// matrix cores busy over each other's barriers; the 256 x 256 tile is alone there and reads one half of a step's
+// operands while the other half's are multiplied (8192 x 4096 x 4096 243 -> 216 us; nn: the turned operands' registers
+// do not fit beside it, 255 us with it and 240 without).
+//
+// fp32 is multiplied as three bfloat16 parts of each value, six of the nine products (148 -> 95 us at 64 x 25088 x
+// 4096 against the fp32 instructions), which is nearer to 64 bits than an fp32 sum in one go.
 //
 // A wave's column block j holds the columns n0 + NB * l + j (l: lane & 15), not 16 j + l: a lane then
 // has NB consecutive values of every output row (one or two 16-byte stores), and where w is [K][N] (nn)
 // the same order lets one load bring NB blocks' values, which are turned in registers (one byte permute
 // for two values).
 //
-// The adapters: when a tile's sum is done, h F_a^T is added for each adapter that the wave's rows have (a
+// The adapters: when a tile's sum is done, h F_a^T is added for each adapter that the tile's rows have (a
 // 16-deep product a rank block against a sum over thousands of inputs), so y is written once.
 //
 // Little work for the chip is split over the depth: the partial tiles go to the workspace in
 // fp32 (the first one with the adapters' part) and a second launch adds them up in their order.
+//
+// Measured: 8192 x 4096 x 4096 bf16 with adapters of rank 16: 212 us, 1.30 PFLOP/s (nn 239; the library's product
+// alone 179), bound by the LDS's bandwidth beside the matrix cores; 2048 x 4096 x 8192 121 us; 1031 x 2048 x 2816 f16, rank 64:
+// 38 us (nn 49), bound by what the L2 gives the LDS (4 rooms instead of 3 change nothing); 64 x 25088 x 4096 fp32 93 us, 4.4 TB/s of W.
 #include <algorithm>
 #include <type_traits>
 
@@ -51,8 +60,10 @@ __device__ __forceinline__ f32x4 mfma_parts(u32x4 a, u32x4 b, f32x4 c) {
   return mfma_bf16(__builtin_bit_cast(u16x8, a), __builtin_bit_cast(u16x8, b), c);
 }
 
-// Adds h F_a^T to a tile, one adapter of its rows after the other: the adapter's ranks, 16 or 32 at a time, of
-// all columns come into the LDS, whatever their strides and alignment, and each wave multiplies them with its own rows.
+// Adds h F_a^T to a tile, up to kE adapters of its rows between two barriers: their ranks, 16 or 32 at a time, of all
+// columns come into the LDS, whatever their strides and alignment, and each wave multiplies them with its own rows.
+// (64 tokens of 64 adapters, 1024 x 1024: 97 us with one adapter at a time, 56 with four.  Straight from memory to
+// the matrix cores the loads' addresses spill: 60 to 80 us more a large tile.)
 //
 // 16-bit types: depth 0 .. 15 of a product are the first parts of h, 16 .. 31 what they leave, against F_a twice
 // (f16: F_a in two parts as well, in two products).  Ranks beyond R are zero in h and read F_a's last one
@@ -613,17 +624,19 @@ constexpr int kShapes = 4, kRows[kShapes] = {128, 128, 64, 256}, kCols[kShapes] 
 
 }  // namespace
 
-// Which shape of tile, and in how many parts its depth: the least time by a model of what was measured at depth 4096
-// (microseconds; 16-bit types, fp32 in brackets): one tile on a compute unit, and two of them, whose waits
-// overlap where the LDS has room for both.
-//   128 x 256: 74, 132 (nn 71, 97)            128 x 128: 37, 75 (nn 43, 84)      [192, 390]
-//   64 x 256: 51, 69 (nn 56, 68) [218, 340; nn 213, 293]      256 x 256: 97, 194, with up to 5 of 8 units busy 80 (nn 97)
-// The parts of a split depth cost their way to memory and back at 2.5 TB/s and a launch of 5 us.  The model's choice was
-// within 10 % of the best of all shapes and splits at 40 sizes of 64 .. 8192 tokens (largest miss 15 %), where the
-// shapes differ by up to 3 times: 100 tokens 25 us (128 x 128 in four parts) against 82 (256 x 256), 8192
-// tokens 222 us (256 x 256) against 331 (128 x 128).
+// Which shape of tile, and in how many parts its depth: the least time by a model of what was measured at a depth of
+// 4096 (microseconds; 16-bit types, fp32 in brackets), one tile on a compute unit and two of them, whose waits
+// overlap where the LDS has room for both:
+//   128 x 256: 74, 132 (nn 74, 116)
+//   128 x 128: 37, 75 (nn 42, 88)  [192, 390; nn 190, 376]
+//    64 x 256: 51, 69 (nn 55, 76)  [218, 340; nn 213, 293]
+//   256 x 256: 97, 194, with up to 5 of 8 units busy 80 (nn 102, 204)
+// The parts of a split depth cost their way to memory and back at 2.5 TB/s and a launch of 5 us.  At 50 sizes of
+// 64 .. 8192 tokens the choice was 3 % from the best of all shapes and splits on the average and 15 % at worst; the shapes
+// differ by up to 3 times: 100 tokens of 4096 x 4096 take 25 us (128 x 128 in four parts) and 82 (256 x 256), 8192 tokens
+// 223 us (256 x 256) and 331 (128 x 128), 6000 tokens nn 206 us (128 x 256), 224 (256 x 256) and 239 (64 x 256).
 TilePlan tile_plan(size_t T, int K, int N, int dtype, bool nn, bool aligned) {
-  static constexpr float k16[2][kShapes][2] = {{{74, 132}, {37, 75}, {51, 69}, {97, 194}}, {{71, 97}, {43, 84}, {56, 68}, {97, 194}}};
+  static constexpr float k16[2][kShapes][2] = {{{74, 132}, {37, 75}, {51, 69}, {97, 194}}, {{74, 116}, {42, 88}, {55, 76}, {102, 204}}};
   static constexpr float k32[2][kShapes][2] = {{{}, {192, 390}, {218, 340}, {}}, {{}, {190, 376}, {213, 293}, {}}};
   const long units = num_compute_units();
   const bool f32 = dtype == CP4_DTYPE_F32, some = f32 || !aligned;

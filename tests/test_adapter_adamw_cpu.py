@@ -55,6 +55,12 @@ def test_adapter_shapes_are_refused(capi):
     assert bwd(s, d=(ONE, ONE, None)) == capi.ERR_NULL_POINTER
 
 
+def test_adapter_tokens_have_a_limit(capi):
+    L = capi.lib()
+    need = lambda T: L.cp4_adapter_kept_bytes(ctypes.byref(capi.AdapterShape(T=T, K=32, N=24, R=4, G=2, ldx=0, ldw=0, lddy=0)), 0)
+    assert need(1 << 26) == 64 << 26 and need((1 << 26) + 1) == 0
+
+
 def test_adapter_workspace_grows_with_its_parts(capi):
     L = capi.lib()
     need = lambda **kw: L.cp4_adapter_backward_workspace_bytes(

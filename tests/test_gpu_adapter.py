@@ -121,6 +121,36 @@ def test_layer_and_gradients(cp4, dtype, size, pattern):
         check(v, want[k], k)
 
 
+@pytest.mark.parametrize("size", [(96, 64, 72, 40, 96), (128, 96, 136, 16, 128), (250, 136, 264, 33, 260), (310, 72, 1040, 7, 400)],
+                         ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_every_token_its_own_adapter(cp4, dtype, size):
+    T, K, N, R, G = size
+    d = make(dtype, T, K, N, R, G, "none", seed=9)
+    d["ids"] = torch.randperm(G, generator=torch.Generator().manual_seed(T))[:T].int()
+    want = formula(d, dtype)
+    g = {k: v.cuda() for k, v in d.items()}
+    y, kept = cp4.adapter_forward(g["x"], g["W"], g["A"], g["B"], g["ids"], g["scale"], g["bias"], keep=True)
+    check(y, want["y"], "y")
+    grads = cp4.adapter_backward(g["dy"], g["x"], g["W"], g["A"], g["B"], g["ids"], g["scale"], kept)
+    for k, v in zip(("dx", "dA", "dB"), grads):
+        check(v, want[k], k)
+
+
+@pytest.mark.parametrize("T,G", [(17, 2), (33, 1), (40, 40), (64, 3)])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_few_tokens_of_a_wide_layer(cp4, dtype, T, G):
+    """Few tokens on tiles and on the kernel of few rows, whichever the number of adapters asks for."""
+    d = make(dtype, T, 1016, 9008, 12, G, "mixed", seed=T)
+    want = formula(d, dtype)
+    g = {k: v.cuda() for k, v in d.items()}
+    y, kept = cp4.adapter_forward(g["x"], g["W"], g["A"], g["B"], g["ids"], g["scale"], g["bias"], keep=True)
+    check(y, want["y"], "y")
+    grads = cp4.adapter_backward(g["dy"], g["x"], g["W"], g["A"], g["B"], g["ids"], g["scale"], kept)
+    for k, v in zip(("dx", "dA", "dB"), grads):
+        check(v, want[k], k)
+
+
 @pytest.mark.parametrize("pattern", ["one", "none", "outside"])
 @pytest.mark.parametrize("size", [(1, 256, 128, 16, 4), (40, 320, 200, 8, 3), (300, 1000, 264, 20, 5)],
                          ids=lambda s: "x".join(map(str, s)))
