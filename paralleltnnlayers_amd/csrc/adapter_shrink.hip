@@ -3,7 +3,7 @@
 //
 // A workgroup takes 16 tokens and one part of the inputs, straight from memory to the matrix cores:
 // nothing is read twice within it, so the LDS would only be a detour (48 tokens of 40 adapters, 4096 inputs: 139 us
-// through the LDS, 8.4 so).  Its eight waves share the adapters that these tokens have - one of a prompt, sixteen of
+// through the LDS, 6.6 so).  Its eight waves share the adapters that these tokens have - one of a prompt, sixteen of
 // single tokens - and, where there are fewer, the inputs.  All rows are multiplied with each adapter and the rows
 // that are not its own keep what they had; the waves' sums meet in the LDS once, at the end.  (32 tokens a workgroup:
 // no gain.)  With few tokens the inputs are split over workgroups as well: each part leaves a plane of h of its own,
@@ -13,7 +13,7 @@
 // (B, in the backward pass) come with loads of RB values.
 //
 // Measured (bf16): 8192 tokens of 4096 inputs, rank 16: 26 us, 2.6 TB/s (a copy reaches 5.1), bound by loads in flight, since
-// every turn waits for memory once; 48 tokens of 40 adapters 8.4 us, which is the latency of four such waits and a launch.
+// every turn waits for memory once; 48 tokens of 40 adapters 6.6 us, which is the latency of a few such waits and a launch.
 #include <algorithm>
 
 #include "adapter.h"
@@ -199,13 +199,13 @@ hipError_t planes_join(float* h, const float* from, size_t n, int planes, hipStr
   return hipGetLastError();
 }
 
-// Parts of the inputs: a workgroup for each compute unit, four turns or more a part.  (Forward pass, bf16, 4096 inputs and
+// Parts of the inputs: a workgroup for each compute unit, two turns or more a part.  (Forward pass, bf16, 4096 inputs and
 // outputs, 48 adapters: 48 tokens 138 us in one part, 43 in 8, 36 in 16; 2077 tokens 119 in one, 114 in 2; 8192 tokens 239 in one,
-// 242 in 2, 243 in 4.)
+// 242 in 2, 243 in 4; 333 tokens of 1001 inputs 23.9 us in one, 21.7 in 4, 20.7 in 8.)
 int shrink_planes(size_t T, int K, int dtype) {
   const int unit = dtype == CP4_DTYPE_F32 ? kUnit<F32> : kUnit<BF16>;
   const size_t tiles = std::max<size_t>(1, (T + 15) / 16);
-  const size_t most = std::max(1, (K + unit - 1) / unit / 4);
+  const size_t most = std::max(1, (K + unit - 1) / unit / 2);
   return (int)std::max<size_t>(1, std::min({((size_t)num_compute_units() + tiles - 1) / tiles, most, (size_t)64}));
 }
 
