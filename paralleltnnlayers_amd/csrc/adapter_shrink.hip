@@ -2,7 +2,7 @@
 // have ranks, bound by reading x and the adapters in use once.
 //
 // A workgroup takes 16 tokens and one part of the inputs, straight from memory to the matrix cores:
-// nothing is read twice within it, so the LDS would only be a detour (48 tokens of 40 adapters, 4096 inputs: 139 us
+// nothing is read twice within it, so the LDS would only be a detour (48 tokens of 32 adapters, 4096 inputs: 139 us
 // through the LDS, 6.6 so).  Its eight waves share the adapters that these tokens have - one of a prompt, sixteen of
 // single tokens - and, where there are fewer, the inputs.  All rows are multiplied with each adapter and the rows
 // that are not its own keep what they had; the waves' sums meet in the LDS once, at the end.  (32 tokens a workgroup:
@@ -13,7 +13,7 @@
 // (B, in the backward pass) come with loads of RB values.
 //
 // Measured (bf16): 8192 tokens of 4096 inputs, rank 16: 26 us, 2.6 TB/s (a copy reaches 5.1), bound by loads in flight, since
-// every turn waits for memory once; 48 tokens of 40 adapters 6.6 us, which is the latency of a few such waits and a launch.
+// every turn waits for memory once; 48 tokens of 32 adapters 6.6 us, which is the latency of a few such waits and a launch.
 #include <algorithm>
 
 #include "adapter.h"
