@@ -60,165 +60,187 @@ __device__ __forceinline__ f32x4 mfma_parts(u32x4 a, u32x4 b, f32x4 c) {
   return mfma_bf16(__builtin_bit_cast(u16x8, a), __builtin_bit_cast(u16x8, b), c);
 }
 
-// Adds h F_a^T to a tile, up to kE adapters of its rows between two barriers: their ranks, 16 or 32 at a time, of all
-// columns come into the LDS, whatever their strides and alignment, and each wave multiplies them with its own rows.
-// (64 tokens of 64 adapters, 1024 x 1024: 97 us with one adapter at a time, 56 with four.  Straight from memory to
-// the matrix cores the loads' addresses spill: 60 to 80 us more a large tile.)
+// Adds h F_a^T to a tile.  h's rows come into one room of the LDS once, 32 or 64 ranks at a time, and the ranks of the
+// tile's adapters into another, 16 of one adapter a unit and up to kE units between two barriers, whatever their strides and
+// alignment; each wave multiplies them with its own rows.  (64 tokens of 64 adapters, 1024 x 1024: 97 us with one adapter
+// at a time, 56 with four.  h in registers instead, 32 ranks a pass: 1024 tokens of 4 adapters of rank 256, 4096 x 4096, 109 us
+// instead of 83.  Straight from memory to the matrix cores the loads' addresses spill: 60 to 80 us more a large tile.)
 //
 // 16-bit types: depth 0 .. 15 of a product are the first parts of h, 16 .. 31 what they leave, against F_a twice
 // (f16: F_a in two parts as well, in two products).  Ranks beyond R are zero in h and read F_a's last one
 // again; columns beyond N read its last ones and are not stored.  A product is added only to the rows that are the
 // adapter's: an infinity or a NaN in one adapter is no other token's.
 template <class T, bool NN, int MB, int NB, int WM, int WN, int RB>
-__device__ __forceinline__ void expand_tile(const ProjectArgs& a, size_t t0, int n0, char* lds0,
+__device__ __forceinline__ void expand_tile(const ProjectArgs& a, size_t t0, int n0, char* lds0, char* lds1,
                                             f32x4 (&acc)[MB][NB]) {
   typedef typename T::raw Raw;
   constexpr bool kF32 = __is_same(T, F32);
-  constexpr int kThreads = 64 * WM * WN, BN = 16 * NB * WN, kUnits = (2 * BN + kThreads - 1) / kThreads;   // 8 ranks of a column each
-  static_assert(MB == 4, "a wave's rows are a ballot");
+  constexpr int kThreads = 64 * WM * WN, BM = 16 * MB * WM, BN = 16 * NB * WN, kRoom = (BM + BN) * RB;
+  constexpr int kUnits = (2 * BN + kThreads - 1) / kThreads;         // 8 ranks of a column each
+  constexpr int kBlock = BN * (__is_same(T, BF16) ? 32 : 64);        // bytes of a unit in the LDS
+  constexpr int kFit = kRoom / kBlock, kMost = NB == 8 || NN ? 4 : 8, kE = kFit < kMost ? kFit : kMost;
+  constexpr int kC = BM * 256 <= kRoom ? 4 : 2;                      // blocks of ranks of h in the LDS: 64 bytes a row each
+  constexpr int kI = (BM * kC * 2 + kThreads - 1) / kThreads;        // 8 ranks of a row each
+  static_assert(MB == 4 && kE >= 1 && BM * kC * 64 <= kRoom, "a wave's rows are a ballot");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 15, g = lane >> 4;
   const int wm = wave / WN, wn = 16 * NB * (wave % WN);
   int id[WM];
-  unsigned long long have[WM], any = 0, have_mine = 0;
+  unsigned long long have[WM], any = 0;
 #pragma unroll
   for (int w = 0; w < WM; ++w) {
     const size_t row = t0 + 64 * w + lane;
     id[w] = row < a.T ? a.ids[row] : -1;
     if (id[w] < 0 || id[w] >= a.G) id[w] = -1;
     any |= have[w] = __ballot(id[w] >= 0);
-    if (w == wm) have_mine = have[w];
   }
   if (!any) return;
-  const float* const h = a.h + (t0 + 64 * wm + l) * a.Rp;
-  constexpr int kB = NB == 2 ? 2 : 1;                                // blocks of ranks a wait for memory, as registers allow
-  constexpr int kBlock = BN * (__is_same(T, BF16) ? 32 : 64);        // bytes of one in the LDS
-  constexpr int kFit = (16 * MB * WM + BN) * RB / (kB * kBlock), kE = WM == 4 ? 2 : kFit < 4 ? kFit : 4;   // adapters a wait
-  for (int r0 = 0; r0 < a.R; r0 += 16 * kB) {
-    const int blocks = min(kB, (a.R - r0 + 15) / 16);
-    f32x4 hv[kB][MB];                                                 // fp32: ranks 4 g ..
-    u16x8 ha[kB][MB];                                                 // 16 bits: ranks 8 (g & 1) .., first parts for g < 2
-#pragma unroll
-    for (int b = 0; b < kB; ++b)
-#pragma unroll
-      for (int i = 0; i < MB; ++i) {
-        float x[8] = {};
-        if (b < blocks && have_mine >> (16 * i + l) & 1) {
-          const float* p = h + (size_t)16 * i * a.Rp + r0 + 16 * b + (kF32 ? 4 * g : 8 * (g & 1));
-          __builtin_memcpy(x, __builtin_assume_aligned(p, 16), 16);
-          if constexpr (!kF32) __builtin_memcpy(x + 4, __builtin_assume_aligned(p + 4, 16), 16);
-        }
-        hv[b][i] = f32x4{x[0], x[1], x[2], x[3]};
-        u16x8 hi, lo;
-        two_parts(x, hi, lo);
-        ha[b][i] = g < 2 ? hi : lo;
-      }
+  for (int c0 = 0; c0 < a.R; c0 += 16 * kC) {
+    const int blocks = min(kC, (a.R - c0 + 15) / 16);
     unsigned long long left[WM];
 #pragma unroll
     for (int w = 0; w < WM; ++w) left[w] = have[w];
-    // The next adapters, which of this wave's rows are each one's own, and their ranks on their way.
-    unsigned long long mine[kE];
-    Raw x[kE][kB][kUnits][8];
+    // The next units, which of this wave's rows are each one's own, and their ranks on their way.
+    int ad = -1, block = 0, of[kE];
+    unsigned long long own = 0, mine[kE];
+    Raw x[kE][kUnits][8];
     auto next = [&]() __attribute__((always_inline)) {
       int count = 0;
 #pragma unroll
       for (int e = 0; e < kE; ++e) {
-        int ad = -1;
+        if (ad < 0) {
 #pragma unroll
-        for (int w = 0; w < WM; ++w)
-          if (ad < 0 && left[w]) ad = __builtin_amdgcn_readlane(id[w], __builtin_ctzll(left[w]));
+          for (int w = 0; w < WM; ++w)
+            if (ad < 0 && left[w]) ad = __builtin_amdgcn_readlane(id[w], __builtin_ctzll(left[w]));
+          if (ad >= 0)
+#pragma unroll
+            for (int w = 0; w < WM; ++w) {
+              const unsigned long long whose = __ballot(id[w] == ad);
+              left[w] &= ~whose;
+              if (w == wm) own = whose;
+            }
+        }
         mine[e] = 0;
+        of[e] = block;
         if (ad < 0) continue;
         ++count;
-#pragma unroll
-        for (int w = 0; w < WM; ++w) {
-          const unsigned long long whose = __ballot(id[w] == ad);
-          left[w] &= ~whose;
-          if (w == wm) mine[e] = whose;
-        }
+        mine[e] = own;
         const Raw* const f = static_cast<const Raw*>(a.f) + (size_t)ad * a.R * a.N;
 #pragma unroll
-        for (int b = 0; b < kB; ++b)
-          if (b < blocks)
+        for (int u = 0; u < kUnits; ++u) {
+          const int at = u * kThreads + threadIdx.x, r = c0 + 16 * block + at / BN * 8;
+          if (at >= 2 * BN) continue;
+          const Raw* const p = f + (size_t)min(n0 + at % BN, a.N - 1) * a.fn;
+          if (!NN && r + 8 <= a.R) {
+            __builtin_memcpy(x[e][u], p + r, sizeof(x[e][u]));
+          } else {
 #pragma unroll
-            for (int u = 0; u < kUnits; ++u) {
-              const int at = u * kThreads + threadIdx.x, r = r0 + 16 * b + at / BN * 8;
-              if (at >= 2 * BN) continue;
-              const Raw* const p = f + (size_t)min(n0 + at % BN, a.N - 1) * a.fn;
-              if (!NN && r + 8 <= a.R) {
-                __builtin_memcpy(x[e][b][u], p + r, sizeof(x[e][b][u]));
-              } else {
-#pragma unroll
-                for (int q = 0; q < 8; ++q) x[e][b][u][q] = p[(size_t)min(r + q, a.R - 1) * a.fr];
-              }
-            }
+            for (int q = 0; q < 8; ++q) x[e][u][q] = p[(size_t)min(r + q, a.R - 1) * a.fr];
+          }
+        }
+        if (++block == blocks) {
+          block = 0;
+          ad = -1;
+        }
       }
       return count;
     };
     int count = next();
+    {
+      f32x4 hv[kI][2];
+#pragma unroll
+      for (int i = 0; i < kI; ++i) {
+        const int at = i * kThreads + threadIdx.x, row = at % BM, r = at / BM * 8;
+        hv[i][0] = hv[i][1] = f32x4{};
+        if (r >= 16 * blocks || t0 + row >= a.T) continue;
+        const float* const p = a.h + (t0 + row) * a.Rp + c0 + r;
+        hv[i][0] = *reinterpret_cast<const f32x4*>(p);
+        hv[i][1] = *reinterpret_cast<const f32x4*>(p + 4);
+      }
+      __syncthreads();                                               // (nobody reads what was there)
+      // [block of ranks][piece][row]: 16 bytes that a lane multiplies, piece g of its row
+#pragma unroll
+      for (int i = 0; i < kI; ++i) {
+        const int at = i * kThreads + threadIdx.x, row = at % BM, r = at / BM * 8, half = r / 8 & 1;
+        if (r >= 16 * blocks) continue;
+        char* const to = lds1 + ((size_t)(r / 16) * 4 * BM + row) * 16;
+        if constexpr (kF32) {
+          *reinterpret_cast<f32x4*>(to + (2 * half) * BM * 16) = hv[i][0];
+          *reinterpret_cast<f32x4*>(to + (2 * half + 1) * BM * 16) = hv[i][1];
+        } else {
+          float y[8];
+          __builtin_memcpy(y, &hv[i][0], 32);
+          u16x8 hi, lo;
+          two_parts(y, hi, lo);
+          *reinterpret_cast<u16x8*>(to + half * BM * 16) = hi;
+          *reinterpret_cast<u16x8*>(to + (2 + half) * BM * 16) = lo;
+        }
+      }
+    }
     while (count) {
       unsigned long long rows[kE];
+      int part[kE];
 #pragma unroll
-      for (int e = 0; e < kE; ++e) rows[e] = mine[e];
-      __syncthreads();                                               // (nobody reads what was there)
+      for (int e = 0; e < kE; ++e) {
+        rows[e] = mine[e];
+        part[e] = of[e];
+      }
 #pragma unroll
       for (int e = 0; e < kE; ++e)
+        if (e < count)
 #pragma unroll
-        for (int b = 0; b < kB; ++b)
-          if (e < count && b < blocks)
+          for (int u = 0; u < kUnits; ++u) {
+            const int at = u * kThreads + threadIdx.x, col = at % BN, half = at / BN;
+            if (at >= 2 * BN) continue;
+            const int in = col % (16 * NB), slot = col - in + 16 * (in % NB) + in / NB;    // block j's columns side by side
+            char* const to = lds0 + e * kBlock;
+            if constexpr (kF32) {
+              __builtin_memcpy(__builtin_assume_aligned(to + slot * 64 + half * 32, 16), x[e][u], 32);
+            } else if constexpr (__is_same(T, F16)) {
+              float y[8];
 #pragma unroll
-            for (int u = 0; u < kUnits; ++u) {
-              const int at = u * kThreads + threadIdx.x, col = at % BN, half = at / BN;
-              if (at >= 2 * BN) continue;
-              const int in = col % (16 * NB), slot = col - in + 16 * (in % NB) + in / NB;    // block j's columns side by side
-              char* const to = lds0 + (e * kB + b) * kBlock;
-              if constexpr (kF32) {
-                __builtin_memcpy(__builtin_assume_aligned(to + slot * 64 + half * 32, 16), x[e][b][u], 32);
-              } else if constexpr (__is_same(T, F16)) {
-                float y[8];
-#pragma unroll
-                for (int q = 0; q < 8; ++q) y[q] = F16::widen(x[e][b][u][q]);
-                u16x8 hi, lo;
-                two_parts(y, hi, lo);
-                *reinterpret_cast<u16x8*>(to + slot * 64 + half * 16) = hi;
-                *reinterpret_cast<u16x8*>(to + slot * 64 + 32 + half * 16) = lo;
-              } else {
-                __builtin_memcpy(__builtin_assume_aligned(to + slot * 32 + half * 16, 16), x[e][b][u], 16);
-              }
+              for (int q = 0; q < 8; ++q) y[q] = F16::widen(x[e][u][q]);
+              u16x8 hi, lo;
+              two_parts(y, hi, lo);
+              *reinterpret_cast<u16x8*>(to + slot * 64 + half * 16) = hi;
+              *reinterpret_cast<u16x8*>(to + slot * 64 + 32 + half * 16) = lo;
+            } else {
+              __builtin_memcpy(__builtin_assume_aligned(to + slot * 32 + half * 16, 16), x[e][u], 16);
             }
+          }
       count = next();
       __syncthreads();
 #pragma unroll
       for (int e = 0; e < kE; ++e) {
         if (!rows[e]) continue;
+        const char* const hp = lds1 + ((size_t)(part[e] * 4 + g) * BM + 64 * wm + l) * 16;
 #pragma unroll
         for (int i = 0; i < MB; ++i) {
           if (!(rows[e] >> (16 * i) & 0xffff)) continue;
+          const u32x4 hv = *reinterpret_cast<const u32x4*>(hp + 16 * i * 16);
           // (a product's bits where the row is the adapter's, none elsewhere)
           const unsigned bits = (unsigned)(rows[e] >> (16 * i)) >> (4 * g);
           unsigned keep[4];
 #pragma unroll
           for (int v = 0; v < 4; ++v) keep[v] = (unsigned)__builtin_amdgcn_sbfe((int)bits, v, 1);
 #pragma unroll
-          for (int b = 0; b < kB; ++b) {
-            if (b >= blocks) continue;
+          for (int j = 0; j < NB; ++j) {
+            const char* const at = lds0 + e * kBlock + (wn + 16 * j + l) * (__is_same(T, BF16) ? 32 : 64);
+            f32x4 d = {};
+            if constexpr (kF32) {
+              const f32x4 fv = *reinterpret_cast<const f32x4*>(at + g * 16);
 #pragma unroll
-            for (int j = 0; j < NB; ++j) {
-              const char* const at = lds0 + (e * kB + b) * kBlock + (wn + 16 * j + l) * (__is_same(T, BF16) ? 32 : 64);
-              f32x4 d = {};
-              if constexpr (kF32) {
-                const f32x4 fv = *reinterpret_cast<const f32x4*>(at + g * 16);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) d = mfma_f32(hv[b][i][q], fv[q], d);
-              } else {
-                if constexpr (__is_same(T, F16)) d = mfma_bf16(ha[b][i], *reinterpret_cast<const u16x8*>(at + 32 + (g & 1) * 16), d);
-                d = mfma_bf16(ha[b][i], *reinterpret_cast<const u16x8*>(at + (g & 1) * 16), d);
-              }
-#pragma unroll
-              for (int v = 0; v < 4; ++v) acc[i][j][v] += __uint_as_float(__float_as_uint(d[v]) & keep[v]);
+              for (int q = 0; q < 4; ++q) d = mfma_f32(__uint_as_float(hv[q]), fv[q], d);
+            } else {
+              const u16x8 hb = __builtin_bit_cast(u16x8, hv);
+              if constexpr (__is_same(T, F16)) d = mfma_bf16(hb, *reinterpret_cast<const u16x8*>(at + 32 + (g & 1) * 16), d);
+              d = mfma_bf16(hb, *reinterpret_cast<const u16x8*>(at + (g & 1) * 16), d);
             }
+#pragma unroll
+            for (int v = 0; v < 4; ++v) acc[i][j][v] += __uint_as_float(__float_as_uint(d[v]) & keep[v]);
           }
         }
       }
+      __syncthreads();                                               // (nobody reads what was there)
     }
   }
 }
@@ -530,7 +552,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
     multiply(lds0);
   }
 
-  if (split == 0) expand_tile<T, NN, MB, NB, WM, WN, RB>(a, t0, n0, lds0, acc);
+  if (split == 0) expand_tile<T, NN, MB, NB, WM, WN, RB>(a, t0, n0, lds0, lds1, acc);
   const int n = n0 + wn + NB * l;
   if (n >= a.N) return;
   if (ta.part) {
