@@ -25,7 +25,7 @@
 //
 // Measured: 8192 x 4096 x 4096 bf16 with adapters of rank 16: 212 us, 1.30 PFLOP/s (nn 239; the library's product
 // alone 179), bound by the LDS's bandwidth beside the matrix cores; 2048 x 4096 x 8192 121 us; 1031 x 2048 x 2816 f16, rank 64:
-// 38 us (nn 49), bound by what the L2 gives the LDS (4 rooms instead of 3 change nothing); 64 x 25088 x 4096 fp32 93 us, 4.4 TB/s of W.
+// 30 us (nn 42), bound by what the L2 gives the LDS (4 rooms instead of 3 change nothing); 64 x 25088 x 4096 fp32 93 us, 4.4 TB/s of W.
 #include <algorithm>
 #include <type_traits>
 
@@ -79,6 +79,7 @@ __device__ __forceinline__ void expand_tile(const ProjectArgs& a, size_t t0, int
   constexpr int kUnits = (2 * BN + kThreads - 1) / kThreads;         // 8 ranks of a column each
   constexpr int kBlock = BN * (__is_same(T, BF16) ? 32 : 64);        // bytes of a unit in the LDS
   constexpr int kFit = kRoom / kBlock, kMost = NB == 8 || NN ? 4 : 8, kE = kFit < kMost ? kFit : kMost;
+  // (nn: eight units of strided loads gain nothing, 91 us for rank 256 instead of 86)
   constexpr int kC = BM * 256 <= kRoom ? 4 : 2;                      // blocks of ranks of h in the LDS: 64 bytes a row each
   constexpr int kI = (BM * kC * 2 + kThreads - 1) / kThreads;        // 8 ranks of a row each
   static_assert(MB == 4 && kE >= 1 && BM * kC * 64 <= kRoom, "a wave's rows are a ballot");
