@@ -657,7 +657,8 @@ constexpr int kShapes = 4, kRows[kShapes] = {128, 128, 64, 256}, kCols[kShapes] 
 // The parts of a split depth cost their way to memory and back at 2.5 TB/s and a launch of 5 us.  At 50 sizes of
 // 64 .. 8192 tokens the choice was 3 % from the best of all shapes and splits on the average and 15 % at worst; the shapes
 // differ by up to 3 times: 100 tokens of 4096 x 4096 take 25 us (128 x 128 in four parts) and 82 (256 x 256), 8192 tokens
-// 223 us (256 x 256) and 331 (128 x 128), 6000 tokens nn 206 us (128 x 256), 224 (256 x 256) and 239 (64 x 256).
+// 223 us (256 x 256) and 331 (128 x 128), 6000 tokens nn 206 us (128 x 256), 224 (256 x 256) and 239 (64 x 256).  Parts other
+// than powers of two fill the chip where those leave a round half empty: 300 tokens fp32 4096 x 4096 97 -> 87 us (nn 103 -> 84).
 TilePlan tile_plan(size_t T, int K, int N, int dtype, bool nn, bool aligned) {
   static constexpr float k16[2][kShapes][2] = {{{74, 132}, {37, 75}, {51, 69}, {97, 194}}, {{74, 116}, {42, 88}, {55, 76}, {102, 204}}};
   static constexpr float k32[2][kShapes][2] = {{{}, {192, 390}, {218, 340}, {}}, {{}, {190, 376}, {213, 293}, {}}};
@@ -668,7 +669,7 @@ TilePlan tile_plan(size_t T, int K, int N, int dtype, bool nn, bool aligned) {
     const int KS = f32 || w == 0 ? 32 : 64, steps = (K + KS - 1) / KS;
     const long tiles = (long)((T + kRows[w] - 1) / kRows[w]) * ((N + kCols[w] - 1) / kCols[w]);
     const float* const us = f32 ? k32[nn][w] : k16[nn][w];
-    for (int s = 1; s <= 64 && s <= std::max(1, steps / 4) && (s == 1 || tiles * s <= 4 * units); s *= 2) {
+    for (int s = 1; s <= 64 && s <= std::max(1, steps / 4) && (s == 1 || tiles * s <= 4 * units); s += s < 8 ? 1 : s < 16 ? 2 : s < 32 ? 4 : 8) {
       const int each = (steps + s - 1) / s, parts = (steps + each - 1) / each;
       const long wgs = tiles * parts, most = (wgs + units - 1) / units;
       const double deep = KS * each / 4096.0;
