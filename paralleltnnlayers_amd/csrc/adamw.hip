@@ -383,7 +383,7 @@ __global__ __launch_bounds__(64 * kNormWaves, 8) void norm_kernel(const NormArgs
   __syncthreads();
   sum = block_sum(sum, lds);
   if (threadIdx.x == 0) {
-    const float norm = (float)(sqrt(sum) * (double)a.scale);
+    const float norm = (float)(sqrt(sum) * fabs((double)a.scale));
     const bool finite = fabsf(norm) < __uint_as_float(0x7f800000u);
     a.coefficient[0] = a.scale * fminf(a.max_norm / (norm + 1e-6f), 1.0f);
     a.coefficient[1] = finite ? 1.0f : 0.0f;
