@@ -291,12 +291,44 @@ def rcp_conv2d(x, K0, K1, KC, pad):
     return RCPConv2dFunction.apply(x, K0, K1, KC, pad)
 
 
+class AdapterLinearFunction(torch.autograd.Function):
+    """``adapter_linear`` as a Python autograd function: stands for the native one
+    (csrc/torch/binding.cpp) where a call has to be seen as an operator, in a trace."""
+
+    @staticmethod
+    def forward(ctx, x, W, A, B, ids, scale=None, bias=None):
+        need = ctx.needs_input_grad
+        if need[1] or need[5] or need[6]:
+            raise ValueError("the projection, its bias and the scales are not trained: detach them")
+        factors = need[2] or need[3]
+        # (made by an operator, or the trace would not know it)
+        y = torch.empty(x.shape[:-1] + W.shape[:1], dtype=x.dtype, device=x.device)
+        kept = None
+        if factors:
+            _, kept = capi.adapter_forward(x, W, A, B, ids, scale, bias, out=y, keep=True)
+        else:
+            capi.adapter_forward(x, W, A, B, ids, scale, bias, out=y)
+        ctx.save_for_backward(x if factors else None, W, A, B, ids, scale, kept)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, W, A, B, ids, scale, kept = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx, dA, dB = capi.adapter_backward(dy.to(W.dtype), x, W, A, B, ids, scale, kept, want_dx=need[0],
+                                           want_factors=need[2] or need[3])
+        return dx, None, dA if need[2] else None, dB if need[3] else None, None, None, None
+
+
 def adapter_linear(x, W, A, B, ids, scale=None, bias=None):
     """Functional form of a dense projection with the low-rank adapters of many requests
     beside it (``capi.adapter_forward``), differentiable in x, A and B.
 
     W and bias are frozen: a call that asks for their gradient raises ``ValueError``."""
-    return capi._native.adapter_linear(x, W, A, B, ids, scale, bias)
+    # torch.jit.trace records operators: the native call would leave a constant in the graph
+    if torch._C._get_tracing_state() is None:
+        return capi._native.adapter_linear(x, W, A, B, ids, scale, bias)
+    return AdapterLinearFunction.apply(x, W, A, B, ids, scale, bias)
 
 
 class AdapterLinear(torch.nn.Module):

@@ -1,0 +1,79 @@
+"""``adapter_linear`` and its module as a program uses them: traced, converted, hooked, differentiated."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from paralleltnnlayers_amd import capi, torch_ops
+    capi.lib()
+    return torch_ops
+
+
+def small(ops, **kw):
+    """A module whose adapters are not nothing, a batch and its ids."""
+    torch.manual_seed(3)
+    layer = ops.AdapterLinear(64, 48, 8, adapters=3, bias=torch.randn(48), **kw)
+    with torch.no_grad():
+        layer.B.copy_(torch.randn(layer.B.shape))
+    x = torch.randn(10, 64, device="cuda").to(layer.A.dtype)
+    return layer, x, torch.tensor([0, 1, 2, -1, 2, 2, 1, 0, 0, 1], device="cuda", dtype=torch.int32)
+
+
+@pytest.mark.parametrize("grad", [True, False], ids=["training", "serving"])
+def test_traced_layer_computes_from_its_inputs(ops, grad):
+    """A trace holds the layer as an operator: run on another batch and other ids it gives their result."""
+    layer, x, ids = small(ops)
+
+    class Program(torch.nn.Module):
+        """(with something that depends on x by itself, so that tracing would not notice a constant part)"""
+        def __init__(self):
+            super().__init__()
+            self.layer = layer
+
+        def forward(self, x, ids):
+            return self.layer(x, ids) + x[:, :48]
+
+    program = Program()
+    with torch.set_grad_enabled(grad):
+        traced = torch.jit.trace(program, (x, ids), check_trace=False)
+        for other, which in ((torch.randn_like(x), ids), (x, ids.flip(0).contiguous()), (torch.randn_like(x), ids.long())):
+            assert torch.equal(traced(other, which), program(other, which))
+
+
+def test_traced_module_has_its_own_gradients(ops):
+    layer, x, ids = small(ops)
+    traced = torch.jit.trace(layer, (x, ids), check_trace=False)
+    dy = torch.randn(10, 48, device="cuda")
+    grads = []
+    for run in (layer, traced):
+        leaf = x.clone().requires_grad_()
+        layer.zero_grad()
+        run(leaf, ids).backward(dy)
+        grads.append([leaf.grad, layer.A.grad, layer.B.grad])
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+@pytest.mark.parametrize("wanted", [("x",), ("A",), ("x", "B"), ("x", "A", "B")], ids="".join)
+def test_python_autograd_function_matches_the_native_one(ops, wanted):
+    layer, x, ids = small(ops)
+    dy = torch.randn(10, 48, device="cuda")
+    results = []
+    for run in (ops.AdapterLinearFunction.apply, ops.adapter_linear):
+        d = dict(x=x.clone(), A=layer.A.detach().clone(), B=layer.B.detach().clone())
+        for k in wanted:
+            d[k].requires_grad_()
+        y = run(d["x"], layer.weight, d["A"], d["B"], ids, layer.scale, layer.bias)
+        results.append([y.detach(), *torch.autograd.grad(y, [d[k] for k in wanted], dy)])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_what_is_frozen_is_refused_in_a_trace(ops):
+    layer, x, ids = small(ops)
+    for frozen in (layer.weight, layer.scale, layer.bias):
+        frozen.requires_grad_()
+        with pytest.raises(ValueError, match="not trained"):
+            torch.jit.trace(layer, (x, ids), check_trace=False)
+        frozen.requires_grad_(False)
