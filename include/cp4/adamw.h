@@ -16,7 +16,8 @@
  * left) share one fp32 scale for m and one for v, their largest magnitude.  m's code is an int8
  * q for sign(q) q^2 scale / 127^2, v's a uint8 q for q^4 scale_sq / 255^4, both rounded to
  * nearest-even in q; a v above zero has a code of at least 1, so that a small second moment never
- * becomes none.  The step itself uses m and v before they are rounded.  A block in which a
+ * becomes none (it reads as 2^-149 or more, the least fp32 value).  The step itself uses m and v
+ * before they are rounded.  A block in which a
  * moment is infinite or NaN has NaN scales (all of its moments read as NaN); one whose largest
  * magnitude is below the smallest normal number has the scale zero.
  */

@@ -119,13 +119,23 @@ __device__ __forceinline__ unsigned wave_max(unsigned x) {
 constexpr float kUnitM = (float)(1.0 / (127.0 * 127.0));
 constexpr float kUnitV = (float)(1.0 / (255.0 * 255.0 * 255.0 * 255.0));
 
-__device__ __forceinline__ float decode_m(signed char q, float unit) {
-  const int i = q;
-  return (float)(i < 0 ? -i * i : i * i) * unit;
+// What a block's codes are multiplied by.  A small scale times a unit would leave the normal numbers (a second moment's
+// from 2^-94 on, where its values are still some): it is taken 2^64 times as large, and the product brought down again.
+struct Unit {
+  float unit, down;
+  unsigned least;                                  // the bits of the smallest value that a code above 0 stands for
+};
+__device__ __forceinline__ Unit unit_of(float scale, float unit) {
+  const bool small = scale < 1.0f;
+  return {(small ? scale * 0x1p64f : scale) * unit, small ? 0x1p-64f : 1.0f, scale > 0.0f ? 1u : 0u};
 }
-__device__ __forceinline__ float decode_v(unsigned char q, float unit) {
+__device__ __forceinline__ float decode_m(signed char q, Unit u) {
+  const int i = q;
+  return (float)(i < 0 ? -i * i : i * i) * u.unit * u.down;
+}
+__device__ __forceinline__ float decode_v(unsigned char q, Unit u) {
   const float q2 = (float)((unsigned)q * q);
-  return q2 * q2 * unit;
+  return __uint_as_float(max(__float_as_uint(q2 * q2 * u.unit * u.down), min((unsigned)q, u.least)));
 }
 // A block's scale and what its values are multiplied by for their codes.
 __device__ __forceinline__ float scale_of(unsigned top, float* over) {
@@ -239,7 +249,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void step_kernel(const StepArgs<Eig
           float m[4], v[4];
           Four<RawP> np;
           Four<float> wide;
-          const float um = Eight ? sm[u] * kUnitM : 0.0f, uv = Eight ? sv[u] * kUnitV : 0.0f;
+          const Unit um = Eight ? unit_of(sm[u], kUnitM) : Unit{}, uv = Eight ? unit_of(sv[u], kUnitV) : Unit{};
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             if constexpr (Eight) {
@@ -421,7 +431,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void moments_kernel(const MomentArg
       Four<signed char> qm[kUnroll];
       Four<unsigned char> qv[kUnroll];
       Four<float> fm[kUnroll], fv[kUnroll];
-      float um[kUnroll], uv[kUnroll];
+      Unit um[kUnroll], uv[kUnroll];
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) {
         const size_t at = at0 + u * kBlock + lane * 4, b = at0 / kBlock + u;
@@ -432,8 +442,8 @@ __global__ __launch_bounds__(64 * kWaves, 4) void moments_kernel(const MomentArg
         } else {
           qm[u] = load_four<kAll>(m8, at, n);
           qv[u] = load_four<kAll>(v8, at, n);
-          um[u] = there ? it.s[b] * kUnitM : 0.0f;
-          uv[u] = there ? it.s2[b] * kUnitV : 0.0f;
+          um[u] = unit_of(there ? it.s[b] : 0.0f, kUnitM);
+          uv[u] = unit_of(there ? it.s2[b] : 0.0f, kUnitV);
         }
       }
 #pragma unroll

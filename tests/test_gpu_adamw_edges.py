@@ -33,3 +33,56 @@ def test_clipping_with_a_negative_grad_scale(optim, scale, most):
     got, want = step(G, scale), step([-g for g in G], -scale)        # (a sign is exact)
     assert float(got[0]) > 0
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def in_64_bits(qm, qv, scales):
+    """What codes and scales stand for, by the definition."""
+    at = torch.arange(qm.numel()) // 256
+    m, v, s = qm.cpu().double(), qv.cpu().double(), scales.cpu().double()
+    return m * m.abs() / 127.0 ** 2 * s[0][at], (v / 255.0) ** 4 * s[1][at]
+
+
+# A moment is read with four roundings or fewer (its units' constant, the scale times that, the code's fourth power, their
+# product), and is a denormal number below 2^-126, 2^-149 apart.
+UNITS, STEP = 4 * 2.0 ** -24, 2.0 ** -149
+
+
+@pytest.mark.parametrize("top", [3e38, 1e10, 1.5, 0.75, 1e-28, 1e-30, 1e-35, 1e-36, 2e-38])
+def test_moments_of_any_scale(optim, top):
+    """Blocks of every level, from the largest scales to the smallest: read as in 64 bits, and a second moment above zero
+    never as zero."""
+    q = torch.arange(256)
+    m, v = ((q - 127).clamp(max=127).double() / 127), (q.double() / 255)
+    m, v = (m * m.abs() * top).float(), (v ** 4 * top).float()
+    v[1:3] = 2.0 ** -149                                             # far below the least level of most of these blocks
+    qm, qv, s = optim.empty_moments(torch.empty(256, device="cuda"), 8)
+    optim.set_moments([qm], [qv], [s], ([m.cuda()], [v.cuda()]))
+    above = v > 0                                                    # (the least levels of the smallest blocks are no numbers)
+    assert torch.equal(qv.cpu() > 0, above)
+    (a,), (b,) = optim.moment_values([qm], [qv], [s])
+    for got, want in zip((a, b), in_64_bits(qm, qv, s)):
+        assert ((got.cpu().double() - want).abs() <= UNITS * want.abs() + STEP).all()
+    assert torch.equal(b.cpu() > 0, above)
+    normal = v >= 2.0 ** -126
+    assert torch.equal(qv.cpu()[normal].long(), q[normal])           # (a level comes back as itself)
+
+
+def test_a_step_without_eps_on_tiny_moments(optim):
+    """eps = 0 and gradients that have become zero: the step divides by what the codes still hold."""
+    gen = torch.Generator().manual_seed(2)
+    n = 512
+    v = (0.1 + 0.9 * torch.rand(n, generator=gen)) * 1e-36
+    m = v.double().sqrt().float() * (0.5 + torch.rand(n, generator=gen)) * (1 - 2 * torch.randint(0, 2, (n,), generator=gen))
+    p = torch.randn(n, generator=gen)
+    qm, qv, s = optim.empty_moments(torch.empty(n, device="cuda"), 8)
+    optim.set_moments([qm], [qv], [s], ([m.cuda()], [v.cuda()]))
+    M, V = in_64_bits(qm, qv, s)
+    lr, (b1, b2), t = 1e-3, (0.9, 0.99), 10
+    count = torch.tensor([t - 1, b1 ** (t - 1), b2 ** (t - 1), 0.0], dtype=torch.float64, device="cuda")
+    got = p.cuda()
+    optim.adamw_step([got], [torch.zeros(n, device="cuda")], [qm], [qv], count, scales=[s], lr=lr, betas=(b1, b2), eps=0.0,
+                     weight_decay=0.0)
+    step = lr * (b1 * M / (1 - b1 ** t)) / (b2 * V / (1 - b2 ** t)).sqrt()
+    # four roundings each in reading m and v, two in each moment's update, a root, a quotient and three factors
+    allowed = 2.0 ** -24 * (16 * step.abs() + 4 * p.double().abs())
+    assert ((got.cpu().double() - (p.double() - step)).abs() <= allowed).all()
