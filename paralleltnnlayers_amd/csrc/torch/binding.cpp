@@ -800,10 +800,10 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     }
     list.push_back(t);
   }
-  const double max_norm = a[8] == Py_None ? 0.0 : PyFloat_AsDouble(a[8]);
+  const float max_norm = a[8] == Py_None ? 0.0f : (float)PyFloat_AsDouble(a[8]);
   const double grad_scale = PyFloat_AsDouble(a[9]);
   if (PyErr_Occurred()) throw python_error();
-  require(a[8] == Py_None || max_norm > 0, "max_norm must be above 0");
+  require(a[8] == Py_None || max_norm > 0, "max_norm must be above 0 (in float32)");
   const c10::DeviceGuard guard(like.device());
   void* st = stream_of(a[10]);
   Tensor norm;
@@ -816,7 +816,7 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
       ws = scratch(need, like);
       norm = empty({}, at::kFloat, like);
     }
-    check(cp4_adamw_step(list.data(), list.size(), groups.data(), n_groups, (float)grad_scale, (float)max_norm,
+    check(cp4_adamw_step(list.data(), list.size(), groups.data(), n_groups, (float)grad_scale, max_norm,
                          static_cast<float*>(ptr(norm)), ptr(ws), need, st));
   }
   for (const auto* l : {&params, &ms, &vs, &scales, &copies}) written(*l);

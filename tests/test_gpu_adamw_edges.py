@@ -86,3 +86,15 @@ def test_a_step_without_eps_on_tiny_moments(optim):
     # four roundings each in reading m and v, two in each moment's update, a root, a quotient and three factors
     allowed = 2.0 ** -24 * (16 * step.abs() + 4 * p.double().abs())
     assert ((got.cpu().double() - (p.double() - step)).abs() <= allowed).all()
+
+
+def test_a_max_norm_that_float32_does_not_have(optim):
+    """One that would round to zero is refused, as zero is; the least one clips to almost nothing."""
+    p, g = torch.zeros(4, device="cuda"), torch.ones(4, device="cuda")
+    m, v, _ = optim.empty_moments(p)
+    step = lambda most: optim.adamw_step([p], [g], [m], [v], optim.counter(), max_norm=most, **HYPER)  # noqa: E731
+    with pytest.raises(AssertionError, match="max_norm"):
+        step(1e-46)
+    assert not m.any()
+    assert float(step(1e-30)) == 2.0
+    assert ((m > 0) & (m < 1e-30)).all()
