@@ -734,10 +734,11 @@ void moments_of(cp4_adamw_tensor& t, const Tensor& m, const Tensor& v, const Ten
   t.scale = static_cast<float*>(scales.data_ptr());
   t.scale_sq = t.scale + scales.stride(0);
 }
-// What autograd has saved of a tensor that is written here is out of date.
-void written(const TensorList& list) {
+// What autograd has saved of a tensor that is written here is out of date (where: those that are, or all).
+void written(const TensorList& list, const TensorList* where = nullptr) {
   for (size_t i = 0; i < list.size(); ++i)
-    if (list.has(i) && !list[i].is_inference()) list[i].unsafeGetTensorImpl()->bump_version();
+    if (list.has(i) && (!where || where->has(i)) && !list[i].is_inference())
+      list[i].unsafeGetTensorImpl()->bump_version();
 }
 
 // (params, grads, exp_avgs, exp_avg_sqs, scales, copies, group of each or None,
@@ -819,7 +820,7 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     check(cp4_adamw_step(list.data(), list.size(), groups.data(), n_groups, (float)grad_scale, max_norm,
                          static_cast<float*>(ptr(norm)), ptr(ws), need, st));
   }
-  for (const auto* l : {&params, &ms, &vs, &scales, &copies}) written(*l);
+  for (const auto* l : {&params, &ms, &vs, &scales, &copies}) written(*l, &grads);
   for (const Tensor& c : counters)
     if (!c.is_inference()) c.unsafeGetTensorImpl()->bump_version();
   if (!norm.defined()) Py_RETURN_NONE;

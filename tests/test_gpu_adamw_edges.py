@@ -98,3 +98,20 @@ def test_a_max_norm_that_float32_does_not_have(optim):
     assert not m.any()
     assert float(step(1e-30)) == 2.0
     assert ((m > 0) & (m < 1e-30)).all()
+
+
+def test_a_parameter_without_a_gradient_is_left_alone(optim):
+    """Nothing of it is written, and what autograd has saved of it stays good."""
+    p, q = torch.ones(4, device="cuda"), torch.full((4,), 2.0, device="cuda")
+    M = [optim.empty_moments(t) for t in (p, q)]
+    copies = [torch.zeros(4, device="cuda"), torch.zeros(4, device="cuda")]
+    x = torch.ones(4, device="cuda", requires_grad=True)
+    y = (x * q).sum()                                                # (saves q)
+    lists = [p, *M[0][:2], copies[0]], [q, *M[1][:2], copies[1]]
+    before = [[t._version for t in ts] for ts in lists]
+    optim.adamw_step([p, q], [torch.ones_like(p), None], [m for m, _, _ in M], [v for _, v, _ in M], optim.counter(),
+                     copies=copies, **HYPER)
+    assert all(t._version > b for t, b in zip(lists[0], before[0]))
+    assert [t._version for t in lists[1]] == before[1] and not copies[1].any()
+    y.backward()
+    assert torch.equal(x.grad, q)
