@@ -64,14 +64,17 @@ def set_moments(exp_avgs, exp_avg_sqs, scales, values, stream=None):
 
 
 class AdamW(torch.optim.Optimizer):
-    """AdamW, all parameters of all groups in one launch (one for every 75 of the same types, 57
+    """AdamW, all parameters of a group in one launch (one for every 75 of the same types, 57
     with 8-bit moments).
 
     state_bits: 32, or 8 for the moments of parameters of at least ``min_8bit_size`` values.
     masters: 16-bit parameters are copies of float32 ones that the optimizer keeps (``True``) or
     are stepped in their own 16 bits.  max_norm: all gradients together are scaled down to this norm;
     ``step`` returns nothing then, the norm is ``last_norm``, and a step whose norm is not finite
-    changes nothing.  Groups may have rates of their own (lr, betas, eps, weight_decay)."""
+    changes nothing.  Groups may have rates of their own (lr, betas, eps, weight_decay).
+
+    Steps are counted for each parameter, from its own first gradient on and only where it has one.  Parameters of a
+    group whose counts have parted are launched apart."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32,
                  min_8bit_size=4096, masters=True, max_norm=None):
@@ -96,6 +99,31 @@ class AdamW(torch.optim.Optimizer):
                 s["master"] = p.detach().float()
         return s
 
+    def _count(self, states, idle):
+        """Gives each of ``states`` (of a group's parameters that are about to step) the count of its own steps
+        and returns the counts and whose is whose.  Parameters that have always stepped together share one, a launch
+        between them; one that others keep as it is (``idle``: the ids of those) is copied for the ones that go on."""
+        counts, place, of = [], {}, []
+        for s in states:
+            old = s.get("counter")
+            k = place.get(id(old))
+            if k is None:
+                if old is None:
+                    new = counter(s["exp_avg"].device)
+                elif id(old) in idle:
+                    if torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("AdamW: parameters that have stepped together so far part here; take such a "
+                                           "step before the capture, a replay would repeat the copy of their count")
+                    new = old.clone()
+                else:
+                    new = old
+                k = place[id(old)] = len(counts)
+                counts.append(new)
+            s["counter"] = counts[k]
+            of.append(k)
+        idle.update(map(id, counts))                                 # (another group's parameters do not share them)
+        return counts, of
+
     @torch.no_grad()
     def step(self, closure=None, grad_scale=1.0):
         loss = None
@@ -103,14 +131,18 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         params, grads, ms, vs, scales, copies, of, groups = [], [], [], [], [], [], [], []
+        idle, parts = set(), []
         for group in self.param_groups:
-            used = False
+            states = []
             for p in group["params"]:
                 if p.grad is None:
+                    if p in self.state:
+                        idle.add(id(self.state[p].get("counter")))
                     continue
                 if not p.is_contiguous():
                     raise ValueError("AdamW takes contiguous parameters")
                 s = self._state(p)
+                states.append(s)
                 master = s.get("master")
                 params.append(p if master is None else master)
                 copies.append(None if master is None else p)
@@ -118,26 +150,46 @@ class AdamW(torch.optim.Optimizer):
                 ms.append(s["exp_avg"])
                 vs.append(s["exp_avg_sq"])
                 scales.append(s.get("scales"))
-                of.append(len(groups))
-                used = True
-            if used:
-                if "counter" not in group:
-                    group["counter"] = counter(params[-1].device)
-                groups.append((group["lr"], *group["betas"], group["eps"], group["weight_decay"],
-                               group["counter"]))
+            parts.append((group, states))
+        for group, states in parts:
+            counts, whose = self._count(states, idle)
+            of += [len(groups) + k for k in whose]
+            rates = group["lr"], *group["betas"], group["eps"], group["weight_decay"]
+            groups += [(*rates, c) for c in counts]
         if groups:
             self.last_norm = capi._native.adamw_step(params, grads, ms, vs, scales, copies, of, groups,
                                                      self.max_norm, grad_scale, None)
         return loss
 
     def load_state_dict(self, state_dict):
-        """As torch's, but every state keeps its own type (torch would cast it to its parameter's)."""
+        """As torch's, but every state keeps its own type (torch would cast it to its parameter's).  A state of
+        ``torch.optim.AdamW`` is taken as well: its moments as 32-bit ones, its count of steps with the powers of the betas."""
+        of = {}                                                      # the saved group of each saved state
+        for saved in state_dict["param_groups"]:
+            of.update((i, saved) for i in saved["params"])
+            if saved.get("amsgrad") or saved.get("maximize"):
+                raise ValueError("AdamW: a state with amsgrad or maximize is not this optimizer's")
+        for i, s in state_dict["state"].items():
+            if s and "counter" not in s and "step" not in s and "counter" not in of[i]:
+                raise ValueError("AdamW: moments without a count of steps")
         super().load_state_dict(state_dict)
-        mine = [p for g in self.param_groups for p in g["params"]]
-        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
-        for i, p in zip(ids, mine):
-            if i in state_dict["state"]:
-                self.state[p] = {k: t.detach().to(p.device, copy=True) for k, t in state_dict["state"][i].items()}
-        for g in self.param_groups:
-            if "counter" in g:
-                g["counter"] = g["counter"].detach().to(g["params"][0].device, copy=True)
+        for saved, group in zip(state_dict["param_groups"], self.param_groups):
+            group.pop("counter", None)                               # (states saved before parameters had their own)
+            shared = {}                                              # counts that are equal go on as one
+            for i, p in zip(saved["params"], group["params"]):
+                if not state_dict["state"].get(i):
+                    continue
+                state = dict(state_dict["state"][i])
+                count = state.pop("counter", saved.get("counter"))
+                step = state.pop("step", None)
+                if count is None:
+                    t, (beta1, beta2) = float(step), group["betas"]
+                    count = torch.tensor([t, beta1 ** t, beta2 ** t, 0.0], dtype=torch.float64)
+                    state = {k: state[k].float() for k in ("exp_avg", "exp_avg_sq")}
+                    if self.masters and p.dtype != torch.float32:
+                        state["master"] = p.detach().float()
+                key = tuple(count.tolist())
+                if key not in shared:
+                    shared[key] = count.detach().to(p.device, torch.float64, copy=True)
+                self.state[p] = {k: t.detach().to(p.device, copy=True) for k, t in state.items()}
+                self.state[p]["counter"] = shared[key]
