@@ -108,6 +108,7 @@ class AdamW(torch.optim.Optimizer):
             old = s.get("counter")
             k = place.get(id(old))
             if k is None:
+                new = old
                 if old is None:
                     new = counter(s["exp_avg"].device)
                 elif id(old) in idle:
@@ -115,11 +116,10 @@ class AdamW(torch.optim.Optimizer):
                         raise RuntimeError("AdamW: parameters that have stepped together so far part here; take such a "
                                            "step before the capture, a replay would repeat the copy of their count")
                     new = old.clone()
-                else:
-                    new = old
                 k = place[id(old)] = len(counts)
                 counts.append(new)
-            s["counter"] = counts[k]
+            if old is not counts[k]:
+                s["counter"] = counts[k]
             of.append(k)
         idle.update(map(id, counts))                                 # (another group's parameters do not share them)
         return counts, of
@@ -135,7 +135,8 @@ class AdamW(torch.optim.Optimizer):
         for group in self.param_groups:
             states = []
             for p in group["params"]:
-                if p.grad is None:
+                g = p.grad
+                if g is None:
                     if p in self.state:
                         idle.add(id(self.state[p].get("counter")))
                     continue
@@ -146,14 +147,14 @@ class AdamW(torch.optim.Optimizer):
                 master = s.get("master")
                 params.append(p if master is None else master)
                 copies.append(None if master is None else p)
-                grads.append(p.grad if p.grad.is_contiguous() else p.grad.contiguous())
+                grads.append(g if g.is_contiguous() else g.contiguous())
                 ms.append(s["exp_avg"])
                 vs.append(s["exp_avg_sq"])
                 scales.append(s.get("scales"))
             parts.append((group, states))
         for group, states in parts:
             counts, whose = self._count(states, idle)
-            of += [len(groups) + k for k in whose]
+            of += [len(groups) + k for k in whose] if groups else whose
             rates = group["lr"], *group["betas"], group["eps"], group["weight_decay"]
             groups += [(*rates, c) for c in counts]
         if groups:
