@@ -88,6 +88,11 @@ class AdamW(torch.optim.Optimizer):
         self.state_bits, self.min_8bit_size = state_bits, min_8bit_size
         self.masters, self.max_norm, self.last_norm = masters, max_norm, None
 
+    def __getstate__(self):
+        """What a copy or a pickle takes along (torch's optimizers keep all of theirs in groups)."""
+        own = ("state_bits", "min_8bit_size", "masters", "max_norm", "last_norm")
+        return {**super().__getstate__(), **{k: getattr(self, k) for k in own}}
+
     def _state(self, p):
         s = self.state[p]
         if not s:

@@ -108,3 +108,18 @@ def test_states_that_are_refused():
     with pytest.raises(ValueError, match="without a count"):
         opt.load_state_dict(bare)
     assert not opt.state                                             # (refused before anything is taken)
+
+
+@pytest.mark.parametrize("how", ["deepcopy", "pickle"])
+def test_copies_of_the_optimizer(how):
+    """A copy has the optimizer's settings and its state, counts still shared."""
+    import pickle
+    P = params(5, 300)
+    count = torch.tensor([2, 0.9 ** 2, 0.999 ** 2, 0.0], dtype=torch.float64)
+    opt = our_state(P, (count, count), bits=8)
+    opt.max_norm, opt.masters = 2.0, False
+    new = copy.deepcopy(opt) if how == "deepcopy" else pickle.loads(pickle.dumps(opt))
+    assert (new.state_bits, new.min_8bit_size, new.masters, new.max_norm, new.last_norm) == (8, 1, False, 2.0, None)
+    a, b = (new.state[p]["counter"] for p in new.param_groups[0]["params"])
+    assert a is b and a is not count and a.tolist() == count.tolist()
+    assert callable(new.step) and new.state_dict()["param_groups"] == opt.state_dict()["param_groups"]
