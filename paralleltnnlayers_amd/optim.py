@@ -96,6 +96,9 @@ class AdamW(torch.optim.Optimizer):
     def _state(self, p):
         s = self.state[p]
         if not s:
+            if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW: a parameter's first step makes its state, and a replay would make it anew; take "
+                                   "that step before the capture")
             bits = 8 if self.state_bits == 8 and p.numel() >= self.min_8bit_size else 32
             s["exp_avg"], s["exp_avg_sq"], scales = empty_moments(p, bits)
             if scales is not None:

@@ -150,3 +150,24 @@ def test_counts_that_part_are_not_captured(optim):
             side.synchronize()
     torch.cuda.current_stream().wait_stream(side)
     assert [float(opt.state[p]["counter"][0]) for p in P] == [5, 1]
+
+
+def test_a_first_step_is_not_captured(optim):
+    """Its moments would be zeroed in every replay: refused, and the parameter has no state then."""
+    P = parameters()[:2]
+    opt = optim.AdamW(P, **HYPER)
+    P[0].grad = torch.ones_like(P[0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        opt.step()
+        P[1].grad = torch.ones_like(P[1])
+        with pytest.raises(RuntimeError, match="first step"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+                opt.step()
+        assert not opt.state.get(P[1])
+        opt.step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert [float(opt.state[p]["counter"][0]) for p in P] == [2, 1]
+    first = P[1].detach() - parameters()[1].detach() * (1 - HYPER["lr"] * HYPER["weight_decay"])
+    assert torch.allclose(first, torch.full_like(first, -HYPER["lr"]), rtol=0, atol=1e-6)
