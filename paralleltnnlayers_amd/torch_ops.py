@@ -337,7 +337,8 @@ class AdapterLinear(torch.nn.Module):
 
     A starts as normal(0, 1 / sqrt(in_features)), B as zero, so that an adapter starts as
     nothing; ``alpha / rank`` scales all of them.  ``weight`` and ``bias``: the projection's, as of
-    a trained layer (kept as buffers); without them it starts as a Kaiming-normal one."""
+    a trained layer (kept as buffers); without them it starts as a Kaiming-normal one.  ``.to(dtype)``, ``.half()``
+    and ``.bfloat16()`` convert the projection and the adapters; scales and bias stay float32."""
 
     def __init__(self, in_features, out_features, rank, adapters=1, alpha=None, weight=None, bias=None,
                  dtype=torch.float32, device="cuda"):
@@ -349,10 +350,20 @@ class AdapterLinear(torch.nn.Module):
         self.register_buffer("weight", weight.detach().to(device, dtype))
         self.register_buffer("bias", None if bias is None else bias.detach().to(device, torch.float32))
         self.register_buffer("scale", torch.full((adapters,), (rank if alpha is None else alpha) / rank,
-                                                 device=device))
+                                                 dtype=torch.float32, device=device))
         self.A = torch.nn.Parameter((torch.randn(adapters, rank, in_features, device=device) *
                                      in_features ** -0.5).to(dtype))
         self.B = torch.nn.Parameter(torch.zeros(adapters, out_features, rank, device=device, dtype=dtype))
+
+    def _apply(self, fn, recurse=True):
+        """Conversions of a network leave the scales and the bias what they are, float32, as the layer takes them."""
+        before = {k: self._buffers[k] for k in ("scale", "bias")}
+        super()._apply(fn, recurse)
+        for k, old in before.items():
+            new = self._buffers[k]
+            if new is not None and new.dtype != torch.float32:
+                self._buffers[k] = old.to(new.device, torch.float32)
+        return self
 
     def forward(self, x, ids):
         return adapter_linear(x, self.weight, self.A, self.B, ids, self.scale, self.bias)

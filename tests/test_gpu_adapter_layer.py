@@ -77,3 +77,22 @@ def test_what_is_frozen_is_refused_in_a_trace(ops):
         with pytest.raises(ValueError, match="not trained"):
             torch.jit.trace(layer, (x, ids), check_trace=False)
         frozen.requires_grad_(False)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+def test_converted_module(ops, dtype):
+    """A converted network's layer runs, forward and backward: as one that was made of that type."""
+    layer, x, ids = small(ops)
+    made = ops.AdapterLinear(64, 48, 8, adapters=3, weight=layer.weight, bias=layer.bias, dtype=dtype)
+    with torch.no_grad():
+        made.A.copy_(layer.A)
+        made.B.copy_(layer.B)
+    layer.to(dtype)
+    dy = torch.randn(10, 48, device="cuda").to(dtype)
+    results = []
+    for m in (layer, made):
+        leaf = x.to(dtype).requires_grad_()
+        y = m(leaf, ids)
+        results.append([y.detach(), *torch.autograd.grad(y, [leaf, m.A, m.B], dy)])
+    assert results[0][0].dtype == dtype
+    assert all(torch.equal(a, b) for a, b in zip(*results))
