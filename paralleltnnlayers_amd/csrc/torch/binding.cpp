@@ -19,6 +19,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <atomic>
@@ -641,6 +642,12 @@ struct AdapterFunction : torch::autograd::Function<AdapterFunction> {
     out[0] = dx;
     if (ctx->needs_input_grad(2)) out[2] = dA;
     if (ctx->needs_input_grad(3)) out[3] = dB;
+    // create_graph: the gradients are the library's and have none of their own; who asks for those is told
+    if (at::GradMode::is_enabled())
+      for (int i : {0, 2, 3})
+        if (out[i].defined())
+          out[i] = (*std::make_shared<torch::autograd::DelayedError>(
+              "the gradients of adapter_linear cannot be differentiated again", 1))({out[i].detach().set_requires_grad(true)})[0];
     return out;
   }
 };

@@ -317,6 +317,9 @@ class AdapterLinearFunction(torch.autograd.Function):
         need = ctx.needs_input_grad
         dx, dA, dB = capi.adapter_backward(dy.to(W.dtype), x, W, A, B, ids, scale, kept, want_dx=need[0],
                                            want_factors=need[2] or need[3])
+        if torch.is_grad_enabled():              # (create_graph: as the native one)
+            told = torch._C._functions.DelayedError(b"the gradients of adapter_linear cannot be differentiated again", 1)
+            dx, dA, dB = (g if g is None else told(g.detach().requires_grad_()) for g in (dx, dA, dB))
         return dx, None, dA if need[2] else None, dB if need[3] else None, None, None, None
 
 
@@ -324,7 +327,8 @@ def adapter_linear(x, W, A, B, ids, scale=None, bias=None):
     """Functional form of a dense projection with the low-rank adapters of many requests
     beside it (``capi.adapter_forward``), differentiable in x, A and B.
 
-    W and bias are frozen: a call that asks for their gradient raises ``ValueError``."""
+    W and bias are frozen: a call that asks for their gradient raises ``ValueError``.  The gradients themselves
+    are not differentiable: after ``create_graph=True`` a second derivative raises."""
     # torch.jit.trace records operators: the native call would leave a constant in the graph
     if torch._C._get_tracing_state() is None:
         return capi._native.adapter_linear(x, W, A, B, ids, scale, bias)

@@ -96,3 +96,24 @@ def test_converted_module(ops, dtype):
         results.append([y.detach(), *torch.autograd.grad(y, [leaf, m.A, m.B], dy)])
     assert results[0][0].dtype == dtype
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.parametrize("traced", [False, True], ids=["native", "python"])
+def test_gradients_are_not_differentiated_again(ops, traced):
+    """create_graph gives the same gradients; a derivative of one of them is refused, not taken as zero."""
+    layer, x, ids = small(ops)
+    apply = ops.AdapterLinearFunction.apply if traced else ops.adapter_linear
+
+    def grads(**kw):
+        leaf = x.clone().requires_grad_()
+        y = apply(leaf, layer.weight, layer.A, layer.B, ids, layer.scale, layer.bias)
+        return leaf, torch.autograd.grad(y.sum(), [leaf, layer.A, layer.B], **kw)
+
+    _, want = grads()
+    leaf, got = grads(create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for g in got:
+        # (what else the loss consists of must not hide it)
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            (g.square().sum() + leaf.sum() + layer.A.sum()).backward(retain_graph=True)
+    assert not want[0].requires_grad
