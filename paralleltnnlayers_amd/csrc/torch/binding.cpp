@@ -577,6 +577,7 @@ PyObject* adapter_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
             "out does not match the result");
     y = adapter_run(p, x.sizes(), y, keep ? &kept : nullptr, st);
   }
+  if (a[7] != Py_None && !y.is_inference()) y.unsafeGetTensorImpl()->bump_version();   // (what autograd saved of it is out of date)
   PyObject* py = THPVariable_Wrap(std::move(y));
   return keep ? Py_BuildValue("(NN)", py, THPVariable_Wrap(std::move(kept))) : py;
   END_HANDLE_TH_ERRORS

@@ -117,3 +117,21 @@ def test_gradients_are_not_differentiated_again(ops, traced):
         with pytest.raises(RuntimeError, match="differentiated again"):
             (g.square().sum() + leaf.sum() + layer.A.sum()).backward(retain_graph=True)
     assert not want[0].requires_grad
+
+
+def test_out_is_written(ops):
+    """A result that goes into a tensor autograd has saved is noticed by its backward pass."""
+    import paralleltnnlayers_amd as cp4
+    layer, x, ids = small(ops)
+    args = x, layer.weight, layer.A.detach(), layer.B.detach(), ids, layer.scale, layer.bias
+    out = torch.zeros(10, 48, device="cuda")
+    leaf = torch.ones(10, 48, device="cuda", requires_grad=True)
+    loss = (leaf * out).sum()
+    y = cp4.adapter_forward(*args, out=out)
+    assert y is out and torch.equal(out, cp4.adapter_forward(*args))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():                 # (a tensor without a version)
+        made = torch.empty(10, 48, device="cuda")
+        cp4.adapter_forward(*args, out=made)
+    assert torch.equal(made, out)
