@@ -466,8 +466,9 @@ std::optional<Tensor> optional_tensor(PyObject* o) {
 // [..., cols] as rows that lie `stride` apart; copied where its last dimensions do not allow that.
 Tensor rows_of(const Tensor& t, size_t* stride) {
   const int64_t cols = t.size(-1);
-  if (t.dim() == 2 && (cols == 1 || t.stride(1) == 1) && t.stride(0) >= cols) {
-    *stride = (size_t)t.stride(0);
+  const bool one = t.dim() == 2 && t.size(0) == 1;  // (a single row's stride says nothing, and may be anything)
+  if (t.dim() == 2 && (cols == 1 || t.stride(1) == 1) && (one || t.stride(0) >= cols)) {
+    *stride = (size_t)(one ? cols : t.stride(0));
     return t;
   }
   *stride = (size_t)cols;

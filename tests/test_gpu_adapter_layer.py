@@ -135,3 +135,20 @@ def test_out_is_written(ops):
         made = torch.empty(10, 48, device="cuda")
         cp4.adapter_forward(*args, out=made)
     assert torch.equal(made, out)
+
+
+@pytest.mark.parametrize("stride", [(1 << 30) + 8, 0, 63], ids=["far", "none", "short"])
+def test_a_single_row_has_no_stride(ops, stride):
+    """The last token of a long sequence: one row, whatever lies between it and the next that is not there."""
+    import paralleltnnlayers_amd as cp4
+    layer, x, ids = small(ops)
+    factors = layer.A.detach(), layer.B.detach(), ids[:1], layer.scale
+    dy = torch.randn(1, 48, device="cuda")
+    row, drow = x[:1].as_strided((1, 64), (stride, 1)), dy.as_strided((1, 48), (stride, 1))
+    one = layer.weight[:1].as_strided((1, 64), (stride, 1))
+    want, kept = cp4.adapter_forward(x[:1], layer.weight, *factors, layer.bias, keep=True)
+    assert torch.equal(cp4.adapter_forward(row, layer.weight, *factors, layer.bias), want)
+    grads = [cp4.adapter_backward(d, r, layer.weight, *factors, kept) for d, r in ((dy, x[:1]), (drow, row))]
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+    narrow = factors[0], factors[1][:, :1].contiguous(), *factors[2:]
+    assert torch.equal(cp4.adapter_forward(row, one, *narrow), cp4.adapter_forward(x[:1], layer.weight[:1], *narrow))
