@@ -1,4 +1,4 @@
-// Device side of the adapters' kernels: operands in registers and the adapters' part of an output tile.
+// Device side of the adapters' kernels: operands from memory in registers, at any alignment, and turned there.
 #ifndef CP4_ADAPTER_LOAD_H
 #define CP4_ADAPTER_LOAD_H
 
