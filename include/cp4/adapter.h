@@ -59,6 +59,17 @@ cp4_status cp4_adapter_backward(const cp4_adapter_shape* shape, int dtype, const
                                 void* dA, void* dB, void* workspace, size_t workspace_bytes,
                                 cp4_stream stream);
 
+/* How the shared projection of a call (backward != 0: that of dx) would run now, for reports and tests: its
+ * launches, the second one for the rows that whole tiles leave over, where those are cheaper on their
+ * own.  aligned: whether its operands' rows start on 16-byte boundaries. */
+typedef struct cp4_adapter_launch {
+  size_t rows;                /* tokens; 0: there is no such launch */
+  int tile_rows, tile_cols;   /* 0 and 0: the kernel of few rows, without tiles */
+  int splits;                 /* parts of the depth */
+} cp4_adapter_launch;
+cp4_status cp4_adapter_plan_query(const cp4_adapter_shape* shape, int dtype, int backward,
+                                  int aligned, cp4_adapter_launch launches[2]);
+
 #ifdef __cplusplus
 }
 #endif

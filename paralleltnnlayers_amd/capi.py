@@ -52,6 +52,11 @@ class AdapterShape(ctypes.Structure):
                 [(k, ctypes.c_size_t) for k in ("ldx", "ldw", "lddy")])
 
 
+class AdapterLaunch(ctypes.Structure):
+    """cp4_adapter_launch."""
+    _fields_ = ([("rows", ctypes.c_size_t)] + [(k, ctypes.c_int) for k in ("tile_rows", "tile_cols", "splits")])
+
+
 class AdamwTensor(ctypes.Structure):
     """cp4_adamw_tensor."""
     _fields_ = ([(k, ctypes.c_void_p) for k in ("param", "grad", "exp_avg", "exp_avg_sq", "scale", "scale_sq",
@@ -229,6 +234,7 @@ def lib():
                                       [ctypes.c_size_t, ctypes.c_void_p])
     L.cp4_adapter_backward.argtypes = ([ctypes.POINTER(AdapterShape), ctypes.c_int] + [ctypes.c_void_p] * 12 +
                                        [ctypes.c_size_t, ctypes.c_void_p])
+    L.cp4_adapter_plan_query.argtypes = [ctypes.POINTER(AdapterShape)] + [ctypes.c_int] * 3 + [ctypes.POINTER(AdapterLaunch)]
     L.cp4_adamw_workspace_bytes.restype = ctypes.c_size_t
     _T = ctypes.POINTER(AdamwTensor)
     L.cp4_adamw_step.argtypes = [_T, ctypes.c_size_t, ctypes.POINTER(AdamwGroup), ctypes.c_size_t, ctypes.c_float,
@@ -345,6 +351,15 @@ def adapter_backward(dy, x, W, A, B, ids, scale=None, kept=None, want_dx=True, w
     if stream is None:
         return _native.adapter_backward(*args)
     return _ordered(stream, _native.adapter_backward, *args)
+
+
+def adapter_plan(T, K, N, R, G, dtype=torch.float32, backward=False, aligned=True):
+    """[(rows, (tile rows, tile columns) or None, parts of the depth)] of the launches that the shared projection of
+    ``adapter_forward`` (``backward``: of dx) would run with now; None: the kernel of few rows.  ``aligned``:
+    whether the operands' rows start on 16-byte boundaries."""
+    s, out = AdapterShape(T=T, K=K, N=N, R=R, G=G), (AdapterLaunch * 2)()
+    check(lib().cp4_adapter_plan_query(ctypes.byref(s), _DTYPES[dtype], int(backward), int(aligned), out))
+    return [(o.rows, (o.tile_rows, o.tile_cols) if o.tile_rows else None, o.splits) for o in out if o.rows]
 
 
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1}

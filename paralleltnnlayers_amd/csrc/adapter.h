@@ -65,6 +65,8 @@ bool project_sums_planes(const ProjectArgs&, int dtype, bool nn);
 // part: project_part_bytes of scratch memory.
 size_t project_part_bytes(size_t T, int K, int N, int G, int dtype, bool nn);
 hipError_t project_launch(const ProjectArgs&, float* part, int dtype, bool nn, hipStream_t);
+// What project_launch runs: one launch, or one of whole tiles and one of the rows that are left over.
+void project_plan(size_t T, int K, int N, int G, int dtype, bool nn, bool direct, cp4_adapter_launch (&launches)[2]);
 // The tiles of a projection on the matrix cores, its depth in `splits` parts of `each` steps, whose partial
 // sums take tile_part_bytes.
 struct TilePlan {
@@ -73,6 +75,8 @@ struct TilePlan {
 };
 TilePlan tile_plan(size_t T, int K, int N, int dtype, bool nn, bool direct);
 size_t tile_part_bytes(const TilePlan&, size_t T, int N);
+int tile_rows(const TilePlan&);
+int tile_cols(const TilePlan&);
 // Whether these operands go from memory to the LDS without passing a register.
 bool tile_direct(const ProjectArgs&, int dtype, bool nn);
 hipError_t tile_launch(const ProjectArgs&, const TilePlan&, float* part, int dtype, bool nn, hipStream_t);

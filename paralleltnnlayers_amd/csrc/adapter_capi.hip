@@ -157,3 +157,15 @@ extern "C" cp4_status cp4_adapter_backward(const cp4_adapter_shape* s, int dtype
   }
   return CP4_OK;
 }
+
+extern "C" cp4_status cp4_adapter_plan_query(const cp4_adapter_shape* s, int dtype, int backward, int aligned,
+                                             cp4_adapter_launch launches[2]) {
+  if (const cp4_status rc = check_shape(s, dtype)) return rc;
+  if (!launches) return fail_with(CP4_ERR_NULL_POINTER, "launches is NULL");
+  cp4_adapter_launch l[2];
+  const int K = (int)(backward ? s->N : s->K), N = (int)(backward ? s->K : s->N);
+  project_plan(s->T, K, N, (int)s->G, dtype, backward != 0, aligned != 0, l);
+  launches[0] = l[0];
+  launches[1] = l[1];
+  return CP4_OK;
+}

@@ -65,6 +65,18 @@ size_t project_part_bytes(size_t T, int K, int N, int G, int dtype, bool nn) {
   return most;
 }
 
+void project_plan(size_t T, int K, int N, int G, int dtype, bool nn, bool direct, cp4_adapter_launch (&launches)[2]) {
+  const auto one = [&](size_t rows) {
+    if (!rows) return cp4_adapter_launch{};
+    if (by_rows(rows, K, N, G, dtype, nn, direct)) return cp4_adapter_launch{rows, 0, 0, rows_plan(rows, K, N, dtype).splits};
+    const TilePlan p = tile_plan(rows, K, N, dtype, nn, direct);
+    return cp4_adapter_launch{rows, tile_rows(p), tile_cols(p), p.splits};
+  };
+  const size_t main = main_rows(T, K, N, G, dtype, nn, direct);
+  launches[0] = one(main);
+  launches[1] = one(T - main);
+}
+
 bool project_sums_planes(const ProjectArgs& a, int dtype, bool nn) {
   return by_rows(a.T, a.K, a.N, a.G, dtype, nn, tile_direct(a, dtype, nn));
 }

@@ -680,6 +680,8 @@ TilePlan tile_plan(size_t T, int K, int N, int dtype, bool nn, bool aligned) {
   }
   return best;
 }
+int tile_rows(const TilePlan& p) { return kRows[p.which]; }
+int tile_cols(const TilePlan& p) { return kCols[p.which]; }
 size_t tile_part_bytes(const TilePlan& p, size_t T, int N) { return p.splits > 1 ? (size_t)p.splits * T * N * 4 : 0; }
 
 // Whether the LDS can be filled directly: 16-byte boundaries, and a thread's places in a tile as 32-bit byte offsets.
