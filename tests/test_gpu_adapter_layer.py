@@ -152,3 +152,66 @@ def test_a_single_row_has_no_stride(ops, stride):
     assert all(torch.equal(a, b) for a, b in zip(*grads))
     narrow = factors[0], factors[1][:, :1].contiguous(), *factors[2:]
     assert torch.equal(cp4.adapter_forward(row, one, *narrow), cp4.adapter_forward(x[:1], layer.weight[:1], *narrow))
+
+
+def test_saved_tensor_hooks_see_what_the_layer_saves(ops):
+    """Offloading the saved tensors changes nothing; what is saved is the operands and h."""
+    layer, x, ids = small(ops)
+    dy = torch.randn(10, 48, device="cuda")
+
+    def grads(run):
+        leaf = x.clone().requires_grad_()
+        return torch.autograd.grad(run(leaf), [leaf, layer.A, layer.B], dy)
+
+    def offloaded(leaf):
+        with torch.autograd.graph.save_on_cpu():
+            return layer(leaf, ids)
+
+    want = grads(lambda leaf: layer(leaf, ids))
+    assert all(torch.equal(a, b) for a, b in zip(grads(offloaded), want))
+    shapes = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: (shapes.append(tuple(t.shape)), t)[1], lambda t: t):
+        layer(x.clone().requires_grad_(), ids)
+    h = (10 * 16,)                               # (10 tokens, rank 8 in rows of 16)
+    assert sorted(shapes) == sorted([tuple(t.shape) for t in (x, layer.weight, layer.A, layer.B, ids, layer.scale)] + [h])
+
+
+def test_what_hooks_spoil_is_refused(ops):
+    """h given back in another type is no h: an error, never a gradient of it."""
+    layer, x, ids = small(ops)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.double() if t.shape == (160,) else t, lambda t: t):
+        y = layer(x, ids)
+    with pytest.raises(AssertionError, match="kept"):
+        y.sum().backward()
+
+
+def test_forward_mode_tangents_are_refused(ops):
+    import torch.autograd.forward_ad as fwd
+    layer, x, ids = small(ops)
+    with torch.no_grad(), fwd.dual_level():
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            layer(fwd.make_dual(x, torch.ones_like(x)), ids)
+
+
+def test_functional_transforms_are_refused(ops):
+    """The library sees memory, not batched or wrapped tensors: an error, never a result."""
+    import paralleltnnlayers_amd as cp4
+    layer, x, ids = small(ops)
+    W, A, B, s = layer.weight, layer.A.detach(), layer.B.detach(), layer.scale
+    both = lambda t: torch.stack([t, t])  # noqa: E731
+    _, kept = cp4.adapter_forward(x, W, A, B, ids, keep=True)
+    dy = torch.randn(10, 48, device="cuda")
+    with torch.no_grad():
+        calls = [lambda: torch.vmap(lambda t: layer(t, ids))(both(x)), lambda: torch.vmap(lambda t: layer(x, t))(both(ids)),
+                 lambda: torch.vmap(lambda t: layer(x, t))(both(ids.long())),
+                 lambda: torch.vmap(lambda t: cp4.adapter_forward(x, W, t, B, ids))(both(A)),
+                 lambda: torch.vmap(lambda t: cp4.adapter_forward(x, W, A, B, ids, t))(both(s)),
+                 lambda: torch.vmap(lambda t: cp4.adapter_backward(t, x, W, A, B, ids, kept=kept)[0])(both(dy))]
+    leaf = x.clone().requires_grad_()
+    y = layer(leaf, ids)
+    calls += [lambda: torch.func.grad(lambda t: layer(t, ids).sum())(x),
+              lambda: torch.func.jvp(lambda t: layer(t, ids), (x,), (x,)),
+              lambda: torch.autograd.grad(y, leaf, both(dy), is_grads_batched=True)]
+    for call in calls:
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            call()
