@@ -16,8 +16,10 @@
  * (16 bits) where the layer's type has 16 bits.  Outputs are rounded once, to nearest-even.  No
  * atomics: results do not change from call to call.  An adapter that no token uses has zero
  * gradients.  What is not finite stays with its own: a token's x and dy with that token's rows of y and dx and with its
- * adapter's gradients, an adapter with its own tokens and gradients.  (An infinity in an fp32 operand, in h or
- * in dh may come out as NaN, since these are taken apart into bfloat16 parts.)
+ * adapter's gradients, an adapter with its own tokens and gradients.  (An infinity may come out as NaN: in an fp32
+ * operand anywhere, in a 16-bit one wherever it meets an adapter.  fp32 operands, h, dh and float16 ranks are taken
+ * apart into bfloat16 parts, of which an infinity's are an infinity and NaN, and places that fill up a block of
+ * products are multiplied by zero.)
  *
  * All pointers are device pointers.  Rows of x, W and dy may be further apart than they are long
  * (ldx, ldw, lddy, in elements); A, B, y, dx, dA and dB are contiguous.  Any alignment of the

@@ -25,7 +25,8 @@
 //
 // Measured: 8192 x 4096 x 4096 bf16 with adapters of rank 16: 212 us, 1.30 PFLOP/s (nn 239; the library's product
 // alone 179), bound by the LDS's bandwidth beside the matrix cores; 2048 x 4096 x 8192 121 us; 1031 x 2048 x 2816 f16, rank 64:
-// 30 us (nn 42), bound by what the L2 gives the LDS (4 rooms instead of 3 change nothing); 64 x 25088 x 4096 fp32 93 us, 4.4 TB/s of W.
+// 30 us (nn 42), one workgroup a compute unit (three rooms of 32 KB leave as little place for a second one as four, and are as
+// fast), so that nothing overlaps its barriers and the adapters' loads behind the depth; 64 x 25088 x 4096 fp32 93 us, 4.4 TB/s of W.
 #include <algorithm>
 #include <type_traits>
 
