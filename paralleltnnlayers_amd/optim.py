@@ -179,7 +179,7 @@ class AdamW(torch.optim.Optimizer):
             if saved.get("amsgrad") or saved.get("maximize"):
                 raise ValueError("AdamW: a state with amsgrad or maximize is not this optimizer's")
         for i, s in state_dict["state"].items():
-            if s and "counter" not in s and "step" not in s and "counter" not in of[i]:
+            if s and "counter" not in s and "step" not in s and "counter" not in of.get(i, {}):
                 raise ValueError("AdamW: moments without a count of steps")
         super().load_state_dict(state_dict)
         for saved, group in zip(state_dict["param_groups"], self.param_groups):

@@ -123,3 +123,12 @@ def test_copies_of_the_optimizer(how):
     a, b = (new.state[p]["counter"] for p in new.param_groups[0]["params"])
     assert a is b and a is not count and a.tolist() == count.tolist()
     assert callable(new.step) and new.state_dict()["param_groups"] == opt.state_dict()["param_groups"]
+
+
+def test_a_state_of_no_group():
+    """One that belongs to no parameter of a group, and has no count: refused like any other."""
+    P = params(5)
+    state = our_state(P, (torch.zeros(4, dtype=torch.float64),)).state_dict()
+    state["state"][9] = {"exp_avg": torch.zeros(5), "exp_avg_sq": torch.zeros(5)}
+    with pytest.raises(ValueError, match="without a count"):
+        optim.AdamW(params(5)).load_state_dict(state)
