@@ -362,6 +362,22 @@ def adapter_plan(T, K, N, R, G, dtype=torch.float32, backward=False, aligned=Tru
     return [(o.rows, (o.tile_rows, o.tile_cols) if o.tile_rows else None, o.splits) for o in out if o.rows]
 
 
+def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, out=None, keep=False, stream=None):
+    """y = (x - mean) / sqrt(variance + eps) * weight + bias over x's last dimension (up to 32768 values).
+
+    x [..., D] float32, bfloat16 or float16; weight and bias [D] float32 (None: 1 and 0).  ``keep``: also returns
+    what ``layer_norm_backward`` needs of this pass."""
+    args = (x, weight, bias, eps, out, keep, stream)
+    return _native.layer_norm_forward(*args) if stream is None else _ordered(stream, _native.layer_norm_forward, *args)
+
+
+def layer_norm_backward(dy, x, weight, stats, want_dx=True, want_weight=True, want_bias=True, stream=None):
+    """(dx, dweight, dbias) of ``layer_norm_forward`` for dy [..., D]; ``stats``: what that call left.  What is not
+    wanted is None."""
+    args = (dy, x, weight, stats, want_dx, want_weight, want_bias, stream)
+    return _native.layer_norm_backward(*args) if stream is None else _ordered(stream, _native.layer_norm_backward, *args)
+
+
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1}
 
 

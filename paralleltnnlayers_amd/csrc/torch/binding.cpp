@@ -30,6 +30,7 @@
 #include "cp4/adamw.h"
 #include "cp4/adapter.h"
 #include "cp4/capi.h"
+#include "cp4/layer_norm.h"
 
 namespace {
 
@@ -681,6 +682,172 @@ PyObject* adapter_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- layer norm (capi.layer_norm_*, torch_ops.layer_norm) -----------------------------------------
+
+struct NormRows {
+  size_t T = 0, ld = 0;
+  unsigned D = 0;
+  int dtype = 0;
+  Tensor x, weight, bias;                          // as the C ABI takes them
+};
+// Checks the operands of a layer norm; x: [..., D].
+NormRows norm_rows(const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias) {
+  NormRows p;
+  require(x.is_cuda(), "expected device tensors");
+  require(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= 32768, "expected x [..., D], D from 1 to 32768");
+  for (const auto& t : {weight, bias})
+    require(!t || (t->is_cuda() && t->device() == x.device() && t->scalar_type() == at::kFloat && t->dim() == 1 &&
+                   t->size(0) == x.size(-1)),
+            "weight and bias must be float32 vectors of x's last dimension, on x's device");
+  p.dtype = dtype_of(x);
+  p.D = (unsigned)x.size(-1);
+  p.T = (size_t)(x.numel() / x.size(-1));
+  p.x = rows_of(x, &p.ld);
+  if (weight) p.weight = weight->contiguous();
+  if (bias) p.bias = bias->contiguous();
+  return p;
+}
+Tensor norm_run(const NormRows& p, at::IntArrayRef sizes, float eps, Tensor y, Tensor* stats, void* st) {
+  if (!y.defined()) y = empty(sizes, p.x.scalar_type(), p.x);
+  if (stats) *stats = empty({(int64_t)p.T, 2}, at::kFloat, p.x);
+  check(cp4_layer_norm_forward(p.T, p.D, p.dtype, ptr(p.x), p.ld, floats(p.weight), floats(p.bias), eps, ptr(y),
+                               stats ? static_cast<float*>(ptr(*stats)) : nullptr, st));
+  return y;
+}
+// dx, dweight, dbias as far as they are wanted.
+void norm_run_backward(const Tensor& dy_in, const Tensor& x, const std::optional<Tensor>& weight, const Tensor& stats,
+                       Tensor* dx, Tensor* dw, Tensor* db, void* st) {
+  const NormRows p = norm_rows(x, weight, std::nullopt);
+  require(dy_in.is_cuda() && dy_in.device() == x.device() && dy_in.scalar_type() == x.scalar_type() &&
+              dy_in.sizes() == x.sizes(),
+          "dy does not match x");
+  require(stats.defined() && stats.is_cuda() && stats.device() == x.device() && stats.scalar_type() == at::kFloat &&
+              stats.is_contiguous() && (size_t)stats.numel() == 2 * p.T,
+          "stats is not what the forward call left");
+  size_t lddy = 0;
+  const Tensor dy = rows_of(dy_in, &lddy);
+  if (dx) *dx = empty(x.sizes(), x.scalar_type(), x);
+  for (Tensor* t : {dw, db})
+    if (t) *t = empty({(int64_t)p.D}, at::kFloat, x);
+  const size_t need = dw || db ? cp4_layer_norm_backward_workspace_bytes(p.T, p.D) : 0;
+  const Tensor ws = scratch(need, x);
+  check(cp4_layer_norm_backward(p.T, p.D, p.dtype, ptr(dy), lddy, ptr(p.x), p.ld, floats(p.weight), floats(stats),
+                                dx ? ptr(*dx) : nullptr, dw ? static_cast<float*>(ptr(*dw)) : nullptr,
+                                db ? static_cast<float*>(ptr(*db)) : nullptr, ptr(ws), need, st));
+}
+float real(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw python_error();
+  return (float)v;
+}
+PyObject* or_none(Tensor&& t) {
+  if (t.defined()) return THPVariable_Wrap(std::move(t));
+  Py_RETURN_NONE;
+}
+
+// (x, weight, bias, eps, out, keep, stream) -> y, or (y, stats)
+PyObject* layer_norm_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  require(n == 7);
+  const Tensor& x = tensor(a[0]);
+  const auto weight = optional_tensor(a[1]), bias = optional_tensor(a[2]);
+  const float eps = real(a[3]);
+  Tensor y = a[4] != Py_None ? tensor(a[4]) : Tensor(), stats;
+  const bool keep = PyObject_IsTrue(a[5]) == 1;
+  require(x.is_cuda(), "expected device tensors");
+  const c10::DeviceGuard guard(x.device());
+  void* st = stream_of(a[6]);
+  {
+    NoGil unlocked;
+    const at::NoGradGuard no_grad;
+    const NormRows p = norm_rows(x, weight, bias);
+    require(!y.defined() || (y.is_cuda() && y.device() == x.device() && y.scalar_type() == x.scalar_type() &&
+                             y.is_contiguous() && y.numel() == x.numel()),
+            "out does not match the result");
+    y = norm_run(p, x.sizes(), eps, y, keep ? &stats : nullptr, st);
+  }
+  if (a[4] != Py_None && !y.is_inference()) y.unsafeGetTensorImpl()->bump_version();
+  PyObject* py = THPVariable_Wrap(std::move(y));
+  return keep ? Py_BuildValue("(NN)", py, THPVariable_Wrap(std::move(stats))) : py;
+  END_HANDLE_TH_ERRORS
+}
+
+// (dy, x, weight, stats, want_dx, want_weight, want_bias, stream) -> (dx, dweight, dbias)
+PyObject* layer_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  require(n == 8);
+  const Tensor &dy = tensor(a[0]), &x = tensor(a[1]), &stats = tensor(a[3]);
+  const auto weight = optional_tensor(a[2]);
+  const bool want[3] = {PyObject_IsTrue(a[4]) == 1, PyObject_IsTrue(a[5]) == 1, PyObject_IsTrue(a[6]) == 1};
+  require(x.is_cuda(), "expected device tensors");
+  const c10::DeviceGuard guard(x.device());
+  void* st = stream_of(a[7]);
+  Tensor g[3];
+  {
+    NoGil unlocked;
+    const at::NoGradGuard no_grad;
+    norm_run_backward(dy, x, weight, stats, want[0] ? &g[0] : nullptr, want[1] ? &g[1] : nullptr, want[2] ? &g[2] : nullptr, st);
+  }
+  return Py_BuildValue("(NNN)", or_none(std::move(g[0])), or_none(std::move(g[1])), or_none(std::move(g[2])));
+  END_HANDLE_TH_ERRORS
+}
+
+struct LayerNormFunction : torch::autograd::Function<LayerNormFunction> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& weight,
+                        const std::optional<Tensor>& bias, double eps) {
+    const NormRows p = norm_rows(x, weight, bias);
+    Tensor stats;
+    Tensor y = norm_run(p, x.sizes(), (float)eps, Tensor(), &stats,
+                        c10::hip::getCurrentHIPStream(x.device().index()).stream());
+    ctx->save_for_backward({x, weight ? *weight : Tensor(), stats});
+    return y;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grad) {
+    const auto s = ctx->get_saved_variables();
+    torch::autograd::variable_list out(4);
+    if (!grad[0].defined()) return out;
+    const Tensor dy = grad[0].scalar_type() == s[0].scalar_type() ? grad[0] : grad[0].to(s[0].scalar_type());
+    const std::optional<Tensor> weight = s[1].defined() ? std::optional<Tensor>(s[1]) : std::nullopt;
+    Tensor g[3];
+    norm_run_backward(dy, s[0], weight, s[2], ctx->needs_input_grad(0) ? &g[0] : nullptr,
+                      ctx->needs_input_grad(1) ? &g[1] : nullptr, ctx->needs_input_grad(2) ? &g[2] : nullptr,
+                      c10::hip::getCurrentHIPStream(dy.device().index()).stream());
+    for (int i = 0; i < 3; ++i) {
+      out[i] = g[i];
+      if (g[i].defined() && at::GradMode::is_enabled())            // (create_graph: as adapter_linear's)
+        out[i] = (*std::make_shared<torch::autograd::DelayedError>(
+            "the gradients of layer_norm cannot be differentiated again", 1))({g[i].detach().set_requires_grad(true)})[0];
+    }
+    return out;
+  }
+};
+
+// (x, weight, bias, eps) -> y; see torch_ops.layer_norm
+PyObject* layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  require(n == 4);
+  const Tensor& x = tensor(a[0]);
+  const auto weight = optional_tensor(a[1]), bias = optional_tensor(a[2]);
+  const float eps = real(a[3]);
+  require(x.is_cuda(), "expected device tensors");
+  const c10::DeviceGuard guard(x.device());
+  auto tracked = [](const Tensor& t) {
+    return (at::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined();
+  };
+  Tensor y;
+  {
+    NoGil unlocked;
+    if (tracked(x) || (weight && tracked(*weight)) || (bias && tracked(*bias)))
+      y = LayerNormFunction::apply(x, weight, bias, eps);
+    else
+      y = norm_run(norm_rows(x, weight, bias), x.sizes(), eps, Tensor(), nullptr,
+                   c10::hip::getCurrentHIPStream(x.device().index()).stream());
+  }
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
 // ---- AdamW over many tensors (optim.py) --------------------------------------------------------
 
 // The tensors of a list or tuple, held by a tuple of their own (a Tensor's count of owners is an atomic: 65
@@ -891,6 +1058,9 @@ PyMethodDef kMethods[] = {
     {"adapter_forward", FAST(adapter_forward), nullptr},
     {"adapter_backward", FAST(adapter_backward), nullptr},
     {"adapter_linear", FAST(adapter_linear), nullptr},
+    {"layer_norm_forward", FAST(layer_norm_forward), nullptr},
+    {"layer_norm_backward", FAST(layer_norm_backward), nullptr},
+    {"layer_norm", FAST(layer_norm), nullptr},
     {"adamw_step", FAST(adamw_step), nullptr},
     {"adamw_moments", FAST(adamw_moments), nullptr},
     {"set_error", set_error, METH_O, nullptr},

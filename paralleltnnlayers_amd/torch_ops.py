@@ -371,3 +371,55 @@ class AdapterLinear(torch.nn.Module):
 
     def forward(self, x, ids):
         return adapter_linear(x, self.weight, self.A, self.B, ids, self.scale, self.bias)
+
+
+class LayerNormFunction(torch.autograd.Function):
+    """``layer_norm`` as a Python autograd function: stands for the native one (csrc/torch/binding.cpp) where a
+    call has to be seen as an operator, in a trace."""
+
+    @staticmethod
+    def forward(ctx, x, weight=None, bias=None, eps=1e-5):
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)     # (made by an operator, or the trace would not know it)
+        _, stats = capi.layer_norm_forward(x, weight, bias, eps, out=y, keep=True)
+        ctx.save_for_backward(x, weight, stats)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, weight, stats = ctx.saved_tensors
+        grads = capi.layer_norm_backward(dy.to(x.dtype), x, weight, stats, *ctx.needs_input_grad[:3])
+        if torch.is_grad_enabled():              # (create_graph: as the native one)
+            told = torch._C._functions.DelayedError(b"the gradients of layer_norm cannot be differentiated again", 1)
+            grads = tuple(g if g is None else told(g.detach().requires_grad_()) for g in grads)
+        return *grads, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """Functional form of the layer norm over x's last dimension (``capi.layer_norm_forward``), differentiable in
+    x, weight and bias.  The gradients themselves are not differentiable."""
+    # torch.jit.trace records operators: the native call would leave a constant in the graph
+    if torch._C._get_tracing_state() is None:
+        return capi._native.layer_norm(x, weight, bias, eps)
+    return LayerNormFunction.apply(x, weight, bias, eps)
+
+
+class LayerNorm(torch.nn.Module):
+    """Layer norm over the last dimension of ``features`` values, with a weight and (``bias``) a bias that start as
+    1 and 0.  ``.to(dtype)``, ``.half()`` and ``.bfloat16()`` of a network leave both float32, as the layer takes them:
+    its output is of its input's type."""
+
+    def __init__(self, features, eps=1e-5, bias=True, device="cuda"):
+        super().__init__()
+        self.eps = eps
+        self.weight = torch.nn.Parameter(torch.ones(features, device=device))
+        self.bias = torch.nn.Parameter(torch.zeros(features, device=device)) if bias else None
+
+    def _apply(self, fn, recurse=True):
+        """Conversions of a network leave weight and bias float32."""
+        def kept(t):
+            new = fn(t)
+            return new if new.dtype == torch.float32 else t.to(new.device)
+        return super()._apply(kept, recurse)
+
+    def forward(self, x):
+        return layer_norm(x, self.weight, self.bias, self.eps)
