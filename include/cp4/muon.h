@@ -1,0 +1,52 @@
+/*
+ * C ABI of the Muon step over many matrices: each is moved along its momentum, orthogonalised by
+ * Newton-Schulz products.  For the CP factors, adapters and dense layers that the library's gradients belong
+ * to, beside the AdamW step of cp4/adamw.h.  No counterpart in the reference.
+ *
+ *   m = momentum m + grad           u = grad + momentum m  (nesterov), or m
+ *   X = u / (|u| + eps)             |u| the root of the sum of squares
+ *   X = a X + (b A + c A A) X,      A = X X^T  (X transposed where it has more rows than columns), `steps` times,
+ *                                   a, b, c = 3.4445, -4.7750, 2.0315
+ *   p = p (1 - lr weight_decay) - lr sqrt(max(1, rows / cols)) X
+ *
+ * The polynomial takes every singular value from 0.01 or so up into 0.68 .. 1.21 in five steps and keeps it there.
+ * m, p's step and all sums are fp32 or wider whatever the types in memory.  Matrices with a side of up to 64 go through
+ * their Gram matrix, summed and iterated in fp64; larger ones through products of values in two float16 parts
+ * (22 bits; accumulated in fp32).  No atomics: results do not change from call to call.  A matrix whose u has
+ * an infinity or a NaN becomes NaN in whole; others are not touched by it.
+ */
+#ifndef CP4_MUON_H
+#define CP4_MUON_H
+
+#include "cp4/capi.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* `count` matrices of the same shape, one behind the other; all pointers are device pointers to
+ * contiguous, row-major values, aligned to their type. */
+typedef struct cp4_muon_matrix {
+  void* param;          /* of param_dtype, updated; NULL: no step is taken */
+  const void* grad;     /* of grad_dtype */
+  float* momentum;      /* updated; NULL: u is grad */
+  void* copy;           /* NULL, or of copy_dtype: the new parameters, rounded (with param) */
+  void* out;            /* NULL, or of out_dtype: X */
+  size_t count;
+  unsigned rows, cols;  /* up to 65536 each; nothing is read or written where one of the three is 0 */
+  int param_dtype, grad_dtype, copy_dtype, out_dtype;   /* cp4_dtype */
+} cp4_muon_matrix;
+
+/* One step.  Asynchronous on `stream`, kernel launches only: three for up to 24 entries with a side of up to 64, and
+ * 3 steps + 2 for up to 16 larger ones whose scratch memory stays below 1 GiB together (a larger matrix on its
+ * own).  steps: 1 to 16.  eps: above 0.  workspace: cp4_muon_workspace_bytes() of device memory, 256-byte aligned, its
+ * contents scratch.  Matrices must not overlap one another. */
+size_t cp4_muon_workspace_bytes(const cp4_muon_matrix* matrices, size_t count);
+cp4_status cp4_muon_step(const cp4_muon_matrix* matrices, size_t count, double lr, double momentum,
+                         int nesterov, double weight_decay, double eps, unsigned steps,
+                         void* workspace, size_t workspace_bytes, cp4_stream stream);
+
+#ifdef __cplusplus
+}
+#endif
+#endif

@@ -1,0 +1,318 @@
+// Products of matrices in two float16 parts for the Muon step (muon.h): C = alpha E + beta P Q^T of many matrices in one
+// launch, on the matrix cores.
+//
+// A value is hi + lo, 22 bits, a product hi hi + hi lo + lo hi: what is dropped is below 2^-22 of it, so three
+// float16 instructions stand for an fp32 product (16 times an fp32 matrix instruction's work a cycle each; bfloat16 would need
+// six for as many bits, and two of its parts leave an orthogonalised 1024 x 1024 matrix 2.4e-5 off 64 bits
+// where these leave 1.8e-6 and fp32 1.7e-6).  Newton-Schulz keeps its matrices' values below 3, so float16's range is no
+// limit.
+//
+// A tile is 128 x 128 (64 x 64 where that leaves compute units without one), four waves of 64 x 64 (32 x 32); a step is
+// 32 of the depth, one cache line of every row, from memory to the LDS without passing a register, the next step under
+// way while one is multiplied.  A wave's column block j holds the columns NB l + j, so that a lane has NB consecutive values
+// of a row; its four rows of a block are consecutive too, so C and C transposed leave in wide stores both.
+// Symmetric products (two of the three of an iteration) have the tiles on and below the diagonal alone, the others are
+// mirrored: 4 instead of 6 m^3 for a square matrix.
+#include <algorithm>
+
+#include "die_order.h"
+#include "muon.h"
+
+namespace cp4 {
+namespace muon {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+enum Kind { kParts, kFinal, kPartial };
+
+struct TileArgs {
+  Product p[kProducts];
+  unsigned first[kProducts];                       // each entry's first workgroup
+  unsigned tiles[kProducts];                       // of a matrix
+  unsigned total;
+  int count, splits, steps;                        // steps: of a part of the depth (the last one may have fewer)
+};
+static_assert(sizeof(TileArgs) <= 4096, "kernel arguments");
+
+constexpr int wait_for(int loads) { return (loads & 15) | (loads >> 4) << 14 | 7 << 4; }
+
+template <int MB, int Rooms, int What>
+__global__ __launch_bounds__(256, 2) void product_kernel(const TileArgs a) {
+  constexpr int NB = MB, B = 32 * MB, kLoads = B * 8 / 256, kRoom = 2 * B * 128;
+  __shared__ __attribute__((aligned(1024))) char lds0[kRoom], lds1[kRoom], lds2[Rooms > 2 ? kRoom : 16], lds3[Rooms > 3 ? kRoom : 16];
+  const int place = die_place(blockIdx.x, a.total);
+  if (place < 0) return;
+  int entry = 0;
+  while (entry + 1 < a.count && (unsigned)place >= a.first[entry + 1]) ++entry;
+  const Product& p = a.p[entry];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 15, g = lane >> 4;
+  const unsigned in_entry = place - a.first[entry];
+  const unsigned split = in_entry % a.splits, matrix = in_entry / a.splits / a.tiles[entry];
+  const int tile = in_entry / a.splits % a.tiles[entry];
+  int tm, tn;
+  if (p.symmetric) {
+    tm = (int)((__builtin_sqrtf(8.0f * tile + 1.0f) - 1.0f) * 0.5f);
+    while (tm * (tm + 1) / 2 > tile) --tm;
+    while ((tm + 1) * (tm + 2) / 2 <= tile) ++tm;
+    tn = tile - tm * (tm + 1) / 2;
+  } else {                                         // up to eight columns of tiles wide, then the next ones
+    const int mt = (p.R + B - 1) / B, nt = (p.N + B - 1) / B, band = tile / (8 * mt), in_band = tile % (8 * mt), wide = min(8, nt - 8 * band);
+    tm = in_band / wide;
+    tn = 8 * band + in_band % wide;
+  }
+  const int R = p.R, N = p.N, m0 = tm * B, n0 = tn * B, wm = 16 * MB * (wave >> 1), wn = 16 * NB * (wave & 1);
+  const size_t ldk = padded(p.K) * 4, ldn = padded(p.N) * 4, ldr = padded(p.R) * 4;
+  const int depth = (int)(ldk / 128), k_first = split * a.steps, steps = min(depth - k_first, a.steps);
+  const char* pb = p.P + (size_t)matrix * p.R * ldk + m0 * ldk + (size_t)k_first * 128;
+  const char* qb = p.Q + (size_t)matrix * p.N * ldk + n0 * ldk + (size_t)k_first * 128;
+  // A thread's places: the LDS is filled in the threads' order; rows beyond the operand's are read again from its
+  // last one (what they give is not stored), and a row's pieces lie in another order in each row, so that a column of
+  // them is in all banks.
+  unsigned po[kLoads], qo[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int at = i * 256 + threadIdx.x, row = at / 8, piece = (at % 8) ^ (row & 7);
+    const int in = row % (16 * NB), col = row - in + NB * (in & 15) + in / 16;
+    po[i] = (unsigned)(min(row, R - 1 - m0) * ldk) + piece * 16;
+    qo[i] = (unsigned)(min(col, N - 1 - n0) * ldk) + piece * 16;
+  }
+  int brought = 0;
+  auto bring = [&](char* lds) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(pb + po[i]),
+                                       (__attribute__((address_space(3))) void*)(lds + (i * 256 + wave * 64) * 16), 16, 0, 0);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(qb + qo[i]),
+                                       (__attribute__((address_space(3))) void*)(lds + B * 128 + (i * 256 + wave * 64) * 16), 16, 0, 0);
+    const bool more = ++brought < steps;           // (beyond the last step that one again)
+    pb += more ? 128 : 0;
+    qb += more ? 128 : 0;
+  };
+  f32x4 acc[MB][NB] = {};
+  const int p_at = (wm + l) * 128, q_at = B * 128 + (wn + l) * 128;
+  auto multiply = [&](const char* lds) __attribute__((always_inline)) {
+    f16x8 ph[MB], pl[MB], qh[NB], ql[NB];
+    const int h = (g ^ (l & 7)) * 16, lo = ((4 + g) ^ (l & 7)) * 16;
+#pragma unroll
+    for (int i = 0; i < MB; ++i) ph[i] = *reinterpret_cast<const f16x8*>(lds + p_at + h + i * 16 * 128);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) qh[j] = *reinterpret_cast<const f16x8*>(lds + q_at + h + j * 16 * 128);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) ql[j] = *reinterpret_cast<const f16x8*>(lds + q_at + lo + j * 16 * 128);
+#pragma unroll
+    for (int i = 0; i < MB; ++i) pl[i] = *reinterpret_cast<const f16x8*>(lds + p_at + lo + i * 16 * 128);
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int i = 0; i < MB; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[i], qh[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int i = 0; i < MB; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[i], ql[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int i = 0; i < MB; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[i], qh[j], acc[i][j], 0, 0, 0);
+  };
+  // A step: its own loads have arrived (those of later ones may still be on their way), and nobody reads the last
+  // one's room any more.
+  auto step = [&](const char* lds, char* into) __attribute__((always_inline)) {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(wait_for((Rooms - 2) * 2 * kLoads));
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    bring(into);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(lds);
+  };
+  if (steps > 0) {
+    auto ahead = [&](char* lds) __attribute__((always_inline)) {
+      bring(lds);
+      asm volatile("" ::: "memory");               // (their order is what the waits count on)
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    ahead(lds0);
+    if constexpr (Rooms > 2) ahead(lds1);
+    if constexpr (Rooms > 3) ahead(lds2);
+    int left = steps;
+    for (; left >= Rooms; left -= Rooms) {
+      if constexpr (Rooms == 2) {
+        step(lds0, lds1);
+        step(lds1, lds0);
+      } else {
+        step(lds0, lds3);
+        step(lds1, lds0);
+        step(lds2, lds1);
+        step(lds3, lds2);
+      }
+    }
+    if (left > 0) step(lds0, Rooms == 2 ? lds1 : lds3);
+    if constexpr (Rooms > 3) {
+      if (left > 1) step(lds1, lds0);
+      if (left > 2) step(lds2, lds1);
+    }
+    __builtin_amdgcn_s_waitcnt(wait_for(0));       // (the loads beyond the last step)
+  }
+
+  const int n = n0 + wn + NB * l;
+  if constexpr (What == kPartial) {
+    float* const out = p.part + ((size_t)matrix * a.splits + split) * R * N;
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const int r = m0 + wm + 16 * i + 4 * g + v;
+        float x[NB];
+#pragma unroll
+        for (int j = 0; j < NB; ++j) x[j] = acc[i][j][v];
+        if (r < R) store_values<NB>(out, CP4_DTYPE_F32, (size_t)r * N + n, N - n, x);
+      }
+    return;
+  }
+  const float alpha = p.alpha, beta = p.beta * (1.0f / kScale);
+  const char* const E = p.E ? p.E + (size_t)matrix * R * ldn : nullptr;
+  char* const C = p.C + (size_t)matrix * R * ldn;
+  char* Ct = nullptr;
+  if constexpr (What == kParts) {
+    if (p.symmetric && tm != tn) Ct = C;           // (R is N)
+    else if (p.Ct) Ct = p.Ct + (size_t)matrix * N * ldr;
+  }
+  Outputs o;
+  Rates rates;
+  if constexpr (What == kFinal) {
+    o = p.o;
+    rates = p.rates;
+    const size_t at = (size_t)matrix * R * N;
+    const auto shift = [&](void* q, int dtype) { return q ? (char*)q + at * (dtype == CP4_DTYPE_F32 ? 4 : 2) : nullptr; };
+    o.param = shift(o.param, o.param_dtype);
+    o.copy = shift(o.copy, o.copy_dtype);
+    o.out = shift(o.out, o.out_dtype);
+  }
+#pragma unroll
+  for (int i = 0; i < MB; ++i) {
+    const int row = m0 + wm + 16 * i + 4 * g;
+    if (row >= (int)padded(R)) continue;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const int r = row + v;
+      float x[NB], e[NB] = {};
+      if (E && r < R && n < (int)padded(N)) load_parts<NB>(E + (size_t)r * ldn, n, e);
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        x[j] = beta * acc[i][j][v];
+        if (E) x[j] += alpha * e[j];
+        if (r >= R || n + j >= N) x[j] = 0.0f;     // (what fills up the last block of 32)
+        acc[i][j][v] = x[j];
+      }
+      if (r >= R || n >= (int)padded(N)) continue;
+      if constexpr (What == kParts) {
+        store_parts<NB>(C + (size_t)r * ldn, n, x);
+      } else {
+#pragma unroll
+        for (int j = 0; j < NB; ++j) x[j] *= 1.0f / kScale;
+        put_out<NB>(o, rates, (size_t)r * N + n, N - n, x);
+      }
+    }
+    if constexpr (What == kParts)
+      if (Ct)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          float x[4];
+#pragma unroll
+          for (int v = 0; v < 4; ++v) x[v] = acc[i][j][v];
+          if (n + j < N) store_parts<4>(Ct + (size_t)(n + j) * ldr, row, x);
+        }
+  }
+}
+
+// A symmetric C from the parts of its depth: four columns of a row a thread; what lies above the diagonal's tiles (of
+// `edge` rows) is read from below it.
+__global__ __launch_bounds__(256) void join_kernel(const TileArgs a, int edge) {
+  int entry = 0;
+  while (entry + 1 < a.count && blockIdx.x >= a.first[entry + 1]) ++entry;
+  const Product& p = a.p[entry];
+  const unsigned fours = (unsigned)padded(p.N) / 4;
+  const size_t at = (size_t)(blockIdx.x - a.first[entry]) * 256 + threadIdx.x;
+  if (at >= (size_t)p.count * p.R * fours) return;
+  const unsigned c = at % fours * 4, r = at / fours % p.R;
+  const size_t matrix = at / fours / p.R, size = (size_t)p.R * p.N;
+  const float* const part = p.part + matrix * a.splits * size;
+  float x[4] = {};
+  const bool below = r / edge >= c / edge;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (c + j >= p.N) continue;
+    const float* const q = part + (below ? (size_t)r * p.N + c + j : (size_t)(c + j) * p.N + r);
+    for (int s = 0; s < a.splits; ++s) x[j] += q[s * size];
+    x[j] *= p.beta * (1.0f / kScale);
+  }
+  store_parts<4>(p.C + (matrix * p.R + r) * padded(p.N) * 4, c, x);
+}
+
+size_t tiles_of(const Product& p, int edge) {
+  const size_t mt = (p.R + edge - 1) / edge, nt = (p.N + edge - 1) / edge;
+  return p.symmetric ? mt * (mt + 1) / 2 : mt * nt;
+}
+size_t all_tiles(const Product* p, int n, int edge) {
+  size_t t = 0;
+  for (int i = 0; i < n; ++i) t += p[i].count * tiles_of(p[i], edge);
+  return t;
+}
+// Large tiles where they leave no compute unit without one.
+int edge_of(const Product* p, int n) { return all_tiles(p, n, 128) >= (size_t)num_compute_units() ? 128 : 64; }
+int depth_of(const Product* p, int n) {
+  size_t d = 0;
+  for (int i = 0; i < n; ++i) d = std::max(d, padded(p[i].K) / 32);
+  return (int)d;
+}
+
+template <int MB, int Rooms>
+hipError_t launch(const TileArgs& t, Kind kind, hipStream_t st) {
+  const unsigned grid = die_grid((long)t.total);
+  if (kind == kParts) product_kernel<MB, Rooms, kParts><<<grid, 256, 0, st>>>(t);
+  else if (kind == kFinal) product_kernel<MB, Rooms, kFinal><<<grid, 256, 0, st>>>(t);
+  else product_kernel<MB, Rooms, kPartial><<<grid, 256, 0, st>>>(t);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+// Enough parts for two small tiles on every compute unit, of eight steps or more each.
+int product_splits(const Product* p, int n) {
+  const size_t tiles = all_tiles(p, n, 64), units = (size_t)num_compute_units();
+  if (!tiles || edge_of(p, n) == 128) return 1;
+  return (int)std::max<size_t>(1, std::min({2 * units / tiles, (size_t)depth_of(p, n) / 8, (size_t)32}));
+}
+
+hipError_t product_launch(const Product* p, int n, int splits, hipStream_t st) {
+  TileArgs t{};
+  const int edge = edge_of(p, n);
+  t.count = n;
+  const int depth = depth_of(p, n);
+  t.steps = (depth + splits - 1) / splits;
+  t.splits = splits;
+  for (int i = 0; i < n; ++i) {
+    t.p[i] = p[i];
+    t.first[i] = t.total;
+    t.tiles[i] = (unsigned)tiles_of(p[i], edge);
+    t.total += p[i].count * t.tiles[i] * splits;
+  }
+  const Kind kind = splits > 1 ? kPartial : p[0].C ? kParts : kFinal;
+  if (const hipError_t e = edge == 128 ? launch<4, 2>(t, kind, st) : launch<2, 4>(t, kind, st)) return e;
+  if (splits == 1) return hipSuccess;
+  unsigned grid = 0;
+  for (int i = 0; i < n; ++i) {
+    t.first[i] = grid;
+    grid += (unsigned)(((size_t)p[i].count * p[i].R * (padded(p[i].N) / 4) + 255) / 256);
+  }
+  join_kernel<<<grid, 256, 0, st>>>(t, edge);
+  return hipGetLastError();
+}
+
+}  // namespace muon
+}  // namespace cp4

@@ -31,6 +31,7 @@
 #include "cp4/adapter.h"
 #include "cp4/capi.h"
 #include "cp4/layer_norm.h"
+#include "cp4/muon.h"
 
 namespace {
 
@@ -1039,6 +1040,78 @@ PyObject* adamw_moments(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- Muon over many matrices (optim.py) ----------------------------------------------------------
+
+// (params or None, grads, momenta or None, copies or None, outs or None, lr, momentum, nesterov, weight_decay, eps, steps,
+//  stream): a parameter without a gradient is left alone
+PyObject* muon_step(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  require(n_args == 12);
+  const size_t n = length(a[1]);
+  const TensorList params(a[0], n, "one parameter a gradient", true), grads(a[1], n, "expected a list of tensors", true);
+  const TensorList momenta(a[2], n, "one momentum a parameter", true), copies(a[3], n, "one copy (or None) a parameter", true);
+  const TensorList outs(a[4], n, "one output a matrix", true);
+  double of[4];
+  for (int k = 0; k < 4; ++k) {
+    PyObject* const o = a[k < 2 ? 5 + k : 6 + k];
+    of[k] = PyFloat_AsDouble(o);
+    if (of[k] == -1.0 && PyErr_Occurred()) throw python_error();
+  }
+  const bool nesterov = PyObject_IsTrue(a[7]) == 1;
+  const long steps = integer(a[10]);
+  require(steps >= 1 && steps <= 16, "1 to 16 steps");
+  std::vector<cp4_muon_matrix> list;
+  list.reserve(n);
+  const Tensor* like = nullptr;
+  for (size_t i = 0; i < n; ++i) {
+    if (!grads.has(i)) continue;
+    const Tensor& g = grads[i];
+    if (!like) like = &g;
+    require(g.dim() >= 2, "matrices have two dimensions or more: [..., rows, cols]");
+    require(g.size(-1) <= 65536 && g.size(-2) <= 65536, "matrices of up to 65536 rows and columns");
+    cp4_muon_matrix m{};
+    m.rows = (unsigned)g.size(-2);
+    m.cols = (unsigned)g.size(-1);
+    m.count = m.rows && m.cols ? (size_t)(g.numel() / g.size(-1) / g.size(-2)) : 0;
+    const auto of_shape = [&](const Tensor& t, const char* what) {
+      require(t.sizes() == g.sizes(), what);
+      return dense(t, g.numel(), *like, what);
+    };
+    m.grad = of_shape(g, "a gradient is not a contiguous tensor on the others' device");
+    m.grad_dtype = dtype_of(g);
+    if (params.has(i)) {
+      m.param = of_shape(params[i], "a parameter is not contiguous or does not match its gradient");
+      m.param_dtype = dtype_of(params[i]);
+    }
+    if (copies.has(i)) {
+      require(m.param, "a copy without a parameter");
+      m.copy = of_shape(copies[i], "a copy is not contiguous or does not match its parameter");
+      m.copy_dtype = dtype_of(copies[i]);
+    }
+    if (momenta.has(i)) {
+      require(momenta[i].scalar_type() == at::kFloat, "a momentum is float32");
+      m.momentum = static_cast<float*>(of_shape(momenta[i], "a momentum is not contiguous or does not match its parameter"));
+    }
+    if (outs.has(i)) {
+      m.out = of_shape(outs[i], "an output is not contiguous or does not match its matrix");
+      m.out_dtype = dtype_of(outs[i]);
+    }
+    list.push_back(m);
+  }
+  if (list.empty()) Py_RETURN_NONE;
+  const c10::DeviceGuard guard(like->device());
+  void* st = stream_of(a[11]);
+  {
+    NoGil unlocked;
+    const size_t need = cp4_muon_workspace_bytes(list.data(), list.size());
+    const Tensor ws = scratch(need, *like);
+    check(cp4_muon_step(list.data(), list.size(), of[0], of[1], nesterov, of[2], of[3], (unsigned)steps, ptr(ws), need, st));
+  }
+  for (const auto* l : {&params, &momenta, &copies, &outs}) written(*l, &grads);
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 PyObject* set_error(PyObject*, PyObject* type) {
   Py_XINCREF(type);
   Py_XSETREF(g_error, type);
@@ -1063,6 +1136,7 @@ PyMethodDef kMethods[] = {
     {"layer_norm", FAST(layer_norm), nullptr},
     {"adamw_step", FAST(adamw_step), nullptr},
     {"adamw_moments", FAST(adamw_moments), nullptr},
+    {"muon_step", FAST(muon_step), nullptr},
     {"set_error", set_error, METH_O, nullptr},
     {"set_check_backward", set_check_backward, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};

@@ -1,7 +1,8 @@
-"""AdamW over many tensors in one launch, moments in 32 or in 8 bits (include/cp4/adamw.h).
+"""AdamW over many tensors in one launch, moments in 32 or in 8 bits (include/cp4/adamw.h), and Muon over many
+matrices (include/cp4/muon.h).
 
-``AdamW`` is the optimizer of a training loop; ``adamw_step`` is the same step for a program that
-keeps its own lists.  All arithmetic is in the HIP library; there is no eager fallback.  The count
+``AdamW`` and ``Muon`` are the optimizers of a training loop; ``adamw_step`` and ``muon_step`` are the same steps for a
+program that keeps its own lists.  All arithmetic is in the HIP library; there is no eager fallback.  AdamW's count
 of steps lives on the device, so a step records into a HIP graph and counts its replays.
 """
 import torch
@@ -202,3 +203,113 @@ class AdamW(torch.optim.Optimizer):
                     shared[key] = count.detach().to(p.device, torch.float64, copy=True)
                 self.state[p] = {k: t.detach().to(p.device, copy=True) for k, t in state.items()}
                 self.state[p]["counter"] = shared[key]
+
+
+def muon_step(params, grads, momenta, *, lr, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, eps=1e-7,
+              copies=None, stream=None):
+    """One Muon step of all ``params`` (contiguous float32, bfloat16 or float16), in place: each matrix along its
+    momentum, orthogonalised by ``steps`` Newton-Schulz products (up to 16), times ``lr sqrt(max(1, rows / cols))``.
+
+    A parameter is [..., rows, cols]: a stack of matrices that are orthogonalised one by one.  grads: one each, of any
+    of the three types (None: that parameter is left alone).  momenta: float32 of the same shape, zero before the first step.
+    copies: tensors (or None) that receive the new parameters rounded to their type.  A matrix whose momentum is not
+    finite becomes NaN."""
+    run = capi._native.muon_step
+    args = (params, grads, momenta, copies, None, lr, momentum, nesterov, weight_decay, eps, steps, stream)
+    return run(*args) if stream is None else capi._ordered(stream, run, *args)
+
+
+def orthogonalize(updates, steps=5, eps=1e-7, out=None, stream=None):
+    """The matrices of ``updates`` (a tensor or a list of them, [..., rows, cols] each) with their singular values brought
+    to about 1 (0.68 to 1.21) by ``steps`` Newton-Schulz products, each of its own type.  ``out``: where they go, of any of
+    the three types."""
+    if isinstance(updates, torch.Tensor):
+        return orthogonalize([updates], steps, eps, None if out is None else [out], stream)[0]
+    if stream is not None:
+        return capi._ordered(stream, _orthogonalize, updates, steps, eps, out, stream)
+    return _orthogonalize(updates, steps, eps, out, None)
+
+
+def _orthogonalize(updates, steps, eps, out, stream):
+    if out is None:
+        out = [torch.empty(u.shape, dtype=u.dtype, device=u.device) for u in updates]
+    updates = [u.detach() if u.is_contiguous() else u.detach().contiguous() for u in updates]
+    capi._native.muon_step(None, updates, None, None, out, 0.0, 0.0, False, 0.0, eps, steps, stream)
+    return out
+
+
+class Muon(torch.optim.Optimizer):
+    """Muon for parameters that are matrices or stacks of them ([..., rows, cols]): factors, adapters, dense
+    layers.  Biases and norms belong to ``AdamW``.  Three launches for up to 24 parameters whose shorter sides round up to
+    the same multiple of 16 up to 64, seventeen for up to 16 larger ones.
+
+    masters: 16-bit parameters are copies of float32 ones that the optimizer keeps (``True``) or are stepped in their own
+    16 bits.  Groups may have settings of their own (lr, momentum, nesterov, weight_decay, steps, eps)."""
+
+    def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, eps=1e-7, masters=True):
+        if not (lr >= 0 and weight_decay >= 0 and 0 <= momentum < 1):
+            raise ValueError("lr and weight_decay must be 0 or more, momentum in [0, 1)")
+        if not eps > 0 or not 1 <= steps <= 16:
+            raise ValueError("eps must be above 0, steps 1 to 16")
+        self.masters = masters
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps, eps=eps))
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "masters": self.masters}
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        if any(p.dim() < 2 for p in self.param_groups[-1]["params"]):
+            self.param_groups.pop()
+            raise ValueError("Muon takes parameters of two dimensions or more; leave the others to AdamW")
+
+    def _state(self, p):
+        s = self.state[p]
+        if not s:
+            if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("Muon: a parameter's first step makes its state, and a replay would make it anew; take "
+                                   "that step before the capture")
+            s["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+            if self.masters and p.dtype != torch.float32:
+                s["master"] = p.detach().float()
+        return s
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            params, grads, momenta, copies = [], [], [], []
+            for p in group["params"]:
+                g = p.grad
+                if g is None:
+                    continue
+                if not p.is_contiguous():
+                    raise ValueError("Muon takes contiguous parameters")
+                s = self._state(p)
+                master = s.get("master")
+                params.append(p if master is None else master)
+                copies.append(None if master is None else p)
+                grads.append(g if g.is_contiguous() else g.contiguous())
+                momenta.append(s["momentum_buffer"])
+            if params:
+                capi._native.muon_step(params, grads, momenta, copies, None, group["lr"], group["momentum"], group["nesterov"],
+                                       group["weight_decay"], group["eps"], group["steps"], None)
+        return loss
+
+    def load_state_dict(self, state_dict):
+        """As torch's, but every state keeps its own type (torch would cast it to its parameter's)."""
+        super().load_state_dict(state_dict)
+        for saved, group in zip(state_dict["param_groups"], self.param_groups):
+            for i, p in zip(saved["params"], group["params"]):
+                state = state_dict["state"].get(i)
+                if not state:
+                    continue
+                if "momentum_buffer" not in state:
+                    raise ValueError("Muon: a state without a momentum")
+                kept = {"momentum_buffer": state["momentum_buffer"].detach().to(p.device, torch.float32, copy=True)}
+                if self.masters and p.dtype != torch.float32:
+                    kept["master"] = state["master"].detach().to(p.device, copy=True) if "master" in state else p.detach().float()
+                self.state[p] = kept
