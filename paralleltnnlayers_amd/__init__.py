@@ -22,6 +22,7 @@ from .capi import (Shape, Geometry, geometry, conv2d_forward_ex, conv2d_backward
                    random_uniform, time_copy, cp3_shape_for, cp3_expand_factors,
                    cp3_fold_gradients, cp3_conv2d_forward, cp3_conv2d_backward_data,
                    cp3_conv2d_backward_filter, adapter_forward, adapter_backward,
-                   adapter_plan, layer_norm_forward, layer_norm_backward)
+                   adapter_plan, layer_norm_forward, layer_norm_backward, Mx4, mx4_quantize,
+                   mx4_dequantize, mx4_linear, mx4_linear_backward)
 
 __all__ = [n for n in dir() if not n.startswith("_")]

@@ -9,6 +9,7 @@ import ctypes
 import functools
 import inspect
 import os
+import typing
 
 import torch
 
@@ -329,13 +330,55 @@ def conv2d_forward(x, FK, FC, FH, FW, pad=1, out=None, variant=-1, stream=None):
     return _ordered(stream, _native.forward, x, FK, FC, FH, FW, pad, out, variant, stream)
 
 
+class Mx4(typing.NamedTuple):
+    """Rows held in microscaled 4-bit floating point (include/cp4/mx4.h): uint8 codes [..., ceil(K / 32) * 16] and scales
+    [..., ceil(K / 32)] of rows of ``features`` = K values."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    features: int
+
+
+def mx4_quantize(x, stream=None):
+    """x [..., K] (float32, bfloat16 or float16) rounded to microscaled 4-bit floating point: an ``Mx4``.
+
+    Each 32 consecutive values of a row share a power of two, four times which is the largest's; each is rounded to the
+    nearest of 0, 0.5, 1, 1.5, 2, 3, 4 and 6 times that, ties to the even code, what lies beyond to 6.  A block with an infinity or a NaN
+    is NaN in whole."""
+    run = _native.mx4_quantize
+    codes, scales = run(x, stream) if stream is None else _ordered(stream, run, x, stream)
+    return Mx4(codes, scales, x.shape[-1])
+
+
+def mx4_dequantize(q, dtype=torch.float32, out=None, stream=None):
+    """The values of an ``Mx4``, of ``dtype`` (bfloat16 and float32 hold them exactly)."""
+    args = (q, dtype, out, stream)
+    return _native.mx4_dequantize(*args) if stream is None else _ordered(stream, _native.mx4_dequantize, *args)
+
+
+def mx4_linear(x, W, bias=None, activations=None, dtype=None, out=None, stream=None):
+    """y = x W^T + bias with W [N, K] in 4 bits (an ``Mx4``), which is read as its values in x's type.
+
+    ``activations=4``: x [..., K] is rounded to 4 bits as well and the product runs on the scaled matrix instructions; so does
+    it for an x that is an ``Mx4`` already (``dtype``: of y, float32 where neither it nor ``out`` says)."""
+    if activations not in (None, 4):
+        raise ValueError("activations must be None or 4")
+    args = (x, W, bias, activations == 4, dtype, out, stream)
+    return _native.mx4_linear(*args) if stream is None else _ordered(stream, _native.mx4_linear, *args)
+
+
+def mx4_linear_backward(dy, W, stream=None):
+    """dx = dy W of ``mx4_linear`` (with x in its own type) for dy [..., N]."""
+    args = (dy, W, stream)
+    return _native.mx4_linear_backward(*args) if stream is None else _ordered(stream, _native.mx4_linear_backward, *args)
+
+
 def adapter_forward(x, W, A, B, ids, scale=None, bias=None, out=None, keep=False, stream=None):
     """y = x W^T + bias with the low-rank adapter of each token beside it.
 
     ``y[t] = W x[t] + bias + scale[a] B[a] (A[a] x[t])`` with ``a = ids[t]``; an id outside
     0 .. adapters - 1 (say -1) is a token without one.  x [..., K], W [N, K], A [adapters, R, K]
-    and B [adapters, N, R] of one type (float32, bfloat16, float16); scale [adapters] and bias
-    [N] float32; ids one int32 or int64 a token, in any order.  ``keep``: also returns what
+    and B [adapters, N, R] of one type (float32, bfloat16, float16), or W an ``Mx4``, read as its
+    values in that type; scale [adapters] and bias [N] float32; ids one int32 or int64 a token, in any order.  ``keep``: also returns what
     ``adapter_backward`` needs of this pass.
     """
     if stream is None:

@@ -27,7 +27,8 @@ struct ShrinkArgs {
 };
 
 // y[t][n] = sum_k z[t][k] w(n, k) + bias[n] + sum_r h[t][r] F_a(n, r), F_a(n, r) at
-// f + a * R * N + n * fn + r * fr; w(n, k) at w + n * ldw + k, or (nn) at w + k * ldw + n.
+// f + a * R * N + n * fn + r * fr; w(n, k) at w + n * ldw + k, or (nn) at w + k * ldw + n.  With `scales` w is held in
+// 4 bits (mx4_codes.h), its rows of ldw blocks.  ids null: there are no adapters.
 struct ProjectArgs {
   const void *z, *w, *f;
   const float *h, *bias;
@@ -39,6 +40,7 @@ struct ProjectArgs {
   int planes;             // h is the sum of so many planes ...
   size_t plane;           // ... so many values apart (more than one: only where project_sums_planes)
   float* keep;            // with planes > 1: where their sum goes as well, or null
+  const unsigned char* scales;   // [rows of w][ldw], or null
 };
 
 // out[a][r][c] = sum over tokens with ids[t] = a of p[t][r] z[t][c], at out + a * R * C + r * outr +
@@ -63,17 +65,17 @@ hipError_t planes_join(float* h, const float* from, size_t n, int planes, hipStr
 // Whether the projection that these operands get adds up the planes of h itself.
 bool project_sums_planes(const ProjectArgs&, int dtype, bool nn);
 // part: project_part_bytes of scratch memory.
-size_t project_part_bytes(size_t T, int K, int N, int G, int dtype, bool nn);
+size_t project_part_bytes(size_t T, int K, int N, int G, int dtype, bool nn, bool four);
 hipError_t project_launch(const ProjectArgs&, float* part, int dtype, bool nn, hipStream_t);
 // What project_launch runs: one launch, or one of whole tiles and one of the rows that are left over.
-void project_plan(size_t T, int K, int N, int G, int dtype, bool nn, bool direct, cp4_adapter_launch (&launches)[2]);
+void project_plan(size_t T, int K, int N, int G, int dtype, bool nn, bool direct, bool four, cp4_adapter_launch (&launches)[2]);
 // The tiles of a projection on the matrix cores, its depth in `splits` parts of `each` steps, whose partial
 // sums take tile_part_bytes.
 struct TilePlan {
   int which, splits, each;
   double cost;            // microseconds, about
 };
-TilePlan tile_plan(size_t T, int K, int N, int dtype, bool nn, bool direct);
+TilePlan tile_plan(size_t T, int K, int N, int dtype, bool nn, bool direct, bool four);
 size_t tile_part_bytes(const TilePlan&, size_t T, int N);
 int tile_rows(const TilePlan&);
 int tile_cols(const TilePlan&);
@@ -87,7 +89,7 @@ struct RowsPlan {
   int splits;
   double cost, adapter;   // microseconds, about, and for each adapter
 };
-RowsPlan rows_plan(size_t T, int K, int N, int dtype);
+RowsPlan rows_plan(size_t T, int K, int N, int dtype, bool four);
 hipError_t rows_launch(const ProjectArgs&, const RowsPlan&, float* part, int dtype, hipStream_t);
 // Two sums over the same tokens and adapters, their R, G and splits the same.
 int grad_splits(size_t T, int C0, int C1, int R, int G);

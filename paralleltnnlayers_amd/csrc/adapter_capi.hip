@@ -2,6 +2,7 @@
 #include <algorithm>
 
 #include "adapter.h"
+#include "cp4/mx4.h"
 
 namespace {
 
@@ -43,14 +44,14 @@ struct BackwardPlan {
   int splits, dh_planes;
   size_t part_at, part_b, total;                       // (dh comes first; B's partial sums: floats behind A's)
 };
-BackwardPlan backward_plan(const cp4_adapter_shape& s, int dtype) {
+BackwardPlan backward_plan(const cp4_adapter_shape& s, int dtype, bool four) {
   BackwardPlan p{};
   p.splits = grad_splits(s.T, (int)s.K, (int)s.N, (int)s.R, (int)s.G);
   p.dh_planes = shrink_planes(s.T, (int)s.N, dtype);
   p.part_at = align256(p.dh_planes * h_bytes(s));
   p.part_b = p.splits > 1 ? (size_t)p.splits * s.G * s.R * s.K : 0;
   const size_t parts = p.splits > 1 ? (p.part_b + (size_t)p.splits * s.G * s.R * s.N) * 4 : 0;
-  p.total = p.part_at + align256(std::max(parts, project_part_bytes(s.T, (int)s.N, (int)s.K, (int)s.G, dtype, true)));  // (one after the other)
+  p.total = p.part_at + align256(std::max(parts, project_part_bytes(s.T, (int)s.N, (int)s.K, (int)s.G, dtype, true, four)));  // (one after the other)
   return p;
 }
 
@@ -60,20 +61,22 @@ extern "C" size_t cp4_adapter_kept_bytes(const cp4_adapter_shape* s, int dtype) 
   return check_shape(s, dtype) == CP4_OK ? h_bytes(*s) : 0;
 }
 
-extern "C" size_t cp4_adapter_forward_workspace_bytes(const cp4_adapter_shape* s, int dtype) {
+namespace {
+
+size_t forward_bytes(const cp4_adapter_shape* s, int dtype, bool four) {
   if (check_shape(s, dtype) != CP4_OK) return 0;
-  return align256(shrink_planes(s->T, (int)s->K, dtype) * h_bytes(*s)) + align256(project_part_bytes(s->T, (int)s->K, (int)s->N, (int)s->G, dtype, false));
+  return align256(shrink_planes(s->T, (int)s->K, dtype) * h_bytes(*s)) + align256(project_part_bytes(s->T, (int)s->K, (int)s->N, (int)s->G, dtype, false, four));
 }
 
-extern "C" cp4_status cp4_adapter_forward(const cp4_adapter_shape* s, int dtype, const void* x, const void* W,
-                                          const void* A, const void* B, const int* ids, const float* scale,
-                                          const float* bias, void* y, float* kept, void* workspace,
-                                          size_t workspace_bytes, cp4_stream stream) {
+// scales: null, or W's in 4 bits.
+cp4_status forward(const cp4_adapter_shape* s, int dtype, const void* x, const void* W, const unsigned char* scales,
+                   const void* A, const void* B, const int* ids, const float* scale, const float* bias, void* y,
+                   float* kept, void* workspace, size_t workspace_bytes, cp4_stream stream) {
   if (const cp4_status rc = check_shape(s, dtype)) return rc;
   if (!s->T) return CP4_OK;
   if (!x || !W || !A || !B || !ids || !y) return fail_with(CP4_ERR_NULL_POINTER, "an operand is NULL");
-  if (const cp4_status rc = check_pointers(value_bytes(dtype), {x, W, A, B, y}, {ids, scale, bias})) return rc;
-  const size_t need = cp4_adapter_forward_workspace_bytes(s, dtype);
+  if (const cp4_status rc = check_pointers(value_bytes(dtype), {x, scales ? nullptr : W, A, B, y}, {ids, scale, bias})) return rc;
+  const size_t need = forward_bytes(s, dtype, scales);
   if (!workspace || workspace_bytes < need || ((size_t)workspace & 255))
     return fail_with(CP4_ERR_WORKSPACE, "workspace missing, too small or not aligned to 256 bytes");
   if ((size_t)kept & 15) return fail_with(CP4_ERR_WORKSPACE, "kept is not aligned to 16 bytes");
@@ -88,7 +91,7 @@ extern "C" cp4_status cp4_adapter_forward(const cp4_adapter_shape* s, int dtype,
   if (const hipError_t e = shrink_launch(sh, dtype, st)) return fail_hip(e, "cp4_adapter_forward");
   ProjectArgs p{};
   p.z = x; p.w = W; p.f = B; p.h = sh.h; p.bias = bias; p.ids = ids; p.y = y;
-  p.T = s->T; p.ldz = sh.ldz; p.ldw = s->ldw ? s->ldw : s->K;
+  p.T = s->T; p.ldz = sh.ldz; p.ldw = scales ? (s->K + 31) / 32 : s->ldw ? s->ldw : s->K; p.scales = scales;
   p.K = (int)s->K; p.N = (int)s->N; p.R = (int)s->R; p.Rp = sh.Rp; p.G = (int)s->G;
   p.fn = (int)s->R; p.fr = 1; p.planes = sh.planes; p.plane = p.T * p.Rp;
   if (p.planes > 1 && project_sums_planes(p, dtype, false)) {
@@ -104,24 +107,57 @@ extern "C" cp4_status cp4_adapter_forward(const cp4_adapter_shape* s, int dtype,
   return CP4_OK;
 }
 
-extern "C" size_t cp4_adapter_backward_workspace_bytes(const cp4_adapter_shape* s, int dtype) {
-  if (check_shape(s, dtype) != CP4_OK) return 0;
-  return backward_plan(*s, dtype).total;
+}  // namespace
+
+extern "C" size_t cp4_adapter_forward_workspace_bytes(const cp4_adapter_shape* s, int dtype) { return forward_bytes(s, dtype, false); }
+extern "C" size_t cp4_adapter_mx4_forward_workspace_bytes(const cp4_adapter_shape* s, int dtype) { return forward_bytes(s, dtype, true); }
+
+extern "C" cp4_status cp4_adapter_forward(const cp4_adapter_shape* s, int dtype, const void* x, const void* W,
+                                          const void* A, const void* B, const int* ids, const float* scale,
+                                          const float* bias, void* y, float* kept, void* workspace,
+                                          size_t workspace_bytes, cp4_stream stream) {
+  return forward(s, dtype, x, W, nullptr, A, B, ids, scale, bias, y, kept, workspace, workspace_bytes, stream);
 }
 
-extern "C" cp4_status cp4_adapter_backward(const cp4_adapter_shape* s, int dtype, const void* dy, const void* x,
-                                           const void* W, const void* A, const void* B, const int* ids,
-                                           const float* scale, const float* kept, void* dx, void* dA, void* dB,
-                                           void* workspace, size_t workspace_bytes, cp4_stream stream) {
+namespace {
+cp4_status check_four(const cp4_mx4* W, size_t T) {
+  if (T && (!W || !W->codes || !W->scales)) return fail_with(CP4_ERR_NULL_POINTER, "an operand is NULL");
+  if (W && ((size_t)W->codes & 15)) return fail_with(CP4_ERR_SHAPE, "codes are not aligned to 16 bytes");
+  return CP4_OK;
+}
+}  // namespace
+
+extern "C" cp4_status cp4_adapter_mx4_forward(const cp4_adapter_shape* s, int dtype, const void* x, const cp4_mx4* W,
+                                              const void* A, const void* B, const int* ids, const float* scale,
+                                              const float* bias, void* y, float* kept, void* workspace,
+                                              size_t workspace_bytes, cp4_stream stream) {
+  if (const cp4_status rc = check_shape(s, dtype)) return rc;
+  if (const cp4_status rc = check_four(W, s->T)) return rc;
+  if (!s->T) return CP4_OK;
+  return forward(s, dtype, x, W->codes, W->scales, A, B, ids, scale, bias, y, kept, workspace, workspace_bytes, stream);
+}
+
+extern "C" size_t cp4_adapter_backward_workspace_bytes(const cp4_adapter_shape* s, int dtype) {
+  return check_shape(s, dtype) == CP4_OK ? backward_plan(*s, dtype, false).total : 0;
+}
+extern "C" size_t cp4_adapter_mx4_backward_workspace_bytes(const cp4_adapter_shape* s, int dtype) {
+  return check_shape(s, dtype) == CP4_OK ? backward_plan(*s, dtype, true).total : 0;
+}
+
+namespace {
+cp4_status backward(const cp4_adapter_shape* s, int dtype, const void* dy, const void* x, const void* W,
+                    const unsigned char* scales, const void* A, const void* B, const int* ids, const float* scale,
+                    const float* kept, void* dx, void* dA, void* dB, void* workspace, size_t workspace_bytes,
+                    cp4_stream stream) {
   if (const cp4_status rc = check_shape(s, dtype)) return rc;
   if (!dA != !dB) return fail_with(CP4_ERR_NULL_POINTER, "dA without dB");
   if (s->T) {
     if (!dy || !W || !A || !B || !ids || (dA && (!x || !kept)))
       return fail_with(CP4_ERR_NULL_POINTER, "an operand is NULL");
-    if (const cp4_status rc = check_pointers(value_bytes(dtype), {dy, x, W, A, B, dx, dA, dB}, {ids, scale})) return rc;
+    if (const cp4_status rc = check_pointers(value_bytes(dtype), {dy, x, scales ? nullptr : W, A, B, dx, dA, dB}, {ids, scale})) return rc;
     if ((size_t)kept & 15) return fail_with(CP4_ERR_WORKSPACE, "kept is not aligned to 16 bytes");
   }
-  const BackwardPlan plan = backward_plan(*s, dtype);
+  const BackwardPlan plan = backward_plan(*s, dtype, scales);
   if (plan.total && (!workspace || workspace_bytes < plan.total || ((size_t)workspace & 255)))
     return fail_with(CP4_ERR_WORKSPACE, "workspace missing, too small or not aligned to 256 bytes");
   const hipStream_t st = static_cast<hipStream_t>(stream);
@@ -142,7 +178,7 @@ extern "C" cp4_status cp4_adapter_backward(const cp4_adapter_shape* s, int dtype
   if (s->T && dx) {
     ProjectArgs p{};
     p.z = dy; p.w = W; p.f = A; p.h = dh; p.ids = ids; p.y = dx;
-    p.T = s->T; p.ldz = lddy; p.ldw = s->ldw ? s->ldw : s->K;
+    p.T = s->T; p.ldz = lddy; p.ldw = scales ? (s->K + 31) / 32 : s->ldw ? s->ldw : s->K; p.scales = scales;
     p.K = (int)s->N; p.N = (int)s->K; p.R = (int)s->R; p.Rp = Rp; p.G = (int)s->G;
     p.fn = 1; p.fr = (int)s->K; p.planes = 1;
     if (const hipError_t e = project_launch(p, part, dtype, true, st)) return fail_hip(e, "cp4_adapter_backward");
@@ -157,6 +193,74 @@ extern "C" cp4_status cp4_adapter_backward(const cp4_adapter_shape* s, int dtype
   }
   return CP4_OK;
 }
+}  // namespace
+
+extern "C" cp4_status cp4_adapter_backward(const cp4_adapter_shape* s, int dtype, const void* dy, const void* x,
+                                           const void* W, const void* A, const void* B, const int* ids,
+                                           const float* scale, const float* kept, void* dx, void* dA, void* dB,
+                                           void* workspace, size_t workspace_bytes, cp4_stream stream) {
+  return backward(s, dtype, dy, x, W, nullptr, A, B, ids, scale, kept, dx, dA, dB, workspace, workspace_bytes, stream);
+}
+extern "C" cp4_status cp4_adapter_mx4_backward(const cp4_adapter_shape* s, int dtype, const void* dy, const void* x,
+                                               const cp4_mx4* W, const void* A, const void* B, const int* ids,
+                                               const float* scale, const float* kept, void* dx, void* dA, void* dB,
+                                               void* workspace, size_t workspace_bytes, cp4_stream stream) {
+  if (const cp4_status rc = check_shape(s, dtype)) return rc;
+  if (const cp4_status rc = check_four(W, s->T)) return rc;
+  return backward(s, dtype, dy, x, W ? W->codes : nullptr, s->T ? W->scales : nullptr, A, B, ids, scale, kept, dx, dA, dB, workspace,
+                  workspace_bytes, stream);
+}
+
+// ---- projections without adapters ---------------------------------------------------------
+
+namespace {
+cp4_status check_linear(size_t T, unsigned K, unsigned N, int dtype, size_t ld, unsigned row, const cp4_mx4* W) {
+  if (dtype != CP4_DTYPE_F32 && dtype != CP4_DTYPE_BF16 && dtype != CP4_DTYPE_F16)
+    return fail_with(CP4_ERR_SHAPE, "unknown dtype");
+  if (!K || !N || K > 1u << 22 || N > 1u << 22) return fail_with(CP4_ERR_SHAPE, "K and N must be 1 to 2^22");
+  if (T > (size_t)1 << 26) return fail_with(CP4_ERR_SHAPE, "more than 2^26 rows");
+  if (ld && ld < row) return fail_with(CP4_ERR_SHAPE, "a row stride is smaller than the row");
+  if (ld > (size_t)1 << 30) return fail_with(CP4_ERR_SHAPE, "a row stride above 2^30");
+  return check_four(W, T);
+}
+// y [T][N] = z w + bias, z [T][K]; nn as in adapter.h.
+cp4_status linear(size_t T, int K, int N, int dtype, const void* z, size_t ldz, const cp4_mx4* W, size_t blocks, const float* bias,
+                  void* y, void* workspace, size_t workspace_bytes, bool nn, cp4_stream stream, const char* where) {
+  if (!T) return CP4_OK;
+  if (!z || !y) return fail_with(CP4_ERR_NULL_POINTER, "an operand is NULL");
+  if (const cp4_status rc = check_pointers(value_bytes(dtype), {z, y}, {bias})) return rc;
+  const size_t need = align256(project_part_bytes(T, K, N, 0, dtype, nn, true));
+  if (need && (!workspace || workspace_bytes < need || ((size_t)workspace & 255)))
+    return fail_with(CP4_ERR_WORKSPACE, "workspace missing, too small or not aligned to 256 bytes");
+  ProjectArgs p{};
+  p.z = z; p.w = W->codes; p.scales = W->scales; p.bias = bias; p.y = y;
+  p.T = T; p.ldz = ldz; p.ldw = blocks;
+  p.K = K; p.N = N; p.planes = 1;
+  if (const hipError_t e = project_launch(p, static_cast<float*>(workspace), dtype, nn, static_cast<hipStream_t>(stream)))
+    return fail_hip(e, where);
+  return CP4_OK;
+}
+}  // namespace
+
+extern "C" size_t cp4_mx4_forward_workspace_bytes(size_t T, unsigned K, unsigned N, int dtype) {
+  if (check_linear(T, K, N, dtype, 0, 0, nullptr) == CP4_ERR_SHAPE || !T) return 0;
+  return align256(project_part_bytes(T, (int)K, (int)N, 0, dtype, false, true));
+}
+extern "C" cp4_status cp4_mx4_forward(size_t T, unsigned K, unsigned N, int dtype, const void* x, size_t ldx, const cp4_mx4* W,
+                                      const float* bias, void* y, void* workspace, size_t workspace_bytes,
+                                      cp4_stream stream) {
+  if (const cp4_status rc = check_linear(T, K, N, dtype, ldx, K, W)) return rc;
+  return linear(T, (int)K, (int)N, dtype, x, ldx ? ldx : K, W, (K + 31) / 32, bias, y, workspace, workspace_bytes, false, stream, "cp4_mx4_forward");
+}
+extern "C" size_t cp4_mx4_backward_workspace_bytes(size_t T, unsigned K, unsigned N, int dtype) {
+  if (check_linear(T, K, N, dtype, 0, 0, nullptr) == CP4_ERR_SHAPE || !T) return 0;
+  return align256(project_part_bytes(T, (int)N, (int)K, 0, dtype, true, true));
+}
+extern "C" cp4_status cp4_mx4_backward(size_t T, unsigned K, unsigned N, int dtype, const void* dy, size_t lddy, const cp4_mx4* W,
+                                       void* dx, void* workspace, size_t workspace_bytes, cp4_stream stream) {
+  if (const cp4_status rc = check_linear(T, K, N, dtype, lddy, N, W)) return rc;
+  return linear(T, (int)N, (int)K, dtype, dy, lddy ? lddy : N, W, (K + 31) / 32, nullptr, dx, workspace, workspace_bytes, true, stream, "cp4_mx4_backward");
+}
 
 extern "C" cp4_status cp4_adapter_plan_query(const cp4_adapter_shape* s, int dtype, int backward, int aligned,
                                              cp4_adapter_launch launches[2]) {
@@ -164,7 +268,7 @@ extern "C" cp4_status cp4_adapter_plan_query(const cp4_adapter_shape* s, int dty
   if (!launches) return fail_with(CP4_ERR_NULL_POINTER, "launches is NULL");
   cp4_adapter_launch l[2];
   const int K = (int)(backward ? s->N : s->K), N = (int)(backward ? s->K : s->N);
-  project_plan(s->T, K, N, (int)s->G, dtype, backward != 0, aligned != 0, l);
+  project_plan(s->T, K, N, (int)s->G, dtype, backward != 0, aligned != 0, false, l);
   launches[0] = l[0];
   launches[1] = l[1];
   return CP4_OK;

@@ -8,12 +8,16 @@
 // are split over workgroups too.  The adapters' parts are shared out over the waves, h's planes are added up while the first
 // turns' loads are on their way, and all sums meet in the LDS.
 //
+// W in 4 bits: a turn is 128 inputs, and a lane has one block of 32 of its row of W (16 bytes of codes and a scale), which it
+// turns into values in its registers; it takes the same 32 inputs of its tokens, so that nothing changes places.
+//
 // Measured: 16 tokens fp32, 9216 -> 4096: 43 us, 3.5 TB/s; 48 tokens of 32 adapters bf16, 4096 x 4096: 22 us (9 us without
 // adapters and with 16 tokens); one token, 1024 x 1024: 6 us.
 #include <algorithm>
 
 #include "adapter.h"
 #include "adapter_load.h"
+#include "mx4_codes.h"
 
 namespace cp4 {
 namespace adapter {
@@ -103,10 +107,12 @@ __device__ __forceinline__ void expand_rows(const ProjectArgs& a, int id, const 
   }
 }
 
-template <class T, int MB>
+template <class T, int MB, bool Four>
 __global__ __launch_bounds__(64 * kWaves, 2) void rows_kernel(const RowsArgs ra) {
   typedef typename T::raw Raw;
-  constexpr int n = 16 / sizeof(Raw), U = 128 / sizeof(Raw), kRow = 20, kAhead = 4;
+  constexpr int n = 16 / sizeof(Raw), U = Four ? 128 : 128 / sizeof(Raw), kRow = 20;
+  // loads of a turn (of a row of x, of W), and how many turns' are under way
+  constexpr int kZ = Four ? 32 / n : 2, kW = Four ? 1 : 2, kAhead = !Four ? 4 : kZ * MB > 8 ? 1 : kZ * MB > 4 ? 2 : 4;
   constexpr int kSum = kWaves * 16 * MB * kRow, kH = 16 * MB * 256;
   __shared__ __attribute__((aligned(16))) float lds[kSum > kH ? kSum : kH];
   float* const hl = lds;                                             // [T][Rp], and then ...
@@ -114,27 +120,54 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows_kernel(const RowsArgs ra)
   const ProjectArgs& a = ra.p;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 15, g = lane >> 4;
   const int rows = (int)a.T, n0 = blockIdx.x * 16, split = blockIdx.y;
-  int id = lane < rows ? a.ids[lane] : -1;
+  int id = lane < rows && (!Four || a.ids) ? a.ids[lane] : -1;
   if (id < 0 || id >= a.G) id = -1;
   const bool adapters = split == 0 && __ballot(id >= 0);
-  const Raw *z[MB], *const w = static_cast<const Raw*>(a.w) + min(n0 + l, a.N - 1) * a.ldw + n * g;
+  const size_t w_row = min(n0 + l, a.N - 1) * a.ldw;
+  const Raw *z[MB], *const w = static_cast<const Raw*>(a.w) + (Four ? 0 : w_row + n * g);
+  const char* const codes = static_cast<const char*>(a.w) + (w_row + g) * 16;
+  const unsigned char* const scales = a.scales + w_row + g;
+  unsigned sv[kAhead];
 #pragma unroll
-  for (int i = 0; i < MB; ++i) z[i] = static_cast<const Raw*>(a.z) + min(16 * i + l, rows - 1) * a.ldz + n * g;
+  for (int i = 0; i < MB; ++i) z[i] = static_cast<const Raw*>(a.z) + min(16 * i + l, rows - 1) * a.ldz + (Four ? 32 : n) * g;
   const int units = (a.K + U - 1) / U, shares = kWaves * ra.splits, share = split * kWaves + wave;
   const int first = (int)((long)units * share / shares), last = (int)((long)units * (share + 1) / shares);
   const int whole = min(last, a.K / U);
 
   f32x4 acc[MB] = {};
-  u32x4 zv[kAhead][MB][2], wv[kAhead][2];
+  u32x4 zv[kAhead][MB][kZ], wv[kAhead][kW];
+  constexpr int kNext = Four ? n : 4 * n;                            // from one load of a row of x to the next one
   auto load = [&](int u, int e) __attribute__((always_inline)) {
+    if constexpr (Four) {
+      wv[e][0] = *reinterpret_cast<const u32x4*>(codes + (size_t)u * 64);
+      sv[e] = scales[(size_t)u * 4];
+    } else {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) wv[e][h] = load_16(w + (size_t)u * U + 4 * n * h);
+      for (int h = 0; h < 2; ++h) wv[e][h] = load_16(w + (size_t)u * U + 4 * n * h);
+    }
 #pragma unroll
     for (int i = 0; i < MB; ++i)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) zv[e][i][h] = load_16(z[i] + (size_t)u * U + 4 * n * h);
+      for (int h = 0; h < kZ; ++h) zv[e][i][h] = load_16(z[i] + (size_t)u * U + kNext * h);
   };
   auto multiply = [&](int e) __attribute__((always_inline)) {
+    if constexpr (Four) {
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        Raw v[8];
+        mx4::values<T>(wv[e][0][h], mx4::scale_of(sv[e]), v);
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+          if constexpr (__is_same(T, F32)) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) acc[i] = mfma_f32(__uint_as_float(zv[e][i][2 * h + q / 4][q % 4]), v[q], acc[i]);
+          } else {
+            acc[i] = mfma_16<T>(__builtin_bit_cast(u16x8, zv[e][i][h]), __builtin_bit_cast(u16x8, v), acc[i]);
+          }
+        }
+      }
+      return;
+    } else {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -147,6 +180,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows_kernel(const RowsArgs ra)
           acc[i] = mfma_16<T>(__builtin_bit_cast(u16x8, zv[e][i][h]), __builtin_bit_cast(u16x8, wv[e][h]), acc[i]);
         }
       }
+    }
   };
   // The first turns' loads, h's planes while they are on their way, and then the other turns.
   int u = first;
@@ -188,12 +222,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows_kernel(const RowsArgs ra)
     multiply(0);
   }
   if (u < last) {                                                    // (the inputs' rest)
+    if constexpr (Four) {
+      const bool there = u * U + 32 * g < a.K;
+      wv[0][0] = there ? *reinterpret_cast<const u32x4*>(codes + (size_t)u * 64) : u32x4{};
+      sv[0] = there ? scales[(size_t)u * 4] : 127u;
+    }
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int left = a.K - u * U - n * g - 4 * n * h;
-      wv[0][h] = load_16(w + (size_t)u * U + 4 * n * h, left);
+    for (int h = 0; h < kZ; ++h) {
+      const int left = a.K - u * U - (Four ? 32 : n) * g - kNext * h;
+      if constexpr (!Four) wv[0][h] = load_16(w + (size_t)u * U + 4 * n * h, left);
 #pragma unroll
-      for (int i = 0; i < MB; ++i) zv[0][i][h] = load_16(z[i] + (size_t)u * U + 4 * n * h, left);
+      for (int i = 0; i < MB; ++i) zv[0][i][h] = load_16(z[i] + (size_t)u * U + kNext * h, left);
     }
     multiply(0);
   }
@@ -219,7 +258,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows_kernel(const RowsArgs ra)
 
 template <class T, int MB>
 void launch(const RowsArgs& r, hipStream_t st) {
-  rows_kernel<T, MB><<<dim3((r.p.N + 15) / 16, r.splits), 64 * kWaves, 0, st>>>(r);
+  const dim3 grid((r.p.N + 15) / 16, r.splits);
+  if (r.p.scales) rows_kernel<T, MB, true><<<grid, 64 * kWaves, 0, st>>>(r);
+  else rows_kernel<T, MB, false><<<grid, 64 * kWaves, 0, st>>>(r);
 }
 template <class T>
 void launch_rows(const RowsArgs& r, hipStream_t st) {
@@ -238,11 +279,11 @@ void launch_rows(const RowsArgs& r, hipStream_t st) {
 // more (16 tokens, 8192 inputs, 256 outputs: 11.7 us against 20.6 in one part; 1024 x 1024 in four 10.9 against 9.3).
 // The cost is what 4096 inputs took: 6, 10, 14, 17 us for up to 16, 32, 48, 64 tokens (fp32: 14, 24) a round of the chip,
 // and 0.15 us an adapter.
-RowsPlan rows_plan(size_t T, int K, int N, int dtype) {
+RowsPlan rows_plan(size_t T, int K, int N, int dtype, bool four) {
   RowsPlan p{};
   const bool f32 = dtype == CP4_DTYPE_F32;
   if (T > (f32 ? 32 : 64)) return p;
-  const int units = (K * (f32 ? 4 : 2) + 127) / 128, tiles = (N + 15) / 16, cus = num_compute_units();
+  const int units = four ? (K + 127) / 128 : (K * (f32 ? 4 : 2) + 127) / 128, tiles = (N + 15) / 16, cus = num_compute_units();
   p.splits = std::max(1, std::min(cus / tiles, units / (2 * kWaves)));
   if (p.splits < 4) p.splits = 1;
   const int rounds = (int)(((long)tiles * p.splits + cus - 1) / cus), blocks = (int)(T + 15) / 16;

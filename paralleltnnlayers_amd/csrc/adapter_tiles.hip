@@ -33,11 +33,26 @@
 #include "adapter.h"
 #include "adapter_load.h"
 #include "die_order.h"
+#include "mx4_codes.h"
 #include "split_bf16.h"
 
 namespace cp4 {
 namespace adapter {
+
+struct TileArgs {
+  ProjectArgs p;
+  float* part;            // [splits][T][N], or null: y
+  int mt, nt, splits;     // tiles, and parts of the depth
+  int steps;              // of a part (the last one may have fewer)
+};
+
 namespace {
+
+// This file is built twice: for w in the operands' type, and for w in 4 bits.
+#ifndef CP4_TILE_FOUR
+#define CP4_TILE_FOUR 0
+#endif
+constexpr bool kFour = CP4_TILE_FOUR;
 
 template <class T>
 constexpr int kVec = 16 / sizeof(typename T::raw);                   // values of a 16-byte load
@@ -91,7 +106,7 @@ __device__ __forceinline__ void expand_tile(const ProjectArgs& a, size_t t0, int
 #pragma unroll
   for (int w = 0; w < WM; ++w) {
     const size_t row = t0 + 64 * w + lane;
-    id[w] = row < a.T ? a.ids[row] : -1;
+    id[w] = row < a.T && (!kFour || a.ids) ? a.ids[row] : -1;
     if (id[w] < 0 || id[w] >= a.G) id[w] = -1;
     any |= have[w] = __ballot(id[w] >= 0);
   }
@@ -247,13 +262,6 @@ __device__ __forceinline__ void expand_tile(const ProjectArgs& a, size_t t0, int
   }
 }
 
-struct TileArgs {
-  ProjectArgs p;
-  float* part;            // [splits][T][N], or null: y
-  int mt, nt, splits;     // tiles, and parts of the depth
-  int steps;              // of a part (the last one may have fewer)
-};
-
 // One wave of a tile: MB x NB blocks of 16 x 16.
 template <class T, bool NN, bool Direct, int MB, int NB, int WM, int WN, int RB, int Rooms>
 __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta) {
@@ -288,15 +296,41 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
   // What each thread brings: the LDS is filled in the threads' order; which 16 bytes come there is theirs to choose.
   // Rows beyond the operand's are read again from its last one: what they give is not stored.
   typedef std::conditional_t<Direct, unsigned, size_t> Offset;       // (bytes)
-  Offset zo[kZ], wo[kW];
-  int w_count[kW];                                                   // values there of a piece of w's row (nn)
+  Offset zo[kZ], wo[kFour ? 1 : kW];
+  int w_count[kFour ? 1 : kW];                                       // values there of a piece of w's row (nn)
+  // w in 4 bits: blocks of 32 values, their codes and scales in registers until put() turns them into values in the LDS
+  constexpr int kBlocks = BN * KS / 32, kC = (kBlocks + kThreads - 1) / kThreads;
+  unsigned co[kFour ? kC : 1], at_lds[kFour ? kC : 1];               // a thread's blocks: where, from the step's first one on, ...
+  int depth_of[kFour ? kC : 1];                                      // ... whither, and the depth of their first value
+  u32x4 codes[kFour ? kC : 1];
+  unsigned scale[kFour ? kC : 1];
+  size_t w_block = NN ? (size_t)k_first * a.ldw + n0 / 32 : (size_t)n0 * a.ldw + k_first / 32;
+  const size_t w_blocks = NN ? (size_t)KS * a.ldw : KS / 32;
+  if constexpr (kFour) {
+#pragma unroll
+    for (int i = 0; i < kC; ++i) {
+      const int at = i * kThreads + threadIdx.x;
+      if constexpr (NN) {
+        constexpr int kRow = BN / 32;
+        const int block = at % kRow;
+        depth_of[i] = at / kRow;
+        co[i] = (unsigned)(depth_of[i] * a.ldw) + min(block, (cols - 1) / 32);
+        at_lds[i] = BM * RB + (unsigned)(depth_of[i] * BN + 32 * block) * sizeof(Raw);
+      } else {
+        const int slot = at % BN, in = slot % (16 * NB), col = slot - in + NB * (in & 15) + in / 16;
+        depth_of[i] = 32 * (at / BN);
+        co[i] = (unsigned)(min(col, cols - 1) * a.ldw) + at / BN;
+        at_lds[i] = BM * RB + slot * RB;
+      }
+    }
+  }
 #pragma unroll
   for (int i = 0; i < kZ; ++i) {
     const int at = i * kThreads + threadIdx.x, row = at / RC, chunk = piece(at % RC, row);
     zo[i] = (Offset)(min(row, rows - 1) * a.ldz * sizeof(Raw)) + chunk * 16;
   }
 #pragma unroll
-  for (int i = 0; i < kW; ++i) {
+  for (int i = 0; i < (kFour ? 0 : kW); ++i) {
     const int at = i * kThreads + threadIdx.x;
     if constexpr (NN) {
       constexpr int kRow = BN / kVec<T>;                             // 16-byte pieces of a row
@@ -314,36 +348,67 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
   auto advance = [&]() __attribute__((always_inline)) {
     const bool more = ++brought < steps;                             // (beyond the last step that one again)
     zb += more ? RB : 0;
-    wb += more ? w_next : 0;
+    if constexpr (kFour) w_block += more ? w_blocks : 0;
+    else wb += more ? w_next : 0;
   };
   // Operands on 16-byte boundaries go from memory to the LDS by themselves; others through registers, which put()
   // writes when the step that hid their way is multiplied.
-  u32x4 zr[Direct ? 1 : kZ], wr[Direct ? 1 : kW];
+  u32x4 zr[Direct ? 1 : kZ], wr[Direct || kFour ? 1 : kW];
   auto bring = [&](char* lds) __attribute__((always_inline)) {
+    if constexpr (kFour) {
+#pragma unroll
+      for (int i = 0; i < kC; ++i) {
+        if (kBlocks % kThreads && i * kThreads + (int)threadIdx.x >= kBlocks) continue;
+        codes[i] = *reinterpret_cast<const u32x4*>(static_cast<const char*>(a.w) + (w_block + co[i]) * 16);
+        scale[i] = a.scales[w_block + co[i]];
+      }
+    }
     if constexpr (Direct) {
 #pragma unroll
       for (int i = 0; i < kZ; ++i)
         __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(zb + zo[i]),
                                          (__attribute__((address_space(3))) void*)(lds + (i * kThreads + wave * 64) * 16), 16, 0, 0);
 #pragma unroll
-      for (int i = 0; i < kW; ++i)
+      for (int i = 0; i < (kFour ? 0 : kW); ++i)
         __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(wb + wo[i]),
                                          (__attribute__((address_space(3))) void*)(lds + BM * RB + (i * kThreads + wave * 64) * 16), 16, 0, 0);
     } else {
 #pragma unroll
       for (int i = 0; i < kZ; ++i) zr[i] = load_16(reinterpret_cast<const Raw*>(zb + zo[i]));
 #pragma unroll
-      for (int i = 0; i < kW; ++i) wr[i] = load_16(reinterpret_cast<const Raw*>(wb + wo[i]), NN ? w_count[i] : kVec<T>);
+      for (int i = 0; i < (kFour ? 0 : kW); ++i) wr[i] = load_16(reinterpret_cast<const Raw*>(wb + wo[i]), NN ? w_count[i] : kVec<T>);
     }
     advance();
+  };
+  auto put_four = [&](char* lds) __attribute__((always_inline)) {
+    if constexpr (kFour) {
+#pragma unroll
+      for (int i = 0; i < kC; ++i) {
+        if (kBlocks % kThreads && i * kThreads + (int)threadIdx.x >= kBlocks) continue;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          Raw v[8];
+          mx4::values<T>(codes[i][q], mx4::scale_of(scale[i]), v);
+#pragma unroll
+          for (int h = 0; h < (int)sizeof(v) / 16; ++h) {
+            const int part = q * ((int)sizeof(v) / 16) + h;          // 16 bytes of the block's
+            char* to = lds + at_lds[i];
+            if constexpr (NN) to += part * 16;
+            else to += piece(depth_of[i] / kVec<T> + part, (i * kThreads + threadIdx.x) % BN) * 16;
+            __builtin_memcpy(__builtin_assume_aligned(to, 16), reinterpret_cast<const char*>(v) + 16 * h, 16);
+          }
+        }
+      }
+    }
   };
   auto put = [&](char* lds) __attribute__((always_inline)) {
     if constexpr (!Direct) {
 #pragma unroll
       for (int i = 0; i < kZ; ++i) *reinterpret_cast<u32x4*>(lds + (i * kThreads + threadIdx.x) * 16) = zr[i];
 #pragma unroll
-      for (int i = 0; i < kW; ++i) *reinterpret_cast<u32x4*>(lds + BM * RB + (i * kThreads + threadIdx.x) * 16) = wr[i];
+      for (int i = 0; i < (kFour ? 0 : kW); ++i) *reinterpret_cast<u32x4*>(lds + BM * RB + (i * kThreads + threadIdx.x) * 16) = wr[i];
     }
+    if constexpr (kFour) put_four(lds);
   };
 
   f32x4 acc[MB][NB] = {};
@@ -412,6 +477,17 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
           __builtin_memcpy(x + 4, __builtin_assume_aligned(lds + w_at + j * 16 * RB + p1, 16), 16);
         }
         u32x4 wh, wmid, wl;
+        if constexpr (kFour) {                                       // (a 4-bit value is its first part alone)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) wh[q] = split::pack_hi16(x[2 * q], x[2 * q + 1]);
+#pragma unroll
+          for (int i = 0; i < MB; ++i) {
+            acc[i][j] = mfma_parts(zl[i], wh, acc[i][j]);
+            acc[i][j] = mfma_parts(zm[i], wh, acc[i][j]);
+            acc[i][j] = mfma_parts(zh[i], wh, acc[i][j]);
+          }
+          continue;
+        }
         split::split8(x, wh, wmid, wl);
 #pragma unroll
         for (int i = 0; i < MB; ++i) {
@@ -437,7 +513,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
   // compiler from counting the loads under way.
   auto step = [&](const char* lds, char* into) __attribute__((always_inline)) {
     asm volatile("" ::: "memory");
-    if constexpr (Direct) __builtin_amdgcn_s_waitcnt(wait_for((Rooms - 2) * (kZ + kW)));
+    if constexpr (Direct) __builtin_amdgcn_s_waitcnt(wait_for((Rooms - 2) * (kZ + (kFour ? 0 : kW))));
     else __builtin_amdgcn_s_waitcnt(wait_for(63));                   // (the LDS alone)
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -476,14 +552,17 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
       products(zc, wc);
       turns();
       __builtin_amdgcn_sched_barrier(0);
+      if constexpr (kFour) put(lds);
     };
     if (steps > 0) {
       bring(lds0);
+      if constexpr (kFour) put(lds0);
       asm volatile("" ::: "memory");                                 // (their order is what the wait counts on)
       __builtin_amdgcn_sched_barrier(0);
       bring(lds1);
+      if constexpr (kFour) put(lds1);
       asm volatile("" ::: "memory");
-      __builtin_amdgcn_s_waitcnt(wait_for(kZ + kW));
+      __builtin_amdgcn_s_waitcnt(wait_for(kFour ? 0 : kZ + kW));
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
       read(lds0, 0, za, wa);
@@ -542,8 +621,19 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
       if (depth < left) x = load_16(reinterpret_cast<const Raw*>(zb + zo[i]), left - depth);
       *reinterpret_cast<u32x4*>(lds0 + at * 16) = x;
     }
+    if constexpr (kFour) {
+      w_block = NN ? (size_t)(k_last - left) * a.ldw + n0 / 32 : (size_t)n0 * a.ldw + (k_last - left) / 32;
 #pragma unroll
-    for (int i = 0; i < kW; ++i) {
+      for (int i = 0; i < kC; ++i) {
+        if (kBlocks % kThreads && i * kThreads + (int)threadIdx.x >= kBlocks) continue;
+        const bool there = depth_of[i] < left;
+        codes[i] = there ? *reinterpret_cast<const u32x4*>(static_cast<const char*>(a.w) + (w_block + co[i]) * 16) : u32x4{};
+        scale[i] = there ? a.scales[w_block + co[i]] : 127u;
+      }
+      put_four(lds0);
+    }
+#pragma unroll
+    for (int i = 0; i < (kFour ? 0 : kW); ++i) {
       const int at = i * kThreads + threadIdx.x;
       const int depth = NN ? at / (BN / kVec<T>) : piece(at % RC, at / RC) * kVec<T>;
       u32x4 x = {};
@@ -590,6 +680,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
     }
 }
 
+#if !CP4_TILE_FOUR
 // The depth's parts, in their order, and the bias.
 template <class T>
 __global__ __launch_bounds__(256) void join_kernel(const float* part, const float* bias, void* y, size_t n, int N, int splits) {
@@ -624,6 +715,8 @@ __global__ __launch_bounds__(256) void join_kernel(const float* part, const floa
   }
 }
 
+#endif
+
 template <class T, bool NN, bool Direct, int MB, int NB, int WM, int WN, int RB, int Rooms>
 void launch(const TileArgs& t, hipStream_t st) {
   tile_kernel<T, NN, Direct, MB, NB, WM, WN, RB, Rooms><<<die_grid((long)t.mt * t.nt * t.splits), 64 * WM * WN, 0, st>>>(t);
@@ -644,9 +737,25 @@ void launch_type(const TileArgs& t, int which, bool nn, bool direct, hipStream_t
   else nn ? launch_shape<T, true, false>(t, which, st) : launch_shape<T, false, false>(t, which, st);
 }
 
+#if !CP4_TILE_FOUR
 constexpr int kShapes = 4, kRows[kShapes] = {128, 128, 64, 256}, kCols[kShapes] = {256, 128, 256, 256};
+#endif
+
+template <class... Args>
+void launch_dtype(const TileArgs& t, int dtype, Args... args) {
+  if (dtype == CP4_DTYPE_F32) launch_type<F32>(t, args...);
+  else if (dtype == CP4_DTYPE_BF16) launch_type<BF16>(t, args...);
+  else launch_type<F16>(t, args...);
+}
 
 }  // namespace
+
+#if CP4_TILE_FOUR
+void four_launch(const TileArgs& t, int dtype, int which, bool nn, bool direct, hipStream_t st) {
+  launch_dtype(t, dtype, which, nn, direct, st);
+}
+#else
+void four_launch(const TileArgs& t, int dtype, int which, bool nn, bool direct, hipStream_t st);
 
 // Which shape of tile, and in how many parts its depth: the least time by a model of what was measured at a depth of
 // 4096 (microseconds; 16-bit types, fp32 in brackets), one tile on a compute unit and two of them, whose waits
@@ -660,7 +769,7 @@ constexpr int kShapes = 4, kRows[kShapes] = {128, 128, 64, 256}, kCols[kShapes] 
 // differ by up to 3 times: 100 tokens of 4096 x 4096 take 25 us (128 x 128 in four parts) and 82 (256 x 256), 8192 tokens
 // 223 us (256 x 256) and 331 (128 x 128), 6000 tokens nn 206 us (128 x 256), 224 (256 x 256) and 239 (64 x 256).  Parts other
 // than powers of two fill the chip where those leave a round half empty: 300 tokens fp32 4096 x 4096 97 -> 87 us (nn 103 -> 84).
-TilePlan tile_plan(size_t T, int K, int N, int dtype, bool nn, bool aligned) {
+TilePlan tile_plan(size_t T, int K, int N, int dtype, bool nn, bool aligned, bool four) {
   static constexpr float k16[2][kShapes][2] = {{{74, 132}, {37, 75}, {51, 69}, {97, 194}}, {{74, 116}, {42, 88}, {55, 76}, {102, 204}}};
   static constexpr float k32[2][kShapes][2] = {{{}, {192, 390}, {218, 340}, {}}, {{}, {190, 376}, {213, 293}, {}}};
   const long units = num_compute_units();
@@ -688,6 +797,7 @@ size_t tile_part_bytes(const TilePlan& p, size_t T, int N) { return p.splits > 1
 // Whether the LDS can be filled directly: 16-byte boundaries, and a thread's places in a tile as 32-bit byte offsets.
 bool tile_direct(const ProjectArgs& a, int dtype, bool nn) {
   const size_t e = dtype == CP4_DTYPE_F32 ? 4 : 2, vec = 16 / e;
+  if (a.scales) return !((size_t)a.z & 15) && a.ldz % vec == 0 && a.ldz * e * 256 < (size_t)1 << 31;
   if (((size_t)a.z & 15) || ((size_t)a.w & 15) || a.ldz % vec || a.ldw % vec || (nn ? a.N : a.K) % vec) return false;
   return a.ldz * e * 256 < (size_t)1 << 31 && a.ldw * e * 256 < (size_t)1 << 31;
 }
@@ -710,12 +820,13 @@ hipError_t tile_launch(const ProjectArgs& a, const TilePlan& plan, float* part, 
   t.splits = plan.splits;
   t.steps = plan.each;
   const bool d = tile_direct(a, dtype, nn);
-  if (dtype == CP4_DTYPE_F32) launch_type<F32>(t, plan.which, nn, d, st);
-  else if (dtype == CP4_DTYPE_BF16) launch_type<BF16>(t, plan.which, nn, d, st);
-  else launch_type<F16>(t, plan.which, nn, d, st);
+  if (a.scales) four_launch(t, dtype, plan.which, nn, d, st);
+  else launch_dtype(t, dtype, plan.which, nn, d, st);
   if (const hipError_t e = hipGetLastError()) return e;
   return plan.splits > 1 ? parts_join(part, a.bias, a.y, a.T, a.N, plan.splits, dtype, st) : hipSuccess;
 }
+
+#endif
 
 }  // namespace adapter
 }  // namespace cp4

@@ -17,6 +17,7 @@
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -32,6 +33,7 @@
 #include "cp4/capi.h"
 #include "cp4/layer_norm.h"
 #include "cp4/muon.h"
+#include "cp4/mx4.h"
 
 namespace {
 
@@ -477,22 +479,61 @@ Tensor rows_of(const Tensor& t, size_t* stride) {
   return t.contiguous();
 }
 
+// The weights of a projection [N, K]: a tensor, or microscaled 4-bit floating point (capi.Mx4: codes, scales, K).
+struct Weight {
+  Tensor W, scales;                                // (scales undefined: W is the tensor)
+  int64_t K = 0;
+  bool four() const { return scales.defined(); }
+  cp4_mx4 mx4() const { return cp4_mx4{W.data_ptr(), static_cast<const unsigned char*>(scales.data_ptr())}; }
+};
+// Rows held in 4 bits as the C ABI takes them: contiguous, codes on a 16-byte boundary.
+Weight packed(const Tensor& codes, const Tensor& scales, int64_t K) {
+  const int64_t blocks = (K + 31) / 32;
+  require(K >= 1 && K <= 1 << 22 && codes.is_cuda() && scales.is_cuda() && scales.device() == codes.device() &&
+              codes.scalar_type() == at::kByte && scales.scalar_type() == at::kByte && codes.dim() >= 1 &&
+              codes.dim() == scales.dim() && codes.size(-1) == blocks * 16 && scales.size(-1) == blocks &&
+              codes.sizes().slice(0, codes.dim() - 1) == scales.sizes().slice(0, codes.dim() - 1),
+          "expected uint8 codes [..., ceil(K / 32) * 16] and scales [..., ceil(K / 32)] on one device");
+  Weight w;
+  w.W = codes.contiguous();
+  if ((size_t)w.W.data_ptr() & 15) w.W = w.W.clone();
+  w.scales = scales.contiguous();
+  w.K = K;
+  return w;
+}
+bool is_packed(PyObject* o) { return PyTuple_Check(o) && PyTuple_GET_SIZE(o) == 3; }
+Weight packed_of(PyObject* o) {
+  require(is_packed(o), "expected codes, scales and the number of values of a row");
+  const Tensor &codes = tensor(PyTuple_GET_ITEM(o, 0)), &scales = tensor(PyTuple_GET_ITEM(o, 1));
+  return packed(codes, scales, integer(PyTuple_GET_ITEM(o, 2)));
+}
+Weight weight_of(PyObject* o) {
+  if (is_packed(o)) return packed_of(o);
+  Weight w;
+  w.W = tensor(o);
+  if (w.W.dim() == 2) w.K = w.W.size(1);
+  return w;
+}
+
 struct Adapters {
   cp4_adapter_shape shape{};
   int dtype = 0;
-  Tensor x, W, A, B, ids, scale, bias;             // as the C ABI takes them
+  bool four = false;
+  Tensor x, W, scales, A, B, ids, scale, bias;     // as the C ABI takes them
+  cp4_mx4 mx4() const { return cp4_mx4{W.data_ptr(), static_cast<const unsigned char*>(scales.data_ptr())}; }
 };
 // Checks the operands of an adapter call; x: [..., K] (dy of a backward call: [..., N]).
-Adapters adapters(const Tensor& x, const Tensor& W, const Tensor& A, const Tensor& B, const Tensor& ids,
+Adapters adapters(const Tensor& x, const Weight& w, const Tensor& A, const Tensor& B, const Tensor& ids,
                   const std::optional<Tensor>& scale, const std::optional<Tensor>& bias, bool is_dy = false) {
   Adapters p;
+  const Tensor& W = w.W;
   require(x.dim() >= 1 && W.dim() == 2 && A.dim() == 3 && B.dim() == 3,
           "expected x [..., K], W [N, K], A [adapters, R, K] and B [adapters, N, R]");
-  const int64_t N = W.size(0), K = W.size(1), G = A.size(0), R = A.size(1);
+  const int64_t N = W.size(0), K = w.K, G = A.size(0), R = A.size(1);
   require(x.size(-1) == (is_dy ? N : K) && A.size(2) == K && B.size(0) == G && B.size(1) == N && B.size(2) == R,
           "x, W, A and B do not match");
   for (const Tensor* t : {&x, &W, &A, &B})
-    require(t->is_cuda() && t->device() == x.device() && t->scalar_type() == x.scalar_type(),
+    require(t->is_cuda() && t->device() == x.device() && (t->scalar_type() == x.scalar_type() || (t == &W && w.four())),
             "x, W, A and B must be of one type on one device");
   p.dtype = dtype_of(x);
   for (const auto& t : {scale, bias})
@@ -508,7 +549,9 @@ Adapters adapters(const Tensor& x, const Tensor& W, const Tensor& A, const Tenso
   p.shape.T = (size_t)ids.numel();
   p.shape.K = (unsigned)K; p.shape.N = (unsigned)N; p.shape.R = (unsigned)R; p.shape.G = (unsigned)G;
   p.x = rows_of(x, is_dy ? &p.shape.lddy : &p.shape.ldx);
-  p.W = rows_of(W, &p.shape.ldw);
+  p.W = w.four() ? W : rows_of(W, &p.shape.ldw);
+  p.scales = w.scales;
+  p.four = w.four();
   p.A = A.contiguous();
   p.B = B.contiguous();
   p.ids = ids.contiguous();
@@ -530,10 +573,18 @@ std::vector<int64_t> with_last(at::IntArrayRef sizes, int64_t last) {
 Tensor adapter_run(const Adapters& p, at::IntArrayRef sizes, Tensor y, Tensor* kept, void* st) {
   if (!y.defined()) y = empty(with_last(sizes, p.shape.N), p.x.scalar_type(), p.x);
   if (kept) *kept = empty({(int64_t)(cp4_adapter_kept_bytes(&p.shape, p.dtype) / 4)}, at::kFloat, p.x);
-  const size_t need = cp4_adapter_forward_workspace_bytes(&p.shape, p.dtype);
+  const size_t need = p.four ? cp4_adapter_mx4_forward_workspace_bytes(&p.shape, p.dtype)
+                             : cp4_adapter_forward_workspace_bytes(&p.shape, p.dtype);
   const Tensor ws = scratch(need, p.x);
-  check(cp4_adapter_forward(&p.shape, p.dtype, ptr(p.x), ptr(p.W), ptr(p.A), ptr(p.B), ints(p.ids), floats(p.scale),
-                            floats(p.bias), ptr(y), kept ? static_cast<float*>(ptr(*kept)) : nullptr, ptr(ws), need, st));
+  float* const keep = kept ? static_cast<float*>(ptr(*kept)) : nullptr;
+  if (p.four) {
+    const cp4_mx4 w = p.mx4();
+    check(cp4_adapter_mx4_forward(&p.shape, p.dtype, ptr(p.x), &w, ptr(p.A), ptr(p.B), ints(p.ids), floats(p.scale),
+                                  floats(p.bias), ptr(y), keep, ptr(ws), need, st));
+  } else {
+    check(cp4_adapter_forward(&p.shape, p.dtype, ptr(p.x), ptr(p.W), ptr(p.A), ptr(p.B), ints(p.ids), floats(p.scale),
+                              floats(p.bias), ptr(y), keep, ptr(ws), need, st));
+  }
   return y;
 }
 // dx, dA, dB as far as they are wanted; p.x is dy.
@@ -553,18 +604,26 @@ void adapter_run_backward(const Adapters& p, const Tensor& x_in, const Tensor& k
     *dB = empty({(int64_t)s.G, (int64_t)s.N, (int64_t)s.R}, p.x.scalar_type(), p.x);
   }
   if (dx) *dx = empty(with_last(sizes, s.K), p.x.scalar_type(), p.x);
-  const size_t need = cp4_adapter_backward_workspace_bytes(&s, p.dtype);
+  const size_t need = p.four ? cp4_adapter_mx4_backward_workspace_bytes(&s, p.dtype) : cp4_adapter_backward_workspace_bytes(&s, p.dtype);
   const Tensor ws = scratch(need, p.x);
-  check(cp4_adapter_backward(&s, p.dtype, ptr(p.x), ptr(x), ptr(p.W), ptr(p.A), ptr(p.B), ints(p.ids), floats(p.scale),
-                             static_cast<const float*>(ptr(kept)), dx ? ptr(*dx) : nullptr, dA ? ptr(*dA) : nullptr,
-                             dB ? ptr(*dB) : nullptr, ptr(ws), need, st));
+  void *const to_x = dx ? ptr(*dx) : nullptr, *const to_A = dA ? ptr(*dA) : nullptr, *const to_B = dB ? ptr(*dB) : nullptr;
+  const float* const h = static_cast<const float*>(ptr(kept));
+  if (p.four) {
+    const cp4_mx4 w = p.mx4();
+    check(cp4_adapter_mx4_backward(&s, p.dtype, ptr(p.x), ptr(x), &w, ptr(p.A), ptr(p.B), ints(p.ids), floats(p.scale), h, to_x,
+                                   to_A, to_B, ptr(ws), need, st));
+  } else {
+    check(cp4_adapter_backward(&s, p.dtype, ptr(p.x), ptr(x), ptr(p.W), ptr(p.A), ptr(p.B), ints(p.ids), floats(p.scale), h, to_x,
+                               to_A, to_B, ptr(ws), need, st));
+  }
 }
 
 // (x, W, A, B, ids, scale, bias, out, keep, stream) -> y, or (y, kept)
 PyObject* adapter_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   require(n == 10);
-  const Tensor &x = tensor(a[0]), &W = tensor(a[1]), &A = tensor(a[2]), &B = tensor(a[3]), &ids = tensor(a[4]);
+  const Tensor &x = tensor(a[0]), &A = tensor(a[2]), &B = tensor(a[3]), &ids = tensor(a[4]);
+  const Weight W = weight_of(a[1]);
   const auto scale = optional_tensor(a[5]), bias = optional_tensor(a[6]);
   require(x.is_cuda(), "expected device tensors");
   const c10::DeviceGuard guard(x.device());
@@ -590,7 +649,8 @@ PyObject* adapter_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* adapter_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   require(n == 11);
-  const Tensor &dy = tensor(a[0]), &W = tensor(a[2]), &A = tensor(a[3]), &B = tensor(a[4]), &ids = tensor(a[5]);
+  const Tensor &dy = tensor(a[0]), &A = tensor(a[3]), &B = tensor(a[4]), &ids = tensor(a[5]);
+  const Weight W = weight_of(a[2]);
   const auto x = optional_tensor(a[1]), scale = optional_tensor(a[6]), kept = optional_tensor(a[7]);
   const bool want_dx = PyObject_IsTrue(a[8]) == 1, want = PyObject_IsTrue(a[9]) == 1;
   require(!want || (x && kept), "the adapters' gradients need x and what the forward call kept");
@@ -620,25 +680,25 @@ PyObject* adapter_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
 struct AdapterFunction : torch::autograd::Function<AdapterFunction> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& W, const Tensor& A,
                         const Tensor& B, const Tensor& ids, const std::optional<Tensor>& scale,
-                        const std::optional<Tensor>& bias) {
-    const Adapters p = adapters(x, W, A, B, ids, scale, bias);
+                        const std::optional<Tensor>& bias, const std::optional<Tensor>& scales, int64_t K) {
+    const Adapters p = adapters(x, Weight{W, scales ? *scales : Tensor(), K}, A, B, ids, scale, bias);
     const bool factors = A.requires_grad() || B.requires_grad();
     Tensor kept;
     Tensor y = adapter_run(p, x.sizes(), Tensor(), factors ? &kept : nullptr,
                            c10::hip::getCurrentHIPStream(x.device().index()).stream());
-    ctx->save_for_backward({factors ? x : Tensor(), W, A, B, ids, scale ? *scale : Tensor(), kept});
+    ctx->save_for_backward({factors ? x : Tensor(), W, A, B, ids, scale ? *scale : Tensor(), kept, scales ? *scales : Tensor()});
     return y;
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grad) {
     const auto s = ctx->get_saved_variables();
-    torch::autograd::variable_list out(7);
+    torch::autograd::variable_list out(9);
     if (!grad[0].defined()) return out;
     Tensor dy = grad[0];
-    if (dy.scalar_type() != s[1].scalar_type()) dy = dy.to(s[1].scalar_type());
+    if (dy.scalar_type() != s[2].scalar_type()) dy = dy.to(s[2].scalar_type());
     const bool want_dx = ctx->needs_input_grad(0), want = ctx->needs_input_grad(2) || ctx->needs_input_grad(3);
     const std::optional<Tensor> scale = s[5].defined() ? std::optional<Tensor>(s[5]) : std::nullopt;
-    const Adapters p = adapters(dy, s[1], s[2], s[3], s[4], scale, std::nullopt, true);
+    const Adapters p = adapters(dy, Weight{s[1], s[7], s[2].size(2)}, s[2], s[3], s[4], scale, std::nullopt, true);
     Tensor dx, dA, dB;
     void* st = c10::hip::getCurrentHIPStream(dy.device().index()).stream();
     adapter_run_backward(p, s[0], s[6], dy.sizes(), want_dx ? &dx : nullptr, want ? &dA : nullptr,
@@ -660,12 +720,13 @@ struct AdapterFunction : torch::autograd::Function<AdapterFunction> {
 PyObject* adapter_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   require(n == 7);
-  const Tensor &x = tensor(a[0]), &W = tensor(a[1]), &A = tensor(a[2]), &B = tensor(a[3]), &ids = tensor(a[4]);
+  const Tensor &x = tensor(a[0]), &A = tensor(a[2]), &B = tensor(a[3]), &ids = tensor(a[4]);
+  const Weight W = weight_of(a[1]);
   const auto scale = optional_tensor(a[5]), bias = optional_tensor(a[6]);
   auto tracked = [](const Tensor& t) {
     return (at::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined();
   };
-  if (tracked(W) || (bias && tracked(*bias)) || (scale && tracked(*scale)))
+  if (tracked(W.W) || (bias && tracked(*bias)) || (scale && tracked(*scale)))
     fail(PyExc_ValueError, "the projection, its bias and the scales are not trained: detach them");
   require(x.is_cuda(), "expected device tensors");
   const c10::DeviceGuard guard(x.device());
@@ -673,7 +734,7 @@ PyObject* adapter_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   {
     NoGil unlocked;
     if (tracked(x) || tracked(A) || tracked(B)) {
-      y = AdapterFunction::apply(x, W, A, B, ids, scale, bias);
+      y = AdapterFunction::apply(x, W.W, A, B, ids, scale, bias, W.four() ? std::optional<Tensor>(W.scales) : std::nullopt, W.K);
     } else {
       const Adapters p = adapters(x, W, A, B, ids, scale, bias);
       y = adapter_run(p, x.sizes(), Tensor(), nullptr, c10::hip::getCurrentHIPStream(x.device().index()).stream());
@@ -844,6 +905,231 @@ PyObject* layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     else
       y = norm_run(norm_rows(x, weight, bias), x.sizes(), eps, Tensor(), nullptr,
                    c10::hip::getCurrentHIPStream(x.device().index()).stream());
+  }
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// ---- microscaled 4-bit floating point (capi.mx4_*, torch_ops.mx4_linear) ---------------------------
+
+at::ScalarType type_of(PyObject* o) {
+  require(THPDtype_Check(o), "expected a dtype");
+  return reinterpret_cast<THPDtype*>(o)->scalar_type;
+}
+Weight mx4_round(const Tensor& x, void* st) {
+  require(x.is_cuda() && x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= 1 << 22, "expected a device tensor [..., K], K from 1 to 2^22");
+  Weight w;
+  w.K = x.size(-1);
+  const int64_t blocks = (w.K + 31) / 32;
+  size_t ld = 0;
+  const int dtype = dtype_of(x);
+  const Tensor rows = rows_of(x, &ld);
+  w.W = empty(with_last(x.sizes(), blocks * 16), at::kByte, x);
+  w.scales = empty(with_last(x.sizes(), blocks), at::kByte, x);
+  check(cp4_mx4_quantize((size_t)(x.numel() / w.K), (unsigned)w.K, dtype, ptr(rows), ld, w.W.data_ptr(),
+                         static_cast<unsigned char*>(w.scales.data_ptr()), st));
+  return w;
+}
+
+// (x, stream) -> (codes, scales)
+PyObject* mx4_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  require(n == 2);
+  const Tensor& x = tensor(a[0]);
+  require(x.is_cuda(), "expected device tensors");
+  const c10::DeviceGuard guard(x.device());
+  void* st = stream_of(a[1]);
+  Weight w;
+  {
+    NoGil unlocked;
+    const at::NoGradGuard no_grad;
+    w = mx4_round(x, st);
+  }
+  return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(w.W)), THPVariable_Wrap(std::move(w.scales)));
+  END_HANDLE_TH_ERRORS
+}
+
+// (q, dtype, out, stream) -> values
+PyObject* mx4_dequantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  require(n == 4);
+  const Weight q = packed_of(a[0]);
+  Tensor y = a[2] != Py_None ? tensor(a[2]) : Tensor();
+  const at::ScalarType type = y.defined() ? y.scalar_type() : type_of(a[1]);
+  const c10::DeviceGuard guard(q.W.device());
+  void* st = stream_of(a[3]);
+  {
+    NoGil unlocked;
+    const at::NoGradGuard no_grad;
+    const std::vector<int64_t> sizes = with_last(q.W.sizes(), q.K);
+    if (!y.defined()) y = empty(sizes, type, q.W);
+    require(y.is_cuda() && y.device() == q.W.device() && y.is_contiguous() && y.sizes() == at::IntArrayRef(sizes), "out does not match the result");
+    const cp4_mx4 m = q.mx4();
+    check(cp4_mx4_dequantize((size_t)(q.scales.numel() / q.scales.size(-1)), (unsigned)q.K, dtype_of(y), &m, ptr(y), st));
+  }
+  if (a[2] != Py_None && !y.is_inference()) y.unsafeGetTensorImpl()->bump_version();
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+Tensor bias_of(const std::optional<Tensor>& bias, int64_t N, const Tensor& like) {
+  require(!bias || (bias->is_cuda() && bias->device() == like.device() && bias->scalar_type() == at::kFloat && bias->dim() == 1 &&
+                    bias->size(0) == N),
+          "bias must be a float32 vector of W's rows, on x's device");
+  return bias ? bias->contiguous() : Tensor();
+}
+void check_weight(const Weight& w, const Tensor& like) {
+  require(w.W.dim() == 2 && w.W.size(0) >= 1 && w.W.size(0) <= 1 << 22, "expected codes of W [N, K], N from 1 to 2^22");
+  require(w.W.device() == like.device(), "x and W must be on one device");
+}
+Tensor output(const std::vector<int64_t>& sizes, at::ScalarType type, const Tensor& like, Tensor y) {
+  if (!y.defined()) return empty(sizes, type, like);
+  int64_t n = 1;
+  for (int64_t d : sizes) n *= d;
+  require(y.is_cuda() && y.device() == like.device() && y.scalar_type() == type && y.is_contiguous() && y.numel() == n,
+          "out does not match the result");
+  return y;
+}
+// x in its own type
+Tensor mx4_run(const Tensor& x, const Weight& w, const std::optional<Tensor>& bias_in, Tensor y, void* st) {
+  require(x.is_cuda() && x.dim() >= 1 && x.size(-1) == w.K, "x and W do not match");
+  check_weight(w, x);
+  const int64_t N = w.W.size(0);
+  const Tensor bias = bias_of(bias_in, N, x);
+  const int dtype = dtype_of(x);
+  size_t ld = 0;
+  const Tensor rows = rows_of(x, &ld);
+  y = output(with_last(x.sizes(), N), x.scalar_type(), x, y);
+  const size_t T = (size_t)(x.numel() / w.K), need = cp4_mx4_forward_workspace_bytes(T, (unsigned)w.K, (unsigned)N, dtype);
+  const Tensor ws = scratch(need, x);
+  const cp4_mx4 m = w.mx4();
+  check(cp4_mx4_forward(T, (unsigned)w.K, (unsigned)N, dtype, ptr(rows), ld, &m, floats(bias), ptr(y), ptr(ws), need, st));
+  return y;
+}
+Tensor mx4_run_backward(const Tensor& dy, const Weight& w, void* st) {
+  check_weight(w, dy);
+  const int64_t N = w.W.size(0);
+  require(dy.is_cuda() && dy.dim() >= 1 && dy.size(-1) == N, "dy and W do not match");
+  const int dtype = dtype_of(dy);
+  size_t ld = 0;
+  const Tensor rows = rows_of(dy, &ld);
+  Tensor dx = empty(with_last(dy.sizes(), w.K), dy.scalar_type(), dy);
+  const size_t T = (size_t)(dy.numel() / N), need = cp4_mx4_backward_workspace_bytes(T, (unsigned)w.K, (unsigned)N, dtype);
+  const Tensor ws = scratch(need, dy);
+  const cp4_mx4 m = w.mx4();
+  check(cp4_mx4_backward(T, (unsigned)w.K, (unsigned)N, dtype, ptr(rows), ld, &m, ptr(dx), ptr(ws), need, st));
+  return dx;
+}
+// x in 4 bits
+Tensor mx4_run_product(const Weight& x, const Weight& w, const std::optional<Tensor>& bias_in, at::ScalarType type, Tensor y, void* st) {
+  require(x.K == w.K, "x and W do not match");
+  check_weight(w, x.W);
+  const int64_t N = w.W.size(0);
+  const Tensor bias = bias_of(bias_in, N, x.W);
+  y = output(with_last(x.W.sizes(), N), type, x.W, y);
+  const size_t T = (size_t)(x.scales.numel() / x.scales.size(-1)), need = cp4_mx4_product_workspace_bytes(T, (unsigned)w.K, (unsigned)N);
+  const Tensor ws = scratch(need, x.W);
+  const cp4_mx4 mx = x.mx4(), mw = w.mx4();
+  check(cp4_mx4_product(T, (unsigned)w.K, (unsigned)N, dtype_of(y), &mx, &mw, floats(bias), ptr(y), ptr(ws), need, st));
+  return y;
+}
+
+// (x or q, W, bias, round, dtype or None, out, stream) -> y
+PyObject* mx4_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  require(n == 7);
+  const bool is_four = is_packed(a[0]), round = PyObject_IsTrue(a[3]) == 1;
+  const Weight w = packed_of(a[1]);
+  const Weight q = is_four ? packed_of(a[0]) : Weight();
+  const Tensor x = is_four ? Tensor() : tensor(a[0]);
+  const auto bias = optional_tensor(a[2]);
+  Tensor y = a[5] != Py_None ? tensor(a[5]) : Tensor();
+  const Tensor& like = is_four ? q.W : x;
+  require(like.is_cuda(), "expected device tensors");
+  const at::ScalarType type = a[4] != Py_None ? type_of(a[4]) : is_four ? (y.defined() ? y.scalar_type() : at::kFloat) : x.scalar_type();
+  require(is_four || type == x.scalar_type() || round, "y is of x's type");
+  const c10::DeviceGuard guard(like.device());
+  void* st = stream_of(a[6]);
+  {
+    NoGil unlocked;
+    const at::NoGradGuard no_grad;
+    if (is_four) {
+      y = mx4_run_product(q, w, bias, type, y, st);
+    } else if (round) {
+      require(x.dim() >= 1 && x.size(-1) == w.K, "x and W do not match");
+      y = mx4_run_product(mx4_round(x, st), w, bias, type, y, st);
+    } else {
+      y = mx4_run(x, w, bias, y, st);
+    }
+  }
+  if (a[5] != Py_None && !y.is_inference()) y.unsafeGetTensorImpl()->bump_version();
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// (dy, W, stream) -> dx
+PyObject* mx4_linear_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  require(n == 3);
+  const Tensor& dy = tensor(a[0]);
+  const Weight w = packed_of(a[1]);
+  require(dy.is_cuda(), "expected device tensors");
+  const c10::DeviceGuard guard(dy.device());
+  void* st = stream_of(a[2]);
+  Tensor dx;
+  {
+    NoGil unlocked;
+    const at::NoGradGuard no_grad;
+    dx = mx4_run_backward(dy, w, st);
+  }
+  return THPVariable_Wrap(std::move(dx));
+  END_HANDLE_TH_ERRORS
+}
+
+struct Mx4LinearFunction : torch::autograd::Function<Mx4LinearFunction> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& codes, const Tensor& scales, int64_t K,
+                        const std::optional<Tensor>& bias) {
+    Tensor y = mx4_run(x, Weight{codes, scales, K}, bias, Tensor(), c10::hip::getCurrentHIPStream(x.device().index()).stream());
+    ctx->save_for_backward({codes, scales});
+    ctx->saved_data["K"] = K;
+    ctx->saved_data["type"] = (int64_t)x.scalar_type();
+    return y;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grad) {
+    const auto s = ctx->get_saved_variables();
+    torch::autograd::variable_list out(5);
+    if (!grad[0].defined()) return out;
+    const auto type = (at::ScalarType)ctx->saved_data["type"].toInt();
+    const Tensor dy = grad[0].scalar_type() == type ? grad[0] : grad[0].to(type);
+    const Weight w{s[0], s[1], ctx->saved_data["K"].toInt()};
+    if (at::GradMode::is_enabled() && grad[0].requires_grad())       // (create_graph: dx is linear in dy, but for W it has no rule)
+      out[0] = (*std::make_shared<torch::autograd::DelayedError>("the gradients of mx4_linear cannot be differentiated again", 1))(
+          {mx4_run_backward(dy.detach(), w, c10::hip::getCurrentHIPStream(dy.device().index()).stream()).set_requires_grad(true)})[0];
+    else
+      out[0] = mx4_run_backward(dy, w, c10::hip::getCurrentHIPStream(dy.device().index()).stream());
+    return out;
+  }
+};
+
+// (x, W, bias) -> y; see torch_ops.mx4_linear
+PyObject* mx4_linear_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  require(n == 3);
+  const Tensor& x = tensor(a[0]);
+  const Weight w = packed_of(a[1]);
+  const auto bias = optional_tensor(a[2]);
+  auto tracked = [](const Tensor& t) {
+    return (at::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined();
+  };
+  if (bias && tracked(*bias)) fail(PyExc_ValueError, "the projection and its bias are not trained: detach them");
+  require(x.is_cuda(), "expected device tensors");
+  const c10::DeviceGuard guard(x.device());
+  Tensor y;
+  {
+    NoGil unlocked;
+    if (tracked(x)) y = Mx4LinearFunction::apply(x, w.W, w.scales, w.K, bias);
+    else y = mx4_run(x, w, bias, Tensor(), c10::hip::getCurrentHIPStream(x.device().index()).stream());
   }
   return THPVariable_Wrap(std::move(y));
   END_HANDLE_TH_ERRORS
@@ -1134,6 +1420,11 @@ PyMethodDef kMethods[] = {
     {"layer_norm_forward", FAST(layer_norm_forward), nullptr},
     {"layer_norm_backward", FAST(layer_norm_backward), nullptr},
     {"layer_norm", FAST(layer_norm), nullptr},
+    {"mx4_quantize", FAST(mx4_quantize), nullptr},
+    {"mx4_dequantize", FAST(mx4_dequantize), nullptr},
+    {"mx4_linear", FAST(mx4_linear), nullptr},
+    {"mx4_linear_backward", FAST(mx4_linear_backward), nullptr},
+    {"mx4_linear_grad", FAST(mx4_linear_grad), nullptr},
     {"adamw_step", FAST(adamw_step), nullptr},
     {"adamw_moments", FAST(adamw_moments), nullptr},
     {"muon_step", FAST(muon_step), nullptr},

@@ -296,43 +296,51 @@ class AdapterLinearFunction(torch.autograd.Function):
     (csrc/torch/binding.cpp) where a call has to be seen as an operator, in a trace."""
 
     @staticmethod
-    def forward(ctx, x, W, A, B, ids, scale=None, bias=None):
+    def forward(ctx, x, W, A, B, ids, scale=None, bias=None, scales=None):
+        """``scales``: of W, whose codes are in its place then (an argument each, so that a trace sees both)."""
         need = ctx.needs_input_grad
+        ctx.codes, ctx.features = scales is not None, A.shape[-1]
+        if scales is not None:
+            W = capi.Mx4(W, scales, A.shape[-1])
+        rows = (W.codes if scales is not None else W).shape[:1]
         if need[1] or need[5] or need[6]:
             raise ValueError("the projection, its bias and the scales are not trained: detach them")
         factors = need[2] or need[3]
         # (made by an operator, or the trace would not know it)
-        y = torch.empty(x.shape[:-1] + W.shape[:1], dtype=x.dtype, device=x.device)
+        y = torch.empty(x.shape[:-1] + rows, dtype=x.dtype, device=x.device)
         kept = None
         if factors:
             _, kept = capi.adapter_forward(x, W, A, B, ids, scale, bias, out=y, keep=True)
         else:
             capi.adapter_forward(x, W, A, B, ids, scale, bias, out=y)
-        ctx.save_for_backward(x if factors else None, W, A, B, ids, scale, kept)
+        ctx.save_for_backward(x if factors else None, W.codes if ctx.codes else W, A, B, ids, scale, kept, scales)
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        x, W, A, B, ids, scale, kept = ctx.saved_tensors
+        x, W, A, B, ids, scale, kept, scales = ctx.saved_tensors
+        if ctx.codes:
+            W = capi.Mx4(W, scales, ctx.features)
         need = ctx.needs_input_grad
-        dx, dA, dB = capi.adapter_backward(dy.to(W.dtype), x, W, A, B, ids, scale, kept, want_dx=need[0],
+        dx, dA, dB = capi.adapter_backward(dy.to(A.dtype), x, W, A, B, ids, scale, kept, want_dx=need[0],
                                            want_factors=need[2] or need[3])
         if torch.is_grad_enabled():              # (create_graph: as the native one)
             told = torch._C._functions.DelayedError(b"the gradients of adapter_linear cannot be differentiated again", 1)
             dx, dA, dB = (g if g is None else told(g.detach().requires_grad_()) for g in (dx, dA, dB))
-        return dx, None, dA if need[2] else None, dB if need[3] else None, None, None, None
+        return dx, None, dA if need[2] else None, dB if need[3] else None, None, None, None, None
 
 
 def adapter_linear(x, W, A, B, ids, scale=None, bias=None):
     """Functional form of a dense projection with the low-rank adapters of many requests
     beside it (``capi.adapter_forward``), differentiable in x, A and B.
 
-    W and bias are frozen: a call that asks for their gradient raises ``ValueError``.  The gradients themselves
+    W may be held in 4 bits (``capi.Mx4``).  W and bias are frozen: a call that asks for their gradient raises ``ValueError``.  The gradients themselves
     are not differentiable: after ``create_graph=True`` a second derivative raises."""
     # torch.jit.trace records operators: the native call would leave a constant in the graph
     if torch._C._get_tracing_state() is None:
         return capi._native.adapter_linear(x, W, A, B, ids, scale, bias)
-    return AdapterLinearFunction.apply(x, W, A, B, ids, scale, bias)
+    codes, scales = (W.codes, W.scales) if isinstance(W, capi.Mx4) else (W, None)
+    return AdapterLinearFunction.apply(x, codes, A, B, ids, scale, bias, scales)
 
 
 class AdapterLinear(torch.nn.Module):
@@ -342,16 +350,25 @@ class AdapterLinear(torch.nn.Module):
     A starts as normal(0, 1 / sqrt(in_features)), B as zero, so that an adapter starts as
     nothing; ``alpha / rank`` scales all of them.  ``weight`` and ``bias``: the projection's, as of
     a trained layer (kept as buffers); without them it starts as a Kaiming-normal one.  ``.to(dtype)``, ``.half()``
-    and ``.bfloat16()`` convert the projection and the adapters; scales and bias stay float32."""
+    and ``.bfloat16()`` convert the projection and the adapters; scales and bias stay float32.  ``weight_bits=4``: the
+    projection is held in microscaled 4-bit floating point (``weight_codes`` and ``weight_scales``, 17 / 32 of a byte a value)."""
 
     def __init__(self, in_features, out_features, rank, adapters=1, alpha=None, weight=None, bias=None,
-                 dtype=torch.float32, device="cuda"):
+                 dtype=torch.float32, device="cuda", weight_bits=None):
         super().__init__()
         if weight is None:
             weight = torch.randn(out_features, in_features, device=device) * (2.0 / in_features) ** 0.5
         if tuple(weight.shape) != (out_features, in_features):
             raise ValueError("weight must be [out_features, in_features]")
-        self.register_buffer("weight", weight.detach().to(device, dtype))
+        if weight_bits not in (None, 4):
+            raise ValueError("weight_bits must be None or 4")
+        self.weight_bits = weight_bits
+        if weight_bits is None:
+            self.register_buffer("weight", weight.detach().to(device, dtype))
+        else:
+            q = capi.mx4_quantize(weight.detach().to(device))
+            self.register_buffer("weight_codes", q.codes)
+            self.register_buffer("weight_scales", q.scales)
         self.register_buffer("bias", None if bias is None else bias.detach().to(device, torch.float32))
         self.register_buffer("scale", torch.full((adapters,), (rank if alpha is None else alpha) / rank,
                                                  dtype=torch.float32, device=device))
@@ -370,7 +387,71 @@ class AdapterLinear(torch.nn.Module):
         return self
 
     def forward(self, x, ids):
-        return adapter_linear(x, self.weight, self.A, self.B, ids, self.scale, self.bias)
+        W = self.weight if self.weight_bits is None else capi.Mx4(self.weight_codes, self.weight_scales, self.A.shape[-1])
+        return adapter_linear(x, W, self.A, self.B, ids, self.scale, self.bias)
+
+
+class Mx4LinearFunction(torch.autograd.Function):
+    """``mx4_linear`` as a Python autograd function: stands for the native one (csrc/torch/binding.cpp) where a
+    call has to be seen as an operator, in a trace."""
+
+    @staticmethod
+    def forward(ctx, x, codes, scales, bias=None):
+        if ctx.needs_input_grad[3]:
+            raise ValueError("the projection and its bias are not trained: detach them")
+        y = torch.empty(x.shape[:-1] + codes.shape[:1], dtype=x.dtype, device=x.device)   # (made by an operator)
+        capi.mx4_linear(x, capi.Mx4(codes, scales, x.shape[-1]), bias, out=y)
+        ctx.save_for_backward(codes, scales)
+        ctx.features, ctx.dtype = x.shape[-1], x.dtype
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        codes, scales = ctx.saved_tensors
+        dx = capi.mx4_linear_backward(dy.detach().to(ctx.dtype), capi.Mx4(codes, scales, ctx.features))
+        if torch.is_grad_enabled() and dy.requires_grad:             # (create_graph: as the native one)
+            told = torch._C._functions.DelayedError(b"the gradients of mx4_linear cannot be differentiated again", 1)
+            dx = told(dx.requires_grad_())
+        return dx, None, None, None
+
+
+def mx4_linear(x, W, bias=None):
+    """Functional form of a dense projection whose weights are held in 4 bits (``capi.mx4_linear``), differentiable
+    in x.  W and bias are frozen: a call that asks for the bias's gradient raises ``ValueError``."""
+    if torch._C._get_tracing_state() is None:
+        return capi._native.mx4_linear_grad(x, W, bias)
+    return Mx4LinearFunction.apply(x, W.codes, W.scales, bias)
+
+
+class Mx4Linear(torch.nn.Module):
+    """A frozen dense projection held in microscaled 4-bit floating point.  ``weight`` [out_features, in_features] and
+    ``bias``: of a trained layer.  ``activations=4``: inputs are rounded to 4 bits as well; such a layer has no gradients."""
+
+    def __init__(self, weight, bias=None, activations=None, device="cuda"):
+        super().__init__()
+        if activations not in (None, 4):
+            raise ValueError("activations must be None or 4")
+        self.in_features, self.activations = weight.shape[1], activations
+        q = capi.mx4_quantize(weight.detach().to(device))
+        self.register_buffer("weight_codes", q.codes)
+        self.register_buffer("weight_scales", q.scales)
+        self.register_buffer("bias", None if bias is None else bias.detach().to(device, torch.float32))
+
+    def _apply(self, fn, recurse=True):
+        """Conversions of a network leave the bias float32."""
+        old = self.bias
+        super()._apply(fn, recurse)
+        if old is not None and self.bias.dtype != torch.float32:
+            self.bias = old.to(self.bias.device, torch.float32)
+        return self
+
+    def forward(self, x):
+        W = capi.Mx4(self.weight_codes, self.weight_scales, self.in_features)
+        if self.activations is None:
+            return mx4_linear(x, W, self.bias)
+        if torch.is_grad_enabled() and x.requires_grad:
+            raise ValueError("activations in 4 bits have no gradient: detach them, or call without gradients")
+        return capi.mx4_linear(x, W, self.bias, activations=4)
 
 
 class LayerNormFunction(torch.autograd.Function):
