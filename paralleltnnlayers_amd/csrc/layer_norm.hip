@@ -7,7 +7,12 @@
 // row), the next row's loads under way while one is reduced.
 //
 // weight's and bias's gradients: a lane adds up its own columns over all rows of its workgroup in registers; the
-// workgroups' sums, [parts][2][D], go to memory and a second launch adds them up in their order.
+// workgroups' sums, [parts][2][D], go to memory and a second launch adds them up in their order.  Rows of more than 16384
+// values leave no registers for those sums: a launch by columns reads x and dy once more.
+//
+// Measured: 8192 x 4096 bf16: forward 27 us, 5.0 TB/s (a large copy reaches 5.1), backward 49 us with the second launch's
+// 5, 4.1 TB/s; fp32 44 and 83 us.  8192 x 1024 bf16: 9.5 and 17 us.  1024 x 25088 bf16: 59 and 89 us, where sixteen waves of 128
+// registers hold a row and nothing overlaps its loads.  One row of 4096: 5 us, a launch and three waits for memory.
 #include <algorithm>
 
 #include "cp4/layer_norm.h"
@@ -66,6 +71,7 @@ template <class T, int VPT, int W>
 struct Row {
   typedef typename T::raw Raw;
   static constexpr int n = 16 / (int)sizeof(Raw), C = VPT / n, kLanes = 64 * W, kRows = W == 1 ? 4 : 1;
+  static constexpr bool kKeep = VPT <= 16;         // whether there are registers for what belongs to a lane's columns
   struct Chunk { Raw v[n]; };
 
   static __device__ __forceinline__ int column(int c, int lane) { return (c * kLanes + lane) * n; }
@@ -84,12 +90,19 @@ struct Row {
   }
   static __device__ __forceinline__ void floats(const float* p, float otherwise, int D, int lane, float (&v)[VPT]) {
 #pragma unroll
-    for (int c = 0; c < C; ++c)
+    for (int i = 0; i < VPT; ++i) v[i] = otherwise;
+    if (!p) return;
 #pragma unroll
-      for (int j = 0; j < n; ++j) {
-        const int at = column(c, lane) + j;
-        v[c * n + j] = p && at < D ? p[at] : otherwise;
+    for (int c = 0; c < C; ++c) {
+      const int at = column(c, lane);
+      if (at + n <= D) {
+        __builtin_memcpy(v + c * n, p + at, n * sizeof(float));
+      } else {
+#pragma unroll
+        for (int j = 0; j < n; ++j)
+          if (at + j < D) v[c * n + j] = p[at + j];
       }
+    }
   }
   static __device__ __forceinline__ void store(Raw* p, int D, int lane, const float (&v)[VPT]) {
 #pragma unroll
@@ -184,29 +197,35 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void backward_kernel(const B
   const size_t step = (size_t)gridDim.x * R::kRows;
   size_t t = (size_t)blockIdx.x * R::kRows + (W == 1 ? wave : 0);
   const float over = 1.0f / (float)D;
-  float w[VPT], dw[VPT] = {}, db[VPT] = {};
-  R::floats(a.weight, 1.0f, D, lane, w);
+  float w[VPT], dw[R::kKeep ? VPT : 1] = {}, db[R::kKeep ? VPT : 1] = {};
+  if constexpr (R::kKeep) R::floats(a.weight, 1.0f, D, lane, w);
   typename R::Chunk x_next[R::C], dy_next[R::C];
   float m_next = 0.0f, r_next = 0.0f;
   auto load = [&](size_t row) __attribute__((always_inline)) {
     R::load(static_cast<const Raw*>(a.x) + row * a.ldx, D, lane, x_next);
     R::load(static_cast<const Raw*>(a.dy) + row * a.lddy, D, lane, dy_next);
-    m_next = a.stats[2 * row];
-    r_next = a.stats[2 * row + 1];
+    // (by a vector load: a scalar one would be waited for with the LDS's sums of this row)
+    size_t at = 2 * row;
+    asm volatile("" : "+v"(at));
+    m_next = a.stats[at];
+    r_next = a.stats[at + 1];
   };
   if (t < a.T) load(t);
   for (int turn = 0; t < a.T; t += step, turn ^= 1) {
     float h[VPT], g[VPT];
     const float m = m_next, r = r_next;
     float s = 0.0f, q = 0.0f;
+    if constexpr (!R::kKeep) R::floats(a.weight, 1.0f, D, lane, w);
+    // (columns beyond the row: dy and with it all that is summed is zero)
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const bool there = R::column(i / R::n, lane) + i % R::n < D;
       const float dy = T::widen(dy_next[i / R::n].v[i % R::n]);
-      h[i] = there ? (T::widen(x_next[i / R::n].v[i % R::n]) - m) * r : 0.0f;
-      g[i] = there ? dy * w[i] : 0.0f;
-      db[i] += dy;
-      dw[i] += dy * h[i];
+      h[i] = (T::widen(x_next[i / R::n].v[i % R::n]) - m) * r;
+      g[i] = dy * w[i];
+      if constexpr (R::kKeep) {
+        db[i] += dy;
+        dw[i] += dy * h[i];
+      }
       s += g[i];
       q += g[i] * h[i];
     }
@@ -219,7 +238,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void backward_kernel(const B
     for (int i = 0; i < VPT; ++i) h[i] = r * (g[i] - s - h[i] * q);
     R::store(static_cast<Raw*>(a.dx) + t * D, D, lane, h);
   }
-  if (!a.dweight && !a.dbias) return;
+  if (!R::kKeep || (!a.dweight && !a.dbias)) return;
   if constexpr (W == 1) {
     // the four waves' sums, one after the other
     for (int k = 0; k < R::kRows; ++k) {
@@ -235,16 +254,71 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void backward_kernel(const B
     }
     if (wave != R::kRows - 1) return;
   }
-  float* const pw = a.dweight ? a.dweight + blockIdx.x * a.next : nullptr;
-  float* const pb = a.dbias ? a.dbias + blockIdx.x * a.next : nullptr;
+  if constexpr (R::kKeep) {
+    float* const pw = a.dweight ? a.dweight + blockIdx.x * a.next : nullptr;
+    float* const pb = a.dbias ? a.dbias + blockIdx.x * a.next : nullptr;
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const int at = R::column(i / R::n, lane) + i % R::n;
-    if (at >= D) continue;
-    if (pw) pw[at] = dw[i];
-    if (pb) pb[at] = db[i];
+    for (int i = 0; i < VPT; ++i) {
+      const int at = R::column(i / R::n, lane) + i % R::n;
+      if (at >= D) continue;
+      if (pw) pw[at] = dw[i];
+      if (pb) pb[at] = db[i];
+    }
   }
 }
+
+// The gradients of weight and bias of rows whose columns leave no registers for them above: 512 columns (fp32: 256) and every
+// gridDim.y-th row a workgroup, four rows at a time, whose sums meet in the LDS.
+template <class T>
+__global__ __launch_bounds__(256) void columns_kernel(const BackwardArgs a) {
+  typedef typename T::raw Raw;
+  constexpr int n = 16 / (int)sizeof(Raw);
+  __shared__ float sums[2][64 * n];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = (blockIdx.x * 64 + lane) * n;
+  float dw[n] = {}, db[n] = {};
+  if (c < a.D) {
+#pragma unroll 4
+    for (size_t t = blockIdx.y * 4 + wave; t < a.T; t += gridDim.y * 4) {
+      const Raw *const px = static_cast<const Raw*>(a.x) + t * a.ldx + c, *const pdy = static_cast<const Raw*>(a.dy) + t * a.lddy + c;
+      Raw x[n], dy[n];
+      if (c + n <= a.D) {
+        __builtin_memcpy(x, px, sizeof(x));
+        __builtin_memcpy(dy, pdy, sizeof(dy));
+      } else {
+#pragma unroll
+        for (int j = 0; j < n; ++j) {
+          x[j] = c + j < a.D ? px[j] : Raw(0);
+          dy[j] = c + j < a.D ? pdy[j] : Raw(0);
+        }
+      }
+      const float m = a.stats[2 * t], r = a.stats[2 * t + 1];
+#pragma unroll
+      for (int j = 0; j < n; ++j) {
+        db[j] += T::widen(dy[j]);
+        dw[j] += T::widen(dy[j]) * ((T::widen(x[j]) - m) * r);
+      }
+    }
+  }
+  for (int k = 0; k < 4; ++k) {
+    if (wave == k) {
+#pragma unroll
+      for (int j = 0; j < n; ++j) {
+        float *const pw = &sums[0][lane * n + j], *const pb = &sums[1][lane * n + j];
+        *pw = dw[j] = k ? *pw + dw[j] : dw[j];
+        *pb = db[j] = k ? *pb + db[j] : db[j];
+      }
+    }
+    __syncthreads();
+  }
+  if (wave != 3) return;
+#pragma unroll
+  for (int j = 0; j < n; ++j) {
+    if (c + j >= a.D) continue;
+    a.dweight[blockIdx.y * a.next + c + j] = dw[j];
+    a.dbias[blockIdx.y * a.next + c + j] = db[j];
+  }
+}
+
 
 // out[c] = sum over p of part[p][c], c < 2 D: weight's gradient, then bias's.  A workgroup has 64 columns, its waves every
 // 16th part.
@@ -299,7 +373,14 @@ unsigned grid_of(size_t T, unsigned D, unsigned on_a_unit) {
   const size_t rows = s.waves == 1 ? 4 : 1, most = (size_t)cp4::num_compute_units() * (s.waves > 4 ? std::max(1u, 4 * on_a_unit / s.waves) : on_a_unit);
   return (unsigned)std::min((T + rows - 1) / rows, most);
 }
-constexpr unsigned kForward = 8, kBackward = 4;
+// Forward from 4 to 16 of them differ by 4 %.  Backward each of them leaves a set of partial sums: 8192 x 4096 bf16 takes 49 us
+// with two of them, 53 with three, 58 with four, 80 with eight (fp32 83, 85, 85, 98).
+constexpr unsigned kForward = 8, kBackward = 2;
+// Partial sums of the gradients of weight and bias: one set a workgroup, or of the kernel that goes by columns.
+bool by_columns(unsigned D) { return split_of(D).vpt > 16; }
+unsigned parts_of(size_t T, unsigned D) {
+  return by_columns(D) ? (unsigned)std::min<size_t>((T + 15) / 16, 64) : grid_of(T, D, kBackward);
+}
 
 template <template <class, int, int> class Launch, class T, class Args>
 void by_size(const Args& a, unsigned grid, hipStream_t st) {
@@ -369,8 +450,8 @@ extern "C" cp4_status cp4_layer_norm_forward(size_t T, unsigned D, int dtype, co
 
 extern "C" size_t cp4_layer_norm_backward_workspace_bytes(size_t T, unsigned D) {
   if (check_rows(T, D, CP4_DTYPE_F32, 0, 0) != CP4_OK || !T) return 0;
-  const unsigned grid = grid_of(T, D, kBackward);
-  return grid > 1 ? (size_t)grid * 2 * D * sizeof(float) : 0;
+  const unsigned parts = parts_of(T, D);
+  return parts > 1 || by_columns(D) ? (size_t)parts * 2 * D * sizeof(float) : 0;
 }
 
 extern "C" cp4_status cp4_layer_norm_backward(size_t T, unsigned D, int dtype, const void* dy, size_t lddy,
@@ -387,8 +468,8 @@ extern "C" cp4_status cp4_layer_norm_backward(size_t T, unsigned D, int dtype, c
     return CP4_OK;
   }
   if (!dy || !x || !stats) return fail_with(CP4_ERR_NULL_POINTER, "an operand is NULL");
-  const unsigned grid = grid_of(T, D, kBackward);
-  const bool sums = dweight || dbias, parts = sums && grid > 1;
+  const unsigned count = parts_of(T, D);
+  const bool sums = dweight || dbias, columns = by_columns(D), parts = sums && (count > 1 || columns);
   if (parts && (!workspace || ((size_t)workspace & 15) || workspace_bytes < cp4_layer_norm_backward_workspace_bytes(T, D)))
     return fail_with(CP4_ERR_WORKSPACE, "workspace missing, too small or not aligned to 16 bytes");
   BackwardArgs a{dy, x, weight, stats, dx, dweight, dbias, T, lddy ? lddy : D, ldx ? ldx : D, 0, (int)D};
@@ -397,9 +478,16 @@ extern "C" cp4_status cp4_layer_norm_backward(size_t T, unsigned D, int dtype, c
     a.dbias = a.dweight + D;
     a.next = 2 * (size_t)D;
   }
-  by_type<Backward>(a, dtype, grid, st);
+  if (dx || !columns) by_type<Backward>(a, dtype, grid_of(T, D, kBackward), st);
+  if (sums && columns) {
+    const unsigned wide = dtype == CP4_DTYPE_F32 ? 256 : 512;
+    const dim3 grid((D + wide - 1) / wide, count);
+    if (dtype == CP4_DTYPE_F32) columns_kernel<F32><<<grid, 256, 0, st>>>(a);
+    else if (dtype == CP4_DTYPE_BF16) columns_kernel<BF16><<<grid, 256, 0, st>>>(a);
+    else columns_kernel<F16><<<grid, 256, 0, st>>>(a);
+  }
   if (parts)
-    parts_kernel<<<(2 * D + 63) / 64, 1024, 0, st>>>(static_cast<const float*>(workspace), (int)grid, (int)D, dweight, dbias);
+    parts_kernel<<<(2 * D + 63) / 64, 1024, 0, st>>>(static_cast<const float*>(workspace), (int)count, (int)D, dweight, dbias);
   if (const hipError_t e = hipGetLastError()) return fail_hip(e, "cp4_layer_norm_backward");
   return CP4_OK;
 }
