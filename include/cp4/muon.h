@@ -30,15 +30,14 @@ typedef struct cp4_muon_matrix {
   void* param;          /* of param_dtype, updated; NULL: no step is taken */
   const void* grad;     /* of grad_dtype */
   float* momentum;      /* updated; NULL: u is grad */
-  void* copy;           /* NULL, or of copy_dtype: the new parameters, rounded (with param) */
-  void* out;            /* NULL, or of out_dtype: X */
+  void* copy;           /* NULL, or of copy_dtype: the new parameters, rounded; without param X itself */
   size_t count;
   unsigned rows, cols;  /* up to 65536 each; nothing is read or written where one of the three is 0 */
-  int param_dtype, grad_dtype, copy_dtype, out_dtype;   /* cp4_dtype */
+  int param_dtype, grad_dtype, copy_dtype;   /* cp4_dtype */
 } cp4_muon_matrix;
 
-/* One step.  Asynchronous on `stream`, kernel launches only: three for up to 24 entries with a side of up to 64, and
- * 3 steps + 2 for up to 16 larger ones whose scratch memory stays below 1 GiB together (a larger matrix on its
+/* One step.  Asynchronous on `stream`, kernel launches only: three for up to 72 entries whose shorter sides round up to
+ * the same multiple of 16 up to 64, and 3 steps + 2 (long ones: 4 steps + 2) for up to 16 larger ones whose scratch memory stays below 1 GiB together (a larger matrix on its
  * own).  steps: 1 to 16.  eps: above 0.  workspace: cp4_muon_workspace_bytes() of device memory, 256-byte aligned, its
  * contents scratch.  Matrices must not overlap one another. */
 size_t cp4_muon_workspace_bytes(const cp4_muon_matrix* matrices, size_t count);

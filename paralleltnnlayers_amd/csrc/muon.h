@@ -15,23 +15,23 @@ constexpr double kA = 3.4445, kB = -4.7750, kC = 2.0315;
 
 // A matrix [rows][cols] in two float16 parts: each 32 columns of a row are 64 bytes of first parts, then 64 of what those
 // leave (one cache line), columns behind the last one up to a multiple of 32 are zero.  Values times kScale: X's, A's
-// and B's magnitudes are below 1.3, 1.5 and 2.9 (the largest that the polynomial makes of singular values in 0 .. 1.21),
+// and a + b A + c A A's magnitudes are below 1.3, 1.5 and 3.45 (of singular values in 0 .. 1.21, where the polynomial keeps them),
 // so that 2^14 keeps them below float16's 65504, and the second parts of an average value of a matrix of 65536 by 65536
 // above its smallest steps.
 constexpr float kScale = 16384.0f;
 inline __host__ __device__ size_t padded(size_t cols) { return (cols + 31) / 32 * 32; }
 inline __host__ __device__ size_t part_bytes(size_t rows, size_t cols) { return rows * padded(cols) * 4; }
 
-// How a matrix's new values leave the last product.
+// How a matrix's new values leave the last product: param null: X goes to `copy`.
 struct Outputs {
-  void *param, *copy, *out;                 // [rows][cols] each, one matrix behind the other; may be null
-  int param_dtype, copy_dtype, out_dtype;
+  void *param, *copy;                       // [rows][cols] each, one matrix behind the other; may be null
+  int param_dtype, copy_dtype;
 };
 struct Rates {
   float decay, rate;                        // p = p decay - rate X
 };
 
-// C[r][c] = alpha E[r][c] + beta sum_k P[r][k] Q[c][k], r < R, c < N, of `count` matrices one behind the other, P [R][K],
+// C[r][c] = alpha E[r][c] + beta sum_k P[r][k] Q[c][k] (+ diagonal where r == c), r < R, c < N, of `count` matrices one behind the other, P [R][K],
 // Q [N][K], E and C [R][N] in two parts.
 struct Product {
   const char *P, *Q, *E;                    // E null: alpha is 0
@@ -40,7 +40,7 @@ struct Product {
   Outputs o;
   Rates rates;
   unsigned R, N, K, count;
-  float alpha, beta;
+  float alpha, beta, diagonal;
   bool symmetric;                           // R == N and C is symmetric: tiles on and below the diagonal, mirrored into C
 };
 constexpr int kProducts = 16;               // of a launch
@@ -50,6 +50,16 @@ int product_splits(const Product* p, int n);
 hipError_t product_launch(const Product* p, int n, int splits, hipStream_t st);
 
 // ---- device side ------------------------------------------------------------------------
+
+// The entry that workgroup `wg` works for, first: the entries' first ones, behind the last entry ~0.  (All of them are loaded
+// at once: one after the other they were 4 us of a launch of 24 entries.)
+template <int n>
+__device__ __forceinline__ int entry_of(const unsigned (&first)[n], unsigned wg) {
+  int k = 0;
+#pragma unroll
+  for (int i = 1; i < n; ++i) k += wg >= first[i];
+  return k;
+}
 
 __device__ __forceinline__ float load_value(const void* p, int dtype, size_t at) {
   if (dtype == CP4_DTYPE_F32) return static_cast<const float*>(p)[at];
@@ -93,13 +103,15 @@ __device__ __forceinline__ void store_values(void* p, int dtype, size_t at, int 
 // The step of up to n consecutive parameters along x, and what else wants the outcome.
 template <int n>
 __device__ __forceinline__ void put_out(const Outputs& o, const Rates& r, size_t at, int count, const float (&x)[n]) {
-  if (o.out) store_values<n>(o.out, o.out_dtype, at, count, x);
-  if (!o.param) return;
   float p[n];
-  load_values<n>(o.param, o.param_dtype, at, count, p);
 #pragma unroll
-  for (int j = 0; j < n; ++j) p[j] = p[j] * r.decay - r.rate * x[j];
-  store_values<n>(o.param, o.param_dtype, at, count, p);
+  for (int j = 0; j < n; ++j) p[j] = x[j];
+  if (o.param) {
+    load_values<n>(o.param, o.param_dtype, at, count, p);
+#pragma unroll
+    for (int j = 0; j < n; ++j) p[j] = p[j] * r.decay - r.rate * x[j];
+    store_values<n>(o.param, o.param_dtype, at, count, p);
+  }
   if (o.copy) store_values<n>(o.copy, o.copy_dtype, at, count, p);
 }
 // A scaled value as two float16 parts.

@@ -11,7 +11,8 @@
 //   apply     X = Q u in fp32 and the parameters' step.
 //
 // So the step is bound by memory where matrices are long (12 bytes a value in gram, 16 in apply) and by the
-// latency of three launches where they are short.  The entries of a launch are a table in the kernel's arguments.
+// latency of three launches where they are short: 28 adapters' factors of 7 x 1001 and 777 x 7 7 + 6 + 8 us.  The entries of a
+// launch are a table in the kernel's arguments.
 #include <algorithm>
 #include <cmath>
 #include <exception>
@@ -26,7 +27,7 @@ namespace {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kSmall = 24, kLarge = 16;            // entries of a launch
+constexpr int kSmall = 72, kLarge = 16;            // entries of a launch
 static_assert(kLarge <= kProducts, "a launch of products holds a group");
 constexpr unsigned kSide = 64;                     // the longest short side that goes through its Gram matrix
 
@@ -35,18 +36,18 @@ constexpr unsigned kSide = 64;                     // the longest short side tha
 struct SmallItem {
   const void* grad;
   float* momentum;
-  Outputs o;
-  int grad_dtype;
-  unsigned rows, cols;
-  unsigned splits, tiles;                          // of a matrix: workgroups of gram, of apply
-  unsigned gram, iterate, apply;                   // the entry's first workgroup of each launch
-  Rates rates;
+  void *param, *copy;
+  unsigned short last_row, last_col;
+  unsigned char splits, param_dtype, grad_dtype, copy_dtype;       // splits: of a matrix, workgroups of gram
+  __device__ unsigned rows() const { return last_row + 1u; }
+  __device__ unsigned cols() const { return last_col + 1u; }
 };
 struct SmallArgs {
   SmallItem item[kSmall];
-  int count, nesterov, steps;
-  float mu;
-  double eps;
+  unsigned gram[kSmall], iterate[kSmall], apply[kSmall];           // an entry's first workgroup of each launch; ~0: no entry
+  int nesterov, steps;
+  float mu, decay;
+  double eps, lr;
   double* part;                                    // [gram's workgroups][blocks][16][16]
   float* q;                                        // [iterate's workgroups][M][M]
 };
@@ -58,13 +59,6 @@ struct Tile {
   static constexpr int M = 16 * MB, JT = MB == 1 ? 256 : MB == 2 ? 128 : 64, S = JT + 4;
   static constexpr int kBlocks = MB * (MB + 1) / 2;                // 16 x 16, on and below the diagonal
 };
-// The entry that workgroup `wg` works for; first: the entries' first ones.
-template <class Item, class First>
-__device__ __forceinline__ int entry_of(const Item* item, int count, unsigned wg, First first) {
-  int k = 0;
-  while (k + 1 < count && wg >= first(item[k + 1])) ++k;
-  return k;
-}
 // Four consecutive values of u, and where they update the momentum its new values.
 template <bool Update>
 __device__ __forceinline__ void direction(const void* grad, int dtype, float* momentum, size_t at, int count, float mu,
@@ -86,8 +80,8 @@ __device__ __forceinline__ void direction(const void* grad, int dtype, float* mo
 template <int MB, class Fn>
 __device__ __forceinline__ void for_tile(const SmallItem& it, int j0, Fn fn) {
   constexpr int JT = Tile<MB>::JT;
-  const int m = min(it.rows, it.cols), n = max(it.rows, it.cols);
-  if (it.rows <= it.cols) {
+  const int m = min(it.rows(), it.cols()), n = max(it.rows(), it.cols());
+  if (it.rows() <= it.cols()) {
     for (int e = threadIdx.x * 4; e < m * JT; e += 1024) {
       const int i = e / JT, j = e % JT;
       if (j0 + j < n) fn((size_t)i * n + j0 + j, n - j0 - j, i, j);
@@ -100,8 +94,8 @@ __device__ __forceinline__ void for_tile(const SmallItem& it, int j0, Fn fn) {
 template <int MB, bool Update>
 __device__ __forceinline__ void load_tile(const SmallArgs& a, const SmallItem& it, size_t base, int j0, float* u) {
   constexpr int JT = Tile<MB>::JT, S = Tile<MB>::S;
-  const int m = min(it.rows, it.cols), n = max(it.rows, it.cols);
-  const bool flat = it.rows <= it.cols;
+  const int m = min(it.rows(), it.cols()), n = max(it.rows(), it.cols());
+  const bool flat = it.rows() <= it.cols();
   if (j0 + JT > n)                                                 // (the last tile: what it lacks is zero)
     for (int e = threadIdx.x; e < m * JT; e += 256)
       if (j0 + e % JT >= n) u[e / JT * S + e % JT] = 0.0f;
@@ -130,13 +124,14 @@ __global__ __launch_bounds__(256) void gram_kernel(const SmallArgs a) {
   typedef Tile<MB> T;
   __shared__ __attribute__((aligned(16))) float u[T::M * T::S];
   __shared__ double sum[T::kBlocks * 256];
-  const SmallItem& it = a.item[entry_of(a.item, a.count, blockIdx.x, [](const SmallItem& i) { return i.gram; })];
+  const int entry = entry_of(a.gram, blockIdx.x);
+  const SmallItem& it = a.item[entry];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
-  const unsigned matrix = (blockIdx.x - it.gram) / it.splits, split = (blockIdx.x - it.gram) % it.splits;
-  const int m = min(it.rows, it.cols);
-  const size_t base = (size_t)matrix * it.rows * it.cols;
+  const unsigned splits = it.splits, matrix = (blockIdx.x - a.gram[entry]) / splits, split = (blockIdx.x - a.gram[entry]) % splits;
+  const int m = min(it.rows(), it.cols()), tiles = (max(it.rows(), it.cols()) + T::JT - 1) / T::JT;
+  const size_t base = (size_t)matrix * it.rows() * it.cols();
   for (int e = m * T::S + threadIdx.x; e < T::M * T::S; e += 256) u[e] = 0.0f;
-  const int first = (int)((size_t)it.tiles * split / it.splits), last = (int)((size_t)it.tiles * (split + 1) / it.splits);
+  const int first = tiles * split / splits, last = tiles * (split + 1) / splits;
   f64x4 acc[T::kBlocks] = {};
   for (int t = first; t < last; ++t) {
     __syncthreads();
@@ -209,19 +204,20 @@ __global__ __launch_bounds__(256) void iterate_kernel(const SmallArgs a) {
   constexpr int M = T::M, S = M + 4;
   __shared__ double lds[4][M * S];
   double *const A = lds[0], *const P = lds[1], *Q = lds[2], *R = lds[3];
-  const SmallItem& it = a.item[entry_of(a.item, a.count, blockIdx.x, [](const SmallItem& i) { return i.iterate; })];
-  const double* const part = a.part + (it.gram + (size_t)(blockIdx.x - it.iterate) * it.splits) * (T::kBlocks * 256);
+  const int entry = entry_of(a.iterate, blockIdx.x);
+  const unsigned splits = a.item[entry].splits;
+  const double* const part = a.part + (a.gram[entry] + (size_t)(blockIdx.x - a.iterate[entry]) * splits) * (T::kBlocks * 256);
   for (int e = threadIdx.x; e < T::kBlocks * 256; e += 256) {
     double x = 0.0;
     unsigned s = 0;
-    for (; s + 8 <= it.splits; s += 8) {
+    for (; s + 8 <= splits; s += 8) {
       double y[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) y[k] = part[(size_t)(s + k) * (T::kBlocks * 256) + e];
 #pragma unroll
       for (int k = 0; k < 8; ++k) x += y[k];
     }
-    for (; s < it.splits; ++s) x += part[(size_t)s * (T::kBlocks * 256) + e];
+    for (; s < splits; ++s) x += part[(size_t)s * (T::kBlocks * 256) + e];
     int i = 0, first = 0;
     while (first + i + 1 <= e / 256) first += ++i;
     const int r = 16 * i + e % 256 / 16, c = 16 * (e / 256 - first) + e % 16;
@@ -259,18 +255,67 @@ __global__ __launch_bounds__(256) void iterate_kernel(const SmallArgs a) {
   for (int e = threadIdx.x; e < M * M; e += 256) q[e] = (float)(Q[e / M * S + e % M] * over);
 }
 
+// A short side of up to 16: one wave does it in its registers.  An fp64 product's result holds, at a lane's place v, row
+// lane / 16 + 4 v and column lane % 16, which is also what its operands want there, the first one turned: so products
+// are X^T Y without a move, and X Y as long as X is symmetric but for roundings, which X^T Y does not let grow (X Y^T
+// would, nine-fold with each step).
+__device__ __forceinline__ f64x4 turned_product(const f64x4& x, const f64x4& y) {
+  f64x4 acc = {};
+#pragma unroll
+  for (int s = 0; s < 4; ++s) acc = __builtin_amdgcn_mfma_f64_16x16x4f64(x[s], y[s], acc, 0, 0, 0);
+  return acc;
+}
+__global__ __launch_bounds__(256) void iterate_16_kernel(const SmallArgs a) {
+  __shared__ double sums[3][256];
+  const int entry = entry_of(a.iterate, blockIdx.x), lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
+  const unsigned splits = a.item[entry].splits;
+  const double* const part = a.part + (a.gram[entry] + (size_t)(blockIdx.x - a.iterate[entry]) * splits) * 256;
+  f64x4 A = {};
+#pragma unroll 4
+  for (unsigned s = wave; s < splits; s += 4)
+#pragma unroll
+    for (int v = 0; v < 4; ++v) A[v] += part[(size_t)s * 256 + (g + 4 * v) * 16 + l];
+  if (wave)
+#pragma unroll
+    for (int v = 0; v < 4; ++v) sums[wave - 1][64 * v + lane] = A[v];
+  __syncthreads();
+  if (wave) return;
+#pragma unroll
+  for (int w = 0; w < 3; ++w)
+#pragma unroll
+    for (int v = 0; v < 4; ++v) A[v] += sums[w][64 * v + lane];
+  double trace = 0.0;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) trace += g + 4 * v == l ? A[v] : 0.0;
+  trace = wave_sum(trace);
+  const double over = trace < INFINITY ? 1.0 / (sqrt(trace) + a.eps) : (double)NAN;
+  A = A * over * over;
+  f64x4 Q = {};
+  for (int s = 0; s < a.steps; ++s) {
+    f64x4 P = turned_product(A, A);                                // a + b A + c A A
+#pragma unroll
+    for (int v = 0; v < 4; ++v) P[v] = kC * P[v] + kB * A[v] + (g + 4 * v == l ? kA : 0.0);
+    Q = s ? turned_product(Q, P) : P;
+    if (s + 1 < a.steps) A = turned_product(turned_product(A, P), P);
+  }
+#pragma unroll
+  for (int v = 0; v < 4; ++v) a.q[(size_t)blockIdx.x * 256 + (g + 4 * v) * 16 + l] = (float)(Q[v] * over);
+}
+
 template <int MB>
 __global__ __launch_bounds__(256) void apply_kernel(const SmallArgs a) {
   typedef Tile<MB> T;
   constexpr int M = T::M, SQ = M + 4;
   __shared__ __attribute__((aligned(16))) float u[M * T::S], q[M * SQ];
-  const SmallItem& it = a.item[entry_of(a.item, a.count, blockIdx.x, [](const SmallItem& i) { return i.apply; })];
+  const int entry = entry_of(a.apply, blockIdx.x);
+  const SmallItem& it = a.item[entry];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
-  const unsigned matrix = (blockIdx.x - it.apply) / it.tiles, tile = (blockIdx.x - it.apply) % it.tiles;
-  const int m = min(it.rows, it.cols), j0 = tile * T::JT;
-  const size_t base = (size_t)matrix * it.rows * it.cols;
+  const unsigned tiles = (max(it.rows(), it.cols()) + T::JT - 1) / T::JT;
+  const unsigned matrix = (blockIdx.x - a.apply[entry]) / tiles, tile = (blockIdx.x - a.apply[entry]) % tiles;
+  const int m = min(it.rows(), it.cols()), j0 = tile * T::JT;
+  const size_t base = (size_t)matrix * it.rows() * it.cols();
   for (int e = m * T::S + threadIdx.x; e < M * T::S; e += 256) u[e] = 0.0f;
-  const float* const from = a.q + (size_t)(it.iterate + matrix) * (M * M);
+  const float* const from = a.q + (size_t)(a.iterate[entry] + matrix) * (M * M);
   for (int e = threadIdx.x; e < M * M; e += 256) q[e / M * SQ + e % M] = from[e];
   load_tile<MB, false>(a, it, base, j0, u);
   __syncthreads();
@@ -290,12 +335,10 @@ __global__ __launch_bounds__(256) void apply_kernel(const SmallArgs a) {
       for (int v = 0; v < 4; ++v) u[(16 * i + 4 * g + v) * T::S + 16 * b + l] = acc[i][v];
   }
   __syncthreads();
-  Outputs o = it.o;
   const auto shift = [&](void* p, int dtype) { return p ? (char*)p + base * (dtype == CP4_DTYPE_F32 ? 4 : 2) : nullptr; };
-  o.param = shift(o.param, o.param_dtype);
-  o.copy = shift(o.copy, o.copy_dtype);
-  o.out = shift(o.out, o.out_dtype);
-  const bool flat = it.rows <= it.cols;
+  const Outputs o{shift(it.param, it.param_dtype), shift(it.copy, it.copy_dtype), it.param_dtype, it.copy_dtype};
+  const bool flat = it.rows() <= it.cols();
+  const Rates rates{a.decay, (float)(a.lr * sqrt(fmax(1.0, (double)it.rows() / it.cols())))};
   for_tile<MB>(it, j0, [&](size_t at, int count, int i, int j) __attribute__((always_inline)) {
     float x[4];
 #pragma unroll
@@ -308,14 +351,15 @@ __global__ __launch_bounds__(256) void apply_kernel(const SmallArgs a) {
         ++j;
       }
     }
-    put_out<4>(o, it.rates, at, count, x);
+    put_out<4>(o, rates, at, count, x);
   });
 }
 
 template <int MB>
 hipError_t small_launch(const SmallArgs& a, unsigned gram, unsigned iterate, unsigned apply, hipStream_t st) {
   gram_kernel<MB><<<gram, 256, 0, st>>>(a);
-  iterate_kernel<MB><<<iterate, 256, 0, st>>>(a);
+  if constexpr (MB == 1) iterate_16_kernel<<<iterate, 256, 0, st>>>(a);
+  else iterate_kernel<MB><<<iterate, 256, 0, st>>>(a);
   apply_kernel<MB><<<apply, 256, 0, st>>>(a);
   return hipGetLastError();
 }
@@ -328,12 +372,12 @@ struct LargeItem {
   char *rows_out, *cols_out;                       // X as [rows][cols] and as [cols][rows], one matrix behind the other
   int grad_dtype;
   unsigned rows, cols;
-  unsigned chunks, norm;                           // of a matrix, and the entry's first workgroup: the norm's launch ...
-  unsigned tiles, split;                           // ... and the split's
+  unsigned chunks, tiles;                          // of a matrix: workgroups of the norm's launch and of the split's
 };
 struct LargeArgs {
   LargeItem item[kLarge];
-  int count, nesterov;
+  unsigned norm[kLarge], split[kLarge];            // an entry's first workgroup of each launch; ~0: no entry
+  int nesterov;
   unsigned chunk;                                  // values of a workgroup of the norm's launch
   float mu;
   double eps;
@@ -342,8 +386,9 @@ struct LargeArgs {
 static_assert(sizeof(LargeArgs) <= 4096, "kernel arguments");
 
 __global__ __launch_bounds__(256) void norm_kernel(const LargeArgs a) {
-  const LargeItem& it = a.item[entry_of(a.item, a.count, blockIdx.x, [](const LargeItem& i) { return i.norm; })];
-  const unsigned matrix = (blockIdx.x - it.norm) / it.chunks, chunk = (blockIdx.x - it.norm) % it.chunks;
+  const int entry = entry_of(a.norm, blockIdx.x);
+  const LargeItem& it = a.item[entry];
+  const unsigned matrix = (blockIdx.x - a.norm[entry]) / it.chunks, chunk = (blockIdx.x - a.norm[entry]) % it.chunks;
   const size_t size = (size_t)it.rows * it.cols, base = matrix * size;
   const size_t first = (size_t)chunk * a.chunk, last = min(size, first + a.chunk);
   double s = 0.0;
@@ -365,11 +410,12 @@ __global__ __launch_bounds__(256) void norm_kernel(const LargeArgs a) {
 __global__ __launch_bounds__(256) void split_kernel(const LargeArgs a) {
   __shared__ float lds[64][65];
   __shared__ double sums[4];
-  const LargeItem& it = a.item[entry_of(a.item, a.count, blockIdx.x, [](const LargeItem& i) { return i.split; })];
-  const unsigned matrix = (blockIdx.x - it.split) / it.tiles, tile = (blockIdx.x - it.split) % it.tiles;
+  const int entry = entry_of(a.split, blockIdx.x);
+  const LargeItem& it = a.item[entry];
+  const unsigned matrix = (blockIdx.x - a.split[entry]) / it.tiles, tile = (blockIdx.x - a.split[entry]) % it.tiles;
   const unsigned wide = (it.cols + 63) / 64, r0 = tile / wide * 64, c0 = tile % wide * 64;
   const size_t size = (size_t)it.rows * it.cols;
-  const double* const part = a.part + it.norm + (size_t)matrix * it.chunks;
+  const double* const part = a.part + a.norm[entry] + (size_t)matrix * it.chunks;
   double s = 0.0;
   for (unsigned i = threadIdx.x; i < it.chunks; i += 256) s += part[i];
   s = wave_sum(s);
@@ -530,8 +576,7 @@ size_t bytes_of(int dtype) { return dtype == CP4_DTYPE_F32 ? 4 : 2; }
 void* ahead(void* p, size_t values, int dtype) { return p ? static_cast<char*>(p) + values * bytes_of(dtype) : nullptr; }
 Outputs outputs_of(const cp4_muon_matrix& x, size_t first) {
   const size_t at = first * x.rows * x.cols;
-  return Outputs{ahead(x.param, at, x.param_dtype), x.param ? ahead(x.copy, at, x.copy_dtype) : nullptr, ahead(x.out, at, x.out_dtype),
-                 x.param_dtype, x.copy_dtype, x.out_dtype};
+  return Outputs{ahead(x.param, at, x.param_dtype), ahead(x.copy, at, x.copy_dtype), x.param_dtype, x.copy_dtype};
 }
 Rates rates_of(const cp4_muon_matrix& x, const Settings& s) {
   return Rates{(float)(1.0 - s.lr * s.weight_decay), (float)(s.lr * std::sqrt(std::max(1.0, (double)x.rows / x.cols)))};
@@ -542,26 +587,34 @@ hipError_t run_small(const cp4_muon_matrix* x, const Group& g, const Settings& s
   size_t matrices = 0;
   for (const Piece& p : g.pieces) matrices += p.count;
   unsigned gram = 0, iterate = 0, apply = 0;
-  for (const Piece& p : g.pieces) {
+  for (int i = 0; i < kSmall; ++i) {
+    a.gram[i] = a.iterate[i] = a.apply[i] = ~0u;
+    if (i >= (int)g.pieces.size()) continue;
+    const Piece& p = g.pieces[i];
     const cp4_muon_matrix& e = x[p.entry];
-    SmallItem& it = a.item[a.count++];
+    SmallItem& it = a.item[i];
     const size_t at = p.first * e.rows * e.cols;
+    const Outputs o = outputs_of(e, p.first);
+    const unsigned tiles = tiles_of(e, g.blocks);
     it.grad = ahead(const_cast<void*>(e.grad), at, e.grad_dtype);
     it.momentum = e.momentum ? e.momentum + at : nullptr;
-    it.o = outputs_of(e, p.first);
-    it.grad_dtype = e.grad_dtype;
-    it.rows = e.rows;
-    it.cols = e.cols;
-    it.tiles = tiles_of(e, g.blocks);
-    it.splits = gram_splits(it.tiles, matrices, g.blocks);
-    it.gram = gram;
-    it.iterate = iterate;
-    it.apply = apply;
-    it.rates = rates_of(e, s);
+    it.param = o.param;
+    it.copy = o.copy;
+    it.param_dtype = (unsigned char)e.param_dtype;
+    it.grad_dtype = (unsigned char)e.grad_dtype;
+    it.copy_dtype = (unsigned char)e.copy_dtype;
+    it.last_row = (unsigned short)(e.rows - 1);
+    it.last_col = (unsigned short)(e.cols - 1);
+    it.splits = (unsigned char)gram_splits(tiles, matrices, g.blocks);
+    a.gram[i] = gram;
+    a.iterate[i] = iterate;
+    a.apply[i] = apply;
     gram += (unsigned)p.count * it.splits;
     iterate += (unsigned)p.count;
-    apply += (unsigned)p.count * it.tiles;
+    apply += (unsigned)p.count * tiles;
   }
+  a.decay = (float)(1.0 - s.lr * s.weight_decay);
+  a.lr = s.lr;
   a.nesterov = s.nesterov;
   a.steps = s.steps;
   a.mu = s.mu;
@@ -602,9 +655,12 @@ hipError_t run_large(const cp4_muon_matrix* x, const Group& g, const Settings& s
   unsigned norm = 0, split = 0;
   struct Buffers { char *x[2], *t[2], *a, *b; };    // X [m][n], transposed [n][m], A and B
   std::vector<Buffers> buffers;
-  for (const Piece& p : g.pieces) {
+  for (unsigned& k : a.norm) k = ~0u;
+  for (unsigned& k : a.split) k = ~0u;
+  for (size_t i = 0; i < g.pieces.size(); ++i) {
+    const Piece& p = g.pieces[i];
     const cp4_muon_matrix& e = x[p.entry];
-    LargeItem& it = a.item[a.count++];
+    LargeItem& it = a.item[i];
     const size_t at = p.first * e.rows * e.cols, m = std::min(e.rows, e.cols), n = std::max(e.rows, e.cols);
     const bool flat = e.rows <= e.cols;
     Buffers b{};
@@ -623,9 +679,9 @@ hipError_t run_large(const cp4_muon_matrix* x, const Group& g, const Settings& s
     it.rows = e.rows;
     it.cols = e.cols;
     it.chunks = (unsigned)(((size_t)e.rows * e.cols + chunk - 1) / chunk);
-    it.norm = norm;
+    a.norm[i] = norm;
     it.tiles = ((e.rows + 63) / 64) * ((e.cols + 63) / 64);
-    it.split = split;
+    a.split[i] = split;
     norm += it.chunks * (unsigned)p.count;
     split += it.tiles * (unsigned)p.count;
   }
@@ -653,20 +709,20 @@ hipError_t run_large(const cp4_muon_matrix* x, const Group& g, const Settings& s
       p.K = p.N;
       p.alpha = (float)kB;
       p.beta = (float)kC;
+      p.diagonal = (float)kA;
       pb.push_back(p);
       p.symmetric = false;
-      p.alpha = (float)kA;
+      p.alpha = p.diagonal = 0.0f;
       p.beta = 1.0f;
+      p.E = nullptr;
       if (k + 1 < s.steps || e.rows <= e.cols) {
         p.N = std::max(e.rows, e.cols);
         p.P = b.b;
         p.Q = Xt;
-        p.E = X;
       } else {                                     // (the parameters lie the other way round)
         p.R = std::max(e.rows, e.cols);
         p.P = Xt;
         p.Q = b.b;
-        p.E = Xt;
       }
       if (k + 1 < s.steps) {
         p.C = b.x[(k + 1) % 2];
@@ -694,11 +750,10 @@ cp4_status check_matrices(const cp4_muon_matrix* x, size_t n) {
     if (e.rows > 65536 || e.cols > 65536) return fail_with(CP4_ERR_SHAPE, "a matrix with a side above 65536");
     if (e.count > (size_t)1 << 24) return fail_with(CP4_ERR_SHAPE, "more than 2^24 matrices in an entry");
     if (!e.grad) return fail_with(CP4_ERR_NULL_POINTER, "a matrix's gradient is NULL");
-    if (!dtype_ok(e.grad_dtype) || (e.param && !dtype_ok(e.param_dtype)) || (e.copy && !dtype_ok(e.copy_dtype)) ||
-        (e.out && !dtype_ok(e.out_dtype)))
+    if (!dtype_ok(e.grad_dtype) || (e.param && !dtype_ok(e.param_dtype)) || (e.copy && !dtype_ok(e.copy_dtype)))
       return fail_with(CP4_ERR_SHAPE, "unknown dtype of a matrix");
     if ((size_t)e.grad % bytes_of(e.grad_dtype) || (size_t)e.momentum % 4 || (e.param && (size_t)e.param % bytes_of(e.param_dtype)) ||
-        (e.copy && (size_t)e.copy % bytes_of(e.copy_dtype)) || (e.out && (size_t)e.out % bytes_of(e.out_dtype)))
+        (e.copy && (size_t)e.copy % bytes_of(e.copy_dtype)))
       return fail_with(CP4_ERR_SHAPE, "a pointer is not aligned to its element type");
   }
   return CP4_OK;

@@ -1379,8 +1379,9 @@ PyObject* muon_step(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
       m.momentum = static_cast<float*>(of_shape(momenta[i], "a momentum is not contiguous or does not match its parameter"));
     }
     if (outs.has(i)) {
-      m.out = of_shape(outs[i], "an output is not contiguous or does not match its matrix");
-      m.out_dtype = dtype_of(outs[i]);
+      require(!m.param && !m.copy, "an output beside a parameter");
+      m.copy = of_shape(outs[i], "an output is not contiguous or does not match its matrix");
+      m.copy_dtype = dtype_of(outs[i]);
     }
     list.push_back(m);
   }

@@ -240,7 +240,7 @@ def _orthogonalize(updates, steps, eps, out, stream):
 
 class Muon(torch.optim.Optimizer):
     """Muon for parameters that are matrices or stacks of them ([..., rows, cols]): factors, adapters, dense
-    layers.  Biases and norms belong to ``AdamW``.  Three launches for up to 24 parameters whose shorter sides round up to
+    layers.  Biases and norms belong to ``AdamW``.  Three launches for up to 72 parameters whose shorter sides round up to
     the same multiple of 16 up to 64, seventeen for up to 16 larger ones.
 
     masters: 16-bit parameters are copies of float32 ones that the optimizer keeps (``True``) or are stepped in their own
