@@ -67,6 +67,10 @@ bool project_sums_planes(const ProjectArgs&, int dtype, bool nn);
 // part: project_part_bytes of scratch memory.
 size_t project_part_bytes(size_t T, int K, int N, int G, int dtype, bool nn, bool four);
 hipError_t project_launch(const ProjectArgs&, float* part, int dtype, bool nn, hipStream_t);
+// W in 4 bits may be cheaper as values in memory: the bytes of scratch memory that takes (0: never for these sizes), and, where it
+// is for these operands, the launch that writes them there; `a` then reads those.
+size_t unpack_bytes(size_t T, int K, int N, int G, int dtype, bool nn);
+hipError_t unpack_launch(ProjectArgs& a, void* room, int dtype, bool nn, hipStream_t st);
 // What project_launch runs: one launch, or one of whole tiles and one of the rows that are left over.
 void project_plan(size_t T, int K, int N, int G, int dtype, bool nn, bool direct, bool four, cp4_adapter_launch (&launches)[2]);
 // The tiles of a projection on the matrix cores, its depth in `splits` parts of `each` steps, whose partial
@@ -94,6 +98,9 @@ hipError_t rows_launch(const ProjectArgs&, const RowsPlan&, float* part, int dty
 // Two sums over the same tokens and adapters, their R, G and splits the same.
 int grad_splits(size_t T, int C0, int C1, int R, int G);
 hipError_t grad_launch(const GradArgs&, const GradArgs&, int dtype, hipStream_t);
+
+// Rows held in 4 bits to values, `ld` apart (mx4.hip).
+hipError_t mx4_unpack(const void* codes, const unsigned char* scales, size_t rows, unsigned K, int dtype, void* out, size_t ld, hipStream_t st);
 
 // ---- device side ------------------------------------------------------------------------
 

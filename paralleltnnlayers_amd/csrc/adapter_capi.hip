@@ -42,7 +42,7 @@ size_t h_bytes(const cp4_adapter_shape& s) { return s.T * padded(s) * 4; }
 
 struct BackwardPlan {
   int splits, dh_planes;
-  size_t part_at, part_b, total;                       // (dh comes first; B's partial sums: floats behind A's)
+  size_t part_at, part_b, w_at, total;                 // (dh comes first; B's partial sums: floats behind A's; W's values last)
 };
 BackwardPlan backward_plan(const cp4_adapter_shape& s, int dtype, bool four) {
   BackwardPlan p{};
@@ -51,7 +51,8 @@ BackwardPlan backward_plan(const cp4_adapter_shape& s, int dtype, bool four) {
   p.part_at = align256(p.dh_planes * h_bytes(s));
   p.part_b = p.splits > 1 ? (size_t)p.splits * s.G * s.R * s.K : 0;
   const size_t parts = p.splits > 1 ? (p.part_b + (size_t)p.splits * s.G * s.R * s.N) * 4 : 0;
-  p.total = p.part_at + align256(std::max(parts, project_part_bytes(s.T, (int)s.N, (int)s.K, (int)s.G, dtype, true, four)));  // (one after the other)
+  p.w_at = p.part_at + align256(std::max(parts, project_part_bytes(s.T, (int)s.N, (int)s.K, (int)s.G, dtype, true, four)));  // (one after the other)
+  p.total = p.w_at + (four ? align256(unpack_bytes(s.T, (int)s.N, (int)s.K, (int)s.G, dtype, true)) : 0);
   return p;
 }
 
@@ -65,7 +66,8 @@ namespace {
 
 size_t forward_bytes(const cp4_adapter_shape* s, int dtype, bool four) {
   if (check_shape(s, dtype) != CP4_OK) return 0;
-  return align256(shrink_planes(s->T, (int)s->K, dtype) * h_bytes(*s)) + align256(project_part_bytes(s->T, (int)s->K, (int)s->N, (int)s->G, dtype, false, four));
+  return align256(shrink_planes(s->T, (int)s->K, dtype) * h_bytes(*s)) + align256(project_part_bytes(s->T, (int)s->K, (int)s->N, (int)s->G, dtype, false, four)) +
+         (four ? align256(unpack_bytes(s->T, (int)s->K, (int)s->N, (int)s->G, dtype, false)) : 0);
 }
 
 // scales: null, or W's in 4 bits.
@@ -94,6 +96,11 @@ cp4_status forward(const cp4_adapter_shape* s, int dtype, const void* x, const v
   p.T = s->T; p.ldz = sh.ldz; p.ldw = scales ? (s->K + 31) / 32 : s->ldw ? s->ldw : s->K; p.scales = scales;
   p.K = (int)s->K; p.N = (int)s->N; p.R = (int)s->R; p.Rp = sh.Rp; p.G = (int)s->G;
   p.fn = (int)s->R; p.fr = 1; p.planes = sh.planes; p.plane = p.T * p.Rp;
+  float* const part = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(sh.planes * h_bytes(*s)));
+  if (scales) {
+    char* const room = reinterpret_cast<char*>(part) + align256(project_part_bytes(p.T, p.K, p.N, p.G, dtype, false, true));
+    if (const hipError_t e = unpack_launch(p, room, dtype, false, st)) return fail_hip(e, "cp4_adapter_mx4_forward");
+  }
   if (p.planes > 1 && project_sums_planes(p, dtype, false)) {
     p.keep = kept;
   } else if (p.planes > 1) {
@@ -102,7 +109,6 @@ cp4_status forward(const cp4_adapter_shape* s, int dtype, const void* x, const v
     p.h = h;
     p.planes = 1;
   }
-  float* const part = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(sh.planes * h_bytes(*s)));
   if (const hipError_t e = project_launch(p, part, dtype, false, st)) return fail_hip(e, "cp4_adapter_forward");
   return CP4_OK;
 }
@@ -181,6 +187,8 @@ cp4_status backward(const cp4_adapter_shape* s, int dtype, const void* dy, const
     p.T = s->T; p.ldz = lddy; p.ldw = scales ? (s->K + 31) / 32 : s->ldw ? s->ldw : s->K; p.scales = scales;
     p.K = (int)s->N; p.N = (int)s->K; p.R = (int)s->R; p.Rp = Rp; p.G = (int)s->G;
     p.fn = 1; p.fr = (int)s->K; p.planes = 1;
+    if (scales)
+      if (const hipError_t e = unpack_launch(p, static_cast<char*>(workspace) + plan.w_at, dtype, true, st)) return fail_hip(e, "cp4_adapter_mx4_backward");
     if (const hipError_t e = project_launch(p, part, dtype, true, st)) return fail_hip(e, "cp4_adapter_backward");
   }
   if (dA) {
@@ -229,13 +237,15 @@ cp4_status linear(size_t T, int K, int N, int dtype, const void* z, size_t ldz, 
   if (!T) return CP4_OK;
   if (!z || !y) return fail_with(CP4_ERR_NULL_POINTER, "an operand is NULL");
   if (const cp4_status rc = check_pointers(value_bytes(dtype), {z, y}, {bias})) return rc;
-  const size_t need = align256(project_part_bytes(T, K, N, 0, dtype, nn, true));
+  const size_t parts = align256(project_part_bytes(T, K, N, 0, dtype, nn, true));
+  const size_t need = parts + align256(unpack_bytes(T, K, N, 0, dtype, nn));
   if (need && (!workspace || workspace_bytes < need || ((size_t)workspace & 255)))
     return fail_with(CP4_ERR_WORKSPACE, "workspace missing, too small or not aligned to 256 bytes");
   ProjectArgs p{};
   p.z = z; p.w = W->codes; p.scales = W->scales; p.bias = bias; p.y = y;
   p.T = T; p.ldz = ldz; p.ldw = blocks;
   p.K = K; p.N = N; p.planes = 1;
+  if (const hipError_t e = unpack_launch(p, static_cast<char*>(workspace) + parts, dtype, nn, static_cast<hipStream_t>(stream))) return fail_hip(e, where);
   if (const hipError_t e = project_launch(p, static_cast<float*>(workspace), dtype, nn, static_cast<hipStream_t>(stream)))
     return fail_hip(e, where);
   return CP4_OK;
@@ -244,7 +254,7 @@ cp4_status linear(size_t T, int K, int N, int dtype, const void* z, size_t ldz, 
 
 extern "C" size_t cp4_mx4_forward_workspace_bytes(size_t T, unsigned K, unsigned N, int dtype) {
   if (check_linear(T, K, N, dtype, 0, 0, nullptr) == CP4_ERR_SHAPE || !T) return 0;
-  return align256(project_part_bytes(T, (int)K, (int)N, 0, dtype, false, true));
+  return align256(project_part_bytes(T, (int)K, (int)N, 0, dtype, false, true)) + align256(unpack_bytes(T, (int)K, (int)N, 0, dtype, false));
 }
 extern "C" cp4_status cp4_mx4_forward(size_t T, unsigned K, unsigned N, int dtype, const void* x, size_t ldx, const cp4_mx4* W,
                                       const float* bias, void* y, void* workspace, size_t workspace_bytes,
@@ -254,7 +264,7 @@ extern "C" cp4_status cp4_mx4_forward(size_t T, unsigned K, unsigned N, int dtyp
 }
 extern "C" size_t cp4_mx4_backward_workspace_bytes(size_t T, unsigned K, unsigned N, int dtype) {
   if (check_linear(T, K, N, dtype, 0, 0, nullptr) == CP4_ERR_SHAPE || !T) return 0;
-  return align256(project_part_bytes(T, (int)N, (int)K, 0, dtype, true, true));
+  return align256(project_part_bytes(T, (int)N, (int)K, 0, dtype, true, true)) + align256(unpack_bytes(T, (int)N, (int)K, 0, dtype, true));
 }
 extern "C" cp4_status cp4_mx4_backward(size_t T, unsigned K, unsigned N, int dtype, const void* dy, size_t lddy, const cp4_mx4* W,
                                        void* dx, void* workspace, size_t workspace_bytes, cp4_stream stream) {

@@ -47,6 +47,42 @@ hipError_t launch(const ProjectArgs& a, float* part, int dtype, bool nn, bool di
 
 }  // namespace
 
+namespace {
+// The operands of a projection with W as values in memory.
+size_t unpacked_row(int cols) { return ((size_t)cols + 7) / 8 * 8; }
+double cost_of(size_t T, int K, int N, int G, int dtype, bool nn, bool direct, bool four) {
+  const size_t main = main_rows(T, K, N, G, dtype, nn, direct, four);
+  double cost = 0.0;
+  for (size_t rows : {main, T - main}) {
+    if (!rows) continue;
+    cost += by_rows(rows, K, N, G, dtype, nn, direct, four) ? rows_plan(rows, K, N, dtype, four).cost
+                                                            : tile_plan(rows, K, N, dtype, nn, direct, four).cost;
+  }
+  return cost;
+}
+// Whether W is unpacked: in 16 bits from some 600 tokens on, where the larger tiles take whole cache lines of W (4096 x 4096:
+// 512 tokens 34 us from codes, 35 through memory; 1024 tokens 50 and 45; 8192 tokens 337 and 195).  fp32 reads codes with three
+// matrix instructions where values take six (8192 tokens 929 us, values 1212).
+bool unpacks(size_t T, int K, int N, int G, int dtype, bool nn) {
+  if (dtype == CP4_DTYPE_F32 || K % 8 || N % 8 || T <= 64) return false;
+  return cost_of(T, K, N, G, dtype, nn, true, false) + 3.0 + (double)K * N * 2.53 / 5.0e6 < cost_of(T, K, N, G, dtype, nn, true, true);
+}
+}  // namespace
+
+size_t unpack_bytes(size_t T, int K, int N, int G, int dtype, bool nn) {
+  return unpacks(T, K, N, G, dtype, nn) ? (size_t)(nn ? K : N) * unpacked_row(nn ? N : K) * 2 : 0;
+}
+hipError_t unpack_launch(ProjectArgs& a, void* room, int dtype, bool nn, hipStream_t st) {
+  if (!a.scales || !tile_direct(a, dtype, nn) || !unpacks(a.T, a.K, a.N, a.G, dtype, nn)) return hipSuccess;
+  const int rows = nn ? a.K : a.N, cols = nn ? a.N : a.K;
+  const size_t ld = unpacked_row(cols);
+  if (const hipError_t e = mx4_unpack(a.w, a.scales, rows, cols, dtype, room, ld, st)) return e;
+  a.w = room;
+  a.ldw = ld;
+  a.scales = nullptr;
+  return hipSuccess;
+}
+
 // Enough for each choice that the operands' alignment makes.
 size_t project_part_bytes(size_t T, int K, int N, int G, int dtype, bool nn, bool four) {
   size_t most = 0;
@@ -55,6 +91,7 @@ size_t project_part_bytes(size_t T, int K, int N, int G, int dtype, bool nn, boo
     if (by_rows(rows, K, N, G, dtype, nn, direct, four)) most = std::max(most, few.splits > 1 ? few.splits * rows * N * 4 : 0);
     else most = std::max(most, tile_part_bytes(tile_plan(rows, K, N, dtype, nn, direct, four), rows, N));
   };
+  if (four && unpacks(T, K, N, G, dtype, nn)) most = project_part_bytes(T, K, N, G, dtype, nn, false);
   for (bool direct : {false, true}) {
     if (direct && dtype == CP4_DTYPE_F32) break;                     // (the same plans)
     const size_t main = main_rows(T, K, N, G, dtype, nn, direct, four);

@@ -120,7 +120,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows_kernel(const RowsArgs ra)
   const ProjectArgs& a = ra.p;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 15, g = lane >> 4;
   const int rows = (int)a.T, n0 = blockIdx.x * 16, split = blockIdx.y;
-  int id = lane < rows && (!Four || a.ids) ? a.ids[lane] : -1;
+  int id = lane < rows && a.ids ? a.ids[lane] : -1;
   if (id < 0 || id >= a.G) id = -1;
   const bool adapters = split == 0 && __ballot(id >= 0);
   const size_t w_row = min(n0 + l, a.N - 1) * a.ldw;

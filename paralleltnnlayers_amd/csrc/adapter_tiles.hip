@@ -106,7 +106,7 @@ __device__ __forceinline__ void expand_tile(const ProjectArgs& a, size_t t0, int
 #pragma unroll
   for (int w = 0; w < WM; ++w) {
     const size_t row = t0 + 64 * w + lane;
-    id[w] = row < a.T && (!kFour || a.ids) ? a.ids[row] : -1;
+    id[w] = row < a.T && a.ids ? a.ids[row] : -1;
     if (id[w] < 0 || id[w] >= a.G) id[w] = -1;
     any |= have[w] = __ballot(id[w] >= 0);
   }
@@ -298,18 +298,22 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
   typedef std::conditional_t<Direct, unsigned, size_t> Offset;       // (bytes)
   Offset zo[kZ], wo[kFour ? 1 : kW];
   int w_count[kFour ? 1 : kW];                                       // values there of a piece of w's row (nn)
-  // w in 4 bits: blocks of 32 values, their codes and scales in registers until put() turns them into values in the LDS
+  // w in 4 bits: blocks of 32 values, their codes and scales in registers for a step until put_four() turns them into values in the
+  // LDS.  (Registers for several steps' gain nothing: 512 tokens of 4096 x 4096 36 us with one step's, 39 with four.  What
+  // bounds w [N][K] is that 64 lanes' blocks lie in 64 rows.)
   constexpr int kBlocks = BN * KS / 32, kC = (kBlocks + kThreads - 1) / kThreads;
   unsigned co[kFour ? kC : 1], at_lds[kFour ? kC : 1];               // a thread's blocks: where, from the step's first one on, ...
   int depth_of[kFour ? kC : 1];                                      // ... whither, and the depth of their first value
   u32x4 codes[kFour ? kC : 1];
   unsigned scale[kFour ? kC : 1];
+  int fetched = 0;
   size_t w_block = NN ? (size_t)k_first * a.ldw + n0 / 32 : (size_t)n0 * a.ldw + k_first / 32;
   const size_t w_blocks = NN ? (size_t)KS * a.ldw : KS / 32;
   if constexpr (kFour) {
 #pragma unroll
     for (int i = 0; i < kC; ++i) {
-      const int at = i * kThreads + threadIdx.x;
+      // (threads beyond the last block read others' again: the waits count the same loads in every wave)
+      const int at = (i * kThreads + threadIdx.x) % kBlocks;
       if constexpr (NN) {
         constexpr int kRow = BN / 32;
         const int block = at % kRow;
@@ -317,9 +321,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
         co[i] = (unsigned)(depth_of[i] * a.ldw) + min(block, (cols - 1) / 32);
         at_lds[i] = BM * RB + (unsigned)(depth_of[i] * BN + 32 * block) * sizeof(Raw);
       } else {
-        const int slot = at % BN, in = slot % (16 * NB), col = slot - in + NB * (in & 15) + in / 16;
-        depth_of[i] = 32 * (at / BN);
-        co[i] = (unsigned)(min(col, cols - 1) * a.ldw) + at / BN;
+        // (a row's blocks of a step side by side: half the lines that 64 lanes touch otherwise)
+        const int slot = at / (KS / 32), block = at % (KS / 32), in = slot % (16 * NB), col = slot - in + NB * (in & 15) + in / 16;
+        depth_of[i] = 32 * block;
+        co[i] = (unsigned)(min(col, cols - 1) * a.ldw) + block;
         at_lds[i] = BM * RB + slot * RB;
       }
     }
@@ -348,21 +353,21 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
   auto advance = [&]() __attribute__((always_inline)) {
     const bool more = ++brought < steps;                             // (beyond the last step that one again)
     zb += more ? RB : 0;
-    if constexpr (kFour) w_block += more ? w_blocks : 0;
-    else wb += more ? w_next : 0;
+    if constexpr (!kFour) wb += more ? w_next : 0;
+  };
+  // the codes of the next step of which none are under way
+  auto fetch = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < (kFour ? kC : 0); ++i) {
+      codes[i] = *reinterpret_cast<const u32x4*>(static_cast<const char*>(a.w) + (w_block + co[i]) * 16);
+      scale[i] = a.scales[w_block + co[i]];
+    }
+    w_block += ++fetched < steps ? w_blocks : 0;
   };
   // Operands on 16-byte boundaries go from memory to the LDS by themselves; others through registers, which put()
   // writes when the step that hid their way is multiplied.
   u32x4 zr[Direct ? 1 : kZ], wr[Direct || kFour ? 1 : kW];
   auto bring = [&](char* lds) __attribute__((always_inline)) {
-    if constexpr (kFour) {
-#pragma unroll
-      for (int i = 0; i < kC; ++i) {
-        if (kBlocks % kThreads && i * kThreads + (int)threadIdx.x >= kBlocks) continue;
-        codes[i] = *reinterpret_cast<const u32x4*>(static_cast<const char*>(a.w) + (w_block + co[i]) * 16);
-        scale[i] = a.scales[w_block + co[i]];
-      }
-    }
     if constexpr (Direct) {
 #pragma unroll
       for (int i = 0; i < kZ; ++i)
@@ -381,22 +386,26 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
     advance();
   };
   auto put_four = [&](char* lds) __attribute__((always_inline)) {
-    if constexpr (kFour) {
 #pragma unroll
-      for (int i = 0; i < kC; ++i) {
-        if (kBlocks % kThreads && i * kThreads + (int)threadIdx.x >= kBlocks) continue;
+    for (int i = 0; i < (kFour ? kC : 0); ++i) {
+      const int at = i * kThreads + threadIdx.x;
+      if (kBlocks % kThreads && at >= kBlocks) continue;
+      // (nn: neighbouring threads' blocks lie 64 bytes apart, and begin with another part each, so that eight are in all banks)
+      const int turn = NN ? at % (BN / 32) >> 1 : 0;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          Raw v[8];
-          mx4::values<T>(codes[i][q], mx4::scale_of(scale[i]), v);
+      for (int q = 0; q < 4; ++q) {
+        const int word = (q + turn) & 3;
+        unsigned c = codes[i][q];
+        if constexpr (NN) c = word & 2 ? (word & 1 ? codes[i][3] : codes[i][2]) : word & 1 ? codes[i][1] : codes[i][0];
+        Raw v[8];
+        mx4::values<T>(c, mx4::scale_of(scale[i]), v);
 #pragma unroll
-          for (int h = 0; h < (int)sizeof(v) / 16; ++h) {
-            const int part = q * ((int)sizeof(v) / 16) + h;          // 16 bytes of the block's
-            char* to = lds + at_lds[i];
-            if constexpr (NN) to += part * 16;
-            else to += piece(depth_of[i] / kVec<T> + part, (i * kThreads + threadIdx.x) % BN) * 16;
-            __builtin_memcpy(__builtin_assume_aligned(to, 16), reinterpret_cast<const char*>(v) + 16 * h, 16);
-          }
+        for (int h = 0; h < (int)sizeof(v) / 16; ++h) {
+          const int part = word * ((int)sizeof(v) / 16) + h;         // 16 bytes of the block's
+          char* to = lds + at_lds[i];
+          if constexpr (NN) to += part * 16;
+          else to += piece(depth_of[i] / kVec<T> + part, at / (KS / 32)) * 16;
+          __builtin_memcpy(__builtin_assume_aligned(to, 16), reinterpret_cast<const char*>(v) + 16 * h, 16);
         }
       }
     }
@@ -408,7 +417,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
 #pragma unroll
       for (int i = 0; i < (kFour ? 0 : kW); ++i) *reinterpret_cast<u32x4*>(lds + BM * RB + (i * kThreads + threadIdx.x) * 16) = wr[i];
     }
-    if constexpr (kFour) put_four(lds);
   };
 
   f32x4 acc[MB][NB] = {};
@@ -513,7 +521,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
   // compiler from counting the loads under way.
   auto step = [&](const char* lds, char* into) __attribute__((always_inline)) {
     asm volatile("" ::: "memory");
-    if constexpr (Direct) __builtin_amdgcn_s_waitcnt(wait_for((Rooms - 2) * (kZ + (kFour ? 0 : kW))));
+    // (w in 4 bits: the codes under way are waited for where they are used, behind the older of these loads)
+    if constexpr (Direct) __builtin_amdgcn_s_waitcnt(wait_for((Rooms - 2) * (kZ + (kFour ? 2 * kC : kW))));
     else __builtin_amdgcn_s_waitcnt(wait_for(63));                   // (the LDS alone)
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -522,8 +531,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
     __builtin_amdgcn_sched_barrier(0);
     multiply(lds);
     put(into);
+    if constexpr (kFour) {
+      put_four(into);
+      fetch();
+    }
   };
-  if constexpr (Direct && !NN && NB == 8 && RB == 128) {
+  if constexpr (Direct && !NN && NB == 8 && RB == 128 && !kFour) {
     // A half step's operands are read while the other half's are multiplied, so that the LDS and the matrix cores
     // work at the same time.  In the middle of a step its room is free - all have read the second half - and
     // the next one's has arrived.  (8192x4096x4096 bf16: 216 us, 243 one after the other.  With w [K][N] the turned
@@ -552,17 +565,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
       products(zc, wc);
       turns();
       __builtin_amdgcn_sched_barrier(0);
-      if constexpr (kFour) put(lds);
     };
     if (steps > 0) {
       bring(lds0);
-      if constexpr (kFour) put(lds0);
       asm volatile("" ::: "memory");                                 // (their order is what the wait counts on)
       __builtin_amdgcn_sched_barrier(0);
       bring(lds1);
-      if constexpr (kFour) put(lds1);
       asm volatile("" ::: "memory");
-      __builtin_amdgcn_s_waitcnt(wait_for(kFour ? 0 : kZ + kW));
+      __builtin_amdgcn_s_waitcnt(wait_for(kZ + kW));
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
       read(lds0, 0, za, wa);
@@ -581,9 +591,22 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
       asm volatile("" ::: "memory");                                 // (their order is what the waits count on)
       __builtin_amdgcn_sched_barrier(0);
     };
+    if constexpr (kFour) fetch();
     ahead(lds0);
     if constexpr (Rooms > 2) ahead(lds1);
     if constexpr (Rooms > 3) ahead(lds2);
+    if constexpr (kFour) {
+      put_four(lds0);
+      fetch();
+      if constexpr (Rooms > 2) {
+        put_four(lds1);
+        fetch();
+      }
+      if constexpr (Rooms > 3) {
+        put_four(lds2);
+        fetch();
+      }
+    }
     int left = steps;                                                // (no way out in the middle: the same reason)
     for (; left >= Rooms; left -= Rooms) {
       if constexpr (Rooms == 2) {
@@ -625,7 +648,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const TileArgs ta
       w_block = NN ? (size_t)(k_last - left) * a.ldw + n0 / 32 : (size_t)n0 * a.ldw + (k_last - left) / 32;
 #pragma unroll
       for (int i = 0; i < kC; ++i) {
-        if (kBlocks % kThreads && i * kThreads + (int)threadIdx.x >= kBlocks) continue;
         const bool there = depth_of[i] < left;
         codes[i] = there ? *reinterpret_cast<const u32x4*>(static_cast<const char*>(a.w) + (w_block + co[i]) * 16) : u32x4{};
         scale[i] = there ? a.scales[w_block + co[i]] : 127u;
@@ -721,10 +743,10 @@ template <class T, bool NN, bool Direct, int MB, int NB, int WM, int WN, int RB,
 void launch(const TileArgs& t, hipStream_t st) {
   tile_kernel<T, NN, Direct, MB, NB, WM, WN, RB, Rooms><<<die_grid((long)t.mt * t.nt * t.splits), 64 * WM * WN, 0, st>>>(t);
 }
-// (fp32: its parts take the registers of 128 columns a wave; through registers: the two smaller shapes)
+// (fp32: its parts take the registers of 128 columns a wave; through registers and w in 4 bits: the two smaller shapes)
 template <class T, bool NN, bool Direct>
 void launch_shape(const TileArgs& t, int which, hipStream_t st) {
-  if constexpr (Direct && !__is_same(T, F32)) {
+  if constexpr (Direct && !__is_same(T, F32) && !kFour) {
     if (which == 0) return launch<T, NN, true, 4, 8, 2, 2, 64, 3>(t, st);
     if (which == 3) return launch<T, NN, true, 4, 8, 4, 2, 128, 2>(t, st);
   }
@@ -772,13 +794,16 @@ void four_launch(const TileArgs& t, int dtype, int which, bool nn, bool direct, 
 TilePlan tile_plan(size_t T, int K, int N, int dtype, bool nn, bool aligned, bool four) {
   static constexpr float k16[2][kShapes][2] = {{{74, 132}, {37, 75}, {51, 69}, {97, 194}}, {{74, 116}, {42, 88}, {55, 76}, {102, 204}}};
   static constexpr float k32[2][kShapes][2] = {{{}, {192, 390}, {218, 340}, {}}, {{}, {190, 376}, {213, 293}, {}}};
+  // (w in 4 bits)
+  static constexpr float k16_four[2][kShapes][2] = {{{}, {48, 90}, {64, 88}, {}}, {{}, {45, 86}, {62, 84}, {}}};
+  static constexpr float k32_four[2][kShapes][2] = {{{}, {134, 230}, {142, 218}, {}}, {{}, {125, 223}, {138, 200}, {}}};
   const long units = num_compute_units();
-  const bool f32 = dtype == CP4_DTYPE_F32, some = f32 || !aligned;
+  const bool f32 = dtype == CP4_DTYPE_F32, some = f32 || !aligned || four;
   TilePlan best{};
   for (int w = some ? 1 : 0; w < (some ? 3 : kShapes); ++w) {
     const int KS = f32 || w == 0 ? 32 : 64, steps = (K + KS - 1) / KS;
     const long tiles = (long)((T + kRows[w] - 1) / kRows[w]) * ((N + kCols[w] - 1) / kCols[w]);
-    const float* const us = f32 ? k32[nn][w] : k16[nn][w];
+    const float* const us = four ? (f32 ? k32_four[nn][w] : k16_four[nn][w]) : f32 ? k32[nn][w] : k16[nn][w];
     for (int s = 1; s <= 64 && s <= std::max(1, steps / 4) && (s == 1 || tiles * s <= 4 * units); s += s < 8 ? 1 : s < 16 ? 2 : s < 32 ? 4 : 8) {
       const int each = (steps + s - 1) / s, parts = (steps + each - 1) / each;
       const long wgs = tiles * parts, most = (wgs + units - 1) / units;

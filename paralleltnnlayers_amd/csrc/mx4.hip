@@ -399,20 +399,27 @@ extern "C" cp4_status cp4_mx4_quantize(size_t T, unsigned K, int dtype, const vo
   return e ? fail_hip(e, "cp4_mx4_quantize") : CP4_OK;
 }
 
+namespace cp4 {
+namespace adapter {
+hipError_t mx4_unpack(const void* codes, const unsigned char* scales, size_t T, unsigned K, int dtype, void* y, size_t ld, hipStream_t st) {
+  return in_slabs(T, K, [&](size_t t, unsigned rows, unsigned blocks, unsigned grid) {
+    const RowsArgs a{static_cast<const char*>(codes) + t * blocks * 16, scales + t * blocks, static_cast<char*>(y) + t * ld * value_bytes(dtype), nullptr,
+                     ld, rows, K, blocks};
+    if (dtype == CP4_DTYPE_F32) dequantize_kernel<F32><<<grid, 256, 0, st>>>(a);
+    else if (dtype == CP4_DTYPE_BF16) dequantize_kernel<BF16><<<grid, 256, 0, st>>>(a);
+    else dequantize_kernel<F16><<<grid, 256, 0, st>>>(a);
+  });
+}
+}  // namespace adapter
+}  // namespace cp4
+
 extern "C" cp4_status cp4_mx4_dequantize(size_t T, unsigned K, int dtype, const cp4_mx4* q, void* y, cp4_stream stream) {
   if (const cp4_status rc = check_rows(T, K, dtype, 0)) return rc;
   if (!T) return CP4_OK;
   if (!q || !y) return fail_with(CP4_ERR_NULL_POINTER, "an operand is NULL");
   if (const cp4_status rc = check_codes(q->codes, q->scales)) return rc;
   if ((size_t)y % value_bytes(dtype)) return fail_with(CP4_ERR_SHAPE, "a pointer is not aligned to its element type");
-  const hipError_t e = in_slabs(T, K, [&](size_t t, unsigned rows, unsigned blocks, unsigned grid) {
-    const RowsArgs a{static_cast<const char*>(q->codes) + t * blocks * 16, q->scales + t * blocks, static_cast<char*>(y) + t * K * value_bytes(dtype), nullptr,
-                     K, rows, K, blocks};
-    const hipStream_t st = static_cast<hipStream_t>(stream);
-    if (dtype == CP4_DTYPE_F32) dequantize_kernel<F32><<<grid, 256, 0, st>>>(a);
-    else if (dtype == CP4_DTYPE_BF16) dequantize_kernel<BF16><<<grid, 256, 0, st>>>(a);
-    else dequantize_kernel<F16><<<grid, 256, 0, st>>>(a);
-  });
+  const hipError_t e = adapter::mx4_unpack(q->codes, q->scales, T, K, dtype, y, K, static_cast<hipStream_t>(stream));
   return e ? fail_hip(e, "cp4_mx4_dequantize") : CP4_OK;
 }
 
