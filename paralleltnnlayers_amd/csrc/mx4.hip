@@ -8,6 +8,12 @@
 // lane, four times bfloat16's rate.  Sums are fp32, products exact.  A tile is fed through the LDS by loads that pass no
 // register; a step is 256 of the depth, 128 bytes of every row; the scales of a step, eight bytes a row, go through a
 // register of one thread a row, since their rows start anywhere.
+//
+// Measured: 4096 x 25088 fp32 to 4 bits 100 us, back 127 (411 MB of values each way, 4.7 and 3.7 TB/s); 8192 x 4096 x 4096 85 us,
+// 3.2 PFLOP/s, bound by the LDS: a step of the 256 x 256 tile reads 240 KB and takes in 68, 2.1 us at the 150 bytes a
+// nanosecond that a compute unit's LDS gives, twice what the matrix cores need.  (Reads of one half of the waves
+// beside the other half's products, 32 x 32 blocks, four steps of 128 under way: 92, 97 and 114 us.  128 x 128 a wave, which reads
+// less, does not fit the registers.)
 #include <algorithm>
 
 #include "adapter.h"
@@ -346,14 +352,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void product_kernel(const ProductA
     }
 }
 
-// Tiles of 256 x 256, 128 x 128 and 32 x 128 and their time a step and compute unit, about (nanoseconds).
+// Tiles of 256 x 256, 128 x 128 and 32 x 128, and the parts of the depth, by the least time of a model of what was measured
+// (microseconds a step of 256 and a launch's ends): 256 x 256 2.2 and 8; 128 x 128 one on a compute unit 0.98 and 4, two 1.72
+// and 3; 32 x 128 0.36 on few units, 0.83 on most of them or with two each, 1.9 with four.
 constexpr int kShapes = 3, kRows[kShapes] = {256, 128, 32}, kCols[kShapes] = {256, 128, 128};
 struct Plan {
   int which, splits, steps;
   double cost;                   // microseconds, about
 };
 Plan plan_of(size_t T, unsigned K, unsigned N) {
-  static constexpr double kStep[kShapes] = {0.95, 0.32, 0.17};
   const int steps = std::max(1, (int)(((K + 31) / 32 + 7) / 8));
   const long units = num_compute_units();
   Plan best{};
@@ -361,9 +368,11 @@ Plan plan_of(size_t T, unsigned K, unsigned N) {
     const long tiles = (long)((T + kRows[w] - 1) / kRows[w]) * ((N + kCols[w] - 1) / kCols[w]);
     for (int s = 1; s <= 32 && (s == 1 || (s <= steps / 2 && tiles * s <= 4 * units)); ++s) {
       const int each = (steps + s - 1) / s, parts = (steps + each - 1) / each;
-      const long rounds = (tiles * parts + units - 1) / units;
-      double cost = 3.0 + rounds * each * kStep[w];
-      if (parts > 1) cost += 5.0 + (double)T * N * (parts + 0.5) * 4.0 / 2.5e6;
+      const long wgs = tiles * parts, once = (wgs + units - 1) / units, twice = (wgs + 2 * units - 1) / (2 * units), fourth = (wgs + 4 * units - 1) / (4 * units);
+      double cost = w == 0 ? once * (2.2 * each + 8.0)
+                    : w == 1 ? (once == 1 ? 0.98 * each + 4.0 : twice * (1.72 * each + 3.0))
+                             : 3.0 + (wgs * 8 <= units ? 0.36 * each : wgs <= 2 * units ? 0.83 * each : fourth * 1.9 * each);
+      if (parts > 1) cost += 4.0 + (double)T * N * (parts + 0.5) * 4.0 / 2.5e6;
       if (!best.splits || cost < best.cost) best = {w, parts, each, cost};
     }
   }
