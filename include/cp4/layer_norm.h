@@ -14,8 +14,8 @@
  * (a row with an infinity or a NaN is NaN in y and dx; weight's gradient is then NaN throughout).
  *
  * All pointers are device pointers.  Rows of x and dy may be further apart than they are long (ldx, lddy, in
- * elements; 0: contiguous); y and dx are contiguous.  Any alignment of the element type runs.  Asynchronous on
- * `stream`, kernel launches only.  D: up to 32768.
+ * elements; 0: contiguous); y and dx are contiguous.  Any alignment of the element type runs.  y may be a contiguous x
+ * itself; otherwise outputs overlap nothing else.  Asynchronous on `stream`, kernel launches only.  D: up to 32768.
  */
 #ifndef CP4_LAYER_NORM_H
 #define CP4_LAYER_NORM_H

@@ -37,9 +37,10 @@ typedef struct cp4_muon_matrix {
 } cp4_muon_matrix;
 
 /* One step.  Asynchronous on `stream`, kernel launches only: three for up to 72 entries whose shorter sides round up to
- * the same multiple of 16 up to 64, and 3 steps + 2 (long ones: 4 steps + 2) for up to 16 larger ones whose scratch memory stays below 1 GiB together (a larger matrix on its
- * own).  steps: 1 to 16.  eps: above 0.  workspace: cp4_muon_workspace_bytes() of device memory, 256-byte aligned, its
- * contents scratch.  Matrices must not overlap one another. */
+ * the same multiple of 16 up to 64, and 3 steps + 2 (long ones: 4 steps + 2) for up to 16 larger ones whose scratch memory
+ * stays below 1 GiB together (a larger matrix on its own).  steps: 1 to 16.  eps: 1e-30 or more.  workspace:
+ * cp4_muon_workspace_bytes() of device memory, 256-byte aligned, its contents scratch.  What is written must not overlap
+ * anything else, but that `copy` without a param may be grad itself, of its type. */
 size_t cp4_muon_workspace_bytes(const cp4_muon_matrix* matrices, size_t count);
 cp4_status cp4_muon_step(const cp4_muon_matrix* matrices, size_t count, double lr, double momentum,
                          int nesterov, double weight_decay, double eps, unsigned steps,

@@ -15,7 +15,8 @@
  * a code times 2^126 or more may be infinite); in float16 values below 2^-14 are rounded to its steps and those of
  * 65536 and more are infinite.  Sums are fp32, outputs are rounded once.
  *
- * All pointers are device pointers, codes on 16-byte boundaries.  Asynchronous on `stream`, kernel launches only.
+ * All pointers are device pointers, codes on 16-byte boundaries; outputs overlap nothing else.  Asynchronous on `stream`,
+ * kernel launches only.  K and N: up to 2^22, T: up to 2^26.
  */
 #ifndef CP4_MX4_H
 #define CP4_MX4_H

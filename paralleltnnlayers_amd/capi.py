@@ -408,8 +408,8 @@ def adapter_plan(T, K, N, R, G, dtype=torch.float32, backward=False, aligned=Tru
 def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, out=None, keep=False, stream=None):
     """y = (x - mean) / sqrt(variance + eps) * weight + bias over x's last dimension (up to 32768 values).
 
-    x [..., D] float32, bfloat16 or float16; weight and bias [D] float32 (None: 1 and 0).  ``keep``: also returns
-    what ``layer_norm_backward`` needs of this pass."""
+    x [..., D] float32, bfloat16 or float16; weight and bias [D] float32 (None: 1 and 0).  ``out`` may be a contiguous x
+    itself.  ``keep``: also returns what ``layer_norm_backward`` needs of this pass."""
     args = (x, weight, bias, eps, out, keep, stream)
     return _native.layer_norm_forward(*args) if stream is None else _ordered(stream, _native.layer_norm_forward, *args)
 

@@ -510,7 +510,7 @@ int large_splits(const cp4_muon_matrix* x, const Group& g, size_t* bytes) {
 
 std::vector<Group> groups_of(const cp4_muon_matrix* x, size_t n) {
   std::vector<Group> out;
-  constexpr size_t kMostWgs = (size_t)1 << 30;     // of a launch
+  constexpr size_t kMostWgs = 1 << 16;             // of a launch: the chip many times over, and up to 36 KB of scratch memory each
   for (int blocks = 1; blocks <= (int)kSide / 16; ++blocks) {
     size_t tiles = 0;
     Group g;
@@ -783,7 +783,8 @@ extern "C" cp4_status cp4_muon_step(const cp4_muon_matrix* x, size_t n, double l
   if (const cp4_status rc = check_matrices(x, n)) return rc;
   if (!(lr >= 0) || !std::isfinite(lr) || !(momentum >= 0 && momentum < 1) || !(weight_decay >= 0) || !std::isfinite(weight_decay))
     return fail_with(CP4_ERR_SHAPE, "lr and weight_decay must be 0 or more, momentum in [0, 1)");
-  if (!(eps > 0) || !std::isfinite(eps)) return fail_with(CP4_ERR_SHAPE, "eps must be above 0");
+  // (what divides by it is held in fp32)
+  if (!(eps >= 1e-30) || !std::isfinite(eps)) return fail_with(CP4_ERR_SHAPE, "eps must be 1e-30 or more");
   if (steps < 1 || steps > 16) return fail_with(CP4_ERR_SHAPE, "1 to 16 steps");
   const std::vector<Group> groups = groups_of(x, n);
   size_t need = 0;

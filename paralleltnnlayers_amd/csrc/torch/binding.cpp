@@ -24,6 +24,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <atomic>
+#include <algorithm>
 #include <optional>
 #include <string>
 #include <vector>
@@ -479,6 +480,19 @@ Tensor rows_of(const Tensor& t, size_t* stride) {
   return t.contiguous();
 }
 
+// The bytes from a tensor's first value to behind its last one, and whether two tensors' overlap.
+std::pair<const char*, const char*> extent(const Tensor& t) {
+  const char* const first = static_cast<const char*>(t.data_ptr());
+  if (!t.numel()) return {first, first};
+  int64_t last = 0;
+  for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+  return {first, first + (last + 1) * t.element_size()};
+}
+bool overlap(const Tensor& a, const Tensor& b) {
+  const auto x = extent(a), y = extent(b);
+  return x.first < y.second && y.first < x.second;
+}
+
 // The weights of a projection [N, K]: a tensor, or microscaled 4-bit floating point (capi.Mx4: codes, scales, K).
 struct Weight {
   Tensor W, scales;                                // (scales undefined: W is the tensor)
@@ -862,6 +876,7 @@ struct LayerNormFunction : torch::autograd::Function<LayerNormFunction> {
     Tensor y = norm_run(p, x.sizes(), (float)eps, Tensor(), &stats,
                         c10::hip::getCurrentHIPStream(x.device().index()).stream());
     ctx->save_for_backward({x, weight ? *weight : Tensor(), stats});
+    ctx->saved_data["bias"] = bias.has_value();
     return y;
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
@@ -872,9 +887,11 @@ struct LayerNormFunction : torch::autograd::Function<LayerNormFunction> {
     const Tensor dy = grad[0].scalar_type() == s[0].scalar_type() ? grad[0] : grad[0].to(s[0].scalar_type());
     const std::optional<Tensor> weight = s[1].defined() ? std::optional<Tensor>(s[1]) : std::nullopt;
     Tensor g[3];
-    norm_run_backward(dy, s[0], weight, s[2], ctx->needs_input_grad(0) ? &g[0] : nullptr,
-                      ctx->needs_input_grad(1) ? &g[1] : nullptr, ctx->needs_input_grad(2) ? &g[2] : nullptr,
-                      c10::hip::getCurrentHIPStream(dy.device().index()).stream());
+    // (needs_input_grad counts the tensors that are there)
+    const bool want_weight = weight && ctx->needs_input_grad(1);
+    const bool want_bias = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(weight ? 2 : 1);
+    norm_run_backward(dy, s[0], weight, s[2], ctx->needs_input_grad(0) ? &g[0] : nullptr, want_weight ? &g[1] : nullptr,
+                      want_bias ? &g[2] : nullptr, c10::hip::getCurrentHIPStream(dy.device().index()).stream());
     for (int i = 0; i < 3; ++i) {
       out[i] = g[i];
       if (g[i].defined() && at::GradMode::is_enabled())            // (create_graph: as adapter_linear's)
@@ -964,6 +981,7 @@ PyObject* mx4_dequantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const std::vector<int64_t> sizes = with_last(q.W.sizes(), q.K);
     if (!y.defined()) y = empty(sizes, type, q.W);
     require(y.is_cuda() && y.device() == q.W.device() && y.is_contiguous() && y.sizes() == at::IntArrayRef(sizes), "out does not match the result");
+    require(!overlap(y, q.W) && !overlap(y, q.scales), "out overlaps the codes");
     const cp4_mx4 m = q.mx4();
     check(cp4_mx4_dequantize((size_t)(q.scales.numel() / q.scales.size(-1)), (unsigned)q.K, dtype_of(y), &m, ptr(y), st));
   }
@@ -988,6 +1006,7 @@ Tensor output(const std::vector<int64_t>& sizes, at::ScalarType type, const Tens
   for (int64_t d : sizes) n *= d;
   require(y.is_cuda() && y.device() == like.device() && y.scalar_type() == type && y.is_contiguous() && y.numel() == n,
           "out does not match the result");
+  require(!overlap(y, like), "out overlaps x");
   return y;
 }
 // x in its own type
@@ -1348,6 +1367,12 @@ PyObject* muon_step(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   require(steps >= 1 && steps <= 16, "1 to 16 steps");
   std::vector<cp4_muon_matrix> list;
   list.reserve(n);
+  struct Place { const char *first, *last; bool written; };
+  std::vector<Place> places;
+  const auto place = [&](const Tensor& t, bool is_written) {
+    const auto e = extent(t);
+    if (e.first != e.second) places.push_back(Place{e.first, e.second, is_written});
+  };
   const Tensor* like = nullptr;
   for (size_t i = 0; i < n; ++i) {
     if (!grads.has(i)) continue;
@@ -1383,7 +1408,18 @@ PyObject* muon_step(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
       m.copy = of_shape(outs[i], "an output is not contiguous or does not match its matrix");
       m.copy_dtype = dtype_of(outs[i]);
     }
+    if (m.copy != m.grad || m.copy_dtype != m.grad_dtype) place(g, false);     // (an output may take its matrix's place)
+    for (const auto* l : {&params, &momenta, &copies, &outs})
+      if (l->has(i)) place((*l)[i], true);
     list.push_back(m);
+  }
+  // (one after the other in memory; of all that came before only the one that reaches furthest matters, and of those written)
+  std::sort(places.begin(), places.end(), [](const Place& a, const Place& b) { return a.first < b.first; });
+  const char *reached = nullptr, *reached_written = nullptr;
+  for (const Place& p : places) {
+    require(p.first >= (p.written ? reached : reached_written), "what is written overlaps another tensor of the step");
+    reached = std::max(reached, p.last);
+    if (p.written) reached_written = std::max(reached_written, p.last);
   }
   if (list.empty()) Py_RETURN_NONE;
   const c10::DeviceGuard guard(like->device());

@@ -213,7 +213,8 @@ def muon_step(params, grads, momenta, *, lr, momentum=0.95, nesterov=True, weigh
     A parameter is [..., rows, cols]: a stack of matrices that are orthogonalised one by one.  grads: one each, of any
     of the three types (None: that parameter is left alone).  momenta: float32 of the same shape, zero before the first step.
     copies: tensors (or None) that receive the new parameters rounded to their type.  A matrix whose momentum is not
-    finite becomes NaN."""
+    finite becomes NaN.  What is written must not overlap another tensor of the call.  A step that is captured into a graph keeps
+    the settings it was captured with."""
     run = capi._native.muon_step
     args = (params, grads, momenta, copies, None, lr, momentum, nesterov, weight_decay, eps, steps, stream)
     return run(*args) if stream is None else capi._ordered(stream, run, *args)
@@ -222,7 +223,7 @@ def muon_step(params, grads, momenta, *, lr, momentum=0.95, nesterov=True, weigh
 def orthogonalize(updates, steps=5, eps=1e-7, out=None, stream=None):
     """The matrices of ``updates`` (a tensor or a list of them, [..., rows, cols] each) with their singular values brought
     to about 1 (0.68 to 1.21) by ``steps`` Newton-Schulz products, each of its own type.  ``out``: where they go, of any of
-    the three types."""
+    the three types (a contiguous matrix itself may be its own)."""
     if isinstance(updates, torch.Tensor):
         return orthogonalize([updates], steps, eps, None if out is None else [out], stream)[0]
     if stream is not None:
@@ -241,7 +242,8 @@ def _orthogonalize(updates, steps, eps, out, stream):
 class Muon(torch.optim.Optimizer):
     """Muon for parameters that are matrices or stacks of them ([..., rows, cols]): factors, adapters, dense
     layers.  Biases and norms belong to ``AdamW``.  Three launches for up to 72 parameters whose shorter sides round up to
-    the same multiple of 16 up to 64, seventeen for up to 16 larger ones.
+    the same multiple of 16 up to 64, 17 (22 where a long depth is taken in parts) for up to 16 larger ones.  A step that is
+    captured into a graph keeps the settings it was captured with.
 
     masters: 16-bit parameters are copies of float32 ones that the optimizer keeps (``True``) or are stepped in their own
     16 bits.  Groups may have settings of their own (lr, momentum, nesterov, weight_decay, steps, eps)."""
@@ -249,8 +251,8 @@ class Muon(torch.optim.Optimizer):
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, eps=1e-7, masters=True):
         if not (lr >= 0 and weight_decay >= 0 and 0 <= momentum < 1):
             raise ValueError("lr and weight_decay must be 0 or more, momentum in [0, 1)")
-        if not eps > 0 or not 1 <= steps <= 16:
-            raise ValueError("eps must be above 0, steps 1 to 16")
+        if not eps >= 1e-30 or not 1 <= steps <= 16:
+            raise ValueError("eps must be 1e-30 or more, steps 1 to 16")
         self.masters = masters
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps, eps=eps))
 

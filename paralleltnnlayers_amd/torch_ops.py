@@ -296,12 +296,13 @@ class AdapterLinearFunction(torch.autograd.Function):
     (csrc/torch/binding.cpp) where a call has to be seen as an operator, in a trace."""
 
     @staticmethod
-    def forward(ctx, x, W, A, B, ids, scale=None, bias=None, scales=None):
-        """``scales``: of W, whose codes are in its place then (an argument each, so that a trace sees both)."""
+    def forward(ctx, x, W, A, B, ids, scale=None, bias=None, scales=None, features=None):
+        """``scales``: of W, whose codes are in its place then (an argument each, so that a trace sees both), of
+        ``features`` values a row."""
         need = ctx.needs_input_grad
-        ctx.codes, ctx.features = scales is not None, A.shape[-1]
+        ctx.codes, ctx.features = scales is not None, features
         if scales is not None:
-            W = capi.Mx4(W, scales, A.shape[-1])
+            W = capi.Mx4(W, scales, features)
         rows = (W.codes if scales is not None else W).shape[:1]
         if need[1] or need[5] or need[6]:
             raise ValueError("the projection, its bias and the scales are not trained: detach them")
@@ -327,7 +328,7 @@ class AdapterLinearFunction(torch.autograd.Function):
         if torch.is_grad_enabled():              # (create_graph: as the native one)
             told = torch._C._functions.DelayedError(b"the gradients of adapter_linear cannot be differentiated again", 1)
             dx, dA, dB = (g if g is None else told(g.detach().requires_grad_()) for g in (dx, dA, dB))
-        return dx, None, dA if need[2] else None, dB if need[3] else None, None, None, None, None
+        return dx, None, dA if need[2] else None, dB if need[3] else None, None, None, None, None, None
 
 
 def adapter_linear(x, W, A, B, ids, scale=None, bias=None):
@@ -340,7 +341,7 @@ def adapter_linear(x, W, A, B, ids, scale=None, bias=None):
     if torch._C._get_tracing_state() is None:
         return capi._native.adapter_linear(x, W, A, B, ids, scale, bias)
     codes, scales = (W.codes, W.scales) if isinstance(W, capi.Mx4) else (W, None)
-    return AdapterLinearFunction.apply(x, codes, A, B, ids, scale, bias, scales)
+    return AdapterLinearFunction.apply(x, codes, A, B, ids, scale, bias, scales, W.features if scales is not None else None)
 
 
 class AdapterLinear(torch.nn.Module):
@@ -352,6 +353,8 @@ class AdapterLinear(torch.nn.Module):
     a trained layer (kept as buffers); without them it starts as a Kaiming-normal one.  ``.to(dtype)``, ``.half()``
     and ``.bfloat16()`` convert the projection and the adapters; scales and bias stay float32.  ``weight_bits=4``: the
     projection is held in microscaled 4-bit floating point (``weight_codes`` and ``weight_scales``, 17 / 32 of a byte a value)."""
+
+    weight_bits = None
 
     def __init__(self, in_features, out_features, rank, adapters=1, alpha=None, weight=None, bias=None,
                  dtype=torch.float32, device="cuda", weight_bits=None):
@@ -386,9 +389,12 @@ class AdapterLinear(torch.nn.Module):
                 self._buffers[k] = old.to(new.device, torch.float32)
         return self
 
+    def projection(self):
+        """The projection as ``capi.adapter_forward`` takes it: ``weight``, or a ``capi.Mx4``."""
+        return self.weight if self.weight_bits is None else capi.Mx4(self.weight_codes, self.weight_scales, self.A.shape[-1])
+
     def forward(self, x, ids):
-        W = self.weight if self.weight_bits is None else capi.Mx4(self.weight_codes, self.weight_scales, self.A.shape[-1])
-        return adapter_linear(x, W, self.A, self.B, ids, self.scale, self.bias)
+        return adapter_linear(x, self.projection(), self.A, self.B, ids, self.scale, self.bias)
 
 
 class Mx4LinearFunction(torch.autograd.Function):
@@ -396,13 +402,13 @@ class Mx4LinearFunction(torch.autograd.Function):
     call has to be seen as an operator, in a trace."""
 
     @staticmethod
-    def forward(ctx, x, codes, scales, bias=None):
+    def forward(ctx, x, codes, scales, bias, features):
         if ctx.needs_input_grad[3]:
             raise ValueError("the projection and its bias are not trained: detach them")
         y = torch.empty(x.shape[:-1] + codes.shape[:1], dtype=x.dtype, device=x.device)   # (made by an operator)
-        capi.mx4_linear(x, capi.Mx4(codes, scales, x.shape[-1]), bias, out=y)
+        capi.mx4_linear(x, capi.Mx4(codes, scales, features), bias, out=y)
         ctx.save_for_backward(codes, scales)
-        ctx.features, ctx.dtype = x.shape[-1], x.dtype
+        ctx.features, ctx.dtype = features, x.dtype
         return y
 
     @staticmethod
@@ -412,7 +418,7 @@ class Mx4LinearFunction(torch.autograd.Function):
         if torch.is_grad_enabled() and dy.requires_grad:             # (create_graph: as the native one)
             told = torch._C._functions.DelayedError(b"the gradients of mx4_linear cannot be differentiated again", 1)
             dx = told(dx.requires_grad_())
-        return dx, None, None, None
+        return dx, None, None, None, None
 
 
 def mx4_linear(x, W, bias=None):
@@ -420,7 +426,7 @@ def mx4_linear(x, W, bias=None):
     in x.  W and bias are frozen: a call that asks for the bias's gradient raises ``ValueError``."""
     if torch._C._get_tracing_state() is None:
         return capi._native.mx4_linear_grad(x, W, bias)
-    return Mx4LinearFunction.apply(x, W.codes, W.scales, bias)
+    return Mx4LinearFunction.apply(x, W.codes, W.scales, bias, W.features)
 
 
 class Mx4Linear(torch.nn.Module):

@@ -178,6 +178,33 @@ def test_python_autograd_function_matches_the_native_one(cp4, wanted):
     assert all(torch.equal(a, b) for a, b in zip(*results))
 
 
+@pytest.mark.parametrize("there", ["", "w", "b", "wb"])
+def test_gradients_of_what_is_there(cp4, there):
+    """The functional form without weight or bias, natively and as a Python function, each input frozen in turn."""
+    from paralleltnnlayers_amd import torch_ops
+    x, dy, w, b = case(11, 70, torch.float32)
+    y, stats = cp4.layer_norm_forward(x, w if "w" in there else None, b if "b" in there else None, keep=True)
+    want = dict(zip("xwb", cp4.layer_norm_backward(dy, x, w if "w" in there else None, stats)))
+    for run in (torch_ops.layer_norm, torch_ops.LayerNormFunction.apply):
+        for frozen in ("", "x", "w", "b"):
+            leaves = {k: t.clone().requires_grad_(k != frozen) for k, t in (("x", x), ("w", w), ("b", b)) if k == "x" or k in there}
+            z = run(leaves["x"], leaves.get("w"), leaves.get("b"), 1e-5)
+            assert torch.equal(z, y)
+            if not z.requires_grad:
+                continue
+            z.backward(dy)
+            for k, t in leaves.items():
+                assert (t.grad is None) == (k == frozen)
+                assert k == frozen or torch.equal(t.grad, want[k])
+
+
+@pytest.mark.parametrize("D", [100, 3000, 9000, 20000])
+def test_in_its_own_place(cp4, D):
+    x, dy, w, b = case(40, D, torch.bfloat16)
+    want = cp4.layer_norm_forward(x, w, b)
+    assert cp4.layer_norm_forward(x, w, b, out=x) is x and torch.equal(x, want)
+
+
 def test_module(cp4):
     from paralleltnnlayers_amd import torch_ops
     m = torch_ops.LayerNorm(64).bfloat16()

@@ -239,3 +239,29 @@ def test_refusals(optim):
         with pytest.raises(ValueError):
             optim.Muon([torch.nn.Parameter(p.clone())], **kw)
     assert torch.equal(p, matrix(8, 16))
+    flat = torch.zeros(200, device="cuda")
+    for call in (lambda: optim.muon_step([p, p], [g, g], [m, torch.zeros_like(m)], lr=0.1),              # the same one twice
+                 lambda: optim.muon_step([p, matrix(8, 16)], [g, g], [m, m], lr=0.1), lambda: optim.muon_step([p], [g], [g], lr=0.1),
+                 lambda: optim.muon_step([p], [p], [m], lr=0.1), lambda: optim.muon_step([p], [g], [m], lr=0.1, copies=[p]),
+                 lambda: optim.orthogonalize([g], out=[g.view(-1)[:0].view(0, 16)]),
+                 lambda: optim.orthogonalize(flat[:128].view(8, 16), out=flat[8:136].view(8, 16)),
+                 lambda: optim.orthogonalize([g, matrix(8, 16)], out=[m, g])):
+        with pytest.raises(AssertionError):
+            call()
+    assert torch.equal(p, matrix(8, 16)) and torch.equal(g, matrix(8, 16, seed=1)) and not m.any()
+
+
+@pytest.mark.parametrize("shape", [(12, 700), (700, 12), (50, 90), (100, 300), (300, 100)], ids=str)
+def test_in_its_own_place(optim, shape):
+    for dtype in DTYPES.values():
+        u = matrix(3, *shape, dtype=dtype)
+        want = optim.orthogonalize(u)
+        assert optim.orthogonalize(u, out=u) is u and torch.equal(u, want)
+
+
+def test_many_small_matrices(optim):
+    """More than one launch takes (each has up to 65536 tiles of its long sides)."""
+    u = torch.randn(70000, 2, 3, generator=torch.Generator().manual_seed(1)).cuda()
+    x = optim.orthogonalize(u)
+    assert off(x, polar(u)) <= allowed(u.dtype)
+    assert torch.equal(optim.orthogonalize(u[65000:].clone()), x[65000:])

@@ -343,6 +343,7 @@ def test_streams_and_graph(cp4):
 def test_refusals(cp4):
     q, _ = weights(cp4, 40, 64, torch.float32)
     x = make(4, 64)
+    both = torch.zeros(256, dtype=torch.uint8, device="cuda")
     bad = [lambda: cp4.mx4_quantize(x.cpu()), lambda: cp4.mx4_quantize(x.double()), lambda: cp4.mx4_quantize(x[:, :0]),
            lambda: cp4.mx4_linear(x[:, :63], q), lambda: cp4.mx4_linear(x.double(), q), lambda: cp4.mx4_linear(x, q, torch.zeros(39, device="cuda")),
            lambda: cp4.mx4_linear(x, cp4.Mx4(q.codes, q.scales, 97)), lambda: cp4.mx4_linear(x, cp4.Mx4(q.codes[:, :31], q.scales, 64)),
@@ -350,10 +351,22 @@ def test_refusals(cp4):
            lambda: cp4.mx4_linear(x, cp4.Mx4(q.codes.int(), q.scales, 64)), lambda: cp4.mx4_linear(x, q.codes), lambda: cp4.mx4_linear(x, q, dtype=torch.float16),
            lambda: cp4.mx4_linear(x, q, out=torch.zeros(4, 39, device="cuda")), lambda: cp4.mx4_linear_backward(x, q),
            lambda: cp4.mx4_dequantize(q, torch.float64), lambda: cp4.mx4_dequantize(q, torch.float32, torch.zeros(40, 63, device="cuda")),
-           lambda: cp4.mx4_linear(cp4.mx4_quantize(make(4, 63)), q)]
+           lambda: cp4.mx4_linear(cp4.mx4_quantize(make(4, 63)), q), lambda: cp4.mx4_linear(x, q, out=x.view(-1)[:160].view(4, 40)),
+           lambda: cp4.mx4_dequantize(cp4.Mx4(both[:32].view(2, 16), both[32:34].view(2, 1), 16), out=both.view(torch.float32)[:32].view(2, 16))]
     for call in bad:
         with pytest.raises(AssertionError):
             call()
     for call in (lambda: cp4.mx4_linear(x, q, activations=8), lambda: __import__("paralleltnnlayers_amd.torch_ops").torch_ops.AdapterLinear(64, 40, 4, weight_bits=8)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_rows_of_another_length_are_refused_in_a_trace(cp4):
+    from paralleltnnlayers_amd import torch_ops
+    q, _ = weights(cp4, 40, 60, torch.float32)
+    A, B, ids = make(1, 4, 64), make(1, 40, 4), torch.zeros(4, dtype=torch.int32, device="cuda")
+    for call in (lambda x: torch_ops.mx4_linear(x, q), lambda x: torch_ops.adapter_linear(x, q, A, B, ids)):
+        with pytest.raises(AssertionError):
+            call(make(4, 64))
+        with pytest.raises(AssertionError):
+            torch.jit.trace(call, (make(4, 64),), check_trace=False)
