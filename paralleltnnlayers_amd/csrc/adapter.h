@@ -93,7 +93,7 @@ struct RowsPlan {
   int splits;
   double cost, adapter;   // microseconds, about, and for each adapter
 };
-RowsPlan rows_plan(size_t T, int K, int N, int dtype, bool four);
+RowsPlan rows_plan(size_t T, int K, int N, int dtype, bool four, bool direct);
 hipError_t rows_launch(const ProjectArgs&, const RowsPlan&, float* part, int dtype, hipStream_t);
 // Two sums over the same tokens and adapters, their R, G and splits the same.
 int grad_splits(size_t T, int C0, int C1, int R, int G);

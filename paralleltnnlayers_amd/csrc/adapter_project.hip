@@ -12,7 +12,7 @@ namespace {
 // (bf16, 4096 x 4096, rank 16, rows kernel and tiles: 20 tokens of 2 adapters 17 us and 21, of 20 adapters 26 and 40; 64 tokens of
 // 2 adapters 26 and 22, of 64 adapters 42 and 55; 4096 x 14336, 20 tokens of 2 adapters 50 and 33.)
 bool by_rows(size_t T, int K, int N, int G, int dtype, bool nn, bool direct, bool four) {
-  const RowsPlan rows = nn ? RowsPlan{} : rows_plan(T, K, N, dtype, four);
+  const RowsPlan rows = nn ? RowsPlan{} : rows_plan(T, K, N, dtype, four, direct);
   if (!rows.splits || T <= 16) return rows.splits;                   // (up to 16 tokens: within 8 % of the tiles at worst)
   const double adapters = (double)std::min<size_t>(T, G);
   return rows.cost + rows.adapter * adapters <=
@@ -28,7 +28,7 @@ size_t main_rows(size_t T, int K, int N, int G, int dtype, bool nn, bool direct,
   for (size_t tile : {256, 128}) {
     const size_t rest = T % tile;
     if (!rest || T <= 2 * tile) continue;
-    const double other = by_rows(rest, K, N, G, dtype, nn, direct, four) ? rows_plan(rest, K, N, dtype, four).cost
+    const double other = by_rows(rest, K, N, G, dtype, nn, direct, four) ? rows_plan(rest, K, N, dtype, four, direct).cost
                                                                    : tile_plan(rest, K, N, dtype, nn, direct, four).cost;
     const double cost = tile_plan(T - rest, K, N, dtype, nn, direct, four).cost + other + 6.0;    // (a launch and its start)
     if (cost < least) {
@@ -41,7 +41,7 @@ size_t main_rows(size_t T, int K, int N, int G, int dtype, bool nn, bool direct,
 
 hipError_t launch(const ProjectArgs& a, float* part, int dtype, bool nn, bool direct, hipStream_t st) {
   const bool four = a.scales;
-  if (by_rows(a.T, a.K, a.N, a.G, dtype, nn, direct, four)) return rows_launch(a, rows_plan(a.T, a.K, a.N, dtype, four), part, dtype, st);
+  if (by_rows(a.T, a.K, a.N, a.G, dtype, nn, direct, four)) return rows_launch(a, rows_plan(a.T, a.K, a.N, dtype, four, direct), part, dtype, st);
   return tile_launch(a, tile_plan(a.T, a.K, a.N, dtype, nn, direct, four), part, dtype, nn, st);
 }
 
@@ -55,7 +55,7 @@ double cost_of(size_t T, int K, int N, int G, int dtype, bool nn, bool direct, b
   double cost = 0.0;
   for (size_t rows : {main, T - main}) {
     if (!rows) continue;
-    cost += by_rows(rows, K, N, G, dtype, nn, direct, four) ? rows_plan(rows, K, N, dtype, four).cost
+    cost += by_rows(rows, K, N, G, dtype, nn, direct, four) ? rows_plan(rows, K, N, dtype, four, direct).cost
                                                             : tile_plan(rows, K, N, dtype, nn, direct, four).cost;
   }
   return cost;
@@ -87,7 +87,7 @@ hipError_t unpack_launch(ProjectArgs& a, void* room, int dtype, bool nn, hipStre
 size_t project_part_bytes(size_t T, int K, int N, int G, int dtype, bool nn, bool four) {
   size_t most = 0;
   const auto part = [&](size_t rows, bool direct) {
-    const RowsPlan few = rows_plan(rows, K, N, dtype, four);
+    const RowsPlan few = rows_plan(rows, K, N, dtype, four, direct);
     if (by_rows(rows, K, N, G, dtype, nn, direct, four)) most = std::max(most, few.splits > 1 ? few.splits * rows * N * 4 : 0);
     else most = std::max(most, tile_part_bytes(tile_plan(rows, K, N, dtype, nn, direct, four), rows, N));
   };
@@ -106,7 +106,7 @@ size_t project_part_bytes(size_t T, int K, int N, int G, int dtype, bool nn, boo
 void project_plan(size_t T, int K, int N, int G, int dtype, bool nn, bool direct, bool four, cp4_adapter_launch (&launches)[2]) {
   const auto one = [&](size_t rows) {
     if (!rows) return cp4_adapter_launch{};
-    if (by_rows(rows, K, N, G, dtype, nn, direct, four)) return cp4_adapter_launch{rows, 0, 0, rows_plan(rows, K, N, dtype, four).splits};
+    if (by_rows(rows, K, N, G, dtype, nn, direct, four)) return cp4_adapter_launch{rows, 0, 0, rows_plan(rows, K, N, dtype, four, direct).splits};
     const TilePlan p = tile_plan(rows, K, N, dtype, nn, direct, four);
     return cp4_adapter_launch{rows, tile_rows(p), tile_cols(p), p.splits};
   };

@@ -9,7 +9,12 @@
 // turns' loads are on their way, and all sums meet in the LDS.
 //
 // W in 4 bits: a turn is 128 inputs, and a lane has one block of 32 of its row of W (16 bytes of codes and a scale), which it
-// turns into values in its registers; it takes the same 32 inputs of its tokens, so that nothing changes places.
+// turns into values in its registers; it takes the same 32 inputs of its tokens.  With W a quarter of its bytes x is what bounds
+// it: a load of the matrix instructions' operand is 16 bytes from each of 16 rows in a quarter of a wave, 16 cache lines looked
+// up one by one, 3.8 us for each 16 tokens of 4096.  So each wave brings its rows of x whole lines at a time into its own part of the
+// LDS and reads them there, without a barrier: 4096 x 4096 bf16 16 tokens 7.2 -> 7.0 us, 32 11.0 -> 8.3, 48 15.0 -> 8.6, 64 10.2 (tiles
+// 16.5); fp32 16 tokens 13.4 -> 9.8, 32 23 -> 15.6.  Rows off 16-byte boundaries, and more of h than the LDS has room for
+// beside them, are read as before.
 //
 // Measured: 16 tokens fp32, 9216 -> 4096: 43 us, 3.5 TB/s; 48 tokens of 32 adapters bf16, 4096 x 4096: 22 us (9 us without
 // adapters and with 16 tokens); one token, 1024 x 1024: 6 us.
@@ -107,16 +112,24 @@ __device__ __forceinline__ void expand_rows(const ProjectArgs& a, int id, const 
   }
 }
 
-template <class T, int MB, bool Four>
+constexpr int kStagedH = 8192;                     // floats of h that the LDS has room for beside the staged rows of x
+constexpr int wait_for(int loads) { return (loads & 15) | (loads >> 4) << 14 | 7 << 4; }
+constexpr int kWaitLds = 15 | 3 << 14 | 7 << 4;
+
+template <class T, int MB, bool Four, bool Staged>
 __global__ __launch_bounds__(64 * kWaves, 2) void rows_kernel(const RowsArgs ra) {
   typedef typename T::raw Raw;
   constexpr int n = 16 / sizeof(Raw), U = Four ? 128 : 128 / sizeof(Raw), kRow = 20;
   // loads of a turn (of a row of x, of W), and how many turns' are under way
   constexpr int kZ = Four ? 32 / n : 2, kW = Four ? 1 : 2, kAhead = !Four ? 4 : kZ * MB > 8 ? 1 : kZ * MB > 4 ? 2 : 4;
   constexpr int kSum = kWaves * 16 * MB * kRow, kH = 16 * MB * 256;
-  __shared__ __attribute__((aligned(16))) float lds[kSum > kH ? kSum : kH];
+  // (staged) bytes of a row of x in a turn and of all rows, loads of a wave for them, turns that the LDS has room for
+  constexpr int kBytes = U * (int)sizeof(Raw), kTurn = 16 * MB * kBytes, kLoads = kTurn / 1024, kRooms = kTurn <= 8192 ? 2 : 1;
+  __shared__ __attribute__((aligned(1024))) char stage0[Staged ? kWaves * kTurn : 16], stage1[Staged && kRooms > 1 ? kWaves * kTurn : 16];
+  __shared__ __attribute__((aligned(16))) float lds[Staged ? (kH < kStagedH ? kH : kStagedH) : kSum > kH ? kSum : kH];
   float* const hl = lds;                                             // [T][Rp], and then ...
-  float* const sum = lds;                                            // ... [kWaves][16 MB][kRow]
+  float* const sum = Staged ? reinterpret_cast<float*>(stage0) : lds;     // ... [kWaves][16 MB][kRow]
+  static_assert(!Staged || kSum * 4 <= kWaves * kTurn, "the sums take the staged rows' place");
   const ProjectArgs& a = ra.p;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 15, g = lane >> 4;
   const int rows = (int)a.T, n0 = blockIdx.x * 16, split = blockIdx.y;
@@ -182,9 +195,57 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows_kernel(const RowsArgs ra)
       }
     }
   };
+  // Staged: a wave brings its own rows of x into its own part of the LDS, so that nobody else is waited for.
+  unsigned zo[Staged ? kLoads : 1];
+  u32x4 code[kRooms];
+  unsigned code_scale[kRooms];
+  if constexpr (Staged) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int at = i * 64 + lane, row = at / (kBytes / 16), piece = at % (kBytes / 16);
+      zo[i] = (unsigned)(min(row, rows - 1) * a.ldz * sizeof(Raw)) + (piece ^ (row & 15)) * 16;
+    }
+  }
+  auto bring = [&](int turn, char* stage, int r) __attribute__((always_inline)) {
+    const int t = min(turn, whole - 1);                              // (beyond the last turn that one again)
+    const char* const from = static_cast<const char*>(a.z) + (size_t)t * kBytes;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + zo[i]),
+                                       (__attribute__((address_space(3))) void*)(stage + wave * kTurn + i * 1024), 16, 0, 0);
+    code[r] = *reinterpret_cast<const u32x4*>(codes + (size_t)t * 64);
+    code_scale[r] = scales[(size_t)t * 4];
+    asm volatile("" ::: "memory");                                   // (their order is what the waits count on)
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto turn = [&](int t, char* stage, int r) __attribute__((always_inline)) {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(wait_for((kRooms - 1) * (kLoads + 2)));
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+      for (int h = 0; h < kZ; ++h)
+        zv[0][i][h] = *reinterpret_cast<const u32x4*>(stage + wave * kTurn + (16 * i + l) * kBytes + ((kZ * g + h) ^ l) * 16);
+    wv[0][0] = code[r];
+    sv[0] = code_scale[r];
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(kWaitLds);                            // (the room has been read)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    bring(t + kRooms, stage, r);
+    multiply(0);
+  };
   // The first turns' loads, h's planes while they are on their way, and then the other turns.
   int u = first;
-  const bool head = u + kAhead <= whole;
+  const bool head = !Staged && u + kAhead <= whole;
+  if constexpr (Staged) {
+    if (u < whole) {
+      bring(u, stage0, 0);
+      if constexpr (kRooms > 1) bring(u + 1, stage1, kRooms - 1);
+    }
+  }
   if (head) {
 #pragma unroll
     for (int e = 0; e < kAhead; ++e) load(u + e, e);
@@ -205,6 +266,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows_kernel(const RowsArgs ra)
       *reinterpret_cast<f32x4*>(hl + i) = x;
       if (a.keep && blockIdx.x == 0) *reinterpret_cast<f32x4*>(a.keep + i) = x;
     }
+  if constexpr (Staged) {
+    if (u < whole) {
+      if constexpr (kRooms > 1) {
+        for (; u + 2 <= whole; u += 2) {
+          turn(u, stage0, 0);
+          turn(u + 1, stage1, 1);
+        }
+        if (u < whole) turn(u++, stage0, 0);
+      } else {
+        for (; u < whole; ++u) turn(u, stage0, 0);
+      }
+      __builtin_amdgcn_s_waitcnt(wait_for(0));                       // (the loads beyond the last turn)
+    }
+  }
   if (head) {
 #pragma unroll
     for (int e = 0; e < kAhead; ++e) multiply(e);
@@ -259,8 +334,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows_kernel(const RowsArgs ra)
 template <class T, int MB>
 void launch(const RowsArgs& r, hipStream_t st) {
   const dim3 grid((r.p.N + 15) / 16, r.splits);
-  if (r.p.scales) rows_kernel<T, MB, true><<<grid, 64 * kWaves, 0, st>>>(r);
-  else rows_kernel<T, MB, false><<<grid, 64 * kWaves, 0, st>>>(r);
+  const ProjectArgs& p = r.p;
+  constexpr size_t e = sizeof(typename T::raw);
+  const bool staged = !((size_t)p.z & 15) && p.ldz * e % 16 == 0 && p.ldz * e * 64 < (size_t)1 << 31 && (!p.ids || p.T * p.Rp <= (size_t)kStagedH);
+  if (!p.scales) rows_kernel<T, MB, false, false><<<grid, 64 * kWaves, 0, st>>>(r);
+  else if (staged) rows_kernel<T, MB, true, true><<<grid, 64 * kWaves, 0, st>>>(r);
+  else rows_kernel<T, MB, true, false><<<grid, 64 * kWaves, 0, st>>>(r);
 }
 template <class T>
 void launch_rows(const RowsArgs& r, hipStream_t st) {
@@ -278,8 +357,8 @@ void launch_rows(const RowsArgs& r, hipStream_t st) {
 // Few columns: the inputs in as many parts as fill the chip with sixteen turns or more each, if that makes four or
 // more (16 tokens, 8192 inputs, 256 outputs: 11.7 us against 20.6 in one part; 1024 x 1024 in four 10.9 against 9.3).
 // The cost is what 4096 inputs took: 6, 10, 14, 17 us for up to 16, 32, 48, 64 tokens (fp32: 14, 24) a round of the chip,
-// and 0.15 us an adapter.
-RowsPlan rows_plan(size_t T, int K, int N, int dtype, bool four) {
+// and 0.15 us an adapter; with W in 4 bits and staged rows 7, 8, 9, 10 (fp32: 10, 15).
+RowsPlan rows_plan(size_t T, int K, int N, int dtype, bool four, bool direct) {
   RowsPlan p{};
   const bool f32 = dtype == CP4_DTYPE_F32;
   if (T > (f32 ? 32 : 64)) return p;
@@ -287,7 +366,7 @@ RowsPlan rows_plan(size_t T, int K, int N, int dtype, bool four) {
   p.splits = std::max(1, std::min(cus / tiles, units / (2 * kWaves)));
   if (p.splits < 4) p.splits = 1;
   const int rounds = (int)(((long)tiles * p.splits + cus - 1) / cus), blocks = (int)(T + 15) / 16;
-  p.cost = 2.0 + rounds * (K / 4096.0 / p.splits) * (f32 ? 5.0 + 9.5 * blocks : 2.5 + 3.7 * blocks) + (p.splits > 1 ? 5.0 : 0.0);
+  p.cost = 2.0 + rounds * (K / 4096.0 / p.splits) * (four && direct ? (f32 ? 2.5 + 5.3 * blocks : 4.0 + 1.1 * blocks) : f32 ? 5.0 + 9.5 * blocks : 2.5 + 3.7 * blocks) + (p.splits > 1 ? 5.0 : 0.0);
   p.adapter = 0.15 * rounds;
   return p;
 }

@@ -9,12 +9,13 @@
 // register; a step is 256 of the depth, 128 bytes of every row; the scales of a step, eight bytes a row, go through a
 // register of one thread a row, since their rows start anywhere.
 //
-// Measured: 4096 x 25088 fp32 to 4 bits 100 us, back 127 (411 MB of values each way, 4.7 and 3.7 TB/s); 8192 x 4096 x 4096 85 us,
+// Measured: 4096 x 25088 fp32 to 4 bits 83 to 100 us, back 64 to 104 (411 MB of values each way); 8192 x 4096 x 4096 85 us,
 // 3.2 PFLOP/s, bound by the LDS: a step of the 256 x 256 tile reads 240 KB and takes in 68, 2.1 us at the 150 bytes a
 // nanosecond that a compute unit's LDS gives, twice what the matrix cores need.  (Reads of one half of the waves
 // beside the other half's products, 32 x 32 blocks, four steps of 128 under way: 92, 97 and 114 us.  128 x 128 a wave, which reads
 // less, does not fit the registers.)
 #include <algorithm>
+#include <type_traits>
 
 #include "adapter.h"
 #include "cp4/mx4.h"
@@ -92,34 +93,55 @@ __global__ __launch_bounds__(256) void quantize_kernel(const RowsArgs a) {
   }
 }
 
-template <class T>
+// 16 bytes of values a store, so that a wave writes whole lines; past the caches what the memory-side one would not hold until
+// somebody reads it: 4096 x 25088 fp32 (411 MB) plain 127 us and 244 with a sum over it behind, streamed 64 to 104 and 207;
+// 4096 x 16384 84 and 152, 44 and 120; but 196 MB of bf16 54 and 80, 51 and 100, 64 MB of fp32 23 and 41, 13 and 44.
+constexpr size_t kStreamFrom = (size_t)224 << 20;  // bytes
+template <class T, bool Streamed>
 __global__ __launch_bounds__(256) void dequantize_kernel(const RowsArgs a) {
   typedef typename T::raw Raw;
-  const unsigned all = a.rows * a.blocks * 4, first = blockIdx.x * (256 * kEach) + threadIdx.x;
-  unsigned codes[kEach], scale[kEach];
+  typedef std::conditional_t<sizeof(Raw) == 4, unsigned short, unsigned> Codes;
+  constexpr int n = 16 / (int)sizeof(Raw), kLanes = 32 / n;          // values of a lane, lanes of a block
+  const unsigned all = a.rows * a.blocks * kLanes, first = blockIdx.x * (256 * kEach * kLanes / 4) + threadIdx.x;
+  constexpr int kTurns = kEach * kLanes / 4;                         // (as many blocks a workgroup for every type)
+  Codes codes[kTurns];
+  unsigned scale[kTurns];
 #pragma unroll
-  for (int e = 0; e < kEach; ++e) {
+  for (int e = 0; e < kTurns; ++e) {
     const unsigned i = first + e * 256;
     if (i >= all) continue;
-    codes[e] = static_cast<const unsigned*>(a.x)[i];
-    scale[e] = a.scales[i / 4];
+    codes[e] = static_cast<const Codes*>(a.x)[i];
+    scale[e] = a.scales[i / kLanes];
   }
 #pragma unroll
-  for (int e = 0; e < kEach; ++e) {
+  for (int e = 0; e < kTurns; ++e) {
     const unsigned i = first + e * 256;
     if (i >= all) continue;
-    const unsigned row = i / 4 / a.blocks, c = (i / 4 % a.blocks) * 32 + i % 4 * 8;
+    const unsigned row = i / kLanes / a.blocks, c = (i / kLanes % a.blocks) * 32 + i % kLanes * n;
     Raw v[8];
-    mx4::values<T>(codes[e], mx4::scale_of(scale[e]), v);
+    mx4::values<T>(codes[e], mx4::scale_of(scale[e]), v);            // (fp32: the last four are not used)
     Raw* const p = static_cast<Raw*>(a.out) + row * a.ld + c;
-    if (c + 8 <= a.K) {
-      __builtin_memcpy(p, v, sizeof(v));
+    if (c + n <= a.K) {
+      if constexpr (Streamed) {
+        typedef u32x4 __attribute__((aligned(2))) Loose;             // (any element's address)
+        u32x4 w;
+        __builtin_memcpy(&w, v, 16);
+        __builtin_nontemporal_store(w, reinterpret_cast<Loose*>(p));
+      } else {
+        __builtin_memcpy(p, v, 16);
+      }
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+      for (int j = 0; j < n; ++j)
         if (c + j < a.K) p[j] = v[j];
     }
   }
+}
+
+template <class T>
+void dequantize_launch(const RowsArgs& a, unsigned grid, bool streamed, hipStream_t st) {
+  if (streamed) dequantize_kernel<T, true><<<grid, 256, 0, st>>>(a);
+  else dequantize_kernel<T, false><<<grid, 256, 0, st>>>(a);
 }
 
 size_t value_bytes(int dtype) { return dtype == CP4_DTYPE_F32 ? 4 : 2; }
@@ -129,7 +151,7 @@ bool dtype_ok(int d) { return d == CP4_DTYPE_F32 || d == CP4_DTYPE_BF16 || d == 
 template <class Launch>
 hipError_t in_slabs(size_t T, unsigned K, Launch launch) {
   const unsigned blocks = (K + 31) / 32;
-  const size_t most = std::max<size_t>(1, ((size_t)1 << 31) / (4 * (size_t)blocks) - 1);
+  const size_t most = std::max<size_t>(1, ((size_t)1 << 31) / (8 * (size_t)blocks) - 1);
   for (size_t t = 0; t < T; t += most) {
     const unsigned rows = (unsigned)std::min(T - t, most);
     launch(t, rows, blocks, (unsigned)(((size_t)rows * blocks * 4 + 256 * kEach - 1) / (256 * kEach)));
@@ -411,12 +433,13 @@ extern "C" cp4_status cp4_mx4_quantize(size_t T, unsigned K, int dtype, const vo
 namespace cp4 {
 namespace adapter {
 hipError_t mx4_unpack(const void* codes, const unsigned char* scales, size_t T, unsigned K, int dtype, void* y, size_t ld, hipStream_t st) {
+  const bool streamed = T * ld * value_bytes(dtype) >= kStreamFrom;
   return in_slabs(T, K, [&](size_t t, unsigned rows, unsigned blocks, unsigned grid) {
     const RowsArgs a{static_cast<const char*>(codes) + t * blocks * 16, scales + t * blocks, static_cast<char*>(y) + t * ld * value_bytes(dtype), nullptr,
                      ld, rows, K, blocks};
-    if (dtype == CP4_DTYPE_F32) dequantize_kernel<F32><<<grid, 256, 0, st>>>(a);
-    else if (dtype == CP4_DTYPE_BF16) dequantize_kernel<BF16><<<grid, 256, 0, st>>>(a);
-    else dequantize_kernel<F16><<<grid, 256, 0, st>>>(a);
+    if (dtype == CP4_DTYPE_F32) dequantize_launch<F32>(a, grid, streamed, st);
+    else if (dtype == CP4_DTYPE_BF16) dequantize_launch<BF16>(a, grid, streamed, st);
+    else dequantize_launch<F16>(a, grid, streamed, st);
   });
 }
 }  // namespace adapter

@@ -182,6 +182,48 @@ def test_both_operands_in_4_bits(cp4, T, K, N, dtype):
     assert torch.equal(y, cp4.mx4_linear(x, q, bias, activations=4))
 
 
+@pytest.mark.parametrize("dtype", list(DTYPES), ids=str)
+@pytest.mark.parametrize("T", [2, 16, 17, 32, 33, 48, 49, 64])
+def test_few_rows(cp4, T, dtype):
+    """Depths from less than a wave's turn to several of each wave, with and without a rest, rows on 16-byte boundaries and off them."""
+    for K, N in ((104, 40), (640, 33), (1024, 300), (3200, 70), (4200, 2000)):
+        q, W = weights(cp4, N, K, DTYPES[dtype])
+        x = make(T, K, dtype=DTYPES[dtype])
+        X = x.double().cpu()
+        for rows in (x, torch.cat([x, x[:, :1]], 1)[:, :K]):
+            close(cp4.mx4_linear(rows, q), X @ W.T, X.abs() @ W.abs().T, DTYPES[dtype], K)
+
+
+@pytest.mark.parametrize("T, ld", [(5, 1 << 29), (40, 1 << 27), (300, 1 << 24)])
+def test_rows_beyond_32_bit_offsets(cp4, T, ld):
+    K, N = 264, 200
+    q, W = weights(cp4, N, K, torch.bfloat16)
+    x, dy = make(T, K, dtype=torch.bfloat16), make(T, N, dtype=torch.bfloat16, seed=3)
+    room = torch.empty((T - 1) * ld + 512, dtype=torch.bfloat16, device="cuda")
+    assert room.numel() * 2 > 1 << 32
+    wide = room.as_strided((T, K), (ld, 1))
+    wide.copy_(x)
+    X, D = x.double().cpu(), dy.double().cpu()
+    close(cp4.mx4_linear(wide, q), X @ W.T, X.abs() @ W.abs().T, torch.bfloat16, K)
+    four, want = cp4.mx4_quantize(wide), cp4.mx4_quantize(x)
+    assert torch.equal(four.codes, want.codes) and torch.equal(four.scales, want.scales)
+    wide = room.as_strided((T, N), (ld, 1))
+    wide.copy_(dy)
+    close(cp4.mx4_linear_backward(wide, q), D @ W, D.abs() @ W.abs(), torch.bfloat16, N)
+
+
+def test_large_results(cp4):
+    """Results that go past the caches are the same ones."""
+    K = (1 << 22) - 3
+    x = make(30, K, dtype=torch.bfloat16)
+    q = cp4.mx4_quantize(x)
+    y = cp4.mx4_dequantize(q, torch.bfloat16)
+    assert y.numel() * 2 >= 224 << 20
+    for t in (0, 13, 29):
+        row = cp4.mx4_quantize(x[t:t + 1])
+        assert torch.equal(q.codes[t:t + 1], row.codes) and torch.equal(y[t:t + 1], cp4.mx4_dequantize(row, torch.bfloat16))
+
+
 def test_large_tiles(cp4):
     """Shapes that every tile has whole ones and edges of."""
     T, K, N = 2100, 1060, 2060
@@ -235,7 +277,7 @@ def test_what_is_not_finite_stays_with_its_row(cp4, T):
 
 @pytest.mark.parametrize("dtype", list(DTYPES), ids=str)
 @pytest.mark.parametrize("T,K,N,R,G", [(1, 64, 48, 4, 2), (7, 1001, 130, 5, 3), (40, 512, 256, 16, 40), (64, 130, 65, 33, 5), (90, 320, 200, 8, 4),
-                                       (300, 1001, 130, 7, 5), (700, 256, 600, 64, 3)])
+                                       (60, 1040, 48, 200, 3), (64, 1040, 48, 100, 6), (30, 2048, 300, 256, 2), (300, 1001, 130, 7, 5), (700, 256, 600, 64, 3)])
 def test_adapters(cp4, T, K, N, R, G, dtype):
     """The adapters beside a projection in 4 bits are those beside one of its values."""
     t = DTYPES[dtype]
