@@ -7,7 +7,7 @@
 //   gram      updates the momentum, adds up G over the long side - fp64 on the matrix cores: G squares u's singular
 //             values, and a small one would drown in fp32's roundings of the largest -, split over workgroups;
 //   iterate   one workgroup a matrix: adds up the splits, |u|^2 is G's trace, then A <- A p(A)^2 and Q <- Q p(A) in
-//             fp64 in the LDS, all of them symmetric, blocks on and below the diagonal alone;
+//             fp64 in the LDS (up to 16: in registers), all of them symmetric, blocks on and below the diagonal alone;
 //   apply     X = Q u in fp32 and the parameters' step.
 //
 // So the step is bound by memory where matrices are long (12 bytes a value in gram, 16 in apply) and by the
@@ -171,88 +171,124 @@ __device__ __forceinline__ double wave_sum(double x) {
   return x;
 }
 
-// out = f(row, column, sum) of X Y, symmetric all three, [M][S] in the LDS.  What is above the diagonal is what is below it to the
+// A matrix of the iteration in the LDS: [MB][MB] blocks of 16 x 16, their rows 17 apart (a column is in all banks).  An fp64 product's
+// result holds, at a lane's place v, row lane / 16 + 4 v and column lane % 16, which is also what its operands want there, the
+// first one turned.  So X^T Y, which is X Y for a symmetric X, reads whole blocks in order.
+constexpr int kRowOf = 17, kBlockOf = 16 * kRowOf;
+template <int MB>
+__device__ __forceinline__ void block_at(int k, int& i, int& j) {  // the k-th on or below the diagonal
+  int first = 0;
+  i = 0;
+  while (first + i + 1 <= k) first += ++i;
+  j = k - first;
+}
+// Such a block of X Y.
+template <int MB>
+__device__ __forceinline__ f64x4 block_product(const double* X, const double* Y, int k) {
+  const int lane = threadIdx.x & 63;
+  int i, j;
+  block_at<MB>(k, i, j);
+  const int at = (lane >> 4) * kRowOf + (lane & 15);
+  f64x4 acc = {};
+#pragma unroll
+  for (int b = 0; b < MB; ++b) {
+    const double *const x = X + (b * MB + i) * kBlockOf + at, *const y = Y + (b * MB + j) * kBlockOf + at;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) acc = __builtin_amdgcn_mfma_f64_16x16x4f64(x[4 * kRowOf * s], y[4 * kRowOf * s], acc, 0, 0, 0);
+  }
+  return acc;
+}
+// f(element of the matrix, sum, whether on the diagonal) of such a block into out.  What is above the diagonal is what is below it to the
 // last bit: what differs would grow nine-fold with each step.
 template <int MB, class Fn>
-__device__ __forceinline__ void multiply(const double* X, const double* Y, double* out, Fn f) {
-  constexpr int M = 16 * MB, S = M + 4;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
-#pragma unroll 1
-  for (int k = wave; k < Tile<MB>::kBlocks; k += 4) {
-    int i = 0, first = 0;
-    while (first + i + 1 <= k) first += ++i;
-    const int j = k - first;
-    f64x4 acc = {};
+__device__ __forceinline__ void put_block(const f64x4& x, double* out, int k, Fn f) {
+  const int lane = threadIdx.x & 63, l = lane & 15, g = lane >> 4;
+  int i, j;
+  block_at<MB>(k, i, j);
 #pragma unroll
-    for (int s = 0; s < M / 4; ++s)
-      acc = __builtin_amdgcn_mfma_f64_16x16x4f64(X[(16 * i + l) * S + 4 * s + g], Y[(16 * j + l) * S + 4 * s + g], acc, 0, 0, 0);
-#pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      const int r = 16 * i + g + 4 * v, c = 16 * j + l;
-      if (r < c) continue;
-      const double x = f(r, c, acc[v]);
-      out[r * S + c] = x;
-      out[c * S + r] = x;
-    }
+  for (int v = 0; v < 4; ++v) {
+    const int r = g + 4 * v, at = (i * MB + j) * kBlockOf + r * kRowOf + l;
+    if (i == j && r < l) continue;
+    const double y = f(at, x[v], i == j && r == l);
+    out[at] = y;
+    out[(j * MB + i) * kBlockOf + l * kRowOf + r] = y;
   }
-  __syncthreads();
 }
 
+// Three products one after the other a step: P, then A P and Q P beside each other, then (A P) P; each stays in its wave's registers
+// until all have read what it takes the place of.  A wave a block: a side of 64 41 us, of 48 24, of 32 15 (four waves, whole
+// matrices and A P behind Q P: 76, 39 and 16).  Of a side of 64 21 us are the matrix core's with most to do, 65 cycles a product.
+constexpr int iterate_waves(int MB) { return MB == 2 ? 8 : 16; }
 template <int MB>
-__global__ __launch_bounds__(256) void iterate_kernel(const SmallArgs a) {
+__global__ __launch_bounds__(64 * iterate_waves(MB)) void iterate_kernel(const SmallArgs a) {
   typedef Tile<MB> T;
-  constexpr int M = T::M, S = M + 4;
-  __shared__ double lds[4][M * S];
-  double *const A = lds[0], *const P = lds[1], *Q = lds[2], *R = lds[3];
-  const int entry = entry_of(a.iterate, blockIdx.x);
+  constexpr int M = T::M, W = iterate_waves(MB), kThreads = 64 * W, B = T::kBlocks, kUnits = (2 * B + W - 1) / W, kAll = MB * MB * kBlockOf;
+  static_assert(B <= W, "a wave a block");
+  __shared__ double A[kAll], P[kAll], Q[kAll];
+  const int entry = entry_of(a.iterate, blockIdx.x), wave = threadIdx.x >> 6;
   const unsigned splits = a.item[entry].splits;
-  const double* const part = a.part + (a.gram[entry] + (size_t)(blockIdx.x - a.iterate[entry]) * splits) * (T::kBlocks * 256);
-  for (int e = threadIdx.x; e < T::kBlocks * 256; e += 256) {
+  const double* const part = a.part + (a.gram[entry] + (size_t)(blockIdx.x - a.iterate[entry]) * splits) * (B * 256);
+  for (int e = threadIdx.x; e < B * 256; e += kThreads) {
     double x = 0.0;
     unsigned s = 0;
     for (; s + 8 <= splits; s += 8) {
       double y[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) y[k] = part[(size_t)(s + k) * (T::kBlocks * 256) + e];
+      for (int k = 0; k < 8; ++k) y[k] = part[(size_t)(s + k) * (B * 256) + e];
 #pragma unroll
       for (int k = 0; k < 8; ++k) x += y[k];
     }
-    for (; s < splits; ++s) x += part[(size_t)s * (T::kBlocks * 256) + e];
-    int i = 0, first = 0;
-    while (first + i + 1 <= e / 256) first += ++i;
-    const int r = 16 * i + e % 256 / 16, c = 16 * (e / 256 - first) + e % 16;
-    if (r < c) continue;
-    A[r * S + c] = x;
-    A[c * S + r] = x;
+    for (; s < splits; ++s) x += part[(size_t)s * (B * 256) + e];
+    int i, j;
+    block_at<MB>(e / 256, i, j);
+    const int r = e % 256 / 16, c = e % 16;
+    if (i == j && r < c) continue;
+    A[(i * MB + j) * kBlockOf + r * kRowOf + c] = x;
+    A[(j * MB + i) * kBlockOf + c * kRowOf + r] = x;
   }
   __syncthreads();
   const int lane = threadIdx.x & 63;
-  const double square = wave_sum(lane < M ? A[lane * S + lane] : 0.0);
+  const double square = wave_sum(lane < M ? A[lane / 16 * (MB + 1) * kBlockOf + lane % 16 * (kRowOf + 1)] : 0.0);
   const double over = square < INFINITY ? 1.0 / (sqrt(square) + a.eps) : (double)NAN;
   __syncthreads();
-  for (int e = threadIdx.x; e < M * S; e += 256)
-    if (e % S < M) A[e] = A[e] * over * over;
+  for (int e = threadIdx.x; e < kAll; e += kThreads)
+    if (e % kRowOf < 16) A[e] = A[e] * over * over;
   __syncthreads();
+  const auto plain = [](int, double x, bool) { return x; };
   for (int s = 0; s < a.steps; ++s) {
-    // P = a + b A + c A A
-    multiply<MB>(A, A, P, [&](int r, int c, double x) { return kC * x + kB * A[r * S + c] + (r == c ? kA : 0.0); });
-    const auto plain = [](int, int, double x) { return x; };
-    if (s == 0) {
-      for (int e = threadIdx.x; e < M * S; e += 256)
-        if (e % S < M) Q[e] = P[e];
-    } else {
-      multiply<MB>(Q, P, R, plain);
-      double* const t = Q;
-      Q = R;
-      R = t;
+    if (wave < B)
+      put_block<MB>(block_product<MB>(A, A, wave), P, wave, [&](int at, double x, bool diagonal) { return kC * x + kB * A[at] + (diagonal ? kA : 0.0); });
+    __syncthreads();
+    // (the first step's Q is P itself; the last step needs no A)
+    const bool last = s + 1 == a.steps;
+    const int from = s ? 0 : B, to = last ? B : 2 * B;
+    f64x4 x[kUnits];
+#pragma unroll
+    for (int e = 0; e < kUnits; ++e) {
+      const int k = from + wave + e * W;
+      if (k < to) x[e] = block_product<MB>(k < B ? Q : A, P, k < B ? k : k - B);
     }
-    if (s + 1 == a.steps) break;
-    multiply<MB>(A, P, R, plain);
-    multiply<MB>(R, P, A, plain);
+    __syncthreads();
+    if (s == 0)
+      for (int e = threadIdx.x; e < kAll; e += kThreads)
+        if (e % kRowOf < 16) Q[e] = P[e];
+#pragma unroll
+    for (int e = 0; e < kUnits; ++e) {
+      const int k = from + wave + e * W;
+      if (k < to) put_block<MB>(x[e], k < B ? Q : A, k < B ? k : k - B, plain);
+    }
+    __syncthreads();
+    if (last) break;
+    if (wave < B) x[0] = block_product<MB>(A, P, wave);
+    __syncthreads();
+    if (wave < B) put_block<MB>(x[0], A, wave, plain);
+    __syncthreads();
   }
-  __syncthreads();
   float* const q = a.q + (size_t)blockIdx.x * (M * M);
-  for (int e = threadIdx.x; e < M * M; e += 256) q[e] = (float)(Q[e / M * S + e % M] * over);
+  for (int e = threadIdx.x; e < M * M; e += kThreads) {
+    const int r = e / M, c = e % M;
+    q[e] = (float)(Q[(r / 16 * MB + c / 16) * kBlockOf + r % 16 * kRowOf + c % 16] * over);
+  }
 }
 
 // A short side of up to 16: one wave does it in its registers.  An fp64 product's result holds, at a lane's place v, row
@@ -359,7 +395,7 @@ template <int MB>
 hipError_t small_launch(const SmallArgs& a, unsigned gram, unsigned iterate, unsigned apply, hipStream_t st) {
   gram_kernel<MB><<<gram, 256, 0, st>>>(a);
   if constexpr (MB == 1) iterate_16_kernel<<<iterate, 256, 0, st>>>(a);
-  else iterate_kernel<MB><<<iterate, 256, 0, st>>>(a);
+  else iterate_kernel<MB><<<iterate, 64 * iterate_waves(MB), 0, st>>>(a);
   apply_kernel<MB><<<apply, 256, 0, st>>>(a);
   return hipGetLastError();
 }
