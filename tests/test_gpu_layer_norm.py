@@ -198,6 +198,21 @@ def test_gradients_of_what_is_there(cp4, there):
                 assert k == frozen or torch.equal(t.grad, want[k])
 
 
+@pytest.mark.parametrize("T, D, ld", [(5, 333, 1 << 29), (40, 5000, 1 << 27), (300, 20000, 1 << 24)])
+def test_rows_beyond_32_bit_offsets(cp4, T, D, ld):
+    x, dy, w, b = case(T, D, torch.bfloat16)
+    y, stats = cp4.layer_norm_forward(x, w, b, keep=True)
+    want = (y,) + cp4.layer_norm_backward(dy, x, w, stats)
+    room = torch.empty((T - 1) * ld + 2 * D, dtype=torch.bfloat16, device="cuda")
+    assert room.numel() * 2 > 1 << 32
+    wx, wdy = room.as_strided((T, D), (ld, 1)), room.as_strided((T, D), (ld, 1), D)
+    wx.copy_(x)
+    wdy.copy_(dy)
+    y, stats = cp4.layer_norm_forward(wx, w, b, keep=True)
+    got = (y,) + cp4.layer_norm_backward(wdy, wx, w, stats)
+    assert all(torch.equal(g, v) for g, v in zip(got, want))
+
+
 @pytest.mark.parametrize("D", [100, 3000, 9000, 20000])
 def test_in_its_own_place(cp4, D):
     x, dy, w, b = case(40, D, torch.bfloat16)

@@ -265,3 +265,15 @@ def test_many_small_matrices(optim):
     x = optim.orthogonalize(u)
     assert off(x, polar(u)) <= allowed(u.dtype)
     assert torch.equal(optim.orthogonalize(u[65000:].clone()), x[65000:])
+
+
+@pytest.mark.parametrize("shape", [(520, 64, 65536), (260, 65, 65536)], ids=str)
+def test_stacks_beyond_32_bit_offsets(optim, shape):
+    u = torch.zeros(shape, device="cuda")
+    assert u.numel() * 4 > 1 << 32
+    last = matrix(*shape[1:], seed=3)
+    u[-1] = last
+    u[0] = matrix(*shape[1:], seed=4)
+    x = optim.orthogonalize(u, out=u)
+    assert x is u and not u[1:-1].any()
+    assert off(u[-1], polar(last)) <= allowed(u.dtype)

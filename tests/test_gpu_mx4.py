@@ -212,6 +212,35 @@ def test_rows_beyond_32_bit_offsets(cp4, T, ld):
     close(cp4.mx4_linear_backward(wide, q), D @ W, D.abs() @ W.abs(), torch.bfloat16, N)
 
 
+def test_codes_beyond_32_bit_offsets(cp4):
+    """W of more than 4 GiB of codes, read by the kernels of few and of many rows, as values and as codes, both ways.  x has 16 values a
+    row, so that sums are short; of dx some columns are looked at."""
+    K, N = 1 << 22, 2100
+    W = torch.empty(N, K, dtype=torch.bfloat16, device="cuda")
+    for n in range(0, N, 300):
+        W[n:n + 300].normal_(generator=torch.Generator("cuda").manual_seed(n))
+    q = cp4.mx4_quantize(W)
+    assert q.codes.numel() > 1 << 32
+    cp4.mx4_dequantize(q, torch.bfloat16, out=W)
+    at = torch.tensor([0, 1, 33, 4095, K // 2 + 5, K - 64, K - 2, K - 1] + [K // 9 * k for k in range(1, 9)])
+    V = W[:, at.cuda()].double().cpu()
+    for n in (0, 1023, N - 1):
+        assert same(W[n], cp4.mx4_dequantize(cp4.Mx4(q.codes[n:n + 1], q.scales[n:n + 1], K), torch.bfloat16)[0])
+    del W
+    for T in (3, 60, 100):
+        x = torch.zeros(T, K, dtype=torch.bfloat16, device="cuda")
+        X = make(T, 16, dtype=torch.bfloat16, seed=T)
+        x[:, at.cuda()] = X
+        X = X.double().cpu()
+        close(cp4.mx4_linear(x, q), X @ V.T, X.abs() @ V.abs().T, torch.bfloat16, 16)
+        four = cp4.mx4_quantize(x)
+        R = cp4.mx4_dequantize(four, torch.bfloat16)[:, at.cuda()].double().cpu()
+        close(cp4.mx4_linear(four, q, dtype=torch.bfloat16), R @ V.T, R.abs() @ V.abs().T, torch.bfloat16, 16)
+        dy = make(T, N, dtype=torch.bfloat16, seed=T + 1)
+        D = dy.double().cpu()
+        close(cp4.mx4_linear_backward(dy, q)[:, at.cuda()], D @ V, D.abs() @ V.abs(), torch.bfloat16, N)
+
+
 def test_large_results(cp4):
     """Results that go past the caches are the same ones."""
     K = (1 << 22) - 3
