@@ -20,6 +20,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -691,6 +692,24 @@ PyObject* adapter_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// In a backward pass that is captured into a graph: a leaf whose gradient torch would add up on the default stream, since an
+// eager graph that uses the leaf still lives, would pull that stream into the capture, which ends the process.
+void check_captured_leaves(const Tensor& grad) {
+  const auto current = c10::hip::getCurrentHIPStream(grad.device().index());
+  const auto none = c10::hip::getDefaultHIPStream(grad.device().index());
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (current == none || hipStreamIsCapturing(current.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+  const std::shared_ptr<torch::autograd::Node> node = torch::autograd::get_current_node();
+  if (!node) return;
+  for (size_t i = 0; i < node->num_outputs(); ++i) {
+    const auto& next = node->next_edge(i).function;
+    if (!next || !node->task_should_compute_output(i) || !dynamic_cast<torch::autograd::AccumulateGrad*>(next.get())) continue;
+    const auto stream = next->stream();                              // (on a device of type cuda, where HIP's own are of type hip)
+    TORCH_CHECK(!stream || stream->id() != none.id(),
+                "a backward pass is being captured while an eager graph of the same leaves lives: drop what was computed from them first");
+  }
+}
+
 struct AdapterFunction : torch::autograd::Function<AdapterFunction> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& W, const Tensor& A,
                         const Tensor& B, const Tensor& ids, const std::optional<Tensor>& scale,
@@ -708,6 +727,7 @@ struct AdapterFunction : torch::autograd::Function<AdapterFunction> {
     const auto s = ctx->get_saved_variables();
     torch::autograd::variable_list out(9);
     if (!grad[0].defined()) return out;
+    check_captured_leaves(grad[0]);
     Tensor dy = grad[0];
     if (dy.scalar_type() != s[2].scalar_type()) dy = dy.to(s[2].scalar_type());
     const bool want_dx = ctx->needs_input_grad(0), want = ctx->needs_input_grad(2) || ctx->needs_input_grad(3);
@@ -884,6 +904,7 @@ struct LayerNormFunction : torch::autograd::Function<LayerNormFunction> {
     const auto s = ctx->get_saved_variables();
     torch::autograd::variable_list out(4);
     if (!grad[0].defined()) return out;
+    check_captured_leaves(grad[0]);
     const Tensor dy = grad[0].scalar_type() == s[0].scalar_type() ? grad[0] : grad[0].to(s[0].scalar_type());
     const std::optional<Tensor> weight = s[1].defined() ? std::optional<Tensor>(s[1]) : std::nullopt;
     Tensor g[3];
@@ -1119,6 +1140,7 @@ struct Mx4LinearFunction : torch::autograd::Function<Mx4LinearFunction> {
     const auto s = ctx->get_saved_variables();
     torch::autograd::variable_list out(5);
     if (!grad[0].defined()) return out;
+    check_captured_leaves(grad[0]);
     const auto type = (at::ScalarType)ctx->saved_data["type"].toInt();
     const Tensor dy = grad[0].scalar_type() == type ? grad[0] : grad[0].to(type);
     const Weight w{s[0], s[1], ctx->saved_data["K"].toInt()};

@@ -126,6 +126,32 @@ def test_training_in_a_graph(cp4, dtype):
             assert torch.equal(a, b)
 
 
+def test_backward_pass_in_a_graph(cp4):
+    """Captured while an eager graph of the same leaves lives: refused.  Without one: replayed."""
+    from paralleltnnlayers_amd import torch_ops
+    net, linear = Net(torch.bfloat16), torch_ops.Mx4Linear(torch.randn(64, D))
+    x, dy, ids = batch(torch.bfloat16)
+    leaf = x.clone().requires_grad_()
+    for run, most in ((lambda: net.norm(leaf), dy[:, :1]), (lambda: net.head(leaf, ids), dy[:, :1]), (lambda: linear(leaf), dy[:, :1])):
+        eager = run()
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="eager graph"):
+            with torch.cuda.graph(graph):
+                torch.autograd.grad(run(), [leaf], most.expand(-1, eager.shape[-1]).contiguous())
+        del eager, graph
+    torch.cuda.synchronize()
+    (want,) = torch.autograd.grad(net(leaf, ids), [leaf], dy)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (got,) = torch.autograd.grad(net(leaf, ids), [leaf], dy)
+    for scale in (1.0, 0.5, 2.0):
+        dy.mul_(scale)
+        graph.replay()
+        (want,) = torch.autograd.grad(net(leaf, ids), [leaf], dy)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
 def test_example_runs_with_all_of_them(cp4):
     import importlib.util
     import math
