@@ -49,6 +49,13 @@ size_t cp4_mx4_backward_workspace_bytes(size_t T, unsigned K, unsigned N, int dt
 cp4_status cp4_mx4_backward(size_t T, unsigned K, unsigned N, int dtype, const void* dy, size_t lddy, const cp4_mx4* W,
                             void* dx, void* workspace, size_t workspace_bytes, cp4_stream stream);
 
+/* How the projection of a call with W in 4 bits (backward != 0: that of dx) would run now, for reports and tests, as
+ * cp4_adapter_plan_query has it.  G: adapters beside it, 0: none.  aligned: whether rows of x (dy) start on 16-byte
+ * boundaries.  room: the bytes of its workspace for the partial sums of a split depth, and for W's values where aligned
+ * calls read those instead of its codes (0: they do not). */
+cp4_status cp4_mx4_plan_query(size_t T, unsigned K, unsigned N, unsigned G, int dtype, int backward, int aligned,
+                              cp4_adapter_launch launches[2], size_t room[2]);
+
 /* y [T][N] = X W^T + bias, both operands in 4 bits, on the scaled matrix instructions; y of dtype.  (cp4_mx4_quantize
  * makes X of activations.) */
 size_t cp4_mx4_product_workspace_bytes(size_t T, unsigned K, unsigned N);

@@ -405,6 +405,16 @@ def adapter_plan(T, K, N, R, G, dtype=torch.float32, backward=False, aligned=Tru
     return [(o.rows, (o.tile_rows, o.tile_cols) if o.tile_rows else None, o.splits) for o in out if o.rows]
 
 
+def mx4_plan(T, K, N, G=0, dtype=torch.float32, backward=False, aligned=True):
+    """The launches that ``mx4_linear`` (``backward``: ``mx4_linear_backward``) would run with now, beside ``G`` adapters those of
+    ``adapter_forward``, as ``adapter_plan`` has them; and the bytes of the workspace for the partial sums of a split depth and for W's
+    values where aligned calls read those (0: they read its codes)."""
+    out, room = (AdapterLaunch * 2)(), (ctypes.c_size_t * 2)()
+    check(lib().cp4_mx4_plan_query(ctypes.c_size_t(T), ctypes.c_uint(K), ctypes.c_uint(N), ctypes.c_uint(G), _DTYPES[dtype], int(backward),
+                                   int(aligned), out, room))
+    return [(o.rows, (o.tile_rows, o.tile_cols) if o.tile_rows else None, o.splits) for o in out if o.rows], tuple(room)
+
+
 def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, out=None, keep=False, stream=None):
     """y = (x - mean) / sqrt(variance + eps) * weight + bias over x's last dimension (up to 32768 values).
 

@@ -64,23 +64,21 @@ hipError_t shrink_launch(const ShrinkArgs&, int dtype, hipStream_t);
 hipError_t planes_join(float* h, const float* from, size_t n, int planes, hipStream_t);
 // Whether the projection that these operands get adds up the planes of h itself.
 bool project_sums_planes(const ProjectArgs&, int dtype, bool nn);
-// part: project_part_bytes of scratch memory.
+// part: project_part_bytes of scratch memory, `four` as its W is given; a plan whose partial sums do not fit is refused.
 size_t project_part_bytes(size_t T, int K, int N, int G, int dtype, bool nn, bool four);
-hipError_t project_launch(const ProjectArgs&, float* part, int dtype, bool nn, hipStream_t);
+hipError_t project_launch(const ProjectArgs&, float* part, size_t part_bytes, int dtype, bool nn, hipStream_t);
 // W in 4 bits may be cheaper as values in memory: the bytes of scratch memory that takes (0: never for these sizes), and, where it
 // is for these operands, the launch that writes them there; `a` then reads those.
 size_t unpack_bytes(size_t T, int K, int N, int G, int dtype, bool nn);
 hipError_t unpack_launch(ProjectArgs& a, void* room, int dtype, bool nn, hipStream_t st);
 // What project_launch runs: one launch, or one of whole tiles and one of the rows that are left over.
 void project_plan(size_t T, int K, int N, int G, int dtype, bool nn, bool direct, bool four, cp4_adapter_launch (&launches)[2]);
-// The tiles of a projection on the matrix cores, its depth in `splits` parts of `each` steps, whose partial
-// sums take tile_part_bytes.
+// The tiles of a projection on the matrix cores, its depth in `splits` parts of `each` steps.
 struct TilePlan {
   int which, splits, each;
   double cost;            // microseconds, about
 };
 TilePlan tile_plan(size_t T, int K, int N, int dtype, bool nn, bool direct, bool four);
-size_t tile_part_bytes(const TilePlan&, size_t T, int N);
 int tile_rows(const TilePlan&);
 int tile_cols(const TilePlan&);
 // Whether these operands go from memory to the LDS without passing a register.

@@ -64,10 +64,20 @@ extern "C" size_t cp4_adapter_kept_bytes(const cp4_adapter_shape* s, int dtype) 
 
 namespace {
 
+struct ForwardPlan {
+  int planes;
+  size_t part_at, w_at, total;                         // (h comes first, W's values last)
+};
+ForwardPlan forward_plan(const cp4_adapter_shape& s, int dtype, bool four) {
+  ForwardPlan p{};
+  p.planes = shrink_planes(s.T, (int)s.K, dtype);
+  p.part_at = align256(p.planes * h_bytes(s));
+  p.w_at = p.part_at + align256(project_part_bytes(s.T, (int)s.K, (int)s.N, (int)s.G, dtype, false, four));
+  p.total = p.w_at + (four ? align256(unpack_bytes(s.T, (int)s.K, (int)s.N, (int)s.G, dtype, false)) : 0);
+  return p;
+}
 size_t forward_bytes(const cp4_adapter_shape* s, int dtype, bool four) {
-  if (check_shape(s, dtype) != CP4_OK) return 0;
-  return align256(shrink_planes(s->T, (int)s->K, dtype) * h_bytes(*s)) + align256(project_part_bytes(s->T, (int)s->K, (int)s->N, (int)s->G, dtype, false, four)) +
-         (four ? align256(unpack_bytes(s->T, (int)s->K, (int)s->N, (int)s->G, dtype, false)) : 0);
+  return check_shape(s, dtype) == CP4_OK ? forward_plan(*s, dtype, four).total : 0;
 }
 
 // scales: null, or W's in 4 bits.
@@ -78,8 +88,8 @@ cp4_status forward(const cp4_adapter_shape* s, int dtype, const void* x, const v
   if (!s->T) return CP4_OK;
   if (!x || !W || !A || !B || !ids || !y) return fail_with(CP4_ERR_NULL_POINTER, "an operand is NULL");
   if (const cp4_status rc = check_pointers(value_bytes(dtype), {x, scales ? nullptr : W, A, B, y}, {ids, scale, bias})) return rc;
-  const size_t need = forward_bytes(s, dtype, scales);
-  if (!workspace || workspace_bytes < need || ((size_t)workspace & 255))
+  const ForwardPlan plan = forward_plan(*s, dtype, scales);
+  if (!workspace || workspace_bytes < plan.total || ((size_t)workspace & 255))
     return fail_with(CP4_ERR_WORKSPACE, "workspace missing, too small or not aligned to 256 bytes");
   if ((size_t)kept & 15) return fail_with(CP4_ERR_WORKSPACE, "kept is not aligned to 16 bytes");
   const hipStream_t st = static_cast<hipStream_t>(stream);
@@ -96,11 +106,9 @@ cp4_status forward(const cp4_adapter_shape* s, int dtype, const void* x, const v
   p.T = s->T; p.ldz = sh.ldz; p.ldw = scales ? (s->K + 31) / 32 : s->ldw ? s->ldw : s->K; p.scales = scales;
   p.K = (int)s->K; p.N = (int)s->N; p.R = (int)s->R; p.Rp = sh.Rp; p.G = (int)s->G;
   p.fn = (int)s->R; p.fr = 1; p.planes = sh.planes; p.plane = p.T * p.Rp;
-  float* const part = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(sh.planes * h_bytes(*s)));
-  if (scales) {
-    char* const room = reinterpret_cast<char*>(part) + align256(project_part_bytes(p.T, p.K, p.N, p.G, dtype, false, true));
-    if (const hipError_t e = unpack_launch(p, room, dtype, false, st)) return fail_hip(e, "cp4_adapter_mx4_forward");
-  }
+  float* const part = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.part_at);
+  if (scales)
+    if (const hipError_t e = unpack_launch(p, static_cast<char*>(workspace) + plan.w_at, dtype, false, st)) return fail_hip(e, "cp4_adapter_mx4_forward");
   if (p.planes > 1 && project_sums_planes(p, dtype, false)) {
     p.keep = kept;
   } else if (p.planes > 1) {
@@ -109,7 +117,7 @@ cp4_status forward(const cp4_adapter_shape* s, int dtype, const void* x, const v
     p.h = h;
     p.planes = 1;
   }
-  if (const hipError_t e = project_launch(p, part, dtype, false, st)) return fail_hip(e, "cp4_adapter_forward");
+  if (const hipError_t e = project_launch(p, part, plan.w_at - plan.part_at, dtype, false, st)) return fail_hip(e, "cp4_adapter_forward");
   return CP4_OK;
 }
 
@@ -189,7 +197,7 @@ cp4_status backward(const cp4_adapter_shape* s, int dtype, const void* dy, const
     p.fn = 1; p.fr = (int)s->K; p.planes = 1;
     if (scales)
       if (const hipError_t e = unpack_launch(p, static_cast<char*>(workspace) + plan.w_at, dtype, true, st)) return fail_hip(e, "cp4_adapter_mx4_backward");
-    if (const hipError_t e = project_launch(p, part, dtype, true, st)) return fail_hip(e, "cp4_adapter_backward");
+    if (const hipError_t e = project_launch(p, part, plan.w_at - plan.part_at, dtype, true, st)) return fail_hip(e, "cp4_adapter_backward");
   }
   if (dA) {
     GradArgs ga{};
@@ -246,7 +254,7 @@ cp4_status linear(size_t T, int K, int N, int dtype, const void* z, size_t ldz, 
   p.T = T; p.ldz = ldz; p.ldw = blocks;
   p.K = K; p.N = N; p.planes = 1;
   if (const hipError_t e = unpack_launch(p, static_cast<char*>(workspace) + parts, dtype, nn, static_cast<hipStream_t>(stream))) return fail_hip(e, where);
-  if (const hipError_t e = project_launch(p, static_cast<float*>(workspace), dtype, nn, static_cast<hipStream_t>(stream)))
+  if (const hipError_t e = project_launch(p, static_cast<float*>(workspace), parts, dtype, nn, static_cast<hipStream_t>(stream)))
     return fail_hip(e, where);
   return CP4_OK;
 }
@@ -279,6 +287,22 @@ extern "C" cp4_status cp4_adapter_plan_query(const cp4_adapter_shape* s, int dty
   cp4_adapter_launch l[2];
   const int K = (int)(backward ? s->N : s->K), N = (int)(backward ? s->K : s->N);
   project_plan(s->T, K, N, (int)s->G, dtype, backward != 0, aligned != 0, false, l);
+  launches[0] = l[0];
+  launches[1] = l[1];
+  return CP4_OK;
+}
+
+extern "C" cp4_status cp4_mx4_plan_query(size_t T, unsigned K, unsigned N, unsigned G, int dtype, int backward, int aligned,
+                                         cp4_adapter_launch launches[2], size_t room[2]) {
+  if (const cp4_status rc = check_linear(T, K, N, dtype, 0, 0, nullptr); rc == CP4_ERR_SHAPE) return rc;
+  if (G > 65535) return fail_with(CP4_ERR_SHAPE, "more than 65535 adapters");
+  if (!launches || !room) return fail_with(CP4_ERR_NULL_POINTER, "launches or room is NULL");
+  const bool nn = backward != 0;
+  const int depth = (int)(nn ? N : K), cols = (int)(nn ? K : N);
+  room[0] = T ? align256(project_part_bytes(T, depth, cols, (int)G, dtype, nn, true)) : 0;
+  room[1] = T ? align256(unpack_bytes(T, depth, cols, (int)G, dtype, nn)) : 0;
+  cp4_adapter_launch l[2];
+  project_plan(T, depth, cols, (int)G, dtype, nn, aligned != 0, !(aligned && room[1]), l);
   launches[0] = l[0];
   launches[1] = l[1];
   return CP4_OK;

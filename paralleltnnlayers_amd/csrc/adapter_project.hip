@@ -7,16 +7,28 @@ namespace cp4 {
 namespace adapter {
 namespace {
 
+// What a launch runs on.
+struct Choice {
+  bool by_rows;
+  RowsPlan rows;
+  TilePlan tile;
+  double cost() const { return by_rows ? rows.cost : tile.cost; }
+  int splits() const { return by_rows ? rows.splits : tile.splits; }
+  size_t part_bytes(size_t T, int N) const { return splits() > 1 ? (size_t)splits() * T * N * 4 : 0; }
+};
 // The rows kernel or tiles, for tokens that both take.  A tile takes its adapters a few at a time, some 0.6 us each
 // (fp32: 1.2), the rows kernel's waves share them; how many different ones there are only the device knows: at most G.
 // (bf16, 4096 x 4096, rank 16, rows kernel and tiles: 20 tokens of 2 adapters 17 us and 21, of 20 adapters 26 and 40; 64 tokens of
 // 2 adapters 26 and 22, of 64 adapters 42 and 55; 4096 x 14336, 20 tokens of 2 adapters 50 and 33.)
-bool by_rows(size_t T, int K, int N, int G, int dtype, bool nn, bool direct, bool four) {
-  const RowsPlan rows = nn ? RowsPlan{} : rows_plan(T, K, N, dtype, four, direct);
-  if (!rows.splits || T <= 16) return rows.splits;                   // (up to 16 tokens: within 8 % of the tiles at worst)
+Choice choose(size_t T, int K, int N, int G, int dtype, bool nn, bool direct, bool four) {
+  Choice c{};
+  if (!nn) c.rows = rows_plan(T, K, N, dtype, four, direct);
+  c.by_rows = c.rows.splits;
+  if (c.by_rows && T <= 16) return c;                                // (up to 16 tokens: within 8 % of the tiles at worst)
+  c.tile = tile_plan(T, K, N, dtype, nn, direct, four);
   const double adapters = (double)std::min<size_t>(T, G);
-  return rows.cost + rows.adapter * adapters <=
-         tile_plan(T, K, N, dtype, nn, direct, four).cost + (dtype == CP4_DTYPE_F32 ? 1.2 : 0.6) * adapters;
+  c.by_rows = c.by_rows && c.rows.cost + c.rows.adapter * adapters <= c.tile.cost + (dtype == CP4_DTYPE_F32 ? 1.2 : 0.6) * adapters;
+  return c;
 }
 
 // Rows of the tiles' launch; the rest, less than a tile's, is cheaper on its own where it would take a round of
@@ -28,8 +40,7 @@ size_t main_rows(size_t T, int K, int N, int G, int dtype, bool nn, bool direct,
   for (size_t tile : {256, 128}) {
     const size_t rest = T % tile;
     if (!rest || T <= 2 * tile) continue;
-    const double other = by_rows(rest, K, N, G, dtype, nn, direct, four) ? rows_plan(rest, K, N, dtype, four, direct).cost
-                                                                   : tile_plan(rest, K, N, dtype, nn, direct, four).cost;
+    const double other = choose(rest, K, N, G, dtype, nn, direct, four).cost();
     const double cost = tile_plan(T - rest, K, N, dtype, nn, direct, four).cost + other + 6.0;    // (a launch and its start)
     if (cost < least) {
       least = cost;
@@ -39,26 +50,16 @@ size_t main_rows(size_t T, int K, int N, int G, int dtype, bool nn, bool direct,
   return best;
 }
 
-hipError_t launch(const ProjectArgs& a, float* part, int dtype, bool nn, bool direct, hipStream_t st) {
-  const bool four = a.scales;
-  if (by_rows(a.T, a.K, a.N, a.G, dtype, nn, direct, four)) return rows_launch(a, rows_plan(a.T, a.K, a.N, dtype, four, direct), part, dtype, st);
-  return tile_launch(a, tile_plan(a.T, a.K, a.N, dtype, nn, direct, four), part, dtype, nn, st);
+hipError_t launch(const ProjectArgs& a, const Choice& c, float* part, int dtype, bool nn, hipStream_t st) {
+  return c.by_rows ? rows_launch(a, c.rows, part, dtype, st) : tile_launch(a, c.tile, part, dtype, nn, st);
 }
 
-}  // namespace
-
-namespace {
 // The operands of a projection with W as values in memory.
 size_t unpacked_row(int cols) { return ((size_t)cols + 7) / 8 * 8; }
 double cost_of(size_t T, int K, int N, int G, int dtype, bool nn, bool direct, bool four) {
   const size_t main = main_rows(T, K, N, G, dtype, nn, direct, four);
-  double cost = 0.0;
-  for (size_t rows : {main, T - main}) {
-    if (!rows) continue;
-    cost += by_rows(rows, K, N, G, dtype, nn, direct, four) ? rows_plan(rows, K, N, dtype, four, direct).cost
-                                                            : tile_plan(rows, K, N, dtype, nn, direct, four).cost;
-  }
-  return cost;
+  const double cost = choose(main, K, N, G, dtype, nn, direct, four).cost();
+  return main == T ? cost : cost + choose(T - main, K, N, G, dtype, nn, direct, four).cost();
 }
 // Whether W is unpacked: in 16 bits from some 600 tokens on, where the larger tiles take whole cache lines of W (4096 x 4096:
 // 512 tokens 34 us from codes, 35 through memory; 1024 tokens 50 and 45; 8192 tokens 337 and 195).  fp32 reads codes with three
@@ -83,22 +84,19 @@ hipError_t unpack_launch(ProjectArgs& a, void* room, int dtype, bool nn, hipStre
   return hipSuccess;
 }
 
-// Enough for each choice that the operands' alignment makes.
+// Enough for each choice that the operands' alignment makes: of the tiles in 16 bits, of the few rows in every type where W is
+// in 4 bits.
 size_t project_part_bytes(size_t T, int K, int N, int G, int dtype, bool nn, bool four) {
   size_t most = 0;
   const auto part = [&](size_t rows, bool direct) {
-    const RowsPlan few = rows_plan(rows, K, N, dtype, four, direct);
-    if (by_rows(rows, K, N, G, dtype, nn, direct, four)) most = std::max(most, few.splits > 1 ? few.splits * rows * N * 4 : 0);
-    else most = std::max(most, tile_part_bytes(tile_plan(rows, K, N, dtype, nn, direct, four), rows, N));
+    most = std::max(most, choose(rows, K, N, G, dtype, nn, direct, four).part_bytes(rows, N));
   };
   if (four && unpacks(T, K, N, G, dtype, nn)) most = project_part_bytes(T, K, N, G, dtype, nn, false);
   for (bool direct : {false, true}) {
-    if (direct && dtype == CP4_DTYPE_F32) break;                     // (the same plans)
+    if (direct && dtype == CP4_DTYPE_F32 && !four) break;            // (the same plans)
     const size_t main = main_rows(T, K, N, G, dtype, nn, direct, four);
-    part(T, direct);
-    if (main == T) continue;
     part(main, direct);
-    part(T - main, direct);
+    if (main != T) part(T - main, direct);
   }
   return most;
 }
@@ -106,9 +104,8 @@ size_t project_part_bytes(size_t T, int K, int N, int G, int dtype, bool nn, boo
 void project_plan(size_t T, int K, int N, int G, int dtype, bool nn, bool direct, bool four, cp4_adapter_launch (&launches)[2]) {
   const auto one = [&](size_t rows) {
     if (!rows) return cp4_adapter_launch{};
-    if (by_rows(rows, K, N, G, dtype, nn, direct, four)) return cp4_adapter_launch{rows, 0, 0, rows_plan(rows, K, N, dtype, four, direct).splits};
-    const TilePlan p = tile_plan(rows, K, N, dtype, nn, direct, four);
-    return cp4_adapter_launch{rows, tile_rows(p), tile_cols(p), p.splits};
+    const Choice c = choose(rows, K, N, G, dtype, nn, direct, four);
+    return cp4_adapter_launch{rows, c.by_rows ? 0 : tile_rows(c.tile), c.by_rows ? 0 : tile_cols(c.tile), c.splits()};
   };
   const size_t main = main_rows(T, K, N, G, dtype, nn, direct, four);
   launches[0] = one(main);
@@ -116,14 +113,17 @@ void project_plan(size_t T, int K, int N, int G, int dtype, bool nn, bool direct
 }
 
 bool project_sums_planes(const ProjectArgs& a, int dtype, bool nn) {
-  return by_rows(a.T, a.K, a.N, a.G, dtype, nn, tile_direct(a, dtype, nn), a.scales);
+  return choose(a.T, a.K, a.N, a.G, dtype, nn, tile_direct(a, dtype, nn), a.scales).by_rows;
 }
 
-hipError_t project_launch(const ProjectArgs& a, float* part, int dtype, bool nn, hipStream_t st) {
+hipError_t project_launch(const ProjectArgs& a, float* part, size_t part_bytes, int dtype, bool nn, hipStream_t st) {
   const bool direct = tile_direct(a, dtype, nn), four = a.scales;
-  const size_t main = main_rows(a.T, a.K, a.N, a.G, dtype, nn, direct, four);
-  if (main == a.T) return launch(a, part, dtype, nn, direct, st);
-  const size_t e = dtype == CP4_DTYPE_F32 ? 4 : 2;
+  const size_t main = main_rows(a.T, a.K, a.N, a.G, dtype, nn, direct, four), e = dtype == CP4_DTYPE_F32 ? 4 : 2;
+  const Choice of_main = choose(main, a.K, a.N, a.G, dtype, nn, direct, four);
+  if (of_main.part_bytes(main, a.N) > part_bytes) return hipErrorInvalidValue;
+  if (main == a.T) return launch(a, of_main, part, dtype, nn, st);
+  const Choice of_rest = choose(a.T - main, a.K, a.N, a.G, dtype, nn, direct, four);
+  if (of_rest.part_bytes(a.T - main, a.N) > part_bytes) return hipErrorInvalidValue;
   ProjectArgs first = a, rest = a;
   first.T = main;
   rest.T = a.T - main;
@@ -131,8 +131,8 @@ hipError_t project_launch(const ProjectArgs& a, float* part, int dtype, bool nn,
   if (a.h) rest.h = a.h + main * a.Rp;
   if (a.ids) rest.ids = a.ids + main;
   rest.y = static_cast<char*>(a.y) + main * a.N * e;
-  if (const hipError_t err = launch(first, part, dtype, nn, direct, st)) return err;
-  return launch(rest, part, dtype, nn, direct, st);
+  if (const hipError_t err = launch(first, of_main, part, dtype, nn, st)) return err;
+  return launch(rest, of_rest, part, dtype, nn, st);
 }
 
 }  // namespace adapter
