@@ -30,7 +30,8 @@ typedef struct cp4_muon_matrix {
   void* param;          /* of param_dtype, updated; NULL: no step is taken */
   const void* grad;     /* of grad_dtype */
   float* momentum;      /* updated; NULL: u is grad */
-  void* copy;           /* NULL, or of copy_dtype: the new parameters, rounded; without param X itself */
+  void* copy;           /* NULL, or of copy_dtype: the new parameters, rounded; without param X itself; with neither the
+                           momentum alone is updated */
   size_t count;
   unsigned rows, cols;  /* up to 65536 each; nothing is read or written where one of the three is 0 */
   int param_dtype, grad_dtype, copy_dtype;   /* cp4_dtype */

@@ -35,13 +35,14 @@ struct Rates {
 // Q [N][K], E and C [R][N] in two parts.
 struct Product {
   const char *P, *Q, *E;                    // E null: alpha is 0
-  char *C, *Ct;                             // Ct: C transposed as well (may be null); C null: the outputs
+  char *C, *Ct;                             // Ct: C transposed as well (may be null)
   float* part;                              // splits > 1: partial sums [count][splits][R][N], and nothing else
-  Outputs o;
+  Outputs o;                                // (final) instead of C
   Rates rates;
   unsigned R, N, K, count;
   float alpha, beta, diagonal;
   bool symmetric;                           // R == N and C is symmetric: tiles on and below the diagonal, mirrored into C
+  bool final;                               // of all of a launch's products, or of none
 };
 constexpr int kProducts = 16;               // of a launch
 

@@ -504,6 +504,8 @@ constexpr size_t kGroupBytes = (size_t)1 << 30;
 constexpr size_t kNormParts = 1 << 16;             // at most, of a group
 
 bool nothing(const cp4_muon_matrix& x) { return !x.count || !x.rows || !x.cols; }
+// (without them the momentum alone is updated)
+bool has_outputs(const cp4_muon_matrix& x) { return x.param || x.copy; }
 
 // Sizes of gram's launch: an entry's splits.  Enough workgroups for four on a compute unit, but no more than one workgroup
 // of iterate adds up in the time of a launch (10 blocks of 2 KB a split at a side of 64).
@@ -536,8 +538,9 @@ Product gram_product(const cp4_muon_matrix& x, unsigned count) {
 // The splits of a group's first product and what they take.
 int large_splits(const cp4_muon_matrix* x, const Group& g, size_t* bytes) {
   std::vector<Product> a;
-  for (const Piece& p : g.pieces) a.push_back(gram_product(x[p.entry], (unsigned)p.count));
-  const int splits = product_splits(a.data(), (int)a.size());
+  for (const Piece& p : g.pieces)
+    if (has_outputs(x[p.entry])) a.push_back(gram_product(x[p.entry], (unsigned)p.count));
+  const int splits = a.empty() ? 1 : product_splits(a.data(), (int)a.size());
   *bytes = 0;
   if (splits > 1)
     for (const Product& p : a) *bytes += align256((size_t)p.count * splits * p.R * p.N * 4);
@@ -716,19 +719,21 @@ hipError_t run_large(const cp4_muon_matrix* x, const Group& g, const Settings& s
     it.cols = e.cols;
     it.chunks = (unsigned)(((size_t)e.rows * e.cols + chunk - 1) / chunk);
     a.norm[i] = norm;
-    it.tiles = ((e.rows + 63) / 64) * ((e.cols + 63) / 64);
+    it.tiles = has_outputs(e) ? ((e.rows + 63) / 64) * ((e.cols + 63) / 64) : 0;
     a.split[i] = split;
     norm += it.chunks * (unsigned)p.count;
     split += it.tiles * (unsigned)p.count;
   }
   norm_kernel<<<norm, 256, 0, st>>>(a);
-  split_kernel<<<split, 256, 0, st>>>(a);
+  if (split) split_kernel<<<split, 256, 0, st>>>(a);
   if (const hipError_t e = hipGetLastError()) return e;
+  if (!split) return hipSuccess;
   for (int k = 0; k < s.steps; ++k) {
     std::vector<Product> pa, pb, px;
     char* to = part;
     for (size_t i = 0; i < g.pieces.size(); ++i) {
       const cp4_muon_matrix& e = x[g.pieces[i].entry];
+      if (!has_outputs(e)) continue;
       const Buffers& b = buffers[i];
       const char *const X = b.x[k % 2], *const Xt = b.t[k % 2];
       Product p = gram_product(e, (unsigned)g.pieces[i].count);
@@ -765,6 +770,7 @@ hipError_t run_large(const cp4_muon_matrix* x, const Group& g, const Settings& s
         p.Ct = b.t[(k + 1) % 2];
       } else {
         p.C = nullptr;
+        p.final = true;
         p.o = outputs_of(e, g.pieces[i].first);
         p.rates = rates_of(e, s);
       }

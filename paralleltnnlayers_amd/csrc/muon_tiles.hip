@@ -342,7 +342,6 @@ int depth_of(const Product* p, int n) {
 }
 
 constexpr int kEdges[3] = {256, 128, 64};
-bool is_final(const Product* p) { return p[0].o.param || p[0].o.copy; }
 // The tiles' edge and the parts of the depth by the least time of a model of what was measured (microseconds a step and for the
 // launch's ends): 64 x 64 0.225 and 5.5; 128 x 128 one on a compute unit 0.63 and 7.5, two 1.3 and 14; 256 x 256 1.58 and 21 where
 // they leave a good part of the units free, 2.2 where all are at work.  (The last product's outputs leave the largest one no
@@ -355,7 +354,7 @@ Choice choose(const Product* p, int n, bool may_split) {
   const size_t units = num_compute_units();
   Choice best{2, 1};
   double least = 0.0;
-  for (int w = is_final(p); w < 3; ++w) {
+  for (int w = p[0].final; w < 3; ++w) {
     const size_t tiles = all_tiles(p, n, kEdges[w]);
     for (int s = 1; s <= 32 && (s == 1 || (may_split && depth / s >= 16)); ++s) {
       const size_t wgs = tiles * s, once = (wgs + units - 1) / units, twice = (wgs + 2 * units - 1) / (2 * units);
@@ -403,7 +402,7 @@ hipError_t product_launch(const Product* p, int n, int splits, hipStream_t st) {
     t.tiles[i] = (unsigned)tiles_of(p[i], edge);
     t.total += p[i].count * t.tiles[i] * splits;
   }
-  const Kind kind = splits > 1 ? kPartial : is_final(p) ? kFinal : kParts;
+  const Kind kind = splits > 1 ? kPartial : p[0].final ? kFinal : kParts;
   const hipError_t e = c.which == 0 ? launch<8, 4, 4, 2>(t, kind, st) : c.which == 1 ? launch<4, 4, 2, 2>(t, kind, st) : launch<2, 2, 2, 8>(t, kind, st);
   if (e || splits == 1) return e;
   unsigned grid = 0;

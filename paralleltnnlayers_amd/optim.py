@@ -210,8 +210,8 @@ def muon_step(params, grads, momenta, *, lr, momentum=0.95, nesterov=True, weigh
     """One Muon step of all ``params`` (contiguous float32, bfloat16 or float16), in place: each matrix along its
     momentum, orthogonalised by ``steps`` Newton-Schulz products (up to 16), times ``lr sqrt(max(1, rows / cols))``.
 
-    A parameter is [..., rows, cols]: a stack of matrices that are orthogonalised one by one.  grads: one each, of any
-    of the three types (None: that parameter is left alone).  momenta: float32 of the same shape, zero before the first step.
+    A parameter is [..., rows, cols]: a stack of matrices that are orthogonalised one by one (None: its momentum alone is
+    updated).  grads: one each, of any of the three types (None: that parameter is left alone).  momenta: float32 of the same shape, zero before the first step.
     copies: tensors (or None) that receive the new parameters rounded to their type.  A matrix whose momentum is not
     finite becomes NaN.  What is written must not overlap another tensor of the call.  A step that is captured into a graph keeps
     the settings it was captured with."""
