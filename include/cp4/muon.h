@@ -11,7 +11,8 @@
  *
  * The polynomial takes every singular value from 0.01 or so up into 0.68 .. 1.21 in five steps and keeps it there.
  * m, p's step and all sums are fp32 or wider whatever the types in memory.  Matrices with a side of up to 64 go through
- * their Gram matrix, summed and iterated in fp64; larger ones through products of values in two float16 parts
+ * their Gram matrix, summed and iterated in fp64 (and past 5 steps applied in it, so that directions a matrix does not
+ * have stay nothing however often they are multiplied by 3.4445); larger ones through products of values in two float16 parts
  * (22 bits; accumulated in fp32).  No atomics: results do not change from call to call.  A matrix whose u has
  * an infinity or a NaN becomes NaN in whole; others are not touched by it.
  */

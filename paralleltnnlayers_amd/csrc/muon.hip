@@ -8,7 +8,7 @@
 //             values, and a small one would drown in fp32's roundings of the largest -, split over workgroups;
 //   iterate   one workgroup a matrix: adds up the splits, |u|^2 is G's trace, then A <- A p(A)^2 and Q <- Q p(A) in
 //             fp64 in the LDS (up to 16: in registers), all of them symmetric, blocks on and below the diagonal alone;
-//   apply     X = Q u in fp32 and the parameters' step.
+//   apply     X = Q u and the parameters' step, in fp32 up to 5 steps, in fp64 beyond (wide()).
 //
 // So the step is bound by memory where matrices are long (12 bytes a value in gram, 16 in apply) and by the
 // latency of three launches where they are short: 28 adapters' factors of 7 x 1001 and 777 x 7 7 + 6 + 8 us.  The entries of a
@@ -24,12 +24,15 @@ namespace cp4 {
 namespace muon {
 namespace {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kSmall = 72, kLarge = 16;            // entries of a launch
 static_assert(kLarge <= kProducts, "a launch of products holds a group");
 constexpr unsigned kSide = 64;                     // the longest short side that goes through its Gram matrix
+// Whether Q and its products with u are fp64.  Q is 3.4445 to the steps in directions that u lacks, and of as much are its roundings,
+// which X sees: in fp32 3e-5 of it in 5 steps (as an iteration of X in fp32 has, 4e-5), 1e-3 in 8, 0.1 in 12, 50 in 16.  fp64
+// takes 131 us for 32 matrices of 64 x 4096, fp32 112; 77 and 71 of 48 x 4096; 51 and 50 for 28 adapters' 7 x 1001 and 777 x 7.
+__host__ __device__ constexpr bool wide(int steps) { return steps > 5; }
 
 // ---- a short side of up to 64 ------------------------------------------------------------
 
@@ -49,7 +52,7 @@ struct SmallArgs {
   float mu, decay;
   double eps, lr;
   double* part;                                    // [gram's workgroups][blocks][16][16]
-  float* q;                                        // [iterate's workgroups][M][M]
+  void* q;                                         // [iterate's workgroups][M][M], fp64 where `steps` is wide(), or fp32
 };
 static_assert(sizeof(SmallArgs) <= 4096, "kernel arguments");
 
@@ -171,6 +174,19 @@ __device__ __forceinline__ double wave_sum(double x) {
   return x;
 }
 
+// What is added to G's diagonal, of its trace.  A step multiplies a small eigenvalue by 11.9.  Where u has fewer directions than rows,
+// G's others are roundings: some 2^-53 times the root of a wave's 16 to n / 4 sums in a row, of either sign, and negative ones
+// would leave the polynomial's range in 15 steps (|X| reaches 94 for one direction in 16 rows at 16 steps).  Lifted they stay
+// in it.  Singular values of 1e-6 of the norm come out 4e-3 off where that counts (from ten steps on); a fp32 iteration's own roundings
+// are 6e-2 of them.
+__device__ __forceinline__ double lift(const SmallItem& it, int steps) {
+  return wide(steps) ? 0x1p-48 * fmax(1.0, max(it.rows(), it.cols()) / 8192.0) : 0.0;
+}
+__device__ __forceinline__ void put_q(const SmallArgs& a, size_t at, double q) {
+  if (wide(a.steps)) static_cast<double*>(a.q)[at] = q;
+  else static_cast<float*>(a.q)[at] = (float)q;
+}
+
 // A matrix of the iteration in the LDS: [MB][MB] blocks of 16 x 16, their rows 17 apart (a column is in all banks).  An fp64 product's
 // result holds, at a lane's place v, row lane / 16 + 4 v and column lane % 16, which is also what its operands want there, the
 // first one turned.  So X^T Y, which is X Y for a symmetric X, reads whole blocks in order.
@@ -249,10 +265,12 @@ __global__ __launch_bounds__(64 * iterate_waves(MB)) void iterate_kernel(const S
   __syncthreads();
   const int lane = threadIdx.x & 63;
   const double square = wave_sum(lane < M ? A[lane / 16 * (MB + 1) * kBlockOf + lane % 16 * (kRowOf + 1)] : 0.0);
-  const double over = square < INFINITY ? 1.0 / (sqrt(square) + a.eps) : (double)NAN;
+  const double over = square < INFINITY ? 1.0 / (sqrt(square) + a.eps) : (double)NAN, more = lift(a.item[entry], a.steps) * square;
   __syncthreads();
-  for (int e = threadIdx.x; e < kAll; e += kThreads)
-    if (e % kRowOf < 16) A[e] = A[e] * over * over;
+  for (int e = threadIdx.x; e < kAll; e += kThreads) {
+    const int r = e % kBlockOf / kRowOf, c = e % kRowOf, i = e / kBlockOf / MB, j = e / kBlockOf % MB;
+    if (c < 16) A[e] = (A[e] + (i == j && r == c ? more : 0.0)) * over * over;
+  }
   __syncthreads();
   const auto plain = [](int, double x, bool) { return x; };
   for (int s = 0; s < a.steps; ++s) {
@@ -284,10 +302,9 @@ __global__ __launch_bounds__(64 * iterate_waves(MB)) void iterate_kernel(const S
     if (wave < B) put_block<MB>(x[0], A, wave, plain);
     __syncthreads();
   }
-  float* const q = a.q + (size_t)blockIdx.x * (M * M);
   for (int e = threadIdx.x; e < M * M; e += kThreads) {
     const int r = e / M, c = e % M;
-    q[e] = (float)(Q[(r / 16 * MB + c / 16) * kBlockOf + r % 16 * kRowOf + c % 16] * over);
+    put_q(a, (size_t)blockIdx.x * (M * M) + e, Q[(r / 16 * MB + c / 16) * kBlockOf + r % 16 * kRowOf + c % 16] * over);
   }
 }
 
@@ -300,6 +317,23 @@ __device__ __forceinline__ f64x4 turned_product(const f64x4& x, const f64x4& y) 
 #pragma unroll
   for (int s = 0; s < 4; ++s) acc = __builtin_amdgcn_mfma_f64_16x16x4f64(x[s], y[s], acc, 0, 0, 0);
   return acc;
+}
+// The mean of such a matrix and its transposed.
+__device__ __forceinline__ f64x4 balanced(const f64x4& x) {
+  const int lane = threadIdx.x & 63, l = lane & 15, g = lane >> 4;
+  f64x4 out;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {
+    const int from = g + 4 * v + 16 * (l & 3);                     // (row l, column g + 4 v: there at the place l / 4)
+    double y = 0.0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const double z = __shfl(x[w], from);
+      y = l >> 2 == w ? z : y;
+    }
+    out[v] = 0.5 * (x[v] + y);
+  }
+  return out;
 }
 __global__ __launch_bounds__(256) void iterate_16_kernel(const SmallArgs a) {
   __shared__ double sums[3][256];
@@ -324,8 +358,9 @@ __global__ __launch_bounds__(256) void iterate_16_kernel(const SmallArgs a) {
 #pragma unroll
   for (int v = 0; v < 4; ++v) trace += g + 4 * v == l ? A[v] : 0.0;
   trace = wave_sum(trace);
-  const double over = trace < INFINITY ? 1.0 / (sqrt(trace) + a.eps) : (double)NAN;
-  A = A * over * over;
+  const double over = trace < INFINITY ? 1.0 / (sqrt(trace) + a.eps) : (double)NAN, more = lift(a.item[entry], a.steps) * trace;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) A[v] = (A[v] + (g + 4 * v == l ? more : 0.0)) * over * over;
   f64x4 Q = {};
   for (int s = 0; s < a.steps; ++s) {
     f64x4 P = turned_product(A, A);                                // a + b A + c A A
@@ -333,16 +368,23 @@ __global__ __launch_bounds__(256) void iterate_16_kernel(const SmallArgs a) {
     for (int v = 0; v < 4; ++v) P[v] = kC * P[v] + kB * A[v] + (g + 4 * v == l ? kA : 0.0);
     Q = s ? turned_product(Q, P) : P;
     if (s + 1 < a.steps) A = turned_product(turned_product(A, P), P);
+    // (what A and its transposed differ by grows in directions that u lacks as their values do: 1e-8 of X in 8 steps, 1e-6 in 10,
+    // 1e-2 in 14)
+    if (wide(a.steps)) A = balanced(A);
   }
 #pragma unroll
-  for (int v = 0; v < 4; ++v) a.q[(size_t)blockIdx.x * 256 + (g + 4 * v) * 16 + l] = (float)(Q[v] * over);
+  for (int v = 0; v < 4; ++v) put_q(a, (size_t)blockIdx.x * 256 + (g + 4 * v) * 16 + l, Q[v] * over);
 }
 
-template <int MB>
+// F: float or double.
+template <int MB, class F>
 __global__ __launch_bounds__(256) void apply_kernel(const SmallArgs a) {
   typedef Tile<MB> T;
-  constexpr int M = T::M, SQ = M + 4;
-  __shared__ __attribute__((aligned(16))) float u[M * T::S], q[M * SQ];
+  typedef F Four __attribute__((ext_vector_type(4)));
+  constexpr bool kWide = sizeof(F) == 8;
+  constexpr int M = T::M, SQ = M + (kWide ? 2 : 4);
+  __shared__ __attribute__((aligned(16))) float u[M * T::S];
+  __shared__ F q[M * SQ];
   const int entry = entry_of(a.apply, blockIdx.x);
   const SmallItem& it = a.item[entry];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
@@ -351,24 +393,27 @@ __global__ __launch_bounds__(256) void apply_kernel(const SmallArgs a) {
   const int m = min(it.rows(), it.cols()), j0 = tile * T::JT;
   const size_t base = (size_t)matrix * it.rows() * it.cols();
   for (int e = m * T::S + threadIdx.x; e < M * T::S; e += 256) u[e] = 0.0f;
-  const float* const from = a.q + (size_t)(a.iterate[entry] + matrix) * (M * M);
+  const F* const from = static_cast<const F*>(a.q) + (size_t)(a.iterate[entry] + matrix) * (M * M);
   for (int e = threadIdx.x; e < M * M; e += 256) q[e / M * SQ + e % M] = from[e];
   load_tile<MB, false>(a, it, base, j0, u);
   __syncthreads();
 #pragma unroll 1
   for (int b = wave; b < T::JT / 16; b += 4) {                     // 16 places of the long side: this wave's alone
-    f32x4 acc[MB] = {};
+    Four acc[MB] = {};
 #pragma unroll 4
     for (int s = 0; s < M / 4; ++s) {
-      const float y = u[(4 * s + g) * T::S + 16 * b + l];
+      const F y = u[(4 * s + g) * T::S + 16 * b + l];
 #pragma unroll
-      for (int i = 0; i < MB; ++i)
-        acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(q[(16 * i + l) * SQ + 4 * s + g], y, acc[i], 0, 0, 0);
+      for (int i = 0; i < MB; ++i) {
+        const F x = q[(16 * i + l) * SQ + 4 * s + g];
+        if constexpr (kWide) acc[i] = __builtin_amdgcn_mfma_f64_16x16x4f64(x, y, acc[i], 0, 0, 0);
+        else acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, y, acc[i], 0, 0, 0);
+      }
     }
 #pragma unroll
     for (int i = 0; i < MB; ++i)
 #pragma unroll
-      for (int v = 0; v < 4; ++v) u[(16 * i + 4 * g + v) * T::S + 16 * b + l] = acc[i][v];
+      for (int v = 0; v < 4; ++v) u[(16 * i + (kWide ? g + 4 * v : 4 * g + v)) * T::S + 16 * b + l] = (float)acc[i][v];
   }
   __syncthreads();
   const auto shift = [&](void* p, int dtype) { return p ? (char*)p + base * (dtype == CP4_DTYPE_F32 ? 4 : 2) : nullptr; };
@@ -396,7 +441,8 @@ hipError_t small_launch(const SmallArgs& a, unsigned gram, unsigned iterate, uns
   gram_kernel<MB><<<gram, 256, 0, st>>>(a);
   if constexpr (MB == 1) iterate_16_kernel<<<iterate, 256, 0, st>>>(a);
   else iterate_kernel<MB><<<iterate, 64 * iterate_waves(MB), 0, st>>>(a);
-  apply_kernel<MB><<<apply, 256, 0, st>>>(a);
+  if (wide(a.steps)) apply_kernel<MB, double><<<apply, 256, 0, st>>>(a);
+  else apply_kernel<MB, float><<<apply, 256, 0, st>>>(a);
   return hipGetLastError();
 }
 
@@ -523,7 +569,7 @@ size_t small_bytes(const cp4_muon_matrix* x, Group& g) {
   for (const Piece& p : g.pieces) matrices += p.count;
   for (const Piece& p : g.pieces) wgs += p.count * gram_splits(tiles_of(x[p.entry], g.blocks), matrices, g.blocks);
   const size_t blocks = (size_t)g.blocks * (g.blocks + 1) / 2;
-  return align256(wgs * blocks * 256 * 8) + align256(matrices * g.blocks * g.blocks * 256 * 4);
+  return align256(wgs * blocks * 256 * 8) + align256(matrices * g.blocks * g.blocks * 256 * 8);
 }
 
 Product gram_product(const cp4_muon_matrix& x, unsigned count) {
@@ -659,7 +705,7 @@ hipError_t run_small(const cp4_muon_matrix* x, const Group& g, const Settings& s
   a.mu = s.mu;
   a.eps = s.eps;
   a.part = reinterpret_cast<double*>(ws);
-  a.q = reinterpret_cast<float*>(ws + align256((size_t)gram * (g.blocks * (g.blocks + 1) / 2) * 256 * 8));
+  a.q = ws + align256((size_t)gram * (g.blocks * (g.blocks + 1) / 2) * 256 * 8);
   switch (g.blocks) {
     case 1: return small_launch<1>(a, gram, iterate, apply, st);
     case 2: return small_launch<2>(a, gram, iterate, apply, st);
