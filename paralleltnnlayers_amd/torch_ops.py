@@ -397,28 +397,33 @@ class AdapterLinear(torch.nn.Module):
         return adapter_linear(x, self.projection(), self.A, self.B, ids, self.scale, self.bias)
 
 
+_NO_GRADIENT = "activations in 4 bits have no gradient: detach them, or call without gradients"
+
+
 class Mx4LinearFunction(torch.autograd.Function):
     """``mx4_linear`` as a Python autograd function: stands for the native one (csrc/torch/binding.cpp) where a
-    call has to be seen as an operator, in a trace."""
+    call has to be seen as an operator, in a trace.  ``activations``: as ``capi.mx4_linear`` takes it."""
 
     @staticmethod
-    def forward(ctx, x, codes, scales, bias, features):
+    def forward(ctx, x, codes, scales, bias, features, activations=None):
         if ctx.needs_input_grad[3]:
             raise ValueError("the projection and its bias are not trained: detach them")
         y = torch.empty(x.shape[:-1] + codes.shape[:1], dtype=x.dtype, device=x.device)   # (made by an operator)
-        capi.mx4_linear(x, capi.Mx4(codes, scales, features), bias, out=y)
+        capi.mx4_linear(x, capi.Mx4(codes, scales, features), bias, activations, out=y)
         ctx.save_for_backward(codes, scales)
-        ctx.features, ctx.dtype = features, x.dtype
+        ctx.features, ctx.dtype, ctx.activations = features, x.dtype, activations
         return y
 
     @staticmethod
     def backward(ctx, dy):
         codes, scales = ctx.saved_tensors
+        if ctx.activations is not None:
+            raise ValueError(_NO_GRADIENT)
         dx = capi.mx4_linear_backward(dy.detach().to(ctx.dtype), capi.Mx4(codes, scales, ctx.features))
         if torch.is_grad_enabled() and dy.requires_grad:             # (create_graph: as the native one)
             told = torch._C._functions.DelayedError(b"the gradients of mx4_linear cannot be differentiated again", 1)
             dx = told(dx.requires_grad_())
-        return dx, None, None, None, None
+        return dx, None, None, None, None, None
 
 
 def mx4_linear(x, W, bias=None):
@@ -456,7 +461,9 @@ class Mx4Linear(torch.nn.Module):
         if self.activations is None:
             return mx4_linear(x, W, self.bias)
         if torch.is_grad_enabled() and x.requires_grad:
-            raise ValueError("activations in 4 bits have no gradient: detach them, or call without gradients")
+            raise ValueError(_NO_GRADIENT)
+        if torch._C._get_tracing_state() is not None:
+            return Mx4LinearFunction.apply(x, W.codes, W.scales, self.bias, W.features, self.activations)
         return capi.mx4_linear(x, W, self.bias, activations=4)
 
 
