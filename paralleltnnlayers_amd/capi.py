@@ -359,7 +359,8 @@ def mx4_linear(x, W, bias=None, activations=None, dtype=None, out=None, stream=N
     """y = x W^T + bias with W [N, K] in 4 bits (an ``Mx4``), which is read as its values in x's type.
 
     ``activations=4``: x [..., K] is rounded to 4 bits as well and the product runs on the scaled matrix instructions; so does
-    it for an x that is an ``Mx4`` already (``dtype``: of y, float32 where neither it nor ``out`` says)."""
+    it for an x that is an ``Mx4`` already (``dtype``: of y, float32 where neither it nor ``out`` says).  ``out`` overlaps no
+    operand."""
     if activations not in (None, 4):
         raise ValueError("activations must be None or 4")
     args = (x, W, bias, activations == 4, dtype, out, stream)
@@ -378,8 +379,8 @@ def adapter_forward(x, W, A, B, ids, scale=None, bias=None, out=None, keep=False
     ``y[t] = W x[t] + bias + scale[a] B[a] (A[a] x[t])`` with ``a = ids[t]``; an id outside
     0 .. adapters - 1 (say -1) is a token without one.  x [..., K], W [N, K], A [adapters, R, K]
     and B [adapters, N, R] of one type (float32, bfloat16, float16), or W an ``Mx4``, read as its
-    values in that type; scale [adapters] and bias [N] float32; ids one int32 or int64 a token, in any order.  ``keep``: also returns what
-    ``adapter_backward`` needs of this pass.
+    values in that type; scale [adapters] and bias [N] float32; ids one int32 or int64 a token, in any order.  ``out`` overlaps no operand.
+    ``keep``: also returns what ``adapter_backward`` needs of this pass.
     """
     if stream is None:
         return _native.adapter_forward(x, W, A, B, ids, scale, bias, out, keep, stream)
@@ -419,7 +420,7 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, out=None, keep=False
     """y = (x - mean) / sqrt(variance + eps) * weight + bias over x's last dimension (up to 32768 values).
 
     x [..., D] float32, bfloat16 or float16; weight and bias [D] float32 (None: 1 and 0).  ``out`` may be a contiguous x
-    itself.  ``keep``: also returns what ``layer_norm_backward`` needs of this pass."""
+    itself and overlaps no operand otherwise.  ``keep``: also returns what ``layer_norm_backward`` needs of this pass."""
     args = (x, weight, bias, eps, out, keep, stream)
     return _native.layer_norm_forward(*args) if stream is None else _ordered(stream, _native.layer_norm_forward, *args)
 

@@ -490,8 +490,13 @@ std::pair<const char*, const char*> extent(const Tensor& t) {
   return {first, first + (last + 1) * t.element_size()};
 }
 bool overlap(const Tensor& a, const Tensor& b) {
+  if (!a.defined() || !b.defined() || !a.numel() || !b.numel()) return false;
   const auto x = extent(a), y = extent(b);
   return x.first < y.second && y.first < x.second;
+}
+// An output that the caller gave is none of the operands'.
+void check_apart(const Tensor& out, std::initializer_list<const Tensor*> operands) {
+  for (const Tensor* t : operands) require(!overlap(out, *t), "out overlaps an operand");
 }
 
 // The weights of a projection [N, K]: a tensor, or microscaled 4-bit floating point (capi.Mx4: codes, scales, K).
@@ -652,6 +657,8 @@ PyObject* adapter_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     require(!y.defined() || (y.is_cuda() && y.device() == x.device() && y.scalar_type() == x.scalar_type() &&
                              y.is_contiguous() && y.numel() == (int64_t)(p.shape.T * p.shape.N)),
             "out does not match the result");
+    const Tensor none;
+    check_apart(y, {&x, &W.W, &W.scales, &A, &B, &ids, scale ? &*scale : &none, bias ? &*bias : &none});
     y = adapter_run(p, x.sizes(), y, keep ? &kept : nullptr, st);
   }
   if (a[7] != Py_None && !y.is_inference()) y.unsafeGetTensorImpl()->bump_version();   // (what autograd saved of it is out of date)
@@ -860,6 +867,9 @@ PyObject* layer_norm_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     require(!y.defined() || (y.is_cuda() && y.device() == x.device() && y.scalar_type() == x.scalar_type() &&
                              y.is_contiguous() && y.numel() == x.numel()),
             "out does not match the result");
+    const Tensor none;
+    const bool in_place = y.defined() && x.is_contiguous() && y.data_ptr() == x.data_ptr();
+    check_apart(y, {in_place ? &none : &x, weight ? &*weight : &none, bias ? &*bias : &none});
     y = norm_run(p, x.sizes(), eps, y, keep ? &stats : nullptr, st);
   }
   if (a[4] != Py_None && !y.is_inference()) y.unsafeGetTensorImpl()->bump_version();
@@ -1002,7 +1012,7 @@ PyObject* mx4_dequantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const std::vector<int64_t> sizes = with_last(q.W.sizes(), q.K);
     if (!y.defined()) y = empty(sizes, type, q.W);
     require(y.is_cuda() && y.device() == q.W.device() && y.is_contiguous() && y.sizes() == at::IntArrayRef(sizes), "out does not match the result");
-    require(!overlap(y, q.W) && !overlap(y, q.scales), "out overlaps the codes");
+    check_apart(y, {&q.W, &q.scales});
     const cp4_mx4 m = q.mx4();
     check(cp4_mx4_dequantize((size_t)(q.scales.numel() / q.scales.size(-1)), (unsigned)q.K, dtype_of(y), &m, ptr(y), st));
   }
@@ -1021,13 +1031,15 @@ void check_weight(const Weight& w, const Tensor& like) {
   require(w.W.dim() == 2 && w.W.size(0) >= 1 && w.W.size(0) <= 1 << 22, "expected codes of W [N, K], N from 1 to 2^22");
   require(w.W.device() == like.device(), "x and W must be on one device");
 }
-Tensor output(const std::vector<int64_t>& sizes, at::ScalarType type, const Tensor& like, Tensor y) {
+Tensor output(const std::vector<int64_t>& sizes, at::ScalarType type, const Tensor& like, Tensor y, const Tensor& scales, const Weight& w,
+              const std::optional<Tensor>& bias) {
   if (!y.defined()) return empty(sizes, type, like);
   int64_t n = 1;
   for (int64_t d : sizes) n *= d;
   require(y.is_cuda() && y.device() == like.device() && y.scalar_type() == type && y.is_contiguous() && y.numel() == n,
           "out does not match the result");
-  require(!overlap(y, like), "out overlaps x");
+  const Tensor none;
+  check_apart(y, {&like, &scales, &w.W, &w.scales, bias ? &*bias : &none});
   return y;
 }
 // x in its own type
@@ -1039,7 +1051,7 @@ Tensor mx4_run(const Tensor& x, const Weight& w, const std::optional<Tensor>& bi
   const int dtype = dtype_of(x);
   size_t ld = 0;
   const Tensor rows = rows_of(x, &ld);
-  y = output(with_last(x.sizes(), N), x.scalar_type(), x, y);
+  y = output(with_last(x.sizes(), N), x.scalar_type(), x, y, Tensor(), w, bias_in);
   const size_t T = (size_t)(x.numel() / w.K), need = cp4_mx4_forward_workspace_bytes(T, (unsigned)w.K, (unsigned)N, dtype);
   const Tensor ws = scratch(need, x);
   const cp4_mx4 m = w.mx4();
@@ -1066,7 +1078,7 @@ Tensor mx4_run_product(const Weight& x, const Weight& w, const std::optional<Ten
   check_weight(w, x.W);
   const int64_t N = w.W.size(0);
   const Tensor bias = bias_of(bias_in, N, x.W);
-  y = output(with_last(x.W.sizes(), N), type, x.W, y);
+  y = output(with_last(x.W.sizes(), N), type, x.W, y, x.scales, w, bias_in);
   const size_t T = (size_t)(x.scales.numel() / x.scales.size(-1)), need = cp4_mx4_product_workspace_bytes(T, (unsigned)w.K, (unsigned)N);
   const Tensor ws = scratch(need, x.W);
   const cp4_mx4 mx = x.mx4(), mw = w.mx4();
