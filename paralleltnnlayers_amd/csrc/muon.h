@@ -13,6 +13,12 @@ namespace muon {
 
 constexpr double kA = 3.4445, kB = -4.7750, kC = 2.0315;
 
+// X of a matrix whose norm is far below eps is small throughout: a power of two t goes with it, X' = X / t in memory.  Of |X| in
+// (t0 / 2, t0] it starts as t0, is four times as much with each step (X grows by up to 3.4445) and 1 in the end; where
+// eps counts little it is 1 from the start.  A' = X' X'^T, then B = (t / next t) (a + b t^2 A' + c t^4 A' A'), X' of the next
+// step is B X', and X in the end next t times that.
+inline __host__ __device__ float scale_at(float t0, float four_to_step) { return fminf(1.0f, t0 * four_to_step); }
+
 // A matrix [rows][cols] in two float16 parts: each 32 columns of a row are 64 bytes of first parts, then 64 of what those
 // leave (one cache line), columns behind the last one up to a multiple of 32 are zero.  Values times kScale: X's, A's
 // and a + b A + c A A's magnitudes are below 1.3, 1.5 and 3.45 (of singular values in 0 .. 1.21, where the polynomial keeps them),
@@ -40,6 +46,8 @@ struct Product {
   Outputs o;                                // (final) instead of C
   Rates rates;
   unsigned R, N, K, count;
+  const float* t0;                          // of each matrix, for B and for X in the end; or null
+  float four_to_step;
   float alpha, beta, diagonal;
   bool symmetric;                           // R == N and C is symmetric: tiles on and below the diagonal, mirrored into C
   bool final;                               // of all of a launch's products, or of none

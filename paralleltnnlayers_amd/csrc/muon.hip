@@ -455,6 +455,7 @@ struct LargeItem {
   int grad_dtype;
   unsigned rows, cols;
   unsigned chunks, tiles;                          // of a matrix: workgroups of the norm's launch and of the split's
+  float* t0;                                       // of each matrix
 };
 struct LargeArgs {
   LargeItem item[kLarge];
@@ -504,7 +505,12 @@ __global__ __launch_bounds__(256) void split_kernel(const LargeArgs a) {
   if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
   __syncthreads();
   s = sums[0] + sums[1] + sums[2] + sums[3];
-  const double over = s < INFINITY ? (double)kScale / (sqrt(s) + a.eps) : (double)NAN;
+  double over = s < INFINITY ? 1.0 / (sqrt(s) + a.eps) : (double)NAN;
+  int power;
+  frexp(s < INFINITY ? sqrt(s) * over : 1.0, &power);              // (|X|: in (0.5, 1), times 2^power, or 0)
+  power = max(-126, min(0, power));
+  if (tile == 0 && threadIdx.x == 0) it.t0[matrix] = ldexpf(1.0f, power);
+  over = ldexp(over * kScale, -power);
   const int line = threadIdx.x / 4, at = threadIdx.x % 4 * 16;
   const unsigned r = r0 + line, c = c0 + at;
   float x[16] = {};
@@ -547,7 +553,7 @@ size_t large_bytes(const cp4_muon_matrix& x) {
   return 2 * (part_bytes(x.rows, x.cols) + part_bytes(x.cols, x.rows)) + 2 * part_bytes(m, m);
 }
 constexpr size_t kGroupBytes = (size_t)1 << 30;
-constexpr size_t kNormParts = 1 << 16;             // at most, of a group
+constexpr size_t kNormParts = 1 << 16, kMatrices = 4096;             // at most, of a group
 
 bool nothing(const cp4_muon_matrix& x) { return !x.count || !x.rows || !x.cols; }
 // (without them the momentum alone is updated)
@@ -578,7 +584,7 @@ Product gram_product(const cp4_muon_matrix& x, unsigned count) {
   p.K = std::max(x.rows, x.cols);
   p.count = count;
   p.symmetric = true;
-  p.beta = 1.0f;
+  p.four_to_step = p.beta = 1.0f;
   return p;
 }
 // The splits of a group's first product and what they take.
@@ -626,7 +632,7 @@ std::vector<Group> groups_of(const cp4_muon_matrix* x, size_t n) {
     if (g.pieces.empty()) return;
     size_t part;
     large_splits(x, g, &part);
-    g.bytes = align256(kNormParts * 8) + part;
+    g.bytes = align256(kNormParts * 8) + align256(kMatrices * 4) + part;
     for (const Piece& p : g.pieces) g.bytes += p.count * large_bytes(x[p.entry]) + 6 * 256;
     out.push_back(std::move(g));
     g = Group();
@@ -636,12 +642,12 @@ std::vector<Group> groups_of(const cp4_muon_matrix* x, size_t n) {
     if (nothing(x[i]) || std::min(x[i].rows, x[i].cols) <= kSide) continue;
     const size_t each = large_bytes(x[i]);
     for (size_t first = 0; first < x[i].count;) {
-      if (!g.pieces.empty() && (g.pieces.size() == kLarge || bytes + each > kGroupBytes || matrices >= 4096)) {
+      if (!g.pieces.empty() && (g.pieces.size() == kLarge || bytes + each > kGroupBytes || matrices >= kMatrices)) {
         done();
         bytes = matrices = 0;
       }
       const size_t room = g.pieces.empty() ? std::max<size_t>(1, kGroupBytes / each) : (kGroupBytes - bytes) / each;
-      const size_t count = std::min({x[i].count - first, room, 4096 - matrices});
+      const size_t count = std::min({x[i].count - first, room, kMatrices - matrices});
       g.pieces.push_back(Piece{i, first, count});
       bytes += count * each;
       matrices += count;
@@ -721,6 +727,8 @@ hipError_t run_large(const cp4_muon_matrix* x, const Group& g, const Settings& s
   a.eps = s.eps;
   a.part = reinterpret_cast<double*>(ws);
   ws += align256(kNormParts * 8);
+  float* const t0 = reinterpret_cast<float*>(ws);
+  ws += align256(kMatrices * 4);
   size_t values = 0, part_total;
   for (const Piece& p : g.pieces) values += p.count * x[p.entry].rows * x[p.entry].cols;
   // (4096 values and more; at most half of the partial sums' room beside one for each matrix's rest)
@@ -737,7 +745,7 @@ hipError_t run_large(const cp4_muon_matrix* x, const Group& g, const Settings& s
     ws += align256(bytes);
     return p;
   };
-  unsigned norm = 0, split = 0;
+  unsigned norm = 0, split = 0, matrices = 0;
   struct Buffers { char *x[2], *t[2], *a, *b; };    // X [m][n], transposed [n][m], A and B
   std::vector<Buffers> buffers;
   for (unsigned& k : a.norm) k = ~0u;
@@ -769,6 +777,8 @@ hipError_t run_large(const cp4_muon_matrix* x, const Group& g, const Settings& s
     a.split[i] = split;
     norm += it.chunks * (unsigned)p.count;
     split += it.tiles * (unsigned)p.count;
+    it.t0 = t0 + matrices;
+    matrices += (unsigned)p.count;
   }
   norm_kernel<<<norm, 256, 0, st>>>(a);
   if (split) split_kernel<<<split, 256, 0, st>>>(a);
@@ -791,6 +801,8 @@ hipError_t run_large(const cp4_muon_matrix* x, const Group& g, const Settings& s
       }
       pa.push_back(p);
       p.part = nullptr;
+      p.t0 = a.item[i].t0;
+      p.four_to_step = std::ldexp(1.0f, 2 * k);
       p.P = p.Q = p.E = b.a;
       p.C = b.b;
       p.K = p.N;
@@ -800,7 +812,8 @@ hipError_t run_large(const cp4_muon_matrix* x, const Group& g, const Settings& s
       pb.push_back(p);
       p.symmetric = false;
       p.alpha = p.diagonal = 0.0f;
-      p.beta = 1.0f;
+      p.beta = p.four_to_step = 1.0f;
+      p.t0 = nullptr;
       p.E = nullptr;
       if (k + 1 < s.steps || e.rows <= e.cols) {
         p.N = std::max(e.rows, e.cols);
@@ -817,6 +830,8 @@ hipError_t run_large(const cp4_muon_matrix* x, const Group& g, const Settings& s
       } else {
         p.C = nullptr;
         p.final = true;
+        p.t0 = a.item[i].t0;
+        p.four_to_step = std::ldexp(1.0f, 2 * k);
         p.o = outputs_of(e, g.pieces[i].first);
         p.rates = rates_of(e, s);
       }

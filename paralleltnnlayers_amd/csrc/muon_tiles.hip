@@ -4,7 +4,7 @@
 // A value is hi + lo, 22 bits, a product hi hi + hi lo + lo hi: what is dropped is below 2^-22 of it, so three
 // float16 instructions stand for an fp32 product (16 times an fp32 matrix instruction's work a cycle each; bfloat16 would need
 // six for as many bits, and two of its parts leave an orthogonalised 1024 x 1024 matrix 2.4e-5 off 64 bits
-// where these leave 1.8e-6 and fp32 1.7e-6).  Newton-Schulz keeps its matrices' values below 3, so float16's range is no
+// where these leave 1.8e-6 and fp32 1.7e-6; of updates of few directions, cp4/muon.h).  Newton-Schulz keeps its matrices' values below 3, so float16's range is no
 // limit.
 //
 // A tile is 256 x 256 (eight waves of 128 x 64), 128 x 128 (four of 64 x 64, two workgroups a compute unit) or 64 x 64 (four
@@ -88,6 +88,13 @@ __global__ __launch_bounds__(128 * WN, Rooms > 2 ? 1 : 2) void product_kernel(co
     const int in = row % (16 * NB), col = row - in + NB * (in & 15) + in / 16;
     po[i] = (unsigned)(min(row, R - 1 - m0) * ldk) + piece * 16;
     qo[i] = (unsigned)(min(col, N - 1 - n0) * ldk) + piece * 16;
+  }
+  // (by a vector load, older than all others, so that nobody waits for it; a product without them: 1)
+  float t0 = 1.0f;
+  if (What != kPartial && p.t0) {
+    unsigned at = matrix;
+    asm volatile("" : "+v"(at));
+    t0 = p.t0[at];
   }
   int brought = 0;
   auto bring = [&](char* lds) __attribute__((always_inline)) {
@@ -243,7 +250,9 @@ __global__ __launch_bounds__(128 * WN, Rooms > 2 ? 1 : 2) void product_kernel(co
       }
     return;
   }
-  const float alpha = p.alpha, beta = p.beta * (1.0f / kScale);
+  const float t = scale_at(t0, p.four_to_step), next = scale_at(t, 4.0f), over = What == kParts ? t / next : 1.0f;
+  const float alpha = p.alpha * (over * (t * t)), beta = p.beta * (1.0f / kScale) * (What == kFinal ? next : over * (t * t) * (t * t));
+  const float diagonal = p.diagonal * kScale * over;
   const char* const E = p.E ? p.E + (size_t)matrix * R * ldn : nullptr;
   char* const C = p.C + (size_t)matrix * R * ldn;
   char* Ct = nullptr;
@@ -278,7 +287,7 @@ __global__ __launch_bounds__(128 * WN, Rooms > 2 ? 1 : 2) void product_kernel(co
       for (int j = 0; j < NB; ++j) {
         x[j] = beta * acc[i][j][v];
         x[j] += alpha * es[v][j];
-        if (r == n + j) x[j] += p.diagonal * kScale;
+        if (r == n + j) x[j] += diagonal;
         if (r >= R || n + j >= N) x[j] = 0.0f;     // (what fills up the last block of 32)
         acc[i][j][v] = x[j];
       }

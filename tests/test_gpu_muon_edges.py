@@ -82,3 +82,30 @@ def test_zeros_stay_zeros(optim, shape, eps, steps):  # noqa: F811
     want = p.clone()
     optim.muon_step([p], [torch.zeros_like(p)], [m], lr=0.1, steps=steps, eps=eps)
     assert torch.equal(p, want) and not m.any()
+
+
+@pytest.mark.parametrize("steps", [1, 5, 16])
+@pytest.mark.parametrize("norm", [1e-1, 1e-6, 1.001e-7, 1e-7, 1e-9, 1e-12, 1e-16, 1e-25])
+@pytest.mark.parametrize("shape", [(20, 50), (65, 100), (300, 130), (512, 768)], ids=str)
+def test_norms_below_eps(optim, shape, norm, steps):  # noqa: F811
+    """X = u / (|u| + eps) is then small throughout, and as near to 64 bits, relative to itself, as any other."""
+    u = matrix(*shape)
+    u *= norm / float(u.double().norm())
+    # (the bounds of the formula's own tests)
+    assert off(optim.orthogonalize(u, steps=steps), polar(u, steps)) <= allowed(u.dtype) * (1 if steps < 16 else 20)
+
+
+def test_norms_of_a_stack(optim):  # noqa: F811
+    """Each matrix has its own, in entries of several matrices and shapes, and beside one that is zero or not finite."""
+    us = [matrix(5, 96, 70), matrix(70, 200), matrix(3, 130, 100)]
+    scale = [torch.tensor([1.0, 1e-9, 0.0, 1e-14, 1e-5]), torch.tensor(1e-11), torch.tensor([1e-20, math.inf, 3.0])]
+    us = [u * s.cuda()[..., None, None] for u, s in zip(us, scale)]
+    us[2][1] = math.inf
+    for u, x in zip(us, optim.orthogonalize(us)):
+        for a, b in zip(u.view(-1, *u.shape[-2:]), x.view(-1, *u.shape[-2:])):
+            if not a.isfinite().all():
+                assert b.isnan().all()
+            elif not a.any():
+                assert not b.any()
+            else:
+                assert off(b, polar(a)) <= allowed(u.dtype)
