@@ -302,15 +302,19 @@ class Muon(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict):
-        """As torch's, but every state keeps its own type (torch would cast it to its parameter's)."""
+        """As torch's, but every state keeps its own type (torch would cast it to its parameter's).  What is not a state of
+        this optimizer is refused before anything of it is taken."""
+        if any(k not in saved for saved in state_dict["param_groups"] for k in self.defaults):
+            raise ValueError("Muon: a saved group without " + ", ".join(self.defaults))
+        for s in state_dict["state"].values():
+            if s and not isinstance(s.get("momentum_buffer"), torch.Tensor):
+                raise ValueError("Muon: a state without a momentum")
         super().load_state_dict(state_dict)
         for saved, group in zip(state_dict["param_groups"], self.param_groups):
             for i, p in zip(saved["params"], group["params"]):
                 state = state_dict["state"].get(i)
                 if not state:
                     continue
-                if "momentum_buffer" not in state:
-                    raise ValueError("Muon: a state without a momentum")
                 kept = {"momentum_buffer": state["momentum_buffer"].detach().to(p.device, torch.float32, copy=True)}
                 if self.masters and p.dtype != torch.float32:
                     kept["master"] = state["master"].detach().to(p.device, copy=True) if "master" in state else p.detach().float()
