@@ -387,9 +387,14 @@ Choice choose(const Product* p, int n, bool may_split) {
 template <int MB, int NB, int WN, int Rooms>
 hipError_t launch(const TileArgs& t, Kind kind, hipStream_t st) {
   const unsigned grid = die_grid((long)t.total);
-  if (kind == kParts) product_kernel<MB, NB, WN, Rooms, kParts><<<grid, 128 * WN, 0, st>>>(t);
-  else if (kind == kFinal) product_kernel<MB, NB, WN, Rooms, kFinal><<<grid, 128 * WN, 0, st>>>(t);
-  else product_kernel<MB, NB, WN, Rooms, kPartial><<<grid, 128 * WN, 0, st>>>(t);
+  if (kind == kParts) {
+    product_kernel<MB, NB, WN, Rooms, kParts><<<grid, 128 * WN, 0, st>>>(t);
+  } else if (kind == kPartial) {
+    product_kernel<MB, NB, WN, Rooms, kPartial><<<grid, 128 * WN, 0, st>>>(t);
+  } else {
+    if constexpr (MB == 8) return hipErrorInvalidValue;            // (choose() takes the others)
+    else product_kernel<MB, NB, WN, Rooms, kFinal><<<grid, 128 * WN, 0, st>>>(t);
+  }
   return hipGetLastError();
 }
 
