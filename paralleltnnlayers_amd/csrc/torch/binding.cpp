@@ -739,7 +739,9 @@ struct AdapterFunction : torch::autograd::Function<AdapterFunction> {
     if (dy.scalar_type() != s[2].scalar_type()) dy = dy.to(s[2].scalar_type());
     const bool want_dx = ctx->needs_input_grad(0), want = ctx->needs_input_grad(2) || ctx->needs_input_grad(3);
     const std::optional<Tensor> scale = s[5].defined() ? std::optional<Tensor>(s[5]) : std::nullopt;
-    const Adapters p = adapters(dy, Weight{s[1], s[7], s[2].size(2)}, s[2], s[3], s[4], scale, std::nullopt, true);
+    Weight W{s[1], s[7], s[2].size(2)};
+    if (W.four()) W = packed(s[1], s[7], W.K);                       // (hooks may have given back something else)
+    const Adapters p = adapters(dy, W, s[2], s[3], s[4], scale, std::nullopt, true);
     Tensor dx, dA, dB;
     void* st = c10::hip::getCurrentHIPStream(dy.device().index()).stream();
     adapter_run_backward(p, s[0], s[6], dy.sizes(), want_dx ? &dx : nullptr, want ? &dA : nullptr,
@@ -1155,7 +1157,7 @@ struct Mx4LinearFunction : torch::autograd::Function<Mx4LinearFunction> {
     check_captured_leaves(grad[0]);
     const auto type = (at::ScalarType)ctx->saved_data["type"].toInt();
     const Tensor dy = grad[0].scalar_type() == type ? grad[0] : grad[0].to(type);
-    const Weight w{s[0], s[1], ctx->saved_data["K"].toInt()};
+    const Weight w = packed(s[0], s[1], ctx->saved_data["K"].toInt());               // (as in adapter_linear's)
     if (at::GradMode::is_enabled() && grad[0].requires_grad())       // (create_graph: dx is linear in dy, but for W it has no rule)
       out[0] = (*std::make_shared<torch::autograd::DelayedError>("the gradients of mx4_linear cannot be differentiated again", 1))(
           {mx4_run_backward(dy.detach(), w, c10::hip::getCurrentHIPStream(dy.device().index()).stream()).set_requires_grad(true)})[0];
