@@ -9,7 +9,8 @@
  *
  * x, y, dy and dx [T, D] of one cp4_dtype; weight, bias and their gradients [D] fp32, the statistics and all sums
  * fp32.  The mean is corrected by the mean of what it leaves, the variance is the sum of squares about it: a row far
- * from zero loses nothing that x itself has.  Outputs are rounded once, to nearest-even.  No atomics: results do not
+ * from zero loses nothing that x itself has.  Squares are fp32: a row with values beyond some 1e19 from its
+ * mean is bias in y (NaN where its sum is infinite) and 0 in dx.  Outputs are rounded once, to nearest-even.  No atomics: results do not
  * change from call to call.  What is not finite stays with its row of y and dx, and with its columns of the gradients
  * (a row with an infinity or a NaN is NaN in y and dx; weight's gradient is then NaN throughout).
  *

@@ -10,9 +10,11 @@
 // workgroups' sums, [parts][2][D], go to memory and a second launch adds them up in their order.  Rows of more than 16384
 // values leave no registers for those sums: a launch by columns reads x and dy once more.
 //
-// Measured: 8192 x 4096 bf16: forward 27 us, 5.0 TB/s (a large copy reaches 5.1), backward 49 us with the second launch's
-// 5, 4.1 TB/s; fp32 44 and 83 us.  8192 x 1024 bf16: 9.5 and 17 us.  1024 x 25088 bf16: 59 and 89 us, where sixteen waves of 128
-// registers hold a row and nothing overlaps its loads.  One row of 4096: 5 us, a launch and three waits for memory.
+// Measured, over so many inputs that no cache holds them: 8192 x 4096 bf16: forward 31 us, 4.3 TB/s (a large copy reaches 4.8 to
+// 5.1 on such cards), backward 47 us with the second launch's 4, 4.3 TB/s; fp32 44 and 83 us, 6.1 and 4.9 TB/s.  Over three inputs,
+// of which the memory-side cache holds a part, forward 27 us; before its backward pass, with both passes' tensors in that cache by
+// turns, 34, and the backward pass 42 + 4.  8192 x 1024 bf16: 10 and 18 us.  1024 x 25088 bf16: 56 and 90 us, where sixteen waves of
+// 128 registers hold a row and nothing overlaps its loads.  One row of 4096: 5 us, a launch and three waits for memory.
 #include <algorithm>
 
 #include "cp4/layer_norm.h"

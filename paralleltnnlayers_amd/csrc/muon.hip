@@ -11,7 +11,7 @@
 //   apply     X = Q u and the parameters' step, in fp32 up to 5 steps, in fp64 beyond (wide()).
 //
 // So the step is bound by memory where matrices are long (12 bytes a value in gram, 16 in apply) and by the
-// latency of three launches where they are short: 28 adapters' factors of 7 x 1001 and 777 x 7 7 + 6 + 8 us.  The entries of a
+// latency of three launches where they are short: 28 adapters' factors of 7 x 1001 and 777 x 7 7 + 7 + 9 us.  The entries of a
 // launch are a table in the kernel's arguments.
 #include <algorithm>
 #include <cmath>

@@ -16,7 +16,7 @@
 // mirrored: 4 instead of 6 m^3 for a square matrix.  a X is no addition but a on the diagonal of b A + c A A, 134 MB less to
 // read of 2048 x 4096 by four.
 //
-// Measured: four matrices of 2048 x 4096, a launch each: A 221 us, b A + c A A 125, X 320, which is 0.99, 0.88 and 1.29 PFLOP/s
+// Measured (traced): four matrices of 2048 x 4096, a launch each: A 247 us, b A + c A A 143, X 333, which is 0.89, 0.77 and 1.24 PFLOP/s
 // of float16 (the library's float16 product of 8192^3 reaches 1.1 on the card): bound by the matrix cores' clock under
 // load, A and its square by 144 tiles on 256 compute units.  777 x 1001: 12 us each, which is seven steps' latency and the
 // launch's ends.

@@ -130,3 +130,19 @@ def test_out_is_written(cp4):
             made = torch.empty(shape, device="cuda")
             call(made)
         assert torch.equal(made, out)
+
+
+def test_rows_whose_squares_are_infinite(cp4):
+    """Finite rows beyond 1e19 from their mean: bias in y, 0 in dx; others are not touched by them."""
+    for dtype in (torch.float32, torch.bfloat16):
+        x, dy = batch().to(dtype), torch.randn(T, K, device="cuda").to(dtype)
+        w, b = torch.randn(K, device="cuda"), torch.randn(K, device="cuda")
+        want, stats = cp4.layer_norm_forward(x, w, b, keep=True)
+        clean = cp4.layer_norm_backward(dy, x, w, stats)[0]
+        x[3] = 1e25
+        x[3, ::2] = -1e25
+        y, stats = cp4.layer_norm_forward(x, w, b, keep=True)
+        dx = cp4.layer_norm_backward(dy, x, w, stats)[0]
+        assert torch.equal(y[3], b.to(dtype)) and not dx[3].any()
+        rest = [t for t in range(T) if t != 3]
+        assert torch.equal(y[rest], want[rest]) and torch.equal(dx[rest], clean[rest])
